@@ -31,7 +31,9 @@ typedef enum ri_status {
 
 enum { RI_BF16 = 0, RI_F16 = 1 };
 enum { RI_HEAD_DIM = 128 };
-enum { RI_STATUS_CACHE_FULL = 60 };   /* in a status word: a row did not fit its cache; other values name the wait that gave up */
+/* in a status word: a row did not fit its dense cache; a page table entry names no page; a row did not fit its request's page
+ * table; other values name the wait that gave up */
+enum { RI_STATUS_CACHE_FULL = 60, RI_STATUS_PAGE_ID = 61, RI_STATUS_PAGES_FULL = 62 };
 
 const char* ri_last_error(void);
 int ri_version(void);
@@ -323,6 +325,51 @@ int ri_weighted_flash_decoding(const void* d_q, const void* d_k, const void* d_v
                                const int32_t* d_seqlens, const void* d_previous_out, const float* d_previous_lse,
                                void* d_out, float* d_lse_out, int32_t groups, int32_t group_size, int64_t rows_stride,
                                int32_t dtype, void* stream);
+
+/* One layer of a paged cache.  Pools of pages [n_pages][kv_heads][page_size][128] of keys and of values, whose pages lie
+ * key_page_stride and value_page_stride elements apart; beside them, dense [n_pages][kv_heads][page_size], the weight that
+ * every slot's key was given so far and the number of its token in its request.  Slot j of request b is row j % page_size of
+ * page d_table[b][j / page_size] for every KV head; the first d_lengths[b] slots are in use (negative: none; more than the
+ * table reaches: as many as it does).  Table entries behind them are not read.  An entry that names no page becomes
+ * RI_STATUS_PAGE_ID in *d_status: nothing outside the pools is touched, and that request's results mean nothing. */
+typedef struct ri_paged {
+  int32_t batch, kv_heads;
+  int32_t group_size;        /* query heads to a KV head */
+  int32_t page_size;         /* a power of two from 8 to 1024 */
+  int32_t n_pages;
+  int32_t table_stride;      /* page table entries of a request */
+  int32_t dtype;             /* RI_BF16 or RI_F16 */
+  int32_t reserved;
+  int64_t key_page_stride, value_page_stride;
+  const void* d_keys;        /* written by ri_rope_paged_append and ri_paged_evict */
+  const void* d_values;
+  float* d_weight;           /* or NULL, where a call says so */
+  int32_t* d_token;
+  const int32_t* d_table;    /* [batch][table_stride] */
+  const int32_t* d_lengths;  /* [batch] */
+  int32_t* d_status;         /* ri_status_word() */
+} ri_paged;
+
+/* Rotary positions with several axes, the split of a fused QKV projection, and the append.  d_qkv: `rows` rows of
+ * (group_size + 2) * kv_heads heads of 128, qkv_stride elements apart.  Frequency i < 64 of a row turns by the row's position
+ * on axis h_axis_of[i] < axes (h_axis_of: 64 bytes of host memory, read before the call returns): with (c, s) =
+ * d_cos_sin[d_positions[axis][row]][i], [64 + i] (fp32 [max_positions, 128]; positions int64 [axes, rows], taken to the table's
+ * ends where they lie outside), channels (i, i + 64) become (x c - y s, y c + x s), for query and key heads.  Rows
+ * d_row_start[b] .. d_row_start[b + 1] - 1 are request b's (NULL: row b); the i-th goes to slot d_lengths[b] + i, its weight
+ * there becomes 0 and its token number d_seen[b] + i (d_weight, d_token, with it d_seen: may be NULL).  d_q [rows, q_heads,
+ * 128]; d_k and d_v [rows, kv_heads, 128] take keys and values a second time (may be NULL).  A row that the page table has no
+ * slot for is left out of the cache (RI_STATUS_PAGES_FULL in *d_status). */
+int ri_rope_paged_append(const ri_paged* p, const void* d_qkv, int64_t qkv_stride, const float* d_cos_sin, int64_t max_positions,
+                         const int64_t* d_positions, const uint8_t* h_axis_of, int32_t axes, int32_t rows,
+                         const int32_t* d_row_start, const int32_t* d_seen, void* d_q, void* d_k, void* d_v, void* stream);
+/* Attention of one query row of every request and head over the slots in use: d_q [batch][kv_heads * group_size][128], requests
+ * q_stride elements apart, group_size 1 to 8; d_out dense; d_lse [batch, q_heads] natural log-sum-exp of the scaled scores or
+ * NULL.  A request without slots has out 0 and lse -infinity.  With d_weight every slot's weight grows by the probabilities it
+ * got from the query heads of its group.  d_scratch: that many bytes of 16-byte aligned device memory, any contents, for
+ * this call alone (more with d_weight). */
+int64_t ri_paged_decode_scratch_bytes(const ri_paged* p);
+int ri_paged_decode(const ri_paged* p, const void* d_q, int64_t q_stride, void* d_out, float* d_lse, float scale, void* d_scratch,
+                    void* stream);
 
 /* Decoding with full attention over a dense cache [batch, kv_heads, rows_stride, 128] (cache_hub/flash_attn_cache.py:133-151,
  * attn_hub/flash_attn.py:17-30).  ri_dense_append stores d_k/d_v [batch, kv_heads, 128] at row d_valid_length[b] of every

@@ -15,7 +15,7 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("RI_B200_LIB") or os.path.join(_PKG, "lib", "libri_b200.so")
 
 RI_BF16, RI_F16 = 0, 1
-RI_STATUS_CACHE_FULL = 60
+RI_STATUS_CACHE_FULL, RI_STATUS_PAGE_ID, RI_STATUS_PAGES_FULL = 60, 61, 62
 
 
 class WaveLayer(C.Structure):
@@ -64,6 +64,18 @@ class KMeansPrompt(C.Structure):
     _fields_ = [
         ("n_sink", C.c_int32), ("n_recent", C.c_int32), ("out_group_rows", C.c_int64), ("steady_group_rows", C.c_int64),
         ("d_steady_keys", C.c_void_p), ("d_steady_values", C.c_void_p), ("d_empty", C.c_void_p),
+    ]
+
+
+class Paged(C.Structure):
+    """Mirror of ``struct ri_paged``."""
+
+    _fields_ = [
+        ("batch", C.c_int32), ("kv_heads", C.c_int32), ("group_size", C.c_int32), ("page_size", C.c_int32),
+        ("n_pages", C.c_int32), ("table_stride", C.c_int32), ("dtype", C.c_int32), ("reserved", C.c_int32),
+        ("key_page_stride", C.c_int64), ("value_page_stride", C.c_int64),
+        ("d_keys", C.c_void_p), ("d_values", C.c_void_p), ("d_weight", C.c_void_p), ("d_token", C.c_void_p),
+        ("d_table", C.c_void_p), ("d_lengths", C.c_void_p), ("d_status", C.c_void_p),
     ]
 
 
@@ -133,6 +145,13 @@ def _load() -> C.CDLL:
     lib.ri_batch_gemm_softmax.argtypes = [C.c_void_p] * 6 + [C.c_int32] * 4 + [C.c_float, C.c_float, C.c_int32, C.c_void_p]
     lib.ri_weighted_flash_decoding.restype = C.c_int
     lib.ri_weighted_flash_decoding.argtypes = [C.c_void_p] * 9 + [C.c_int32, C.c_int32, C.c_int64, C.c_int32, C.c_void_p]
+    lib.ri_rope_paged_append.restype = C.c_int
+    lib.ri_rope_paged_append.argtypes = [C.POINTER(Paged), C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_char_p,
+                                         C.c_int32, C.c_int32] + [C.c_void_p] * 6
+    lib.ri_paged_decode_scratch_bytes.restype = C.c_int64
+    lib.ri_paged_decode_scratch_bytes.argtypes = [C.POINTER(Paged)]
+    lib.ri_paged_decode.restype = C.c_int
+    lib.ri_paged_decode.argtypes = [C.POINTER(Paged), C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p, C.c_void_p]
     lib.ri_dense_append.restype = C.c_int
     lib.ri_dense_append.argtypes = [C.c_void_p] * 6 + [C.c_int32, C.c_int32, C.c_int64, C.c_void_p]
     lib.ri_dense_decode_scratch_bytes.restype = C.c_int64

@@ -20,6 +20,7 @@
 // of the scores is therefore key 8jj + s(n), which makes a lane's two columns keys t and t + 4: the rows of V it holds.
 #include <atomic>
 
+#include "ri_step_sequence.cuh"
 #include "ri_tc.cuh"
 #include "ri_wave_attend.cuh"
 
@@ -50,60 +51,14 @@ struct DenseArgs {
 __device__ __forceinline__ int rows_of(const DenseArgs& a, int b) {
   return (int)min((int64_t)max(a.valid[b] + a.extra, 0), a.stride);
 }
-__device__ __forceinline__ int steps_of(int rows) { return (rows + 15) >> 4; }
-
-// All steps of the cache (whole warps).
-__device__ __forceinline__ int count_steps(const DenseArgs& a) {
-  int sum = 0;
-  for (int b = threadIdx.x & 31; b < a.batch; b += 32) sum += steps_of(rows_of(a, b));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return sum * a.hk;
-}
+using ri_seq::Place;
+using ri_seq::count_steps;
+using ri_seq::cta_start;
+using ri_seq::find_place;
+using ri_seq::next_place;
+using ri_seq::steps_of;
 // How many CTAs share `total` steps: at least a step per warp, at most one CTA per SM.
-__device__ __forceinline__ int used_ctas(int total, int max_ctas) {
-  return min(max_ctas, max(1, (total + kDenseWarps - 1) / kDenseWarps));
-}
-__device__ __forceinline__ int cta_start(int c, int total, int n) { return (int)((int64_t)c * total / n); }
-
-// A place in the sequence of steps: group g, its first step in the sequence, its rows.
-struct Place {
-  int g, first, rows;
-};
-// The group that holds step s (whole warps; s < total).
-__device__ __forceinline__ Place find_place(const DenseArgs& a, int s) {
-  const int lane = threadIdx.x & 31;
-  int before = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 32) {
-    const int b = b0 + lane;
-    const int rows = b < a.batch ? rows_of(a, b) : 0, n = steps_of(rows) * a.hk;
-    int incl = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, s < before + incl);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      const int r = __shfl_sync(0xffffffffu, rows, src), start = before + __shfl_sync(0xffffffffu, incl - n, src);
-      const int per = steps_of(r), h = (s - start) / per;
-      return {(b0 + src) * a.hk + h, start + h * per, r};
-    }
-    before += __shfl_sync(0xffffffffu, incl, 31);
-  }
-  return {0, 0, 0};
-}
-// The next group with rows (there is one: the caller has steps left).
-__device__ __forceinline__ void next_place(const DenseArgs& a, Place& p) {
-  p.first += steps_of(p.rows);
-  ++p.g;
-  if (p.g % a.hk == 0) {
-    int b = p.g / a.hk;
-    while ((p.rows = rows_of(a, b)) == 0 && b + 1 < a.batch) ++b;
-    p.g = b * a.hk;
-  }
-}
+__device__ __forceinline__ int used_ctas(int total, int max_ctas) { return ri_seq::used_ctas<kDenseWarps>(total, max_ctas); }
 
 template <int DT>
 __global__ void __launch_bounds__(kDenseThreads, 1) dense_decode_kernel(const __grid_constant__ CUtensorMap map_k,

@@ -1,0 +1,473 @@
+// Attention of one new token over a paged cache, and the weight that it gives to every slot.
+//   out_h = sum_j p_hj v_j,  p_hj = e^{s_hj - lse_h},  s_hj = scale q_h.k_j,  lse_h = log sum_j e^{s_hj}
+//   weight_j += sum_h p_hj over the query heads of a KV head (what ri_paged_evict goes by), where asked for
+// A request without slots has out 0 and lse -infinity.
+//
+// Bound by the rows of K and V, read once: with at most eight query heads to a KV head there are 16 operations for each byte
+// read, a sixteenth of what the tensor cores need to be the limit, so m16n8k16 with the heads in M is enough.
+// The split is that of the dense cache (ri_step_sequence.cuh): 16-row steps of all groups behind one another, an equal
+// contiguous range per SM and again per warp, whatever the requests' lengths; a warp streams its steps through its own ring,
+// filled by TMA, a box of 16 rows (8 where a page has no more) of both halves of the channels; the number of the next step's
+// page is fetched a step ahead.  Layout in shared memory and the order of the keys in a step: as in ri_dense_decode.cu.
+// The probabilities enter the second product as two 16-bit parts, so out is within its own rounding of 32-bit arithmetic.
+// A second kernel merges a group's partial results by log-sum-exp in a fixed order.  For the weights the first kernel
+// leaves the scores behind (4 bytes a slot and query head, against 512 a slot for K and V), and a third turns them into
+// probabilities once lse is known; every slot has one thread, so the sums have one order and no atomics.
+#include <atomic>
+
+#include "ri_paged.cuh"
+#include "ri_step_sequence.cuh"
+#include "ri_tc.cuh"
+#include "ri_wave_attend.cuh"
+
+namespace ri_wave {
+namespace {
+
+using namespace ri_tc;
+using ri_page::Pages;
+using ri_page::page_of;
+using ri_page::record_at;
+using ri_seq::Place;
+using ri_seq::count_steps;
+using ri_seq::cta_start;
+using ri_seq::find_place;
+using ri_seq::next_place;
+using ri_seq::steps_of;
+
+constexpr int kPagedWarps = 8;
+constexpr int kPagedThreads = kPagedWarps * 32;
+constexpr int kPagedMaxCtas = 160;                    // the grid is one CTA per SM, at most this many
+constexpr int kPagedRing = kPagedWarps * kStages * kStageBytes;   // 192 KB, on a 1024-byte boundary
+constexpr int kPagedSmem = 1024 + kPagedRing;
+constexpr int kJoinThreads = 256;
+constexpr int kFoldThreads = 256;
+
+struct PagedArgs : Pages {
+  const uint4* q;
+  float* part_o;             // [slots][gs][128]
+  float2* part_ml;           // [slots][gs]: (maximum in the log2 domain, sum)
+  float* scores;             // [step][gs][16] in the log2 domain, or null; inside a step the order of the lanes that made them
+  float* lse2;               // [groups][gs]: log-sum-exp in the log2 domain, for the weights
+  float* lse;                // [groups][gs] or null
+  uint16_t* out;
+  int64_t q_stride;          // 16-byte pieces from request to request
+  int gs, max_ctas;
+  float scale2;
+};
+__device__ __forceinline__ int used_ctas(int total, int max_ctas) { return ri_seq::used_ctas<kPagedWarps>(total, max_ctas); }
+
+// BOX: rows of a TMA box.
+template <int DT, int BOX, bool WEIGHTS>
+__global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __grid_constant__ CUtensorMap map_k,
+                                                                     const __grid_constant__ CUtensorMap map_v,
+                                                                     const __grid_constant__ PagedArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  __shared__ __align__(8) uint64_t s_full[kPagedWarps][kStages];
+  __shared__ int s_abort;
+  __shared__ float sm_m[kPagedWarps][kMaxHeads], sm_l[kPagedWarps][kMaxHeads];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int r = lane >> 2, t = lane & 3, gs = a.gs;
+  const int sr = ((r & 1) << 2) | (r >> 1);              // the lane's row and pieces, see ri_dense_decode.cu
+  if (tid == 0) s_abort = 0;
+  if (lane == 0) {                                       // a warp's barriers are set up and fed by the same lane
+    for (int i = 0; i < kStages; ++i) mbar_init(smem_u32(&s_full[warp][i]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  __syncthreads();
+  volatile int* abort_flag = &s_abort;
+  ri_pdl_enter();
+  const int total = count_steps(a), n_ctas = used_ctas(total, a.max_ctas), c = (int)blockIdx.x;
+  if (c >= n_ctas || total == 0) return;
+  const int c_lo = cta_start(c, total, n_ctas), c_hi = cta_start(c + 1, total, n_ctas), c_n = c_hi - c_lo;
+  const int lo = c_lo + c_n * warp / kPagedWarps, hi = c_lo + c_n * (warp + 1) / kPagedWarps;
+  const Place c_first = find_place(a, c_lo);
+  const bool merged = c_hi <= c_first.first + steps_of(c_first.rows);      // the CTA's range lies inside one group
+
+  // a stage: K, then V; of each the boxes one behind the other, a box as two halves of 64 channels
+  constexpr int kTensor = kStageBytes / 2, kBox = BOX * 256, kHalf = BOX * 128, kStageStride = kPagedWarps * kStageBytes;
+  uint8_t* my_ring = ring + warp * kStageBytes;
+  const uint32_t my_ring_u32 = smem_u32(my_ring), my_full = smem_u32(&s_full[warp][0]);
+  auto row_at = [&](int row) { return BOX == 16 ? row * 128 : (row >> 3) * kBox + (row & 7) * 128; };
+
+  float m_run = -INFINITY, l_run = 0.f;    // head r (l: this lane's share, reduced over the quad at the end)
+  float acc[8][4];
+  auto clear = [&] {
+    m_run = -INFINITY;
+    l_run = 0.f;
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[x][i] = 0.f;
+  };
+  auto reduce_sum = [&] {
+    l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
+    l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
+  };
+  // accumulators to rows of 128 floats, one per head (heads 2t and 2t+1 are this lane's)
+  auto put = [&](float* o) {
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const int ch = (x < 4) ? 8 * sr + 2 * x : 64 + 8 * sr + 2 * (x - 4);
+      if (2 * t < gs) *reinterpret_cast<float2*>(o + (2 * t) * RI_HEAD_DIM + ch) = make_float2(acc[x][0], acc[x][2]);
+      if (2 * t + 1 < gs) *reinterpret_cast<float2*>(o + (2 * t + 1) * RI_HEAD_DIM + ch) = make_float2(acc[x][1], acc[x][3]);
+    }
+  };
+  // Slots: along the sequence (warp, group) goes up by one of the two at a time, so their sum names a partial result.
+  auto store_partial = [&](int g) {
+    const int64_t slot = (int64_t)(c * kPagedWarps + warp) + g;
+    reduce_sum();
+    put(a.part_o + slot * gs * RI_HEAD_DIM);
+    if (t == 0 && r < gs) a.part_ml[slot * gs + r] = make_float2(m_run, l_run);
+  };
+
+  clear();
+  if (lo < hi) {
+    Place at_issue = find_place(a, lo), at = at_issue;
+    // pages of the next step to issue; the second one only where a page is half a step
+    int id0 = 0, id1 = 0;
+    auto fetch_ids = [&](int s) {
+      while (s >= at_issue.first + steps_of(at_issue.rows)) next_place(a, at_issue);
+      const int b = at_issue.g / a.hk, row = (s - at_issue.first) * 16;
+      id0 = page_of(a, b, row >> a.shift);
+      if (BOX == 8 && row + 8 < at_issue.rows) id1 = page_of(a, b, (row + 8) >> a.shift);
+    };
+    auto issue = [&](int s, int stage) {
+      if (lane == 0) {
+        const uint32_t dst = my_ring_u32 + stage * kStageStride, bar = my_full + 8 * stage;
+        const int row = (s - at_issue.first) * 16, in_page = ((at_issue.g % a.hk) << a.shift) + (row & ((1 << a.shift) - 1));
+        const bool second = BOX == 8 && row + 8 < at_issue.rows;
+        mbar_arrive_expect_tx(bar, (BOX == 16 || second) ? kStageBytes : kStageBytes / 2);
+        tma_load_4d(dst, &map_k, bar, 0, in_page, 0, id0);
+        tma_load_4d(dst + kTensor, &map_v, bar, 0, in_page, 0, id0);
+        if (second) {
+          const int in_next = ((at_issue.g % a.hk) << a.shift) + ((row + 8) & ((1 << a.shift) - 1));
+          tma_load_4d(dst + kBox, &map_k, bar, 0, in_next, 0, id1);
+          tma_load_4d(dst + kTensor + kBox, &map_v, bar, 0, in_next, 0, id1);
+        }
+      }
+    };
+    int s_issue = lo;
+#pragma unroll
+    for (int st = 0; st < kStages; ++st)
+      if (s_issue < hi) {
+        fetch_ids(s_issue);
+        issue(s_issue++, st);
+      }
+    if (s_issue < hi) fetch_ids(s_issue);
+    uint4 qa[4];
+    auto load_q = [&] {
+      const int b = at.g / a.hk, h = at.g - b * a.hk;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        qa[kk] = r < gs ? ri_ldg16(a.q + b * a.q_stride + (h * gs + r) * 16 + t + kk * 4) : make_uint4(0, 0, 0, 0);
+    };
+    load_q();
+    int stage = 0, phase = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (int s = lo; s < hi; ++s) {
+      if (s >= at.first + steps_of(at.rows)) {
+        store_partial(at.g);
+        clear();
+        do next_place(a, at);
+        while (s >= at.first + steps_of(at.rows));
+        load_q();
+      }
+      const int base = (s - at.first) * 16;
+      ok = __all_sync(0xffffffffu, mbar_wait(my_full + 8 * stage, phase, abort_flag, 71));
+      if (!ok) break;
+      const uint8_t* src = my_ring + stage * kStageStride;
+      float s2[2][2];
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj) {
+        float c1[4] = {0.f, 0.f, 0.f, 0.f}, c2[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const uint4 kb = *reinterpret_cast<const uint4*>(src + (kk >> 1) * kHalf + row_at(8 * jj + sr) +
+                                                           (((t ^ sr) << 4) ^ ((kk & 1) << 6)));
+          Elem<DT>::mma16816(c1, qa[kk].x, 0u, qa[kk].y, 0u, kb.x, kb.y);
+          Elem<DT>::mma16816(c2, qa[kk].z, 0u, qa[kk].w, 0u, kb.z, kb.w);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          s2[jj][e] = base + jj * 8 + t + 4 * e < at.rows ? (c1[e] + c2[e]) * a.scale2 : -INFINITY;
+      }
+      if (WEIGHTS && r < gs)
+        reinterpret_cast<float4*>(a.scores)[((int64_t)s * gs + r) * 4 + t] = make_float4(s2[0][0], s2[0][1], s2[1][0], s2[1][1]);
+      // online softmax for head r
+      float mx = fmaxf(fmaxf(s2[0][0], s2[0][1]), fmaxf(s2[1][0], s2[1][1]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float m_new = fmaxf(m_run, mx), m_safe = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = exp2f(m_run - m_safe);
+      float p[2][2], psum = 0.f;
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          p[jj][e] = exp2f(s2[jj][e] - m_safe);
+          psum += p[jj][e];
+        }
+      l_run = l_run * alpha + psum;
+      m_run = m_new;
+      const float f0 = __shfl_sync(0xffffffffu, alpha, (2 * t) * 4), f1 = __shfl_sync(0xffffffffu, alpha, (2 * t + 1) * 4);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) { acc[x][0] *= f0; acc[x][1] *= f1; acc[x][2] *= f0; acc[x][3] *= f1; }
+      uint4 v[4][2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* at_v = src + kTensor + row_at(t + 4 * i) + (((sr ^ t) << 4) ^ ((i & 1) << 6));
+        v[i][0] = *reinterpret_cast<const uint4*>(at_v);
+        v[i][1] = *reinterpret_cast<const uint4*>(at_v + kHalf);
+      }
+      __syncwarp();
+      if (s_issue < hi) {                             // the stage is in registers: refill it before the products
+        issue(s_issue++, stage);
+        if (s_issue < hi) fetch_ids(s_issue);
+      }
+      if (base + 16 > at.rows) {                      // a group's last step: what lies behind its rows may be anything
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (base + t + 4 * i >= at.rows) v[i][0] = v[i][1] = make_uint4(0, 0, 0, 0);
+      }
+      const uint2 b0 = split2<DT>(p[0][0], p[0][1]), b1 = split2<DT>(p[1][0], p[1][1]);
+      pv_step<DT, true>(acc, v, b0.x, b1.x, b0.y, b1.y);
+      if (++stage == kStages) { stage = 0; phase ^= 1; }
+    }
+    if (!ok) {               // leave a bounded chance to the copies in flight before their memory goes
+      if (lane == 0) {
+        for (int i = 0; i < kStages; ++i) mbar_wait(my_full + 8 * ((stage + i) % kStages), phase ^ (stage + i >= kStages), abort_flag, 72);
+        *a.status = s_abort;
+      }
+      __syncwarp();
+    } else if (!merged) {
+      store_partial(at.g);
+    }
+  }
+  if (!merged) return;
+
+  reduce_sum();
+  if (t == 0) { sm_m[warp][r] = m_run; sm_l[warp][r] = l_run; }
+  auto warp_o = [&](int w) { return reinterpret_cast<float*>(ring + w * kStageBytes); };
+  put(warp_o(warp));
+  __syncthreads();
+  const int64_t slot = (int64_t)c * kPagedWarps + c_first.g;
+  for (int idx = tid; idx < gs * RI_HEAD_DIM; idx += kPagedThreads) {
+    const int h = idx >> 7;
+    float M = -INFINITY, L = 0.f, O = 0.f;
+#pragma unroll
+    for (int w = 0; w < kPagedWarps; ++w) M = fmaxf(M, sm_m[w][h]);
+    const float Ms = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int w = 0; w < kPagedWarps; ++w) {
+      const float f = exp2f(sm_m[w][h] - Ms);
+      L += sm_l[w][h] * f;
+      O += warp_o(w)[idx] * f;
+    }
+    a.part_o[slot * gs * RI_HEAD_DIM + idx] = O;
+    if ((idx & 127) == 0) a.part_ml[slot * gs + h] = make_float2(M, L);
+  }
+}
+
+// One head of one group per block: the slots of its partial results in sequence order, then two halves of the block each
+// sum every second one.
+template <int DT>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a) {
+  ri_pdl_enter();
+  __shared__ int s_slot[kPagedMaxCtas * kPagedWarps];
+  __shared__ float s_w[kPagedMaxCtas * kPagedWarps];
+  __shared__ float s_l, s_o[RI_HEAD_DIM];
+  __shared__ int s_n;
+  const int tid = threadIdx.x, lane = tid & 31, h = blockIdx.x, g = blockIdx.y, gs = a.gs;
+  uint16_t* out = a.out + ((int64_t)g * gs + h) * RI_HEAD_DIM;
+  const int b = g / a.hk, n = steps_of(rows_of(a, b));
+  if (n == 0) {
+    if (tid < RI_HEAD_DIM) out[tid] = 0;
+    if (tid == 0 && a.lse != nullptr) a.lse[g * gs + h] = -INFINITY;
+    return;
+  }
+  if (tid < 32) {
+    int before = 0;
+    for (int i = lane; i < b; i += 32) before += steps_of(rows_of(a, i));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    const int lo = before * a.hk + (g - b * a.hk) * n, hi = lo + n;
+    const int total = count_steps(a), n_ctas = used_ctas(total, a.max_ctas);
+    int c0 = (int)((int64_t)lo * n_ctas / total);           // the CTA that holds step lo
+    while (c0 > 0 && cta_start(c0, total, n_ctas) > lo) --c0;
+    while (cta_start(c0 + 1, total, n_ctas) <= lo) ++c0;
+    int count = 0;
+    for (int c_base = c0; c_base < n_ctas && cta_start(c_base, total, n_ctas) < hi; c_base += 4) {      // 4 CTAs a warp step
+      const int c = c_base + (lane >> 3), w = lane & 7;
+      bool mine = false;
+      if (c < n_ctas) {
+        const int c_lo = cta_start(c, total, n_ctas), c_n = cta_start(c + 1, total, n_ctas) - c_lo;
+        if (c_lo >= lo && c_lo + c_n <= hi) {
+          mine = w == 0;
+        } else {
+          const int w_lo = c_lo + c_n * w / kPagedWarps, w_hi = c_lo + c_n * (w + 1) / kPagedWarps;
+          mine = max(w_lo, lo) < min(w_hi, hi);
+        }
+      }
+      const unsigned votes = __ballot_sync(0xffffffffu, mine);
+      if (mine) s_slot[count + __popc(votes & ((1u << lane) - 1))] = c * kPagedWarps + w + g;
+      count += __popc(votes);
+    }
+    __syncwarp();
+    float M = -INFINITY, L = 0.f;
+    for (int i = lane; i < count; i += 32) M = fmaxf(M, a.part_ml[(int64_t)s_slot[i] * gs + h].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float Ms = M == -INFINITY ? 0.f : M;
+    for (int i = lane; i < count; i += 32) {
+      const float2 ml = a.part_ml[(int64_t)s_slot[i] * gs + h];
+      const float f = exp2f(ml.x - Ms);
+      s_w[i] = f;
+      L += ml.y * f;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if (lane == 0) {
+      s_l = L;
+      s_n = count;
+      const float lse2 = M + log2f(L);
+      if (a.lse2 != nullptr) a.lse2[g * gs + h] = lse2;
+      if (a.lse != nullptr) a.lse[g * gs + h] = lse2 * 0.69314718055994531f;
+    }
+  }
+  __syncthreads();
+  const int ch = tid & (RI_HEAD_DIM - 1), half = tid >> 7, count = s_n;
+  float O = 0.f;
+#pragma unroll 8
+  for (int i = half; i < count; i += 2) O += a.part_o[((int64_t)s_slot[i] * gs + h) * RI_HEAD_DIM + ch] * s_w[i];
+  if (half) s_o[ch] = O;
+  __syncthreads();
+  if (!half) out[ch] = Elem<DT>::bits(s_l > 0.f ? (O + s_o[ch]) / s_l : 0.f);
+}
+
+// weight_j += sum_h 2^(s_hj - lse_h): a thread per slot, 256 slots of one group per block.
+__global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const __grid_constant__ PagedArgs a) {
+  ri_pdl_enter();
+  __shared__ int s_first;
+  const int tid = threadIdx.x, lane = tid & 31, g = blockIdx.y, gs = a.gs, b = g / a.hk;
+  const int rows = rows_of(a, b), base = blockIdx.x * kFoldThreads;
+  if (base >= rows) return;
+  if (tid < 32) {
+    int before = 0;
+    for (int i = lane; i < b; i += 32) before += steps_of(rows_of(a, i));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    if (lane == 0) s_first = before * a.hk + (g - b * a.hk) * steps_of(rows);
+  }
+  __syncthreads();
+  // place i of a step holds its key (i / 2 % 2) * 8 + i / 4 + (i % 2) * 4
+  const int step = (base + tid) >> 4, i = tid & 15, slot = step * 16 + ((i >> 1) & 1) * 8 + (i >> 2) + (i & 1) * 4;
+  if (slot >= rows) return;
+  const float* sc = a.scores + (int64_t)(s_first + step) * gs * 16 + i;
+  float sum = 0.f;
+  for (int h = 0; h < gs; ++h) sum += exp2f(sc[h * 16] - a.lse2[g * gs + h]);
+  a.weight[record_at(a, page_of(a, b, slot >> a.shift), g - b * a.hk, slot & ((1 << a.shift) - 1))] += sum;
+}
+
+int64_t paged_slots(int64_t groups) { return (int64_t)kPagedMaxCtas * kPagedWarps + groups; }
+int64_t paged_most_steps(const ri_paged& p) {
+  return (int64_t)p.batch * p.kv_heads * (((int64_t)p.table_stride * p.page_size + 15) / 16);
+}
+
+// Pages as (64 channels, row of the page's heads, half, page).
+int make_page_map(CUtensorMap* map, const void* base, const ri_paged& p, int64_t page_stride, int box) {
+  EncodeTiledFn enc;
+  const int rc = get_encode_fn(&enc);
+  if (rc != RI_OK) return rc;
+  const cuuint64_t dims[4] = {64, (cuuint64_t)p.kv_heads * p.page_size, 2, (cuuint64_t)p.n_pages};
+  const cuuint64_t strides[3] = {256, 128, (cuuint64_t)page_stride * 2};
+  const cuuint32_t boxes[4] = {64, (cuuint32_t)box, 2, 1}, estr[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, p.dtype == RI_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                         const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  RI_REQUIRE(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code %d", (int)r);
+  return RI_OK;
+}
+
+template <int DT, int BOX, bool WEIGHTS>
+int launch_paged(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t s) {
+  static std::atomic<bool> known[64];                   // per device; asked for again where it is not remembered
+  int dev = 0;
+  RI_CUDA_OK(cudaGetDevice(&dev));
+  const bool track = dev >= 0 && dev < 64;
+  if (!track || !known[dev].load(std::memory_order_relaxed)) {
+    RI_CUDA_OK(cudaFuncSetAttribute(paged_decode_kernel<DT, BOX, WEIGHTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPagedSmem));
+    if (track) known[dev].store(true, std::memory_order_relaxed);
+  }
+  RI_CUDA_OK(ri_launch_pdl_id(11, paged_decode_kernel<DT, BOX, WEIGHTS>, dim3(a.max_ctas), dim3(kPagedThreads), (size_t)kPagedSmem,
+                              s, map_k, map_v, a));
+  RI_CUDA_OK(ri_launch_pdl_id(11, paged_join_kernel<DT>, dim3(a.gs, a.batch * a.hk), dim3(kJoinThreads), 0, s, a));
+  if (WEIGHTS) {
+    const int64_t most = (int64_t)a.table_stride << a.shift;
+    RI_CUDA_OK(ri_launch_pdl_id(11, paged_fold_kernel, dim3((unsigned)((most + kFoldThreads - 1) / kFoldThreads), a.batch * a.hk),
+                                dim3(kFoldThreads), 0, s, a));
+  }
+  return RI_OK;
+}
+template <int DT>
+int launch_paged(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, int box, cudaStream_t s) {
+  if (box == 8)
+    return a.weight ? launch_paged<DT, 8, true>(a, map_k, map_v, s) : launch_paged<DT, 8, false>(a, map_k, map_v, s);
+  return a.weight ? launch_paged<DT, 16, true>(a, map_k, map_v, s) : launch_paged<DT, 16, false>(a, map_k, map_v, s);
+}
+
+}  // namespace
+}  // namespace ri_wave
+
+extern "C" int64_t ri_paged_decode_scratch_bytes(const ri_paged* p) {
+  const int rc = ri_page::check(p, "ri_paged_decode");
+  if (rc != RI_OK) return rc;
+  if (p->group_size < 1 || p->group_size > ri_wave::kMaxHeads) return ri_fail(RI_ERR_INVALID, "ri_paged_decode: group_size=%d unsupported", p->group_size);
+  const int64_t groups = (int64_t)p->batch * p->kv_heads;
+  int64_t floats = ri_wave::paged_slots(groups) * p->group_size * (RI_HEAD_DIM + 2);
+  if (p->d_weight) floats += groups * p->group_size + 4 + ri_wave::paged_most_steps(*p) * p->group_size * 16;
+  return floats * 4;
+}
+
+extern "C" int ri_paged_decode(const ri_paged* p, const void* d_q, int64_t q_stride, void* d_out, float* d_lse, float scale,
+                               void* d_scratch, void* stream) {
+  using namespace ri_wave;
+  int rc;
+  if ((rc = ri_page::check(p, "ri_paged_decode")) != RI_OK) return rc;
+  RI_REQUIRE(p->d_values && d_q && d_out && d_scratch, "ri_paged_decode: null pointer");
+  RI_REQUIRE(p->group_size >= 1 && p->group_size <= kMaxHeads, "ri_paged_decode: group_size=%d unsupported (1 to %d)", p->group_size,
+             kMaxHeads);
+  RI_REQUIRE(q_stride >= (int64_t)p->kv_heads * p->group_size * RI_HEAD_DIM && q_stride % 8 == 0,
+             "ri_paged_decode: queries overlap or lie at odd places");
+  RI_REQUIRE(((uintptr_t)d_q | (uintptr_t)d_out | (uintptr_t)d_scratch) % 16 == 0, "q, out and the scratch must be 16-byte aligned");
+  RI_REQUIRE(scale > 0.f && scale < 1e30f, "ri_paged_decode: scale must be positive and finite");
+  const int64_t groups = (int64_t)p->batch * p->kv_heads;
+  PagedArgs a = {};
+  static_cast<ri_page::Pages&>(a) = ri_page::view(*p);
+  a.q = static_cast<const uint4*>(d_q);
+  a.q_stride = q_stride / 8;
+  a.gs = p->group_size;
+  a.part_o = static_cast<float*>(d_scratch);
+  float* next = a.part_o + paged_slots(groups) * a.gs * RI_HEAD_DIM;
+  a.part_ml = reinterpret_cast<float2*>(next);
+  next += paged_slots(groups) * a.gs * 2;
+  if (p->d_weight) {
+    a.lse2 = next;
+    next += groups * a.gs;
+    a.scores = reinterpret_cast<float*>(ri_align16((size_t)next));
+  }
+  a.lse = d_lse;
+  a.out = static_cast<uint16_t*>(d_out);
+  a.scale2 = RI_LOG2E * scale;
+  int sms = 0;
+  if ((rc = ri_sm_count(&sms)) != RI_OK) return rc;
+  a.max_ctas = sms < kPagedMaxCtas ? sms : kPagedMaxCtas;
+  const int box = p->page_size < 16 ? 8 : 16;
+  CUtensorMap map_k, map_v;
+  if ((rc = make_page_map(&map_k, p->d_keys, *p, p->key_page_stride, box)) != RI_OK) return rc;
+  if ((rc = make_page_map(&map_v, p->d_values, *p, p->value_page_stride, box)) != RI_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return p->dtype == RI_BF16 ? launch_paged<RI_BF16>(a, map_k, map_v, box, s) : launch_paged<RI_F16>(a, map_k, map_v, box, s);
+}

@@ -1,7 +1,7 @@
 """The process's status word, on the host.
 
-Prefill, dense decode and wave decode kernels record in it that a device-side wait gave up, and the dense append that a row did
-not fit (0: none of it): one word in page-locked host memory for all devices and streams, replays of CUDA graphs among them.  The
+Prefill, decode (dense, paged, wave) kernels record in it that a device-side wait gave up, the appends that a row did not fit, and
+the kernels over paged caches that a page table names no page (0: none of it): one word in page-locked host memory for all devices and streams, replays of CUDA graphs among them.  The
 kernels only write it, so a failure stays inside its call; it stays set until it is reported, by ``check`` or by the first call
 that finds it set.
 """
@@ -31,7 +31,8 @@ def word(device) -> C.c_int32:
 
 def _kernel(code: int) -> str:
     # what the kernels' waits are numbered by; a second bound of a wait, by count, adds 100
-    return {2: "ri_prefill_attn", 3: "ri_prefill_attn", 4: "ri_dense_decode", 5: "ri_wave_decode_layer"}.get(code % 100 // 10, "a kernel")
+    return {2: "ri_prefill_attn", 3: "ri_prefill_attn", 4: "ri_dense_decode", 5: "ri_wave_decode_layer",
+            7: "ri_paged_decode"}.get(code % 100 // 10, "a kernel")
 
 
 def check() -> None:
@@ -44,6 +45,10 @@ def check() -> None:
         _word.value = 0
         if code == _lib.RI_STATUS_CACHE_FULL:
             raise RuntimeError("a token's rows did not fit the dense cache (more decode steps than max_length has room for)")
+        if code == _lib.RI_STATUS_PAGE_ID:
+            raise RuntimeError("a page table entry names no page of the pool")
+        if code == _lib.RI_STATUS_PAGES_FULL:
+            raise RuntimeError("a token's rows did not fit the pages of its request")
         raise RuntimeError(f"{_kernel(code)} gave up on a device-side wait (code {code})")
 
 
