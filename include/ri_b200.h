@@ -370,6 +370,15 @@ int ri_rope_paged_append(const ri_paged* p, const void* d_qkv, int64_t qkv_strid
 int64_t ri_paged_decode_scratch_bytes(const ri_paged* p);
 int ri_paged_decode(const ri_paged* p, const void* d_q, int64_t q_stride, void* d_out, float* d_lse, float scale, void* d_scratch,
                     void* stream);
+/* Eviction by accumulated weight, in place: requests of more than `keep` slots keep `keep` for every KV head, those of the first
+ * n_sink and the last n_recent of their d_seen[b] tokens (n_sink + n_recent <= keep) and then the ones of largest weight, the
+ * lower slot first among equals (NaN: less than any weight).  The i-th slot in front of `keep` that goes takes the key, value,
+ * weight and token number of the i-th one behind it that stays; slots behind `keep` are left as they were, and so are lengths
+ * and page tables: afterwards a request's length is at most `keep`, and the pages behind are the caller's.  Requests must not
+ * share pages.  d_scratch: that many bytes of 16-byte aligned device memory, any contents, for this call alone. */
+int64_t ri_paged_evict_scratch_bytes(const ri_paged* p, int32_t keep);
+int ri_paged_evict(const ri_paged* p, const int32_t* d_seen, int32_t keep, int32_t n_sink, int32_t n_recent, void* d_scratch,
+                   void* stream);
 
 /* Decoding with full attention over a dense cache [batch, kv_heads, rows_stride, 128] (cache_hub/flash_attn_cache.py:133-151,
  * attn_hub/flash_attn.py:17-30).  ri_dense_append stores d_k/d_v [batch, kv_heads, 128] at row d_valid_length[b] of every

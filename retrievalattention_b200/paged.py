@@ -2,7 +2,8 @@
 
 * ``rope_paged_append``  rotary positions with several axes (text, images, video) on a fused QKV projection; queries out, keys and
                          values into the cache's pages;
-* ``paged_decode``       attention of one new token over the pages, optionally adding up the weight that every slot gets.
+* ``paged_decode``       attention of one new token over the pages, optionally adding up the weight that every slot gets;
+* ``paged_evict``        the slots of least weight give way, in place.
 
 The layer is a handful of tensors that the caller owns (``cache_hub.paged_cache`` keeps them for a whole model):
 
@@ -190,3 +191,29 @@ def paged_decode(q, key_pages, value_pages, page_table, lengths, *, out=None, ls
     torch.autograd.graph.increment_version([x for x in (out, lse, weight) if x is not None])
     _status.report(status)
     return out
+
+
+def paged_evict(key_pages, value_pages, weight, token, page_table, lengths, seen, keep, n_sink=0, n_recent=0):
+    """Requests of more than ``keep`` slots keep ``keep`` for every KV head: the slots of the first ``n_sink`` and the last
+    ``n_recent`` of their ``seen[b]`` tokens (int32 ``[batch]``; together at most ``keep``), then those of largest weight, the lower
+    slot first among equals.  In place: the i-th slot in front of ``keep`` that goes takes the key, value, weight and token number
+    of the i-th one behind it that stays, so slots are no longer in the order of their tokens.  ``lengths`` and the page tables are
+    left alone: clamp the lengths to ``keep`` when the last layer is done, and the pages behind are free.  Requests must not share
+    pages."""
+    what = "paged_evict"
+    if _elsewhere(key_pages):
+        with torch.cuda.device(key_pages.device):
+            return paged_evict(key_pages, value_pages, weight, token, page_table, lengths, seen, keep, n_sink, n_recent)
+    if value_pages is None or weight is None or token is None:
+        _fail(what, "keys, values, weights and token numbers move together: none may be missing")
+    layer, status = _layer(what, key_pages, value_pages, page_table, lengths, weight, token, 1)
+    if seen.shape != (layer.batch,) or seen.dtype != torch.int32 or seen.device != key_pages.device or not seen.is_contiguous():
+        _fail(what, "expected dense int32 seen [batch]")
+    size = _lib.lib.ri_paged_evict_scratch_bytes(C.byref(layer), keep)
+    if size < 0:
+        _lib.check(size, what)
+    scratch = torch.empty((size,), dtype=torch.uint8, device=key_pages.device)
+    _lib.check(_lib.lib.ri_paged_evict(C.byref(layer), seen.data_ptr(), keep, n_sink, n_recent, scratch.data_ptr(),
+                                       _lib.current_stream()), what)
+    torch.autograd.graph.increment_version((key_pages, value_pages, weight, token))
+    _status.report(status)
