@@ -370,6 +370,13 @@ int ri_rope_paged_append(const ri_paged* p, const void* d_qkv, int64_t qkv_strid
 int64_t ri_paged_decode_scratch_bytes(const ri_paged* p);
 int ri_paged_decode(const ri_paged* p, const void* d_q, int64_t q_stride, void* d_out, float* d_lse, float scale, void* d_scratch,
                     void* stream);
+/* The weight that the last `window` queries of every request give to its slots: d_q [batch][window][q_heads][128]; query w sees
+ * the slots up to d_lengths[b] - window + w (one that sees none, of a request shorter than the window, may hold anything and
+ * gives nothing); every slot's weight grows by the sum of its probabilities over queries and heads of its group.  window *
+ * group_size below 2^20.  Writes d_weight only; d_values may be NULL.  d_scratch: that many bytes of 16-byte aligned device
+ * memory, any contents, for this call alone. */
+int64_t ri_paged_observe_scratch_bytes(const ri_paged* p);
+int ri_paged_observe(const ri_paged* p, const void* d_q, int32_t window, float scale, void* d_scratch, void* stream);
 /* Eviction by accumulated weight, in place: requests of more than `keep` slots keep `keep` for every KV head, those of the first
  * n_sink and the last n_recent of their d_seen[b] tokens (n_sink + n_recent <= keep) and then the ones of largest weight, the
  * lower slot first among equals (NaN: less than any weight).  The i-th slot in front of `keep` that goes takes the key, value,

@@ -152,6 +152,10 @@ def _load() -> C.CDLL:
     lib.ri_paged_decode_scratch_bytes.argtypes = [C.POINTER(Paged)]
     lib.ri_paged_decode.restype = C.c_int
     lib.ri_paged_decode.argtypes = [C.POINTER(Paged), C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p, C.c_void_p]
+    lib.ri_paged_observe_scratch_bytes.restype = C.c_int64
+    lib.ri_paged_observe_scratch_bytes.argtypes = [C.POINTER(Paged)]
+    lib.ri_paged_observe.restype = C.c_int
+    lib.ri_paged_observe.argtypes = [C.POINTER(Paged), C.c_void_p, C.c_int32, C.c_float, C.c_void_p, C.c_void_p]
     lib.ri_paged_evict_scratch_bytes.restype = C.c_int64
     lib.ri_paged_evict_scratch_bytes.argtypes = [C.POINTER(Paged), C.c_int32]
     lib.ri_paged_evict.restype = C.c_int

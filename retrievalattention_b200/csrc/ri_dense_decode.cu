@@ -37,6 +37,7 @@ constexpr int kDenseSmem = 1024 + kDenseRing;
 constexpr int kCombineThreads = 256;
 
 struct DenseArgs {
+  static constexpr int kStep = 16;
   const uint4* q;
   const int32_t* valid;      // [batch]; a group attends valid[b] + extra rows, at most `stride`
   float* part_o;             // [slots][gs][128]
@@ -56,7 +57,7 @@ using ri_seq::count_steps;
 using ri_seq::cta_start;
 using ri_seq::find_place;
 using ri_seq::next_place;
-using ri_seq::steps_of;
+__device__ __forceinline__ int steps_of(int rows) { return ri_seq::steps_of<16>(rows); }
 // How many CTAs share `total` steps: at least a step per warp, at most one CTA per SM.
 __device__ __forceinline__ int used_ctas(int total, int max_ctas) { return ri_seq::used_ctas<kDenseWarps>(total, max_ctas); }
 

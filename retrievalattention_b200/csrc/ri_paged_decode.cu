@@ -32,7 +32,7 @@ using ri_seq::count_steps;
 using ri_seq::cta_start;
 using ri_seq::find_place;
 using ri_seq::next_place;
-using ri_seq::steps_of;
+__device__ __forceinline__ int steps_of(int rows) { return ri_seq::steps_of<16>(rows); }
 
 constexpr int kPagedWarps = 8;
 constexpr int kPagedThreads = kPagedWarps * 32;
@@ -43,6 +43,7 @@ constexpr int kJoinThreads = 256;
 constexpr int kFoldThreads = 256;
 
 struct PagedArgs : Pages {
+  static constexpr int kStep = 16;
   const uint4* q;
   float* part_o;             // [slots][gs][128]
   float2* part_ml;           // [slots][gs]: (maximum in the log2 domain, sum)

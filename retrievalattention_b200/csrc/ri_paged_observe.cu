@@ -1,0 +1,393 @@
+// The attention weight that the last `window` queries of every request give to the slots of a paged cache.
+//   weight_j += sum over query rows r (window query w, query head h of the KV head):  e^{s_rj - lse_r},
+//   s_rj = scale q_r.k_j,  lse_r = log sum_j e^{s_rj},  both over the slots that query w sees: j <= length - window + w.
+// Rows that see no slot (prompts shorter than the window) give nothing.
+//
+// Two passes over K, both on the tensor cores, with the query rows of a KV head (window x group, 256 at a time) in shared memory:
+//   pass 1  S = Q.K^T, M 128 query rows x N 128 keys: a thread holds a query row and keeps its running maximum and sum;
+//   pass 2  S^T = K.Q^T, M 128 keys x N query rows: a thread holds a key and adds the probabilities of the rows.
+// Either way the reduction stays inside a thread; the operands lie in shared memory the same way for both (rows of 128 channels in
+// two 128-byte-swizzled halves), only their roles change.  A slot's weight has one thread, so there are no atomics.
+// The split is that of the decode kernels: tiles of 128 slots of all groups behind one another, an equal contiguous range per SM.
+// Pass 1 leaves a (maximum, sum) per row and range; a small kernel between the passes merges them.
+// Four warps bring in tiles, issue the products and idle, eight work on scores: two halves of four, one per tile of
+// query rows in pass 1 (or every second tile of keys, where there is only one), every second tile of keys in pass 2.
+// TMEM: 256 columns of scores for each half.  Every wait is bounded; one that runs out is recorded in the
+// status word.  Bound by the exponentials, two for each slot and query row.
+#include <cuda.h>
+
+#include <atomic>
+
+#include "ri_paged.cuh"
+#include "ri_step_sequence.cuh"
+#include "ri_tc.cuh"
+
+namespace {
+
+using namespace ri_tc;
+using namespace ri_page;
+using ri_seq::Place;
+
+constexpr int kTile = 128;                       // slots of a tile
+constexpr int kRows = 256;                       // query rows that are worked on together
+constexpr int kKeyHalf = kTile * 128, kKeyTile = 2 * kKeyHalf;
+constexpr int kRowHalf = kRows * 128, kRowTile = 2 * kRowHalf;
+constexpr int kRing = 4;                         // K tiles in shared memory
+constexpr int kObsThreads = 384;
+constexpr uint32_t kTmemCols = 512;
+constexpr int kObsSmem = 1024 + kRowTile + kRing * kKeyTile;
+constexpr int kObsMaxCtas = 160;
+
+struct ObsArgs : Pages {
+  static constexpr int kStep = kTile;
+  const uint4* q;                                // [batch][window][hk * gs][16 pieces]
+  float2* part;                                  // [slots][kRows]: (maximum in the log2 domain, sum)
+  float* lse2;                                   // [groups][kRows]; +infinity: the row gives nothing
+  int window, gs, first_row, rows;               // rows first_row .. first_row + rows - 1 of window * gs
+  int max_ctas;
+  float scale2;
+  uint32_t idesc;
+};
+
+__device__ __forceinline__ float ex2(float x) {       // 2^x; results below 2^-126 become 0
+  float d;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
+  return d;
+}
+// The last slot that query row `row` sees in a request of n slots (negative: none).
+__device__ __forceinline__ int last_seen(const ObsArgs& a, int n, int row) { return n - a.window + row / a.gs; }
+
+// STATS: pass 1.
+template <int DT, bool STATS>
+__global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ ObsArgs a) {
+  constexpr int kBuffers = STATS ? 2 : 1;        // of scores, for each half of the score warps: 128 columns each, or 256
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* q_rows = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t sQ = base, sK = base + kRowTile;
+  __shared__ __align__(8) uint64_t s_bars[1 + 2 * kRing + 8];
+  __shared__ uint32_t s_tmem_base;
+  __shared__ int s_abort;
+  __shared__ __align__(16) float s_lse[kRows];
+  __shared__ __align__(16) int s_last[kRows];
+  const uint32_t bars = smem_u32(s_bars);
+  const uint32_t bar_q = bars;                                              // the group's query rows are there
+  auto bar_full = [&](int s) { return bars + 8u * (1 + s); };               // a K tile is there, is free
+  auto bar_empty = [&](int s) { return bars + 8u * (1 + kRing + s); };
+  auto bar_s_full = [&](int g, int i) { return bars + 8u * (1 + 2 * kRing + 2 * g + i); };      // scores are there, are read
+  auto bar_s_empty = [&](int g, int i) { return bars + 8u * (5 + 2 * kRing + 2 * g + i); };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    mbar_init(bar_q, 8);
+    for (int s = 0; s < kRing; ++s) { mbar_init(bar_full(s), 1); mbar_init(bar_empty(s), 1); }
+    for (int g = 0; g < 2; ++g)
+      for (int i = 0; i < 2; ++i) { mbar_init(bar_s_full(g, i), 1); mbar_init(bar_s_empty(g, i), 4); }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)), "r"(kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem_base;
+  volatile int* abort_flag = &s_abort;
+  ri_pdl_enter();
+
+  // this CTA's tiles [lo, hi) of the sequence, segment by segment (the part of a group that falls to it)
+  const int total = ri_seq::count_steps(a), n_ctas = min(a.max_ctas, total), c = (int)blockIdx.x;
+  const int lo = c < n_ctas ? ri_seq::cta_start(c, total, n_ctas) : 0, hi = c < n_ctas ? ri_seq::cta_start(c + 1, total, n_ctas) : 0;
+  // both halves of the score warps work on the same keys where there are query rows for both, on every second tile otherwise
+  const bool both = STATS && a.rows > kTile;
+
+  if (lo < hi) {
+    if (warp == 0) {
+      // ---------------- K tiles, a box of at most a page per lane ----------------
+      Place at = ri_seq::find_place(a, lo);
+      const int box = min(1 << a.shift, kTile), mask = (1 << a.shift) - 1;
+      bool ok = true;
+      int issued = 0;
+      for (int t = lo; t < hi; ++t, ++issued) {
+        while (t >= at.first + ri_seq::steps_of<kTile>(at.rows)) ri_seq::next_place(a, at);
+        const int b = at.g / a.hk, h = at.g - b * a.hk, slot0 = (t - at.first) * kTile;
+        const int boxes = (min(kTile, at.rows - slot0) + box - 1) / box, s = issued % kRing;
+        const int id = lane < boxes ? page_of(a, b, (slot0 + lane * box) >> a.shift) : 0;
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_empty(s), ((issued / kRing) & 1) ^ 1, abort_flag, 81));
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(bar_full(s), boxes * box * 256);
+        __syncwarp();
+        if (lane < boxes) {
+          const int y = (h << a.shift) + ((slot0 + lane * box) & mask);
+          const uint32_t dst = sK + s * kKeyTile + lane * box * 128;
+          tma_load_3d(dst, &map_k, bar_full(s), 0, y, id);
+          tma_load_3d(dst + kKeyHalf, &map_k, bar_full(s), 64, y, id);
+        }
+      }
+      if (*abort_flag)         // give the copies still in flight a bounded chance to land before the CTA exits
+        for (int t = max(0, issued - kRing); t < issued; ++t) mbar_wait(bar_full(t % kRing), (t / kRing) & 1, abort_flag, 82);
+    } else if (warp == 1) {
+      // ---------------- products ----------------
+      Place at = ri_seq::find_place(a, lo);
+      if (lane == 0) {
+        bool ok = true;
+        int used = 0, groups = 0, made[2] = {0, 0};
+        for (int t = lo; ok && t < hi; ++t, ++used) {
+          bool fresh = t == lo;
+          while (t >= at.first + ri_seq::steps_of<kTile>(at.rows)) { ri_seq::next_place(a, at); fresh = true; }
+          if (fresh) ok = mbar_wait(bar_q, groups++ & 1, abort_flag, 83);
+          const int s = used % kRing;
+          ok = ok && mbar_wait(bar_full(s), (used / kRing) & 1, abort_flag, 84);
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            if (!both && g != (used & 1)) continue;
+            const int i = made[g] % kBuffers;
+            ok = ok && mbar_wait(bar_s_empty(g, i), ((made[g] / kBuffers) & 1) ^ 1, abort_flag, 85);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t d = STATS ? tmem + (2 * g + i) * 128 : tmem + g * 256;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+              const uint64_t dk = umma_desc_sw128(sK + s * kKeyTile + kb * kKeyHalf);
+              const uint64_t dq = umma_desc_sw128(sQ + kb * kRowHalf + (both && g ? kTile * 128 : 0));
+#pragma unroll
+              for (int k = 0; k < 4; ++k) tc_mma_f16(d, (STATS ? dq : dk) + 2 * k, (STATS ? dk : dq) + 2 * k, a.idesc, (kb | k) != 0);
+            }
+            tc_commit(bar_s_full(g, i));
+            ++made[g];
+          }
+          if (ok) tc_commit(bar_empty(s));
+        }
+      }
+    } else if (warp >= 4) {
+      // ---------------- scores ----------------
+      const int g = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane, tid = threadIdx.x - 128;
+      const uint32_t t_lane = (uint32_t)(quarter * 32) << 16;
+      Place at = ri_seq::find_place(a, lo);
+      bool ok = true;
+      int done = 0, used = 0;                          // tiles of this half, of the CTA
+      for (int t = lo; t < hi;) {
+        while (t >= at.first + ri_seq::steps_of<kTile>(at.rows)) ri_seq::next_place(a, at);
+        const int end = min(hi, at.first + ri_seq::steps_of<kTile>(at.rows)), n = at.rows;
+        const int b = at.g / a.hk, h = at.g - b * a.hk;
+        // the group's query rows: a thread brings a row, its pieces swizzled as TMA would; every product over the rows before
+        // has completed, since its scores have been read
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        {
+          const int r = a.first_row + tid;
+          const uint4* src = a.q + ((int64_t)(b * a.window + r / a.gs) * a.hk * a.gs + h * a.gs + r % a.gs) * 16;
+#pragma unroll
+          for (int piece = 0; piece < 16; ++piece) {
+            const uint4 x = tid < a.rows ? ri_ldg16(src + piece) : make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(q_rows + (piece >> 3) * kRowHalf + tid * 128 + (((piece & 7) ^ (tid & 7)) << 4)) = x;
+          }
+          if (!STATS) {
+            s_lse[tid] = a.lse2[(int64_t)at.g * kRows + tid];
+            s_last[tid] = last_seen(a, n, r);
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (lane == 0) mbar_arrive(bar_q);
+        if (STATS) {
+          const int r = both ? g * kTile + row : row;
+          const int last = r < a.rows ? min(last_seen(a, n, a.first_row + r), n - 1) : -1;
+          float m = -INFINITY, l = 0.f;
+          for (; t < end; ++t, ++used) {
+            if (!both && g != (used & 1)) continue;
+            const int i = done % kBuffers;
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(bar_s_full(g, i), (done / kBuffers) & 1, abort_flag, 86));
+            if (!ok) continue;
+            tc_fence_after();
+            uint32_t sr[4][32];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) tc_ld32(tmem + (2 * g + i) * 128 + t_lane + k * 32, sr[k]);
+            tc_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) tc_ld_landed(sr[k]);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_s_empty(g, i));
+            ++done;
+            const int slot0 = (t - at.first) * kTile;
+            if (slot0 + kTile - 1 > last) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int x = 0; x < 32; ++x)
+                  if (slot0 + k * 32 + x > last) sr[k][x] = 0xff800000u;     // -inf
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+              for (int x = 0; x < 32; x += 2) mx = max3(mx, __uint_as_float(sr[k][x]), __uint_as_float(sr[k][x + 1]));
+            const float m_new = fmaxf(m, mx * a.scale2);
+            if (m_new == -INFINITY) continue;
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+              for (int x = 0; x < 32; ++x) sum += ex2(__uint_as_float(sr[k][x]) * a.scale2 - m_new);
+            l = l * ex2(m - m_new) + sum;
+            m = m_new;
+          }
+          a.part[(int64_t)(c + at.g) * kRows + tid] = make_float2(m, l);
+        } else {
+          for (; t < end; ++t, ++used) {
+            if (g != (used & 1)) continue;
+            const int slot0 = (t - at.first) * kTile, slot = slot0 + row;
+            float* weight = nullptr;
+            float old = 0.f;
+            if (slot < n) {
+              weight = a.weight + record_at(a, page_of(a, b, slot >> a.shift), h, slot & ((1 << a.shift) - 1));
+              old = *weight;
+            }
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(bar_s_full(g, 0), done & 1, abort_flag, 87));
+            if (!ok) continue;
+            tc_fence_after();
+            const bool edge = slot0 + kTile - 1 > n - a.window;
+            float sum = 0.f;
+            for (int k = 0; k * 32 < a.rows; ++k) {
+              uint32_t sr[32];
+              tc_ld32(tmem + g * 256 + t_lane + k * 32, sr);
+              tc_wait_ld();
+              tc_ld_landed(sr);
+#pragma unroll
+              for (int x = 0; x < 32; ++x) {
+                const float e = ex2(__uint_as_float(sr[x]) * a.scale2 - s_lse[k * 32 + x]);
+                sum += edge && slot > s_last[k * 32 + x] ? 0.f : e;
+              }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_s_empty(g, 0));
+            ++done;
+            if (weight != nullptr) *weight = old + sum;
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && s_abort) *a.status = s_abort;
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+  }
+}
+
+// lse of 32 query rows of one group: the partial results of the CTAs that worked on it, every eighth one by one warp.
+__global__ void __launch_bounds__(256) observe_merge_kernel(const __grid_constant__ ObsArgs a) {
+  ri_pdl_enter();
+  __shared__ float2 s_part[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = blockIdx.y, b = g / a.hk;
+  const int row = blockIdx.x * 32 + lane, tiles = ri_seq::steps_of<kTile>(rows_of(a, b));
+  const bool both = a.rows > kTile;
+  float m = -INFINITY, l = 0.f;
+  auto add = [&](float2 x) {
+    const float m_new = fmaxf(m, x.x);
+    if (m_new == -INFINITY) return;
+    l = l * exp2f(m - m_new) + x.y * exp2f(x.x - m_new);
+    m = m_new;
+  };
+  if (tiles > 0 && row < a.rows) {
+    int before = 0;
+    for (int i = 0; i < b; ++i) before += ri_seq::steps_of<kTile>(rows_of(a, i));
+    int total = before;
+    for (int i = b; i < a.batch; ++i) total += ri_seq::steps_of<kTile>(rows_of(a, i));
+    total *= a.hk;
+    const int n_ctas = min(a.max_ctas, total), lo = before * a.hk + (g - b * a.hk) * tiles, hi = lo + tiles;
+    int c0 = (int)((int64_t)lo * n_ctas / total);           // the CTA that holds tile lo
+    while (c0 > 0 && ri_seq::cta_start(c0, total, n_ctas) > lo) --c0;
+    while (ri_seq::cta_start(c0 + 1, total, n_ctas) <= lo) ++c0;
+    for (int c = c0 + warp; c < n_ctas && ri_seq::cta_start(c, total, n_ctas) < hi; c += 8) {
+      add(a.part[(int64_t)(c + g) * kRows + row]);
+      if (!both) add(a.part[(int64_t)(c + g) * kRows + kTile + row]);      // the other half's tiles
+    }
+  }
+  s_part[warp][lane] = make_float2(m, l);
+  __syncthreads();
+  if (warp == 0) {
+    m = -INFINITY;
+    l = 0.f;
+    for (int w = 0; w < 8; ++w) add(s_part[w][lane]);
+    a.lse2[(int64_t)g * kRows + row] = l > 0.f ? m + log2f(l) : INFINITY;
+  }
+}
+
+// Keys as (channel, row of the page's heads, page); a box is one half of the channels of at most a page.
+int make_key_map(CUtensorMap* map, const ri_paged& p) {
+  EncodeTiledFn enc;
+  const int rc = get_encode_fn(&enc);
+  if (rc != RI_OK) return rc;
+  const cuuint64_t dims[3] = {RI_HEAD_DIM, (cuuint64_t)p.kv_heads * p.page_size, (cuuint64_t)p.n_pages};
+  const cuuint64_t strides[2] = {256, (cuuint64_t)p.key_page_stride * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)(p.page_size < kTile ? p.page_size : kTile), 1}, estr[3] = {1, 1, 1};
+  const CUresult r = enc(map, p.dtype == RI_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                         const_cast<void*>(p.d_keys), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  RI_REQUIRE(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code %d", (int)r);
+  return RI_OK;
+}
+
+template <int DT>
+int launch_observe(ObsArgs a, const CUtensorMap& map_k, cudaStream_t s) {
+  static std::atomic<bool> known[64];                   // per device; asked for again where it is not remembered
+  int dev = 0;
+  RI_CUDA_OK(cudaGetDevice(&dev));
+  const bool track = dev >= 0 && dev < 64;
+  if (!track || !known[dev].load(std::memory_order_relaxed)) {
+    RI_CUDA_OK(cudaFuncSetAttribute(observe_kernel<DT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kObsSmem));
+    RI_CUDA_OK(cudaFuncSetAttribute(observe_kernel<DT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kObsSmem));
+    if (track) known[dev].store(true, std::memory_order_relaxed);
+  }
+  const int rows = a.window * a.gs;
+  for (a.first_row = 0; a.first_row < rows; a.first_row += kRows) {
+    a.rows = rows - a.first_row < kRows ? rows - a.first_row : kRows;
+    a.idesc = idesc_f16(DT, 128, 128);
+    RI_CUDA_OK(ri_launch_pdl_id(11, observe_kernel<DT, true>, dim3(a.max_ctas), dim3(kObsThreads), (size_t)kObsSmem, s, map_k, a));
+    RI_CUDA_OK(ri_launch_pdl_id(11, observe_merge_kernel, dim3(kRows / 32, a.batch * a.hk), dim3(256), 0, s, a));
+    a.idesc = idesc_f16(DT, 128, (a.rows + 31) / 32 * 32);      // the scores are read 32 columns at a time
+    RI_CUDA_OK(ri_launch_pdl_id(11, observe_kernel<DT, false>, dim3(a.max_ctas), dim3(kObsThreads), (size_t)kObsSmem, s, map_k, a));
+  }
+  return RI_OK;
+}
+
+int64_t obs_slots(const ri_paged& p) { return kObsMaxCtas + (int64_t)p.batch * p.kv_heads; }
+
+}  // namespace
+
+extern "C" int64_t ri_paged_observe_scratch_bytes(const ri_paged* p) {
+  const int rc = check(p, "ri_paged_observe");
+  if (rc != RI_OK) return rc;
+  return obs_slots(*p) * kRows * 8 + (int64_t)p->batch * p->kv_heads * kRows * 4;
+}
+
+extern "C" int ri_paged_observe(const ri_paged* p, const void* d_q, int32_t window, float scale, void* d_scratch, void* stream) {
+  int rc;
+  if ((rc = check(p, "ri_paged_observe")) != RI_OK) return rc;
+  RI_REQUIRE(p->d_weight && d_q && d_scratch, "ri_paged_observe: null pointer");
+  RI_REQUIRE(window >= 1 && p->group_size >= 1 && (int64_t)window * p->group_size < (1 << 20),
+             "ri_paged_observe: window=%d group_size=%d unsupported", window, p->group_size);
+  RI_REQUIRE(((uintptr_t)d_q | (uintptr_t)d_scratch) % 16 == 0, "q and the scratch must be 16-byte aligned");
+  RI_REQUIRE(scale > 0.f && scale < 1e30f, "ri_paged_observe: scale must be positive and finite");
+  ObsArgs a = {};
+  static_cast<Pages&>(a) = view(*p);
+  a.q = static_cast<const uint4*>(d_q);
+  a.part = static_cast<float2*>(d_scratch);
+  a.lse2 = reinterpret_cast<float*>(a.part + obs_slots(*p) * kRows);
+  a.window = window;
+  a.gs = p->group_size;
+  a.scale2 = RI_LOG2E * scale;
+  int sms = 0;
+  if ((rc = ri_sm_count(&sms)) != RI_OK) return rc;
+  a.max_ctas = sms < kObsMaxCtas ? sms : kObsMaxCtas;
+  CUtensorMap map_k;
+  if ((rc = make_key_map(&map_k, *p)) != RI_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return p->dtype == RI_BF16 ? launch_observe<RI_BF16>(a, map_k, s) : launch_observe<RI_F16>(a, map_k, s);
+}

@@ -1,5 +1,5 @@
-// Splitting attention over a cache evenly: the cache's 16-row steps, all groups (request, KV head) behind one another, are
-// cut into one contiguous range per CTA.  Groups without rows take no steps.  The requests' lengths are read on the device.
+// Splitting work over a cache evenly: the cache's steps of Args::kStep rows, all groups (request, KV head) behind one another,
+// are cut into one contiguous range per CTA.  Groups without rows take no steps.  The requests' lengths are read on the device.
 // `Args` has batch, hk (KV heads) and a function int rows_of(const Args&, int b).
 #pragma once
 
@@ -7,13 +7,14 @@
 
 namespace ri_seq {
 
-__device__ __forceinline__ int steps_of(int rows) { return (rows + 15) >> 4; }
+template <int STEP>
+__device__ __forceinline__ int steps_of(int rows) { return (int)((unsigned)(rows + STEP - 1) / STEP); }
 
 // All steps of the cache (whole warps).
 template <class Args>
 __device__ __forceinline__ int count_steps(const Args& a) {
   int sum = 0;
-  for (int b = threadIdx.x & 31; b < a.batch; b += 32) sum += steps_of(rows_of(a, b));
+  for (int b = threadIdx.x & 31; b < a.batch; b += 32) sum += steps_of<Args::kStep>(rows_of(a, b));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return sum * a.hk;
@@ -36,7 +37,7 @@ __device__ __forceinline__ Place find_place(const Args& a, int s) {
   int before = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
     const int b = b0 + lane;
-    const int rows = b < a.batch ? rows_of(a, b) : 0, n = steps_of(rows) * a.hk;
+    const int rows = b < a.batch ? rows_of(a, b) : 0, n = steps_of<Args::kStep>(rows) * a.hk;
     int incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -47,7 +48,7 @@ __device__ __forceinline__ Place find_place(const Args& a, int s) {
     if (hit) {
       const int src = __ffs(hit) - 1;
       const int r = __shfl_sync(0xffffffffu, rows, src), start = before + __shfl_sync(0xffffffffu, incl - n, src);
-      const int per = steps_of(r), h = (s - start) / per;
+      const int per = steps_of<Args::kStep>(r), h = (s - start) / per;
       return {(b0 + src) * a.hk + h, start + h * per, r};
     }
     before += __shfl_sync(0xffffffffu, incl, 31);
@@ -57,7 +58,7 @@ __device__ __forceinline__ Place find_place(const Args& a, int s) {
 // The next group with rows (there is one: the caller has steps left).
 template <class Args>
 __device__ __forceinline__ void next_place(const Args& a, Place& p) {
-  p.first += steps_of(p.rows);
+  p.first += steps_of<Args::kStep>(p.rows);
   ++p.g;
   if (p.g % a.hk == 0) {
     int b = p.g / a.hk;

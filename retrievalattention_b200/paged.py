@@ -3,6 +3,7 @@
 * ``rope_paged_append``  rotary positions with several axes (text, images, video) on a fused QKV projection; queries out, keys and
                          values into the cache's pages;
 * ``paged_decode``       attention of one new token over the pages, optionally adding up the weight that every slot gets;
+* ``paged_observe``      the weight that a prompt's last queries give to its slots;
 * ``paged_evict``        the slots of least weight give way, in place.
 
 The layer is a handful of tensors that the caller owns (``cache_hub.paged_cache`` keeps them for a whole model):
@@ -191,6 +192,34 @@ def paged_decode(q, key_pages, value_pages, page_table, lengths, *, out=None, ls
     torch.autograd.graph.increment_version([x for x in (out, lse, weight) if x is not None])
     _status.report(status)
     return out
+
+
+def paged_observe(q, key_pages, page_table, lengths, weight, *, scale=None):
+    """Add to every slot's ``weight`` the probabilities that the last queries of its request give it: ``q`` dense ``[batch, window,
+    q_heads, 128]``, the rows of the last ``window`` tokens in use, each of which sees the slots up to its own; summed over queries
+    and over the query heads of a KV head.  What ``paged_evict`` goes by after a prompt.  Requests shorter than the window are
+    padded in front, with anything.  Slots must be in the order of their tokens (no eviction before)."""
+    what = "paged_observe"
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return paged_observe(q, key_pages, page_table, lengths, weight, scale=scale)
+    if q.dim() != 4 or key_pages.dim() != 4 or weight is None:
+        _fail(what, "expected q [batch, window, q_heads, 128], pages [pages, kv_heads, page_size, 128] and weights")
+    b, window, hq, d = q.shape
+    hk = key_pages.shape[1]
+    if d != DIM or window < 1 or hk < 1 or hq < hk or hq % hk or page_table.shape[0] != b or not q.is_contiguous():
+        _fail(what, "expected dense q [batch, window, q_heads, 128], q_heads a multiple of kv_heads, one page table row per request")
+    if q.dtype != key_pages.dtype or q.device != key_pages.device or q.requires_grad:
+        _fail(what, "expected q and the pages of one type on one GPU, without gradients")
+    layer, status = _layer(what, key_pages, None, page_table, lengths, weight, None, hq // hk)
+    size = _lib.lib.ri_paged_observe_scratch_bytes(C.byref(layer))
+    if size < 0:
+        _lib.check(size, what)
+    scratch = torch.empty((size,), dtype=torch.uint8, device=q.device)
+    _lib.check(_lib.lib.ri_paged_observe(C.byref(layer), q.data_ptr(), window, _SCALE if scale is None else scale, scratch.data_ptr(),
+                                         _lib.current_stream()), what)
+    torch.autograd.graph.increment_version(weight)
+    _status.report(status)
 
 
 def paged_evict(key_pages, value_pages, weight, token, page_table, lengths, seen, keep, n_sink=0, n_recent=0):
