@@ -10,6 +10,9 @@ add folded in, ``ri_rope_split``, ``ri_silu_and_mul``); the attention is
 
 Every buffer is allocated once, positions live on the device, and nothing synchronises: one
 decode step can be captured in a CUDA graph and replayed.
+
+``PagedDecoder`` runs the same layers, prompts included, over a ``paged_cache``: positions may have several
+axes (text, images, video), and requests of uneven lengths share a pool of pages and are held to a number of slots.
 """
 from __future__ import annotations
 
@@ -147,3 +150,81 @@ class SyntheticDecoder:
         """Bytes of weights one decode step reads (every matrix once; one embedding row per request)."""
         per_layer = sum(t.numel() * t.element_size() for t in self.layers[0].values())
         return per_layer * self.n_layers + self.lm_head.numel() * self.lm_head.element_size()
+
+
+class PagedDecoder(SyntheticDecoder):
+    """The same model over a ``paged_cache``: prompts of uneven lengths in one pass, then a token of every request a step.
+    ``axis_of``: the position axis of each rotary frequency (``paged.rope_sections``); ``window``: the last queries of a prompt that
+    its slots' weights come from, where the cache evicts."""
+
+    def __init__(self, shape: ModelShape, cache, batch: int, max_positions: int, device, dtype=torch.bfloat16, seed: int = 0,
+                 std: float = 0.02, layers: int | None = None, axis_of=None, window: int = 32):
+        super().__init__(shape, cache, batch, max_positions, device, dtype, seed, std, layers)
+        self.axis_of = (0,) * 64 if axis_of is None else tuple(axis_of)
+        self.axes, self.window = max(self.axis_of) + 1, window
+        self.positions = torch.zeros((self.axes, batch), dtype=torch.int64, device=device)       # of the next token
+
+    def _layer(self, ldx, residual, x, positions, q, attend, keys=None, values=None):
+        """One layer over the step's rows; ``attend()`` is called with queries, keys and values in place."""
+        s, L = self.shape, self.layers[ldx]
+        normed = torch.empty_like(residual)
+        rmsnorm(residual if x is None else x, L["norm1"], s.rms_eps, normed, residual=None if x is None else residual)
+        self.cache.append(ldx, F.linear(normed, L["wqkv"]), self.cos_sin, positions, self.axis_of, q, keys, values)
+        o = F.linear(attend().view(residual.shape[0], -1), L["wo"])
+        rmsnorm(o, L["norm2"], s.rms_eps, normed, residual=residual)
+        gated = torch.empty((residual.shape[0], s.intermediate), dtype=self.dtype, device=self.device)
+        silu_and_mul(F.linear(normed, L["gate_up"]), gated)
+        return F.linear(gated, L["down"])
+
+    def _logits(self, residual, x):
+        normed = torch.empty_like(residual)
+        rmsnorm(x, self.final_norm, self.shape.rms_eps, normed, residual=residual)
+        logits = F.linear(normed, self.lm_head).float()
+        torch.argmax(logits, dim=-1, out=self.next_ids)
+        self.input_ids.copy_(self.next_ids)
+        return logits
+
+    def prefill_forward(self, prompts, positions=None) -> torch.Tensor:
+        """``prompts``: a tensor of token ids for every request; ``positions``: ``[axes, tokens]`` for each (default: counted up on
+        every axis).  Logits ``[batch, vocab]`` of the last tokens; the cache is brought down to its ``keep`` slots."""
+        from .attn_hub import retroinfer_prefill_attn
+
+        s, counts = self.shape, [int(p.numel()) for p in prompts]
+        if min(counts) < 1:
+            raise ValueError("every prompt has a token")
+        if positions is None:
+            positions = [torch.arange(n, device=self.device).expand(self.axes, n) for n in counts]
+        where = torch.cat(list(positions), 1).to(torch.int64).contiguous()
+        self.positions.copy_(torch.stack([p.max() + 1 for p in positions]).expand(self.axes, -1))
+        rows = sum(counts)
+        starts = [sum(counts[:i]) for i in range(len(counts))]
+        new = lambda heads: torch.empty((rows, heads, s.head_dim), dtype=self.dtype, device=self.device)  # noqa: E731
+        q, k, v = new(s.q_heads), new(s.kv_heads), new(s.kv_heads)
+        residual = self.embed[torch.cat(list(prompts)).to(self.device)]
+        recent = torch.zeros((self.batch, self.window, s.q_heads, s.head_dim), dtype=self.dtype, device=self.device)
+        self.cache.begin(counts)
+        x = None
+        for ldx in range(self.n_layers):
+            def attend():
+                return torch.cat([retroinfer_prefill_attn(*(t[None, i:i + n] for t in (q, k, v)), True)[0]
+                                  for i, n in zip(starts, counts)])
+            x = self._layer(ldx, residual, x, where, q, attend, k, v)
+            if self.cache.keep is not None:
+                for b, (i, n) in enumerate(zip(starts, counts)):
+                    w = min(n, self.window)
+                    recent[b, self.window - w:] = q[i + n - w:i + n]
+                self.cache.observe(recent, ldx)
+        self.cache.evict(slack=0)
+        last = torch.tensor([i + n - 1 for i, n in zip(starts, counts)], device=self.device)
+        return self._logits(residual[last], x[last])
+
+    def decode_forward(self) -> torch.Tensor:
+        """One token of every request: logits ``[batch, vocab]``, the greedy next ids become ``input_ids``."""
+        torch.index_select(self.embed, 0, self.input_ids, out=self.residual)
+        self.cache.begin(1)
+        x, q = None, self.q.view(self.batch, self.shape.q_heads, self.shape.head_dim)
+        for ldx in range(self.n_layers):
+            x = self._layer(ldx, self.residual, x, self.positions, q, lambda: self.cache.attend(self.q, ldx, out=self.attn))
+        self.cache.evict()
+        self.positions.add_(1)
+        return self._logits(self.residual, x)

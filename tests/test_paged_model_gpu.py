@@ -1,0 +1,137 @@
+"""The operators over a paged cache together: a small model that takes prompts with images and generates, against the same model in
+32 bits recomputed over the whole sequence; and what eviction does to its cache."""
+import pytest
+import torch
+
+from paged_helpers import DIM
+
+pytestmark = pytest.mark.gpu
+
+
+def small(window=16, keep=None, slack=8, page=16, pages=None, batch=3, layers=2, max_length=600):
+    from retrievalattention_b200.cache_hub import paged_cache
+    from retrievalattention_b200.decode_layer import ModelShape, PagedDecoder
+    from retrievalattention_b200.paged import rope_sections
+
+    shape = ModelShape(256, 512, 1000, layers, 8, 2, rope_theta=1e4)
+    cache = paged_cache(layers, batch, max_length, 2, 8, DIM, torch.bfloat16, {str(i): "cuda:0" for i in range(layers)}, 1, 1,
+                        page_size=page, num_pages=pages, keep=keep, sink=2, recent=12, slack=slack)
+    return PagedDecoder(shape, cache, batch, 2000, "cuda", seed=3, std=0.05, axis_of=rope_sections(16, 24, 24), window=window)
+
+
+def with_image(n):
+    """Positions of n tokens, an image of 4 x 5 patches from token 6 on where there is room."""
+    p = torch.arange(n).expand(3, n).clone()
+    if n > 26:
+        p[:, 6:26] = torch.stack([torch.full((20,), 6), 6 + torch.arange(20) // 5, 6 + torch.arange(20) % 5])
+        p[:, 26:] -= 15
+    return p.cuda()
+
+
+def in_32_bits(model, ids, positions):
+    """Logits of the last token, everything recomputed."""
+    s = model.shape
+    norm = lambda x, w: x * torch.rsqrt(x.square().mean(-1, keepdim=True) + s.rms_eps) * w.float()  # noqa: E731
+    axis = torch.tensor(model.axis_of, device="cuda")
+    i = torch.arange(64, device="cuda")
+    angle = model.cos_sin[positions]
+    c, z = angle[axis, :, i].t()[:, None], angle[axis, :, 64 + i].t()[:, None]
+    x = model.embed[ids].float()
+    for L in model.layers:
+        heads = (norm(x, L["norm1"]) @ L["wqkv"].float().t()).view(len(ids), -1, DIM)
+        a, b = heads[:, :10, :64], heads[:, :10, 64:]
+        turned = torch.cat([a * c - b * z, b * c + a * z], -1)
+        q, k = turned[:, :8].transpose(0, 1), turned[:, 8:].transpose(0, 1).repeat_interleave(4, 0)
+        v = heads[:, 10:].transpose(0, 1).repeat_interleave(4, 0)
+        w = (q @ k.transpose(1, 2)) * DIM ** -0.5
+        w = w.masked_fill(torch.ones_like(w[0], dtype=torch.bool).triu(1), float("-inf")).softmax(-1)
+        x = x + (w @ v).transpose(0, 1).reshape(len(ids), -1) @ L["wo"].float().t()
+        g, u = (norm(x, L["norm2"]) @ L["gate_up"].float().t()).chunk(2, -1)
+        x = x + (torch.nn.functional.silu(g) * u) @ L["down"].float().t()
+    return (norm(x, model.final_norm) @ model.lm_head.float().t())[-1]
+
+
+def test_prompts_and_steps_against_32_bits():
+    model = small()
+    gen = torch.Generator().manual_seed(1)
+    counts = (37, 5, 90)
+    prompts = [torch.randint(0, 1000, (n,), generator=gen).cuda() for n in counts]
+    positions = [with_image(n) for n in counts]
+    logits = model.prefill_forward(prompts, positions)
+    ids = [list(p) for p in prompts]
+    for step in range(20):
+        for b in range(3):
+            want = in_32_bits(model, torch.stack(ids[b]), positions[b])
+            # 16-bit activations of two layers: 2^-8 a rounding, a dozen of them one behind the other
+            assert (logits[b] - want).norm() <= 0.05 * want.norm(), (step, b)
+            ids[b].append(model.input_ids[b].clone())
+            positions[b] = torch.cat([positions[b], (positions[b].max() + 1).expand(3, 1)], 1)
+        logits = model.decode_forward()
+    assert model.cache.lengths.tolist() == [n + 20 for n in counts] == model.cache.length_of
+    assert model.cache.free_pages == model.cache.num_pages - sum(-(-(n + 20) // 16) for n in counts)
+
+
+def test_eviction_holds_requests_to_their_slots_and_gives_pages_back():
+    from retrievalattention_b200.attn_hub.retroinfer_attn import check_prefill_errors
+
+    keep, slack = 40, 8
+    model = small(keep=keep, slack=slack)
+    cache, counts = model.cache, (37, 5, 200)
+    gen = torch.Generator().manual_seed(2)
+    model.prefill_forward([torch.randint(0, 1000, (n,), generator=gen).cuda() for n in counts])
+    assert cache.lengths.tolist() == [37, 5, keep] == cache.length_of
+    assert cache.free_pages == cache.num_pages - (3 + 1 + 3)
+    evicted = 0
+    for step in range(60):
+        logits = model.decode_forward()
+        assert torch.isfinite(logits).all()
+        assert cache.lengths.tolist() == cache.length_of and max(cache.length_of) <= keep + slack
+        seen = [n + step + 1 for n in counts]
+        assert cache.seen_after.tolist() == seen
+        for b in range(3):
+            n = cache.length_of[b]
+            ids = cache.page_table[b, :-(-n // 16)].long()
+            assert ids.tolist() == cache._pages[b]
+            for layer in range(2):
+                tokens = cache.token[layer][ids].transpose(0, 1).reshape(2, -1)[:, :n]
+                weight = cache.weight[layer][ids].transpose(0, 1).reshape(2, -1)[:, :n]
+                for h in range(2):
+                    have = set(tokens[h].tolist())
+                    assert len(have) == n and have <= set(range(seen[b]))
+                    assert set(range(min(2, seen[b]))) <= have and set(range(max(0, seen[b] - 12), seen[b])) <= have
+                assert (weight >= 0).all() and (weight[:, 0] > 0).all()
+        evicted += max(cache.length_of) <= keep
+    assert evicted >= 5
+    check_prefill_errors()
+
+
+def test_a_place_is_taken_by_another_request():
+    model = small(batch=2, pages=12)
+    gen = torch.Generator().manual_seed(3)
+    prompt = lambda n: torch.randint(0, 1000, (n,), generator=gen).cuda()  # noqa: E731
+    model.prefill_forward([prompt(100), prompt(60)])
+    assert model.cache.free_pages == 12 - 7 - 4
+    with pytest.raises(RuntimeError, match="pool has 1 pages left"):
+        model.cache.begin([20, 20])
+    assert model.cache.length_of == [100, 60]                 # nothing was taken
+    model.cache.release(0)
+    assert model.cache.free_pages == 8 and model.cache.length_of == [0, 60]
+    model.cache.begin([5, 1])
+    assert model.cache.lengths.tolist() == [5, 61] and model.cache.held.tolist() == [0, 60]
+    with pytest.raises(RuntimeError, match="more than"):
+        model.cache.begin([600, 0])
+
+
+def test_refusals():
+    from retrievalattention_b200.cache_hub import paged_cache
+
+    one = {"0": "cuda:0"}
+    with pytest.raises(ValueError, match="head_dim"):
+        paged_cache(1, 1, 100, 2, 8, 64, torch.bfloat16, one, 1, 1)
+    with pytest.raises(ValueError, match="keep"):
+        paged_cache(1, 1, 100, 2, 8, 128, torch.bfloat16, one, 1, 1, keep=10)
+    with pytest.raises(ValueError, match="one GPU"):
+        paged_cache(2, 1, 100, 2, 8, 128, torch.bfloat16, {"0": "cuda:0", "1": "cuda:1"}, 1, 1)
+    cache = paged_cache(1, 2, 100, 2, 8, 128, torch.bfloat16, one, 1, 1)
+    with pytest.raises(ValueError, match="every request"):
+        cache.begin([1])
