@@ -7,6 +7,8 @@
 #include <stdint.h>
 #include <stdlib.h>
 
+#include <atomic>
+
 #include "ri_b200.h"
 
 // ---- error reporting (ri_error.cu) ---------------------------------------------------------
@@ -43,6 +45,20 @@ static inline int ri_sm_count(int* out) {
     return RI_OK;
   }
   *out = cached[dev];
+  return RI_OK;
+}
+
+// Let KERNEL have `bytes` of dynamic shared memory (asked for once per device; again where the device is not remembered).
+template <auto KERNEL>
+inline int ri_allow_smem(int bytes) {
+  static std::atomic<bool> known[64];
+  int dev = 0;
+  RI_CUDA_OK(cudaGetDevice(&dev));
+  const bool track = dev >= 0 && dev < 64;
+  if (!track || !known[dev].load(std::memory_order_relaxed)) {
+    RI_CUDA_OK(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (track) known[dev].store(true, std::memory_order_relaxed);
+  }
   return RI_OK;
 }
 

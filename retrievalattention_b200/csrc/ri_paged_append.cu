@@ -4,19 +4,25 @@
 // One axis is the ordinary rotary embedding; text, images and video take (time, height, width).
 // (reference: model_hub/llama.py:232-235 the split, :312-320 the rotation; cache_hub/flash_attn_cache.py:133-151 the append)
 //
-// Bound by the projection, read once and written once.  One CTA per row: a head is sixteen 16-byte pieces, a half-warp per
-// head, and a piece's partner (the channels 64 away) comes by shuffle.  The row's 128 cosines and sines are fetched once, each
-// by its own axis, and serve all heads from shared memory; they and the row's place in the cache (request, slot, page: three
-// dependent loads) come in while the row's pieces do.
+// Bound by the projection, read once and written once.  A row of it lies in one piece and comes in by one bulk copy, four
+// rows on their way to each of four CTAs of an SM.  Two warps issue the copies and fetch what the rows need beside them: 128
+// cosines and sines, each by its own axis, which serve all heads from shared memory, and the row's place in the cache (request,
+// slot, page: three loads that depend on one another).  Eight warps rotate, a half-warp per head and 16 bytes per lane.
+// Every wait is bounded; one that runs out is recorded in the status word.
 #include "ri_paged.cuh"
+#include "ri_tc.cuh"
 
 namespace {
 
 using namespace ri_page;
+using namespace ri_tc;
 
-constexpr int kAppendThreads = 256;
-constexpr int kHeadsAtOnce = kAppendThreads / 16;      // one round of the CTA
-constexpr int kRounds = 4;                             // rounds whose loads are in flight together
+constexpr int kWorkWarps = 8, kServiceWarps = 2;
+constexpr int kWorkThreads = kWorkWarps * 32;
+constexpr int kAppendThreads = kWorkThreads + kServiceWarps * 32;
+constexpr int kAppendCtas = 4;                         // of an SM
+constexpr int kStages = 4;                             // units on their way to a CTA
+constexpr int kUnitHeads = 48;                         // 12 KB
 
 struct AxisOf {
   uint8_t of[64];
@@ -35,7 +41,7 @@ struct AppendArgs {
   uint4* values;
   int64_t qkv_stride;           // 16-byte pieces
   int64_t max_positions;
-  int rows, hq;
+  int rows, hq, unit_heads, units_per_row;
   AxisOf axis;
 };
 
@@ -56,101 +62,138 @@ __device__ __forceinline__ uint4 rotate(const uint4& mine, const uint4& other, c
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kAppendThreads) rope_append_kernel(const __grid_constant__ AppendArgs a) {
-  __shared__ float s_cs[128];
-  __shared__ int s_id, s_row, s_token;
-  ri_pdl_enter();
+// What a row needs beside its pieces, fetched by a service warp.
+struct alignas(16) RowPlan {
+  float cs[128];             // cosines, sines; read 16 bytes at a time
+  int id, row, token;        // page (-1: none), row in it, token number
+};
+
+__device__ __forceinline__ void plan_row(const AppendArgs& a, int row, int lane, RowPlan& plan) {
   const Pages& p = a.pages;
-  const int row = blockIdx.x, tid = threadIdx.x, c = tid & 15, first = tid >> 4;
-  const int heads = a.hq + 2 * p.hk;
-  const uint4* src = a.qkv + row * a.qkv_stride;
-  uint4 x[kRounds];
-#pragma unroll
-  for (int u = 0; u < kRounds; ++u) {
-    const int head = first + u * kHeadsAtOnce;
-    x[u] = head < heads ? ri_ldg16(src + head * 16 + c) : make_uint4(0, 0, 0, 0);
+  int b = row;
+  if (a.row_start != nullptr) {
+    b = 0;
+    for (int b0 = 0;; b0 += 32) {                      // requests that end at or before this row
+      const bool passed = b0 + lane < p.batch && a.row_start[b0 + lane + 1] <= row;
+      const unsigned votes = __ballot_sync(0xffffffffu, passed);
+      b += __popc(votes);
+      if (votes != 0xffffffffu) break;
+    }
   }
-  if (tid < 128) {
-    int64_t pos = a.positions[(int64_t)a.axis.of[tid & 63] * a.rows + row];
+  float cs[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int64_t pos = a.positions[(int64_t)a.axis.of[lane + 32 * i] * a.rows + row];
     pos = pos < 0 ? 0 : (pos >= a.max_positions ? a.max_positions - 1 : pos);
-    s_cs[tid] = a.cos_sin[pos * 128 + tid];
-  } else if (tid >= kAppendThreads - 32) {             // the last warp: which request, slot and page
-    const int lane = tid & 31;
-    int b = row;
-    if (a.row_start != nullptr) {
-      b = 0;
-      for (int b0 = 0;; b0 += 32) {                    // requests that end at or before this row
-        const bool passed = b0 + lane < p.batch && a.row_start[b0 + lane + 1] <= row;
-        const unsigned votes = __ballot_sync(0xffffffffu, passed);
-        b += __popc(votes);
-        if (votes != 0xffffffffu) break;
+    cs[i] = a.cos_sin[pos * 128 + lane + 32 * i];
+    cs[2 + i] = a.cos_sin[pos * 128 + 64 + lane + 32 * i];
+  }
+  if (lane == 0) {
+    plan.id = -1;
+    plan.row = plan.token = 0;
+    const int i = b < p.batch ? row - (a.row_start != nullptr ? a.row_start[b] : b) : -1;
+    if (i >= 0) {                                      // rows that belong to no request are rotated, no more
+      const int64_t slot = (int64_t)max(p.lengths[b], 0) + i;
+      if (slot < ((int64_t)p.table_stride << p.shift)) {
+        plan.id = page_to_write(p, b, (int)(slot >> p.shift));
+        plan.row = (int)slot & ((1 << p.shift) - 1);
+        plan.token = (a.seen != nullptr ? a.seen[b] : (int)slot - i) + i;
+      } else {
+        *p.status = RI_STATUS_PAGES_FULL;
       }
     }
-    if (lane == 0) {
-      s_id = -1;
-      s_row = s_token = 0;
-      const int i = b < p.batch ? row - (a.row_start != nullptr ? a.row_start[b] : b) : -1;
-      if (i >= 0) {                                    // rows that belong to no request are rotated, no more
-        const int64_t slot = (int64_t)max(p.lengths[b], 0) + i;
-        if (slot < ((int64_t)p.table_stride << p.shift)) {
-          s_id = page_to_write(p, b, (int)(slot >> p.shift));
-          s_row = (int)slot & ((1 << p.shift) - 1);
-          s_token = (a.seen != nullptr ? a.seen[b] : (int)slot - i) + i;
-        } else {
-          *p.status = RI_STATUS_PAGES_FULL;
-        }
-      }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) plan.cs[lane + 32 * i] = cs[i];
+}
+
+// Work goes by units: a row, or an equal part of its heads where there are more than kUnitHeads.
+template <int DT>
+__global__ void __launch_bounds__(kAppendThreads, kAppendCtas) rope_append_kernel(const __grid_constant__ AppendArgs a) {
+  extern __shared__ __align__(128) uint8_t s_rows[];       // [kStages][unit_heads * 256]
+  __shared__ RowPlan s_plan[kStages];
+  __shared__ __align__(8) uint64_t s_full[kStages], s_empty[kStages];
+  __shared__ int s_abort;
+  const Pages& p = a.pages;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int heads = a.hq + 2 * p.hk, unit_bytes = a.unit_heads * 256;
+  if (tid == 0) {
+    s_abort = 0;
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(smem_u32(&s_full[s]), 2);                  // the copy, the plan
+      mbar_init(smem_u32(&s_empty[s]), kWorkWarps);
     }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   __syncthreads();
-  const int id = s_id, at = s_row;
-  float cs[16];                                        // this piece's eight cosines, then its eight sines
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    cs[i] = s_cs[(c & 7) * 8 + i];
-    cs[8 + i] = s_cs[64 + (c & 7) * 8 + i];
-  }
-  const float sign = c < 8 ? -1.f : 1.f;
-  if (id >= 0) {
-    for (int h = tid; h < p.hk; h += kAppendThreads) {
-      if (p.weight != nullptr) p.weight[record_at(p, id, h, at)] = 0.f;
-      if (p.token != nullptr) p.token[record_at(p, id, h, at)] = s_token;
+  volatile int* abort_flag = &s_abort;
+  ri_pdl_enter();
+  const int units = a.rows * a.units_per_row, mine = ((int)blockIdx.x < units) ? (units - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+  auto unit = [&](int i) { return (int)blockIdx.x + i * (int)gridDim.x; };
+  bool ok = true;
+  if (warp >= kWorkWarps) {
+    // ---------------- service warps: every second unit each ----------------
+    int i = warp - kWorkWarps;
+    for (; ok && i < mine; i += kServiceWarps) {
+      const int s = i % kStages, u = unit(i), row = u / a.units_per_row, head0 = (u - row * a.units_per_row) * a.unit_heads;
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_empty[s]), ((i / kStages) & 1) ^ 1, abort_flag, 91));
+      if (!ok) break;
+      const uint32_t full = smem_u32(&s_full[s]), bytes = (uint32_t)min(a.unit_heads, heads - head0) * 256;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(full, bytes);
+        bulk_load(smem_u32(s_rows) + s * unit_bytes, a.qkv + row * a.qkv_stride + head0 * 16, bytes, full);
+      }
+      plan_row(a, row, lane, s_plan[s]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full);
     }
-  }
-  for (int base = 0; base < heads; base += kRounds * kHeadsAtOnce) {
+    if (!ok && lane == 0)      // give this warp's copies in flight a bounded chance to land before the CTA exits
+      for (int j = i - kServiceWarps; j >= 0 && j >= i - kStages; j -= kServiceWarps)
+        mbar_wait(smem_u32(&s_full[j % kStages]), (j / kStages) & 1, abort_flag, 92);
+  } else {
+    const int c = tid & 15, half = tid >> 4;
+    const float sign = c < 8 ? -1.f : 1.f;
+    for (int i = 0; ok && i < mine; ++i) {
+      const int s = i % kStages, u = unit(i), row = u / a.units_per_row, head0 = (u - row * a.units_per_row) * a.unit_heads;
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[s]), (i / kStages) & 1, abort_flag, 93));
+      if (!ok) break;
+      const RowPlan& plan = s_plan[s];
+      const int id = plan.id, at = plan.row, n = min(a.unit_heads, heads - head0);
+      const uint4* src = reinterpret_cast<const uint4*>(s_rows + s * unit_bytes);
+      float cs[16];                                    // this piece's eight cosines, then its eight sines
 #pragma unroll
-    for (int u = 0; u < kRounds; ++u) {
-      const int head = base + first + u * kHeadsAtOnce;
-      uint4 other;
-      other.x = __shfl_xor_sync(0xffffffffu, x[u].x, 8);
-      other.y = __shfl_xor_sync(0xffffffffu, x[u].y, 8);
-      other.z = __shfl_xor_sync(0xffffffffu, x[u].z, 8);
-      other.w = __shfl_xor_sync(0xffffffffu, x[u].w, 8);
-      if (head >= heads) continue;
-      const int h = head - a.hq, hv = h - p.hk;
-      const uint4 res = hv >= 0 ? x[u] : rotate<DT>(x[u], other, cs, sign);
-      if (h < 0) {
-        a.q[((int64_t)row * a.hq + head) * 16 + c] = res;
-      } else {
-        uint4* dense = hv >= 0 ? a.v : a.k;
-        if (dense != nullptr) dense[((int64_t)row * p.hk + (hv >= 0 ? hv : h)) * 16 + c] = res;
-        if (id >= 0) {
-          const int64_t in_page = ((int64_t)((hv >= 0 ? hv : h) << p.shift) + at) * 16 + c;
-          if (hv >= 0) a.values[id * (p.value_stride / 8) + in_page] = res;
-          else a.keys[id * (p.key_stride / 8) + in_page] = res;
+      for (int k = 0; k < 4; ++k) {
+        const float4 f = reinterpret_cast<const float4*>(plan.cs)[(k >> 1) * 16 + (c & 7) * 2 + (k & 1)];
+        cs[4 * k] = f.x; cs[4 * k + 1] = f.y; cs[4 * k + 2] = f.z; cs[4 * k + 3] = f.w;
+      }
+      if (id >= 0 && head0 == 0) {
+        for (int h = tid; h < p.hk; h += kWorkThreads) {
+          if (p.weight != nullptr) p.weight[record_at(p, id, h, at)] = 0.f;
+          if (p.token != nullptr) p.token[record_at(p, id, h, at)] = plan.token;
         }
       }
-    }
-    const int next = base + kRounds * kHeadsAtOnce;
-    if (next < heads) {
-#pragma unroll
-      for (int u = 0; u < kRounds; ++u) {
-        const int head = next + first + u * kHeadsAtOnce;
-        x[u] = head < heads ? ri_ldg16(src + head * 16 + c) : make_uint4(0, 0, 0, 0);
+      for (int j = half; j < n; j += kWorkThreads / 16) {
+        const int head = head0 + j, h = head - a.hq, hv = h - p.hk;
+        const uint4 x = src[j * 16 + c];
+        const uint4 res = hv >= 0 ? x : rotate<DT>(x, src[j * 16 + (c ^ 8)], cs, sign);
+        if (h < 0) {
+          a.q[((int64_t)row * a.hq + head) * 16 + c] = res;
+        } else {
+          uint4* dense = hv >= 0 ? a.v : a.k;
+          if (dense != nullptr) dense[((int64_t)row * p.hk + (hv >= 0 ? hv : h)) * 16 + c] = res;
+          if (id >= 0) {
+            const int64_t in_page = ((int64_t)((hv >= 0 ? hv : h) << p.shift) + at) * 16 + c;
+            if (hv >= 0) a.values[id * (p.value_stride / 8) + in_page] = res;
+            else a.keys[id * (p.key_stride / 8) + in_page] = res;
+          }
+        }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&s_empty[s]));
     }
   }
+  if (!ok && lane == 0) *p.status = s_abort;
 }
 
 }  // namespace
@@ -192,7 +235,19 @@ extern "C" int ri_rope_paged_append(const ri_paged* p, const void* d_qkv, int64_
   a.rows = rows;
   a.hq = (int)hq;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  auto go = [&](auto kernel) { return ri_launch_pdl_id(8, kernel, dim3(rows), dim3(kAppendThreads), 0, s, a); };
+  int sms = 0;
+  if ((rc = ri_sm_count(&sms)) != RI_OK) return rc;
+  const int heads = (int)hq + 2 * p->kv_heads;
+  a.units_per_row = (heads + kUnitHeads - 1) / kUnitHeads;
+  a.unit_heads = (heads + a.units_per_row - 1) / a.units_per_row;
+  const int64_t units = (int64_t)rows * a.units_per_row, most = (int64_t)sms * kAppendCtas;
+  RI_REQUIRE(units < (1ll << 30), "ri_rope_paged_append: too large");
+  const dim3 grid((unsigned)(units < most ? units : most));
+  const size_t smem = (size_t)kStages * a.unit_heads * 256;
+  constexpr int kMost = kStages * kUnitHeads * 256;
+  if ((rc = p->dtype == RI_BF16 ? ri_allow_smem<rope_append_kernel<RI_BF16>>(kMost) : ri_allow_smem<rope_append_kernel<RI_F16>>(kMost)) != RI_OK)
+    return rc;
+  auto go = [&](auto kernel) { return ri_launch_pdl_id(8, kernel, grid, dim3(kAppendThreads), smem, s, a); };
   RI_CUDA_OK(p->dtype == RI_BF16 ? go(rope_append_kernel<RI_BF16>) : go(rope_append_kernel<RI_F16>));
   return RI_OK;
 }

@@ -13,8 +13,6 @@
 // A second kernel merges a group's partial results by log-sum-exp in a fixed order.  For the weights the first kernel
 // leaves the scores behind (4 bytes a slot and query head, against 512 a slot for K and V), and a third turns them into
 // probabilities once lse is known; every slot has one thread, so the sums have one order and no atomics.
-#include <atomic>
-
 #include "ri_paged.cuh"
 #include "ri_step_sequence.cuh"
 #include "ri_tc.cuh"
@@ -394,14 +392,8 @@ int make_page_map(CUtensorMap* map, const void* base, const ri_paged& p, int64_t
 
 template <int DT, int BOX, bool WEIGHTS>
 int launch_paged(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t s) {
-  static std::atomic<bool> known[64];                   // per device; asked for again where it is not remembered
-  int dev = 0;
-  RI_CUDA_OK(cudaGetDevice(&dev));
-  const bool track = dev >= 0 && dev < 64;
-  if (!track || !known[dev].load(std::memory_order_relaxed)) {
-    RI_CUDA_OK(cudaFuncSetAttribute(paged_decode_kernel<DT, BOX, WEIGHTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPagedSmem));
-    if (track) known[dev].store(true, std::memory_order_relaxed);
-  }
+  int rc;
+  if ((rc = ri_allow_smem<paged_decode_kernel<DT, BOX, WEIGHTS>>(kPagedSmem)) != RI_OK) return rc;
   RI_CUDA_OK(ri_launch_pdl_id(11, paged_decode_kernel<DT, BOX, WEIGHTS>, dim3(a.max_ctas), dim3(kPagedThreads), (size_t)kPagedSmem,
                               s, map_k, map_v, a));
   RI_CUDA_OK(ri_launch_pdl_id(11, paged_join_kernel<DT>, dim3(a.gs, a.batch * a.hk), dim3(kJoinThreads), 0, s, a));

@@ -13,8 +13,6 @@
 // Moves: a half-warp per row, four rows in flight.  Bound by the moved rows, read once and written once.
 #include <cooperative_groups.h>
 
-#include <atomic>
-
 #include "ri_paged.cuh"
 
 namespace {
@@ -242,14 +240,7 @@ extern "C" int ri_paged_evict(const ri_paged* p, const int32_t* d_seen, int32_t 
   a.most = (int)most_moves(*p, keep);
   int sms = 0;
   if ((rc = ri_sm_count(&sms)) != RI_OK) return rc;
-  static std::atomic<bool> known[64];
-  int dev = 0;
-  RI_CUDA_OK(cudaGetDevice(&dev));
-  const bool track = dev >= 0 && dev < 64;
-  if (!track || !known[dev].load(std::memory_order_relaxed)) {
-    RI_CUDA_OK(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kCachedKeys * 4));
-    if (track) known[dev].store(true, std::memory_order_relaxed);
-  }
+  if ((rc = ri_allow_smem<evict_select_kernel>(kCachedKeys * 4)) != RI_OK) return rc;
   int ctas = 1;                                        // as many CTAs to a group as fit the chip at once
   while (ctas < kSelMaxCluster && groups * ctas * 2 <= sms) ctas *= 2;
   const int64_t slice = (room + ctas - 1) / ctas;

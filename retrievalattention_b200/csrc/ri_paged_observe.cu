@@ -16,8 +16,6 @@
 // status word.  Bound by the exponentials, two for each slot and query row.
 #include <cuda.h>
 
-#include <atomic>
-
 #include "ri_paged.cuh"
 #include "ri_step_sequence.cuh"
 #include "ri_tc.cuh"
@@ -336,15 +334,9 @@ int make_key_map(CUtensorMap* map, const ri_paged& p) {
 
 template <int DT>
 int launch_observe(ObsArgs a, const CUtensorMap& map_k, cudaStream_t s) {
-  static std::atomic<bool> known[64];                   // per device; asked for again where it is not remembered
-  int dev = 0;
-  RI_CUDA_OK(cudaGetDevice(&dev));
-  const bool track = dev >= 0 && dev < 64;
-  if (!track || !known[dev].load(std::memory_order_relaxed)) {
-    RI_CUDA_OK(cudaFuncSetAttribute(observe_kernel<DT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kObsSmem));
-    RI_CUDA_OK(cudaFuncSetAttribute(observe_kernel<DT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kObsSmem));
-    if (track) known[dev].store(true, std::memory_order_relaxed);
-  }
+  int rc;
+  if ((rc = ri_allow_smem<observe_kernel<DT, true>>(kObsSmem)) != RI_OK) return rc;
+  if ((rc = ri_allow_smem<observe_kernel<DT, false>>(kObsSmem)) != RI_OK) return rc;
   const int rows = a.window * a.gs;
   for (a.first_row = 0; a.first_row < rows; a.first_row += kRows) {
     a.rows = rows - a.first_row < kRows ? rows - a.first_row : kRows;

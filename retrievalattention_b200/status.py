@@ -32,7 +32,8 @@ def word(device) -> C.c_int32:
 def _kernel(code: int) -> str:
     # what the kernels' waits are numbered by; a second bound of a wait, by count, adds 100
     return {2: "ri_prefill_attn", 3: "ri_prefill_attn", 4: "ri_dense_decode", 5: "ri_wave_decode_layer",
-            7: "ri_paged_decode", 8: "ri_paged_observe"}.get(code % 100 // 10, "a kernel")
+            7: "ri_paged_decode", 8: "ri_paged_observe",
+            9: "ri_rope_paged_append"}.get(code % 100 // 10, "a kernel")
 
 
 def check() -> None:

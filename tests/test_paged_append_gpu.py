@@ -96,6 +96,9 @@ def sections(*n):
     ((100,), [130], 8, 8, 64, torch.bfloat16, (10, 20, 30, 4)),                     # 80 heads: two rounds of a CTA
     ((3,) * 40, [1] * 40, 1, 8, 16, torch.bfloat16, (16, 24, 24)),                  # more requests than lanes
     ((1,) * 64, [2] * 64, 1, 1, 8, torch.float16, (64,)),                           # two full rounds of requests
+    ((333, 9, 0), [1501, 77, 40], 2, 3, 32, torch.float16, (16, 24, 24)),           # several rows to a CTA
+    ((64, 1), [700, 1], 8, 4, 16, torch.bfloat16, (24, 20, 20)),
+    ((0,), [1333], 8, 8, 128, torch.bfloat16, (64,)),                               # the same with two rounds a row
 ])
 def test_rows_and_places(lengths, counts, kv_heads, group, page, dtype, axes):
     layer = Layer(lengths, kv_heads, page, dtype, seed=1, room=max(counts))
