@@ -24,15 +24,15 @@ struct Pages {
 __device__ __forceinline__ int rows_of(const Pages& p, int b) {
   return (int)min((int64_t)max(p.lengths[b], 0), (int64_t)p.table_stride << p.shift);
 }
-// Page i of request b.  A number that names no page is reported, and page 0 stands in for it: nothing outside the pool is
-// touched, and the call's results for that request mean nothing.
+// Page i of request b, for readers.  A number that names no page is reported, and page 0 stands in for it: nothing outside the
+// pool is touched, and the call's results for that request mean nothing.
 __device__ __forceinline__ int page_of(const Pages& p, int b, int i) {
   const int id = p.table[(int64_t)b * p.table_stride + i];
   if ((unsigned)id < (unsigned)p.n_pages) return id;
   *p.status = RI_STATUS_PAGE_ID;
   return 0;
 }
-// The same for writers: -1 where there is no such page.
+// The same for writers: -1 where there is no such page, and nothing is written.
 __device__ __forceinline__ int page_to_write(const Pages& p, int b, int i) {
   const int id = p.table[(int64_t)b * p.table_stride + i];
   if ((unsigned)id < (unsigned)p.n_pages) return id;

@@ -24,6 +24,7 @@ namespace {
 using namespace ri_tc;
 using ri_page::Pages;
 using ri_page::page_of;
+using ri_page::page_to_write;
 using ri_page::record_at;
 using ri_seq::Place;
 using ri_seq::count_steps;
@@ -367,7 +368,8 @@ __global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const __grid_c
   const float* sc = a.scores + (int64_t)(s_first + step) * gs * 16 + i;
   float sum = 0.f;
   for (int h = 0; h < gs; ++h) sum += exp2f(sc[h * 16] - a.lse2[g * gs + h]);
-  a.weight[record_at(a, page_of(a, b, slot >> a.shift), g - b * a.hk, slot & ((1 << a.shift) - 1))] += sum;
+  const int id = page_to_write(a, b, slot >> a.shift);
+  if (id >= 0) a.weight[record_at(a, id, g - b * a.hk, slot & ((1 << a.shift) - 1))] += sum;
 }
 
 int64_t paged_slots(int64_t groups) { return (int64_t)kPagedMaxCtas * kPagedWarps + groups; }

@@ -177,13 +177,15 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
   const int c = threadIdx.x & 15, half = threadIdx.x >> 4;
   const int2* moves = a.moves + (int64_t)g * a.most;
   for (int i0 = blockIdx.x * kMovesPerBlock + half * kMovesAtOnce; i0 < n; i0 += gridDim.x * kMovesPerBlock) {
-    int64_t to_k[kMovesAtOnce], to_v[kMovesAtOnce];
+    int64_t to_k[kMovesAtOnce], to_v[kMovesAtOnce];    // negative: nothing to move
     uint4 k[kMovesAtOnce], v[kMovesAtOnce];
 #pragma unroll
     for (int u = 0; u < kMovesAtOnce; ++u) {
+      to_k[u] = -1;
       if (i0 + u >= n) continue;
       const int2 m = moves[i0 + u];
-      const int id_to = page_of(p, b, m.x >> p.shift), id_of = page_of(p, b, m.y >> p.shift), mask = (1 << p.shift) - 1;
+      const int id_to = page_to_write(p, b, m.x >> p.shift), id_of = page_to_write(p, b, m.y >> p.shift), mask = (1 << p.shift) - 1;
+      if ((id_to | id_of) < 0) continue;
       const int64_t in_to = ((int64_t)(h << p.shift) + (m.x & mask)) * 16 + c, in_of = ((int64_t)(h << p.shift) + (m.y & mask)) * 16 + c;
       to_k[u] = id_to * (p.key_stride / 8) + in_to;
       to_v[u] = id_to * (p.value_stride / 8) + in_to;
@@ -197,7 +199,7 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
     }
 #pragma unroll
     for (int u = 0; u < kMovesAtOnce; ++u) {
-      if (i0 + u >= n) continue;
+      if (to_k[u] < 0) continue;
       a.keys[to_k[u]] = k[u];
       a.values[to_v[u]] = v[u];
     }

@@ -52,6 +52,63 @@ __device__ __forceinline__ float ex2(float x) {       // 2^x; results below 2^-1
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
   return d;
 }
+constexpr float kFarAbove = 1.2676506e30f;            // 2^100
+
+__device__ __forceinline__ void load_scores(uint32_t taddr, uint32_t (&r)[32]) {
+  tc_ld32(taddr, r);
+  tc_wait_ld();
+  tc_ld_landed(r);
+}
+// Sum of 2^(s * scale + shift) over 32 scores, added to `sum`; `shift` holds one value a pair of scores.
+template <class Shift>
+__device__ __forceinline__ void add_exps(const uint32_t (&sr)[32], uint64_t scale, Shift shift, uint64_t (&sum)[2]) {
+#pragma unroll
+  for (int x = 0; x < 16; ++x) {
+    float e0, e1;
+    unpack_f2(fma_f2(pack_f2(__uint_as_float(sr[2 * x]), __uint_as_float(sr[2 * x + 1])), scale, shift(x)), e0, e1);
+    sum[x & 1] = add_f2(sum[x & 1], pack_f2(ex2(e0), ex2(e1)));
+  }
+}
+__device__ __forceinline__ float total_of(const uint64_t (&sum)[2]) {
+  float a, b;
+  unpack_f2(add_f2(sum[0], sum[1]), a, b);
+  return a + b;
+}
+// Pass 1: over a row's 128 scores, one shift for all; the next 32 come down while these are worked on.
+__device__ __forceinline__ float row_sum(uint32_t taddr, float scale, float shift) {
+  const uint64_t scale_2 = pack_f2(scale, scale), shift_2 = pack_f2(shift, shift);
+  uint64_t sum[2] = {0ull, 0ull};
+  uint32_t sr[2][32];
+  tc_ld32(taddr, sr[0]);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    tc_wait_ld();
+    tc_ld_landed(sr[k & 1]);
+    if (k < 3) tc_ld32(taddr + (k + 1) * 32, sr[(k + 1) & 1]);
+    add_exps(sr[k & 1], scale_2, [&](int) { return shift_2; }, sum);
+  }
+  return total_of(sum);
+}
+// Pass 2: over a slot's scores with `chunks` * 32 query rows, a shift for each.
+__device__ __forceinline__ float column_sum(uint32_t taddr, int chunks, float scale, const float* shift) {
+  const uint64_t scale_2 = pack_f2(scale, scale);
+  uint64_t sum[2] = {0ull, 0ull};
+  uint32_t sr[2][32];
+  tc_ld32(taddr, sr[0]);
+  for (int k = 0; k < chunks; k += 2) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (k + u < chunks) {
+        tc_wait_ld();
+        tc_ld_landed(sr[u]);
+        if (k + u + 1 < chunks) tc_ld32(taddr + (k + u + 1) * 32, sr[u ^ 1]);
+        const ulonglong2* at = reinterpret_cast<const ulonglong2*>(shift + (k + u) * 32);
+        add_exps(sr[u], scale_2, [&](int x) { const ulonglong2 two = at[x >> 1]; return (x & 1) ? two.y : two.x; }, sum);
+      }
+    }
+  }
+  return total_of(sum);
+}
 // The last slot that query row `row` sees in a request of n slots (negative: none).
 __device__ __forceinline__ int last_seen(const ObsArgs& a, int n, int row) { return n - a.window + row / a.gs; }
 
@@ -66,7 +123,7 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
   __shared__ __align__(8) uint64_t s_bars[1 + 2 * kRing + 8];
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
-  __shared__ __align__(16) float s_lse[kRows];
+  __shared__ __align__(16) float s_neg_lse[kRows];
   __shared__ __align__(16) int s_last[kRows];
   const uint32_t bars = smem_u32(s_bars);
   const uint32_t bar_q = bars;                                              // the group's query rows are there
@@ -182,7 +239,7 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
             *reinterpret_cast<uint4*>(q_rows + (piece >> 3) * kRowHalf + tid * 128 + (((piece & 7) ^ (tid & 7)) << 4)) = x;
           }
           if (!STATS) {
-            s_lse[tid] = a.lse2[(int64_t)at.g * kRows + tid];
+            s_neg_lse[tid] = -a.lse2[(int64_t)at.g * kRows + tid];
             s_last[tid] = last_seen(a, n, r);
           }
         }
@@ -191,7 +248,7 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
         if (lane == 0) mbar_arrive(bar_q);
         if (STATS) {
           const int r = both ? g * kTile + row : row;
-          const int last = r < a.rows ? min(last_seen(a, n, a.first_row + r), n - 1) : -1;
+          const int last = r < a.rows ? last_seen(a, n, a.first_row + r) : n - 1;      // rows that fill up a tile hold nobody up
           float m = -INFINITY, l = 0.f;
           for (; t < end; ++t, ++used) {
             if (!both && g != (used & 1)) continue;
@@ -199,38 +256,45 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
             ok = ok && __all_sync(0xffffffffu, mbar_wait(bar_s_full(g, i), (done / kBuffers) & 1, abort_flag, 86));
             if (!ok) continue;
             tc_fence_after();
-            uint32_t sr[4][32];
+            const uint32_t scores = tmem + (2 * g + i) * 128 + t_lane;
+            const int slot0 = (t - at.first) * kTile;
+            const bool edge = slot0 + kTile - 1 > last;      // some scores are masked for this row
+            float sum = 0.f;
+            // With a reference from earlier tiles the exponentials need no maximum: it is near this tile's, and where it is
+            // so far below that the sum grows out of hand the tile is done again from its own maximum.
+            bool again = edge || m == -INFINITY;
+            if (!__any_sync(0xffffffffu, again)) {
+              sum = row_sum(scores, a.scale2, -m);
+              again = !(sum < kFarAbove);
+            }
+            if (__any_sync(0xffffffffu, again)) {
+              float mx = -INFINITY;
+#pragma unroll 1
+              for (int k = 0; k < 4; ++k) {
+                uint32_t sr[32];
+                load_scores(scores + k * 32, sr);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) tc_ld32(tmem + (2 * g + i) * 128 + t_lane + k * 32, sr[k]);
-            tc_wait_ld();
+                for (int x = 0; x < 32; ++x)
+                  if (slot0 + k * 32 + x <= last) mx = fmaxf(mx, __uint_as_float(sr[x]));
+              }
+              const float m_new = fmaxf(m, mx * a.scale2);
+              l = m == -INFINITY ? 0.f : l * ex2(m - m_new);
+              m = m_new;
+              sum = 0.f;
+#pragma unroll 1
+              for (int k = 0; k < 4; ++k) {
+                uint32_t sr[32];
+                load_scores(scores + k * 32, sr);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) tc_ld_landed(sr[k]);
+                for (int x = 0; x < 32; ++x)
+                  if (slot0 + k * 32 + x <= last) sum += ex2(__uint_as_float(sr[x]) * a.scale2 - m_new);
+              }
+            }
+            l += sum;
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_s_empty(g, i));
             ++done;
-            const int slot0 = (t - at.first) * kTile;
-            if (slot0 + kTile - 1 > last) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int x = 0; x < 32; ++x)
-                  if (slot0 + k * 32 + x > last) sr[k][x] = 0xff800000u;     // -inf
-            }
-            float mx = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-              for (int x = 0; x < 32; x += 2) mx = max3(mx, __uint_as_float(sr[k][x]), __uint_as_float(sr[k][x + 1]));
-            const float m_new = fmaxf(m, mx * a.scale2);
-            if (m_new == -INFINITY) continue;
-            float sum = 0.f;
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-              for (int x = 0; x < 32; ++x) sum += ex2(__uint_as_float(sr[k][x]) * a.scale2 - m_new);
-            l = l * ex2(m - m_new) + sum;
-            m = m_new;
           }
           a.part[(int64_t)(c + at.g) * kRows + tid] = make_float2(m, l);
         } else {
@@ -239,24 +303,27 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
             const int slot0 = (t - at.first) * kTile, slot = slot0 + row;
             float* weight = nullptr;
             float old = 0.f;
-            if (slot < n) {
-              weight = a.weight + record_at(a, page_of(a, b, slot >> a.shift), h, slot & ((1 << a.shift) - 1));
+            const int id = slot < n ? page_to_write(a, b, slot >> a.shift) : -1;
+            if (id >= 0) {
+              weight = a.weight + record_at(a, id, h, slot & ((1 << a.shift) - 1));
               old = *weight;
             }
             ok = ok && __all_sync(0xffffffffu, mbar_wait(bar_s_full(g, 0), done & 1, abort_flag, 87));
             if (!ok) continue;
             tc_fence_after();
-            const bool edge = slot0 + kTile - 1 > n - a.window;
+            const bool edge = slot0 + kTile - 1 > n - a.window;      // some query rows do not see some of the tile's slots
+            const uint32_t scores = tmem + g * 256 + t_lane;
             float sum = 0.f;
-            for (int k = 0; k * 32 < a.rows; ++k) {
-              uint32_t sr[32];
-              tc_ld32(tmem + g * 256 + t_lane + k * 32, sr);
-              tc_wait_ld();
-              tc_ld_landed(sr);
+            if (!edge) {
+              sum = column_sum(scores, (a.rows + 31) / 32, a.scale2, s_neg_lse);
+            } else {
+#pragma unroll 1
+              for (int k = 0; k * 32 < a.rows; ++k) {
+                uint32_t sr[32];
+                load_scores(scores + k * 32, sr);
 #pragma unroll
-              for (int x = 0; x < 32; ++x) {
-                const float e = ex2(__uint_as_float(sr[x]) * a.scale2 - s_lse[k * 32 + x]);
-                sum += edge && slot > s_last[k * 32 + x] ? 0.f : e;
+                for (int x = 0; x < 32; ++x)
+                  if (slot <= s_last[k * 32 + x]) sum += ex2(__uint_as_float(sr[x]) * a.scale2 + s_neg_lse[k * 32 + x]);
               }
             }
             tc_fence_before();

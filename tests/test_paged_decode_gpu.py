@@ -163,18 +163,19 @@ def test_page_number_outside_the_pool_is_reported():
     from retrievalattention_b200 import paged
     from retrievalattention_b200.attn_hub.retroinfer_attn import check_prefill_errors
 
-    layer = Layer((100, 40), 1, 16, torch.bfloat16, seed=12)
+    layer = Layer((100, 40), 1, 16, torch.bfloat16, seed=12, spare=0)
     q = torch.randn((2, 1, 2, DIM), generator=layer.gen).bfloat16().cuda()
     for bad in (-1, layer.keys.shape[0], 1 << 30):
         table = layer.table.clone()
         table[0, 2] = bad
-        out = torch.empty_like(q)
+        out, weight = torch.empty_like(q), layer.weight.clone()
         check_prefill_errors()
         with pytest.raises(RuntimeError, match="names no page"):       # by the call itself, if the kernel is done by then
-            paged.paged_decode(q, layer.keys, layer.values, table, layer.lengths, out=out, weight=layer.weight.clone())
+            paged.paged_decode(q, layer.keys, layer.values, table, layer.lengths, out=out, weight=weight)
             check_prefill_errors()
-        want = attend(q[1, 0].cpu().double()[None], layer.k[1], layer.v[1])[0][0]
-        assert ((out[1, 0].cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-3).all()       # the other request is served
+        want, _, p = attend(q[1, 0].cpu().double()[None], layer.k[1], layer.v[1])       # the other request is served
+        assert ((out[1, 0].cpu().double() - want[0]).abs() <= 2.0 ** -8 * want[0].abs() + 1e-3).all()
+        assert ((layer.gather(weight, 1).double() - layer.w[1] - p.sum(1)).abs() <= 1e-4 * p.sum(1) + 2.0 ** -22).all()
 
 
 def test_refusals():

@@ -145,6 +145,26 @@ def test_attention_after_eviction_is_that_of_the_slots_that_stayed():
         assert ((out[b, 0].cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-4 * v.abs().max()).all()
 
 
+def test_page_number_outside_the_pool_is_reported_and_other_requests_are_served():
+    from retrievalattention_b200 import paged
+    from retrievalattention_b200.attn_hub.retroinfer_attn import check_prefill_errors
+
+    layer = Layer((100, 90), 2, 16, torch.bfloat16, seed=29, spare=0)
+    want = Layer((100, 90), 2, 16, torch.bfloat16, seed=29, spare=0)
+    run(want, 40, 2, 8)
+    for entry in (0, 4):                                                 # a hole's page, a filler's
+        table = layer.table.clone()
+        table[0, entry] = layer.keys.shape[0] + 5
+        with pytest.raises(RuntimeError, match="names no page"):
+            paged.paged_evict(layer.keys, layer.values, layer.weight, layer.token, table, layer.lengths,
+                              torch.tensor([100, 90], dtype=torch.int32, device="cuda"), 40, 2, 8)
+            check_prefill_errors()
+        for name in ("keys", "values", "weight", "token"):
+            a, b = layer.gather(getattr(layer, name), 1), want.gather(getattr(want, name), 1)
+            assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8)), name
+        layer = Layer((100, 90), 2, 16, torch.bfloat16, seed=29, spare=0)
+
+
 def test_refusals():
     from retrievalattention_b200 import paged
 

@@ -121,7 +121,7 @@ def test_page_number_outside_the_pool_is_reported():
     from retrievalattention_b200 import paged
     from retrievalattention_b200.attn_hub.retroinfer_attn import check_prefill_errors
 
-    layer = Layer((100, 40), 1, 16, torch.bfloat16, seed=37)
+    layer = Layer((100, 40), 1, 16, torch.bfloat16, seed=37, spare=0)
     q = torch.randn((2, 3, 2, DIM), generator=layer.gen).bfloat16().cuda()
     table = layer.table.clone()
     table[0, 2] = layer.keys.shape[0]
