@@ -10,9 +10,10 @@
 // two 128-byte-swizzled halves), only their roles change.  A slot's weight has one thread, so there are no atomics.
 // The split is that of the decode kernels: tiles of 128 slots of all groups behind one another, an equal contiguous range per SM.
 // Pass 1 leaves a (maximum, sum) per row and range; a small kernel between the passes merges them.
-// Four warps bring in tiles, issue the products and idle, eight work on scores: two halves of four, one per tile of
-// query rows in pass 1 (or every second tile of keys, where there is only one), every second tile of keys in pass 2.
-// TMEM: 256 columns of scores for each half.  Every wait is bounded; one that runs out is recorded in the
+// Four warps bring in tiles, issue the products and idle, sixteen work on scores: two sides of eight, one per tile of query
+// rows in pass 1 (or every second tile of keys, where there is only one), every second tile of keys in pass 2; of a side's
+// scores four warps take the first half of the columns and four the second.
+// TMEM: 256 columns of scores for each side.  Every wait is bounded; one that runs out is recorded in the
 // status word.  Bound by the exponentials, two for each slot and query row.
 #include <cuda.h>
 
@@ -31,7 +32,9 @@ constexpr int kRows = 256;                       // query rows that are worked o
 constexpr int kKeyHalf = kTile * 128, kKeyTile = 2 * kKeyHalf;
 constexpr int kRowHalf = kRows * 128, kRowTile = 2 * kRowHalf;
 constexpr int kRing = 4;                         // K tiles in shared memory
-constexpr int kObsThreads = 384;
+constexpr int kScoreWarps = 16, kScoreThreads = kScoreWarps * 32;
+constexpr int kObsThreads = 128 + kScoreThreads;
+constexpr int kPartials = 2 * kRows;             // a (maximum, sum) for each row and half of the columns
 constexpr uint32_t kTmemCols = 512;
 constexpr int kObsSmem = 1024 + kRowTile + kRing * kKeyTile;
 constexpr int kObsMaxCtas = 160;
@@ -39,7 +42,7 @@ constexpr int kObsMaxCtas = 160;
 struct ObsArgs : Pages {
   static constexpr int kStep = kTile;
   const uint4* q;                                // [batch][window][hk * gs][16 pieces]
-  float2* part;                                  // [slots][kRows]: (maximum in the log2 domain, sum)
+  float2* part;                                  // [slots][half][kRows]: (maximum in the log2 domain, sum)
   float* lse2;                                   // [groups][kRows]; +infinity: the row gives nothing
   int window, gs, first_row, rows;               // rows first_row .. first_row + rows - 1 of window * gs
   int max_ctas;
@@ -59,14 +62,43 @@ __device__ __forceinline__ void load_scores(uint32_t taddr, uint32_t (&r)[32]) {
   tc_wait_ld();
   tc_ld_landed(r);
 }
+// 2^x for a pair on the FMA pipe: 2^n * p(x - n), n the nearest whole number, p the polynomial of degree 5 that is nearest to
+// 2^f on [-1/2, 1/2] in relative error (found by Remez's exchange; with 32-bit Horner steps 2.2e-7, as ex2.approx).  From 2^-126
+// to 2^126; NaN gives 2^126.
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
+  constexpr float kWhole = 12582912.f;                 // 1.5 * 2^23: a sum with it has the whole number in its low bits
+  float x0, x1, t0, t1, p0, p1;
+  unpack_f2(x, x0, x1);
+  x = pack_f2(fmaxf(fminf(x0, 126.f), -126.f), fmaxf(fminf(x1, 126.f), -126.f));
+  const uint64_t t = add_f2(x, pack_f2(kWhole, kWhole));
+  const uint64_t f = fma_f2(add_f2(t, pack_f2(-kWhole, -kWhole)), pack_f2(-1.f, -1.f), x);
+  auto both = [](float c) { return pack_f2(c, c); };
+  uint64_t p = fma_f2(both(0.001327647199f), f, both(0.009675541334f));
+  p = fma_f2(p, f, both(0.05550713273f));
+  p = fma_f2(p, f, both(0.2402211972f));
+  p = fma_f2(p, f, both(0.6931469671f));
+  p = fma_f2(p, f, both(1.000000072f));
+  unpack_f2(t, t0, t1);
+  unpack_f2(p, p0, p1);
+  return pack_f2(__int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23)), __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23)));
+}
+#ifndef V_POLY
+#define V_POLY 0
+#endif
+constexpr int kPolynomials = V_POLY;        // of 16 pairs
 // Sum of 2^(s * scale + shift) over 32 scores, added to `sum`; `shift` holds one value a pair of scores.
 template <class Shift>
 __device__ __forceinline__ void add_exps(const uint32_t (&sr)[32], uint64_t scale, Shift shift, uint64_t (&sum)[2]) {
 #pragma unroll
   for (int x = 0; x < 16; ++x) {
-    float e0, e1;
-    unpack_f2(fma_f2(pack_f2(__uint_as_float(sr[2 * x]), __uint_as_float(sr[2 * x + 1])), scale, shift(x)), e0, e1);
-    sum[x & 1] = add_f2(sum[x & 1], pack_f2(ex2(e0), ex2(e1)));
+    const uint64_t e = fma_f2(pack_f2(__uint_as_float(sr[2 * x]), __uint_as_float(sr[2 * x + 1])), scale, shift(x));
+    if ((x + 1) * kPolynomials / 16 != x * kPolynomials / 16) {
+      sum[x & 1] = add_f2(sum[x & 1], exp2_pair(e));
+    } else {
+      float e0, e1;
+      unpack_f2(e, e0, e1);
+      sum[x & 1] = add_f2(sum[x & 1], pack_f2(ex2(e0), ex2(e1)));
+    }
   }
 }
 __device__ __forceinline__ float total_of(const uint64_t (&sum)[2]) {
@@ -74,18 +106,15 @@ __device__ __forceinline__ float total_of(const uint64_t (&sum)[2]) {
   unpack_f2(add_f2(sum[0], sum[1]), a, b);
   return a + b;
 }
-// Pass 1: over a row's 128 scores, one shift for all; the next 32 come down while these are worked on.
+// Pass 1: over 64 scores of a row, one shift for all.
 __device__ __forceinline__ float row_sum(uint32_t taddr, float scale, float shift) {
   const uint64_t scale_2 = pack_f2(scale, scale), shift_2 = pack_f2(shift, shift);
   uint64_t sum[2] = {0ull, 0ull};
-  uint32_t sr[2][32];
-  tc_ld32(taddr, sr[0]);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    tc_wait_ld();
-    tc_ld_landed(sr[k & 1]);
-    if (k < 3) tc_ld32(taddr + (k + 1) * 32, sr[(k + 1) & 1]);
-    add_exps(sr[k & 1], scale_2, [&](int) { return shift_2; }, sum);
+  for (int k = 0; k < 2; ++k) {
+    uint32_t sr[32];
+    load_scores(taddr + k * 32, sr);
+    add_exps(sr, scale_2, [&](int) { return shift_2; }, sum);
   }
   return total_of(sum);
 }
@@ -93,19 +122,12 @@ __device__ __forceinline__ float row_sum(uint32_t taddr, float scale, float shif
 __device__ __forceinline__ float column_sum(uint32_t taddr, int chunks, float scale, const float* shift) {
   const uint64_t scale_2 = pack_f2(scale, scale);
   uint64_t sum[2] = {0ull, 0ull};
-  uint32_t sr[2][32];
-  tc_ld32(taddr, sr[0]);
-  for (int k = 0; k < chunks; k += 2) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if (k + u < chunks) {
-        tc_wait_ld();
-        tc_ld_landed(sr[u]);
-        if (k + u + 1 < chunks) tc_ld32(taddr + (k + u + 1) * 32, sr[u ^ 1]);
-        const ulonglong2* at = reinterpret_cast<const ulonglong2*>(shift + (k + u) * 32);
-        add_exps(sr[u], scale_2, [&](int x) { const ulonglong2 two = at[x >> 1]; return (x & 1) ? two.y : two.x; }, sum);
-      }
-    }
+#pragma unroll 1
+  for (int k = 0; k < chunks; ++k) {
+    uint32_t sr[32];
+    load_scores(taddr + k * 32, sr);
+    const ulonglong2* at = reinterpret_cast<const ulonglong2*>(shift + k * 32);
+    add_exps(sr, scale_2, [&](int x) { const ulonglong2 two = at[x >> 1]; return (x & 1) ? two.y : two.x; }, sum);
   }
   return total_of(sum);
 }
@@ -115,7 +137,7 @@ __device__ __forceinline__ int last_seen(const ObsArgs& a, int n, int row) { ret
 // STATS: pass 1.
 template <int DT, bool STATS>
 __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ ObsArgs a) {
-  constexpr int kBuffers = STATS ? 2 : 1;        // of scores, for each half of the score warps: 128 columns each, or 256
+  constexpr int kBuffers = STATS ? 2 : 1;        // of scores, for each side of the score warps: 128 columns each, or 256
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* q_rows = smem_raw + (base - smem_u32(smem_raw));
@@ -125,6 +147,8 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
   __shared__ int s_abort;
   __shared__ __align__(16) float s_neg_lse[kRows];
   __shared__ __align__(16) int s_last[kRows];
+  __shared__ float s_sum[2][2][kTile];             // pass 2: what the second half of the query rows gives
+  __shared__ int s_nan;                            // some row's lse is no number
   const uint32_t bars = smem_u32(s_bars);
   const uint32_t bar_q = bars;                                              // the group's query rows are there
   auto bar_full = [&](int s) { return bars + 8u * (1 + s); };               // a K tile is there, is free
@@ -134,10 +158,10 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     s_abort = 0;
-    mbar_init(bar_q, 8);
+    mbar_init(bar_q, kScoreWarps);
     for (int s = 0; s < kRing; ++s) { mbar_init(bar_full(s), 1); mbar_init(bar_empty(s), 1); }
     for (int g = 0; g < 2; ++g)
-      for (int i = 0; i < 2; ++i) { mbar_init(bar_s_full(g, i), 1); mbar_init(bar_s_empty(g, i), 4); }
+      for (int i = 0; i < 2; ++i) { mbar_init(bar_s_full(g, i), 1); mbar_init(bar_s_empty(g, i), kScoreWarps / 2); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -155,7 +179,7 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
   // this CTA's tiles [lo, hi) of the sequence, segment by segment (the part of a group that falls to it)
   const int total = ri_seq::count_steps(a), n_ctas = min(a.max_ctas, total), c = (int)blockIdx.x;
   const int lo = c < n_ctas ? ri_seq::cta_start(c, total, n_ctas) : 0, hi = c < n_ctas ? ri_seq::cta_start(c + 1, total, n_ctas) : 0;
-  // both halves of the score warps work on the same keys where there are query rows for both, on every second tile otherwise
+  // both sides of the score warps work on the same keys where there are query rows for both, on every second tile otherwise
   const bool both = STATS && a.rows > kTile;
 
   if (lo < hi) {
@@ -218,33 +242,47 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
       }
     } else if (warp >= 4) {
       // ---------------- scores ----------------
-      const int g = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane, tid = threadIdx.x - 128;
+      const int side = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, quarter = warp & 3, row = quarter * 32 + lane;
+      const int tid = threadIdx.x - 128, g = side;
       const uint32_t t_lane = (uint32_t)(quarter * 32) << 16;
       Place at = ri_seq::find_place(a, lo);
       bool ok = true;
-      int done = 0, used = 0;                          // tiles of this half, of the CTA
+      int done = 0, used = 0;                          // tiles of this side, of the CTA
       for (int t = lo; t < hi;) {
         while (t >= at.first + ri_seq::steps_of<kTile>(at.rows)) ri_seq::next_place(a, at);
         const int end = min(hi, at.first + ri_seq::steps_of<kTile>(at.rows)), n = at.rows;
         const int b = at.g / a.hk, h = at.g - b * a.hk;
-        // the group's query rows: a thread brings a row, its pieces swizzled as TMA would; every product over the rows before
-        // has completed, since its scores have been read
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        // the group's query rows, their pieces swizzled as TMA would; every product over the rows before has completed, since
+        // its scores have been read
+        asm volatile("bar.sync 1, %0;" ::"n"(kScoreThreads) : "memory");
         {
-          const int r = a.first_row + tid;
-          const uint4* src = a.q + ((int64_t)(b * a.window + r / a.gs) * a.hk * a.gs + h * a.gs + r % a.gs) * 16;
+          // a half-warp per row, eight rows of a thread on their way together
+          const int piece = tid & 15;
+          uint4 x[8];
 #pragma unroll
-          for (int piece = 0; piece < 16; ++piece) {
-            const uint4 x = tid < a.rows ? ri_ldg16(src + piece) : make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4*>(q_rows + (piece >> 3) * kRowHalf + tid * 128 + (((piece & 7) ^ (tid & 7)) << 4)) = x;
+          for (int u = 0; u < 8; ++u) {
+            const int i = u * 32 + (tid >> 4), r = a.first_row + i, w = r / a.gs;
+            x[u] = i < a.rows ? ri_ldg16(a.q + ((int64_t)(b * a.window + w) * a.hk * a.gs + h * a.gs + r - w * a.gs) * 16 + piece)
+                              : make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const int i = u * 32 + (tid >> 4);
+            *reinterpret_cast<uint4*>(q_rows + (piece >> 3) * kRowHalf + i * 128 + (((piece & 7) ^ (i & 7)) << 4)) = x[u];
           }
           if (!STATS) {
-            s_neg_lse[tid] = -a.lse2[(int64_t)at.g * kRows + tid];
-            s_last[tid] = last_seen(a, n, r);
+            if (tid == 0) s_nan = 0;
+            asm volatile("bar.sync 1, %0;" ::"n"(kScoreThreads) : "memory");
+            if (tid < kRows) {
+              const float lse2 = a.lse2[(int64_t)at.g * kRows + tid];
+              s_neg_lse[tid] = -lse2;
+              if (lse2 != lse2) s_nan = 1;
+              s_last[tid] = last_seen(a, n, a.first_row + tid);
+            }
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(kScoreThreads) : "memory");
         if (lane == 0) mbar_arrive(bar_q);
         if (STATS) {
           const int r = both ? g * kTile + row : row;
@@ -256,9 +294,9 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
             ok = ok && __all_sync(0xffffffffu, mbar_wait(bar_s_full(g, i), (done / kBuffers) & 1, abort_flag, 86));
             if (!ok) continue;
             tc_fence_after();
-            const uint32_t scores = tmem + (2 * g + i) * 128 + t_lane;
-            const int slot0 = (t - at.first) * kTile;
-            const bool edge = slot0 + kTile - 1 > last;      // some scores are masked for this row
+            const uint32_t scores = tmem + (2 * g + i) * 128 + half * 64 + t_lane;
+            const int slot0 = (t - at.first) * kTile + half * 64;
+            const bool edge = slot0 + 63 > last;      // some scores are masked for this row
             float sum = 0.f;
             // With a reference from earlier tiles the exponentials need no maximum: it is near this tile's, and where it is
             // so far below that the sum grows out of hand the tile is done again from its own maximum.
@@ -270,7 +308,7 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
             if (__any_sync(0xffffffffu, again)) {
               float mx = -INFINITY;
 #pragma unroll 1
-              for (int k = 0; k < 4; ++k) {
+              for (int k = 0; k < 2; ++k) {
                 uint32_t sr[32];
                 load_scores(scores + k * 32, sr);
 #pragma unroll
@@ -282,7 +320,7 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
               m = m_new;
               sum = 0.f;
 #pragma unroll 1
-              for (int k = 0; k < 4; ++k) {
+              for (int k = 0; k < 2; ++k) {
                 uint32_t sr[32];
                 load_scores(scores + k * 32, sr);
 #pragma unroll
@@ -296,41 +334,49 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
             if (lane == 0) mbar_arrive(bar_s_empty(g, i));
             ++done;
           }
-          a.part[(int64_t)(c + at.g) * kRows + tid] = make_float2(m, l);
+          a.part[(int64_t)(c + at.g) * kPartials + half * kRows + side * kTile + row] = make_float2(m, l);
         } else {
           for (; t < end; ++t, ++used) {
             if (g != (used & 1)) continue;
             const int slot0 = (t - at.first) * kTile, slot = slot0 + row;
             float* weight = nullptr;
             float old = 0.f;
-            const int id = slot < n ? page_to_write(a, b, slot >> a.shift) : -1;
+            const int id = !half && slot < n ? page_to_write(a, b, slot >> a.shift) : -1;
             if (id >= 0) {
               weight = a.weight + record_at(a, id, h, slot & ((1 << a.shift) - 1));
               old = *weight;
             }
             ok = ok && __all_sync(0xffffffffu, mbar_wait(bar_s_full(g, 0), done & 1, abort_flag, 87));
-            if (!ok) continue;
             tc_fence_after();
-            const bool edge = slot0 + kTile - 1 > n - a.window;      // some query rows do not see some of the tile's slots
-            const uint32_t scores = tmem + g * 256 + t_lane;
+            // some query rows do not see some of the tile's slots
+            const bool edge = slot0 + kTile - 1 > n - a.window || s_nan;
+            const int chunks = (a.rows + 31) / 32, chunk0 = half ? (chunks + 1) / 2 : 0, my_chunks = half ? chunks / 2 : (chunks + 1) / 2;
+            const uint32_t scores = tmem + g * 256 + chunk0 * 32 + t_lane;
             float sum = 0.f;
-            if (!edge) {
-              sum = column_sum(scores, (a.rows + 31) / 32, a.scale2, s_neg_lse);
+            if (!ok) {                 // no scores to read, but the warp that shares the slots is still met below
+            } else if (!edge) {
+              sum = column_sum(scores, my_chunks, a.scale2, s_neg_lse + chunk0 * 32);
             } else {
 #pragma unroll 1
-              for (int k = 0; k * 32 < a.rows; ++k) {
+              for (int k = 0; k < my_chunks; ++k) {
                 uint32_t sr[32];
                 load_scores(scores + k * 32, sr);
+                const int r0 = (chunk0 + k) * 32;
 #pragma unroll
                 for (int x = 0; x < 32; ++x)
-                  if (slot <= s_last[k * 32 + x]) sum += ex2(__uint_as_float(sr[x]) * a.scale2 + s_neg_lse[k * 32 + x]);
+                  if (slot <= s_last[r0 + x]) sum += ex2(__uint_as_float(sr[x]) * a.scale2 + s_neg_lse[r0 + x]);
               }
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_s_empty(g, 0));
             ++done;
-            if (weight != nullptr) *weight = old + sum;
+            // the two warps that share a slot's query rows meet; the sums of two tiles lie in turn in two places, so that one
+            // is read before the meeting after which it is written again
+            const int place = done & 1, meeting = 2 + side * 4 + quarter;
+            if (half) s_sum[side][place][row] = sum;
+            asm volatile("bar.sync %0, 64;" ::"r"(meeting) : "memory");
+            if (!half && weight != nullptr) *weight = old + (sum + s_sum[side][place][row]);
           }
         }
       }
@@ -370,8 +416,13 @@ __global__ void __launch_bounds__(256) observe_merge_kernel(const __grid_constan
     while (c0 > 0 && ri_seq::cta_start(c0, total, n_ctas) > lo) --c0;
     while (ri_seq::cta_start(c0 + 1, total, n_ctas) <= lo) ++c0;
     for (int c = c0 + warp; c < n_ctas && ri_seq::cta_start(c, total, n_ctas) < hi; c += 8) {
-      add(a.part[(int64_t)(c + g) * kRows + row]);
-      if (!both) add(a.part[(int64_t)(c + g) * kRows + kTile + row]);      // the other half's tiles
+      const float2* part = a.part + (int64_t)(c + g) * kPartials + row;
+      add(part[0]);
+      add(part[kRows]);
+      if (!both) {                                       // the other side's tiles
+        add(part[kTile]);
+        add(part[kRows + kTile]);
+      }
     }
   }
   s_part[warp][lane] = make_float2(m, l);
@@ -423,7 +474,7 @@ int64_t obs_slots(const ri_paged& p) { return kObsMaxCtas + (int64_t)p.batch * p
 extern "C" int64_t ri_paged_observe_scratch_bytes(const ri_paged* p) {
   const int rc = check(p, "ri_paged_observe");
   if (rc != RI_OK) return rc;
-  return obs_slots(*p) * kRows * 8 + (int64_t)p->batch * p->kv_heads * kRows * 4;
+  return obs_slots(*p) * kPartials * 8 + (int64_t)p->batch * p->kv_heads * kRows * 4;
 }
 
 extern "C" int ri_paged_observe(const ri_paged* p, const void* d_q, int32_t window, float scale, void* d_scratch, void* stream) {
@@ -438,7 +489,7 @@ extern "C" int ri_paged_observe(const ri_paged* p, const void* d_q, int32_t wind
   static_cast<Pages&>(a) = view(*p);
   a.q = static_cast<const uint4*>(d_q);
   a.part = static_cast<float2*>(d_scratch);
-  a.lse2 = reinterpret_cast<float*>(a.part + obs_slots(*p) * kRows);
+  a.lse2 = reinterpret_cast<float*>(a.part + obs_slots(*p) * kPartials);
   a.window = window;
   a.gs = p->group_size;
   a.scale2 = RI_LOG2E * scale;
