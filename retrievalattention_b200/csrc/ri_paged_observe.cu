@@ -62,43 +62,15 @@ __device__ __forceinline__ void load_scores(uint32_t taddr, uint32_t (&r)[32]) {
   tc_wait_ld();
   tc_ld_landed(r);
 }
-// 2^x for a pair on the FMA pipe: 2^n * p(x - n), n the nearest whole number, p the polynomial of degree 5 that is nearest to
-// 2^f on [-1/2, 1/2] in relative error (found by Remez's exchange; with 32-bit Horner steps 2.2e-7, as ex2.approx).  From 2^-126
-// to 2^126; NaN gives 2^126.
-__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
-  constexpr float kWhole = 12582912.f;                 // 1.5 * 2^23: a sum with it has the whole number in its low bits
-  float x0, x1, t0, t1, p0, p1;
-  unpack_f2(x, x0, x1);
-  x = pack_f2(fmaxf(fminf(x0, 126.f), -126.f), fmaxf(fminf(x1, 126.f), -126.f));
-  const uint64_t t = add_f2(x, pack_f2(kWhole, kWhole));
-  const uint64_t f = fma_f2(add_f2(t, pack_f2(-kWhole, -kWhole)), pack_f2(-1.f, -1.f), x);
-  auto both = [](float c) { return pack_f2(c, c); };
-  uint64_t p = fma_f2(both(0.001327647199f), f, both(0.009675541334f));
-  p = fma_f2(p, f, both(0.05550713273f));
-  p = fma_f2(p, f, both(0.2402211972f));
-  p = fma_f2(p, f, both(0.6931469671f));
-  p = fma_f2(p, f, both(1.000000072f));
-  unpack_f2(t, t0, t1);
-  unpack_f2(p, p0, p1);
-  return pack_f2(__int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23)), __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23)));
-}
-#ifndef V_POLY
-#define V_POLY 0
-#endif
-constexpr int kPolynomials = V_POLY;        // of 16 pairs
 // Sum of 2^(s * scale + shift) over 32 scores, added to `sum`; `shift` holds one value a pair of scores.
 template <class Shift>
 __device__ __forceinline__ void add_exps(const uint32_t (&sr)[32], uint64_t scale, Shift shift, uint64_t (&sum)[2]) {
 #pragma unroll
   for (int x = 0; x < 16; ++x) {
     const uint64_t e = fma_f2(pack_f2(__uint_as_float(sr[2 * x]), __uint_as_float(sr[2 * x + 1])), scale, shift(x));
-    if ((x + 1) * kPolynomials / 16 != x * kPolynomials / 16) {
-      sum[x & 1] = add_f2(sum[x & 1], exp2_pair(e));
-    } else {
-      float e0, e1;
-      unpack_f2(e, e0, e1);
-      sum[x & 1] = add_f2(sum[x & 1], pack_f2(ex2(e0), ex2(e1)));
-    }
+    float e0, e1;
+    unpack_f2(e, e0, e1);
+    sum[x & 1] = add_f2(sum[x & 1], pack_f2(ex2(e0), ex2(e1)));
   }
 }
 __device__ __forceinline__ float total_of(const uint64_t (&sum)[2]) {
@@ -174,7 +146,11 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
   tc_fence_after();
   const uint32_t tmem = s_tmem_base;
   volatile int* abort_flag = &s_abort;
-  ri_pdl_enter();
+  // Pass 1 lets the next kernel start when the kernel in front of it has ended, not before.  So pass 2, which starts behind
+  // pass 1 and beside the merge between them, finds queries, keys and lengths as they are, and waits for the merge only where it
+  // reads what that wrote.
+  if (STATS) ri_pdl_wait();
+  ri_pdl_trigger();
 
   // this CTA's tiles [lo, hi) of the sequence, segment by segment (the part of a group that falls to it)
   const int total = ri_seq::count_steps(a), n_ctas = min(a.max_ctas, total), c = (int)blockIdx.x;
@@ -272,6 +248,7 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
           }
           if (!STATS) {
             if (tid == 0) s_nan = 0;
+            ri_pdl_wait();
             asm volatile("bar.sync 1, %0;" ::"n"(kScoreThreads) : "memory");
             if (tid < kRows) {
               const float lse2 = a.lse2[(int64_t)at.g * kRows + tid];
@@ -298,10 +275,18 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
             const int slot0 = (t - at.first) * kTile + half * 64;
             const bool edge = slot0 + 63 > last;      // some scores are masked for this row
             float sum = 0.f;
-            // With a reference from earlier tiles the exponentials need no maximum: it is near this tile's, and where it is
-            // so far below that the sum grows out of hand the tile is done again from its own maximum.
-            bool again = edge || m == -INFINITY;
-            if (!__any_sync(0xffffffffu, again)) {
+            // The exponentials need no maximum, just a reference near it: the largest of the first 32 scores, for all tiles.  A
+            // tile where the sum grows out of hand against it, or where scores are masked, is done from its own maximum.
+            bool again = edge;
+            if (!__any_sync(0xffffffffu, edge)) {
+              if (__any_sync(0xffffffffu, m == -INFINITY)) {
+                uint32_t sr[32];
+                load_scores(scores, sr);
+                float mx = __uint_as_float(sr[0]);
+#pragma unroll
+                for (int x = 1; x < 31; x += 2) mx = max3(mx, __uint_as_float(sr[x]), __uint_as_float(sr[x + 1]));
+                if (m == -INFINITY) m = fmaxf(mx, __uint_as_float(sr[31])) * a.scale2;
+              }
               sum = row_sum(scores, a.scale2, -m);
               again = !(sum < kFarAbove);
             }
@@ -382,6 +367,7 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
       }
     }
   }
+  ri_pdl_wait();                                   // CTAs without tiles too: the kernel behind waits for this one alone
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && s_abort) *a.status = s_abort;
