@@ -4,7 +4,8 @@
 
 One translation unit per ``csrc/*.cu`` / ``csrc/*.cpp`` file, compiled in parallel, then
 linked into ``retrievalattention_b200/lib/libri_b200.so``.  nvcc cross-compiles, so no GPU is
-needed to build.
+needed to build.  Beside it ``binding/paged.cpp``, the host side of ``paged.py`` (C++ on torch's
+headers), becomes ``lib/_paged_binding.so``.
 """
 from __future__ import annotations
 
@@ -20,6 +21,8 @@ INCLUDE = os.path.join(os.path.dirname(PKG), "include")
 LIB_DIR = os.path.join(PKG, "lib")
 OBJ_DIR = os.path.join(LIB_DIR, "obj")
 LIB_PATH = os.path.join(LIB_DIR, "libri_b200.so")
+BINDING_SOURCE = os.path.join(PKG, "binding", "paged.cpp")
+BINDING_PATH = os.path.join(LIB_DIR, "_paged_binding.so")
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", f"-I{INCLUDE}", f"-I{CSRC}"]
@@ -63,5 +66,29 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     return LIB_PATH
 
 
+def build_binding(force: bool = False) -> str:
+    """Compile the host side of ``paged.py`` if it is missing or older than what it is made from.  Returns its path."""
+    newest = max(os.path.getmtime(f) for f in (BINDING_SOURCE, os.path.join(INCLUDE, "ri_b200.h")))
+    if not force and os.path.exists(BINDING_PATH) and os.path.getmtime(BINDING_PATH) >= newest:
+        return BINDING_PATH
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    include = [INCLUDE, os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    os.makedirs(LIB_DIR, exist_ok=True)
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-I{d}" for d in include), BINDING_SOURCE, "-o", BINDING_PATH, "-L" + os.path.join(root, "lib"),
+           "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on {BINDING_SOURCE}:\n{res.stdout}\n{res.stderr}")
+    return BINDING_PATH
+
+
 if __name__ == "__main__":
     print(build_library(force="--force" in sys.argv, verbose="-v" in sys.argv))
+    print(build_binding(force="--force" in sys.argv))

@@ -17,14 +17,21 @@ _word = None
 _devices: set = set()
 
 
-def word(device) -> C.c_int32:
-    """The word, for calls that run on ``device``."""
+def address() -> int:
+    """Where the word lies; ``word`` names the device of a call that uses it."""
     global _word
     if _word is None:
-        address = _lib.lib.ri_status_word()          # the same for every thread that gets here
-        if not address:
+        where = _lib.lib.ri_status_word()            # the same for every thread that gets here
+        if not where:
             raise RuntimeError(f"ri_status_word: {_lib.lib.ri_last_error().decode()}")
-        _word = C.c_int32.from_address(address)
+        _word = C.c_int32.from_address(where)
+    return C.addressof(_word)
+
+
+def word(device) -> C.c_int32:
+    """The word, for calls that run on ``device``."""
+    if _word is None:
+        address()
     _devices.add(device)
     return _word
 
