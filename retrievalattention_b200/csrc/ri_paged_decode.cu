@@ -7,12 +7,12 @@
 // read, a sixteenth of what the tensor cores need to be the limit, so m16n8k16 with the heads in M is enough.
 // The split is that of the dense cache (ri_step_sequence.cuh): 16-row steps of all groups behind one another, an equal
 // contiguous range per SM and again per warp, whatever the requests' lengths; a warp streams its steps through its own ring,
-// filled by TMA, a box of 16 rows (8 where a page has no more) of both halves of the channels; the number of the next step's
-// page is fetched a step ahead.  Layout in shared memory and the order of the keys in a step: as in ri_dense_decode.cu.
+// filled by TMA, a box of 16 rows (8 where a page has no more) of both halves of the channels; the number of the next
+// step's page is fetched a step ahead.  Layout in shared memory and the order of the keys in a step: as in ri_dense_decode.cu.
 // The probabilities enter the second product as two 16-bit parts, so out is within its own rounding of 32-bit arithmetic.
 // A second kernel merges a group's partial results by log-sum-exp in a fixed order.  For the weights the first kernel
-// leaves the scores behind (4 bytes a slot and query head, against 512 a slot for K and V), and a third turns them into
-// probabilities once lse is known; every slot has one thread, so the sums have one order and no atomics.
+// leaves the scores behind (4 bytes a slot and query head, against 512 a slot for K and V), and the second turns them into
+// probabilities; every slot has one thread, so the sums have one order and no atomics.
 #include "ri_paged.cuh"
 #include "ri_step_sequence.cuh"
 #include "ri_tc.cuh"
@@ -38,8 +38,7 @@ constexpr int kPagedThreads = kPagedWarps * 32;
 constexpr int kPagedMaxCtas = 160;                    // the grid is one CTA per SM, at most this many
 constexpr int kPagedRing = kPagedWarps * kStages * kStageBytes;   // 192 KB, on a 1024-byte boundary
 constexpr int kPagedSmem = 1024 + kPagedRing;
-constexpr int kJoinThreads = 256;
-constexpr int kFoldThreads = 256;
+constexpr int kFinishThreads = 256;
 
 struct PagedArgs : Pages {
   static constexpr int kStep = 16;
@@ -47,7 +46,6 @@ struct PagedArgs : Pages {
   float* part_o;             // [slots][gs][128]
   float2* part_ml;           // [slots][gs]: (maximum in the log2 domain, sum)
   float* scores;             // [step][gs][16] in the log2 domain, or null; inside a step the order of the lanes that made them
-  float* lse2;               // [groups][gs]: log-sum-exp in the log2 domain, for the weights
   float* lse;                // [groups][gs] or null
   uint16_t* out;
   int64_t q_stride;          // 16-byte pieces from request to request
@@ -77,7 +75,10 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
   }
   __syncthreads();
   volatile int* abort_flag = &s_abort;
-  ri_pdl_enter();
+  // The next kernel may start when the kernel in front of this one has ended, not before: it finds lengths and page tables as
+  // they are without waiting for this one.
+  ri_pdl_wait();
+  ri_pdl_trigger();
   const int total = count_steps(a), n_ctas = used_ctas(total, a.max_ctas), c = (int)blockIdx.x;
   if (c >= n_ctas || total == 0) return;
   const int c_lo = cta_start(c, total, n_ctas), c_hi = cta_start(c + 1, total, n_ctas), c_n = c_hi - c_lo;
@@ -271,40 +272,47 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
   }
 }
 
-// One head of one group per block: the slots of its partial results in sequence order, then two halves of the block each
-// sum every second one.
+// What is left once every partial result is there, a group per blockIdx.y: its blocks join the partial results, a query head at
+// a time, and with weights turn the group's scores into probabilities, kFoldSlots slots at a time, a thread per slot.  Every
+// block works out lse of all heads (warp h of head h), so none waits for another.  Which partial results the group has
+// follows from the lengths, so a warp lists them, in the order of the sequence, before the wait for the kernel that makes them.
+constexpr int kFoldEach = 4, kFoldSlots = kFoldEach * kFinishThreads;
+constexpr int kFinishBlocks = 2;                         // of an SM
+constexpr int kTogether = 8;                             // partial results of a warp on their way
 template <int DT>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a) {
-  ri_pdl_enter();
-  __shared__ int s_slot[kPagedMaxCtas * kPagedWarps];
-  __shared__ float s_w[kPagedMaxCtas * kPagedWarps];
-  __shared__ float s_l, s_o[RI_HEAD_DIM];
+__global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_kernel(const __grid_constant__ PagedArgs a) {
+  extern __shared__ int s_slot[];                        // [most partial results of a group]
+  __shared__ float s_m[kMaxHeads], s_l[kMaxHeads], s_o[kFinishThreads / 32][RI_HEAD_DIM];
   __shared__ int s_n;
-  const int tid = threadIdx.x, lane = tid & 31, h = blockIdx.x, g = blockIdx.y, gs = a.gs;
-  uint16_t* out = a.out + ((int64_t)g * gs + h) * RI_HEAD_DIM;
-  const int b = g / a.hk, n = steps_of(rows_of(a, b));
-  if (n == 0) {
-    if (tid < RI_HEAD_DIM) out[tid] = 0;
-    if (tid == 0 && a.lse != nullptr) a.lse[g * gs + h] = -INFINITY;
-    return;
+  ri_pdl_trigger();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.y, gs = a.gs, b = g / a.hk, h_kv = g - b * a.hk;
+  int before = 0, all = 0, rows = 0;                     // steps in front of the request (of one KV head), of all; its rows
+  for (int i = lane; i < a.batch; i += 32) {
+    const int r = rows_of(a, i), steps = steps_of(r);
+    all += steps;
+    if (i < b) before += steps;
+    if (i == b) rows = r;
   }
-  if (tid < 32) {
-    int before = 0;
-    for (int i = lane; i < b; i += 32) before += steps_of(rows_of(a, i));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-    const int lo = before * a.hk + (g - b * a.hk) * n, hi = lo + n;
-    const int total = count_steps(a), n_ctas = used_ctas(total, a.max_ctas);
-    int c0 = (int)((int64_t)lo * n_ctas / total);           // the CTA that holds step lo
-    while (c0 > 0 && cta_start(c0, total, n_ctas) > lo) --c0;
-    while (cta_start(c0 + 1, total, n_ctas) <= lo) ++c0;
-    int count = 0;
-    for (int c_base = c0; c_base < n_ctas && cta_start(c_base, total, n_ctas) < hi; c_base += 4) {      // 4 CTAs a warp step
+  for (int o = 16; o > 0; o >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    rows += __shfl_xor_sync(0xffffffffu, rows, o);
+  }
+  all *= a.hk;
+  const int n = steps_of(rows), lo = before * a.hk + h_kv * n, hi = lo + n;
+  int count = 0;
+  if (warp == 0 && n > 0) {
+    const int n_ctas = used_ctas(all, a.max_ctas);
+    int c0 = (int)((int64_t)lo * n_ctas / all);          // the CTA that holds step lo
+    while (c0 > 0 && cta_start(c0, all, n_ctas) > lo) --c0;
+    while (cta_start(c0 + 1, all, n_ctas) <= lo) ++c0;
+    for (int c_base = c0; c_base < n_ctas && cta_start(c_base, all, n_ctas) < hi; c_base += 4) {      // 4 CTAs a warp step
       const int c = c_base + (lane >> 3), w = lane & 7;
       bool mine = false;
       if (c < n_ctas) {
-        const int c_lo = cta_start(c, total, n_ctas), c_n = cta_start(c + 1, total, n_ctas) - c_lo;
-        if (c_lo >= lo && c_lo + c_n <= hi) {
+        const int c_lo = cta_start(c, all, n_ctas), c_n = cta_start(c + 1, all, n_ctas) - c_lo;
+        if (c_lo >= lo && c_lo + c_n <= hi) {            // merged by the CTA
           mine = w == 0;
         } else {
           const int w_lo = c_lo + c_n * w / kPagedWarps, w_hi = c_lo + c_n * (w + 1) / kPagedWarps;
@@ -315,64 +323,142 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
       if (mine) s_slot[count + __popc(votes & ((1u << lane) - 1))] = c * kPagedWarps + w + g;
       count += __popc(votes);
     }
-    __syncwarp();
+  }
+  // a tile of slots: pages (their tables do not change either), then scores and weights
+  int id[kFoldEach];
+  float sc[kFoldEach][kMaxHeads], old[kFoldEach];
+  auto slot_of = [&](int tile, int e) {      // place i of a step holds its key (i / 2 % 2) * 8 + i / 4 + (i % 2) * 4
+    const int place = tile * kFoldSlots + e * kFinishThreads + tid, i = place & 15;
+    return (place & ~15) + ((i >> 1) & 1) * 8 + (i >> 2) + (i & 1) * 4;
+  };
+  auto weight_at = [&](int tile, int e) { return a.weight + record_at(a, id[e], h_kv, slot_of(tile, e) & ((1 << a.shift) - 1)); };
+  auto find_pages = [&](int tile) {
+#pragma unroll
+    for (int e = 0; e < kFoldEach; ++e) {
+      const int slot = slot_of(tile, e);
+      id[e] = slot < rows ? page_to_write(a, b, slot >> a.shift) : -1;
+    }
+  };
+  auto fetch = [&](int tile) {
+#pragma unroll
+    for (int e = 0; e < kFoldEach; ++e) {
+      const int place = tile * kFoldSlots + e * kFinishThreads + tid;
+      const float* of = a.scores + ((int64_t)(lo + (place >> 4)) * gs) * 16 + (place & 15);
+#pragma unroll
+      for (int h = 0; h < kMaxHeads; ++h)
+        if (h < gs && id[e] >= 0) sc[e][h] = of[h * 16];
+      if (id[e] >= 0) old[e] = *weight_at(tile, e);
+    }
+  };
+  const bool folds = a.weight != nullptr && (int)blockIdx.x * kFoldSlots < rows;
+  if (folds) find_pages(blockIdx.x);
+  if (tid == 0) s_n = count;
+  ri_pdl_wait();
+  if (n == 0) {
+    for (int h = blockIdx.x; h < gs; h += gridDim.x) {
+      if (tid < RI_HEAD_DIM) a.out[((int64_t)g * gs + h) * RI_HEAD_DIM + tid] = 0;
+      if (tid == 0 && a.lse != nullptr) a.lse[g * gs + h] = -INFINITY;
+    }
+    return;
+  }
+  if (folds) fetch(blockIdx.x);
+  __syncthreads();
+  count = s_n;
+  if (warp < gs) {
     float M = -INFINITY, L = 0.f;
-    for (int i = lane; i < count; i += 32) M = fmaxf(M, a.part_ml[(int64_t)s_slot[i] * gs + h].x);
+    for (int i0 = 0; i0 < count; i0 += 32 * kTogether) {
+      float2 ml[kTogether];
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) {
+        const int i = i0 + u * 32 + lane;
+        ml[u] = i < count ? a.part_ml[(int64_t)s_slot[i] * gs + warp] : make_float2(-INFINITY, 0.f);
+      }
+      float most = M;
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) most = fmaxf(most, ml[u].x);
+      const float ref = most == -INFINITY ? 0.f : most;
+      L *= exp2f(M - ref);
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) L += ml[u].y * exp2f(ml[u].x - ref);
+      M = most;
+    }
+    const float own = M;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     const float Ms = M == -INFINITY ? 0.f : M;
-    for (int i = lane; i < count; i += 32) {
-      const float2 ml = a.part_ml[(int64_t)s_slot[i] * gs + h];
-      const float f = exp2f(ml.x - Ms);
-      s_w[i] = f;
-      L += ml.y * f;
-    }
+    L *= exp2f(own - Ms);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
     if (lane == 0) {
-      s_l = L;
-      s_n = count;
-      const float lse2 = M + log2f(L);
-      if (a.lse2 != nullptr) a.lse2[g * gs + h] = lse2;
-      if (a.lse != nullptr) a.lse[g * gs + h] = lse2 * 0.69314718055994531f;
+      s_m[warp] = Ms;
+      s_l[warp] = L;
+      if (blockIdx.x == 0 && a.lse != nullptr) a.lse[g * gs + warp] = (M + log2f(L)) * 0.69314718055994531f;
     }
   }
-  __syncthreads();
-  const int ch = tid & (RI_HEAD_DIM - 1), half = tid >> 7, count = s_n;
-  float O = 0.f;
-#pragma unroll 8
-  for (int i = half; i < count; i += 2) O += a.part_o[((int64_t)s_slot[i] * gs + h) * RI_HEAD_DIM + ch] * s_w[i];
-  if (half) s_o[ch] = O;
-  __syncthreads();
-  if (!half) out[ch] = Elem<DT>::bits(s_l > 0.f ? (O + s_o[ch]) / s_l : 0.f);
-}
-
-// weight_j += sum_h 2^(s_hj - lse_h): a thread per slot, 256 slots of one group per block.
-__global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const __grid_constant__ PagedArgs a) {
-  ri_pdl_enter();
-  __shared__ int s_first;
-  const int tid = threadIdx.x, lane = tid & 31, g = blockIdx.y, gs = a.gs, b = g / a.hk;
-  const int rows = rows_of(a, b), base = blockIdx.x * kFoldThreads;
-  if (base >= rows) return;
-  if (tid < 32) {
-    int before = 0;
-    for (int i = lane; i < b; i += 32) before += steps_of(rows_of(a, i));
+  for (int head = blockIdx.x; head < gs; head += gridDim.x) {
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);          // a warp per partial result, four channels a lane
+    float M = -INFINITY;                                 // this warp's reference; it need not wait for the head's
+    for (int i0 = warp; i0 < count; i0 += kTogether * (kFinishThreads / 32)) {
+      float4 x[kTogether];
+      float m[kTogether];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-    if (lane == 0) s_first = before * a.hk + (g - b * a.hk) * steps_of(rows);
+      for (int u = 0; u < kTogether; ++u) {
+        const int i = i0 + u * (kFinishThreads / 32);
+        m[u] = -INFINITY;
+        if (i < count) {
+          const int64_t at = (int64_t)s_slot[i] * gs + head;
+          m[u] = a.part_ml[at].x;
+          x[u] = reinterpret_cast<const float4*>(a.part_o + at * RI_HEAD_DIM)[lane];
+        }
+      }
+      float most = M;
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) most = fmaxf(most, m[u]);
+      if (most == -INFINITY) continue;
+      const float f0 = exp2f(M - most);
+      o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u)
+        if (i0 + u * (kFinishThreads / 32) < count) {
+          const float f = exp2f(m[u] - most);
+          o.x += x[u].x * f; o.y += x[u].y * f; o.z += x[u].z * f; o.w += x[u].w * f;
+        }
+      M = most;
+    }
+    __syncthreads();                                     // the head's maximum and sum are there, the last head's rows are read
+    const float f = exp2f(M - s_m[head]);
+    reinterpret_cast<float4*>(s_o[warp])[lane] = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+    __syncthreads();
+    if (tid < RI_HEAD_DIM) {
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kFinishThreads / 32; ++w) sum += s_o[w][tid];
+      a.out[((int64_t)g * gs + head) * RI_HEAD_DIM + tid] = Elem<DT>::bits(s_l[head] > 0.f ? sum / s_l[head] : 0.f);
+    }
   }
+  if (!folds) return;
   __syncthreads();
-  // place i of a step holds its key (i / 2 % 2) * 8 + i / 4 + (i % 2) * 4
-  const int step = (base + tid) >> 4, i = tid & 15, slot = step * 16 + ((i >> 1) & 1) * 8 + (i >> 2) + (i & 1) * 4;
-  if (slot >= rows) return;
-  const float* sc = a.scores + (int64_t)(s_first + step) * gs * 16 + i;
-  float sum = 0.f;
-  for (int h = 0; h < gs; ++h) sum += exp2f(sc[h * 16] - a.lse2[g * gs + h]);
-  const int id = page_to_write(a, b, slot >> a.shift);
-  if (id >= 0) a.weight[record_at(a, id, g - b * a.hk, slot & ((1 << a.shift) - 1))] += sum;
+  float lse2[kMaxHeads];
+#pragma unroll
+  for (int h = 0; h < kMaxHeads; ++h) lse2[h] = h < gs && s_l[h] > 0.f ? s_m[h] + log2f(s_l[h]) : INFINITY;      // nothing to give: 0
+  for (int tile = blockIdx.x; tile * kFoldSlots < rows; tile += gridDim.x) {
+    if (tile != (int)blockIdx.x) {
+      find_pages(tile);
+      fetch(tile);
+    }
+#pragma unroll
+    for (int e = 0; e < kFoldEach; ++e) {
+      if (id[e] < 0) continue;
+      float sum = 0.f;
+#pragma unroll
+      for (int h = 0; h < kMaxHeads; ++h)
+        if (h < gs) sum += exp2f(sc[e][h] - lse2[h]);
+      *weight_at(tile, e) = old[e] + sum;
+    }
+  }
 }
 
-int64_t paged_slots(int64_t groups) { return (int64_t)kPagedMaxCtas * kPagedWarps + groups; }
+int64_t paged_slots(const ri_paged& p) { return (int64_t)kPagedMaxCtas * kPagedWarps + (int64_t)p.batch * p.kv_heads; }
 int64_t paged_most_steps(const ri_paged& p) {
   return (int64_t)p.batch * p.kv_heads * (((int64_t)p.table_stride * p.page_size + 15) / 16);
 }
@@ -393,24 +479,31 @@ int make_page_map(CUtensorMap* map, const void* base, const ri_paged& p, int64_t
 }
 
 template <int DT, int BOX, bool WEIGHTS>
-int launch_paged(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t s) {
+int launch_steps(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t s) {
   int rc;
   if ((rc = ri_allow_smem<paged_decode_kernel<DT, BOX, WEIGHTS>>(kPagedSmem)) != RI_OK) return rc;
-  RI_CUDA_OK(ri_launch_pdl_id(11, paged_decode_kernel<DT, BOX, WEIGHTS>, dim3(a.max_ctas), dim3(kPagedThreads), (size_t)kPagedSmem,
-                              s, map_k, map_v, a));
-  RI_CUDA_OK(ri_launch_pdl_id(11, paged_join_kernel<DT>, dim3(a.gs, a.batch * a.hk), dim3(kJoinThreads), 0, s, a));
-  if (WEIGHTS) {
-    const int64_t most = (int64_t)a.table_stride << a.shift;
-    RI_CUDA_OK(ri_launch_pdl_id(11, paged_fold_kernel, dim3((unsigned)((most + kFoldThreads - 1) / kFoldThreads), a.batch * a.hk),
-                                dim3(kFoldThreads), 0, s, a));
-  }
+  RI_CUDA_OK(ri_launch_pdl_id(11, paged_decode_kernel<DT, BOX, WEIGHTS>, dim3(a.max_ctas), dim3(kPagedThreads), (size_t)kPagedSmem, s,
+                              map_k, map_v, a));
   return RI_OK;
+}
+template <int DT, int BOX>
+int launch_steps(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t s) {
+  return a.weight ? launch_steps<DT, BOX, true>(a, map_k, map_v, s) : launch_steps<DT, BOX, false>(a, map_k, map_v, s);
 }
 template <int DT>
 int launch_paged(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, int box, cudaStream_t s) {
-  if (box == 8)
-    return a.weight ? launch_paged<DT, 8, true>(a, map_k, map_v, s) : launch_paged<DT, 8, false>(a, map_k, map_v, s);
-  return a.weight ? launch_paged<DT, 16, true>(a, map_k, map_v, s) : launch_paged<DT, 16, false>(a, map_k, map_v, s);
+  int rc = box == 8 ? launch_steps<DT, 8>(a, map_k, map_v, s) : launch_steps<DT, 16>(a, map_k, map_v, s);
+  if (rc != RI_OK) return rc;
+  const int64_t groups = (int64_t)a.batch * a.hk, most = (int64_t)a.table_stride << a.shift;
+  // blocks of a group: for its heads, or with weights its tiles of slots, as many as the chip holds at once
+  const int64_t tiles = a.weight ? (most + kFoldSlots - 1) / kFoldSlots : 0, room = kFinishBlocks * (int64_t)a.max_ctas / groups;
+  int64_t blocks = tiles > a.gs ? tiles : a.gs;
+  if (blocks > room) blocks = room > 1 ? room : 1;
+  // partial results of a group: its steps, or all that there are and one more
+  const int64_t steps = (most + 15) / 16, parts = (int64_t)a.max_ctas * kPagedWarps;
+  const size_t smem = (size_t)(steps < parts ? steps : parts) * 4 + 4;
+  RI_CUDA_OK(ri_launch_pdl_id(11, paged_finish_kernel<DT>, dim3((unsigned)blocks, (unsigned)groups), dim3(kFinishThreads), smem, s, a));
+  return RI_OK;
 }
 
 }  // namespace
@@ -420,9 +513,8 @@ extern "C" int64_t ri_paged_decode_scratch_bytes(const ri_paged* p) {
   const int rc = ri_page::check(p, "ri_paged_decode");
   if (rc != RI_OK) return rc;
   if (p->group_size < 1 || p->group_size > ri_wave::kMaxHeads) return ri_fail(RI_ERR_INVALID, "ri_paged_decode: group_size=%d unsupported", p->group_size);
-  const int64_t groups = (int64_t)p->batch * p->kv_heads;
-  int64_t floats = ri_wave::paged_slots(groups) * p->group_size * (RI_HEAD_DIM + 2);
-  if (p->d_weight) floats += groups * p->group_size + 4 + ri_wave::paged_most_steps(*p) * p->group_size * 16;
+  int64_t floats = ri_wave::paged_slots(*p) * p->group_size * (RI_HEAD_DIM + 2);
+  if (p->d_weight) floats += 4 + ri_wave::paged_most_steps(*p) * p->group_size * 16;
   return floats * 4;
 }
 
@@ -438,21 +530,16 @@ extern "C" int ri_paged_decode(const ri_paged* p, const void* d_q, int64_t q_str
              "ri_paged_decode: queries overlap or lie at odd places");
   RI_REQUIRE(((uintptr_t)d_q | (uintptr_t)d_out | (uintptr_t)d_scratch) % 16 == 0, "q, out and the scratch must be 16-byte aligned");
   RI_REQUIRE(scale > 0.f && scale < 1e30f, "ri_paged_decode: scale must be positive and finite");
-  const int64_t groups = (int64_t)p->batch * p->kv_heads;
   PagedArgs a = {};
   static_cast<ri_page::Pages&>(a) = ri_page::view(*p);
   a.q = static_cast<const uint4*>(d_q);
   a.q_stride = q_stride / 8;
   a.gs = p->group_size;
   a.part_o = static_cast<float*>(d_scratch);
-  float* next = a.part_o + paged_slots(groups) * a.gs * RI_HEAD_DIM;
+  float* next = a.part_o + paged_slots(*p) * a.gs * RI_HEAD_DIM;
   a.part_ml = reinterpret_cast<float2*>(next);
-  next += paged_slots(groups) * a.gs * 2;
-  if (p->d_weight) {
-    a.lse2 = next;
-    next += groups * a.gs;
-    a.scores = reinterpret_cast<float*>(ri_align16((size_t)next));
-  }
+  next += paged_slots(*p) * a.gs * 2;
+  if (p->d_weight) a.scores = reinterpret_cast<float*>(ri_align16((size_t)next));
   a.lse = d_lse;
   a.out = static_cast<uint16_t*>(d_out);
   a.scale2 = RI_LOG2E * scale;
