@@ -6,11 +6,12 @@
 // slots about keep (n - keep) / n where weights are in no order, and no more than n - keep where a few generated tokens are
 // trimmed; sources lie behind `keep` and destinations in front, so no row is read after it was written.
 //
-// Two kernels.  Selection: a cluster of CTAs per group (request, KV head) maps weights to order-preserving 32-bit keys in shared
-// memory (slots beyond that are mapped again when they are needed), finds the keep-th largest by a radix select of four
-// 8-bit levels whose histograms the CTAs add up through distributed shared memory, and writes the lists of holes and of the
-// slots that fill them, both ascending.  Every thread takes a run of consecutive slots, of odd length against bank conflicts.
-// Moves: a half-warp per row, four rows in flight.  Bound by the moved rows, read once and written once.
+// Selection: a cluster of CTAs per group (request, KV head) maps weights to order-preserving 32-bit keys in shared memory (slots
+// beyond that are mapped again when they are needed), finds the keep-th largest by a radix select of three levels whose
+// histograms the CTAs add up through distributed shared memory, and writes the lists of holes and of the slots that fill them,
+// both ascending.  Every thread takes a run of consecutive slots, of odd length against bank conflicts.
+// Moves: a half-warp per row, four rows in flight; where there are few, by the same clusters, else by a second kernel over the
+// whole chip.  Bound by the moved rows, read once and written once, or by the selection's chain of dependent steps.
 #include <cooperative_groups.h>
 
 #include "ri_paged.cuh"
@@ -24,9 +25,14 @@ constexpr int kSelThreads = 512;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kCachedKeys = 40 * 1024;               // keys of a CTA's slice that shared memory holds
 constexpr int kSelMaxCluster = 8;
+#ifndef V_SLOTS
+#define V_SLOTS 512
+#endif
+constexpr int kSlotsWorthACta = V_SLOTS;
 constexpr int kMoveThreads = 256;
 constexpr int kMovesAtOnce = 4;                      // per half-warp
 constexpr int kMovesPerBlock = kMoveThreads / 16 * kMovesAtOnce;
+constexpr int kMovesInside = 256;                    // per CTA: up to that many the selection's clusters move the rows
 constexpr uint32_t kProtected = 0xffffffffu;         // above +infinity
 
 struct EvictArgs {
@@ -46,137 +52,34 @@ __device__ __forceinline__ uint32_t order_key(float w) {
 }
 
 // Exclusive scan over the block, and its total.
-__device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, T* warp_sums, T& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int incl = v;
+  T incl = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, incl, o);
+    const T x = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += x;
   }
   __syncthreads();                                     // warp_sums may still be read by the scan before
   if (lane == 31) warp_sums[warp] = incl;
   __syncthreads();
-  int before = 0;
+  T before = 0;
   total = 0;
 #pragma unroll
   for (int w = 0; w < kSelWarps; ++w) {
-    const int s = warp_sums[w];
+    const T s = warp_sums[w];
     if (w < warp) before += s;
     total += s;
   }
   return before + incl - v;
 }
 
-struct SelShared {
-  int hist[4][256];            // per level: this CTA's slots by digit
-  int totals[2];               // holes and fillers of this CTA
-  int warp_sums[kSelWarps];
-  int bin, before;             // the cut's digit, and slots of larger digits
-};
-
-__global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const __grid_constant__ EvictArgs a) {
-  extern __shared__ uint32_t s_keys[];
-  __shared__ SelShared sh;
-  ri_pdl_enter();
-  cg::cluster_group cluster = cg::this_cluster();
-  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
-  const int tid = threadIdx.x, g = blockIdx.x / ctas;
+// The moves of group (b, h): half-warp `half` of `halves` takes kMovesAtOnce neighbours at a time, whose rows often lie together.
+__device__ __forceinline__ void move_rows(const EvictArgs& a, const int2* moves, int b, int h, int half, int halves, int n) {
   const Pages& p = a.pages;
-  const int b = g / p.hk, h = g - b * p.hk, n = rows_of(p, b);
-  if (n <= a.keep) {                                   // the whole cluster leaves
-    if (rank == 0 && tid == 0) a.counts[g] = 0;
-    return;
-  }
-  const int slice = (n + ctas - 1) / ctas, lo = min(n, rank * slice), hi = min(n, lo + slice), mine = hi - lo;
-  const int newest = a.seen[b] - a.recent;
-  auto make_key = [&](int j) {
-    const int id = page_of(p, b, j >> p.shift);
-    const int64_t at = record_at(p, id, h, j & ((1 << p.shift) - 1));
-    const int t = p.token[at];
-    return (t < a.sink || t >= newest) ? kProtected : order_key(p.weight[at]);
-  };
-  for (int i = tid; i < 4 * 256; i += kSelThreads) (&sh.hist[0][0])[i] = 0;
-  for (int j = tid; j < min(mine, kCachedKeys); j += kSelThreads) s_keys[j] = make_key(lo + j);
-  __syncthreads();
-  auto key_of = [&](int j) { return j < kCachedKeys ? s_keys[j] : make_key(lo + j); };
-
-  // the keep-th largest key: digit by digit, `need` slots still to be found among those that agree so far
-  uint32_t prefix = 0;
-  int need = a.keep;
-#pragma unroll 1
-  for (int level = 0; level < 4; ++level) {
-    const int shift = 24 - 8 * level;
-    for (int j = tid; j < mine; j += kSelThreads) {
-      const uint32_t k = key_of(j);
-      if (level == 0 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&sh.hist[level][(k >> shift) & 255u], 1);
-    }
-    cluster.sync();
-    int sum = 0;
-    if (tid < 256) {                                   // thread 0 takes the largest digit
-      const int digit = 255 - tid;
-      for (int c = 0; c < ctas; ++c) sum += cluster.map_shared_rank(&sh.hist[level][0], c)[digit];
-    }
-    int total;
-    const int before = block_scan(sum, sh.warp_sums, total);
-    if (tid < 256 && before < need && before + sum >= need) {
-      sh.bin = 255 - tid;
-      sh.before = before;
-    }
-    __syncthreads();
-    prefix |= (uint32_t)sh.bin << shift;
-    need -= sh.before;
-    __syncthreads();
-  }
-  // slots with the cut's key: the first `need` of the group stay
-  int equal_before = 0;
-  for (int c = 0; c < rank; ++c) equal_before += cluster.map_shared_rank(&sh.hist[3][0], c)[prefix & 255u];
-
-  const int run = ((mine + kSelThreads - 1) / kSelThreads) | 1, first = min(mine, tid * run), last = min(mine, first + run);
-  int equal = 0;
-  for (int j = first; j < last; ++j) equal += key_of(j) == prefix;
-  int total, holes = 0, fillers = 0;
-  equal_before += block_scan(equal, sh.warp_sums, total);
-  int rank_eq = equal_before;
-  for (int j = first; j < last; ++j) {
-    const uint32_t k = key_of(j);
-    const bool stays = k > prefix || (k == prefix && rank_eq++ < need), front = lo + j < a.keep;
-    holes += front && !stays;
-    fillers += !front && stays;
-  }
-  int hole_at = block_scan(holes, sh.warp_sums, total);
-  if (tid == 0) sh.totals[0] = total;
-  int filler_at = block_scan(fillers, sh.warp_sums, total);
-  if (tid == 0) sh.totals[1] = total;
-  cluster.sync();
-  int all = 0;
-  for (int c = 0; c < ctas; ++c) {
-    const int* t = cluster.map_shared_rank(sh.totals, c);
-    if (c < rank) {
-      hole_at += t[0];
-      filler_at += t[1];
-    }
-    all += t[0];
-  }
-  int2* moves = a.moves + (int64_t)g * a.most;
-  rank_eq = equal_before;
-  for (int j = first; j < last; ++j) {
-    const uint32_t k = key_of(j);
-    const bool stays = k > prefix || (k == prefix && rank_eq++ < need), front = lo + j < a.keep;
-    if (front && !stays) moves[hole_at++].x = lo + j;
-    if (!front && stays) moves[filler_at++].y = lo + j;
-  }
-  if (rank == 0 && tid == 0) a.counts[g] = all;
-  cluster.sync();                                      // nobody's shared memory goes while others may read it
-}
-
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ EvictArgs a) {
-  ri_pdl_enter();
-  const Pages& p = a.pages;
-  const int g = blockIdx.y, b = g / p.hk, h = g - b * p.hk, n = a.counts[g];
-  const int c = threadIdx.x & 15, half = threadIdx.x >> 4;
-  const int2* moves = a.moves + (int64_t)g * a.most;
-  for (int i0 = blockIdx.x * kMovesPerBlock + half * kMovesAtOnce; i0 < n; i0 += gridDim.x * kMovesPerBlock) {
+  const int c = threadIdx.x & 15, mask = (1 << p.shift) - 1;
+  for (int i0 = half * kMovesAtOnce; i0 < n; i0 += halves * kMovesAtOnce) {
     int64_t to_k[kMovesAtOnce], to_v[kMovesAtOnce];    // negative: nothing to move
     uint4 k[kMovesAtOnce], v[kMovesAtOnce];
 #pragma unroll
@@ -184,7 +87,7 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
       to_k[u] = -1;
       if (i0 + u >= n) continue;
       const int2 m = moves[i0 + u];
-      const int id_to = page_to_write(p, b, m.x >> p.shift), id_of = page_to_write(p, b, m.y >> p.shift), mask = (1 << p.shift) - 1;
+      const int id_to = page_to_write(p, b, m.x >> p.shift), id_of = page_to_write(p, b, m.y >> p.shift);
       if ((id_to | id_of) < 0) continue;
       const int64_t in_to = ((int64_t)(h << p.shift) + (m.x & mask)) * 16 + c, in_of = ((int64_t)(h << p.shift) + (m.y & mask)) * 16 + c;
       to_k[u] = id_to * (p.key_stride / 8) + in_to;
@@ -204,6 +107,153 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
       a.values[to_v[u]] = v[u];
     }
   }
+}
+
+constexpr int kLevels = 3, kDigits = 2048;             // 11, 11 and 10 bits of the key
+struct SelShared {
+  int hist[kLevels][kDigits];  // per level: this CTA's slots by digit
+  unsigned long long totals;   // holes and fillers of this CTA, 32 bits each
+  unsigned long long warp_sums[kSelWarps];
+  int warp_counts[kSelWarps];
+  int digit, before;           // the cut's digit, and slots of larger digits
+};
+
+// MOVES: the cluster moves the rows itself.
+template <bool MOVES>
+__global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const __grid_constant__ EvictArgs a) {
+  extern __shared__ uint32_t s_keys[];
+  __shared__ __align__(16) SelShared sh;
+  ri_pdl_enter();
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
+  const int tid = threadIdx.x, g = blockIdx.x / ctas;
+  const Pages& p = a.pages;
+  const int b = g / p.hk, h = g - b * p.hk, n = rows_of(p, b);
+  if (n <= a.keep) {                                   // the whole cluster leaves
+    if (rank == 0 && tid == 0) a.counts[g] = 0;
+    return;
+  }
+  const int slice = (n + ctas - 1) / ctas, lo = min(n, rank * slice), hi = min(n, lo + slice), mine = hi - lo;
+  const int newest = a.seen[b] - a.recent;
+  auto meet = [&] {                                    // of the cluster
+    if (ctas > 1) cluster.sync();
+    else __syncthreads();
+  };
+  auto record_of = [&](int j) { return record_at(p, page_of(p, b, j >> p.shift), h, j & ((1 << p.shift) - 1)); };
+  auto key_from = [&](float w, int t) { return (t < a.sink || t >= newest) ? kProtected : order_key(w); };
+  for (int i = tid; i < kLevels * kDigits / 4; i += kSelThreads) reinterpret_cast<int4*>(&sh.hist[0][0])[i] = make_int4(0, 0, 0, 0);
+  const int cached = min(mine, kCachedKeys);
+  for (int j0 = tid; j0 < cached; j0 += 4 * kSelThreads) {      // four slots' loads on their way together
+    int64_t at[4];
+    float w[4];
+    int t[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) at[u] = j0 + u * kSelThreads < cached ? record_of(lo + j0 + u * kSelThreads) : -1;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (at[u] >= 0) {
+        w[u] = p.weight[at[u]];
+        t[u] = p.token[at[u]];
+      }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (at[u] >= 0) s_keys[j0 + u * kSelThreads] = key_from(w[u], t[u]);
+  }
+  __syncthreads();
+  auto key_of = [&](int j) {
+    if (j < kCachedKeys) return s_keys[j];
+    const int64_t at = record_of(lo + j);
+    return key_from(p.weight[at], p.token[at]);
+  };
+
+  // the keep-th largest key: digit by digit, `need` slots still to be found among those that agree so far
+  uint32_t prefix = 0;
+  int need = a.keep, ties = 0;                         // ties: slots of the group with the cut's digit
+#pragma unroll
+  for (int level = 0; level < kLevels; ++level) {
+    const int shift = level == 0 ? 21 : level == 1 ? 10 : 0;
+    const uint32_t mask = level == 2 ? 1023u : 2047u;
+    for (int j = tid; j < mine; j += kSelThreads) {
+      const uint32_t k = key_of(j);
+      if (level == 0 || (k >> (level == 1 ? 21 : 10)) == (prefix >> (level == 1 ? 21 : 10))) atomicAdd(&sh.hist[level][(k >> shift) & mask], 1);
+    }
+    meet();
+    int4 sum = make_int4(0, 0, 0, 0);                  // of four digits, the largest ones at thread 0
+    const int digit = kDigits - 4 - 4 * tid;
+    int4 of[kSelMaxCluster];
+#pragma unroll
+    for (int c = 0; c < kSelMaxCluster; ++c)
+      of[c] = c < ctas ? *reinterpret_cast<const int4*>(cluster.map_shared_rank(&sh.hist[level][0], c) + digit) : make_int4(0, 0, 0, 0);
+#pragma unroll
+    for (int c = 0; c < kSelMaxCluster; ++c) { sum.x += of[c].x; sum.y += of[c].y; sum.z += of[c].z; sum.w += of[c].w; }
+    const int four = sum.x + sum.y + sum.z + sum.w;
+    int total;
+    int before = block_scan(four, sh.warp_counts, total);
+    if (before < need && before + four >= need) {
+      int d = digit + 3;
+      const int each[4] = {sum.w, sum.z, sum.y, sum.x};
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (d == digit + 3 - i && before + each[i] < need) {
+          before += each[i];
+          --d;
+        }
+      sh.digit = d;
+      sh.before = before;
+    }
+    __syncthreads();
+    prefix |= (uint32_t)sh.digit << shift;
+    need -= sh.before;
+  }
+  for (int c = 0; c < ctas; ++c) ties += cluster.map_shared_rank(&sh.hist[kLevels - 1][0], c)[prefix & 1023u];
+  // the first `need` slots of the group with the cut's key stay; mostly that is all of them
+  const int run = ((mine + kSelThreads - 1) / kSelThreads) | 1, first = min(mine, tid * run), last = min(mine, first + run);
+  int rank_eq = 0;
+  if (ties > need) {
+    int equal = 0, total;
+    for (int c = 0; c < rank; ++c) rank_eq += cluster.map_shared_rank(&sh.hist[kLevels - 1][0], c)[prefix & 1023u];
+    for (int j = first; j < last; ++j) equal += key_of(j) == prefix;
+    rank_eq += block_scan(equal, sh.warp_counts, total);
+  } else {
+    need = ties;
+  }
+  int eq = rank_eq;
+  unsigned holes = 0, fillers = 0;
+  for (int j = first; j < last; ++j) {
+    const uint32_t k = key_of(j);
+    const bool stays = k > prefix || (k == prefix && eq++ < need), front = lo + j < a.keep;
+    holes += front && !stays;
+    fillers += !front && stays;
+  }
+  unsigned long long total, at = block_scan((unsigned long long)fillers << 32 | holes, sh.warp_sums, total);
+  if (tid == 0) sh.totals = total;
+  meet();
+  unsigned long long all = 0;
+  for (int c = 0; c < ctas; ++c) {
+    const unsigned long long x = *cluster.map_shared_rank(&sh.totals, c);
+    if (c < rank) at += x;
+    all += x;
+  }
+  int hole_at = (int)(unsigned)at, filler_at = (int)(at >> 32);
+  int2* moves = a.moves + (int64_t)g * a.most;
+  eq = rank_eq;
+  if (holes + fillers > 0)
+    for (int j = first; j < last; ++j) {
+      const uint32_t k = key_of(j);
+      const bool stays = k > prefix || (k == prefix && eq++ < need), front = lo + j < a.keep;
+      if (front && !stays) moves[hole_at++].x = lo + j;
+      if (!front && stays) moves[filler_at++].y = lo + j;
+    }
+  if (rank == 0 && tid == 0) a.counts[g] = (int)(unsigned)all;
+  meet();                                      // the list is there; nobody's shared memory goes while others may read it
+  if (MOVES) move_rows(a, moves, b, h, rank * (kSelThreads / 16) + (tid >> 4), ctas * (kSelThreads / 16), (int)(unsigned)all);
+}
+
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ EvictArgs a) {
+  ri_pdl_enter();
+  const int g = blockIdx.y, b = g / a.pages.hk, half = threadIdx.x >> 4;
+  move_rows(a, a.moves + (int64_t)g * a.most, b, g - b * a.pages.hk, blockIdx.x * (kMoveThreads / 16) + half,
+            gridDim.x * (kMoveThreads / 16), a.counts[g]);
 }
 
 int64_t most_moves(const ri_paged& p, int64_t keep) {
@@ -242,13 +292,17 @@ extern "C" int ri_paged_evict(const ri_paged* p, const int32_t* d_seen, int32_t 
   a.most = (int)most_moves(*p, keep);
   int sms = 0;
   if ((rc = ri_sm_count(&sms)) != RI_OK) return rc;
-  if ((rc = ri_allow_smem<evict_select_kernel>(kCachedKeys * 4)) != RI_OK) return rc;
-  int ctas = 1;                                        // as many CTAs to a group as fit the chip at once
-  while (ctas < kSelMaxCluster && groups * ctas * 2 <= sms) ctas *= 2;
+  int ctas = 1;                                        // as many CTAs to a group as fit the chip at once and have enough to do
+  while (ctas < kSelMaxCluster && groups * ctas * 2 <= sms && room > (int64_t)ctas * kSlotsWorthACta) ctas *= 2;
   const int64_t slice = (room + ctas - 1) / ctas;
   const size_t smem = (size_t)(slice < kCachedKeys ? slice : kCachedKeys) * 4;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  RI_CUDA_OK(ri_launch_pdl_cluster(11, ctas, evict_select_kernel, dim3((unsigned)(groups * ctas)), dim3(kSelThreads), smem, s, a));
+  const bool moves = a.most <= (int64_t)ctas * kMovesInside;
+  if ((rc = moves ? ri_allow_smem<evict_select_kernel<true>>(kCachedKeys * 4) : ri_allow_smem<evict_select_kernel<false>>(kCachedKeys * 4)) != RI_OK)
+    return rc;
+  RI_CUDA_OK(ri_launch_pdl_cluster(11, ctas, moves ? evict_select_kernel<true> : evict_select_kernel<false>, dim3((unsigned)(groups * ctas)),
+                                   dim3(kSelThreads), smem, s, a));
+  if (moves) return RI_OK;
   const int64_t blocks = ((int64_t)a.most + kMovesPerBlock - 1) / kMovesPerBlock, wanted = (int64_t)sms * 16 / groups + 1;
   RI_CUDA_OK(ri_launch_pdl_id(11, evict_move_kernel, dim3((unsigned)(blocks < wanted ? blocks : wanted), (unsigned)groups),
                               dim3(kMoveThreads), 0, s, a));
