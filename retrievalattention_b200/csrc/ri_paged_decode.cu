@@ -13,6 +13,9 @@
 // A second kernel merges a group's partial results by log-sum-exp in a fixed order.  For the weights the first kernel
 // leaves the scores behind (4 bytes a slot and query head, against 512 a slot for K and V), and the second turns them into
 // probabilities; every slot has one thread, so the sums have one order and no atomics.
+// Short requests that leave the chip room give every group a cluster of CTAs, which does all of this in one kernel.
+#include <cooperative_groups.h>
+
 #include "ri_paged.cuh"
 #include "ri_step_sequence.cuh"
 #include "ri_tc.cuh"
@@ -39,6 +42,7 @@ constexpr int kPagedMaxCtas = 160;                    // the grid is one CTA per
 constexpr int kPagedRing = kPagedWarps * kStages * kStageBytes;   // 192 KB, on a 1024-byte boundary
 constexpr int kPagedSmem = 1024 + kPagedRing;
 constexpr int kFinishThreads = 256;
+constexpr int kMaxCluster = 8;
 
 struct PagedArgs : Pages {
   static constexpr int kStep = 16;
@@ -54,8 +58,12 @@ struct PagedArgs : Pages {
 };
 __device__ __forceinline__ int used_ctas(int total, int max_ctas) { return ri_seq::used_ctas<kPagedWarps>(total, max_ctas); }
 
-// BOX: rows of a TMA box.
-template <int DT, int BOX, bool WEIGHTS>
+// The scores of a step lie in the order of the lanes that made them: place i holds key (i / 2 % 2) * 8 + i / 4 + (i % 2) * 4.
+__device__ __forceinline__ int slot_in_step(int place) { return (place & ~15) + ((place >> 1) & 1) * 8 + ((place >> 2) & 3) + (place & 1) * 4; }
+
+// BOX: rows of a TMA box.  CLUSTER: a group per cluster, which shares out the group's steps, joins the partial results through
+// distributed shared memory and adds the weights: no second kernel.
+template <int DT, int BOX, bool WEIGHTS, bool CLUSTER>
 __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                      const __grid_constant__ CUtensorMap map_v,
                                                                      const __grid_constant__ PagedArgs a) {
@@ -64,6 +72,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
   __shared__ __align__(8) uint64_t s_full[kPagedWarps][kStages];
   __shared__ int s_abort;
   __shared__ float sm_m[kPagedWarps][kMaxHeads], sm_l[kPagedWarps][kMaxHeads];
+  __shared__ float2 s_ml[kMaxHeads];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = lane >> 2, t = lane & 3, gs = a.gs;
   const int sr = ((r & 1) << 2) | (r >> 1);              // the lane's row and pieces, see ri_dense_decode.cu
@@ -79,12 +88,33 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
   // they are without waiting for this one.
   ri_pdl_wait();
   ri_pdl_trigger();
-  const int total = count_steps(a), n_ctas = used_ctas(total, a.max_ctas), c = (int)blockIdx.x;
-  if (c >= n_ctas || total == 0) return;
-  const int c_lo = cta_start(c, total, n_ctas), c_hi = cta_start(c + 1, total, n_ctas), c_n = c_hi - c_lo;
-  const int lo = c_lo + c_n * warp / kPagedWarps, hi = c_lo + c_n * (warp + 1) / kPagedWarps;
-  const Place c_first = find_place(a, c_lo);
-  const bool merged = c_hi <= c_first.first + steps_of(c_first.rows);      // the CTA's range lies inside one group
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = CLUSTER ? (int)cluster.num_blocks() : 1, rank = CLUSTER ? (int)cluster.block_rank() : 0;
+  const int c = (int)blockIdx.x;
+  int c_lo, c_hi;                                        // this CTA's steps: of the whole sequence, or of its group
+  Place c_first;
+  int64_t score_step = 0;                                // where the group's scores begin, if steps are counted by group
+  if (CLUSTER) {
+    const int g = c / ctas, b = g / a.hk, rows = rows_of(a, b), n = steps_of(rows);
+    if (n == 0) {                                        // the whole cluster leaves
+      for (int i = tid + rank * kPagedThreads; i < gs * RI_HEAD_DIM; i += ctas * kPagedThreads) a.out[(int64_t)g * gs * RI_HEAD_DIM + i] = 0;
+      if (rank == 0 && tid < gs && a.lse != nullptr) a.lse[g * gs + tid] = -INFINITY;
+      return;
+    }
+    c_first = {g, 0, rows};
+    c_lo = (int)((int64_t)n * rank / ctas);
+    c_hi = (int)((int64_t)n * (rank + 1) / ctas);
+    score_step = (int64_t)g * steps_of(a.table_stride << a.shift);
+  } else {
+    const int total = count_steps(a), n_ctas = used_ctas(total, a.max_ctas);
+    if (c >= n_ctas || total == 0) return;
+    c_lo = cta_start(c, total, n_ctas);
+    c_hi = cta_start(c + 1, total, n_ctas);
+    c_first = find_place(a, c_lo);
+  }
+  const int c_n = c_hi - c_lo, lo = c_lo + c_n * warp / kPagedWarps, hi = c_lo + c_n * (warp + 1) / kPagedWarps;
+  const bool merged = CLUSTER || c_hi <= c_first.first + steps_of(c_first.rows);      // the CTA's range lies inside one group
 
   // a stage: K, then V; of each the boxes one behind the other, a box as two halves of 64 channels
   constexpr int kTensor = kStageBytes / 2, kBox = BOX * 256, kHalf = BOX * 128, kStageStride = kPagedWarps * kStageBytes;
@@ -125,7 +155,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
 
   clear();
   if (lo < hi) {
-    Place at_issue = find_place(a, lo), at = at_issue;
+    Place at_issue = CLUSTER ? c_first : find_place(a, lo), at = at_issue;
     // pages of the next step to issue; the second one only where a page is half a step
     int id0 = 0, id1 = 0;
     auto fetch_ids = [&](int s) {
@@ -196,7 +226,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
           s2[jj][e] = base + jj * 8 + t + 4 * e < at.rows ? (c1[e] + c2[e]) * a.scale2 : -INFINITY;
       }
       if (WEIGHTS && r < gs)
-        reinterpret_cast<float4*>(a.scores)[((int64_t)s * gs + r) * 4 + t] = make_float4(s2[0][0], s2[0][1], s2[1][0], s2[1][1]);
+        reinterpret_cast<float4*>(a.scores)[((score_step + s) * gs + r) * 4 + t] = make_float4(s2[0][0], s2[0][1], s2[1][0], s2[1][1]);
       // online softmax for head r
       float mx = fmaxf(fmaxf(s2[0][0], s2[0][1]), fmaxf(s2[1][0], s2[1][1]));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -252,6 +282,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
   reduce_sum();
   if (t == 0) { sm_m[warp][r] = m_run; sm_l[warp][r] = l_run; }
   auto warp_o = [&](int w) { return reinterpret_cast<float*>(ring + w * kStageBytes); };
+  float* cta_o = reinterpret_cast<float*>(ring + kPagedWarps * kStageBytes);      // CLUSTER: this CTA's partial result
   put(warp_o(warp));
   __syncthreads();
   const int64_t slot = (int64_t)c * kPagedWarps + c_first.g;
@@ -267,9 +298,62 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
       L += sm_l[w][h] * f;
       O += warp_o(w)[idx] * f;
     }
-    a.part_o[slot * gs * RI_HEAD_DIM + idx] = O;
-    if ((idx & 127) == 0) a.part_ml[slot * gs + h] = make_float2(M, L);
+    if (CLUSTER) {
+      cta_o[idx] = O;
+      if ((idx & 127) == 0) s_ml[h] = make_float2(M, L);
+    } else {
+      a.part_o[slot * gs * RI_HEAD_DIM + idx] = O;
+      if ((idx & 127) == 0) a.part_ml[slot * gs + h] = make_float2(M, L);
+    }
   }
+  if (!CLUSTER) return;
+
+  cluster.sync();
+  // reference and sum of head h over the cluster
+  auto joined = [&](int h, float2 (&ml)[kMaxCluster]) {
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMaxCluster; ++i) {
+      ml[i] = i < ctas ? *cluster.map_shared_rank(&s_ml[h], i) : make_float2(-INFINITY, 0.f);
+      M = fmaxf(M, ml[i].x);
+    }
+    M = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int i = 0; i < kMaxCluster; ++i) L += ml[i].y * exp2f(ml[i].x - M);
+    return make_float2(M, L);
+  };
+  for (int idx = tid + rank * kPagedThreads; idx < gs * RI_HEAD_DIM; idx += ctas * kPagedThreads) {
+    float2 ml[kMaxCluster];
+    float o[kMaxCluster], O = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMaxCluster; ++i) o[i] = i < ctas ? cluster.map_shared_rank(cta_o, i)[idx] : 0.f;
+    const float2 all = joined(idx >> 7, ml);
+#pragma unroll
+    for (int i = 0; i < kMaxCluster; ++i) O += o[i] * exp2f(ml[i].x - all.x);
+    a.out[(int64_t)c_first.g * gs * RI_HEAD_DIM + idx] = Elem<DT>::bits(all.y > 0.f ? O / all.y : 0.f);
+    if ((idx & 127) == 0 && a.lse != nullptr) a.lse[c_first.g * gs + (idx >> 7)] = all.y > 0.f ? (all.x + log2f(all.y)) * 0.69314718055994531f : -INFINITY;
+  }
+  if (WEIGHTS) {
+    if (tid < gs) {
+      float2 ml[kMaxCluster];
+      const float2 all = joined(tid, ml);
+      sm_l[0][tid] = all.y > 0.f ? all.x + log2f(all.y) : INFINITY;      // nothing to give: 0
+    }
+    __syncthreads();
+    const int b = c_first.g / a.hk, h_kv = c_first.g - b * a.hk;
+    for (int place = c_lo * 16 + tid; place < c_hi * 16; place += kPagedThreads) {      // this CTA's own scores
+      const int i = place & 15, at = slot_in_step(place);
+      const int id = at < c_first.rows ? page_to_write(a, b, at >> a.shift) : -1;
+      if (id < 0) continue;
+      const float* of = a.scores + ((score_step + (place >> 4)) * gs) * 16 + i;
+      float sum = 0.f;
+#pragma unroll
+      for (int h = 0; h < kMaxHeads; ++h)
+        if (h < gs) sum += exp2f(of[h * 16] - sm_l[0][h]);
+      a.weight[record_at(a, id, h_kv, at & ((1 << a.shift) - 1))] += sum;
+    }
+  }
+  cluster.sync();                                        // nobody's shared memory goes while others may read it
 }
 
 // What is left once every partial result is there, a group per blockIdx.y: its blocks join the partial results, a query head at
@@ -327,10 +411,7 @@ __global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_ke
   // a tile of slots: pages (their tables do not change either), then scores and weights
   int id[kFoldEach];
   float sc[kFoldEach][kMaxHeads], old[kFoldEach];
-  auto slot_of = [&](int tile, int e) {      // place i of a step holds its key (i / 2 % 2) * 8 + i / 4 + (i % 2) * 4
-    const int place = tile * kFoldSlots + e * kFinishThreads + tid, i = place & 15;
-    return (place & ~15) + ((i >> 1) & 1) * 8 + (i >> 2) + (i & 1) * 4;
-  };
+  auto slot_of = [&](int tile, int e) { return slot_in_step(tile * kFoldSlots + e * kFinishThreads + tid); };
   auto weight_at = [&](int tile, int e) { return a.weight + record_at(a, id[e], h_kv, slot_of(tile, e) & ((1 << a.shift) - 1)); };
   auto find_pages = [&](int tile) {
 #pragma unroll
@@ -478,22 +559,40 @@ int make_page_map(CUtensorMap* map, const void* base, const ri_paged& p, int64_t
   return RI_OK;
 }
 
+// CTAs of a cluster where every group can have a cluster at once and the longest request that fits the tables is short; 0: no
+// clusters.  Clusters lie inside one GPC, so not every SM can be in one.  A second kernel costs 2 us of host and device time; an even
+// split over all SMs gains more than that from five steps a warp on (8 heads of 4, a call: 777 slots 11.3 us with two kernels,
+// 9.6 with clusters; 4000 slots, four steps a warp, 11.6 and 9.7; 8000 slots 13.9 and 14.9).
+constexpr int kClusterSteps = 4;                       // of a warp, at most
+int cluster_size(const PagedArgs& a) {
+  const int64_t groups = (int64_t)a.batch * a.hk, steps = (((int64_t)a.table_stride << a.shift) + 15) / 16;
+  int ctas = 0;
+  for (int n = 1; n <= kMaxCluster; n *= 2)
+    if (groups * n <= a.max_ctas * 4 / 5 && (ctas == 0 || steps > (int64_t)ctas * kPagedWarps)) ctas = n;
+  return ctas > 0 && steps <= (int64_t)ctas * kPagedWarps * kClusterSteps ? ctas : 0;
+}
 template <int DT, int BOX, bool WEIGHTS>
-int launch_steps(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t s) {
+int launch_steps(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, int ctas, cudaStream_t s) {
   int rc;
-  if ((rc = ri_allow_smem<paged_decode_kernel<DT, BOX, WEIGHTS>>(kPagedSmem)) != RI_OK) return rc;
-  RI_CUDA_OK(ri_launch_pdl_id(11, paged_decode_kernel<DT, BOX, WEIGHTS>, dim3(a.max_ctas), dim3(kPagedThreads), (size_t)kPagedSmem, s,
+  if (ctas > 0) {
+    if ((rc = ri_allow_smem<paged_decode_kernel<DT, BOX, WEIGHTS, true>>(kPagedSmem)) != RI_OK) return rc;
+    RI_CUDA_OK(ri_launch_pdl_cluster(11, ctas, paged_decode_kernel<DT, BOX, WEIGHTS, true>, dim3(a.batch * a.hk * ctas), dim3(kPagedThreads),
+                                     (size_t)kPagedSmem, s, map_k, map_v, a));
+    return RI_OK;
+  }
+  if ((rc = ri_allow_smem<paged_decode_kernel<DT, BOX, WEIGHTS, false>>(kPagedSmem)) != RI_OK) return rc;
+  RI_CUDA_OK(ri_launch_pdl_id(11, paged_decode_kernel<DT, BOX, WEIGHTS, false>, dim3(a.max_ctas), dim3(kPagedThreads), (size_t)kPagedSmem, s,
                               map_k, map_v, a));
   return RI_OK;
 }
 template <int DT, int BOX>
-int launch_steps(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t s) {
-  return a.weight ? launch_steps<DT, BOX, true>(a, map_k, map_v, s) : launch_steps<DT, BOX, false>(a, map_k, map_v, s);
+int launch_steps(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, int ctas, cudaStream_t s) {
+  return a.weight ? launch_steps<DT, BOX, true>(a, map_k, map_v, ctas, s) : launch_steps<DT, BOX, false>(a, map_k, map_v, ctas, s);
 }
 template <int DT>
 int launch_paged(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, int box, cudaStream_t s) {
-  int rc = box == 8 ? launch_steps<DT, 8>(a, map_k, map_v, s) : launch_steps<DT, 16>(a, map_k, map_v, s);
-  if (rc != RI_OK) return rc;
+  const int ctas = cluster_size(a), rc = box == 8 ? launch_steps<DT, 8>(a, map_k, map_v, ctas, s) : launch_steps<DT, 16>(a, map_k, map_v, ctas, s);
+  if (rc != RI_OK || ctas > 0) return rc;
   const int64_t groups = (int64_t)a.batch * a.hk, most = (int64_t)a.table_stride << a.shift;
   // blocks of a group: for its heads, or with weights its tiles of slots, as many as the chip holds at once
   const int64_t tiles = a.weight ? (most + kFoldSlots - 1) / kFoldSlots : 0, room = kFinishBlocks * (int64_t)a.max_ctas / groups;

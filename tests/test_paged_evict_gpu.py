@@ -179,3 +179,6 @@ def test_refusals():
     for change in (dict(keep=0), dict(keep=13), dict(n_sink=-1), dict(n_recent=-1), dict(n_sink=2 ** 31 - 1, n_recent=2 ** 31 - 1)):
         with pytest.raises(RuntimeError, match="keep"):
             paged.paged_evict(**{**good, **change})
+    odd = torch.zeros(layer.weight.numel() + 1, device="cuda")[1:].view(layer.weight.shape)
+    with pytest.raises(RuntimeError, match="aligned"):
+        paged.paged_evict(**{**good, "weight": odd})
