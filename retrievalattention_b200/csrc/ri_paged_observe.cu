@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
             const int i = u * 32 + (tid >> 4), r = a.first_row + i, w = r / a.gs;
-            x[u] = i < a.rows ? ri_ldg16(a.q + ((int64_t)(b * a.window + w) * a.hk * a.gs + h * a.gs + r - w * a.gs) * 16 + piece)
+            x[u] = i < a.rows ? ri_ldg16(a.q + (((int64_t)b * a.window + w) * a.hk * a.gs + h * a.gs + r - w * a.gs) * 16 + piece)
                               : make_uint4(0, 0, 0, 0);
           }
 #pragma unroll

@@ -190,8 +190,8 @@ class PagedDecoder(SyntheticDecoder):
         from .attn_hub import retroinfer_prefill_attn
 
         s, counts = self.shape, [int(p.numel()) for p in prompts]
-        if min(counts) < 1:
-            raise ValueError("every prompt has a token")
+        if len(counts) != self.batch or min(counts) < 1 or any(self.cache.length_of):
+            raise ValueError("expected a prompt of a token or more for every request, and an empty cache")
         if positions is None:
             positions = [torch.arange(n, device=self.device).expand(self.axes, n) for n in counts]
         where = torch.cat(list(positions), 1).to(torch.int64).contiguous()

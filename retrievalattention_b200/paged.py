@@ -32,8 +32,12 @@ _SCALE = DIM ** -0.5
 _BINDING = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "_paged_binding.so")
 
 
-def _load_binding():
-    """The checks of the arguments and the calls (``binding/paged.cpp``), connected to the library's functions."""
+_native = None                             # the checks of the arguments and the calls (binding/paged.cpp)
+
+
+def _connect():
+    """Load them on first use, and hand over the library's functions."""
+    global _native
     if not os.path.exists(_BINDING):
         raise ImportError(f"{_BINDING} is missing: build it with `python -m retrievalattention_b200.build`")
     spec = importlib.util.spec_from_file_location("_paged_binding", _BINDING)
@@ -42,10 +46,8 @@ def _load_binding():
     names = ("ri_last_error", "ri_rope_paged_append", "ri_paged_decode_scratch_bytes", "ri_paged_decode",
              "ri_paged_observe_scratch_bytes", "ri_paged_observe", "ri_paged_evict_scratch_bytes", "ri_paged_evict")
     module.connect({n: C.cast(getattr(_lib.lib, n), C.c_void_p).value for n in names})
+    _native = module
     return module
-
-
-_native = _load_binding()
 
 
 def rope_sections(*sections: int) -> tuple:
@@ -84,8 +86,9 @@ def rope_paged_append(qkv, cos_sin, positions, axis_of, q, key_pages, value_page
     is.  Where ``weight`` and ``token`` are given, the new slots start with weight 0 and the token numbers ``seen[b]``,
     ``seen[b] + 1``, ...  ``keys`` and ``values`` ``[rows, kv_heads, 128]`` take the rows a second time, as
     ``retroinfer_prefill_attn`` reads them."""
-    _native.append(qkv, cos_sin, positions, _axes(axis_of), q, key_pages, value_pages, page_table, lengths, row_start, weight, token,
-                   seen, keys, values, _status.address())
+    native = _native or _connect()
+    native.append(qkv, cos_sin, positions, _axes(axis_of), q, key_pages, value_pages, page_table, lengths, row_start, weight, token,
+                  seen, keys, values, _status.address())
     _status.report(_status.word(qkv.device))
 
 
@@ -94,8 +97,9 @@ def paged_decode(q, key_pages, value_pages, page_table, lengths, *, out=None, ls
     head) over the slots in use, which the token's own row is one of.  Returns ``out`` like ``q``; ``lse`` fp32 ``[batch, q_heads]``
     takes the log-sum-exp of the scaled scores (``scale``: 1/sqrt(128)).  A request without slots has out 0 and lse -infinity.
     ``weight``: every slot's weight grows by the probabilities it got, summed over the query heads of its KV head."""
-    out = _native.decode(q, key_pages, value_pages, page_table, lengths, out, lse, weight, _SCALE if scale is None else scale,
-                         _status.address())
+    native = _native or _connect()
+    out = native.decode(q, key_pages, value_pages, page_table, lengths, out, lse, weight, _SCALE if scale is None else scale,
+                        _status.address())
     _status.report(_status.word(q.device))
     return out
 
@@ -105,7 +109,8 @@ def paged_observe(q, key_pages, page_table, lengths, weight, *, scale=None):
     q_heads, 128]``, the rows of the last ``window`` tokens in use, each of which sees the slots up to its own; summed over queries
     and over the query heads of a KV head.  What ``paged_evict`` goes by after a prompt.  Requests shorter than the window are
     padded in front, with anything.  Slots must be in the order of their tokens (no eviction before)."""
-    _native.observe(q, key_pages, page_table, lengths, weight, _SCALE if scale is None else scale, _status.address())
+    native = _native or _connect()
+    native.observe(q, key_pages, page_table, lengths, weight, _SCALE if scale is None else scale, _status.address())
     _status.report(_status.word(q.device))
 
 
@@ -116,5 +121,6 @@ def paged_evict(key_pages, value_pages, weight, token, page_table, lengths, seen
     of the i-th one behind it that stays, so slots are no longer in the order of their tokens.  ``lengths`` and the page tables are
     left alone: clamp the lengths to ``keep`` when the last layer is done, and the pages behind are free.  Requests must not share
     pages."""
-    _native.evict(key_pages, value_pages, weight, token, page_table, lengths, seen, keep, n_sink, n_recent, _status.address())
+    native = _native or _connect()
+    native.evict(key_pages, value_pages, weight, token, page_table, lengths, seen, keep, n_sink, n_recent, _status.address())
     _status.report(_status.word(key_pages.device))
