@@ -89,7 +89,7 @@ def rope_paged_append(qkv, cos_sin, positions, axis_of, q, key_pages, value_page
     native = _native or _connect()
     native.append(qkv, cos_sin, positions, _axes(axis_of), q, key_pages, value_pages, page_table, lengths, row_start, weight, token,
                   seen, keys, values, _status.address())
-    _status.report(_status.word(qkv.device))
+    _status.done(qkv.device)
 
 
 def paged_decode(q, key_pages, value_pages, page_table, lengths, *, out=None, lse=None, weight=None, scale=None):
@@ -100,7 +100,7 @@ def paged_decode(q, key_pages, value_pages, page_table, lengths, *, out=None, ls
     native = _native or _connect()
     out = native.decode(q, key_pages, value_pages, page_table, lengths, out, lse, weight, _SCALE if scale is None else scale,
                         _status.address())
-    _status.report(_status.word(q.device))
+    _status.done(q.device)
     return out
 
 
@@ -111,7 +111,7 @@ def paged_observe(q, key_pages, page_table, lengths, weight, *, scale=None):
     padded in front, with anything.  Slots must be in the order of their tokens (no eviction before)."""
     native = _native or _connect()
     native.observe(q, key_pages, page_table, lengths, weight, _SCALE if scale is None else scale, _status.address())
-    _status.report(_status.word(q.device))
+    _status.done(q.device)
 
 
 def paged_evict(key_pages, value_pages, weight, token, page_table, lengths, seen, keep, n_sink=0, n_recent=0):
@@ -123,4 +123,4 @@ def paged_evict(key_pages, value_pages, weight, token, page_table, lengths, seen
     pages."""
     native = _native or _connect()
     native.evict(key_pages, value_pages, weight, token, page_table, lengths, seen, keep, n_sink, n_recent, _status.address())
-    _status.report(_status.word(key_pages.device))
+    _status.done(key_pages.device)

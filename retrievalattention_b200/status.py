@@ -65,3 +65,10 @@ def report(status: C.c_int32) -> None:
     set it."""
     if status.value and not torch.cuda.is_current_stream_capturing():
         check()
+
+
+def done(device) -> None:
+    """``report`` for a call that ran on ``device``."""
+    _devices.add(device)
+    if _word.value:
+        report(_word)
