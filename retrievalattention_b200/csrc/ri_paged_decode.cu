@@ -360,9 +360,9 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
 // a time, and with weights turn the group's scores into probabilities, kFoldSlots slots at a time, a thread per slot.  Every
 // block works out lse of all heads (warp h of head h), so none waits for another.  Which partial results the group has
 // follows from the lengths, so a warp lists them, in the order of the sequence, before the wait for the kernel that makes them.
-constexpr int kFoldEach = 4, kFoldSlots = kFoldEach * kFinishThreads;
-constexpr int kFinishBlocks = 2;                         // of an SM
-constexpr int kTogether = 8;                             // partial results of a warp on their way
+constexpr int kFoldEach = 2, kFoldSlots = kFoldEach * kFinishThreads;
+constexpr int kFinishBlocks = 4;                         // of an SM
+constexpr int kTogether = 4;                             // partial results of a warp on their way
 template <int DT>
 __global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_kernel(const __grid_constant__ PagedArgs a) {
   extern __shared__ int s_slot[];                        // [most partial results of a group]
