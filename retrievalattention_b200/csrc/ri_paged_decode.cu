@@ -14,6 +14,10 @@
 // leaves the scores behind (4 bytes a slot and query head, against 512 a slot for K and V), and the second turns them into
 // probabilities; every slot has one thread, so the sums have one order and no atomics.
 // Short requests that leave the chip room give every group a cluster of CTAs, which does all of this in one kernel.
+// B200, bf16, 8 heads of 4: 4 x 131072 slots 340 us, 6.3 TB/s (a copy: 6.6); 4 requests of 20K to 32K with weights 91 us, 4.8 TB/s:
+// 3.4 us until the first rows are there, the SMs done after 57 to 76 us (40 of the 148 read an eighth slower, the same ones in
+// every run), 2 until the second kernel knows, 7 for it.  CTAs that take work from ones not launched yet ended together, but the
+// units that this takes have few steps a warp and many partial results: 340 -> 362 and 98 -> 108 us.
 #include <cooperative_groups.h>
 
 #include "ri_paged.cuh"

@@ -9,12 +9,17 @@
 // Either way the reduction stays inside a thread; the operands lie in shared memory the same way for both (rows of 128 channels in
 // two 128-byte-swizzled halves), only their roles change.  A slot's weight has one thread, so there are no atomics.
 // The split is that of the decode kernels: tiles of 128 slots of all groups behind one another, an equal contiguous range per SM.
-// Pass 1 leaves a (maximum, sum) per row and range; a small kernel between the passes merges them.
+// Pass 1 leaves a (maximum, sum) per row and range; pass 2 merges its group's, or where they are many a kernel between the passes.
 // Four warps bring in tiles, issue the products and idle, sixteen work on scores: two sides of eight, one per tile of query
 // rows in pass 1 (or every second tile of keys, where there is only one), every second tile of keys in pass 2; of a side's
 // scores four warps take the first half of the columns and four the second.
 // TMEM: 256 columns of scores for each side.  Every wait is bounded; one that runs out is recorded in the
-// status word.  Bound by the exponentials, two for each slot and query row.
+// status word.
+// Bound by the exponentials, two for each slot and query row.  B200, 4 requests of 20K to 32K slots, 8 heads, 256 query rows: 171 us
+// in a repeated run, 1.26 Tera-exponentials a second each way against 2.1 that the SMs have at 16 a clock; pass 1 takes 71 us
+// from rest (exponentials busy 79 % of the active cycles, tensor pipe 39 %), pass 2 82 (69 %: it also reads each row's lse).  With
+// eight score warps 188 us: two warps of a scheduler do not cover each other's loads and barriers.  Some of the exponentials as
+// polynomials on the FMA pipe gained nothing with either.
 #include <cuda.h>
 
 #include "ri_paged.cuh"
@@ -38,12 +43,13 @@ constexpr int kPartials = 2 * kRows;             // a (maximum, sum) for each ro
 constexpr uint32_t kTmemCols = 512;
 constexpr int kObsSmem = 1024 + kRowTile + kRing * kKeyTile;
 constexpr int kObsMaxCtas = 160;
+constexpr int kMergedInside = 16;                // CTAs of a group, see ri_paged_observe
 
 struct ObsArgs : Pages {
   static constexpr int kStep = kTile;
   const uint4* q;                                // [batch][window][hk * gs][16 pieces]
   float2* part;                                  // [slots][half][kRows]: (maximum in the log2 domain, sum)
-  float* lse2;                                   // [groups][kRows]; +infinity: the row gives nothing
+  float* lse2;                                   // [groups][kRows], +infinity: the row gives nothing; null: pass 2 merges `part`
   int window, gs, first_row, rows;               // rows first_row .. first_row + rows - 1 of window * gs
   int max_ctas;
   float scale2;
@@ -106,6 +112,42 @@ __device__ __forceinline__ float column_sum(uint32_t taddr, int chunks, float sc
 // The last slot that query row `row` sees in a request of n slots (negative: none).
 __device__ __forceinline__ int last_seen(const ObsArgs& a, int n, int row) { return n - a.window + row / a.gs; }
 
+struct Sum {                                         // of 2^(x - m)
+  float m = -INFINITY, l = 0.f;
+  template <int N>
+  __device__ __forceinline__ void add(const float2 (&x)[N]) {
+    float m_new = m, each = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m_new = fmaxf(m_new, x[i].x);
+    if (m_new == -INFINITY) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i) each += x[i].y * ex2(x[i].x - m_new);
+    l = l * ex2(m - m_new) + each;
+    m = m_new;
+  }
+  __device__ __forceinline__ float lse2() const { return l > 0.f || l != l ? m + log2f(l) : INFINITY; }      // no slot: gives nothing
+};
+// The CTA that pass 1 gave tile t to.
+__device__ __forceinline__ int cta_of(int t, int total, int n_ctas) {
+  int c = (int)((int64_t)t * n_ctas / total);
+  while (c > 0 && ri_seq::cta_start(c, total, n_ctas) > t) --c;
+  while (ri_seq::cta_start(c + 1, total, n_ctas) <= t) ++c;
+  return c;
+}
+// Adds row `row`'s partial results of CTAs c0, c0 + step, ... below c1.
+__device__ __forceinline__ void add_partials(const ObsArgs& a, Sum& sum, int g, int row, int c0, int c1, int step) {
+  const int each = a.rows <= kTile ? 4 : 2;          // partial results of a CTA: two halves of the columns, and of one or both sides
+  for (int c = c0; c < c1; c += 4 * step) {          // four CTAs' on their way together
+    float2 x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int u = c + (i >> 2) * step, k = i & 3;
+      x[i] = u < c1 && k < each ? a.part[(int64_t)(u + g) * kPartials + (k & 1) * kRows + (k >> 1) * kTile + row] : make_float2(-INFINITY, 0.f);
+    }
+    sum.add(x);
+  }
+}
+
 // STATS: pass 1.
 template <int DT, bool STATS>
 __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ ObsArgs a) {
@@ -147,8 +189,7 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
   const uint32_t tmem = s_tmem_base;
   volatile int* abort_flag = &s_abort;
   // Pass 1 lets the next kernel start when the kernel in front of it has ended, not before.  So pass 2, which starts behind
-  // pass 1 and beside the merge between them, finds queries, keys and lengths as they are, and waits for the merge only where it
-  // reads what that wrote.
+  // pass 1 or beside the merge, finds queries, keys and lengths as they are, and waits only where it reads what those wrote.
   if (STATS) ri_pdl_wait();
   ri_pdl_trigger();
 
@@ -251,7 +292,16 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
             ri_pdl_wait();
             asm volatile("bar.sync 1, %0;" ::"n"(kScoreThreads) : "memory");
             if (tid < kRows) {
-              const float lse2 = a.lse2[(int64_t)at.g * kRows + tid];
+              float lse2;
+              if (a.lse2 != nullptr) {
+                lse2 = a.lse2[(int64_t)at.g * kRows + tid];
+              } else {
+                Sum sum;
+                const int last_tile = at.first + ri_seq::steps_of<kTile>(n) - 1;
+                if (tid < a.rows)
+                  add_partials(a, sum, at.g, tid, cta_of(at.first, total, n_ctas), cta_of(last_tile, total, n_ctas) + 1, 1);
+                lse2 = sum.lse2();
+              }
               s_neg_lse[tid] = -lse2;
               if (lse2 != lse2) s_nan = 1;
               s_last[tid] = last_seen(a, n, a.first_row + tid);
@@ -383,41 +433,32 @@ __global__ void __launch_bounds__(256) observe_merge_kernel(const __grid_constan
   __shared__ float2 s_part[8][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = blockIdx.y, b = g / a.hk;
   const int row = blockIdx.x * 32 + lane, tiles = ri_seq::steps_of<kTile>(rows_of(a, b));
-  const bool both = a.rows > kTile;
-  float m = -INFINITY, l = 0.f;
-  auto add = [&](float2 x) {
-    const float m_new = fmaxf(m, x.x);
-    if (m_new == -INFINITY) return;
-    l = l * exp2f(m - m_new) + x.y * exp2f(x.x - m_new);
-    m = m_new;
-  };
-  if (tiles > 0 && row < a.rows) {
-    int before = 0;
-    for (int i = 0; i < b; ++i) before += ri_seq::steps_of<kTile>(rows_of(a, i));
-    int total = before;
-    for (int i = b; i < a.batch; ++i) total += ri_seq::steps_of<kTile>(rows_of(a, i));
-    total *= a.hk;
-    const int n_ctas = min(a.max_ctas, total), lo = before * a.hk + (g - b * a.hk) * tiles, hi = lo + tiles;
-    int c0 = (int)((int64_t)lo * n_ctas / total);           // the CTA that holds tile lo
-    while (c0 > 0 && ri_seq::cta_start(c0, total, n_ctas) > lo) --c0;
-    while (ri_seq::cta_start(c0 + 1, total, n_ctas) <= lo) ++c0;
-    for (int c = c0 + warp; c < n_ctas && ri_seq::cta_start(c, total, n_ctas) < hi; c += 8) {
-      const float2* part = a.part + (int64_t)(c + g) * kPartials + row;
-      add(part[0]);
-      add(part[kRows]);
-      if (!both) {                                       // the other side's tiles
-        add(part[kTile]);
-        add(part[kRows + kTile]);
-      }
-    }
+  Sum sum;
+  int before = 0, total = 0;
+  for (int i = lane; i < a.batch; i += 32) {
+    const int t = ri_seq::steps_of<kTile>(rows_of(a, i));
+    total += t;
+    if (i < b) before += t;
   }
-  s_part[warp][lane] = make_float2(m, l);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
+  total *= a.hk;
+  if (tiles > 0 && row < a.rows) {
+    const int lo = before * a.hk + (g - b * a.hk) * tiles, n_ctas = min(a.max_ctas, total);
+    add_partials(a, sum, g, row, cta_of(lo, total, n_ctas) + warp, cta_of(lo + tiles - 1, total, n_ctas) + 1, 8);
+  }
+  s_part[warp][lane] = make_float2(sum.m, sum.l);
   __syncthreads();
   if (warp == 0) {
-    m = -INFINITY;
-    l = 0.f;
-    for (int w = 0; w < 8; ++w) add(s_part[w][lane]);
-    a.lse2[(int64_t)g * kRows + row] = l > 0.f ? m + log2f(l) : INFINITY;
+    float2 x[8];
+#pragma unroll
+    for (int w = 0; w < 8; ++w) x[w] = s_part[w][lane];
+    sum = Sum();
+    sum.add(x);
+    a.lse2[(int64_t)g * kRows + row] = sum.lse2();
   }
 }
 
@@ -446,7 +487,7 @@ int launch_observe(ObsArgs a, const CUtensorMap& map_k, cudaStream_t s) {
     a.rows = rows - a.first_row < kRows ? rows - a.first_row : kRows;
     a.idesc = idesc_f16(DT, 128, 128);
     RI_CUDA_OK(ri_launch_pdl_id(11, observe_kernel<DT, true>, dim3(a.max_ctas), dim3(kObsThreads), (size_t)kObsSmem, s, map_k, a));
-    RI_CUDA_OK(ri_launch_pdl_id(11, observe_merge_kernel, dim3(kRows / 32, a.batch * a.hk), dim3(256), 0, s, a));
+    if (a.lse2 != nullptr) RI_CUDA_OK(ri_launch_pdl_id(11, observe_merge_kernel, dim3(kRows / 32, a.batch * a.hk), dim3(256), 0, s, a));
     a.idesc = idesc_f16(DT, 128, (a.rows + 31) / 32 * 32);      // the scores are read 32 columns at a time
     RI_CUDA_OK(ri_launch_pdl_id(11, observe_kernel<DT, false>, dim3(a.max_ctas), dim3(kObsThreads), (size_t)kObsSmem, s, map_k, a));
   }
@@ -475,7 +516,11 @@ extern "C" int ri_paged_observe(const ri_paged* p, const void* d_q, int32_t wind
   static_cast<Pages&>(a) = view(*p);
   a.q = static_cast<const uint4*>(d_q);
   a.part = static_cast<float2*>(d_scratch);
-  a.lse2 = reinterpret_cast<float*>(a.part + obs_slots(*p) * kPartials);
+  // A group that few CTAs share: pass 2 merges its partial results by itself; else a kernel between the passes does, once for all.
+  // 1001 slots, 8 heads, 8 CTAs a group: 11.5 us merged inside, 13.2 by a kernel; 4000 slots of one head, 32 CTAs: 17.1 and 16.2.
+  const int64_t groups = (int64_t)p->batch * p->kv_heads, tiles = ((int64_t)p->table_stride * p->page_size + kTile - 1) / kTile;
+  const int64_t most = kObsMaxCtas / groups + 2;
+  if ((most < tiles ? most : tiles) > kMergedInside) a.lse2 = reinterpret_cast<float*>(a.part + obs_slots(*p) * kPartials);
   a.window = window;
   a.gs = p->group_size;
   a.scale2 = RI_LOG2E * scale;
