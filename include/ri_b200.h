@@ -330,7 +330,8 @@ int ri_weighted_flash_decoding(const void* d_q, const void* d_k, const void* d_v
  * key_page_stride and value_page_stride elements apart; beside them, dense [n_pages][kv_heads][page_size], the weight that
  * every slot's key was given so far and the number of its token in its request.  Slot j of request b is row j % page_size of
  * page d_table[b][j / page_size] for every KV head; the first d_lengths[b] slots are in use (negative: none; more than the
- * table reaches: as many as it does).  Table entries behind them are not read.  An entry that names no page becomes
+ * table reaches: as many as it does).  Table entries behind them are not read.  Requests may share pages that nothing is written
+ * to: not where weights grow, and not where rows are appended or evicted.  An entry that names no page becomes
  * RI_STATUS_PAGE_ID in *d_status: nothing outside the pools is touched, and that request's results mean nothing. */
 typedef struct ri_paged {
   int32_t batch, kv_heads;

@@ -102,6 +102,7 @@ ri_paged describe(const char* what, const Tensor& key_pages, const OptTensor& va
   if (!dense(lengths, {batch}, at::kInt, device)) fail(what, "expected dense int32 lengths [batch] on the pools' GPU");
   if (given(weight) && !dense(*weight, {pages, heads, page}, at::kFloat, device))
     fail(what, "expected dense fp32 weight [pages, kv_heads, page_size] on the pools' GPU");
+  if (given(weight) && weight->requires_grad()) fail(what, "there are no gradients");
   if (given(token) && !dense(*token, {pages, heads, page}, at::kInt, device))
     fail(what, "expected dense int32 token [pages, kv_heads, page_size] on the pools' GPU");
   for (int64_t n : {batch, heads, group, page, pages, width})
@@ -185,8 +186,10 @@ Tensor decode(const Tensor& q, const Tensor& key_pages, const OptTensor& value_p
   if (q.scalar_type() != key_pages.scalar_type() || q.device() != key_pages.device() || q.requires_grad())
     fail(what, "expected q and the pages of one type on one GPU, without gradients");
   const ri_paged p = describe(what, key_pages, value_pages, page_table, lengths, weight, std::nullopt, q_heads / heads, status);
-  if (given(given_out) && !dense(*given_out, q.sizes(), q.scalar_type(), q.device())) fail(what, "expected dense out like q");
-  if (given(lse) && !dense(*lse, {batch, q_heads}, at::kFloat, q.device())) fail(what, "expected dense fp32 lse [batch, q_heads]");
+  if (given(given_out) && (!dense(*given_out, q.sizes(), q.scalar_type(), q.device()) || given_out->requires_grad()))
+    fail(what, "expected dense out like q");
+  if (given(lse) && (!dense(*lse, {batch, q_heads}, at::kFloat, q.device()) || lse->requires_grad()))
+    fail(what, "expected dense fp32 lse [batch, q_heads]");
   const OnDevice on(key_pages);
   const Tensor out = given(given_out) ? *given_out : at::empty(q.sizes(), q.options());
   const Tensor scratch = workspace(lib.decode_bytes(&p), q, what);

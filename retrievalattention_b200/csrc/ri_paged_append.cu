@@ -4,10 +4,11 @@
 // One axis is the ordinary rotary embedding; text, images and video take (time, height, width).
 // (reference: model_hub/llama.py:232-235 the split, :312-320 the rotation; cache_hub/flash_attn_cache.py:133-151 the append)
 //
-// Bound by the projection, read once and written once.  A row of it lies in one piece and comes in by one bulk copy, three
-// rows on their way to each of three CTAs of an SM, which take neighbouring rows.  Two warps issue the copies and fetch what the rows need beside them: 128
-// cosines and sines, each by its own axis, which serve all heads from shared memory, and the row's place in the cache (request,
-// slot, page: three loads that depend on one another).  Eight warps rotate, a half-warp per head and 16 bytes per lane.
+// Bound by the projection, read once and written once.  A row of it lies in one piece and comes in by one bulk copy, three rows
+// on their way to each of three CTAs of an SM, which take neighbouring rows.  Two warps issue the copies and fetch what the rows
+// need beside them: 128 cosines and sines, each by its own axis, which serve all heads from shared memory, and the row's place
+// in the cache (request, slot, page: three loads that depend on one another).  Eight warps rotate, a half-warp per head and 16
+// bytes per lane.
 // Every wait is bounded; one that runs out is recorded in the status word.
 // 32768 rows of 32 + 8 heads, bf16: 149 us, 5.5 TB/s (a copy: 6.6).  A CTA per row, plain loads: 200; the next row's loads in
 // registers: 170; bulk copies, four CTAs of four rows each with the CTAs' rows interleaved: 157, with neighbouring rows 154;

@@ -16,7 +16,7 @@
 // TMEM: 256 columns of scores for each side.  Every wait is bounded; one that runs out is recorded in the
 // status word.
 // Bound by the exponentials, two for each slot and query row.  B200, 4 requests of 20K to 32K slots, 8 heads, 256 query rows: 171 us
-// in a repeated run, 1.26 Tera-exponentials a second each way against 2.1 that the SMs have at 16 a clock; pass 1 takes 71 us
+// in a repeated run, 2.5 of the 4.2 exponentials a picosecond that the SMs have at 16 a clock and 1.76 GHz; pass 1 takes 71 us
 // from rest (exponentials busy 79 % of the active cycles, tensor pipe 39 %), pass 2 82 (69 %: it also reads each row's lse).  With
 // eight score warps 188 us: two warps of a scheduler do not cover each other's loads and barriers.  Some of the exponentials as
 // polynomials on the FMA pipe gained nothing with either.

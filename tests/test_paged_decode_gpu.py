@@ -193,6 +193,7 @@ def test_refusals():
                    dict(page_table=layer.table.long()), dict(page_table=layer.table.t()), dict(page_table=layer.table.cpu()),
                    dict(lengths=ints), dict(lengths=layer.lengths[:1]), dict(lengths=layer.lengths.cpu()),
                    dict(weight=layer.weight.double()), dict(weight=layer.weight[:-1]), dict(weight=layer.weight.transpose(1, 2)),
+                   dict(weight=layer.weight.clone().requires_grad_()),
                    dict(lse=torch.empty((2, 7), device="cuda")), dict(lse=torch.empty((2, 8))),
                    dict(out=torch.empty((2, 1, 8, DIM), device="cuda"))):
         with pytest.raises(ValueError):
