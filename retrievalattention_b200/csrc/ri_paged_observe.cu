@@ -196,18 +196,28 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
   // this CTA's tiles [lo, hi) of the sequence, segment by segment (the part of a group that falls to it)
   const int total = ri_seq::count_steps(a), n_ctas = min(a.max_ctas, total), c = (int)blockIdx.x;
   const int lo = c < n_ctas ? ri_seq::cta_start(c, total, n_ctas) : 0, hi = c < n_ctas ? ri_seq::cta_start(c + 1, total, n_ctas) : 0;
+  // Pass 2 walks its range backwards: what pass 1 read last is still in L2.
+  auto tile_at = [&](int i) { return STATS ? lo + i : hi - 1 - i; };
+  auto walk_to = [&](Place& at, int t) {
+    if (STATS) {
+      while (t >= at.first + ri_seq::steps_of<kTile>(at.rows)) ri_seq::next_place(a, at);
+    } else {
+      while (t < at.first) ri_seq::previous_place(a, at);
+    }
+  };
   // both sides of the score warps work on the same keys where there are query rows for both, on every second tile otherwise
   const bool both = STATS && a.rows > kTile;
 
   if (lo < hi) {
     if (warp == 0) {
       // ---------------- K tiles, a box of at most a page per lane ----------------
-      Place at = ri_seq::find_place(a, lo);
+      Place at = ri_seq::find_place(a, tile_at(0));
       const int box = min(1 << a.shift, kTile), mask = (1 << a.shift) - 1;
       bool ok = true;
       int issued = 0;
-      for (int t = lo; t < hi; ++t, ++issued) {
-        while (t >= at.first + ri_seq::steps_of<kTile>(at.rows)) ri_seq::next_place(a, at);
+      for (; issued < hi - lo; ++issued) {
+        const int t = tile_at(issued);
+        walk_to(at, t);
         const int b = at.g / a.hk, h = at.g - b * a.hk, slot0 = (t - at.first) * kTile;
         const int boxes = (min(kTile, at.rows - slot0) + box - 1) / box, s = issued % kRing;
         const int id = lane < boxes ? page_of(a, b, (slot0 + lane * box) >> a.shift) : 0;
@@ -226,14 +236,14 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
         for (int t = max(0, issued - kRing); t < issued; ++t) mbar_wait(bar_full(t % kRing), (t / kRing) & 1, abort_flag, 82);
     } else if (warp == 1) {
       // ---------------- products ----------------
-      Place at = ri_seq::find_place(a, lo);
+      Place at = ri_seq::find_place(a, tile_at(0));
       if (lane == 0) {
         bool ok = true;
         int used = 0, groups = 0, made[2] = {0, 0};
-        for (int t = lo; ok && t < hi; ++t, ++used) {
-          bool fresh = t == lo;
-          while (t >= at.first + ri_seq::steps_of<kTile>(at.rows)) { ri_seq::next_place(a, at); fresh = true; }
-          if (fresh) ok = mbar_wait(bar_q, groups++ & 1, abort_flag, 83);
+        for (; ok && used < hi - lo; ++used) {
+          const int g_before = at.g;
+          walk_to(at, tile_at(used));
+          if (used == 0 || at.g != g_before) ok = mbar_wait(bar_q, groups++ & 1, abort_flag, 83);
           const int s = used % kRing;
           ok = ok && mbar_wait(bar_full(s), (used / kRing) & 1, abort_flag, 84);
 #pragma unroll
@@ -262,12 +272,14 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
       const int side = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, quarter = warp & 3, row = quarter * 32 + lane;
       const int tid = threadIdx.x - 128, g = side;
       const uint32_t t_lane = (uint32_t)(quarter * 32) << 16;
-      Place at = ri_seq::find_place(a, lo);
+      Place at = ri_seq::find_place(a, tile_at(0));
       bool ok = true;
       int done = 0, used = 0;                          // tiles of this side, of the CTA
-      for (int t = lo; t < hi;) {
-        while (t >= at.first + ri_seq::steps_of<kTile>(at.rows)) ri_seq::next_place(a, at);
-        const int end = min(hi, at.first + ri_seq::steps_of<kTile>(at.rows)), n = at.rows;
+      while (used < hi - lo) {
+        walk_to(at, tile_at(used));
+        const int g_first = at.first, g_end = at.first + ri_seq::steps_of<kTile>(at.rows), n = at.rows;
+        // of the group's tiles, those in this CTA's range: up to place `end` of its walk
+        const int end = STATS ? min(hi, g_end) - lo : hi - max(lo, g_first);
         const int b = at.g / a.hk, h = at.g - b * a.hk;
         // the group's query rows, their pieces swizzled as TMA would; every product over the rows before has completed, since
         // its scores have been read
@@ -315,7 +327,8 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
           const int r = both ? g * kTile + row : row;
           const int last = r < a.rows ? last_seen(a, n, a.first_row + r) : n - 1;      // rows that fill up a tile hold nobody up
           float m = -INFINITY, l = 0.f;
-          for (; t < end; ++t, ++used) {
+          for (; used < end; ++used) {
+            const int t = tile_at(used);
             if (!both && g != (used & 1)) continue;
             const int i = done % kBuffers;
             ok = ok && __all_sync(0xffffffffu, mbar_wait(bar_s_full(g, i), (done / kBuffers) & 1, abort_flag, 86));
@@ -371,7 +384,8 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
           }
           a.part[(int64_t)(c + at.g) * kPartials + half * kRows + side * kTile + row] = make_float2(m, l);
         } else {
-          for (; t < end; ++t, ++used) {
+          for (; used < end; ++used) {
+            const int t = tile_at(used);
             if (g != (used & 1)) continue;
             const int slot0 = (t - at.first) * kTile, slot = slot0 + row;
             float* weight = nullptr;

@@ -67,4 +67,16 @@ __device__ __forceinline__ void next_place(const Args& a, Place& p) {
   }
 }
 
+// The group with rows in front of it (there is one).
+template <class Args>
+__device__ __forceinline__ void previous_place(const Args& a, Place& p) {
+  if (p.g % a.hk == 0) {
+    int b = p.g / a.hk - 1;
+    while ((p.rows = rows_of(a, b)) == 0 && b > 0) --b;
+    p.g = (b + 1) * a.hk;
+  }
+  --p.g;
+  p.first -= steps_of<Args::kStep>(p.rows);
+}
+
 }  // namespace ri_seq
