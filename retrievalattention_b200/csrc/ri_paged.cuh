@@ -24,20 +24,23 @@ struct Pages {
 __device__ __forceinline__ int rows_of(const Pages& p, int b) {
   return (int)min((int64_t)max(p.lengths[b], 0), (int64_t)p.table_stride << p.shift);
 }
-// Page i of request b, for readers.  A number that names no page is reported, and page 0 stands in for it: nothing outside the
-// pool is touched, and the call's results for that request mean nothing.
-__device__ __forceinline__ int page_of(const Pages& p, int b, int i) {
-  const int id = p.table[(int64_t)b * p.table_stride + i];
+// A page number out of a table, for readers.  One that names no page is reported, and page 0 stands in for it: nothing outside
+// the pool is touched, and the call's results for that request mean nothing.
+__device__ __forceinline__ int page_or_first(const Pages& p, int id) {
   if ((unsigned)id < (unsigned)p.n_pages) return id;
   *p.status = RI_STATUS_PAGE_ID;
   return 0;
 }
 // The same for writers: -1 where there is no such page, and nothing is written.
-__device__ __forceinline__ int page_to_write(const Pages& p, int b, int i) {
-  const int id = p.table[(int64_t)b * p.table_stride + i];
+__device__ __forceinline__ int page_or_none(const Pages& p, int id) {
   if ((unsigned)id < (unsigned)p.n_pages) return id;
   *p.status = RI_STATUS_PAGE_ID;
   return -1;
+}
+// Page i of request b.
+__device__ __forceinline__ int page_of(const Pages& p, int b, int i) { return page_or_first(p, p.table[(int64_t)b * p.table_stride + i]); }
+__device__ __forceinline__ int page_to_write(const Pages& p, int b, int i) {
+  return page_or_none(p, p.table[(int64_t)b * p.table_stride + i]);
 }
 // Row `row` of head h in page `id`: its place in the tensors of weights and token numbers.
 __device__ __forceinline__ int64_t record_at(const Pages& p, int id, int h, int row) {

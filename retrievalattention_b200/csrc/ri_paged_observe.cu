@@ -215,21 +215,32 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
       const int box = min(1 << a.shift, kTile), mask = (1 << a.shift) - 1;
       bool ok = true;
       int issued = 0;
-      for (; issued < hi - lo; ++issued) {
-        const int t = tile_at(issued);
+      // a tile's boxes, and the page of this lane's; the next tile's page numbers are on their way while a tile's copies are issued
+      struct Tile {
+        int boxes, id, y;
+      };
+      auto plan = [&](int i) {
+        const int t = tile_at(i);
         walk_to(at, t);
         const int b = at.g / a.hk, h = at.g - b * a.hk, slot0 = (t - at.first) * kTile;
-        const int boxes = (min(kTile, at.rows - slot0) + box - 1) / box, s = issued % kRing;
-        const int id = lane < boxes ? page_of(a, b, (slot0 + lane * box) >> a.shift) : 0;
+        Tile tile = {(min(kTile, at.rows - slot0) + box - 1) / box, 0, (h << a.shift) + ((slot0 + lane * box) & mask)};
+        if (lane < tile.boxes) tile.id = a.table[(int64_t)b * a.table_stride + ((slot0 + lane * box) >> a.shift)];
+        return tile;
+      };
+      Tile next = plan(0);
+      for (; issued < hi - lo; ++issued) {
+        const Tile tile = next;
+        if (issued + 1 < hi - lo) next = plan(issued + 1);
+        const int s = issued % kRing;
         ok = __all_sync(0xffffffffu, mbar_wait(bar_empty(s), ((issued / kRing) & 1) ^ 1, abort_flag, 81));
         if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(bar_full(s), boxes * box * 256);
+        if (lane == 0) mbar_arrive_expect_tx(bar_full(s), tile.boxes * box * 256);
         __syncwarp();
-        if (lane < boxes) {
-          const int y = (h << a.shift) + ((slot0 + lane * box) & mask);
+        if (lane < tile.boxes) {
+          const int id = page_or_first(a, tile.id);
           const uint32_t dst = sK + s * kKeyTile + lane * box * 128;
-          tma_load_3d(dst, &map_k, bar_full(s), 0, y, id);
-          tma_load_3d(dst + kKeyHalf, &map_k, bar_full(s), 64, y, id);
+          tma_load_3d(dst, &map_k, bar_full(s), 0, tile.y, id);
+          tma_load_3d(dst + kKeyHalf, &map_k, bar_full(s), 64, tile.y, id);
         }
       }
       if (*abort_flag)         // give the copies still in flight a bounded chance to land before the CTA exits
@@ -384,13 +395,19 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
           }
           a.part[(int64_t)(c + at.g) * kPartials + half * kRows + side * kTile + row] = make_float2(m, l);
         } else {
-          for (; used < end; ++used) {
-            const int t = tile_at(used);
-            if (g != (used & 1)) continue;
-            const int slot0 = (t - at.first) * kTile, slot = slot0 + row;
+          // this thread's slot in the tile at place i of the walk, and the number of its page as the table has it
+          auto slot_at = [&](int i) { return (tile_at(i) - at.first) * kTile + row; };
+          auto page_at = [&](int i) {
+            return i < end && !half && slot_at(i) < n ? a.table[(int64_t)b * a.table_stride + (slot_at(i) >> a.shift)] : 0;
+          };
+          if (g != (used & 1)) ++used;
+          int next_page = page_at(used);
+          for (; used < end; used += 2) {
+            const int slot = slot_at(used), slot0 = slot - row;
             float* weight = nullptr;
             float old = 0.f;
-            const int id = !half && slot < n ? page_to_write(a, b, slot >> a.shift) : -1;
+            const int id = !half && slot < n ? page_or_none(a, next_page) : -1;
+            next_page = page_at(used + 2);
             if (id >= 0) {
               weight = a.weight + record_at(a, id, h, slot & ((1 << a.shift) - 1));
               old = *weight;
@@ -427,6 +444,7 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
             asm volatile("bar.sync %0, 64;" ::"r"(meeting) : "memory");
             if (!half && weight != nullptr) *weight = old + (sum + s_sum[side][place][row]);
           }
+          used = end;
         }
       }
     }
