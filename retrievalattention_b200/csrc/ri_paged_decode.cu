@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_ke
     }
   }
   // a tile of slots: pages (their tables do not change either), then scores and weights
-  int id[kFoldEach];
+  int id[kFoldEach] = {};
   float sc[kFoldEach][kMaxHeads], old[kFoldEach];
   auto slot_of = [&](int tile, int e) { return slot_in_step(tile * kFoldSlots + e * kFinishThreads + tid); };
   auto weight_at = [&](int tile, int e) { return a.weight + record_at(a, id[e], h_kv, slot_of(tile, e) & ((1 << a.shift) - 1)); };
@@ -563,17 +563,46 @@ int make_page_map(CUtensorMap* map, const void* base, const ri_paged& p, int64_t
   return RI_OK;
 }
 
+// How many clusters of `ctas` CTAs the device holds at once: they lie inside one GPC, so that is not SMs / ctas.
+int clusters_at_once(int ctas, int* out) {
+  static std::atomic<int> known[64][kMaxCluster + 1];
+  int dev = 0, rc;
+  RI_CUDA_OK(cudaGetDevice(&dev));
+  const bool track = dev >= 0 && dev < 64;
+  if (track && (*out = known[dev][ctas].load(std::memory_order_relaxed)) > 0) return RI_OK;
+  auto* kernel = paged_decode_kernel<RI_BF16, 16, true, true>;      // all of them have the same shared memory and threads
+  if ((rc = ri_allow_smem<paged_decode_kernel<RI_BF16, 16, true, true>>(kPagedSmem)) != RI_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kPagedThreads);
+  cfg.dynamicSmemBytes = kPagedSmem;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ctas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  RI_CUDA_OK(cudaOccupancyMaxActiveClusters(out, kernel, &cfg));
+  if (track) known[dev][ctas].store(*out, std::memory_order_relaxed);
+  return RI_OK;
+}
 // CTAs of a cluster where every group can have a cluster at once and the longest request that fits the tables is short; 0: no
-// clusters.  Clusters lie inside one GPC, so not every SM can be in one.  A second kernel costs 2 us of host and device time; an even
-// split over all SMs gains more than that from five steps a warp on (8 heads of 4, a call: 777 slots 11.3 us with two kernels,
-// 9.6 with clusters; 4000 slots, four steps a warp, 11.6 and 9.7; 8000 slots 13.9 and 14.9).
+// clusters.  A second kernel costs 2 us of host and device time; an even split over all SMs gains more than that from five steps a
+// warp on (8 heads of 4, a call: 777 slots 11.3 us with two kernels, 9.6 with clusters; 4000 slots, four steps a warp, 11.6 and
+// 9.7; 8000 slots 13.9 and 14.9).
 constexpr int kClusterSteps = 4;                       // of a warp, at most
-int cluster_size(const PagedArgs& a) {
+int cluster_size(const PagedArgs& a, int* ctas) {
   const int64_t groups = (int64_t)a.batch * a.hk, steps = (((int64_t)a.table_stride << a.shift) + 15) / 16;
-  int ctas = 0;
-  for (int n = 1; n <= kMaxCluster; n *= 2)
-    if (groups * n <= a.max_ctas * 4 / 5 && (ctas == 0 || steps > (int64_t)ctas * kPagedWarps)) ctas = n;
-  return ctas > 0 && steps <= (int64_t)ctas * kPagedWarps * kClusterSteps ? ctas : 0;
+  *ctas = 0;
+  if (groups > a.max_ctas || steps > kMaxCluster * kPagedWarps * kClusterSteps) return RI_OK;
+  for (int n = 1; n <= kMaxCluster; n *= 2) {
+    int fit = 0;
+    const int rc = clusters_at_once(n, &fit);
+    if (rc != RI_OK) return rc;
+    if (groups <= fit && (*ctas == 0 || steps > (int64_t)*ctas * kPagedWarps)) *ctas = n;
+  }
+  if (steps > (int64_t)*ctas * kPagedWarps * kClusterSteps) *ctas = 0;
+  return RI_OK;
 }
 template <int DT, int BOX, bool WEIGHTS>
 int launch_steps(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, int ctas, cudaStream_t s) {
@@ -595,7 +624,9 @@ int launch_steps(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap
 }
 template <int DT>
 int launch_paged(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, int box, cudaStream_t s) {
-  const int ctas = cluster_size(a), rc = box == 8 ? launch_steps<DT, 8>(a, map_k, map_v, ctas, s) : launch_steps<DT, 16>(a, map_k, map_v, ctas, s);
+  int ctas, rc;
+  if ((rc = cluster_size(a, &ctas)) != RI_OK) return rc;
+  rc = box == 8 ? launch_steps<DT, 8>(a, map_k, map_v, ctas, s) : launch_steps<DT, 16>(a, map_k, map_v, ctas, s);
   if (rc != RI_OK || ctas > 0) return rc;
   const int64_t groups = (int64_t)a.batch * a.hk, most = (int64_t)a.table_stride << a.shift;
   // blocks of a group: for its heads, or with weights its tiles of slots, as many as the chip holds at once

@@ -23,8 +23,8 @@ namespace {
 using namespace ri_page;
 namespace cg = cooperative_groups;
 
-constexpr int kSelThreads = 512;
-constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kFewThreads = 256, kManyThreads = 512;  // of a CTA of the selection
+constexpr int kFewPerSm = 3;                         // CTAs of few threads on an SM
 constexpr int kCachedKeys = 40 * 1024;               // keys of a CTA's slice that shared memory holds
 constexpr int kSelMaxCluster = 8;
 constexpr int kSlotsWorthACta = 512;
@@ -51,7 +51,7 @@ __device__ __forceinline__ uint32_t order_key(float w) {
 }
 
 // Exclusive scan over the block, and its total.
-template <typename T>
+template <int WARPS, typename T>
 __device__ __forceinline__ T block_scan(T v, T* warp_sums, T& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   T incl = v;
@@ -66,7 +66,7 @@ __device__ __forceinline__ T block_scan(T v, T* warp_sums, T& total) {
   T before = 0;
   total = 0;
 #pragma unroll
-  for (int w = 0; w < kSelWarps; ++w) {
+  for (int w = 0; w < WARPS; ++w) {
     const T s = warp_sums[w];
     if (w < warp) before += s;
     total += s;
@@ -112,19 +112,20 @@ constexpr int kLevels = 3, kDigits = 2048;             // 11, 11 and 10 bits of 
 struct SelShared {
   int hist[kLevels][kDigits];  // per level: this CTA's slots by digit
   unsigned long long totals;   // holes and fillers of this CTA, 32 bits each
-  unsigned long long warp_sums[kSelWarps];
-  int warp_counts[kSelWarps];
+  unsigned long long warp_sums[kManyThreads / 32];
+  int warp_counts[kManyThreads / 32];
   int digit, before;           // the cut's digit, and slots of larger digits
 };
 
-// MOVES: the cluster moves the rows itself.
-template <bool MOVES>
-__global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const __grid_constant__ EvictArgs a) {
+// MOVES: the cluster moves the rows itself.  CTAs of few threads are clusters by themselves.
+template <int THREADS, bool MOVES>
+__global__ void __launch_bounds__(THREADS, THREADS == kFewThreads ? kFewPerSm : 1) evict_select_kernel(const __grid_constant__ EvictArgs a) {
   extern __shared__ __align__(16) uint32_t s_keys[];
   __shared__ __align__(16) SelShared sh;
   ri_pdl_enter();
+  constexpr int kMaxCtas = THREADS == kFewThreads ? 1 : kSelMaxCluster;
   cg::cluster_group cluster = cg::this_cluster();
-  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
+  const int rank = kMaxCtas > 1 ? (int)cluster.block_rank() : 0, ctas = kMaxCtas > 1 ? (int)cluster.num_blocks() : 1;
   const int tid = threadIdx.x, g = blockIdx.x / ctas;
   const Pages& p = a.pages;
   const int b = g / p.hk, h = g - b * p.hk, n = rows_of(p, b);
@@ -140,15 +141,15 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const __gr
   };
   auto record_of = [&](int j) { return record_at(p, page_of(p, b, j >> p.shift), h, j & ((1 << p.shift) - 1)); };
   auto key_from = [&](float w, int t) { return (t < a.sink || t >= newest) ? kProtected : order_key(w); };
-  for (int i = tid; i < kLevels * kDigits / 4; i += kSelThreads) reinterpret_cast<int4*>(&sh.hist[0][0])[i] = make_int4(0, 0, 0, 0);
+  for (int i = tid; i < kLevels * kDigits / 4; i += THREADS) reinterpret_cast<int4*>(&sh.hist[0][0])[i] = make_int4(0, 0, 0, 0);
   // four slots of a page at a time, and four such pieces of a thread on their way together; the slice begins where a piece does
   const int cached = min(mine, kCachedKeys);
-  for (int j0 = 4 * tid; j0 < cached; j0 += 16 * kSelThreads) {
+  for (int j0 = 4 * tid; j0 < cached; j0 += 16 * THREADS) {
     int64_t at[4];
     float4 w[4];
     int4 t[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) at[u] = j0 + 4 * u * kSelThreads < cached ? record_of(lo + j0 + 4 * u * kSelThreads) : -1;
+    for (int u = 0; u < 4; ++u) at[u] = j0 + 4 * u * THREADS < cached ? record_of(lo + j0 + 4 * u * THREADS) : -1;
 #pragma unroll
     for (int u = 0; u < 4; ++u)
       if (at[u] >= 0) {
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const __gr
 #pragma unroll
     for (int u = 0; u < 4; ++u)
       if (at[u] >= 0)                                  // up to three slots behind the last one: there is room, and nobody reads them
-        *reinterpret_cast<uint4*>(s_keys + j0 + 4 * u * kSelThreads) =
+        *reinterpret_cast<uint4*>(s_keys + j0 + 4 * u * THREADS) =
             make_uint4(key_from(w[u].x, t[u].x), key_from(w[u].y, t[u].y), key_from(w[u].z, t[u].z), key_from(w[u].w, t[u].w));
   }
   __syncthreads();
@@ -175,32 +176,37 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const __gr
   for (int level = 0; level < kLevels; ++level) {
     const int shift = level == 0 ? 21 : level == 1 ? 10 : 0;
     const uint32_t mask = level == 2 ? 1023u : 2047u;
-    for (int j = tid; j < mine; j += kSelThreads) {
+    for (int j = tid; j < mine; j += THREADS) {
       const uint32_t k = key_of(j);
       if (level == 0 || (k >> (level == 1 ? 21 : 10)) == (prefix >> (level == 1 ? 21 : 10))) atomicAdd(&sh.hist[level][(k >> shift) & mask], 1);
     }
     meet();
-    int4 sum = make_int4(0, 0, 0, 0);                  // of four digits, the largest ones at thread 0
-    const int digit = kDigits - 4 - 4 * tid;
-    int4 of[kSelMaxCluster];
+    // each thread adds up kEach neighbouring digits over the cluster, the largest ones at thread 0
+    constexpr int kEach = kDigits / THREADS;
+    const int digit = kDigits - kEach - kEach * tid;
+    int each[kEach], mine_all = 0;
 #pragma unroll
-    for (int c = 0; c < kSelMaxCluster; ++c)
-      of[c] = c < ctas ? *reinterpret_cast<const int4*>(cluster.map_shared_rank(&sh.hist[level][0], c) + digit) : make_int4(0, 0, 0, 0);
+    for (int q = 0; q < kEach; q += 4) {
+      int4 of[kMaxCtas], sum = make_int4(0, 0, 0, 0);
 #pragma unroll
-    for (int c = 0; c < kSelMaxCluster; ++c) { sum.x += of[c].x; sum.y += of[c].y; sum.z += of[c].z; sum.w += of[c].w; }
-    const int four = sum.x + sum.y + sum.z + sum.w;
+      for (int c = 0; c < kMaxCtas; ++c)
+        of[c] = c < ctas ? *reinterpret_cast<const int4*>(cluster.map_shared_rank(&sh.hist[level][0], c) + digit + q) : make_int4(0, 0, 0, 0);
+#pragma unroll
+      for (int c = 0; c < kMaxCtas; ++c) { sum.x += of[c].x; sum.y += of[c].y; sum.z += of[c].z; sum.w += of[c].w; }
+      each[q] = sum.x; each[q + 1] = sum.y; each[q + 2] = sum.z; each[q + 3] = sum.w;
+      mine_all += sum.x + sum.y + sum.z + sum.w;
+    }
     int total;
-    int before = block_scan(four, sh.warp_counts, total);
-    if (before < need && before + four >= need) {
-      int d = digit + 3;
-      const int each[4] = {sum.w, sum.z, sum.y, sum.x};
+    int before = block_scan<THREADS / 32>(mine_all, sh.warp_counts, total);
+    if (before < need && before + mine_all >= need) {
+      int d = kEach - 1;
 #pragma unroll
-      for (int i = 0; i < 3; ++i)
-        if (d == digit + 3 - i && before + each[i] < need) {
+      for (int i = kEach - 1; i > 0; --i)
+        if (d == i && before + each[i] < need) {
           before += each[i];
           --d;
         }
-      sh.digit = d;
+      sh.digit = digit + d;
       sh.before = before;
     }
     __syncthreads();
@@ -209,13 +215,13 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const __gr
   }
   for (int c = 0; c < ctas; ++c) ties += cluster.map_shared_rank(&sh.hist[kLevels - 1][0], c)[prefix & 1023u];
   // the first `need` slots of the group with the cut's key stay; mostly that is all of them
-  const int run = ((mine + kSelThreads - 1) / kSelThreads) | 1, first = min(mine, tid * run), last = min(mine, first + run);
+  const int run = ((mine + THREADS - 1) / THREADS) | 1, first = min(mine, tid * run), last = min(mine, first + run);
   int rank_eq = 0;
   if (ties > need) {
     int equal = 0, total;
     for (int c = 0; c < rank; ++c) rank_eq += cluster.map_shared_rank(&sh.hist[kLevels - 1][0], c)[prefix & 1023u];
     for (int j = first; j < last; ++j) equal += key_of(j) == prefix;
-    rank_eq += block_scan(equal, sh.warp_counts, total);
+    rank_eq += block_scan<THREADS / 32>(equal, sh.warp_counts, total);
   } else {
     need = ties;
   }
@@ -227,7 +233,7 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const __gr
     holes += front && !stays;
     fillers += !front && stays;
   }
-  unsigned long long total, at = block_scan((unsigned long long)fillers << 32 | holes, sh.warp_sums, total);
+  unsigned long long total, at = block_scan<THREADS / 32>((unsigned long long)fillers << 32 | holes, sh.warp_sums, total);
   if (tid == 0) sh.totals = total;
   meet();
   unsigned long long all = 0;
@@ -248,7 +254,7 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const __gr
     }
   if (rank == 0 && tid == 0) a.counts[g] = (int)(unsigned)all;
   meet();                                      // the list is there; nobody's shared memory goes while others may read it
-  if (MOVES) move_rows(a, moves, b, h, rank * (kSelThreads / 16) + (tid >> 4), ctas * (kSelThreads / 16), (int)(unsigned)all);
+  if (MOVES) move_rows(a, moves, b, h, rank * (THREADS / 16) + (tid >> 4), ctas * (THREADS / 16), (int)(unsigned)all);
 }
 
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ EvictArgs a) {
@@ -295,16 +301,30 @@ extern "C" int ri_paged_evict(const ri_paged* p, const int32_t* d_seen, int32_t 
   a.most = (int)most_moves(*p, keep);
   int sms = 0;
   if ((rc = ri_sm_count(&sms)) != RI_OK) return rc;
-  int ctas = 1;                                        // as many CTAs to a group as fit the chip at once and have enough to do
-  while (ctas < kSelMaxCluster && groups * ctas * 2 <= sms && room > (int64_t)ctas * kSlotsWorthACta) ctas *= 2;
-  const int64_t slice = ri_align_up((room + ctas - 1) / ctas, 4);
-  const size_t smem = (size_t)(slice < kCachedKeys ? slice : kCachedKeys) * 4;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool moves = a.most <= (int64_t)ctas * kMovesInside;
-  if ((rc = moves ? ri_allow_smem<evict_select_kernel<true>>(kCachedKeys * 4) : ri_allow_smem<evict_select_kernel<false>>(kCachedKeys * 4)) != RI_OK)
-    return rc;
-  RI_CUDA_OK(ri_launch_pdl_cluster(11, ctas, moves ? evict_select_kernel<true> : evict_select_kernel<false>, dim3((unsigned)(groups * ctas)),
-                                   dim3(kSelThreads), smem, s, a));
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t key_bytes = ri_align_up(room, 4) * 4;
+  bool moves;
+  if (groups > sms && (key_bytes + (int64_t)sizeof(SelShared) + 1024) * kFewPerSm <= 227 * 1024) {
+    // more groups than SMs, each small: three CTAs an SM take them side by side (304 groups, 969 -> 590
+    // slots: 46 us with one, 33 with three; 160 groups, 6000 -> 5900: 35 and 27)
+    moves = a.most <= kMovesInside;
+    const int most = 227 * 1024 / kFewPerSm - 1024 - (int)sizeof(SelShared);
+    auto kernel = moves ? evict_select_kernel<kFewThreads, true> : evict_select_kernel<kFewThreads, false>;
+    if ((rc = moves ? ri_allow_smem<evict_select_kernel<kFewThreads, true>>(most) : ri_allow_smem<evict_select_kernel<kFewThreads, false>>(most)) != RI_OK)
+      return rc;
+    RI_CUDA_OK(ri_launch_pdl_id(11, kernel, dim3((unsigned)groups), dim3(kFewThreads), (size_t)key_bytes, s, a));
+  } else {
+    int ctas = 1;                                      // as many CTAs to a group as fit the chip at once and have enough to do
+    while (ctas < kSelMaxCluster && groups * ctas * 2 <= sms && room > (int64_t)ctas * kSlotsWorthACta) ctas *= 2;
+    const int64_t slice = ri_align_up((room + ctas - 1) / ctas, 4);
+    const size_t smem = (size_t)(slice < kCachedKeys ? slice : kCachedKeys) * 4;
+    moves = a.most <= (int64_t)ctas * kMovesInside;
+    auto kernel = moves ? evict_select_kernel<kManyThreads, true> : evict_select_kernel<kManyThreads, false>;
+    if ((rc = moves ? ri_allow_smem<evict_select_kernel<kManyThreads, true>>(kCachedKeys * 4)
+                    : ri_allow_smem<evict_select_kernel<kManyThreads, false>>(kCachedKeys * 4)) != RI_OK)
+      return rc;
+    RI_CUDA_OK(ri_launch_pdl_cluster(11, ctas, kernel, dim3((unsigned)(groups * ctas)), dim3(kManyThreads), smem, s, a));
+  }
   if (moves) return RI_OK;
   const int64_t blocks = ((int64_t)a.most + kMovesPerBlock - 1) / kMovesPerBlock, wanted = (int64_t)sms * 16 / groups + 1;
   RI_CUDA_OK(ri_launch_pdl_id(11, evict_move_kernel, dim3((unsigned)(blocks < wanted ? blocks : wanted), (unsigned)groups),

@@ -49,6 +49,9 @@ def check(layer, q, out, lse=None, before=None, scale=DIM ** -0.5):
     ((9001, 1), 2, 8, 256, torch.bfloat16),
     ((37,) * 90, 8, 2, 16, torch.bfloat16),                    # more groups than warps
     ((129, 640, 1023), 8, 4, 1024, torch.bfloat16),            # the largest pages
+    ((980, 0, 31) * 5, 4, 7, 16, torch.float16),               # two CTAs to a group
+    ((100, 5) * 8, 8, 1, 8, torch.bfloat16),                   # one
+    ((2100,) * 3, 8, 2, 32, torch.bfloat16),                   # longer than a group's CTAs take: an even split over the chip
 ])
 def test_against_64_bits(lengths, kv_heads, group, page, dtype, weights):
     layer = Layer(lengths, kv_heads, page, dtype, seed=3)
