@@ -55,6 +55,7 @@ def run(layer, keep, sink, recent, seen=None):
     ((300,) * 20, 8, 64, torch.bfloat16, 100, 100, 0),                # one CTA a group; the first tokens fill it
     ((300,) * 3, 2, 256, torch.bfloat16, 100, 0, 100),                # the last ones do
     ((700,) * 19, 8, 16, torch.bfloat16, 300, 4, 16),                 # the same, and more moves than it does itself
+    ((20000, 3000), 2, 128, torch.bfloat16, 5000, 4, 64),             # slots left over after one digit and after two
     ((513, 12), 4, 1024, torch.bfloat16, 12, 5, 7),
     ((4160, 4160), 4, 32, torch.float16, 4096, 4, 64),
 ])
