@@ -33,6 +33,10 @@ struct Library {
   decltype(&ri_paged_observe) observe = nullptr;
   decltype(&ri_paged_evict_scratch_bytes) evict_bytes = nullptr;
   decltype(&ri_paged_evict) evict = nullptr;
+  int32_t* status = nullptr;               // the process's status word
+  py::object* first_use = nullptr;         // told of every GPU that a call runs on, once
+  py::object* report = nullptr;            // raises what the status word says
+  bool used[64] = {};
 } lib;
 
 [[noreturn]] void fail(const char* what, const std::string& message) { throw py::value_error(std::string(what) + ": " + message); }
@@ -82,7 +86,7 @@ int64_t page_stride(const char* what, const Tensor& pages, const char* name) {
 }
 
 ri_paged describe(const char* what, const Tensor& key_pages, const OptTensor& value_pages, const Tensor& page_table,
-                  const Tensor& lengths, const OptTensor& weight, const OptTensor& token, int64_t group, int64_t status) {
+                  const Tensor& lengths, const OptTensor& weight, const OptTensor& token, int64_t group) {
   if (key_pages.dim() != 4 || key_pages.size(3) != kDim || !key_pages.is_cuda())
     fail(what, "expected key_pages [pages, kv_heads, page_size, 128] on a GPU");
   const int64_t pages = key_pages.size(0), heads = key_pages.size(1), page = key_pages.size(2);
@@ -119,8 +123,18 @@ ri_paged describe(const char* what, const Tensor& key_pages, const OptTensor& va
   p.d_token = static_cast<int32_t*>(address(token));
   p.d_table = static_cast<const int32_t*>(page_table.data_ptr());
   p.d_lengths = static_cast<const int32_t*>(lengths.data_ptr());
-  p.d_status = reinterpret_cast<int32_t*>(status);
+  p.d_status = lib.status;
   return p;
+}
+
+// Behind a call's launches: what the status word says of it or of an earlier call.
+void done(const Tensor& x) {
+  const int device = x.device().index();
+  if (device >= 64 || !lib.used[device]) {
+    (*lib.first_use)(device);
+    if (device < 64) lib.used[device] = true;
+  }
+  if (*static_cast<volatile int32_t*>(lib.status)) (*lib.report)();
 }
 
 Tensor workspace(int64_t bytes, const Tensor& like, const char* what) {
@@ -131,7 +145,7 @@ Tensor workspace(int64_t bytes, const Tensor& like, const char* what) {
 void append(const Tensor& qkv, const Tensor& cos_sin, const Tensor& positions, const py::bytes& axis_of, const Tensor& q,
             const Tensor& key_pages, const OptTensor& value_pages, const Tensor& page_table, const Tensor& lengths,
             const OptTensor& row_start, const OptTensor& weight, const OptTensor& token, const OptTensor& seen, const OptTensor& keys,
-            const OptTensor& values, int64_t status) {
+            const OptTensor& values) {
   const char* what = "rope_paged_append";
   const int64_t heads = key_pages.dim() == 4 ? key_pages.size(1) : 0;
   if (qkv.dim() != 2 || q.dim() != 3 || heads < 1 || q.size(1) < heads || q.size(1) % heads)
@@ -159,7 +173,7 @@ void append(const Tensor& qkv, const Tensor& cos_sin, const Tensor& positions, c
   if (PyBytes_AsStringAndSize(axis_of.ptr(), &of, &n_of) != 0) throw py::error_already_set();
   if (n_of != kDim / 2) fail(what, "axis_of names an axis for each of the 64 frequencies");
   if (rows > INT_MAX || axes > INT_MAX) fail(what, "too large");
-  const ri_paged p = describe(what, key_pages, value_pages, page_table, lengths, weight, token, q_heads / heads, status);
+  const ri_paged p = describe(what, key_pages, value_pages, page_table, lengths, weight, token, q_heads / heads);
   if (given(row_start) && !dense(*row_start, {p.batch + 1}, at::kInt, device)) fail(what, "expected dense int32 row_start [batch + 1]");
   if (given(seen) && !dense(*seen, {p.batch}, at::kInt, device)) fail(what, "expected dense int32 seen [batch]");
   if (given(token) && !given(seen)) fail(what, "token numbers need `seen`");
@@ -172,10 +186,11 @@ void append(const Tensor& qkv, const Tensor& cos_sin, const Tensor& positions, c
   touched(q);
   touched(key_pages);
   for (const OptTensor* x : {&value_pages, &weight, &token, &keys, &values}) touched(*x);
+  done(key_pages);
 }
 
 Tensor decode(const Tensor& q, const Tensor& key_pages, const OptTensor& value_pages, const Tensor& page_table, const Tensor& lengths,
-              const OptTensor& given_out, const OptTensor& lse, const OptTensor& weight, double scale, int64_t status) {
+              const OptTensor& given_out, const OptTensor& lse, const OptTensor& weight, double scale) {
   const char* what = "paged_decode";
   if (q.dim() != 4 || key_pages.dim() != 4 || page_table.dim() != 2 || !given(value_pages))
     fail(what, "expected q [batch, 1, q_heads, 128] and pages [pages, kv_heads, page_size, 128]");
@@ -185,7 +200,7 @@ Tensor decode(const Tensor& q, const Tensor& key_pages, const OptTensor& value_p
   if (!dense_rows(q, 1)) fail(what, "the heads of a request must lie dense in q");
   if (q.scalar_type() != key_pages.scalar_type() || q.device() != key_pages.device() || q.requires_grad())
     fail(what, "expected q and the pages of one type on one GPU, without gradients");
-  const ri_paged p = describe(what, key_pages, value_pages, page_table, lengths, weight, std::nullopt, q_heads / heads, status);
+  const ri_paged p = describe(what, key_pages, value_pages, page_table, lengths, weight, std::nullopt, q_heads / heads);
   if (given(given_out) && (!dense(*given_out, q.sizes(), q.scalar_type(), q.device()) || given_out->requires_grad()))
     fail(what, "expected dense out like q");
   if (given(lse) && (!dense(*lse, {batch, q_heads}, at::kFloat, q.device()) || lse->requires_grad()))
@@ -198,11 +213,12 @@ Tensor decode(const Tensor& q, const Tensor& key_pages, const OptTensor& value_p
   touched(given_out);
   touched(lse);
   touched(weight);
+  done(key_pages);
   return out;
 }
 
 void observe(const Tensor& q, const Tensor& key_pages, const Tensor& page_table, const Tensor& lengths, const OptTensor& weight,
-             double scale, int64_t status) {
+             double scale) {
   const char* what = "paged_observe";
   if (q.dim() != 4 || key_pages.dim() != 4 || page_table.dim() != 2 || !given(weight))
     fail(what, "expected q [batch, window, q_heads, 128], pages [pages, kv_heads, page_size, 128] and weights");
@@ -213,19 +229,19 @@ void observe(const Tensor& q, const Tensor& key_pages, const Tensor& page_table,
   if (q.scalar_type() != key_pages.scalar_type() || q.device() != key_pages.device() || q.requires_grad())
     fail(what, "expected q and the pages of one type on one GPU, without gradients");
   if (window > INT_MAX) fail(what, "too large");
-  const ri_paged p = describe(what, key_pages, std::nullopt, page_table, lengths, weight, std::nullopt, q_heads / heads, status);
+  const ri_paged p = describe(what, key_pages, std::nullopt, page_table, lengths, weight, std::nullopt, q_heads / heads);
   const OnDevice on(key_pages);
   const Tensor scratch = workspace(lib.observe_bytes(&p), q, what);
   check(lib.observe(&p, q.data_ptr(), (int32_t)window, (float)scale, scratch.data_ptr(), on.stream()), what);
   touched(weight);
+  done(key_pages);
 }
 
 void evict(const Tensor& key_pages, const OptTensor& value_pages, const OptTensor& weight, const OptTensor& token,
-           const Tensor& page_table, const Tensor& lengths, const Tensor& seen, int64_t keep, int64_t n_sink, int64_t n_recent,
-           int64_t status) {
+           const Tensor& page_table, const Tensor& lengths, const Tensor& seen, int64_t keep, int64_t n_sink, int64_t n_recent) {
   const char* what = "paged_evict";
   if (!given(value_pages) || !given(weight) || !given(token)) fail(what, "keys, values, weights and token numbers move together: none may be missing");
-  const ri_paged p = describe(what, key_pages, value_pages, page_table, lengths, weight, token, 1, status);
+  const ri_paged p = describe(what, key_pages, value_pages, page_table, lengths, weight, token, 1);
   if (!dense(seen, {p.batch}, at::kInt, key_pages.device())) fail(what, "expected dense int32 seen [batch]");
   for (int64_t n : {keep, n_sink, n_recent})
     if (n > INT_MAX || n < INT_MIN) fail(what, "too large");
@@ -235,9 +251,10 @@ void evict(const Tensor& key_pages, const OptTensor& value_pages, const OptTenso
                   scratch.data_ptr(), on.stream()), what);
   touched(key_pages);
   for (const OptTensor* x : {&value_pages, &weight, &token}) touched(*x);
+  done(key_pages);
 }
 
-void connect(const py::dict& addresses) {
+void connect(const py::dict& addresses, const py::object& first_use, const py::object& report) {
   auto take = [&](const char* name, auto& slot) {
     slot = reinterpret_cast<std::remove_reference_t<decltype(slot)>>(addresses[name].cast<uintptr_t>());
   };
@@ -249,6 +266,9 @@ void connect(const py::dict& addresses) {
   take("ri_paged_observe", lib.observe);
   take("ri_paged_evict_scratch_bytes", lib.evict_bytes);
   take("ri_paged_evict", lib.evict);
+  lib.status = addresses["status_word"].is_none() ? nullptr : reinterpret_cast<int32_t*>(addresses["status_word"].cast<uintptr_t>());
+  lib.first_use = new py::object(first_use);             // for the life of the process
+  lib.report = new py::object(report);
 }
 
 }  // namespace

@@ -46,7 +46,9 @@ def _connect():
     spec.loader.exec_module(module)
     names = ("ri_last_error", "ri_rope_paged_append", "ri_paged_decode_scratch_bytes", "ri_paged_decode",
              "ri_paged_observe_scratch_bytes", "ri_paged_observe", "ri_paged_evict_scratch_bytes", "ri_paged_evict")
-    module.connect({n: C.cast(getattr(_lib.lib, n), C.c_void_p).value for n in names})
+    addresses = {n: C.cast(getattr(_lib.lib, n), C.c_void_p).value for n in names}
+    addresses["status_word"] = _status.address()
+    module.connect(addresses, _status.used, _status.report_word)
     _native = module
     return module
 
@@ -89,8 +91,7 @@ def rope_paged_append(qkv, cos_sin, positions, axis_of, q, key_pages, value_page
     ``retroinfer_prefill_attn`` reads them."""
     native = _native or _connect()
     native.append(qkv, cos_sin, positions, _axes(axis_of), q, key_pages, value_pages, page_table, lengths, row_start, weight, token,
-                  seen, keys, values, _status.address())
-    _status.done(qkv.device)
+                  seen, keys, values)
 
 
 def paged_decode(q, key_pages, value_pages, page_table, lengths, *, out=None, lse=None, weight=None, scale=None):
@@ -99,10 +100,7 @@ def paged_decode(q, key_pages, value_pages, page_table, lengths, *, out=None, ls
     takes the log-sum-exp of the scaled scores (``scale``: 1/sqrt(128)).  A request without slots has out 0 and lse -infinity.
     ``weight``: every slot's weight grows by the probabilities it got, summed over the query heads of its KV head."""
     native = _native or _connect()
-    out = native.decode(q, key_pages, value_pages, page_table, lengths, out, lse, weight, _SCALE if scale is None else scale,
-                        _status.address())
-    _status.done(q.device)
-    return out
+    return native.decode(q, key_pages, value_pages, page_table, lengths, out, lse, weight, _SCALE if scale is None else scale)
 
 
 def paged_observe(q, key_pages, page_table, lengths, weight, *, scale=None):
@@ -111,8 +109,7 @@ def paged_observe(q, key_pages, page_table, lengths, weight, *, scale=None):
     and over the query heads of a KV head.  What ``paged_evict`` goes by after a prompt.  Requests shorter than the window are
     padded in front, with anything.  Slots must be in the order of their tokens (no eviction before)."""
     native = _native or _connect()
-    native.observe(q, key_pages, page_table, lengths, weight, _SCALE if scale is None else scale, _status.address())
-    _status.done(q.device)
+    native.observe(q, key_pages, page_table, lengths, weight, _SCALE if scale is None else scale)
 
 
 def paged_evict(key_pages, value_pages, weight, token, page_table, lengths, seen, keep, n_sink=0, n_recent=0):
@@ -123,5 +120,4 @@ def paged_evict(key_pages, value_pages, weight, token, page_table, lengths, seen
     left alone: clamp the lengths to ``keep`` when the last layer is done, and the pages behind are free.  Requests must not share
     pages."""
     native = _native or _connect()
-    native.evict(key_pages, value_pages, weight, token, page_table, lengths, seen, keep, n_sink, n_recent, _status.address())
-    _status.done(key_pages.device)
+    native.evict(key_pages, value_pages, weight, token, page_table, lengths, seen, keep, n_sink, n_recent)

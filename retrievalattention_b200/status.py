@@ -67,8 +67,11 @@ def report(status: C.c_int32) -> None:
         check()
 
 
-def done(device) -> None:
-    """``report`` for a call that ran on ``device``."""
-    _devices.add(device)
-    if _word.value:
-        report(_word)
+def used(index: int) -> None:
+    """A call runs on GPU ``index``."""
+    _devices.add(torch.device("cuda", index))
+
+
+def report_word() -> None:
+    """``report`` for a caller that has seen the word set."""
+    report(_word)

@@ -158,3 +158,6 @@ def test_refusals():
         paged.rope_paged_append(**{**good, "axis_of": (3,) * 64})
     with pytest.raises(RuntimeError, match="need row_start"):
         paged.rope_paged_append(**{**good, "row_start": None})
+    odd = torch.zeros(good["qkv"].numel() + 4, dtype=torch.bfloat16, device="cuda")[4:].view(good["qkv"].shape)
+    with pytest.raises(RuntimeError, match="aligned"):
+        paged.rope_paged_append(**{**good, "qkv": odd})

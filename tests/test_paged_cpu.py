@@ -90,16 +90,20 @@ def test_axes_of_the_frequencies():
 
 
 def test_binding_checks_before_it_touches_a_device():
+    import importlib.util
+
     import torch
 
     from retrievalattention_b200 import paged
 
-    native = paged._native or paged._connect()
+    spec = importlib.util.spec_from_file_location("_paged_binding", paged._BINDING)      # not connected: that needs a GPU
+    native = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(native)
     pages, table, lengths = torch.zeros(4, 2, 16, 128, dtype=torch.bfloat16), torch.zeros(1, 3, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
     q = torch.zeros(1, 1, 8, 128, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="on a GPU"):
-        native.decode(q, pages, pages, table, lengths, None, None, None, 0.1, 0)
+        native.decode(q, pages, pages, table, lengths, None, None, None, 0.1)
     with pytest.raises(ValueError, match="q_heads a multiple"):
-        native.decode(q[:, :, :7], pages, pages, table, lengths, None, None, None, 0.1, 0)
+        native.decode(q[:, :, :7], pages, pages, table, lengths, None, None, None, 0.1)
     with pytest.raises(TypeError):
-        native.decode("q", pages, pages, table, lengths, None, None, None, 0.1, 0)
+        native.decode("q", pages, pages, table, lengths, None, None, None, 0.1)

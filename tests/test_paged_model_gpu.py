@@ -122,6 +122,25 @@ def test_a_place_is_taken_by_another_request():
         model.cache.begin([600, 0])
 
 
+def test_decode_entry_point_reads_the_cache():
+    from paged_helpers import attend
+    from retrievalattention_b200.attn_hub import paged_decode_attn
+
+    model = small(batch=2, keep=40)
+    cache, gen = model.cache, torch.Generator().manual_seed(4)
+    model.prefill_forward([torch.randint(0, 1000, (n,), generator=gen).cuda() for n in (30, 9)])
+    q = torch.randn((2, 1, 8, DIM), generator=gen).bfloat16().cuda()
+    before = cache.weight[1].clone()
+    out = paged_decode_attn(q, None, None, 1, cache)
+    for b, n in enumerate((30, 9)):
+        ids = cache.page_table[b, :-(-n // 16)].long()
+        k, v, old, new = (p[ids].transpose(0, 1).flatten(1, 2)[:, :n].cpu().double()
+                          for p in (cache.key_pages[1], cache.value_pages[1], before, cache.weight[1]))
+        want, _, p = attend(q[b, 0].cpu().double().view(2, 4, DIM), k, v)
+        assert ((out[b, 0].cpu().double() - want.view(8, DIM)).abs() <= 2.0 ** -8 * want.view(8, DIM).abs() + 1e-4 * v.abs().max()).all()
+        assert ((new - old - p.sum(1)).abs() <= 1e-4 * p.sum(1) + 2.0 ** -22 * new).all()
+
+
 def test_refusals():
     from retrievalattention_b200.cache_hub import paged_cache
 
