@@ -13,6 +13,9 @@
 // 32768 rows of 32 + 8 heads, bf16: 149 us, 5.5 TB/s (a copy: 6.6).  A CTA per row, plain loads: 200; the next row's loads in
 // registers: 170; bulk copies, four CTAs of four rows each with the CTAs' rows interleaved: 157, with neighbouring rows 154;
 // three of three 149, three of six 185, two of eight 161: more rows in flight than the memory needs spread its accesses.
+// Short rows (half of kUnitHeads or less) go up to four together, or the latency of a row's place and angles is what counts: 30000
+// rows of 8 + 1 heads 77 -> 52 us, 15000 of 4 + 4 39 -> 31.  Longer rows have a kernel of their own without the bookkeeping, which
+// costs them more than it gives (32768 rows of 32 + 8 heads: 163 us with it).
 #include "ri_paged.cuh"
 #include "ri_tc.cuh"
 
@@ -26,7 +29,8 @@ constexpr int kWorkThreads = kWorkWarps * 32;
 constexpr int kAppendThreads = kWorkThreads + kServiceWarps * 32;
 constexpr int kAppendCtas = 3;                         // of an SM
 constexpr int kStages = 3;                             // units on their way to a CTA
-constexpr int kUnitHeads = 48;                         // 12 KB
+constexpr int kUnitHeads = 48;                         // 12 KB: a row, a part of one, or a few short ones
+constexpr int kUnitRows = 4;                           // at most
 
 struct AxisOf {
   uint8_t of[64];
@@ -45,7 +49,8 @@ struct AppendArgs {
   uint4* values;
   int64_t qkv_stride;           // 16-byte pieces
   int64_t max_positions;
-  int rows, hq, unit_heads, units_per_row;
+  int rows, hq;
+  int unit_rows, unit_heads, units_per_row;      // a unit: that many rows, of each that many heads
   AxisOf axis;
 };
 
@@ -72,55 +77,74 @@ struct alignas(16) RowPlan {
   int id, row, token;        // page (-1: none), row in it, token number
 };
 
-__device__ __forceinline__ void plan_row(const AppendArgs& a, int row, int lane, RowPlan& plan) {
+// The plans of rows row0 .. row0 + n - 1 (n <= ROWS), whose loads are on their way together: lane r looks for row r's place.
+template <int ROWS>
+__device__ __forceinline__ void plan_rows(const AppendArgs& a, int row0, int n, int lane, RowPlan* plans) {
   const Pages& p = a.pages;
-  int b = row;
+  int64_t pos[ROWS][2];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (r < n) pos[r][i] = a.positions[(int64_t)a.axis.of[lane + 32 * i] * a.rows + row0 + r];
+  int b = row0 + lane;
   if (a.row_start != nullptr) {
     b = 0;
-    for (int b0 = 0;; b0 += 32) {                      // requests that end at or before this row
-      const bool passed = b0 + lane < p.batch && a.row_start[b0 + lane + 1] <= row;
+    for (int b0 = 0;; b0 += 32) {                      // requests that end at or before the first row
+      const bool passed = b0 + lane < p.batch && a.row_start[b0 + lane + 1] <= row0;
       const unsigned votes = __ballot_sync(0xffffffffu, passed);
       b += __popc(votes);
       if (votes != 0xffffffffu) break;
     }
+    if (ROWS > 1 && lane < n)
+      while (b < p.batch && a.row_start[b + 1] <= row0 + lane) ++b;
   }
-  float cs[4];
+  // rows that belong to no request (i < 0) are rotated, no more
+  int i_row = -1, length = 0, token = 0;
+  if (lane < n && b < p.batch) {
+    i_row = row0 + lane - (a.row_start != nullptr ? a.row_start[b] : b);
+    length = p.lengths[b];
+    token = a.seen != nullptr ? a.seen[b] : length;
+  }
+  float cs[ROWS][4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    int64_t pos = a.positions[(int64_t)a.axis.of[lane + 32 * i] * a.rows + row];
-    pos = pos < 0 ? 0 : (pos >= a.max_positions ? a.max_positions - 1 : pos);
-    cs[i] = a.cos_sin[pos * 128 + lane + 32 * i];
-    cs[2 + i] = a.cos_sin[pos * 128 + 64 + lane + 32 * i];
-  }
-  if (lane == 0) {
-    plan.id = -1;
-    plan.row = plan.token = 0;
-    const int i = b < p.batch ? row - (a.row_start != nullptr ? a.row_start[b] : b) : -1;
-    if (i >= 0) {                                      // rows that belong to no request are rotated, no more
-      const int64_t slot = (int64_t)max(p.lengths[b], 0) + i;
-      if (slot < ((int64_t)p.table_stride << p.shift)) {
-        plan.id = page_to_write(p, b, (int)(slot >> p.shift));
-        plan.row = (int)slot & ((1 << p.shift) - 1);
-        plan.token = (a.seen != nullptr ? a.seen[b] : (int)slot - i) + i;
-      } else {
-        *p.status = RI_STATUS_PAGES_FULL;
+  for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (r < n) {
+        const int64_t at = (pos[r][i] < 0 ? 0 : (pos[r][i] >= a.max_positions ? a.max_positions - 1 : pos[r][i])) * 128 + lane + 32 * i;
+        cs[r][i] = a.cos_sin[at];
+        cs[r][2 + i] = a.cos_sin[at + 64];
       }
+  if (lane < n) {
+    const int64_t slot = (int64_t)max(length, 0) + i_row;
+    int id = -1;
+    if (i_row >= 0) {
+      if (slot < ((int64_t)p.table_stride << p.shift)) id = page_to_write(p, b, (int)(slot >> p.shift));
+      else *p.status = RI_STATUS_PAGES_FULL;
     }
+    plans[lane].id = id;
+    plans[lane].row = (int)slot & ((1 << p.shift) - 1);
+    plans[lane].token = token + i_row;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) plan.cs[lane + 32 * i] = cs[i];
+  for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (r < n) plans[r].cs[lane + 32 * i] = cs[r][i];
 }
 
-// Work goes by units: a row, or an equal part of its heads where there are more than kUnitHeads.
-template <int DT>
+// Work goes by units: an equal part of a row's heads where there are more than kUnitHeads, else a row or a few.
+// ROWS: rows of a unit, at most.
+template <int DT, int ROWS>
 __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) rope_append_kernel(const __grid_constant__ AppendArgs a) {
   extern __shared__ __align__(128) uint8_t s_rows[];       // [kStages][unit_heads * 256]
-  __shared__ RowPlan s_plan[kStages];
+  __shared__ RowPlan s_plan[kStages][ROWS];
   __shared__ __align__(8) uint64_t s_full[kStages], s_empty[kStages];
   __shared__ int s_abort;
   const Pages& p = a.pages;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int heads = a.hq + 2 * p.hk, unit_bytes = a.unit_heads * 256;
+  const int heads = a.hq + 2 * p.hk, unit_rows = ROWS == 1 ? 1 : a.unit_rows, unit_bytes = unit_rows * a.unit_heads * 256;
   if (tid == 0) {
     s_abort = 0;
     for (int s = 0; s < kStages; ++s) {
@@ -133,22 +157,24 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) rope_append_kerne
   __syncthreads();
   volatile int* abort_flag = &s_abort;
   ri_pdl_enter();
-  const int units = a.rows * a.units_per_row;            // a contiguous range per CTA: neighbouring rows lie in one page
+  // a contiguous range per CTA: neighbouring rows lie in one page
+  const int units = ROWS == 1 ? a.rows * a.units_per_row : (a.rows + unit_rows - 1) / unit_rows;
   const int u_lo = (int)((int64_t)blockIdx.x * units / gridDim.x), mine = (int)((int64_t)(blockIdx.x + 1) * units / gridDim.x) - u_lo;
   bool ok = true;
   if (warp >= kWorkWarps) {
     // ---------------- service warps: every second unit each ----------------
     int i = warp - kWorkWarps;
     for (; ok && i < mine; i += kServiceWarps) {
-      const int s = i % kStages, u = u_lo + i, row = u / a.units_per_row, head0 = (u - row * a.units_per_row) * a.unit_heads;
+      const int s = i % kStages, u = u_lo + i, row = ROWS == 1 ? u / a.units_per_row : u * unit_rows;
+      const int head0 = ROWS == 1 ? (u - row * a.units_per_row) * a.unit_heads : 0, n_rows = ROWS == 1 ? 1 : min(unit_rows, a.rows - row);
       ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_empty[s]), ((i / kStages) & 1) ^ 1, abort_flag, 91));
       if (!ok) break;
       const uint32_t full = smem_u32(&s_full[s]), bytes = (uint32_t)min(a.unit_heads, heads - head0) * 256;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(full, bytes);
-        bulk_load(smem_u32(s_rows) + s * unit_bytes, a.qkv + row * a.qkv_stride + head0 * 16, bytes, full);
-      }
-      plan_row(a, row, lane, s_plan[s]);
+      if (lane == 0) mbar_arrive_expect_tx(full, n_rows * bytes);
+      __syncwarp();
+      if (lane < n_rows)
+        bulk_load(smem_u32(s_rows) + s * unit_bytes + lane * bytes, a.qkv + (row + lane) * a.qkv_stride + head0 * 16, bytes, full);
+      plan_rows<ROWS>(a, row, n_rows, lane, s_plan[s]);
       __syncwarp();
       if (lane == 0) mbar_arrive(full);
     }
@@ -159,26 +185,36 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) rope_append_kerne
     const int c = tid & 15, half = tid >> 4;
     const float sign = c < 8 ? -1.f : 1.f;
     for (int i = 0; ok && i < mine; ++i) {
-      const int s = i % kStages, u = u_lo + i, row = u / a.units_per_row, head0 = (u - row * a.units_per_row) * a.unit_heads;
+      const int s = i % kStages, u = u_lo + i, row0 = ROWS == 1 ? u / a.units_per_row : u * unit_rows;
+      const int head0 = ROWS == 1 ? (u - row0 * a.units_per_row) * a.unit_heads : 0, n_rows = ROWS == 1 ? 1 : min(unit_rows, a.rows - row0);
+      const int n = min(a.unit_heads, heads - head0);      // heads of each row
       ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[s]), (i / kStages) & 1, abort_flag, 93));
       if (!ok) break;
-      const RowPlan& plan = s_plan[s];
-      const int id = plan.id, at = plan.row, n = min(a.unit_heads, heads - head0);
       const uint4* src = reinterpret_cast<const uint4*>(s_rows + s * unit_bytes);
-      float cs[16];                                    // this piece's eight cosines, then its eight sines
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float4 f = reinterpret_cast<const float4*>(plan.cs)[(k >> 1) * 16 + (c & 7) * 2 + (k & 1)];
-        cs[4 * k] = f.x; cs[4 * k + 1] = f.y; cs[4 * k + 2] = f.z; cs[4 * k + 3] = f.w;
-      }
-      if (id >= 0 && head0 == 0) {
-        for (int h = tid; h < p.hk; h += kWorkThreads) {
-          if (p.weight != nullptr) p.weight[record_at(p, id, h, at)] = 0.f;
-          if (p.token != nullptr) p.token[record_at(p, id, h, at)] = plan.token;
+      if (head0 == 0) {
+        for (int k = tid; k < n_rows * p.hk; k += kWorkThreads) {
+          const RowPlan& plan = s_plan[s][ROWS == 1 ? 0 : k / p.hk];
+          if (plan.id < 0) continue;
+          const int64_t at = record_at(p, plan.id, ROWS == 1 ? k : k % p.hk, plan.row);
+          if (p.weight != nullptr) p.weight[at] = 0.f;
+          if (p.token != nullptr) p.token[at] = plan.token;
         }
       }
-      for (int j = half; j < n; j += kWorkThreads / 16) {
-        const int head = head0 + j, h = head - a.hq, hv = h - p.hk;
+      float cs[16];                                    // this piece's eight cosines, then its eight sines
+      int r = -1, id = -1, at = 0;                     // of row r of the unit
+      for (int j = half; j < n_rows * n; j += kWorkThreads / 16) {
+        if (r < 0 || (ROWS > 1 && j >= (r + 1) * n)) {
+          r = ROWS == 1 ? 0 : j / n;
+          const RowPlan& plan = s_plan[s][r];
+          id = plan.id;
+          at = plan.row;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float4 f = reinterpret_cast<const float4*>(plan.cs)[(k >> 1) * 16 + (c & 7) * 2 + (k & 1)];
+            cs[4 * k] = f.x; cs[4 * k + 1] = f.y; cs[4 * k + 2] = f.z; cs[4 * k + 3] = f.w;
+          }
+        }
+        const int row = row0 + r, head = head0 + j - r * n, h = head - a.hq, hv = h - p.hk;
         const uint4 x = src[j * 16 + c];
         const uint4 res = hv >= 0 ? x : rotate<DT>(x, src[j * 16 + (c ^ 8)], cs, sign);
         if (h < 0) {
@@ -244,14 +280,26 @@ extern "C" int ri_rope_paged_append(const ri_paged* p, const void* d_qkv, int64_
   const int heads = (int)hq + 2 * p->kv_heads;
   a.units_per_row = (heads + kUnitHeads - 1) / kUnitHeads;
   a.unit_heads = (heads + a.units_per_row - 1) / a.units_per_row;
-  const int64_t units = (int64_t)rows * a.units_per_row, most = (int64_t)sms * kAppendCtas;
+  // short rows go a few together, where there is more than a unit for every CTA: with fewer they would leave CTAs idle
+  a.unit_rows = 1;
+  const int64_t most = (int64_t)sms * kAppendCtas;
+  while (a.unit_rows < kUnitRows && (a.unit_rows + 1) * heads <= kUnitHeads && rows > most * a.unit_rows) ++a.unit_rows;
+  const int64_t units = a.units_per_row > 1 ? (int64_t)rows * a.units_per_row : ((int64_t)rows + a.unit_rows - 1) / a.unit_rows;
   RI_REQUIRE(units < (1ll << 30), "ri_rope_paged_append: too large");
   const dim3 grid((unsigned)(units < most ? units : most));
-  const size_t smem = (size_t)kStages * a.unit_heads * 256;
-  constexpr int kMost = kStages * kUnitHeads * 256;
-  if ((rc = p->dtype == RI_BF16 ? ri_allow_smem<rope_append_kernel<RI_BF16>>(kMost) : ri_allow_smem<rope_append_kernel<RI_F16>>(kMost)) != RI_OK)
-    return rc;
+  const size_t smem = (size_t)kStages * a.unit_rows * a.unit_heads * 256;
   auto go = [&](auto kernel) { return ri_launch_pdl_id(8, kernel, grid, dim3(kAppendThreads), smem, s, a); };
-  RI_CUDA_OK(p->dtype == RI_BF16 ? go(rope_append_kernel<RI_BF16>) : go(rope_append_kernel<RI_F16>));
+  constexpr int kMost = kStages * kUnitHeads * 256;
+  if (a.unit_rows > 1) {
+    if ((rc = ri_allow_smem<rope_append_kernel<RI_BF16, kUnitRows>>(kMost)) != RI_OK ||
+        (rc = ri_allow_smem<rope_append_kernel<RI_F16, kUnitRows>>(kMost)) != RI_OK)
+      return rc;
+    RI_CUDA_OK(p->dtype == RI_BF16 ? go(rope_append_kernel<RI_BF16, kUnitRows>) : go(rope_append_kernel<RI_F16, kUnitRows>));
+  } else {
+    if ((rc = ri_allow_smem<rope_append_kernel<RI_BF16, 1>>(kMost)) != RI_OK ||
+        (rc = ri_allow_smem<rope_append_kernel<RI_F16, 1>>(kMost)) != RI_OK)
+      return rc;
+    RI_CUDA_OK(p->dtype == RI_BF16 ? go(rope_append_kernel<RI_BF16, 1>) : go(rope_append_kernel<RI_F16, 1>));
+  }
   return RI_OK;
 }

@@ -98,6 +98,9 @@ def sections(*n):
     ((1,) * 64, [2] * 64, 1, 1, 8, torch.float16, (64,)),                           # two full rounds of requests
     ((333, 9, 0), [1501, 77, 40], 2, 3, 32, torch.float16, (16, 24, 24)),           # several rows to a CTA
     ((64, 1), [700, 1], 8, 4, 16, torch.bfloat16, (24, 20, 20)),
+    ((3, 0, 77) * 3, [700, 1, 2, 0, 3, 555, 700, 1, 40], 1, 8, 32, torch.bfloat16, (16, 24, 24)),      # four rows to a unit, of several requests
+    ((3, 9), [2001, 700], 2, 5, 16, torch.float16, (24, 20, 20)),                   # three
+    ((5,) * 70, [31] * 70, 2, 8, 8, torch.bfloat16, (64,)),                         # two, more requests than lanes
     ((0,), [1333], 8, 8, 128, torch.bfloat16, (64,)),                               # the same with two rounds a row
 ])
 def test_rows_and_places(lengths, counts, kv_heads, group, page, dtype, axes):
