@@ -54,6 +54,7 @@ struct ObsArgs : Pages {
   int max_ctas;
   float scale2;
   uint32_t idesc;
+  int mixed_halves;                              // pages of eight slots: the halves of eight keys lie behind one another
 };
 
 __device__ __forceinline__ float ex2(float x) {       // 2^x; results below 2^-126 become 0
@@ -238,9 +239,9 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
         __syncwarp();
         if (lane < tile.boxes) {
           const int id = page_or_first(a, tile.id);
-          const uint32_t dst = sK + s * kKeyTile + lane * box * 128;
-          tma_load_3d(dst, &map_k, bar_full(s), 0, tile.y, id);
-          tma_load_3d(dst + kKeyHalf, &map_k, bar_full(s), 64, tile.y, id);
+          const uint32_t dst = sK + s * kKeyTile + lane * box * (a.mixed_halves ? 256 : 128);
+          tma_load_4d(dst, &map_k, bar_full(s), 0, tile.y, 0, id);
+          if (!a.mixed_halves) tma_load_4d(dst + kKeyHalf, &map_k, bar_full(s), 0, tile.y, 1, id);
         }
       }
       if (*abort_flag)         // give the copies still in flight a bounded chance to land before the CTA exits
@@ -248,6 +249,7 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
     } else if (warp == 1) {
       // ---------------- products ----------------
       Place at = ri_seq::find_place(a, tile_at(0));
+      const uint32_t key_half = a.mixed_halves ? 1024 : kKeyHalf, key_eight = a.mixed_halves ? 2048 : 1024;
       if (lane == 0) {
         bool ok = true;
         int used = 0, groups = 0, made[2] = {0, 0};
@@ -267,7 +269,7 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
             const uint32_t d = STATS ? tmem + (2 * g + i) * 128 : tmem + g * 256;
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
-              const uint64_t dk = umma_desc_sw128(sK + s * kKeyTile + kb * kKeyHalf);
+              const uint64_t dk = umma_desc_sw128(sK + s * kKeyTile + kb * key_half, key_eight);
               const uint64_t dq = umma_desc_sw128(sQ + kb * kRowHalf + (both && g ? kTile * 128 : 0));
 #pragma unroll
               for (int k = 0; k < 4; ++k) tc_mma_f16(d, (STATS ? dq : dk) + 2 * k, (STATS ? dk : dq) + 2 * k, a.idesc, (kb | k) != 0);
@@ -494,15 +496,19 @@ __global__ void __launch_bounds__(256) observe_merge_kernel(const __grid_constan
   }
 }
 
-// Keys as (channel, row of the page's heads, page); a box is one half of the channels of at most a page.
-int make_key_map(CUtensorMap* map, const ri_paged& p) {
+// Keys as (channel of a half, row of the page's heads, half, page); a box is one half of the channels of at most a page.  Pages of
+// eight slots would take 32 boxes of 1 KB a tile, which cost more than their bytes: a box holds both halves there, one behind the
+// other (2 requests of 26508 slots, 4 heads, 70 query rows: 48.7 -> 39.1 us).  Boxes of more rows with both halves would leave the
+// operand's groups of eight rows at unequal distances, and there are few enough of them: 40 us at 16 slots a page, 37 at 128.
+int make_key_map(CUtensorMap* map, const ri_paged& p, bool mixed_halves) {
   EncodeTiledFn enc;
   const int rc = get_encode_fn(&enc);
   if (rc != RI_OK) return rc;
-  const cuuint64_t dims[3] = {RI_HEAD_DIM, (cuuint64_t)p.kv_heads * p.page_size, (cuuint64_t)p.n_pages};
-  const cuuint64_t strides[2] = {256, (cuuint64_t)p.key_page_stride * 2};
-  const cuuint32_t box[3] = {64, (cuuint32_t)(p.page_size < kTile ? p.page_size : kTile), 1}, estr[3] = {1, 1, 1};
-  const CUresult r = enc(map, p.dtype == RI_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+  const cuuint64_t dims[4] = {RI_HEAD_DIM / 2, (cuuint64_t)p.kv_heads * p.page_size, 2, (cuuint64_t)p.n_pages};
+  const cuuint64_t strides[3] = {256, 128, (cuuint64_t)p.key_page_stride * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)(p.page_size < kTile ? p.page_size : kTile), mixed_halves ? 2u : 1u, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, p.dtype == RI_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                          const_cast<void*>(p.d_keys), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   RI_REQUIRE(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code %d", (int)r);
@@ -556,11 +562,12 @@ extern "C" int ri_paged_observe(const ri_paged* p, const void* d_q, int32_t wind
   a.window = window;
   a.gs = p->group_size;
   a.scale2 = RI_LOG2E * scale;
+  a.mixed_halves = p->page_size == 8;
   int sms = 0;
   if ((rc = ri_sm_count(&sms)) != RI_OK) return rc;
   a.max_ctas = sms < kObsMaxCtas ? sms : kObsMaxCtas;
   CUtensorMap map_k;
-  if ((rc = make_key_map(&map_k, *p)) != RI_OK) return rc;
+  if ((rc = make_key_map(&map_k, *p, a.mixed_halves)) != RI_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return p->dtype == RI_BF16 ? launch_observe<RI_BF16>(a, map_k, s) : launch_observe<RI_F16>(a, map_k, s);
 }

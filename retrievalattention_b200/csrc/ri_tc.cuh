@@ -150,10 +150,10 @@ __device__ __forceinline__ void tc_ld_landed(uint32_t (&r)[32]) {
                  "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
 }
 
-// K-major operand tile, 128-byte swizzle: rows of 128 B (64 channels), 8-row atoms 1024 B apart.
-__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr) {
+// K-major operand tile, 128-byte swizzle: rows of 128 B (64 channels), 8-row atoms `eight_rows` bytes apart.
+__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr, uint32_t eight_rows = 1024) {
   const uint64_t lo = (uint64_t)((smem_addr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16);            // LBO field = 1 (unused)
-  const uint64_t hi = (uint64_t)(1024 >> 4) | ((uint64_t)1 << 14) | ((uint64_t)2 << 29);      // SBO, version 1, SW128
+  const uint64_t hi = (uint64_t)(eight_rows >> 4) | ((uint64_t)1 << 14) | ((uint64_t)2 << 29);  // SBO, version 1, SW128
   return lo | (hi << 32);
 }
 

@@ -51,6 +51,7 @@ def check(layer, q, scale=None, calls=1):
     ((900,), 1, 5, 110, 1024, torch.float16),                        # 550 rows
     ((40,) * 50, 4, 2, 7, 16, torch.bfloat16),                       # more groups than SMs
     ((9001, 1), 2, 7, 9, 8, torch.bfloat16),                         # 63 rows; one group over many SMs
+    ((390, 7, 8, 9), 2, 6, 40, 8, torch.float16),                    # 240 rows, the smallest pages
 ])
 def test_against_64_bits(lengths, kv_heads, group, window, page, dtype):
     layer = Layer(lengths, kv_heads, page, dtype, seed=31)
