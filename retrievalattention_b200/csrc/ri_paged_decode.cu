@@ -47,6 +47,7 @@ constexpr int kPagedRing = kPagedWarps * kStages * kStageBytes;   // 192 KB, on 
 constexpr int kPagedSmem = 1024 + kPagedRing;
 constexpr int kFinishThreads = 256;
 constexpr int kMaxCluster = 8;
+constexpr int kApart = 8;                             // steps whose products the tensor cores add up among themselves
 
 struct PagedArgs : Pages {
   static constexpr int kStep = 16;
@@ -126,15 +127,31 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
   const uint32_t my_ring_u32 = smem_u32(my_ring), my_full = smem_u32(&s_full[warp][0]);
   auto row_at = [&](int row) { return BOX == 16 ? row * 128 : (row >> 3) * kBox + (row & 7) * 128; };
 
-  float m_run = -INFINITY, l_run = 0.f;    // head r (l: this lane's share, reduced over the quad at the end)
-  float acc[8][4];
-  auto clear = [&] {
-    m_run = -INFINITY;
-    l_run = 0.f;
+  // Head r: a reference near the largest score so far, and the sum of the probabilities against it (this lane's share, reduced over
+  // the quad at the end).  The reference is a whole number, so that it seldom moves and a power of two does the rescaling.
+  float m_run = -INFINITY, l_run = 0.f;
+  // Tensor cores cut a sum off where an addition rounds to nearest, always towards zero, and over hundreds of steps that adds up
+  // (400 steps: 5 % of fp16 outputs rounded to the wrong side).  So the products of up to kApart steps are summed by themselves.
+  float acc[8][4], last[8][4];
+  int apart = 0;                           // steps in `last`
+  auto add_last = [&](float f0, float f1) {      // and rescale heads 2t and 2t + 1
 #pragma unroll
     for (int x = 0; x < 8; ++x)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[x][i] = 0.f;
+      for (int i = 0; i < 4; ++i) {
+        acc[x][i] = (acc[x][i] + last[x][i]) * (i & 1 ? f1 : f0);
+        last[x][i] = 0.f;
+      }
+    apart = 0;
+  };
+  auto clear = [&] {
+    m_run = -INFINITY;
+    l_run = 0.f;
+    apart = 0;
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[x][i] = last[x][i] = 0.f;
   };
   auto reduce_sum = [&] {
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
@@ -153,6 +170,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
   auto store_partial = [&](int g) {
     const int64_t slot = (int64_t)(c * kPagedWarps + warp) + g;
     reduce_sum();
+    add_last(1.f, 1.f);
     put(a.part_o + slot * gs * RI_HEAD_DIM);
     if (t == 0 && r < gs) a.part_ml[slot * gs + r] = make_float2(m_run, l_run);
   };
@@ -231,12 +249,18 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
       }
       if (WEIGHTS && r < gs)
         reinterpret_cast<float4*>(a.scores)[((score_step + s) * gs + r) * 4 + t] = make_float4(s2[0][0], s2[0][1], s2[1][0], s2[1][1]);
-      // online softmax for head r
+      // softmax for head r against a running reference
       float mx = fmaxf(fmaxf(s2[0][0], s2[0][1]), fmaxf(s2[1][0], s2[1][1]));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float m_new = fmaxf(m_run, mx), m_safe = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = exp2f(m_run - m_safe);
+      const float m_new = fmaxf(m_run, ceilf(mx)), m_safe = m_new == -INFINITY ? 0.f : m_new;
+      if (apart == kApart || __any_sync(0xffffffffu, m_new != m_run)) {
+        const float alpha = exp2f(m_run - m_safe);
+        l_run *= alpha;
+        m_run = m_new;
+        add_last(__shfl_sync(0xffffffffu, alpha, (2 * t) * 4), __shfl_sync(0xffffffffu, alpha, (2 * t + 1) * 4));
+      }
+      ++apart;
       float p[2][2], psum = 0.f;
 #pragma unroll
       for (int jj = 0; jj < 2; ++jj)
@@ -245,11 +269,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
           p[jj][e] = exp2f(s2[jj][e] - m_safe);
           psum += p[jj][e];
         }
-      l_run = l_run * alpha + psum;
-      m_run = m_new;
-      const float f0 = __shfl_sync(0xffffffffu, alpha, (2 * t) * 4), f1 = __shfl_sync(0xffffffffu, alpha, (2 * t + 1) * 4);
-#pragma unroll
-      for (int x = 0; x < 8; ++x) { acc[x][0] *= f0; acc[x][1] *= f1; acc[x][2] *= f0; acc[x][3] *= f1; }
+      l_run += psum;
       uint4 v[4][2];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -268,7 +288,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
           if (base + t + 4 * i >= at.rows) v[i][0] = v[i][1] = make_uint4(0, 0, 0, 0);
       }
       const uint2 b0 = split2<DT>(p[0][0], p[0][1]), b1 = split2<DT>(p[1][0], p[1][1]);
-      pv_step<DT, true>(acc, v, b0.x, b1.x, b0.y, b1.y);
+      pv_step<DT, true>(last, v, b0.x, b1.x, b0.y, b1.y);
       if (++stage == kStages) { stage = 0; phase ^= 1; }
     }
     if (!ok) {               // leave a bounded chance to the copies in flight before their memory goes
@@ -284,6 +304,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
   if (!merged) return;
 
   reduce_sum();
+  add_last(1.f, 1.f);
   if (t == 0) { sm_m[warp][r] = m_run; sm_l[warp][r] = l_run; }
   auto warp_o = [&](int w) { return reinterpret_cast<float*>(ring + w * kStageBytes); };
   float* cta_o = reinterpret_cast<float*>(ring + kPagedWarps * kStageBytes);      // CLUSTER: this CTA's partial result
