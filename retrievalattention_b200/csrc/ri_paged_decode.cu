@@ -9,7 +9,8 @@
 // contiguous range per SM and again per warp, whatever the requests' lengths; a warp streams its steps through its own ring,
 // filled by TMA, a box of 16 rows (8 where a page has no more) of both halves of the channels; the number of the next
 // step's page is fetched a step ahead.  Layout in shared memory and the order of the keys in a step: as in ri_dense_decode.cu.
-// The probabilities enter the second product as two 16-bit parts, so out is within its own rounding of 32-bit arithmetic.
+// The probabilities enter the second product as two 16-bit parts: 16 bits of them with bf16, 22 with fp16, whose short exponent a
+// moving reference makes up for (see m_run).  Either is a hundredth of the output's own rounding.
 // A second kernel merges a group's partial results by log-sum-exp in a fixed order.  For the weights the first kernel
 // leaves the scores behind (4 bytes a slot and query head, against 512 a slot for K and V), and the second turns them into
 // probabilities; every slot has one thread, so the sums have one order and no atomics.
@@ -65,6 +66,16 @@ __device__ __forceinline__ int used_ctas(int total, int max_ctas) { return ri_se
 
 // The scores of a step lie in the order of the lanes that made them: place i holds key (i / 2 % 2) * 8 + i / 4 + (i % 2) * 4.
 __device__ __forceinline__ int slot_in_step(int place) { return (place & ~15) + ((place >> 1) & 1) * 8 + ((place >> 2) & 3) + (place & 1) * 4; }
+
+// Two probabilities as two 16-bit parts each.  One that fp16 has no value for takes the smallest and what is too much of it, so
+// that it gives finite values nothing and an infinite one its infinity.
+template <int DT>
+__device__ __forceinline__ uint2 two_parts(float p0, float p1) {
+  if (DT != RI_F16) return split2<DT>(p0, p1);
+  constexpr float kSmallest = 5.9604645e-8f;           // 2^-24
+  const uint32_t hi = Elem<DT>::pack2(p0 > 0.f ? fmaxf(p0, kSmallest) : p0, p1 > 0.f ? fmaxf(p1, kSmallest) : p1);
+  return make_uint2(hi, Elem<DT>::pack2(p0 - Elem<DT>::from_bits((uint16_t)(hi & 0xffffu)), p1 - Elem<DT>::from_bits((uint16_t)(hi >> 16))));
+}
 
 // BOX: rows of a TMA box.  CLUSTER: a group per cluster, which shares out the group's steps, joins the partial results through
 // distributed shared memory and adds the weights: no second kernel.
@@ -129,7 +140,11 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
 
   // Head r: a reference near the largest score so far, and the sum of the probabilities against it (this lane's share, reduced over
   // the quad at the end).  The reference is a whole number, so that it seldom moves and a power of two does the rescaling.
-  float m_run = -INFINITY, l_run = 0.f;
+  // bf16 holds probabilities of any size.  fp16 ends at 2^-24: there the reference lies kAbove below the largest score, so that
+  // probabilities go up to 2^15, and follows steps down whose largest is kSmallSteps smaller, to kDeepest below the largest
+  // of all (`peak`; sums stay below 2^105).  What a probability may lose is 2^-25 against the 2^6 and more of its step's largest.
+  constexpr float kAbove = DT == RI_F16 ? 15.f : 0.f, kSmallSteps = 8.f, kDeepest = 60.f;
+  float m_run = -INFINITY, l_run = 0.f, peak = -INFINITY;
   // Tensor cores cut a sum off where an addition rounds to nearest, always towards zero, and over hundreds of steps that adds up
   // (400 steps: 5 % of fp16 outputs rounded to the wrong side).  So the products of up to kApart steps are summed by themselves.
   float acc[8][4], last[8][4];
@@ -145,7 +160,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
     apart = 0;
   };
   auto clear = [&] {
-    m_run = -INFINITY;
+    m_run = peak = -INFINITY;
     l_run = 0.f;
     apart = 0;
 #pragma unroll
@@ -253,7 +268,13 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
       float mx = fmaxf(fmaxf(s2[0][0], s2[0][1]), fmaxf(s2[1][0], s2[1][1]));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float m_new = fmaxf(m_run, ceilf(mx)), m_safe = m_new == -INFINITY ? 0.f : m_new;
+      const float here = ceilf(mx) - kAbove;               // NaN where all scores are: that moves nothing
+      float m_new = fmaxf(m_run, here);
+      if (DT == RI_F16) {
+        peak = fmaxf(peak, here);
+        if (here < m_run - kSmallSteps) m_new = fmaxf(here, peak - kDeepest);
+      }
+      const float m_safe = m_new == -INFINITY ? 0.f : m_new;
       if (apart == kApart || __any_sync(0xffffffffu, m_new != m_run)) {
         const float alpha = exp2f(m_run - m_safe);
         l_run *= alpha;
@@ -287,7 +308,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
         for (int i = 0; i < 4; ++i)
           if (base + t + 4 * i >= at.rows) v[i][0] = v[i][1] = make_uint4(0, 0, 0, 0);
       }
-      const uint2 b0 = split2<DT>(p[0][0], p[0][1]), b1 = split2<DT>(p[1][0], p[1][1]);
+      const uint2 b0 = two_parts<DT>(p[0][0], p[0][1]), b1 = two_parts<DT>(p[1][0], p[1][1]);
       pv_step<DT, true>(last, v, b0.x, b1.x, b0.y, b1.y);
       if (++stage == kStages) { stage = 0; phase ^= 1; }
     }
