@@ -365,8 +365,9 @@ int ri_rope_paged_append(const ri_paged* p, const void* d_qkv, int64_t qkv_strid
                          const int32_t* d_row_start, const int32_t* d_seen, void* d_q, void* d_k, void* d_v, void* stream);
 /* Attention of one query row of every request and head over the slots in use: d_q [batch][kv_heads * group_size][128], requests
  * q_stride elements apart, group_size 1 to 8; d_out dense; d_lse [batch, q_heads] natural log-sum-exp of the scaled scores or
- * NULL.  A request without slots has out 0 and lse -infinity.  With d_weight every slot's weight grows by the probabilities it
- * got from the query heads of its group.  d_scratch: that many bytes of 16-byte aligned device memory, any contents, for
+ * NULL.  A request without slots has out 0 and lse -infinity, as has a head all of whose scores are -infinity; a score that is NaN
+ * or +infinity makes that head's out and lse NaN.  With d_weight every slot's weight grows by the probabilities it got from the
+ * query heads of its group (NaN where one of them is).  d_scratch: that many bytes of 16-byte aligned device memory, any contents, for
  * this call alone (more with d_weight). */
 int64_t ri_paged_decode_scratch_bytes(const ri_paged* p);
 int ri_paged_decode(const ri_paged* p, const void* d_q, int64_t q_stride, void* d_out, float* d_lse, float scale, void* d_scratch,

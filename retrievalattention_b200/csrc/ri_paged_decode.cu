@@ -1,7 +1,8 @@
 // Attention of one new token over a paged cache, and the weight that it gives to every slot.
 //   out_h = sum_j p_hj v_j,  p_hj = e^{s_hj - lse_h},  s_hj = scale q_h.k_j,  lse_h = log sum_j e^{s_hj}
 //   weight_j += sum_h p_hj over the query heads of a KV head (what ri_paged_evict goes by), where asked for
-// A request without slots has out 0 and lse -infinity.
+// A request without slots has out 0 and lse -infinity, and so has a head all of whose scores are -infinity.  A score that is NaN or
+// +infinity makes its head's out and lse and the group's weights NaN, as the formulas do.
 //
 // Bound by the rows of K and V, read once: with at most eight query heads to a KV head there are 16 operations for each byte
 // read, a sixteenth of what the tensor cores need to be the limit, so m16n8k16 with the heads in M is enough.
@@ -376,14 +377,14 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
     const float2 all = joined(idx >> 7, ml);
 #pragma unroll
     for (int i = 0; i < kMaxCluster; ++i) O += o[i] * exp2f(ml[i].x - all.x);
-    a.out[(int64_t)c_first.g * gs * RI_HEAD_DIM + idx] = Elem<DT>::bits(all.y > 0.f ? O / all.y : 0.f);
-    if ((idx & 127) == 0 && a.lse != nullptr) a.lse[c_first.g * gs + (idx >> 7)] = all.y > 0.f ? (all.x + log2f(all.y)) * 0.69314718055994531f : -INFINITY;
+    a.out[(int64_t)c_first.g * gs * RI_HEAD_DIM + idx] = Elem<DT>::bits(all.y == 0.f ? 0.f : O / all.y);
+    if ((idx & 127) == 0 && a.lse != nullptr) a.lse[c_first.g * gs + (idx >> 7)] = all.y == 0.f ? -INFINITY : (all.x + log2f(all.y)) * 0.69314718055994531f;
   }
   if (WEIGHTS) {
     if (tid < gs) {
       float2 ml[kMaxCluster];
       const float2 all = joined(tid, ml);
-      sm_l[0][tid] = all.y > 0.f ? all.x + log2f(all.y) : INFINITY;      // nothing to give: 0
+      sm_l[0][tid] = all.y == 0.f ? INFINITY : all.x + log2f(all.y);      // nothing to give: 0
     }
     __syncthreads();
     const int b = c_first.g / a.hk, h_kv = c_first.g - b * a.hk;
@@ -560,14 +561,14 @@ __global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_ke
       float sum = 0.f;
 #pragma unroll
       for (int w = 0; w < kFinishThreads / 32; ++w) sum += s_o[w][tid];
-      a.out[((int64_t)g * gs + head) * RI_HEAD_DIM + tid] = Elem<DT>::bits(s_l[head] > 0.f ? sum / s_l[head] : 0.f);
+      a.out[((int64_t)g * gs + head) * RI_HEAD_DIM + tid] = Elem<DT>::bits(s_l[head] == 0.f ? 0.f : sum / s_l[head]);
     }
   }
   if (!folds) return;
   __syncthreads();
   float lse2[kMaxHeads];
 #pragma unroll
-  for (int h = 0; h < kMaxHeads; ++h) lse2[h] = h < gs && s_l[h] > 0.f ? s_m[h] + log2f(s_l[h]) : INFINITY;      // nothing to give: 0
+  for (int h = 0; h < kMaxHeads; ++h) lse2[h] = h < gs && s_l[h] != 0.f ? s_m[h] + log2f(s_l[h]) : INFINITY;      // nothing to give: 0
   for (int tile = blockIdx.x; tile * kFoldSlots < rows; tile += gridDim.x) {
     if (tile != (int)blockIdx.x) {
       find_pages(tile);

@@ -1,0 +1,100 @@
+"""Infinite and NaN keys, queries and scores in ``paged.paged_decode``.
+
+A score of -infinity is a slot that gets nothing; a NaN or +infinity makes the softmax of its query row NaN, as the definition does:
+that head's output and log-sum-exp, and the weights of the slots that the row sees.  Everything else is as without it."""
+import pytest
+import torch
+
+from paged_helpers import DIM, Layer, attend, rounding
+
+pytestmark = pytest.mark.gpu
+
+INF, NAN = float("inf"), float("nan")
+SHORT, LONG = (300, 77), (9001, 70)            # a cluster of CTAs per group; an even split over the chip
+
+
+def prepared(lengths, kv_heads, dtype, seed, at, value, slot, channel=5):
+    """A layer whose request 0 has `value` in one channel of the key of `slot` of KV head `at`, and its keys before."""
+    layer = Layer(lengths, kv_heads, 16, dtype, seed=seed)
+    k = layer.k[0].clone()
+    k[at, slot, channel] = value
+    layer.fill(0, k.to(dtype), layer.v[0].to(dtype), layer.w[0].float(), layer.t[0])
+    return layer
+
+
+def decode(layer, q):
+    from retrievalattention_b200 import paged
+
+    lse = torch.zeros((q.shape[0], q.shape[2]), device="cuda")
+    out = paged.paged_decode(q, layer.keys, layer.values, layer.table, layer.lengths, lse=lse, weight=layer.weight)
+    return out, lse
+
+
+def check_decode(layer, q, out, lse, dead=()):
+    """Heads of `dead`, of request 0, are NaN, and so are the weights of their KV heads; everything else as defined."""
+    half, tiny = rounding(layer.dtype)
+    group = q.shape[2] // layer.hk
+    for b in range(q.shape[0]):
+        want, want_lse, p = attend(q[b, 0].cpu().double().view(layer.hk, group, DIM), layer.k[b], layer.v[b])
+        got_w = layer.gather(layer.weight, b).double()
+        for h in range(layer.hk):
+            heads = range(h * group, (h + 1) * group)
+            lost = [b == 0 and x in dead for x in heads]
+            for i, x in enumerate(heads):
+                got, got_lse = out[b, 0, x].cpu().double(), lse[b, x].item()
+                if lost[i]:
+                    assert got.isnan().all() and got_lse != got_lse, (b, x)
+                else:
+                    assert ((got - want[h, i]).abs() <= half * want[h, i].abs() + 1e-4 * 6 + tiny).all(), (b, x)
+                    assert abs(got_lse - want_lse[h, i].item()) <= 3e-5
+            if any(lost):
+                assert got_w[h].isnan().all(), (b, h)
+            else:
+                given = p[h].sum(0)
+                assert ((got_w[h] - layer.w[b][h] - given).abs() <= 6e-5 * given + 2.0 ** -23 * (1 + given)).all(), (b, h)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lengths", [SHORT, LONG])
+@pytest.mark.parametrize("slot", [0, 40, -1])
+def test_decode_nan_key(lengths, dtype, slot):
+    layer = prepared(lengths, 2, dtype, 61, 1, NAN, slot)
+    q = torch.randn((2, 1, 8, DIM), generator=layer.gen).to(dtype).cuda()
+    check_decode(layer, q, *decode(layer, q), dead=range(4, 8))
+
+
+@pytest.mark.parametrize("lengths", [SHORT, LONG])
+def test_decode_infinite_key(lengths):
+    """-infinity for heads whose query is positive in the channel, +infinity for the others."""
+    layer = prepared(lengths, 2, torch.float16, 62, 0, -INF, 33)
+    q = torch.randn((2, 1, 8, DIM), generator=layer.gen)
+    q[0, 0, :4, 5] = torch.tensor([0.5, 1.0, 2.0, 0.25])
+    whole = q.half().cuda()
+    check_decode(layer, whole, *decode(layer, whole))
+    layer = prepared(lengths, 2, torch.float16, 62, 0, -INF, 33)
+    q[0, 0, 2, 5] = -1.0
+    q = q.half().cuda()
+    check_decode(layer, q, *decode(layer, q), dead=(2,))
+
+
+@pytest.mark.parametrize("lengths", [SHORT, LONG])
+def test_decode_nan_query(lengths):
+    layer = Layer(lengths, 2, 16, torch.bfloat16, seed=63)
+    q = torch.randn((2, 1, 8, DIM), generator=layer.gen)
+    q[0, 0, 5, 100] = NAN
+    q = q.bfloat16().cuda()
+    check_decode(layer, q, *decode(layer, q), dead=(5,))
+
+
+@pytest.mark.parametrize("lengths", [SHORT, LONG])
+def test_decode_only_minus_infinity(lengths):
+    """A head all of whose scores are -infinity is as one without slots."""
+    layer = Layer(lengths, 1, 16, torch.bfloat16, seed=64)
+    k = layer.k[0].clone()
+    k[:, :, 7] = -INF
+    layer.fill(0, k.bfloat16(), layer.v[0].bfloat16(), layer.w[0].float(), layer.t[0])
+    q = torch.randn((2, 1, 2, DIM), generator=layer.gen)
+    q[0, 0, :, 7] = 1.0
+    out, lse = decode(layer, q.bfloat16().cuda())
+    assert (out[0] == 0).all() and (lse[0] == -INF).all() and torch.isfinite(out[1].float()).all()
+    assert torch.equal(layer.gather(layer.weight, 0).double(), layer.w[0])
