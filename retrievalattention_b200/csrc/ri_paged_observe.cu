@@ -295,7 +295,8 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
         const int end = STATS ? min(hi, g_end) - lo : hi - max(lo, g_first);
         const int b = at.g / a.hk, h = at.g - b * a.hk;
         // the group's query rows, their pieces swizzled as TMA would; every product over the rows before has completed, since
-        // its scores have been read
+        // its scores have been read.  Rows that fill up a tile repeat the last one, with nothing to give: zeros would make NaN of
+        // an infinite key where no query does
         asm volatile("bar.sync 1, %0;" ::"n"(kScoreThreads) : "memory");
         {
           // a half-warp per row, eight rows of a thread on their way together
@@ -303,9 +304,8 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
           uint4 x[8];
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
-            const int i = u * 32 + (tid >> 4), r = a.first_row + i, w = r / a.gs;
-            x[u] = i < a.rows ? ri_ldg16(a.q + (((int64_t)b * a.window + w) * a.hk * a.gs + h * a.gs + r - w * a.gs) * 16 + piece)
-                              : make_uint4(0, 0, 0, 0);
+            const int r = a.first_row + min(u * 32 + (tid >> 4), a.rows - 1), w = r / a.gs;
+            x[u] = ri_ldg16(a.q + (((int64_t)b * a.window + w) * a.hk * a.gs + h * a.gs + r - w * a.gs) * 16 + piece);
           }
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
               }
               s_neg_lse[tid] = -lse2;
               if (lse2 != lse2) s_nan = 1;
-              s_last[tid] = last_seen(a, n, a.first_row + tid);
+              s_last[tid] = tid < a.rows ? last_seen(a, n, a.first_row + tid) : -1;
             }
           }
         }

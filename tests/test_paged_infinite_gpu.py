@@ -1,4 +1,4 @@
-"""Infinite and NaN keys, queries and scores in ``paged.paged_decode``.
+"""Infinite and NaN keys, queries and scores in ``paged.paged_decode`` and ``paged.paged_observe``.
 
 A score of -infinity is a slot that gets nothing; a NaN or +infinity makes the softmax of its query row NaN, as the definition does:
 that head's output and log-sum-exp, and the weights of the slots that the row sees.  Everything else is as without it."""
@@ -98,3 +98,68 @@ def test_decode_only_minus_infinity(lengths):
     out, lse = decode(layer, q.bfloat16().cuda())
     assert (out[0] == 0).all() and (lse[0] == -INF).all() and torch.isfinite(out[1].float()).all()
     assert torch.equal(layer.gather(layer.weight, 0).double(), layer.w[0])
+
+
+def observe(layer, q):
+    from retrievalattention_b200 import paged
+
+    paged.paged_observe(q, layer.keys, layer.table, layer.lengths, layer.weight)
+    return [layer.gather(layer.weight, b).double() - layer.w[b] for b in range(q.shape[0])]
+
+
+def given(layer, q, b):
+    window, gs, n = q.shape[1], q.shape[2] // layer.hk, layer.lengths_list[b]
+    rows = q[b].cpu().double().view(window, layer.hk, gs, DIM).transpose(0, 1).reshape(layer.hk, window * gs, DIM)
+    allowed = (torch.arange(n) <= (n - window + torch.arange(window))[:, None]).repeat_interleave(gs, 0)
+    s = (rows @ layer.k[b].transpose(1, 2)) * DIM ** -0.5
+    return torch.where(allowed, torch.softmax(s.masked_fill(~allowed, -INF), -1), 0.0).sum(1)
+
+
+def check_observe(layer, q, got):
+    for b in range(q.shape[0]):
+        want = given(layer, q, b)
+        assert torch.equal(got[b].isnan(), want.isnan()), b
+        ok = ~want.isnan()
+        assert ((got[b] - want).abs()[ok] <= 9e-5 * want[ok] + 2.0 ** -23 * (layer.w[b][ok] + want[ok]) + 1e-12).all(), b
+
+
+ROWS = [(1, 1), (10, 2), (11, 3), (16, 4), (35, 2), (43, 3), (50, 5)]           # window, heads to a KV head: 1 to 250 rows
+
+
+@pytest.mark.parametrize("window,group", ROWS)
+@pytest.mark.parametrize("slot", [0, 100, 512, -60])
+def test_observe_minus_infinity(window, group, slot):
+    """No row gives the slot anything, rows that fill up a tile included."""
+    layer = prepared((577, 90), 2, torch.float16, 65, 1, -INF, slot)
+    q = torch.randn((2, window, 2 * group, DIM), generator=layer.gen)
+    q[0, :, :, 5] = q[0, :, :, 5].abs() + 0.1
+    q = q.half().cuda()
+    got = observe(layer, q)
+    check_observe(layer, q, got)
+    assert got[0][1, slot] == 0
+
+
+@pytest.mark.parametrize("window,group", ROWS)
+@pytest.mark.parametrize("slot,value", [(0, NAN), (64, NAN), (576, NAN), (200, INF), (576, INF)])
+def test_observe_nan_and_plus_infinity(window, group, slot, value):
+    """577 slots: the last one is alone in its part of a tile."""
+    layer = prepared((577, 90), 2, torch.bfloat16, 66, 0, value, slot)
+    q = torch.randn((2, window, 2 * group, DIM), generator=layer.gen)
+    q[0, :, :, 5] = q[0, :, :, 5].abs() + 0.1
+    q = q.bfloat16().cuda()
+    got = observe(layer, q)
+    assert got[0][0].isnan().all() and torch.isfinite(got[0][1]).all()
+    check_observe(layer, q, got)
+
+
+@pytest.mark.parametrize("window,group", ROWS)
+def test_observe_nan_query(window, group):
+    """Slots that the row does not see keep what they have."""
+    layer = Layer((577, 90), 2, 16, torch.bfloat16, seed=67)
+    q = torch.randn((2, window, 2 * group, DIM), generator=layer.gen)
+    q[0, window // 2, group, 9] = NAN
+    q = q.bfloat16().cuda()
+    got = observe(layer, q)
+    last = 577 - window + window // 2
+    assert got[0][1, :last + 1].isnan().all() and torch.isfinite(got[0][1, last + 1:]).all() and torch.isfinite(got[0][0]).all()
+    check_observe(layer, q, got)
