@@ -374,8 +374,9 @@ int ri_paged_decode(const ri_paged* p, const void* d_q, int64_t q_stride, void* 
                     void* stream);
 /* The weight that the last `window` queries of every request give to its slots: d_q [batch][window][q_heads][128]; query w sees
  * the slots up to d_lengths[b] - window + w (one that sees none, of a request shorter than the window, may hold anything and
- * gives nothing); every slot's weight grows by the sum of its probabilities over queries and heads of its group.  window *
- * group_size below 2^20.  Writes d_weight only; d_values may be NULL.  d_scratch: that many bytes of 16-byte aligned device
+ * gives nothing); every slot's weight grows by the sum of its probabilities over queries and heads of its group.  A query all of
+ * whose scores are -infinity gives nothing; a score that is NaN or +infinity makes the weights of all slots that its query sees
+ * NaN.  window * group_size below 2^20.  Writes d_weight only; d_values may be NULL.  d_scratch: that many bytes of 16-byte aligned device
  * memory, any contents, for this call alone. */
 int64_t ri_paged_observe_scratch_bytes(const ri_paged* p);
 int ri_paged_observe(const ri_paged* p, const void* d_q, int32_t window, float scale, void* d_scratch, void* stream);

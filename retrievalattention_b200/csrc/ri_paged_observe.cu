@@ -1,7 +1,7 @@
 // The attention weight that the last `window` queries of every request give to the slots of a paged cache.
 //   weight_j += sum over query rows r (window query w, query head h of the KV head):  e^{s_rj - lse_r},
 //   s_rj = scale q_r.k_j,  lse_r = log sum_j e^{s_rj},  both over the slots that query w sees: j <= length - window + w.
-// Rows that see no slot (prompts shorter than the window) give nothing.
+// Rows that see no slot (prompts shorter than the window), or only slots of score -infinity, give nothing.
 //
 // Two passes over K, both on the tensor cores, with the query rows of a KV head (window x group, 256 at a time) in shared memory:
 //   pass 1  S = Q.K^T, M 128 query rows x N 128 keys: a thread holds a query row and keeps its running maximum and sum;
@@ -113,6 +113,8 @@ __device__ __forceinline__ float column_sum(uint32_t taddr, int chunks, float sc
 // The last slot that query row `row` sees in a request of n slots (negative: none).
 __device__ __forceinline__ int last_seen(const ObsArgs& a, int n, int row) { return n - a.window + row / a.gs; }
 
+// Where all scores so far are -infinity (or NaN), a reference that leaves them what they are.
+__device__ __forceinline__ float reference(float m) { return m == -INFINITY ? 0.f : m; }
 struct Sum {                                         // of 2^(x - m)
   float m = -INFINITY, l = 0.f;
   template <int N>
@@ -120,10 +122,10 @@ struct Sum {                                         // of 2^(x - m)
     float m_new = m, each = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) m_new = fmaxf(m_new, x[i].x);
-    if (m_new == -INFINITY) return;
+    const float ref = reference(m_new);
 #pragma unroll
-    for (int i = 0; i < N; ++i) each += x[i].y * ex2(x[i].x - m_new);
-    l = l * ex2(m - m_new) + each;
+    for (int i = 0; i < N; ++i) each += x[i].y * ex2(x[i].x - ref);
+    l = l * ex2(m - ref) + each;
     m = m_new;
   }
   __device__ __forceinline__ float lse2() const { return l > 0.f || l != l ? m + log2f(l) : INFINITY; }      // no slot: gives nothing
@@ -376,8 +378,8 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
                 for (int x = 0; x < 32; ++x)
                   if (slot0 + k * 32 + x <= last) mx = fmaxf(mx, __uint_as_float(sr[x]));
               }
-              const float m_new = fmaxf(m, mx * a.scale2);
-              l = m == -INFINITY ? 0.f : l * ex2(m - m_new);
+              const float m_new = fmaxf(m, mx * a.scale2), ref = reference(m_new);
+              l *= ex2(m - ref);
               m = m_new;
               sum = 0.f;
 #pragma unroll 1
@@ -386,7 +388,7 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
                 load_scores(scores + k * 32, sr);
 #pragma unroll
                 for (int x = 0; x < 32; ++x)
-                  if (slot0 + k * 32 + x <= last) sum += ex2(__uint_as_float(sr[x]) * a.scale2 - m_new);
+                  if (slot0 + k * 32 + x <= last) sum += ex2(__uint_as_float(sr[x]) * a.scale2 - ref);
               }
             }
             l += sum;

@@ -127,9 +127,9 @@ ROWS = [(1, 1), (10, 2), (11, 3), (16, 4), (35, 2), (43, 3), (50, 5)]           
 
 
 @pytest.mark.parametrize("window,group", ROWS)
-@pytest.mark.parametrize("slot", [0, 100, 512, -60])
+@pytest.mark.parametrize("slot", [0, 100, 512, -60, -1])
 def test_observe_minus_infinity(window, group, slot):
-    """No row gives the slot anything, rows that fill up a tile included."""
+    """No row gives the slot anything, rows that fill up a tile included; the last slot is alone in its part of a tile."""
     layer = prepared((577, 90), 2, torch.float16, 65, 1, -INF, slot)
     q = torch.randn((2, window, 2 * group, DIM), generator=layer.gen)
     q[0, :, :, 5] = q[0, :, :, 5].abs() + 0.1
@@ -163,3 +163,35 @@ def test_observe_nan_query(window, group):
     last = 577 - window + window // 2
     assert got[0][1, :last + 1].isnan().all() and torch.isfinite(got[0][1, last + 1:]).all() and torch.isfinite(got[0][0]).all()
     check_observe(layer, q, got)
+
+
+def test_observe_only_minus_infinity():
+    """Rows all of whose scores are -infinity are as rows that see no slot."""
+    layer = Layer((300, 77), 1, 16, torch.bfloat16, seed=68)
+    k = layer.k[0].clone()
+    k[:, :, 7] = -INF
+    layer.fill(0, k.bfloat16(), layer.v[0].bfloat16(), layer.w[0].float(), layer.t[0])
+    q = torch.randn((2, 9, 3, DIM), generator=layer.gen)
+    q[0, :, :, 7] = 1.0
+    got = observe(layer, q.bfloat16().cuda())
+    assert (got[0] == 0).all() and torch.isfinite(got[1]).all() and (got[1][0, :60] > 0).all()
+
+
+@pytest.mark.parametrize("slots", [range(64, 128), range(0, 577, 2), range(0, 576)])
+def test_observe_many_minus_infinity(slots):
+    """Whole parts of tiles of them, and every second slot."""
+    layer = Layer((577, 90), 1, 16, torch.bfloat16, seed=69)
+    k = layer.k[0].clone()
+    k[:, list(slots), 7] = -INF
+    layer.fill(0, k.bfloat16(), layer.v[0].bfloat16(), layer.w[0].float(), layer.t[0])
+    q = torch.randn((2, 9, 3, DIM), generator=layer.gen)
+    q[0, :, :, 7] = 1.0
+    q = q.bfloat16().cuda()
+    rows = q[0].cpu().double().reshape(27, DIM)
+    s = (rows @ layer.k[0][0].t()) * DIM ** -0.5
+    allowed = (torch.arange(577) <= (577 - 9 + torch.arange(9))[:, None]).repeat_interleave(3, 0)
+    p = torch.softmax(s.masked_fill(~allowed, -INF), -1)
+    want = torch.where(p.isnan(), 0.0, p).sum(0)                  # NaN: every slot that the row sees is at -infinity
+    got = observe(layer, q)[0][0]
+    assert (got[list(slots)] == 0).all()
+    assert ((got - want).abs() <= 9e-5 * want + 2.0 ** -23 * (layer.w[0][0] + want) + 1e-12).all()
