@@ -26,15 +26,24 @@ class paged_cache(KV_Cache):
     def __init__(self, layer_num: int, batch_size: int, max_length: int, num_key_value_heads: int, num_heads: int,
                  head_dim: int, dtype: torch.dtype, layer_mapping: dict, num_gpus: int, model_size: int, page_size: int = 16,
                  num_pages: int | None = None, keep: int | None = None, sink: int = 4, recent: int = 64, slack: int = 64) -> None:
-        super().__init__(layer_num, batch_size, max_length, num_key_value_heads, num_heads, head_dim, dtype, layer_mapping,
-                         num_gpus, model_size)
+        # whatever a later call would refuse, before a prompt has run
         if head_dim != paged.DIM:
             raise ValueError("the paged kernels are built for head_dim 128")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"the paged kernels are built for bfloat16 and float16, not {dtype}")
+        if num_key_value_heads < 1 or num_heads % num_key_value_heads or not 1 <= num_heads // num_key_value_heads <= paged.MAX_GROUP:
+            raise ValueError(f"{num_heads} query heads over {num_key_value_heads} KV heads: decode takes 1 to {paged.MAX_GROUP} to a KV head")
+        if page_size & (page_size - 1) or not 8 <= page_size <= 1024:
+            raise ValueError(f"page_size={page_size} is not a power of two from 8 to 1024")
+        if min(layer_num, batch_size, max_length) < 1 or (num_pages is not None and num_pages < 1):
+            raise ValueError("expected a layer, a request, a slot and a page or more")
         devices = {torch.device(layer_mapping[str(ldx)]) for ldx in range(layer_num)}
         if len(devices) != 1:
             raise ValueError("the layers of a paged cache lie on one GPU (several GPUs share a model by its heads)")
-        if keep is not None and not sink + recent <= keep:
-            raise ValueError(f"keep={keep} slots for {sink} first and {recent} last tokens")
+        if keep is not None and (min(sink, recent, slack) < 0 or keep < 1 or sink + recent > keep):
+            raise ValueError(f"keep={keep} slots for {sink} first and {recent} last tokens, slack={slack}")
+        super().__init__(layer_num, batch_size, max_length, num_key_value_heads, num_heads, head_dim, dtype, layer_mapping,
+                         num_gpus, model_size)
         self.device = devices.pop()
         self.page_size, self.keep, self.sink, self.recent, self.slack = page_size, keep, sink, recent, slack
         width = -(-max_length // page_size)                     # pages of the longest request

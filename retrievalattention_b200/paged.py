@@ -29,6 +29,7 @@ import os
 from . import _lib, status as _status
 
 DIM = 128
+MAX_GROUP = 8                              # query heads to a KV head that paged_decode takes
 _SCALE = DIM ** -0.5
 _BINDING = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "_paged_binding.so")
 

@@ -1,0 +1,50 @@
+"""``cache_hub.paged_cache`` on the host: what it refuses, its lengths and pages.  The pools lie on the CPU here; no kernel runs."""
+import types
+
+import pytest
+import torch
+
+
+@pytest.fixture
+def make(monkeypatch):
+    from retrievalattention_b200.cache_hub import paged_cache
+
+    monkeypatch.setattr(torch.cuda, "get_device_properties", lambda device: types.SimpleNamespace(total_memory=1 << 37))
+    monkeypatch.setattr(paged_cache, "_to_device", lambda self, values: torch.tensor(values, dtype=torch.int32))
+
+    def build(**change):
+        args = dict(layer_num=1, batch_size=2, max_length=100, num_key_value_heads=2, num_heads=8, head_dim=128, dtype=torch.bfloat16,
+                    layer_mapping={"0": "cpu"}, num_gpus=1, model_size=1)
+        return paged_cache(**{**args, **change})
+
+    return build
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(num_heads=18), "18 query heads"), (dict(num_heads=32), "32 query heads"), (dict(num_heads=7), "7 query heads"),
+    (dict(num_heads=1), "1 query heads"), (dict(num_key_value_heads=0), "0 KV heads"),
+    (dict(page_size=4), "page_size=4"), (dict(page_size=24), "page_size=24"), (dict(page_size=2048), "page_size=2048"), (dict(page_size=0), "page_size=0"),
+    (dict(dtype=torch.float32), "float32"), (dict(head_dim=64), "head_dim"), (dict(batch_size=0), "or more"), (dict(max_length=0), "or more"),
+    (dict(num_pages=0), "or more"), (dict(keep=0, sink=0, recent=0), "keep=0"), (dict(keep=10), "keep=10"), (dict(keep=80, sink=-1), "keep=80"),
+    (dict(keep=80, slack=-1), "slack=-1"),
+])
+def test_what_no_call_would_take_is_refused_at_once(make, change, words):
+    with pytest.raises(ValueError, match=words):
+        make(**change)
+
+
+def test_limits_are_the_kernels(make):
+    """The largest group and the page sizes that the constructor takes are those of the C entry points."""
+    import ctypes as C
+
+    from retrievalattention_b200 import _lib, paged
+
+    for group, page, ok in ((1, 8, True), (paged.MAX_GROUP, 1024, True), (paged.MAX_GROUP + 1, 16, False), (1, 4, False), (1, 2048, False)):
+        p = _lib.Paged(2, 2, group, page, 100, 8, _lib.RI_BF16, 0, 2 * page * 128, 2 * page * 128, 1 << 20, 1 << 21, 1 << 22, 1 << 23,
+                       1 << 24, 1 << 25, 1 << 26)
+        assert (_lib.lib.ri_paged_decode_scratch_bytes(C.byref(p)) > 0) == ok
+        if ok:
+            make(num_heads=2 * group, page_size=page)
+        else:
+            with pytest.raises(ValueError):
+                make(num_heads=2 * group, page_size=page)
