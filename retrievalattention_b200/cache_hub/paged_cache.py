@@ -11,8 +11,9 @@ accumulated attention weight (``paged.paged_evict``), and the pages behind go ba
     cache.evict()                                           # does nothing until a request is `slack` slots over `keep`
 
 and of a prompt: ``begin`` with every request's tokens, ``append`` with ``keys`` and ``values`` for ``retroinfer_prefill_attn``, then
-``observe`` with the last queries and ``evict(slack=0)``.  Lengths and pages are known on the host without asking the GPU, so
-nothing synchronises.
+``observe`` with the last queries and ``evict(slack=0)``.  A prompt that takes a released place beside running requests names itself:
+``begin([0, 57, 0])``, ``append`` with its rows, ``observe(queries, layer, requests=[1])``; so do decode steps of some requests.
+Lengths and pages are known on the host without asking the GPU, so nothing synchronises.
 """
 from __future__ import annotations
 
@@ -63,6 +64,9 @@ class paged_cache(KV_Cache):
         self.length_of = [0] * batch_size                       # `lengths` on the host
         self._free = list(range(self.num_pages - 1, -1, -1))
         self._pages = [[] for _ in range(batch_size)]
+        self._evicted = [False] * batch_size                    # whose slots are no longer in the order of their tokens
+        self._fed = [0] * batch_size                            # tokens of the step
+        self._chosen = {}                                       # the step's tables and lengths of some requests
 
     def _to_device(self, values) -> torch.Tensor:
         return torch.tensor(values, dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
@@ -89,6 +93,7 @@ class paged_cache(KV_Cache):
             both = self._to_device([where, what])
             self.page_table.view(-1).index_copy_(0, both[0].long(), both[1])
         self.length_of = [n + more for n, more in zip(self.length_of, each)]
+        self._fed, self._chosen = each, {}
         self.held.copy_(self.lengths)
         self.seen.copy_(self.seen_after)
         if same:
@@ -113,16 +118,38 @@ class paged_cache(KV_Cache):
                                 self.page_table, self.held, self.row_start, weight=self.weight[layer_idx],
                                 token=self.token[layer_idx], seen=self.seen, keys=keys, values=values)
 
-    def attend(self, query_states, layer_idx, out=None, lse=None) -> torch.Tensor:
-        """Attention of one new token of every request, ``[batch, 1, heads, 128]``, over its slots (``paged.paged_decode``); with
-        ``keep`` the slots' weights grow by what they are given."""
-        return paged.paged_decode(query_states, self.key_pages[layer_idx], self.value_pages[layer_idx], self.page_table, self.lengths,
-                                  out=out, lse=lse, weight=self.weight[layer_idx])
+    def _of(self, requests):
+        """Page table and lengths, of all requests or of some; the layers of a step share them."""
+        if requests is None:
+            return self.page_table, self.lengths
+        key = tuple(int(b) for b in requests)
+        if key not in self._chosen:
+            if not key or len(set(key)) < len(key) or min(key) < 0 or max(key) >= self.batch_size:
+                raise ValueError(f"{key} are not different requests of 0 to {self.batch_size - 1}")
+            at = self._to_device(key).long()
+            self._chosen[key] = self.page_table[at], self.lengths[at]
+        return self._chosen[key]
 
-    def observe(self, query_states, layer_idx) -> None:
-        """Weights from a prompt's last queries ``[batch, window, heads, 128]`` (``paged.paged_observe``)."""
-        if self.keep is not None:
-            paged.paged_observe(query_states, self.key_pages[layer_idx], self.page_table, self.lengths, self.weight[layer_idx])
+    def attend(self, query_states, layer_idx, out=None, lse=None, requests=None) -> torch.Tensor:
+        """Attention of one new token of every request, ``[batch, 1, heads, 128]``, over its slots (``paged.paged_decode``); with
+        ``keep`` the slots' weights grow by what they are given.  ``requests``: of these alone, in the order of their queries."""
+        table, lengths = self._of(requests)
+        return paged.paged_decode(query_states, self.key_pages[layer_idx], self.value_pages[layer_idx], table, lengths, out=out, lse=lse,
+                                  weight=self.weight[layer_idx])
+
+    def observe(self, query_states, layer_idx, requests=None) -> None:
+        """Weights from the last queries ``[batch, window, heads, 128]`` of the step's prompts (``paged.paged_observe``).  ``requests``:
+        of these alone, in the order of their queries; without it every request must have had tokens in the step, or have none at all.
+        A request that was evicted from cannot be observed: its slots are not in the order of its tokens."""
+        if self.keep is None:
+            return
+        table, lengths = self._of(requests)
+        for b in range(self.batch_size) if requests is None else requests:
+            if self._evicted[b]:
+                raise RuntimeError(f"slots of request {b} were evicted: what its queries see is not known any more")
+            if requests is None and self.length_of[b] and not self._fed[b]:
+                raise ValueError(f"request {b} had no tokens in this step: name the `requests` that are to be observed")
+        paged.paged_observe(query_states, self.key_pages[layer_idx], table, lengths, self.weight[layer_idx])
 
     def evict(self, slack: int | None = None) -> bool:
         """Once a request is ``slack`` slots over ``keep``, bring every request down to ``keep`` and give the pages behind back."""
@@ -133,6 +160,8 @@ class paged_cache(KV_Cache):
             paged.paged_evict(self.key_pages[ldx], self.value_pages[ldx], self.weight[ldx], self.token[ldx], self.page_table,
                               self.lengths, self.seen_after, self.keep, self.sink, self.recent)
         self.lengths.clamp_(max=self.keep)
+        self._evicted = [e or n > self.keep for e, n in zip(self._evicted, self.length_of)]
+        self._chosen = {}
         self.length_of = [min(n, self.keep) for n in self.length_of]
         for b, n in enumerate(self.length_of):
             self._give_back(b, -(-n // self.page_size))
@@ -141,7 +170,7 @@ class paged_cache(KV_Cache):
     def release(self, bdx: int) -> None:
         """Request ``bdx`` is done: its pages go back, and its place may take another one."""
         self._give_back(bdx, 0)
-        self.length_of[bdx] = 0
+        self.length_of[bdx], self._evicted[bdx], self._fed[bdx], self._chosen = 0, False, 0, {}
         for x in (self.lengths, self.seen_after):
             x[bdx].zero_()
 
