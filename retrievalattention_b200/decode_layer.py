@@ -153,15 +153,16 @@ class SyntheticDecoder:
 
 
 class PagedDecoder(SyntheticDecoder):
-    """The same model over a ``paged_cache``: prompts of uneven lengths in one pass, then a token of every request a step.
-    ``axis_of``: the position axis of each rotary frequency (``paged.rope_sections``); ``window``: the last queries of a prompt that
+    """The same model over a ``paged_cache``: prompts of uneven lengths in one pass, then a token of every running request a step.
+    A request that is done gives its place back (``release``), and another prompt may take it while the rest run on.  ``axis_of``: the position axis of each rotary frequency (``paged.rope_sections``); ``window``: the last queries of a prompt that
     its slots' weights come from, where the cache evicts."""
 
     def __init__(self, shape: ModelShape, cache, batch: int, max_positions: int, device, dtype=torch.bfloat16, seed: int = 0,
                  std: float = 0.02, layers: int | None = None, axis_of=None, window: int = 32):
         super().__init__(shape, cache, batch, max_positions, device, dtype, seed, std, layers)
         self.axis_of = (0,) * 64 if axis_of is None else tuple(axis_of)
-        self.axes, self.window = max(self.axis_of) + 1, window
+        self.axes, self.window, self._places = max(self.axis_of) + 1, window, {}
+        self._released = set()                                  # places that no request runs in
         self.positions = torch.zeros((self.axes, batch), dtype=torch.int64, device=device)       # of the next token
 
     def _layer(self, ldx, residual, x, positions, q, attend, keys=None, values=None):
@@ -176,33 +177,61 @@ class PagedDecoder(SyntheticDecoder):
         silu_and_mul(F.linear(normed, L["gate_up"]), gated)
         return F.linear(gated, L["down"])
 
-    def _logits(self, residual, x):
+    def _logits(self, residual, x, at=None):
+        """``at``: the requests that the rows are of, where they are not all."""
         normed = torch.empty_like(residual)
         rmsnorm(x, self.final_norm, self.shape.rms_eps, normed, residual=residual)
         logits = F.linear(normed, self.lm_head).float()
-        torch.argmax(logits, dim=-1, out=self.next_ids)
+        if at is None:
+            torch.argmax(logits, dim=-1, out=self.next_ids)
+        else:
+            self.next_ids.index_copy_(0, at, logits.argmax(-1))
         self.input_ids.copy_(self.next_ids)
         return logits
 
-    def prefill_forward(self, prompts, positions=None) -> torch.Tensor:
-        """``prompts``: a tensor of token ids for every request; ``positions``: ``[axes, tokens]`` for each (default: counted up on
-        every axis).  Logits ``[batch, vocab]`` of the last tokens; the cache is brought down to its ``keep`` slots."""
+    def _at(self, requests):
+        """Their numbers on the device."""
+        if requests not in self._places:
+            self._places = {requests: self.cache._to_device(requests).long()}
+        return self._places[requests]
+
+    def release(self, request: int) -> None:
+        """The request is done: its pages go back, and its place may take another prompt."""
+        self.cache.release(request)
+        self._released.add(request)
+
+    def prefill_forward(self, prompts, positions=None, requests=None) -> torch.Tensor:
+        """``prompts``: a tensor of token ids for every request, or for each of ``requests`` (ascending; the others run on);
+        ``positions``: ``[axes, tokens]`` for each (default: counted up on every axis).  Logits ``[prompts, vocab]`` of the last tokens;
+        the cache is brought down to its ``keep`` slots."""
         from .attn_hub import retroinfer_prefill_attn
 
         s, counts = self.shape, [int(p.numel()) for p in prompts]
-        if len(counts) != self.batch or min(counts) < 1 or any(self.cache.length_of):
-            raise ValueError("expected a prompt of a token or more for every request, and an empty cache")
+        places = tuple(range(self.batch)) if requests is None else tuple(int(b) for b in requests)
+        if len(places) != len(counts) or not places or list(places) != sorted(set(places) & set(range(self.batch))):
+            raise ValueError(f"expected a prompt for each of the requests, which ascend from 0 to {self.batch - 1}")
+        if min(counts) < 1 or any(self.cache.length_of[b] for b in places):
+            raise ValueError("expected prompts of a token or more, and their places in the cache empty")
+        all_of_them = len(places) == self.batch
+        at, each = None if all_of_them else self._at(places), [0] * self.batch
+        for b, n in zip(places, counts):
+            each[b] = n
         if positions is None:
             positions = [torch.arange(n, device=self.device).expand(self.axes, n) for n in counts]
         where = torch.cat(list(positions), 1).to(torch.int64).contiguous()
-        self.positions.copy_(torch.stack([p.max() + 1 for p in positions]).expand(self.axes, -1))
+        after = torch.stack([p.max() + 1 for p in positions]).to(torch.int64).expand(self.axes, -1)
         rows = sum(counts)
         starts = [sum(counts[:i]) for i in range(len(counts))]
         new = lambda heads: torch.empty((rows, heads, s.head_dim), dtype=self.dtype, device=self.device)  # noqa: E731
         q, k, v = new(s.q_heads), new(s.kv_heads), new(s.kv_heads)
         residual = self.embed[torch.cat(list(prompts)).to(self.device)]
-        recent = torch.zeros((self.batch, self.window, s.q_heads, s.head_dim), dtype=self.dtype, device=self.device)
-        self.cache.begin(counts)
+        recent = torch.zeros((len(places), self.window, s.q_heads, s.head_dim), dtype=self.dtype, device=self.device)
+        self.cache.begin(each)
+        self._released.difference_update(places)
+        if at is None:
+            self.positions.copy_(after)
+        else:
+            self.positions.index_copy_(1, at, after.contiguous())
         x = None
         for ldx in range(self.n_layers):
             def attend():
@@ -213,13 +242,19 @@ class PagedDecoder(SyntheticDecoder):
                 for b, (i, n) in enumerate(zip(starts, counts)):
                     w = min(n, self.window)
                     recent[b, self.window - w:] = q[i + n - w:i + n]
-                self.cache.observe(recent, ldx)
+                self.cache.observe(recent, ldx, None if all_of_them else places)
         self.cache.evict(slack=0)
         last = torch.tensor([i + n - 1 for i, n in zip(starts, counts)], device=self.device)
-        return self._logits(residual[last], x[last])
+        return self._logits(residual[last], x[last], at)
 
     def decode_forward(self) -> torch.Tensor:
-        """One token of every request: logits ``[batch, vocab]``, the greedy next ids become ``input_ids``."""
+        """One token of every request that was not released: logits ``[running, vocab]``, the greedy next ids become their
+        ``input_ids``."""
+        running = tuple(b for b in range(self.batch) if b not in self._released)
+        if not running:
+            raise ValueError("no request is running")
+        if len(running) < self.batch:
+            return self._decode_some(running)
         torch.index_select(self.embed, 0, self.input_ids, out=self.residual)
         self.cache.begin(1)
         x, q = None, self.q.view(self.batch, self.shape.q_heads, self.shape.head_dim)
@@ -228,3 +263,16 @@ class PagedDecoder(SyntheticDecoder):
         self.cache.evict()
         self.positions.add_(1)
         return self._logits(self.residual, x)
+
+    def _decode_some(self, running) -> torch.Tensor:
+        at, s = self._at(running), self.shape
+        residual, positions = self.embed[self.input_ids[at]], self.positions[:, at]
+        q = torch.empty((len(running), 1, s.q_heads, s.head_dim), dtype=self.dtype, device=self.device)
+        self.cache.begin([int(b in running) for b in range(self.batch)])
+        x = None
+        for ldx in range(self.n_layers):
+            x = self._layer(ldx, residual, x, positions, q.view(len(running), s.q_heads, s.head_dim),
+                            lambda: self.cache.attend(q, ldx, requests=running))
+        self.cache.evict()
+        self.positions.index_add_(1, at, torch.ones_like(positions))
+        return self._logits(residual, x, at)

@@ -154,3 +154,64 @@ def test_refusals():
     cache = paged_cache(1, 2, 100, 2, 8, 128, torch.bfloat16, one, 1, 1)
     with pytest.raises(ValueError, match="every request"):
         cache.begin([1])
+
+
+@pytest.mark.parametrize("keep", [None, 500])
+def test_prompts_take_the_places_of_requests_that_are_done(keep):
+    """Three places, five requests, against 32 bits."""
+    model = small(keep=keep, slack=8)
+    gen = torch.Generator().manual_seed(7)
+    prompt = lambda n: torch.randint(0, 1000, (n,), generator=gen).cuda()  # noqa: E731
+    ids, positions = {}, {}
+
+    def admit(prompts, requests=None):
+        where = [with_image(p.numel()) for p in prompts]
+        logits = model.prefill_forward(prompts, where, requests)
+        for i, b in enumerate(range(3) if requests is None else requests):
+            ids[b], positions[b] = list(prompts[i]), where[i]
+        return logits
+
+    def check(logits, requests):
+        assert logits.shape[0] == len(requests)
+        for i, b in enumerate(requests):
+            want = in_32_bits(model, torch.stack(ids[b]), positions[b])
+            assert (logits[i] - want).norm() <= 0.05 * want.norm(), b
+            ids[b].append(model.input_ids[b].clone())
+            assert ids[b][-1] == logits[i].argmax()
+            positions[b] = torch.cat([positions[b], (positions[b].max() + 1).expand(3, 1)], 1)
+
+    check(admit([prompt(37), prompt(5), prompt(90)]), range(3))
+    check(model.decode_forward(), range(3))
+    model.release(1)
+    for _ in range(3):
+        check(model.decode_forward(), (0, 2))
+    free = model.cache.free_pages
+    check(admit([prompt(61)], [1]), (1,))
+    assert model.cache.free_pages == free - 4
+    for _ in range(2):
+        check(model.decode_forward(), range(3))
+    model.release(0)
+    model.release(2)
+    check(model.decode_forward(), (1,))
+    check(admit([prompt(3), prompt(40)], [0, 2]), (0, 2))
+    check(model.decode_forward(), range(3))
+    assert model.cache.length_of == [4, 61 + 4, 41] == model.cache.lengths.tolist()
+    for bad in ([1], [0, 0], [3], [-1]):
+        with pytest.raises(ValueError):
+            model.prefill_forward([prompt(4)] * len(bad), requests=bad)
+    for b in range(3):
+        model.release(b)
+    with pytest.raises(ValueError, match="no request"):
+        model.decode_forward()
+    assert model.cache.free_pages == model.cache.num_pages
+
+
+def test_steps_from_an_empty_cache():
+    model = small()
+    ids = [[model.input_ids[b].clone()] for b in range(3)]
+    for step in range(4):
+        logits = model.decode_forward()
+        for b in range(3):
+            want = in_32_bits(model, torch.stack(ids[b]), torch.arange(step + 1, device="cuda").expand(3, -1))
+            assert (logits[b] - want).norm() <= 0.05 * want.norm()
+            ids[b].append(model.input_ids[b].clone())
