@@ -8,7 +8,7 @@ accumulated attention weight (``paged.paged_evict``), and the pages behind go ba
     for layer in range(layers):
         cache.append(layer, qkv, cos_sin, positions, axis_of, q)
         out = paged_decode_attn(q, None, None, layer, cache)
-    cache.evict()                                           # does nothing until a request is `slack` slots over `keep`
+    cache.evict()                                           # does nothing until a request is `slack` slots over `keep`, or room ends
 
 and of a prompt: ``begin`` with every request's tokens, ``append`` with ``keys`` and ``values`` for ``retroinfer_prefill_attn``, then
 ``observe`` with the last queries and ``evict(slack=0)``.  A prompt that takes a released place beside running requests names itself:
@@ -152,9 +152,11 @@ class paged_cache(KV_Cache):
         paged.paged_observe(query_states, self.key_pages[layer_idx], table, lengths, self.weight[layer_idx])
 
     def evict(self, slack: int | None = None) -> bool:
-        """Once a request is ``slack`` slots over ``keep``, bring every request down to ``keep`` and give the pages behind back."""
+        """Once a request is ``slack`` slots over ``keep``, or over ``keep`` at all where another token of every request would not fit
+        ``max_length`` or the pool, bring every request down to ``keep`` and give the pages behind back."""
         over = self.slack if slack is None else slack
-        if self.keep is None or max(self.length_of) <= self.keep + over:
+        most = max(self.length_of)
+        if self.keep is None or most <= self.keep or (most <= self.keep + over and self._room_for_a_token()):
             return False
         for ldx in range(self.layer_num):
             paged.paged_evict(self.key_pages[ldx], self.value_pages[ldx], self.weight[ldx], self.token[ldx], self.page_table,
@@ -166,6 +168,11 @@ class paged_cache(KV_Cache):
         for b, n in enumerate(self.length_of):
             self._give_back(b, -(-n // self.page_size))
         return True
+
+    def _room_for_a_token(self) -> bool:
+        """Of every request."""
+        fresh = sum(n + 1 > len(p) * self.page_size for n, p in zip(self.length_of, self._pages))
+        return max(self.length_of) < self.max_length and fresh <= len(self._free)
 
     def release(self, bdx: int) -> None:
         """Request ``bdx`` is done: its pages go back, and its place may take another one."""

@@ -48,3 +48,57 @@ def test_limits_are_the_kernels(make):
         else:
             with pytest.raises(ValueError):
                 make(num_heads=2 * group, page_size=page)
+
+
+@pytest.fixture
+def evictions(monkeypatch):
+    """Lengths of the requests at every call of the eviction kernel."""
+    from retrievalattention_b200 import paged
+
+    seen = []
+    monkeypatch.setattr(paged, "paged_evict", lambda *a: seen.append(a[5].tolist()))
+    return seen
+
+
+def generate(cache, steps):
+    for _ in range(steps):
+        cache.begin(1)
+        cache.evict()
+
+
+@pytest.mark.parametrize("max_length", [65, 66, 80, 128])
+def test_generation_goes_on_where_max_length_is_near_keep(make, evictions, max_length):
+    """With slack=64 no request ever gets to keep + slack."""
+    cache = make(keep=64, sink=2, recent=12, max_length=max_length, slack=64)
+    generate(cache, 300)
+    assert max(cache.length_of) <= max_length and cache.lengths.tolist() == cache.length_of and cache.seen_after.tolist() == [300, 300]
+    assert evictions and all(max(n) > 64 for n in evictions)
+    assert [len(p) for p in cache._pages] == [-(-n // 16) for n in cache.length_of]
+
+
+def test_generation_goes_on_in_a_pool_sized_for_keep(make, evictions):
+    """Two requests of 64 slots, and the page that each needs for one more."""
+    cache = make(keep=64, sink=2, recent=12, max_length=400, slack=64, num_pages=10)
+    generate(cache, 300)
+    assert max(cache.length_of) <= 64 + 16 and len(evictions) > 10
+    assert sorted(cache._free + sum(cache._pages, [])) == list(range(10))
+
+
+def test_requests_run_to_the_slack_where_there_is_room(make, evictions):
+    cache = make(keep=32, sink=2, recent=12, max_length=400, slack=20)
+    generate(cache, 53)
+    assert evictions == [[53, 53]] and cache.length_of == [32, 32]
+    cache.begin([3, 0])
+    assert not cache.evict() and cache.evict(slack=0) and not cache.evict(slack=0)
+
+
+def test_nothing_to_evict_is_still_an_error(make, evictions):
+    cache = make(keep=32, sink=2, recent=12, max_length=32)
+    generate(cache, 32)
+    with pytest.raises(RuntimeError, match="more than max_length"):
+        cache.begin(1)
+    cache = make(keep=32, sink=2, recent=12, num_pages=3)
+    generate(cache, 16)
+    with pytest.raises(RuntimeError, match="pool has 1 pages left"):
+        cache.begin(1)
+    assert not evictions
