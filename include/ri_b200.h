@@ -338,9 +338,10 @@ typedef struct ri_paged {
   int32_t group_size;        /* query heads to a KV head */
   int32_t page_size;         /* a power of two from 8 to 1024 */
   int32_t n_pages;
-  int32_t table_stride;      /* page table entries of a request */
+  int32_t table_stride;      /* entries from one request's row of the page table to the next */
   int32_t dtype;             /* RI_BF16 or RI_F16 */
-  int32_t reserved;
+  int32_t table_width;       /* entries of a row that count, 0: all; a length reaches no further, and what the calls need of scratch
+                                memory, and which kernels they take, follows the slots that this has room for */
   int64_t key_page_stride, value_page_stride;
   const void* d_keys;        /* written by ri_rope_paged_append and ri_paged_evict */
   const void* d_values;

@@ -72,7 +72,7 @@ class Paged(C.Structure):
 
     _fields_ = [
         ("batch", C.c_int32), ("kv_heads", C.c_int32), ("group_size", C.c_int32), ("page_size", C.c_int32),
-        ("n_pages", C.c_int32), ("table_stride", C.c_int32), ("dtype", C.c_int32), ("reserved", C.c_int32),
+        ("n_pages", C.c_int32), ("table_stride", C.c_int32), ("dtype", C.c_int32), ("table_width", C.c_int32),
         ("key_page_stride", C.c_int64), ("value_page_stride", C.c_int64),
         ("d_keys", C.c_void_p), ("d_values", C.c_void_p), ("d_weight", C.c_void_p), ("d_token", C.c_void_p),
         ("d_table", C.c_void_p), ("d_lengths", C.c_void_p), ("d_status", C.c_void_p),

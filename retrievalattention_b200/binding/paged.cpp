@@ -100,23 +100,25 @@ ri_paged describe(const char* what, const Tensor& key_pages, const OptTensor& va
     p.value_page_stride = page_stride(what, *value_pages, "value_pages");
   }
   if (key_pages.requires_grad() || (given(value_pages) && value_pages->requires_grad())) fail(what, "there are no gradients");
-  if (page_table.dim() != 2 || page_table.scalar_type() != at::kInt || page_table.device() != device || !page_table.is_contiguous())
-    fail(what, "expected a dense int32 page_table [batch, pages of a request] on the pools' GPU");
-  const int64_t batch = page_table.size(0), width = page_table.size(1);
+  if (page_table.dim() != 2 || page_table.scalar_type() != at::kInt || page_table.device() != device || !dense_rows(page_table, 1))
+    fail(what, "expected an int32 page_table [batch, pages of a request] with dense rows on the pools' GPU");
+  const int64_t batch = page_table.size(0), width = page_table.size(1), stride = batch > 1 ? page_table.stride(0) : width;
+  if (stride < width) fail(what, "the rows of page_table overlap");
   if (!dense(lengths, {batch}, at::kInt, device)) fail(what, "expected dense int32 lengths [batch] on the pools' GPU");
   if (given(weight) && !dense(*weight, {pages, heads, page}, at::kFloat, device))
     fail(what, "expected dense fp32 weight [pages, kv_heads, page_size] on the pools' GPU");
   if (given(weight) && weight->requires_grad()) fail(what, "there are no gradients");
   if (given(token) && !dense(*token, {pages, heads, page}, at::kInt, device))
     fail(what, "expected dense int32 token [pages, kv_heads, page_size] on the pools' GPU");
-  for (int64_t n : {batch, heads, group, page, pages, width})
+  for (int64_t n : {batch, heads, group, page, pages, stride})
     if (n > INT_MAX) fail(what, "too large");
   p.batch = (int32_t)batch;
   p.kv_heads = (int32_t)heads;
   p.group_size = (int32_t)group;
   p.page_size = (int32_t)page;
   p.n_pages = (int32_t)pages;
-  p.table_stride = (int32_t)width;
+  p.table_stride = (int32_t)stride;
+  p.table_width = (int32_t)width;
   p.d_keys = key_pages.data_ptr();
   p.d_values = address(value_pages);
   p.d_weight = static_cast<float*>(address(weight));

@@ -66,7 +66,7 @@ class paged_cache(KV_Cache):
         self._pages = [[] for _ in range(batch_size)]
         self._evicted = [False] * batch_size                    # whose slots are no longer in the order of their tokens
         self._fed = [0] * batch_size                            # tokens of the step
-        self._chosen = {}                                       # the step's tables and lengths of some requests
+        self._chosen = {}                                       # the step's tables and lengths, of all and of some requests
 
     def _to_device(self, values) -> torch.Tensor:
         return torch.tensor(values, dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
@@ -119,15 +119,23 @@ class paged_cache(KV_Cache):
                                 token=self.token[layer_idx], seen=self.seen, keys=keys, values=values)
 
     def _of(self, requests):
-        """Page table and lengths, of all requests or of some; the layers of a step share them."""
-        if requests is None:
+        """Page table and lengths, of all requests or of some; the layers of a step share them.  A captured call is replayed in later
+        steps, whose requests may be longer: it takes the whole table."""
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            if requests is not None:
+                raise RuntimeError("calls over some of the requests cannot be captured: which ones is known on the host")
             return self.page_table, self.lengths
-        key = tuple(int(b) for b in requests)
+        key = None if requests is None else tuple(int(b) for b in requests)
         if key not in self._chosen:
+            # no more columns than the longest request has pages: workspaces and the choice of kernels go by them
+            table = self.page_table[:, :max(1, max(len(p) for p in self._pages))]
+            if key is None:
+                self._chosen[key] = table, self.lengths
+                return self._chosen[key]
             if not key or len(set(key)) < len(key) or min(key) < 0 or max(key) >= self.batch_size:
                 raise ValueError(f"{key} are not different requests of 0 to {self.batch_size - 1}")
             at = self._to_device(key).long()
-            self._chosen[key] = self.page_table[at], self.lengths[at]
+            self._chosen[key] = table[at], self.lengths[at]
         return self._chosen[key]
 
     def attend(self, query_states, layer_idx, out=None, lse=None, requests=None) -> torch.Tensor:
@@ -158,9 +166,10 @@ class paged_cache(KV_Cache):
         most = max(self.length_of)
         if self.keep is None or most <= self.keep or (most <= self.keep + over and self._room_for_a_token()):
             return False
+        table, lengths = self._of(None)
         for ldx in range(self.layer_num):
-            paged.paged_evict(self.key_pages[ldx], self.value_pages[ldx], self.weight[ldx], self.token[ldx], self.page_table,
-                              self.lengths, self.seen_after, self.keep, self.sink, self.recent)
+            paged.paged_evict(self.key_pages[ldx], self.value_pages[ldx], self.weight[ldx], self.token[ldx], table, lengths, self.seen_after,
+                              self.keep, self.sink, self.recent)
         self.lengths.clamp_(max=self.keep)
         self._evicted = [e or n > self.keep for e, n in zip(self._evicted, self.length_of)]
         self._chosen = {}

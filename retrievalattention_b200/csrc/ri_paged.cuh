@@ -17,12 +17,12 @@ struct Pages {
   int32_t* token;            // the same, or null
   int* status;               // 0, or what went wrong
   int64_t key_stride, value_stride;   // elements from page to page
-  int batch, hk, n_pages, table_stride, shift;   // page_size = 1 << shift
+  int batch, hk, n_pages, table_stride, width, shift;   // width: table entries that count; page_size = 1 << shift
 };
 
-// Slots of request b that are in use: its length as far as its page table reaches.
+// Slots of request b that are in use: its length as far as its page table counts.
 __device__ __forceinline__ int rows_of(const Pages& p, int b) {
-  return (int)min((int64_t)max(p.lengths[b], 0), (int64_t)p.table_stride << p.shift);
+  return (int)min((int64_t)max(p.lengths[b], 0), (int64_t)p.width << p.shift);
 }
 // A page number out of a table, for readers.  One that names no page is reported, and page 0 stands in for it: nothing outside
 // the pool is touched, and the call's results for that request mean nothing.
@@ -47,6 +47,9 @@ __device__ __forceinline__ int64_t record_at(const Pages& p, int id, int h, int 
   return (((int64_t)id * p.hk + h) << p.shift) + row;
 }
 
+inline int width_of(const ri_paged& p) { return p.table_width > 0 ? p.table_width : p.table_stride; }
+inline int64_t slots_of(const ri_paged& p) { return (int64_t)width_of(p) * p.page_size; }      // of the longest request there may be
+
 inline Pages view(const ri_paged& p) {
   Pages v = {};
   v.table = p.d_table;
@@ -57,6 +60,7 @@ inline Pages view(const ri_paged& p) {
   v.key_stride = p.key_page_stride;
   v.value_stride = p.value_page_stride;
   v.batch = p.batch; v.hk = p.kv_heads; v.n_pages = p.n_pages; v.table_stride = p.table_stride;
+  v.width = width_of(p);
   while ((1 << v.shift) < p.page_size) ++v.shift;
   return v;
 }
@@ -68,8 +72,9 @@ inline int check(const ri_paged* p, const char* what) {
   RI_REQUIRE(p->page_size >= 8 && p->page_size <= 1024 && (p->page_size & (p->page_size - 1)) == 0,
              "%s: page_size=%d unsupported (a power of two from 8 to 1024)", what, p->page_size);
   RI_REQUIRE(p->n_pages >= 1 && p->table_stride >= 1, "%s: n_pages=%d table_stride=%d unsupported", what, p->n_pages, p->table_stride);
-  RI_REQUIRE((int64_t)p->table_stride * p->page_size < (1ll << 31) - 1024 &&
-                 (int64_t)p->batch * p->kv_heads * ((int64_t)p->table_stride * p->page_size / 8 + 1) < (1ll << 31) - 1024,
+  RI_REQUIRE(p->table_width >= 0 && p->table_width <= p->table_stride, "%s: table_width=%d of table_stride=%d unsupported", what,
+             p->table_width, p->table_stride);
+  RI_REQUIRE(slots_of(*p) < (1ll << 31) - 1024 && (int64_t)p->batch * p->kv_heads * (slots_of(*p) / 8 + 1) < (1ll << 31) - 1024,
              "%s: the page table reaches too far", what);
   RI_REQUIRE(p->dtype == RI_BF16 || p->dtype == RI_F16, "dtype=%d unsupported", p->dtype);
   const int64_t page = (int64_t)p->kv_heads * p->page_size * RI_HEAD_DIM;

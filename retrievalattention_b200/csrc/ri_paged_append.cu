@@ -120,7 +120,7 @@ __device__ __forceinline__ void plan_rows(const AppendArgs& a, int row0, int n, 
     const int64_t slot = (int64_t)max(length, 0) + i_row;
     int id = -1;
     if (i_row >= 0) {
-      if (slot < ((int64_t)p.table_stride << p.shift)) id = page_to_write(p, b, (int)(slot >> p.shift));
+      if (slot < ((int64_t)p.width << p.shift)) id = page_to_write(p, b, (int)(slot >> p.shift));
       else *p.status = RI_STATUS_PAGES_FULL;
     }
     plans[lane].id = id;

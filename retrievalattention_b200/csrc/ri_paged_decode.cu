@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
     c_first = {g, 0, rows};
     c_lo = (int)((int64_t)n * rank / ctas);
     c_hi = (int)((int64_t)n * (rank + 1) / ctas);
-    score_step = (int64_t)g * steps_of(a.table_stride << a.shift);
+    score_step = (int64_t)g * steps_of(a.width << a.shift);
   } else {
     const int total = count_steps(a), n_ctas = used_ctas(total, a.max_ctas);
     if (c >= n_ctas || total == 0) return;
@@ -588,7 +588,7 @@ __global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_ke
 
 int64_t paged_slots(const ri_paged& p) { return (int64_t)kPagedMaxCtas * kPagedWarps + (int64_t)p.batch * p.kv_heads; }
 int64_t paged_most_steps(const ri_paged& p) {
-  return (int64_t)p.batch * p.kv_heads * (((int64_t)p.table_stride * p.page_size + 15) / 16);
+  return (int64_t)p.batch * p.kv_heads * ((ri_page::slots_of(p) + 15) / 16);
 }
 
 // Pages as (64 channels, row of the page's heads, half, page).
@@ -635,7 +635,7 @@ int clusters_at_once(int ctas, int* out) {
 // 9.7; 8000 slots 13.9 and 14.9).
 constexpr int kClusterSteps = 4;                       // of a warp, at most
 int cluster_size(const PagedArgs& a, int* ctas) {
-  const int64_t groups = (int64_t)a.batch * a.hk, steps = (((int64_t)a.table_stride << a.shift) + 15) / 16;
+  const int64_t groups = (int64_t)a.batch * a.hk, steps = (((int64_t)a.width << a.shift) + 15) / 16;
   *ctas = 0;
   if (groups > a.max_ctas || steps > kMaxCluster * kPagedWarps * kClusterSteps) return RI_OK;
   for (int n = 1; n <= kMaxCluster; n *= 2) {
@@ -671,7 +671,7 @@ int launch_paged(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap
   if ((rc = cluster_size(a, &ctas)) != RI_OK) return rc;
   rc = box == 8 ? launch_steps<DT, 8>(a, map_k, map_v, ctas, s) : launch_steps<DT, 16>(a, map_k, map_v, ctas, s);
   if (rc != RI_OK || ctas > 0) return rc;
-  const int64_t groups = (int64_t)a.batch * a.hk, most = (int64_t)a.table_stride << a.shift;
+  const int64_t groups = (int64_t)a.batch * a.hk, most = (int64_t)a.width << a.shift;
   // blocks of a group: for its heads, or with weights its tiles of slots, as many as the chip holds at once
   const int64_t tiles = a.weight ? (most + kFoldSlots - 1) / kFoldSlots : 0, room = kFinishBlocks * (int64_t)a.max_ctas / groups;
   int64_t blocks = tiles > a.gs ? tiles : a.gs;

@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
 }
 
 int64_t most_moves(const ri_paged& p, int64_t keep) {
-  const int64_t room = (int64_t)p.table_stride * p.page_size;
+  const int64_t room = slots_of(p);
   return keep >= room ? 0 : (keep < room - keep ? keep : room - keep);
 }
 
@@ -288,7 +288,7 @@ extern "C" int ri_paged_evict(const ri_paged* p, const int32_t* d_seen, int32_t 
              "ri_paged_evict: keep=%d slots for %d first and %d last tokens", keep, n_sink, n_recent);
   RI_REQUIRE(((uintptr_t)d_scratch | (uintptr_t)p->d_weight | (uintptr_t)p->d_token) % 16 == 0,
              "ri_paged_evict: weights, token numbers and the scratch must be 16-byte aligned");
-  const int64_t groups = (int64_t)p->batch * p->kv_heads, room = (int64_t)p->table_stride * p->page_size;
+  const int64_t groups = (int64_t)p->batch * p->kv_heads, room = slots_of(*p);
   if (room <= keep) return RI_OK;                      // no request can hold more
   EvictArgs a = {};
   a.pages = view(*p);

@@ -558,7 +558,7 @@ extern "C" int ri_paged_observe(const ri_paged* p, const void* d_q, int32_t wind
   a.part = static_cast<float2*>(d_scratch);
   // A group that few CTAs share: pass 2 merges its partial results by itself; else a kernel between the passes does, once for all.
   // 1001 slots, 8 heads, 8 CTAs a group: 11.5 us merged inside, 13.2 by a kernel; 4000 slots of one head, 32 CTAs: 17.1 and 16.2.
-  const int64_t groups = (int64_t)p->batch * p->kv_heads, tiles = ((int64_t)p->table_stride * p->page_size + kTile - 1) / kTile;
+  const int64_t groups = (int64_t)p->batch * p->kv_heads, tiles = (slots_of(*p) + kTile - 1) / kTile;
   const int64_t most = kObsMaxCtas / groups + 2;
   if ((most < tiles ? most : tiles) > kMergedInside) a.lse2 = reinterpret_cast<float*>(a.part + obs_slots(*p) * kPartials);
   a.window = window;

@@ -14,7 +14,9 @@ The layer is a handful of tensors that the caller owns (``cache_hub.paged_cache`
 ``page_table``, ``lengths``     int32 ``[batch, most pages of a request]`` and ``[batch]``: slot ``j`` of request ``b`` is row
                                 ``j % page_size`` of page ``page_table[b, j // page_size]`` for every head, and the first
                                 ``lengths[b]`` slots are in use; table entries behind them are not read.  Requests may share pages
-                                that nothing is written to (no weights, rows or evictions)
+                                that nothing is written to (no weights, rows or evictions).  Rows of the table may lie apart: workspaces
+                                and the choice of kernels follow the slots that its width has room for, so hand in no more of
+                                a wide one than the longest request needs (``page_table[:, :pages]``)
 
 Every call is asynchronous on the current stream, allocates its workspace from torch's caching allocator and can be captured in a
 CUDA graph.  Lengths and page tables are read on the device: an entry that names no page, or a row that its request's table has no

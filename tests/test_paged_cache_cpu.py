@@ -102,3 +102,20 @@ def test_nothing_to_evict_is_still_an_error(make, evictions):
     with pytest.raises(RuntimeError, match="pool has 1 pages left"):
         cache.begin(1)
     assert not evictions
+
+
+def test_table_width_bounds_the_workspaces():
+    import ctypes as C
+
+    from retrievalattention_b200 import _lib
+
+    def sizes(stride, width):
+        p = _lib.Paged(2, 4, 7, 16, 100, stride, _lib.RI_BF16, width, 4 * 16 * 128, 4 * 16 * 128, 1 << 20, 1 << 21, 1 << 22, 1 << 23,
+                       1 << 24, 1 << 25, 1 << 26)
+        return [_lib.lib.ri_paged_decode_scratch_bytes(C.byref(p)), _lib.lib.ri_paged_observe_scratch_bytes(C.byref(p)),
+                _lib.lib.ri_paged_evict_scratch_bytes(C.byref(p), 100)]
+
+    assert sizes(8000, 40) == sizes(40, 0) == sizes(40, 40) != sizes(8000, 0)
+    assert min(sizes(1 << 28, 40)) > 0                            # where a row begins does not count
+    for width in (-1, 41):
+        assert sizes(40, width) == [-1] * 3 and b"table_width" in _lib.lib.ri_last_error()
