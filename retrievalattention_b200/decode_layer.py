@@ -164,6 +164,7 @@ class PagedDecoder(SyntheticDecoder):
         self.axes, self.window, self._places = max(self.axis_of) + 1, window, {}
         self._released = set()                                  # places that no request runs in
         self.positions = torch.zeros((self.axes, batch), dtype=torch.int64, device=device)       # of the next token
+        self._next_position = [0] * batch                       # the largest of them, on the host
 
     def _layer(self, ldx, residual, x, positions, q, attend, keys=None, values=None):
         """One layer over the step's rows; ``attend()`` is called with queries, keys and values in place."""
@@ -202,8 +203,9 @@ class PagedDecoder(SyntheticDecoder):
 
     def prefill_forward(self, prompts, positions=None, requests=None) -> torch.Tensor:
         """``prompts``: a tensor of token ids for every request, or for each of ``requests`` (ascending; the others run on);
-        ``positions``: ``[axes, tokens]`` for each (default: counted up on every axis).  Logits ``[prompts, vocab]`` of the last tokens;
-        the cache is brought down to its ``keep`` slots."""
+        ``positions``: ``[axes, tokens]`` for each, from 0 to ``max_positions - 1`` (default: counted up on every axis; given ones are
+        looked at, which waits for them).  Logits ``[prompts, vocab]`` of the last tokens; the cache is brought down to its ``keep``
+        slots."""
         from .attn_hub import retroinfer_prefill_attn
 
         s, counts = self.shape, [int(p.numel()) for p in prompts]
@@ -217,9 +219,17 @@ class PagedDecoder(SyntheticDecoder):
         for b, n in zip(places, counts):
             each[b] = n
         if positions is None:
+            ends, least = counts, 0
             positions = [torch.arange(n, device=self.device).expand(self.axes, n) for n in counts]
+        else:
+            if len(positions) != len(counts) or any(p.dim() != 2 or p.shape[0] < self.axes or p.shape[1] != n for p, n in zip(positions, counts)):
+                raise ValueError(f"expected positions [{self.axes}, tokens] for every prompt")
+            ends = [n + 1 for n in torch.stack([p.max() for p in positions]).tolist()]
+            least = torch.stack([p.min() for p in positions]).min().item()
+        if least < 0 or max(ends) > self.cos_sin.shape[0]:
+            raise ValueError(f"positions {least} to {max(ends) - 1}: the table has 0 to {self.cos_sin.shape[0] - 1}")
         where = torch.cat(list(positions), 1).to(torch.int64).contiguous()
-        after = torch.stack([p.max() + 1 for p in positions]).to(torch.int64).expand(self.axes, -1)
+        after = self.cache._to_device(ends).long().expand(self.axes, -1)
         rows = sum(counts)
         starts = [sum(counts[:i]) for i in range(len(counts))]
         new = lambda heads: torch.empty((rows, heads, s.head_dim), dtype=self.dtype, device=self.device)  # noqa: E731
@@ -228,6 +238,8 @@ class PagedDecoder(SyntheticDecoder):
         recent = torch.zeros((len(places), self.window, s.q_heads, s.head_dim), dtype=self.dtype, device=self.device)
         self.cache.begin(each)
         self._released.difference_update(places)
+        for b, end in zip(places, ends):
+            self._next_position[b] = end
         if at is None:
             self.positions.copy_(after)
         else:
@@ -253,10 +265,14 @@ class PagedDecoder(SyntheticDecoder):
         running = tuple(b for b in range(self.batch) if b not in self._released)
         if not running:
             raise ValueError("no request is running")
+        # eviction bounds the slots, not the positions: behind the table's end every token would turn by the same angles
+        past = [b for b in running if self._next_position[b] >= self.cos_sin.shape[0]]
+        if past:
+            raise RuntimeError(f"requests {past} are at the end of the {self.cos_sin.shape[0]} positions that the model was made for")
         if len(running) < self.batch:
             return self._decode_some(running)
         torch.index_select(self.embed, 0, self.input_ids, out=self.residual)
-        self.cache.begin(1)
+        self._step(running, 1)
         x, q = None, self.q.view(self.batch, self.shape.q_heads, self.shape.head_dim)
         for ldx in range(self.n_layers):
             x = self._layer(ldx, self.residual, x, self.positions, q, lambda: self.cache.attend(self.q, ldx, out=self.attn))
@@ -264,11 +280,16 @@ class PagedDecoder(SyntheticDecoder):
         self.positions.add_(1)
         return self._logits(self.residual, x)
 
+    def _step(self, running, counts) -> None:
+        self.cache.begin(counts)
+        for b in running:
+            self._next_position[b] += 1
+
     def _decode_some(self, running) -> torch.Tensor:
         at, s = self._at(running), self.shape
         residual, positions = self.embed[self.input_ids[at]], self.positions[:, at]
         q = torch.empty((len(running), 1, s.q_heads, s.head_dim), dtype=self.dtype, device=self.device)
-        self.cache.begin([int(b in running) for b in range(self.batch)])
+        self._step(running, [int(b in running) for b in range(self.batch)])
         x = None
         for ldx in range(self.n_layers):
             x = self._layer(ldx, residual, x, positions, q.view(len(running), s.q_heads, s.head_dim),

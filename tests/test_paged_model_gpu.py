@@ -215,3 +215,36 @@ def test_steps_from_an_empty_cache():
             want = in_32_bits(model, torch.stack(ids[b]), torch.arange(step + 1, device="cuda").expand(3, -1))
             assert (logits[b] - want).norm() <= 0.05 * want.norm()
             ids[b].append(model.input_ids[b].clone())
+
+
+def test_generation_ends_where_the_positions_do():
+    """Eviction holds the slots, not the positions; and nothing was taken by the call that raises."""
+    model = small(keep=40)
+    model.cos_sin = model.cos_sin[:120].contiguous()
+    gen = torch.Generator().manual_seed(8)
+    prompt = lambda n: torch.randint(0, 1000, (n,), generator=gen).cuda()  # noqa: E731
+    with pytest.raises(ValueError, match="0 to 119"):
+        model.prefill_forward([prompt(4), prompt(121), prompt(4)])
+    for far in (120, -1):
+        where = [torch.arange(4).expand(3, 4).cuda() for _ in range(3)]
+        where[1] = where[1].clone()
+        where[1][2, 1] = far
+        with pytest.raises(ValueError, match="the table has"):
+            model.prefill_forward([prompt(4)] * 3, where)
+    with pytest.raises(ValueError, match="positions"):
+        model.prefill_forward([prompt(4)] * 3, [torch.zeros(2, 4, dtype=torch.int64).cuda()] * 3)
+    assert model.cache.length_of == [0, 0, 0]
+    model.prefill_forward([prompt(100), prompt(110), prompt(20)], [with_image(100), with_image(110), with_image(20)])
+    assert model.positions.tolist() == [[85, 95, 20]] * 3         # an image takes 5 positions for its 20 tokens
+    for _ in range(25):
+        model.decode_forward()
+    with pytest.raises(RuntimeError, match=r"requests \[1\] are at the end"):
+        model.decode_forward()
+    seen = model.cache.seen_after.tolist()
+    assert seen == [125, 135, 45] and model.positions[0].tolist() == [110, 120, 45]
+    model.release(1)
+    for _ in range(10):
+        model.decode_forward()                                    # the others go on
+    assert model.positions[0].tolist() == [120, 120, 55]
+    with pytest.raises(RuntimeError, match=r"requests \[0\] are at the end"):
+        model.decode_forward()
