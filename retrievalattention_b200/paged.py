@@ -75,7 +75,7 @@ def rope_interleaved(*sections: int) -> tuple:
 
 def _axes(axis_of) -> bytes:
     try:
-        return bytes(axis_of)
+        return bytes(list(axis_of))                             # a number, which bytes() takes for a length, is no list
     except (TypeError, ValueError):
         raise ValueError("rope_paged_append: axis_of names an axis for each of the 64 frequencies") from None
 

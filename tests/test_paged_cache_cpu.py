@@ -119,3 +119,12 @@ def test_table_width_bounds_the_workspaces():
     assert min(sizes(1 << 28, 40)) > 0                            # where a row begins does not count
     for width in (-1, 41):
         assert sizes(40, width) == [-1] * 3 and b"table_width" in _lib.lib.ri_last_error()
+
+
+def test_axes_that_are_no_list_of_them():
+    from retrievalattention_b200 import paged
+
+    assert paged._axes((1,) * 64) == paged._axes(bytes([1] * 64)) == paged._axes(torch.ones(64, dtype=torch.int64)) == bytes([1] * 64)
+    for bad in (64, 64.0, None, torch.tensor(64), "0" * 64, [256] * 64):
+        with pytest.raises(ValueError, match="axis_of"):
+            paged._axes(bad)
