@@ -56,15 +56,21 @@ def _connect():
     return module
 
 
+def _sections(sections) -> list:
+    if any(int(n) != n or n < 0 for n in sections):
+        raise ValueError(f"sections {sections}: expected numbers of frequencies")
+    return [int(n) for n in sections]
+
+
 def rope_sections(*sections: int) -> tuple:
     """``axis_of`` for frequencies that follow one axis section after section: ``rope_sections(64)`` is the ordinary rotary
     embedding, ``rope_sections(16, 24, 24)`` time, height and width."""
-    return tuple(a for a, n in enumerate(sections) for _ in range(n))
+    return tuple(a for a, n in enumerate(_sections(sections)) for _ in range(n))
 
 
 def rope_interleaved(*sections: int) -> tuple:
     """``axis_of`` for frequencies that are dealt out to the axes in turn, while an axis has any left."""
-    left, axes, a = list(sections), [], 0
+    left, axes, a = _sections(sections), [], 0
     while any(left):
         if left[a]:
             left[a] -= 1

@@ -128,3 +128,14 @@ def test_axes_that_are_no_list_of_them():
     for bad in (64, 64.0, None, torch.tensor(64), "0" * 64, [256] * 64):
         with pytest.raises(ValueError, match="axis_of"):
             paged._axes(bad)
+
+
+@pytest.mark.timeout(20)
+def test_sections_that_are_no_numbers_of_frequencies():
+    from retrievalattention_b200 import paged
+
+    assert paged.rope_interleaved() == paged.rope_sections() == () and paged.rope_interleaved(0, 2) == (1, 1)
+    for make_axes in (paged.rope_sections, paged.rope_interleaved):
+        for bad in ((-1,), (65, -1), (32.5, 31.5)):
+            with pytest.raises(ValueError, match="sections"):
+                make_axes(*bad)
