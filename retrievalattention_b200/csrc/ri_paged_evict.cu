@@ -27,11 +27,15 @@ constexpr int kFewThreads = 256, kManyThreads = 512;  // of a CTA of the selecti
 constexpr int kFewPerSm = 3;                         // CTAs of few threads on an SM
 constexpr int kCachedKeys = 40 * 1024;               // keys of a CTA's slice that shared memory holds
 constexpr int kSelMaxCluster = 8;
+// Slots of a group that are worth another CTA (8 groups, a call; 512 against 2048): 600 slots 14.7 and 16.0 us, 1001 16.6 and 16.0,
+// 2000 18.7 and 16.1, 4160 20.7 and 17.1.
 constexpr int kSlotsWorthACta = 512;
 constexpr int kMoveThreads = 256;
 constexpr int kMovesAtOnce = 2;                      // per half-warp
 constexpr int kMovesPerBlock = kMoveThreads / 16 * kMovesAtOnce;
-constexpr int kMovesInside = 256;                    // per CTA: up to that many the selection's clusters move the rows
+// Moves per CTA up to which the selection's clusters do them: with 128 groups of 4096 slots and a few, 256 take 21.7 us inside and 23.4
+// by a kernel of their own, 512 33.0 and 30.9.
+constexpr int kMovesInside = 256;
 constexpr uint32_t kProtected = 0xffffffffu;         // above +infinity
 
 struct EvictArgs {
