@@ -50,6 +50,9 @@ constexpr int kPagedSmem = 1024 + kPagedRing;
 constexpr int kFinishThreads = 256;
 constexpr int kMaxCluster = 8;
 constexpr int kApart = 8;                             // steps whose products the tensor cores add up among themselves
+// More steps than that to a warp, if every request were as long as its table has room for: sums in two levels.  32 steps that are
+// cut off lose 64 * 2^-25 at most, 2e-6; the second level costs 0.4 us (8 heads: 8000 slots 14.0 and 14.4 us).
+constexpr int kLongSteps = 32;
 
 struct PagedArgs : Pages {
   static constexpr int kStep = 16;
@@ -79,8 +82,8 @@ __device__ __forceinline__ uint2 two_parts(float p0, float p1) {
 }
 
 // BOX: rows of a TMA box.  CLUSTER: a group per cluster, which shares out the group's steps, joins the partial results through
-// distributed shared memory and adds the weights: no second kernel.
-template <int DT, int BOX, bool WEIGHTS, bool CLUSTER>
+// distributed shared memory and adds the weights: no second kernel.  LONG: see kLongSteps.
+template <int DT, int BOX, bool WEIGHTS, bool CLUSTER, bool LONG>
 __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                      const __grid_constant__ CUtensorMap map_v,
                                                                      const __grid_constant__ PagedArgs a) {
@@ -147,21 +150,24 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
   constexpr float kAbove = DT == RI_F16 ? 15.f : 0.f, kSmallSteps = 8.f, kDeepest = 60.f;
   float m_run = -INFINITY, l_run = 0.f, peak = -INFINITY;
   // Tensor cores cut a sum off where an addition rounds to nearest, always towards zero, and over hundreds of steps that adds up
-  // (400 steps: 5 % of fp16 outputs rounded to the wrong side).  So the products of up to kApart steps are summed by themselves.
-  float acc[8][4], last[8][4];
+  // (400 steps: 5 % of fp16 outputs rounded to the wrong side).  So where there may be many (LONG) the products of up to kApart steps
+  // are summed by themselves, in `last`, and `acc` holds those before them against the reference that they had, `m_acc`.
+  float acc[8][4], last[8][4], m_acc = -INFINITY;
   int apart = 0;                           // steps in `last`
-  auto add_last = [&](float f0, float f1) {      // and rescale heads 2t and 2t + 1
+  auto heads_2t = [&](float f, float& f0, float& f1) {      // what belongs to heads 2t and 2t + 1, of which this lane has the sums
+    f0 = __shfl_sync(0xffffffffu, f, (2 * t) * 4);
+    f1 = __shfl_sync(0xffffffffu, f, (2 * t + 1) * 4);
+  };
+  auto add_up = [&](float (&sum)[8][4]) {      // sum = acc + last
+    float f0, f1;
+    heads_2t(exp2f(m_acc - (m_run == -INFINITY ? 0.f : m_run)), f0, f1);
 #pragma unroll
     for (int x = 0; x < 8; ++x)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        acc[x][i] = (acc[x][i] + last[x][i]) * (i & 1 ? f1 : f0);
-        last[x][i] = 0.f;
-      }
-    apart = 0;
+      for (int i = 0; i < 4; ++i) sum[x][i] = fmaf(acc[x][i], i & 1 ? f1 : f0, last[x][i]);
   };
   auto clear = [&] {
-    m_run = peak = -INFINITY;
+    m_run = m_acc = peak = -INFINITY;
     l_run = 0.f;
     apart = 0;
 #pragma unroll
@@ -173,20 +179,20 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
   };
-  // accumulators to rows of 128 floats, one per head (heads 2t and 2t+1 are this lane's)
+  // sums to rows of 128 floats, one per head (heads 2t and 2t+1 are this lane's)
   auto put = [&](float* o) {
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
       const int ch = (x < 4) ? 8 * sr + 2 * x : 64 + 8 * sr + 2 * (x - 4);
-      if (2 * t < gs) *reinterpret_cast<float2*>(o + (2 * t) * RI_HEAD_DIM + ch) = make_float2(acc[x][0], acc[x][2]);
-      if (2 * t + 1 < gs) *reinterpret_cast<float2*>(o + (2 * t + 1) * RI_HEAD_DIM + ch) = make_float2(acc[x][1], acc[x][3]);
+      if (2 * t < gs) *reinterpret_cast<float2*>(o + (2 * t) * RI_HEAD_DIM + ch) = make_float2(last[x][0], last[x][2]);
+      if (2 * t + 1 < gs) *reinterpret_cast<float2*>(o + (2 * t + 1) * RI_HEAD_DIM + ch) = make_float2(last[x][1], last[x][3]);
     }
   };
   // Slots: along the sequence (warp, group) goes up by one of the two at a time, so their sum names a partial result.
   auto store_partial = [&](int g) {
     const int64_t slot = (int64_t)(c * kPagedWarps + warp) + g;
     reduce_sum();
-    add_last(1.f, 1.f);
+    if (LONG) add_up(last);
     put(a.part_o + slot * gs * RI_HEAD_DIM);
     if (t == 0 && r < gs) a.part_ml[slot * gs + r] = make_float2(m_run, l_run);
   };
@@ -276,13 +282,17 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
         if (here < m_run - kSmallSteps) m_new = fmaxf(here, peak - kDeepest);
       }
       const float m_safe = m_new == -INFINITY ? 0.f : m_new;
-      if (apart == kApart || __any_sync(0xffffffffu, m_new != m_run)) {
-        const float alpha = exp2f(m_run - m_safe);
-        l_run *= alpha;
-        m_run = m_new;
-        add_last(__shfl_sync(0xffffffffu, alpha, (2 * t) * 4), __shfl_sync(0xffffffffu, alpha, (2 * t + 1) * 4));
+      if (LONG && apart == kApart) {
+        add_up(acc);
+        m_acc = m_run;
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) last[x][i] = 0.f;
+        apart = 0;
       }
       ++apart;
+      const float alpha = exp2f(m_run - m_safe);
       float p[2][2], psum = 0.f;
 #pragma unroll
       for (int jj = 0; jj < 2; ++jj)
@@ -291,7 +301,12 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
           p[jj][e] = exp2f(s2[jj][e] - m_safe);
           psum += p[jj][e];
         }
-      l_run += psum;
+      l_run = l_run * alpha + psum;
+      m_run = m_new;
+      float f0, f1;
+      heads_2t(alpha, f0, f1);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) { last[x][0] *= f0; last[x][1] *= f1; last[x][2] *= f0; last[x][3] *= f1; }
       uint4 v[4][2];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -326,7 +341,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
   if (!merged) return;
 
   reduce_sum();
-  add_last(1.f, 1.f);
+  if (LONG) add_up(last);
   if (t == 0) { sm_m[warp][r] = m_run; sm_l[warp][r] = l_run; }
   auto warp_o = [&](int w) { return reinterpret_cast<float*>(ring + w * kStageBytes); };
   float* cta_o = reinterpret_cast<float*>(ring + kPagedWarps * kStageBytes);      // CLUSTER: this CTA's partial result
@@ -613,8 +628,8 @@ int clusters_at_once(int ctas, int* out) {
   RI_CUDA_OK(cudaGetDevice(&dev));
   const bool track = dev >= 0 && dev < 64;
   if (track && (*out = known[dev][ctas].load(std::memory_order_relaxed)) > 0) return RI_OK;
-  auto* kernel = paged_decode_kernel<RI_BF16, 16, true, true>;      // all of them have the same shared memory and threads
-  if ((rc = ri_allow_smem<paged_decode_kernel<RI_BF16, 16, true, true>>(kPagedSmem)) != RI_OK) return rc;
+  auto* kernel = paged_decode_kernel<RI_BF16, 16, true, true, false>;      // all of them have the same shared memory and threads
+  if ((rc = ri_allow_smem<paged_decode_kernel<RI_BF16, 16, true, true, false>>(kPagedSmem)) != RI_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kPagedThreads);
@@ -647,19 +662,26 @@ int cluster_size(const PagedArgs& a, int* ctas) {
   if (steps > (int64_t)*ctas * kPagedWarps * kClusterSteps) *ctas = 0;
   return RI_OK;
 }
+template <int DT, int BOX, bool WEIGHTS, bool LONG>
+int launch_split(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t s) {
+  const int rc = ri_allow_smem<paged_decode_kernel<DT, BOX, WEIGHTS, false, LONG>>(kPagedSmem);
+  if (rc != RI_OK) return rc;
+  RI_CUDA_OK(ri_launch_pdl_id(11, paged_decode_kernel<DT, BOX, WEIGHTS, false, LONG>, dim3(a.max_ctas), dim3(kPagedThreads), (size_t)kPagedSmem, s,
+                              map_k, map_v, a));
+  return RI_OK;
+}
 template <int DT, int BOX, bool WEIGHTS>
 int launch_steps(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, int ctas, cudaStream_t s) {
   int rc;
   if (ctas > 0) {
-    if ((rc = ri_allow_smem<paged_decode_kernel<DT, BOX, WEIGHTS, true>>(kPagedSmem)) != RI_OK) return rc;
-    RI_CUDA_OK(ri_launch_pdl_cluster(11, ctas, paged_decode_kernel<DT, BOX, WEIGHTS, true>, dim3(a.batch * a.hk * ctas), dim3(kPagedThreads),
+    if ((rc = ri_allow_smem<paged_decode_kernel<DT, BOX, WEIGHTS, true, false>>(kPagedSmem)) != RI_OK) return rc;
+    RI_CUDA_OK(ri_launch_pdl_cluster(11, ctas, paged_decode_kernel<DT, BOX, WEIGHTS, true, false>, dim3(a.batch * a.hk * ctas), dim3(kPagedThreads),
                                      (size_t)kPagedSmem, s, map_k, map_v, a));
     return RI_OK;
   }
-  if ((rc = ri_allow_smem<paged_decode_kernel<DT, BOX, WEIGHTS, false>>(kPagedSmem)) != RI_OK) return rc;
-  RI_CUDA_OK(ri_launch_pdl_id(11, paged_decode_kernel<DT, BOX, WEIGHTS, false>, dim3(a.max_ctas), dim3(kPagedThreads), (size_t)kPagedSmem, s,
-                              map_k, map_v, a));
-  return RI_OK;
+  const int64_t steps = (int64_t)a.batch * a.hk * ((((int64_t)a.width << a.shift) + 15) / 16);
+  return steps > (int64_t)a.max_ctas * kPagedWarps * kLongSteps ? launch_split<DT, BOX, WEIGHTS, true>(a, map_k, map_v, s)
+                                                                : launch_split<DT, BOX, WEIGHTS, false>(a, map_k, map_v, s);
 }
 template <int DT, int BOX>
 int launch_steps(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, int ctas, cudaStream_t s) {
