@@ -297,8 +297,7 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
         const int end = STATS ? min(hi, g_end) - lo : hi - max(lo, g_first);
         const int b = at.g / a.hk, h = at.g - b * a.hk;
         // the group's query rows, their pieces swizzled as TMA would; every product over the rows before has completed, since
-        // its scores have been read.  Rows that fill up a tile repeat the last one, with nothing to give: zeros would make NaN of
-        // an infinite key where no query does
+        // its scores have been read
         asm volatile("bar.sync 1, %0;" ::"n"(kScoreThreads) : "memory");
         {
           // a half-warp per row, eight rows of a thread on their way together
@@ -306,8 +305,9 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
           uint4 x[8];
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
-            const int r = a.first_row + min(u * 32 + (tid >> 4), a.rows - 1), w = r / a.gs;
-            x[u] = ri_ldg16(a.q + (((int64_t)b * a.window + w) * a.hk * a.gs + h * a.gs + r - w * a.gs) * 16 + piece);
+            const int i = u * 32 + (tid >> 4), r = a.first_row + i, w = r / a.gs;
+            x[u] = i < a.rows ? ri_ldg16(a.q + (((int64_t)b * a.window + w) * a.hk * a.gs + h * a.gs + r - w * a.gs) * 16 + piece)
+                              : make_uint4(0, 0, 0, 0);
           }
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
@@ -423,10 +423,15 @@ __global__ void __launch_bounds__(kObsThreads, 1) observe_kernel(const __grid_co
             const int chunks = (a.rows + 31) / 32, chunk0 = half ? (chunks + 1) / 2 : 0, my_chunks = half ? chunks / 2 : (chunks + 1) / 2;
             const uint32_t scores = tmem + g * 256 + chunk0 * 32 + t_lane;
             float sum = 0.f;
-            if (!ok) {                 // no scores to read, but the warp that shares the slots is still met below
-            } else if (!edge) {
+            // Where every row sees every slot, rows that fill up the last 32 give nothing by their shift of -infinity.  They are zeros,
+            // though, and make NaN of an infinite key: a sum that is NaN is done again without them.
+            bool masked = edge;
+            if (ok && !edge) {
               sum = column_sum(scores, my_chunks, a.scale2, s_neg_lse + chunk0 * 32);
-            } else {
+              masked = __any_sync(0xffffffffu, sum != sum);
+            }
+            if (ok && masked) {        // without `ok` there are no scores to read, but the warp that shares the slots is still met below
+              sum = 0.f;
 #pragma unroll 1
               for (int k = 0; k < my_chunks; ++k) {
                 uint32_t sr[32];
