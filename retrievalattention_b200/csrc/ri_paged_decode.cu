@@ -11,15 +11,17 @@
 // filled by TMA, a box of 16 rows (8 where a page has no more) of both halves of the channels; the number of the next
 // step's page is fetched a step ahead.  Layout in shared memory and the order of the keys in a step: as in ri_dense_decode.cu.
 // The probabilities enter the second product as two 16-bit parts: 16 bits of them with bf16, 22 with fp16, whose short exponent a
-// moving reference makes up for (see m_run).  Either is a hundredth of the output's own rounding.
+// moving reference makes up for (see m_run).  Either is a hundredth of the output's own rounding: 0.3 % of bf16 outputs are not the
+// ones that 32-bit probabilities give, but their neighbours.  A third part: 0.07 %, and 318 -> 330 us at 4 x 131072 slots.
 // A second kernel merges a group's partial results by log-sum-exp in a fixed order.  For the weights the first kernel
 // leaves the scores behind (4 bytes a slot and query head, against 512 a slot for K and V), and the second turns them into
 // probabilities; every slot has one thread, so the sums have one order and no atomics.
 // Short requests that leave the chip room give every group a cluster of CTAs, which does all of this in one kernel.
-// B200, bf16, 8 heads of 4: 4 x 131072 slots 340 us, 6.3 TB/s (a copy: 6.6); 4 requests of 20K to 32K with weights 91 us, 4.8 TB/s:
-// 3.4 us until the first rows are there, the SMs done after 57 to 76 us (40 of the 148 read an eighth slower, the same ones in
-// every run), 2 until the second kernel knows, 7 for it.  CTAs that take work from ones not launched yet ended together, but the
-// units that this takes have few steps a warp and many partial results: 340 -> 362 and 98 -> 108 us.
+// B200, bf16, 8 heads of 4: 4 x 131072 slots 318 to 345 us by the GPU, 6.2 to 6.8 TB/s (a copy: 6.6); 4 requests of 20K to 32K with
+// weights 91 us, 4.8 TB/s: the SMs are done after 64 to 78 us, half of them by 68 (some two dozen SMs are the last in every case,
+// whatever the page size, the lengths or the groups of a CTA; without the scores all are done 5 us earlier), and the second kernel
+// has 10.  CTAs that take work from ones not launched yet ended together, but the units that this takes have few steps a warp and
+// many partial results: 340 -> 362 and 98 -> 108 us.
 #include <cooperative_groups.h>
 
 #include "ri_paged.cuh"

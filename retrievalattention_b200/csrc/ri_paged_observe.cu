@@ -15,9 +15,9 @@
 // scores four warps take the first half of the columns and four the second.
 // TMEM: 256 columns of scores for each side.  Every wait is bounded; one that runs out is recorded in the
 // status word.
-// Bound by the exponentials, two for each slot and query row.  B200, 4 requests of 20K to 32K slots, 8 heads, 256 query rows: 171 us
-// in a repeated run, 2.5 of the 4.2 exponentials a picosecond that the SMs have at 16 a clock and 1.76 GHz; pass 1 takes 71 us
-// from rest (exponentials busy 79 % of the active cycles, tensor pipe 39 %), pass 2 82 (69 %: it also reads each row's lse).  With
+// Bound by the exponentials, two for each slot and query row.  B200, 4 requests of 20K to 32K slots, 8 heads, 256 query rows: 165 to 170 us
+// by the GPU in a repeated run, 2.5 of the 4.2 exponentials a picosecond that the SMs have at 16 a clock and 1.76 GHz; pass 1 takes 71 us
+// from rest (exponentials busy 79 % of the active cycles, tensor pipe 39 %), pass 2 82 (68 %: it also reads each row's lse).  With
 // eight score warps 188 us: two warps of a scheduler do not cover each other's loads and barriers.  Some of the exponentials as
 // polynomials on the FMA pipe gained nothing with either.
 #include <cuda.h>
@@ -57,7 +57,9 @@ struct ObsArgs : Pages {
   int mixed_halves;                              // pages of eight slots: the halves of eight keys lie behind one another
 };
 
-__device__ __forceinline__ float ex2(float x) {       // 2^x; results below 2^-126 become 0
+// 2^x to within 2^-22 of itself, as exp2f; results below 2^-126 become 0 (they are added to sums of 1 and more, or are weights that
+// no eviction tells from 0).  The weights come out within 1.5e-7 of 64 bits where 32-bit torch operations are within 1.0e-7.
+__device__ __forceinline__ float ex2(float x) {
   float d;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
   return d;
