@@ -66,6 +66,7 @@ class paged_cache(KV_Cache):
         self._pages = [[] for _ in range(batch_size)]
         self._evicted = [False] * batch_size                    # whose slots are no longer in the order of their tokens
         self._fed = [0] * batch_size                            # tokens of the step
+        self._weighed, self._weighing = set(), set()            # requests whose slots were given weights before this step, in it
         self._chosen = {}                                       # the step's tables and lengths, of all and of some requests
 
     def _to_device(self, values) -> torch.Tensor:
@@ -94,6 +95,8 @@ class paged_cache(KV_Cache):
             self.page_table.view(-1).index_copy_(0, both[0].long(), both[1])
         self.length_of = [n + more for n, more in zip(self.length_of, each)]
         self._fed, self._chosen = each, {}
+        self._weighed |= self._weighing
+        self._weighing = set()
         self.held.copy_(self.lengths)
         self.seen.copy_(self.seen_after)
         if same:
@@ -142,21 +145,25 @@ class paged_cache(KV_Cache):
         """Attention of one new token of every request, ``[batch, 1, heads, 128]``, over its slots (``paged.paged_decode``); with
         ``keep`` the slots' weights grow by what they are given.  ``requests``: of these alone, in the order of their queries."""
         table, lengths = self._of(requests)
+        if self.keep is not None:
+            self._weighing.update(range(self.batch_size) if requests is None else map(int, requests))
         return paged.paged_decode(query_states, self.key_pages[layer_idx], self.value_pages[layer_idx], table, lengths, out=out, lse=lse,
                                   weight=self.weight[layer_idx])
 
     def observe(self, query_states, layer_idx, requests=None) -> None:
         """Weights from the last queries ``[batch, window, heads, 128]`` of the step's prompts (``paged.paged_observe``).  ``requests``:
-        of these alone, in the order of their queries; without it every request must have had tokens in the step, or have none at all.
-        A request that was evicted from cannot be observed: its slots are not in the order of its tokens."""
+        of these alone, in the order of their queries; without it, requests without tokens in the step may not have been observed or
+        attended before.  A request that was evicted from cannot be observed: its slots are not in the order of its tokens."""
         if self.keep is None:
             return
         table, lengths = self._of(requests)
-        for b in range(self.batch_size) if requests is None else requests:
+        which = range(self.batch_size) if requests is None else [int(b) for b in requests]
+        for b in which:
             if self._evicted[b]:
                 raise RuntimeError(f"slots of request {b} were evicted: what its queries see is not known any more")
-            if requests is None and self.length_of[b] and not self._fed[b]:
+            if requests is None and not self._fed[b] and b in self._weighed and self.length_of[b]:
                 raise ValueError(f"request {b} had no tokens in this step: name the `requests` that are to be observed")
+        self._weighing.update(which)
         paged.paged_observe(query_states, self.key_pages[layer_idx], table, lengths, self.weight[layer_idx])
 
     def evict(self, slack: int | None = None) -> bool:
@@ -187,6 +194,8 @@ class paged_cache(KV_Cache):
         """Request ``bdx`` is done: its pages go back, and its place may take another one."""
         self._give_back(bdx, 0)
         self.length_of[bdx], self._evicted[bdx], self._fed[bdx], self._chosen = 0, False, 0, {}
+        self._weighed.discard(bdx)
+        self._weighing.discard(bdx)
         for x in (self.lengths, self.seen_after):
             x[bdx].zero_()
 

@@ -109,3 +109,19 @@ def test_steps_of_some_requests_in_their_order():
     for bad in ([], [0, 0], [4], [-1]):
         with pytest.raises(ValueError, match="different requests"):
             cache.attend(q, 0, requests=bad)
+
+
+def test_prompts_of_several_steps_are_observed_at_once():
+    """A request whose prompt ended a step before the others' is observed with them."""
+    cache, gen = make(2, keep=400), torch.Generator().manual_seed(7)
+    first = feed(cache, [70, 90], gen)[70:]
+    q = feed(cache, [50, 0], gen)
+    queries = torch.cat([last_queries(x, x.shape[0], 16) for x in (q, first)])
+    cache.observe(queries, 0)
+    cache.evict(slack=0)
+    for b in range(2):
+        want = given(cache, b, queries[b:b + 1])
+        assert ((slots(cache, cache.weight[0], b) - want).abs() <= 1e-4 * want + 1e-12).all()
+    feed(cache, [9, 0], gen)
+    with pytest.raises(ValueError, match="request 1 had no tokens"):
+        cache.observe(queries, 0)
