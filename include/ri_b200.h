@@ -222,6 +222,11 @@ int ri_rope_split(const void* d_qkv, const float* d_cos_sin, const int64_t* d_po
                   void* d_k, void* d_v, int32_t rows, int32_t q_heads, int32_t kv_heads,
                   int64_t max_positions, int32_t dtype, void* stream);
 
+/* The same behind an RMS norm of every query and key head, as ri_rope_paged_append_norm has it. */
+int ri_rope_split_norm(const void* d_qkv, const float* d_cos_sin, const int64_t* d_positions, const void* d_q_norm,
+                       const void* d_k_norm, int32_t q_norm_heads, int32_t k_norm_heads, float eps, void* d_q, void* d_k, void* d_v,
+                       int32_t rows, int32_t q_heads, int32_t kv_heads, int64_t max_positions, int32_t dtype, void* stream);
+
 /* out[r, j] = silu(in[r, j]) * in[r, inter + j].  Replaces flashinfer.activation.silu_and_mul
  * (model_hub/llama.py:267-275).  d_in: [rows, 2*inter]; d_out: [rows, inter]; inter a multiple of 8. */
 int ri_silu_and_mul(const void* d_in, void* d_out, int32_t rows, int32_t inter, int32_t dtype, void* stream);
@@ -364,6 +369,13 @@ typedef struct ri_paged {
 int ri_rope_paged_append(const ri_paged* p, const void* d_qkv, int64_t qkv_stride, const float* d_cos_sin, int64_t max_positions,
                          const int64_t* d_positions, const uint8_t* h_axis_of, int32_t axes, int32_t rows,
                          const int32_t* d_row_start, const int32_t* d_seen, void* d_q, void* d_k, void* d_v, void* stream);
+/* The same behind an RMS norm: every query and key head is first x_i <- x_i w_i / sqrt(mean x^2 + eps), in 32 bits, then rotated.
+ * d_q_norm: the weights w of the pools' type, 128 for all query heads (q_norm_heads 1) or 128 for each ([q_heads][128], q_norm_heads
+ * q_heads); d_k_norm and k_norm_heads likewise.  eps: not negative. */
+int ri_rope_paged_append_norm(const ri_paged* p, const void* d_qkv, int64_t qkv_stride, const float* d_cos_sin, int64_t max_positions,
+                              const int64_t* d_positions, const uint8_t* h_axis_of, int32_t axes, int32_t rows,
+                              const int32_t* d_row_start, const int32_t* d_seen, const void* d_q_norm, const void* d_k_norm,
+                              int32_t q_norm_heads, int32_t k_norm_heads, float eps, void* d_q, void* d_k, void* d_v, void* stream);
 /* Attention of one query row of every request and head over the slots in use: d_q [batch][kv_heads * group_size][128], requests
  * q_stride elements apart, group_size 1 to 8; d_out dense; d_lse [batch, q_heads] natural log-sum-exp of the scaled scores or
  * NULL.  A request without slots has out 0 and lse -infinity, as has a head all of whose scores are -infinity; a score that is NaN
@@ -373,6 +385,28 @@ int ri_rope_paged_append(const ri_paged* p, const void* d_qkv, int64_t qkv_strid
 int64_t ri_paged_decode_scratch_bytes(const ri_paged* p);
 int ri_paged_decode(const ri_paged* p, const void* d_q, int64_t q_stride, void* d_out, float* d_lse, float scale, void* d_scratch,
                     void* stream);
+/* The same where only the last `window` slots in use and the first `sink` are seen.  Steps of 16 slots that hold none of them are not read,
+ * nor are their page numbers.  Slots must be in the order of their tokens (no eviction before); d_weight must be NULL.  Scratch as for
+ * ri_paged_decode. */
+int ri_paged_decode_window(const ri_paged* p, const void* d_q, int64_t q_stride, int32_t window, int32_t sink, void* d_out, float* d_lse,
+                           float scale, void* d_scratch, void* stream);
+/* Attention of the last tokens in use, several of every request: d_q `rows` rows of kv_heads * group_size heads of 128, q_stride elements
+ * apart; rows d_row_start[b] .. d_row_start[b + 1] - 1 (ascending, within `rows`) are those of request b's last tokens, whose keys and values
+ * are in the cache.  The token at slot s sees the slots j <= s with j > s - window (window 0: all of them) or j < sink.  d_out [rows,
+ * q_heads, 128] and d_lse [rows, q_heads] (or NULL) as for ri_paged_decode; rows that belong to no request are left as they were, and
+ * a row in front of its request's first slot sees nothing.  group_size 1 to 8, batch at most 16384.  Slots must be in the order of their
+ * tokens.  Pages that no row sees are not read, nor are their numbers.  d_scratch: that many bytes of 16-byte aligned device memory
+ * (0: none, it may be NULL), any contents, for this call alone. */
+int64_t ri_paged_prompt_scratch_bytes(const ri_paged* p, int32_t rows, int32_t window, int32_t sink);
+int ri_paged_prompt(const ri_paged* p, const void* d_q, int64_t q_stride, int32_t rows, const int32_t* d_row_start, int32_t window,
+                    int32_t sink, void* d_out, float* d_lse, float scale, void* d_scratch, void* stream);
+/* ri_paged_decode where requests have their first slots in common, which are read once for all of them: requests d_group_start[g] ..
+ * d_group_start[g + 1] - 1 (ascending; int32 [groups + 1]) have the first d_shared[g] slots in common, which are read through the
+ * first one's row of the page table; requests in no group have none.  A request shorter than that sees what it has.  batch + groups at
+ * most 16384.  d_weight is not used. */
+int64_t ri_paged_shared_decode_scratch_bytes(const ri_paged* p, int32_t groups);
+int ri_paged_shared_decode(const ri_paged* p, const void* d_q, int64_t q_stride, const int32_t* d_group_start, int32_t groups,
+                           const int32_t* d_shared, void* d_out, float* d_lse, float scale, void* d_scratch, void* stream);
 /* The weight that the last `window` queries of every request give to its slots: d_q [batch][window][q_heads][128]; query w sees
  * the slots up to d_lengths[b] - window + w (one that sees none, of a request shorter than the window, may hold anything and
  * gives nothing); every slot's weight grows by the sum of its probabilities over queries and heads of its group.  A query all of

@@ -148,6 +148,22 @@ def _load() -> C.CDLL:
     lib.ri_rope_paged_append.restype = C.c_int
     lib.ri_rope_paged_append.argtypes = [C.POINTER(Paged), C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_char_p,
                                          C.c_int32, C.c_int32] + [C.c_void_p] * 6
+    lib.ri_rope_paged_append_norm.restype = C.c_int
+    lib.ri_rope_paged_append_norm.argtypes = [C.POINTER(Paged), C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_char_p,
+                                              C.c_int32, C.c_int32] + [C.c_void_p] * 4 + [C.c_int32, C.c_int32, C.c_float] + [C.c_void_p] * 4
+    lib.ri_paged_decode_window.restype = C.c_int
+    lib.ri_paged_decode_window.argtypes = [C.POINTER(Paged), C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_float,
+                                           C.c_void_p, C.c_void_p]
+    lib.ri_paged_prompt_scratch_bytes.restype = C.c_int64
+    lib.ri_paged_prompt_scratch_bytes.argtypes = [C.POINTER(Paged)] + [C.c_int32] * 3
+    lib.ri_paged_prompt.restype = C.c_int
+    lib.ri_paged_prompt.argtypes = [C.POINTER(Paged), C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p,
+                                    C.c_void_p, C.c_float, C.c_void_p, C.c_void_p]
+    lib.ri_paged_shared_decode_scratch_bytes.restype = C.c_int64
+    lib.ri_paged_shared_decode_scratch_bytes.argtypes = [C.POINTER(Paged), C.c_int32]
+    lib.ri_paged_shared_decode.restype = C.c_int
+    lib.ri_paged_shared_decode.argtypes = [C.POINTER(Paged), C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                           C.c_float, C.c_void_p, C.c_void_p]
     lib.ri_paged_decode_scratch_bytes.restype = C.c_int64
     lib.ri_paged_decode_scratch_bytes.argtypes = [C.POINTER(Paged)]
     lib.ri_paged_decode.restype = C.c_int
@@ -178,6 +194,9 @@ def _load() -> C.CDLL:
     lib.ri_rmsnorm.argtypes = [C.c_void_p] * 4 + [C.c_int32, C.c_int32, C.c_float, C.c_int32, C.c_void_p]
     lib.ri_rope_split.restype = C.c_int
     lib.ri_rope_split.argtypes = [C.c_void_p] * 6 + [C.c_int32, C.c_int32, C.c_int32, C.c_int64, C.c_int32, C.c_void_p]
+    lib.ri_rope_split_norm.restype = C.c_int
+    lib.ri_rope_split_norm.argtypes = ([C.c_void_p] * 5 + [C.c_int32, C.c_int32, C.c_float] + [C.c_void_p] * 3 + [C.c_int32] * 3 +
+                                       [C.c_int64, C.c_int32, C.c_void_p])
     lib.ri_silu_and_mul.restype = C.c_int
     lib.ri_silu_and_mul.argtypes = [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p]
     lib.ri_prefill_attn_scratch_bytes.restype = C.c_int64

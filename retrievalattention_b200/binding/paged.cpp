@@ -10,9 +10,11 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <climits>
 #include <optional>
 #include <string>
+#include <tuple>
 
 #include "ri_b200.h"
 
@@ -27,8 +29,14 @@ constexpr int64_t kDim = RI_HEAD_DIM;
 struct Library {
   decltype(&ri_last_error) last_error = nullptr;
   decltype(&ri_rope_paged_append) append = nullptr;
+  decltype(&ri_rope_paged_append_norm) append_norm = nullptr;
   decltype(&ri_paged_decode_scratch_bytes) decode_bytes = nullptr;
   decltype(&ri_paged_decode) decode = nullptr;
+  decltype(&ri_paged_decode_window) decode_window = nullptr;
+  decltype(&ri_paged_prompt_scratch_bytes) prompt_bytes = nullptr;
+  decltype(&ri_paged_prompt) prompt = nullptr;
+  decltype(&ri_paged_shared_decode_scratch_bytes) shared_bytes = nullptr;
+  decltype(&ri_paged_shared_decode) shared = nullptr;
   decltype(&ri_paged_observe_scratch_bytes) observe_bytes = nullptr;
   decltype(&ri_paged_observe) observe = nullptr;
   decltype(&ri_paged_evict_scratch_bytes) evict_bytes = nullptr;
@@ -147,7 +155,7 @@ Tensor workspace(int64_t bytes, const Tensor& like, const char* what) {
 void append(const Tensor& qkv, const Tensor& cos_sin, const Tensor& positions, const py::bytes& axis_of, const Tensor& q,
             const Tensor& key_pages, const OptTensor& value_pages, const Tensor& page_table, const Tensor& lengths,
             const OptTensor& row_start, const OptTensor& weight, const OptTensor& token, const OptTensor& seen, const OptTensor& keys,
-            const OptTensor& values) {
+            const OptTensor& values, const OptTensor& q_norm, const OptTensor& k_norm, double eps) {
   const char* what = "rope_paged_append";
   const int64_t heads = key_pages.dim() == 4 ? key_pages.size(1) : 0;
   if (qkv.dim() != 2 || q.dim() != 3 || heads < 1 || q.size(1) < heads || q.size(1) % heads)
@@ -179,20 +187,45 @@ void append(const Tensor& qkv, const Tensor& cos_sin, const Tensor& positions, c
   if (given(row_start) && !dense(*row_start, {p.batch + 1}, at::kInt, device)) fail(what, "expected dense int32 row_start [batch + 1]");
   if (given(seen) && !dense(*seen, {p.batch}, at::kInt, device)) fail(what, "expected dense int32 seen [batch]");
   if (given(token) && !given(seen)) fail(what, "token numbers need `seen`");
+  if (given(q_norm) != given(k_norm)) fail(what, "q_norm and k_norm come together");
+  const bool norm = given(q_norm);
+  if (norm) {
+    for (const auto& [w, of_heads, name] : {std::tuple{&*q_norm, q_heads, "q_norm"}, std::tuple{&*k_norm, heads, "k_norm"}})
+      if (!dense(*w, {kDim}, type, device) && !dense(*w, {of_heads, kDim}, type, device))
+        fail(what, std::string("expected dense ") + name + " [128] or [heads, 128] of the pages' type on their GPU");
+    if (q_norm->requires_grad() || k_norm->requires_grad()) fail(what, "there are no gradients");
+    if (!(eps >= 0 && eps < 1e30)) fail(what, "eps must be finite and not negative");
+  }
   if (rows == 0) return;
   const OnDevice on(key_pages);
-  check(lib.append(&p, qkv.data_ptr(), rows > 1 ? qkv.stride(0) : qkv.size(1), static_cast<const float*>(cos_sin.data_ptr()),
-                   cos_sin.size(0), static_cast<const int64_t*>(positions.data_ptr()), reinterpret_cast<const uint8_t*>(of), (int32_t)axes,
-                   (int32_t)rows, static_cast<const int32_t*>(address(row_start)), static_cast<const int32_t*>(address(seen)),
-                   q.data_ptr(), address(keys), address(values), on.stream()), what);
+  const int64_t stride = rows > 1 ? qkv.stride(0) : qkv.size(1);
+  const float* angles = static_cast<const float*>(cos_sin.data_ptr());
+  const int64_t* where = static_cast<const int64_t*>(positions.data_ptr());
+  const uint8_t* axis = reinterpret_cast<const uint8_t*>(of);
+  const int32_t *starts = static_cast<const int32_t*>(address(row_start)), *before = static_cast<const int32_t*>(address(seen));
+  if (norm)
+    check(lib.append_norm(&p, qkv.data_ptr(), stride, angles, cos_sin.size(0), where, axis, (int32_t)axes, (int32_t)rows, starts, before,
+                          q_norm->data_ptr(), k_norm->data_ptr(), q_norm->dim() == 2 ? (int32_t)q_heads : 1,
+                          k_norm->dim() == 2 ? (int32_t)heads : 1, (float)eps, q.data_ptr(), address(keys), address(values), on.stream()), what);
+  else
+    check(lib.append(&p, qkv.data_ptr(), stride, angles, cos_sin.size(0), where, axis, (int32_t)axes, (int32_t)rows, starts, before,
+                     q.data_ptr(), address(keys), address(values), on.stream()), what);
   touched(q);
   touched(key_pages);
   for (const OptTensor* x : {&value_pages, &weight, &token, &keys, &values}) touched(*x);
   done(key_pages);
 }
 
+// Slots of a window, 0: no window.  More than a cache has room for are all of them.
+int32_t slots(const char* what, const std::optional<int64_t>& window, const char* name, int64_t least) {
+  if (!window.has_value()) return 0;
+  if (*window < least) fail(what, std::string(name) + "=" + std::to_string(*window) + " slots");
+  return (int32_t)std::min<int64_t>(*window, 1 << 30);
+}
+
 Tensor decode(const Tensor& q, const Tensor& key_pages, const OptTensor& value_pages, const Tensor& page_table, const Tensor& lengths,
-              const OptTensor& given_out, const OptTensor& lse, const OptTensor& weight, double scale) {
+              const OptTensor& given_out, const OptTensor& lse, const OptTensor& weight, double scale, const std::optional<int64_t>& window,
+              int64_t sink) {
   const char* what = "paged_decode";
   if (q.dim() != 4 || key_pages.dim() != 4 || page_table.dim() != 2 || !given(value_pages))
     fail(what, "expected q [batch, 1, q_heads, 128] and pages [pages, kv_heads, page_size, 128]");
@@ -202,6 +235,8 @@ Tensor decode(const Tensor& q, const Tensor& key_pages, const OptTensor& value_p
   if (!dense_rows(q, 1)) fail(what, "the heads of a request must lie dense in q");
   if (q.scalar_type() != key_pages.scalar_type() || q.device() != key_pages.device() || q.requires_grad())
     fail(what, "expected q and the pages of one type on one GPU, without gradients");
+  const int32_t last = slots(what, window, "window", 1), first = slots(what, sink, "sink", 0);
+  if (last > 0 && given(weight)) fail(what, "weights are added up over all slots, not over a window");
   const ri_paged p = describe(what, key_pages, value_pages, page_table, lengths, weight, std::nullopt, q_heads / heads);
   if (given(given_out) && (!dense(*given_out, q.sizes(), q.scalar_type(), q.device()) || given_out->requires_grad()))
     fail(what, "expected dense out like q");
@@ -210,11 +245,81 @@ Tensor decode(const Tensor& q, const Tensor& key_pages, const OptTensor& value_p
   const OnDevice on(key_pages);
   const Tensor out = given(given_out) ? *given_out : at::empty(q.sizes(), q.options());
   const Tensor scratch = workspace(lib.decode_bytes(&p), q, what);
-  check(lib.decode(&p, q.data_ptr(), batch > 1 ? q.stride(0) : q_heads * kDim, out.data_ptr(), static_cast<float*>(address(lse)),
-                   (float)scale, scratch.data_ptr(), on.stream()), what);
+  const int64_t stride = batch > 1 ? q.stride(0) : q_heads * kDim;
+  float* sums = static_cast<float*>(address(lse));
+  check(last > 0 ? lib.decode_window(&p, q.data_ptr(), stride, last, first, out.data_ptr(), sums, (float)scale, scratch.data_ptr(), on.stream())
+                 : lib.decode(&p, q.data_ptr(), stride, out.data_ptr(), sums, (float)scale, scratch.data_ptr(), on.stream()), what);
   touched(given_out);
   touched(lse);
   touched(weight);
+  done(key_pages);
+  return out;
+}
+
+Tensor prompt(const Tensor& q, const Tensor& key_pages, const OptTensor& value_pages, const Tensor& page_table, const Tensor& lengths,
+              const Tensor& row_start, const std::optional<int64_t>& window, int64_t sink, const OptTensor& given_out, const OptTensor& lse,
+              double scale) {
+  const char* what = "paged_prompt";
+  const int64_t heads = key_pages.dim() == 4 ? key_pages.size(1) : 0;
+  if (q.dim() != 3 || heads < 1 || !given(value_pages)) fail(what, "expected q [rows, q_heads, 128] and pages [pages, kv_heads, page_size, 128]");
+  const int64_t rows = q.size(0), q_heads = q.size(1);
+  if (q.size(2) != kDim || q_heads < heads || q_heads % heads || q_heads / heads > 8)
+    fail(what, "expected q [rows, q_heads, 128], one to eight query heads to a KV head");
+  if (!dense_rows(q, 1)) fail(what, "the heads of a row must lie dense in q");
+  if (q.scalar_type() != key_pages.scalar_type() || q.device() != key_pages.device() || q.requires_grad())
+    fail(what, "expected q and the pages of one type on one GPU, without gradients");
+  if (rows > INT_MAX) fail(what, "too large");
+  const int32_t last = slots(what, window, "window", 1), first = slots(what, sink, "sink", 0);
+  const ri_paged p = describe(what, key_pages, value_pages, page_table, lengths, std::nullopt, std::nullopt, q_heads / heads);
+  if (!dense(row_start, {p.batch + 1}, at::kInt, q.device())) fail(what, "expected dense int32 row_start [batch + 1] on the pools' GPU");
+  if (given(given_out) && (!dense(*given_out, q.sizes(), q.scalar_type(), q.device()) || given_out->requires_grad()))
+    fail(what, "expected dense out like q");
+  if (given(lse) && (!dense(*lse, {rows, q_heads}, at::kFloat, q.device()) || lse->requires_grad()))
+    fail(what, "expected dense fp32 lse [rows, q_heads]");
+  const OnDevice on(key_pages);
+  const Tensor out = given(given_out) ? *given_out : at::empty(q.sizes(), q.options());
+  if (rows == 0) return out;
+  const int64_t bytes = lib.prompt_bytes(&p, (int32_t)rows, last, first);
+  const Tensor scratch = workspace(bytes, q, what);
+  check(lib.prompt(&p, q.data_ptr(), rows > 1 ? q.stride(0) : q_heads * kDim, (int32_t)rows, static_cast<const int32_t*>(row_start.data_ptr()),
+                   last, first, out.data_ptr(), static_cast<float*>(address(lse)), (float)scale, bytes > 0 ? scratch.data_ptr() : nullptr,
+                   on.stream()), what);
+  touched(given_out);
+  touched(lse);
+  done(key_pages);
+  return out;
+}
+
+Tensor shared_decode(const Tensor& q, const Tensor& key_pages, const OptTensor& value_pages, const Tensor& page_table,
+                     const Tensor& lengths, const Tensor& group_start, const Tensor& shared, const OptTensor& given_out,
+                     const OptTensor& lse, double scale) {
+  const char* what = "paged_shared_decode";
+  if (q.dim() != 4 || key_pages.dim() != 4 || page_table.dim() != 2 || !given(value_pages))
+    fail(what, "expected q [batch, 1, q_heads, 128] and pages [pages, kv_heads, page_size, 128]");
+  const int64_t batch = q.size(0), q_heads = q.size(2), heads = key_pages.size(1);
+  if (q.size(1) != 1 || q.size(3) != kDim || heads < 1 || q_heads < heads || q_heads % heads || q_heads / heads > 8 ||
+      page_table.size(0) != batch)
+    fail(what, "expected q [batch, 1, q_heads, 128], one to eight query heads to a KV head, one page table row per request");
+  if (!dense_rows(q, 1)) fail(what, "the heads of a request must lie dense in q");
+  if (q.scalar_type() != key_pages.scalar_type() || q.device() != key_pages.device() || q.requires_grad())
+    fail(what, "expected q and the pages of one type on one GPU, without gradients");
+  const ri_paged p = describe(what, key_pages, value_pages, page_table, lengths, std::nullopt, std::nullopt, q_heads / heads);
+  if (shared.dim() != 1 || shared.size(0) < 1 || shared.size(0) > batch || !dense(shared, {shared.size(0)}, at::kInt, q.device()) ||
+      !dense(group_start, {shared.size(0) + 1}, at::kInt, q.device()))
+    fail(what, "expected dense int32 group_start [groups + 1] and shared [groups] on the pools' GPU, one to `batch` groups");
+  if (given(given_out) && (!dense(*given_out, q.sizes(), q.scalar_type(), q.device()) || given_out->requires_grad()))
+    fail(what, "expected dense out like q");
+  if (given(lse) && (!dense(*lse, {batch, q_heads}, at::kFloat, q.device()) || lse->requires_grad()))
+    fail(what, "expected dense fp32 lse [batch, q_heads]");
+  const OnDevice on(key_pages);
+  const Tensor out = given(given_out) ? *given_out : at::empty(q.sizes(), q.options());
+  const int32_t groups = (int32_t)shared.size(0);
+  const Tensor scratch = workspace(lib.shared_bytes(&p, groups), q, what);
+  check(lib.shared(&p, q.data_ptr(), batch > 1 ? q.stride(0) : q_heads * kDim, static_cast<const int32_t*>(group_start.data_ptr()), groups,
+                   static_cast<const int32_t*>(shared.data_ptr()), out.data_ptr(), static_cast<float*>(address(lse)), (float)scale,
+                   scratch.data_ptr(), on.stream()), what);
+  touched(given_out);
+  touched(lse);
   done(key_pages);
   return out;
 }
@@ -262,8 +367,14 @@ void connect(const py::dict& addresses, const py::object& first_use, const py::o
   };
   take("ri_last_error", lib.last_error);
   take("ri_rope_paged_append", lib.append);
+  take("ri_rope_paged_append_norm", lib.append_norm);
   take("ri_paged_decode_scratch_bytes", lib.decode_bytes);
   take("ri_paged_decode", lib.decode);
+  take("ri_paged_decode_window", lib.decode_window);
+  take("ri_paged_prompt_scratch_bytes", lib.prompt_bytes);
+  take("ri_paged_prompt", lib.prompt);
+  take("ri_paged_shared_decode_scratch_bytes", lib.shared_bytes);
+  take("ri_paged_shared_decode", lib.shared);
   take("ri_paged_observe_scratch_bytes", lib.observe_bytes);
   take("ri_paged_observe", lib.observe);
   take("ri_paged_evict_scratch_bytes", lib.evict_bytes);
@@ -277,8 +388,14 @@ void connect(const py::dict& addresses, const py::object& first_use, const py::o
 
 PYBIND11_MODULE(_paged_binding, m) {
   m.def("connect", &connect);
-  m.def("append", &append);
-  m.def("decode", &decode);
+  m.def("append", &append, py::arg("qkv"), py::arg("cos_sin"), py::arg("positions"), py::arg("axis_of"), py::arg("q"), py::arg("key_pages"),
+        py::arg("value_pages"), py::arg("page_table"), py::arg("lengths"), py::arg("row_start"), py::arg("weight"), py::arg("token"),
+        py::arg("seen"), py::arg("keys"), py::arg("values"), py::arg("q_norm") = py::none(), py::arg("k_norm") = py::none(),
+        py::arg("eps") = 1e-6);
+  m.def("decode", &decode, py::arg("q"), py::arg("key_pages"), py::arg("value_pages"), py::arg("page_table"), py::arg("lengths"),
+        py::arg("out"), py::arg("lse"), py::arg("weight"), py::arg("scale"), py::arg("window") = py::none(), py::arg("sink") = 0);
+  m.def("prompt", &prompt);
+  m.def("shared_decode", &shared_decode);
   m.def("observe", &observe);
   m.def("evict", &evict);
 }

@@ -89,10 +89,17 @@ __global__ void __launch_bounds__(kNormThreads) rmsnorm_kernel(const uint4* __re
 // first half when t < 8, of the second half otherwise, and reads its partner piece from the other
 // half (neox pairing: element j with element j + 64).  cos_sin: fp32 [positions, 128], cosines in
 // the first 64 columns, sines in the last 64, as the reference builds it (model_hub/llama.py:81-84, :109).
-template <int DT>
+// NORM: query and key heads are first x_i <- x_i w_i / sqrt(mean x^2 + eps); `q_norm` and `k_norm` step by 0 or 16 pieces a head.
+struct HeadNorms {
+  const uint4* q;
+  const uint4* k;
+  int q_stride, k_stride;
+  float eps;
+};
+template <int DT, bool NORM>
 __global__ void __launch_bounds__(16) rope_split_kernel(const uint4* __restrict__ qkv, const float4* __restrict__ cos_sin,
                                                         const int64_t* __restrict__ positions, uint4* q, uint4* k, uint4* v,
-                                                        int q_heads, int kv_heads, int64_t max_positions) {
+                                                        int q_heads, int kv_heads, int64_t max_positions, HeadNorms norm) {
   ri_pdl_enter();
   const int row = blockIdx.x, head = blockIdx.y, t = threadIdx.x;
   const int heads = q_heads + 2 * kv_heads;
@@ -113,6 +120,22 @@ __global__ void __launch_bounds__(16) rope_split_kernel(const uint4* __restrict_
   float a[8], b[8], o[8];
   unpack8<DT>(mine, a);
   unpack8<DT>(other, b);
+  if (NORM) {
+    const uint4* w = head < q_heads ? norm.q + head * norm.q_stride : norm.k + (head - q_heads) * norm.k_stride;
+    float sum = 0.f, wa[8], wb[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += a[i] * a[i];
+#pragma unroll
+    for (int s = 8; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffu, sum, s);
+    const float inv = rsqrtf(sum * (1.f / RI_HEAD_DIM) + norm.eps);
+    unpack8<DT>(w[t], wa);
+    unpack8<DT>(w[t ^ 8], wb);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      a[i] = a[i] * inv * wa[i];
+      b[i] = b[i] * inv * wb[i];
+    }
+  }
   const float sign = t < 8 ? -1.f : 1.f;   // first half: x1*cos - x2*sin; second half: x2*cos + x1*sin
 #pragma unroll
   for (int i = 0; i < 8; ++i) o[i] = a[i] * cs[i] + sign * b[i] * sn[i];
@@ -134,6 +157,26 @@ __global__ void __launch_bounds__(256) silu_and_mul_kernel(const uint4* __restri
 #pragma unroll
   for (int j = 0; j < 8; ++j) o[j] = g[j] / (1.f + __expf(-g[j])) * u[j];
   out[i] = pack8<DT>(o);
+}
+
+template <bool NORM>
+int rope_split(const char* what, const void* d_qkv, const float* d_cos_sin, const int64_t* d_positions, void* d_q, void* d_k, void* d_v,
+               int32_t rows, int32_t q_heads, int32_t kv_heads, int64_t max_positions, HeadNorms norm, int32_t dtype, void* stream) {
+  RI_REQUIRE(d_qkv && d_cos_sin && d_positions && d_q && d_k && d_v, "%s: null pointer", what);
+  RI_REQUIRE(rows >= 1 && q_heads >= 1 && kv_heads >= 1 && q_heads + 2 * kv_heads <= 65535 && max_positions >= 1,
+             "%s: bad sizes", what);
+  RI_REQUIRE(dtype == RI_BF16 || dtype == RI_F16, "dtype=%d unsupported", dtype);
+  RI_REQUIRE(((uintptr_t)d_qkv | (uintptr_t)d_cos_sin | (uintptr_t)d_q | (uintptr_t)d_k | (uintptr_t)d_v) % 16 == 0,
+             "%s: pointers must be 16-byte aligned", what);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const dim3 grid(rows, q_heads + 2 * kv_heads);
+  auto go = [&](auto kernel) {
+    return ri_launch_pdl_id(8, kernel, grid, dim3(16), 0, s, static_cast<const uint4*>(d_qkv),
+                            reinterpret_cast<const float4*>(d_cos_sin), d_positions, static_cast<uint4*>(d_q),
+                            static_cast<uint4*>(d_k), static_cast<uint4*>(d_v), q_heads, kv_heads, max_positions, norm);
+  };
+  RI_CUDA_OK(dtype == RI_BF16 ? go(rope_split_kernel<RI_BF16, NORM>) : go(rope_split_kernel<RI_F16, NORM>));
+  return RI_OK;
 }
 
 }  // namespace
@@ -159,21 +202,23 @@ extern "C" int ri_rmsnorm(const void* d_x, void* d_residual, const void* d_weigh
 extern "C" int ri_rope_split(const void* d_qkv, const float* d_cos_sin, const int64_t* d_positions, void* d_q, void* d_k,
                              void* d_v, int32_t rows, int32_t q_heads, int32_t kv_heads, int64_t max_positions,
                              int32_t dtype, void* stream) {
-  RI_REQUIRE(d_qkv && d_cos_sin && d_positions && d_q && d_k && d_v, "ri_rope_split: null pointer");
-  RI_REQUIRE(rows >= 1 && q_heads >= 1 && kv_heads >= 1 && q_heads + 2 * kv_heads <= 65535 && max_positions >= 1,
-             "ri_rope_split: bad sizes");
-  RI_REQUIRE(dtype == RI_BF16 || dtype == RI_F16, "dtype=%d unsupported", dtype);
-  RI_REQUIRE(((uintptr_t)d_qkv | (uintptr_t)d_cos_sin | (uintptr_t)d_q | (uintptr_t)d_k | (uintptr_t)d_v) % 16 == 0,
-             "ri_rope_split: pointers must be 16-byte aligned");
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const dim3 grid(rows, q_heads + 2 * kv_heads);
-  auto go = [&](auto kernel) {
-    return ri_launch_pdl_id(8, kernel, grid, dim3(16), 0, s, static_cast<const uint4*>(d_qkv),
-                            reinterpret_cast<const float4*>(d_cos_sin), d_positions, static_cast<uint4*>(d_q),
-                            static_cast<uint4*>(d_k), static_cast<uint4*>(d_v), q_heads, kv_heads, max_positions);
-  };
-  RI_CUDA_OK(dtype == RI_BF16 ? go(rope_split_kernel<RI_BF16>) : go(rope_split_kernel<RI_F16>));
-  return RI_OK;
+  return rope_split<false>("ri_rope_split", d_qkv, d_cos_sin, d_positions, d_q, d_k, d_v, rows, q_heads, kv_heads, max_positions, {},
+                           dtype, stream);
+}
+
+extern "C" int ri_rope_split_norm(const void* d_qkv, const float* d_cos_sin, const int64_t* d_positions, const void* d_q_norm,
+                                  const void* d_k_norm, int32_t q_norm_heads, int32_t k_norm_heads, float eps, void* d_q, void* d_k,
+                                  void* d_v, int32_t rows, int32_t q_heads, int32_t kv_heads, int64_t max_positions, int32_t dtype,
+                                  void* stream) {
+  RI_REQUIRE(d_q_norm && d_k_norm, "ri_rope_split_norm: null pointer");
+  RI_REQUIRE(((uintptr_t)d_q_norm | (uintptr_t)d_k_norm) % 16 == 0, "ri_rope_split_norm: pointers must be 16-byte aligned");
+  RI_REQUIRE((q_norm_heads == 1 || q_norm_heads == q_heads) && (k_norm_heads == 1 || k_norm_heads == kv_heads),
+             "ri_rope_split_norm: weights of %d and %d heads for %d and %d", q_norm_heads, k_norm_heads, q_heads, kv_heads);
+  RI_REQUIRE(eps >= 0.f && eps < 1e30f, "ri_rope_split_norm: eps must be finite and not negative");
+  const HeadNorms norm = {static_cast<const uint4*>(d_q_norm), static_cast<const uint4*>(d_k_norm), q_norm_heads > 1 ? 16 : 0,
+                          k_norm_heads > 1 ? 16 : 0, eps};
+  return rope_split<true>("ri_rope_split_norm", d_qkv, d_cos_sin, d_positions, d_q, d_k, d_v, rows, q_heads, kv_heads, max_positions,
+                          norm, dtype, stream);
 }
 
 extern "C" int ri_silu_and_mul(const void* d_in, void* d_out, int32_t rows, int32_t inter, int32_t dtype, void* stream) {

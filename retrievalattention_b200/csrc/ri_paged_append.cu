@@ -2,6 +2,8 @@
 //   for i < 64, (c, s) the table's row at the row's position on axis axis_of[i], columns i and 64 + i:
 //     x'_i = x_i c - x_{i+64} s,    x'_{i+64} = x_{i+64} c + x_i s          (query and key heads; values as they are)
 // One axis is the ordinary rotary embedding; text, images and video take (time, height, width).
+// With norms a query or key head is first  x_i <- x_i w_i / sqrt(mean x^2 + eps),  in 32 bits up to the one rounding behind the rotation;
+// the half-warp that has a head has its sum of squares in four shuffles.
 // (reference: model_hub/llama.py:232-235 the split, :312-320 the rotation; cache_hub/flash_attn_cache.py:133-151 the append)
 //
 // Bound by the projection, read once and written once.  A row of it lies in one piece and comes in by one bulk copy, three rows
@@ -51,6 +53,10 @@ struct AppendArgs {
   int64_t max_positions;
   int rows, hq;
   int unit_rows, unit_heads, units_per_row;      // a unit: that many rows, of each that many heads
+  const uint4* q_norm;          // [16 pieces] or [heads][16]: the strides say which
+  const uint4* k_norm;
+  int q_norm_stride, k_norm_stride;              // pieces from head to head: 0 or 16
+  float eps;
   AxisOf axis;
 };
 
@@ -69,6 +75,41 @@ __device__ __forceinline__ uint4 rotate(const uint4& mine, const uint4& other, c
     o[i] = Elem<DT>::pack2(r[0], r[1]);
   }
   return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// The same behind an RMS norm: `inv` is one over the head's root mean square, w and v the weights of the two pieces.
+template <int DT>
+__device__ __forceinline__ uint4 rotate_normed(const uint4& mine, const uint4& other, const uint4& w_mine, const uint4& w_other, float inv,
+                                               const float* cs, float sign) {
+  const uint32_t a[4] = {mine.x, mine.y, mine.z, mine.w}, b[4] = {other.x, other.y, other.z, other.w};
+  const uint32_t w[4] = {w_mine.x, w_mine.y, w_mine.z, w_mine.w}, v[4] = {w_other.x, w_other.y, w_other.z, w_other.w};
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float r[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      auto part = [&](const uint32_t (&p)[4]) { return Elem<DT>::from_bits((uint16_t)(p[i] >> (16 * e))); };
+      const float x = part(a) * inv * part(w), y = part(b) * inv * part(v);
+      r[e] = x * cs[2 * i + e] + sign * y * cs[8 + 2 * i + e];
+    }
+    o[i] = Elem<DT>::pack2(r[0], r[1]);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+// Sum of the squares of a head, whose sixteen pieces lie in the lanes of a half-warp.
+template <int DT>
+__device__ __forceinline__ float head_squares(const uint4& mine, unsigned half_warp) {
+  const uint32_t a[4] = {mine.x, mine.y, mine.z, mine.w};
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float x = Elem<DT>::from_bits((uint16_t)(a[i] & 0xffffu)), y = Elem<DT>::from_bits((uint16_t)(a[i] >> 16));
+    sum += x * x + y * y;
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(half_warp, sum, o);
+  return sum;
 }
 
 // What a row needs beside its pieces, fetched by a service warp.
@@ -135,8 +176,8 @@ __device__ __forceinline__ void plan_rows(const AppendArgs& a, int row0, int n, 
 }
 
 // Work goes by units: an equal part of a row's heads where there are more than kUnitHeads, else a row or a few.
-// ROWS: rows of a unit, at most.
-template <int DT, int ROWS>
+// ROWS: rows of a unit, at most.  NORM: query and key heads are normalised before they are rotated.
+template <int DT, int ROWS, bool NORM>
 __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) rope_append_kernel(const __grid_constant__ AppendArgs a) {
   extern __shared__ __align__(128) uint8_t s_rows[];       // [kStages][unit_heads * 256]
   __shared__ RowPlan s_plan[kStages][ROWS];
@@ -183,6 +224,7 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) rope_append_kerne
         mbar_wait(smem_u32(&s_full[j % kStages]), (j / kStages) & 1, abort_flag, 92);
   } else {
     const int c = tid & 15, half = tid >> 4;
+    const unsigned half_warp = 0xffffu << (lane & 16);
     const float sign = c < 8 ? -1.f : 1.f;
     for (int i = 0; ok && i < mine; ++i) {
       const int s = i % kStages, u = u_lo + i, row0 = ROWS == 1 ? u / a.units_per_row : u * unit_rows;
@@ -216,7 +258,17 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) rope_append_kerne
         }
         const int row = row0 + r, head = head0 + j - r * n, h = head - a.hq, hv = h - p.hk;
         const uint4 x = src[j * 16 + c];
-        const uint4 res = hv >= 0 ? x : rotate<DT>(x, src[j * 16 + (c ^ 8)], cs, sign);
+        uint4 res = x;
+        if (hv < 0) {
+          const uint4 other = src[j * 16 + (c ^ 8)];
+          if (NORM) {
+            const uint4* w = h < 0 ? a.q_norm + head * a.q_norm_stride : a.k_norm + h * a.k_norm_stride;
+            const float inv = rsqrtf(head_squares<DT>(x, half_warp) * (1.f / RI_HEAD_DIM) + a.eps);
+            res = rotate_normed<DT>(x, other, ri_ldg16(w + c), ri_ldg16(w + (c ^ 8)), inv, cs, sign);
+          } else {
+            res = rotate<DT>(x, other, cs, sign);
+          }
+        }
         if (h < 0) {
           a.q[((int64_t)row * a.hq + head) * 16 + c] = res;
         } else {
@@ -236,27 +288,43 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) rope_append_kerne
   if (!ok && lane == 0) *p.status = s_abort;
 }
 
-}  // namespace
+template <int DT, int ROWS, bool NORM>
+int launch_kernel(const AppendArgs& a, dim3 grid, size_t smem, cudaStream_t s) {
+  const int rc = ri_allow_smem<rope_append_kernel<DT, ROWS, NORM>>(kStages * kUnitHeads * 256);
+  if (rc != RI_OK) return rc;
+  RI_CUDA_OK(ri_launch_pdl_id(8, rope_append_kernel<DT, ROWS, NORM>, grid, dim3(kAppendThreads), smem, s, a));
+  return RI_OK;
+}
+template <int DT, int ROWS>
+int launch(const AppendArgs& a, dim3 grid, size_t smem, cudaStream_t s) {
+  return a.q_norm != nullptr ? launch_kernel<DT, ROWS, true>(a, grid, smem, s) : launch_kernel<DT, ROWS, false>(a, grid, smem, s);
+}
 
-extern "C" int ri_rope_paged_append(const ri_paged* p, const void* d_qkv, int64_t qkv_stride, const float* d_cos_sin,
-                                    int64_t max_positions, const int64_t* d_positions, const uint8_t* h_axis_of, int32_t axes,
-                                    int32_t rows, const int32_t* d_row_start, const int32_t* d_seen, void* d_q, void* d_k, void* d_v,
-                                    void* stream) {
+struct Norms {
+  const void* q;
+  const void* k;
+  int32_t q_heads, k_heads;     // that have a weight of their own: 1 or all
+  float eps;
+};
+
+int append(const char* what, const ri_paged* p, const void* d_qkv, int64_t qkv_stride, const float* d_cos_sin, int64_t max_positions,
+           const int64_t* d_positions, const uint8_t* h_axis_of, int32_t axes, int32_t rows, const int32_t* d_row_start,
+           const int32_t* d_seen, const Norms* norms, void* d_q, void* d_k, void* d_v, void* stream) {
   int rc;
-  if ((rc = check(p, "ri_rope_paged_append")) != RI_OK) return rc;
-  RI_REQUIRE(p->d_values && d_qkv && d_cos_sin && d_positions && h_axis_of && d_q, "ri_rope_paged_append: null pointer");
-  RI_REQUIRE(!p->d_token || d_seen, "ri_rope_paged_append: token numbers need the count of tokens seen");
+  if ((rc = check(p, what)) != RI_OK) return rc;
+  RI_REQUIRE(p->d_values && d_qkv && d_cos_sin && d_positions && h_axis_of && d_q, "%s: null pointer", what);
+  RI_REQUIRE(!p->d_token || d_seen, "%s: token numbers need the count of tokens seen", what);
   RI_REQUIRE(rows >= 1 && max_positions >= 1 && axes >= 1 && axes <= 64 && p->group_size >= 1 && p->group_size <= 65535,
-             "ri_rope_paged_append: rows=%d axes=%d group_size=%d unsupported", rows, axes, p->group_size);
-  RI_REQUIRE(d_row_start || rows == p->batch, "ri_rope_paged_append: %d rows for %d requests need row_start", rows, p->batch);
+             "%s: rows=%d axes=%d group_size=%d unsupported", what, rows, axes, p->group_size);
+  RI_REQUIRE(d_row_start || rows == p->batch, "%s: %d rows for %d requests need row_start", what, rows, p->batch);
   const int64_t hq = (int64_t)p->group_size * p->kv_heads;
   RI_REQUIRE(hq + 2 * p->kv_heads < (1 << 24) && qkv_stride >= (hq + 2 * p->kv_heads) * RI_HEAD_DIM && qkv_stride % 8 == 0,
-             "ri_rope_paged_append: rows of the projection overlap or lie at odd places");
+             "%s: rows of the projection overlap or lie at odd places", what);
   RI_REQUIRE(((uintptr_t)d_qkv | (uintptr_t)d_q | (uintptr_t)d_k | (uintptr_t)d_v) % 16 == 0,
-             "ri_rope_paged_append: tensors must be 16-byte aligned");
+             "%s: tensors must be 16-byte aligned", what);
   AppendArgs a = {};
   for (int i = 0; i < 64; ++i) {
-    RI_REQUIRE(h_axis_of[i] < axes, "ri_rope_paged_append: frequency %d follows axis %d of %d", i, h_axis_of[i], axes);
+    RI_REQUIRE(h_axis_of[i] < axes, "%s: frequency %d follows axis %d of %d", what, i, h_axis_of[i], axes);
     a.axis.of[i] = h_axis_of[i];
   }
   a.pages = view(*p);
@@ -274,6 +342,18 @@ extern "C" int ri_rope_paged_append(const ri_paged* p, const void* d_qkv, int64_
   a.values = static_cast<uint4*>(const_cast<void*>(p->d_values));
   a.rows = rows;
   a.hq = (int)hq;
+  if (norms != nullptr) {
+    RI_REQUIRE(norms->q && norms->k, "%s: null pointer", what);
+    RI_REQUIRE(((uintptr_t)norms->q | (uintptr_t)norms->k) % 16 == 0, "%s: tensors must be 16-byte aligned", what);
+    RI_REQUIRE((norms->q_heads == 1 || norms->q_heads == hq) && (norms->k_heads == 1 || norms->k_heads == p->kv_heads),
+               "%s: weights of %d and %d heads for %d and %d", what, norms->q_heads, norms->k_heads, (int)hq, p->kv_heads);
+    RI_REQUIRE(norms->eps >= 0.f && norms->eps < 1e30f, "%s: eps must be finite and not negative", what);
+    a.q_norm = static_cast<const uint4*>(norms->q);
+    a.k_norm = static_cast<const uint4*>(norms->k);
+    a.q_norm_stride = norms->q_heads > 1 ? 16 : 0;
+    a.k_norm_stride = norms->k_heads > 1 ? 16 : 0;
+    a.eps = norms->eps;
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int sms = 0;
   if ((rc = ri_sm_count(&sms)) != RI_OK) return rc;
@@ -285,21 +365,29 @@ extern "C" int ri_rope_paged_append(const ri_paged* p, const void* d_qkv, int64_
   const int64_t most = (int64_t)sms * kAppendCtas;
   while (a.unit_rows < kUnitRows && (a.unit_rows + 1) * heads <= kUnitHeads && rows > most * a.unit_rows) ++a.unit_rows;
   const int64_t units = a.units_per_row > 1 ? (int64_t)rows * a.units_per_row : ((int64_t)rows + a.unit_rows - 1) / a.unit_rows;
-  RI_REQUIRE(units < (1ll << 30), "ri_rope_paged_append: too large");
+  RI_REQUIRE(units < (1ll << 30), "%s: too large", what);
   const dim3 grid((unsigned)(units < most ? units : most));
   const size_t smem = (size_t)kStages * a.unit_rows * a.unit_heads * 256;
-  auto go = [&](auto kernel) { return ri_launch_pdl_id(8, kernel, grid, dim3(kAppendThreads), smem, s, a); };
-  constexpr int kMost = kStages * kUnitHeads * 256;
-  if (a.unit_rows > 1) {
-    if ((rc = ri_allow_smem<rope_append_kernel<RI_BF16, kUnitRows>>(kMost)) != RI_OK ||
-        (rc = ri_allow_smem<rope_append_kernel<RI_F16, kUnitRows>>(kMost)) != RI_OK)
-      return rc;
-    RI_CUDA_OK(p->dtype == RI_BF16 ? go(rope_append_kernel<RI_BF16, kUnitRows>) : go(rope_append_kernel<RI_F16, kUnitRows>));
-  } else {
-    if ((rc = ri_allow_smem<rope_append_kernel<RI_BF16, 1>>(kMost)) != RI_OK ||
-        (rc = ri_allow_smem<rope_append_kernel<RI_F16, 1>>(kMost)) != RI_OK)
-      return rc;
-    RI_CUDA_OK(p->dtype == RI_BF16 ? go(rope_append_kernel<RI_BF16, 1>) : go(rope_append_kernel<RI_F16, 1>));
-  }
-  return RI_OK;
+  if (a.unit_rows > 1) return p->dtype == RI_BF16 ? launch<RI_BF16, kUnitRows>(a, grid, smem, s) : launch<RI_F16, kUnitRows>(a, grid, smem, s);
+  return p->dtype == RI_BF16 ? launch<RI_BF16, 1>(a, grid, smem, s) : launch<RI_F16, 1>(a, grid, smem, s);
+}
+
+}  // namespace
+
+extern "C" int ri_rope_paged_append(const ri_paged* p, const void* d_qkv, int64_t qkv_stride, const float* d_cos_sin,
+                                    int64_t max_positions, const int64_t* d_positions, const uint8_t* h_axis_of, int32_t axes,
+                                    int32_t rows, const int32_t* d_row_start, const int32_t* d_seen, void* d_q, void* d_k, void* d_v,
+                                    void* stream) {
+  return append("ri_rope_paged_append", p, d_qkv, qkv_stride, d_cos_sin, max_positions, d_positions, h_axis_of, axes, rows, d_row_start,
+                d_seen, nullptr, d_q, d_k, d_v, stream);
+}
+
+extern "C" int ri_rope_paged_append_norm(const ri_paged* p, const void* d_qkv, int64_t qkv_stride, const float* d_cos_sin,
+                                         int64_t max_positions, const int64_t* d_positions, const uint8_t* h_axis_of, int32_t axes,
+                                         int32_t rows, const int32_t* d_row_start, const int32_t* d_seen, const void* d_q_norm,
+                                         const void* d_k_norm, int32_t q_norm_heads, int32_t k_norm_heads, float eps, void* d_q,
+                                         void* d_k, void* d_v, void* stream) {
+  const Norms norms = {d_q_norm, d_k_norm, q_norm_heads, k_norm_heads, eps};
+  return append("ri_rope_paged_append_norm", p, d_qkv, qkv_stride, d_cos_sin, max_positions, d_positions, h_axis_of, axes, rows,
+                d_row_start, d_seen, &norms, d_q, d_k, d_v, stream);
 }

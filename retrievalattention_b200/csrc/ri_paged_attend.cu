@@ -1,0 +1,1116 @@
+// Attention of many query rows over a paged cache, on the tensor cores.
+//   out_r = sum_j p_rj v_j,  p_rj = e^{s_rj - lse_r},  s_rj = scale q_r.k_j,  lse_r = log sum_j e^{s_rj},  over the slots j that row r sees:
+// ri_paged_prompt         several new tokens of every request: the token at slot s sees j <= s with j > s - window or j < sink;
+// ri_paged_shared_decode  one new token of every request, where groups of requests have their first slots in common: a group's rows over
+//                         those slots are worked on together, each request's over the slots of its own, and both are joined by log-sum-exp.
+// A row that sees nothing, or only scores of -infinity, has out 0 and lse -infinity; a NaN or +infinity among its scores makes both NaN.
+//
+// The rows of a tile of 128 are tokens (or requests) times the query heads of one KV head, so K and V serve a whole group of heads and a
+// tile spans few tokens: with four heads 32, which is what keeps the masked part of a window small.  An item is up to two neighbouring
+// tiles and a KV head; it walks the tiles of 128 slots that its rows may see, its first slots' and its window's, and no others:
+// of a tile that is brought in, boxes that no row sees are not read but filled with zeros.
+//   S_g = Q_g.K^T     M 128 x N 128 x K 128, both operands by TMA with the 128-byte swizzle, pages through the page table;
+//   softmax           a thread per query row (= TMEM lane), online, against a lazy reference maximum; P goes back over S as 16-bit pairs;
+//   O_g += P_g.V      A from TMEM, B the V tile as it lies (MN-major), the accumulator in TMEM for the whole walk.
+// Items of two tiles: a group of four softmax warps for each, which share every tile of K and V.  Items of one tile: the groups take
+// its even and its odd steps, and join what they have at the end.
+// Work: the steps of all items, head by head, are cut into one contiguous range per CTA, of equal length; every CTA works out where its own
+// begins.  An item that falls to several CTAs leaves partial results behind, which a second kernel joins in the order of the sequence.
+// TMEM: S_0 | S_1 | O_0 | O_1.  Warps: TMA producer, MMA issuer, the one that hands out segments (the part of an item that falls to the
+// CTA), one idle, eight softmax warps.  Every wait is bounded; one that runs out is recorded in the status word.
+// A tile's slots that a row does not see have a probability of 0, and what they hold is finite where it was written as such; where it
+// was not, 0 * infinity leaves a NaN, and the row is done again over what it sees (`redo`).  Slots behind a request's last one may
+// hold anything: they are zeros in shared memory before the product.
+#include <cuda.h>
+
+#include "ri_paged.cuh"
+#include "ri_tc.cuh"
+
+namespace {
+
+using namespace ri_tc;
+using namespace ri_page;
+
+constexpr int kTile = 128;                 // query rows of a tile, slots of a step
+constexpr int kHalf = kTile * 128;         // bytes of a 128-row x 64-channel half-tile
+constexpr int kRing = 5;                   // tiles of K and V in shared memory: K0, V0, K1, V1, ...
+constexpr int kThreads = 384;
+constexpr int kSegments = 4;               // segments on their way from the warp that hands them out
+constexpr uint32_t kTmemCols = 512;
+constexpr int kMaxCtas = 160;
+constexpr int kMaxRequests = 16384;        // of a call, or groups and requests together
+constexpr int kMaxEntries = 8192;          // of the table of steps
+// An item's end this many steps from the end of a CTA's range becomes the end of the range: a part of an item costs as much again
+// for its partial result and the second kernel.  Items of at most twice as many are never cut.
+constexpr int kSnap = 4;
+constexpr int kHeadsMost = 8;              // query heads of a KV head
+constexpr int kMeta = 8;                   // ints that a CTA leaves for the kernel that joins
+
+struct Walk {
+  int step, n;                             // the first of the item's steps here, and how many; 0: no more segments
+  int front, skip;                         // step i is tile i, i < front, else tile i + skip
+  int two;                                 // two tiles of rows
+  __device__ __forceinline__ int tile(int j) const { return step + j < front ? step + j : step + j + skip; }      // of the j-th step here
+  __device__ __forceinline__ int steps(int g) const { return two ? n : (n + 1 - g) >> 1; }      // of group g; its j-th one:
+  __device__ __forceinline__ int nth(int g, int j) const { return two ? j : 2 * j + g; }
+};
+struct Segment : Walk {
+  int table_row, head;
+  int q_row, n_tok;                        // the item's first token (or request), and how many
+  int low, high, sink;                     // slots that some row of the item sees: [low, high) and [0, sink)
+  int rows;                                // slots of the request: there is nothing behind
+  int slot0;                               // ri_paged_prompt: the first token's slot
+  int part;                                // rows of partial results in front of this segment's, -1: the item is whole
+  int pad;
+};
+
+// Shared memory.  It has no room to spare, so the barriers and the rest stand behind the ring, in what 227 KB leave.
+struct Control {
+  uint64_t bars[16 + 2 * kRing + 2 * kSegments];
+  Segment segments[kSegments];
+  float2 stat[2][kTile];                   // items of one tile: a row's (maximum, sum) in either group
+  int scan[kThreads / 32 + 1];
+  int begin[4], end[4];                    // where the CTA's range begins and ends: head, sequence, pair of tiles, step
+  int first;                               // the first sequence with rows
+  uint32_t tmem;
+  int abort;
+};
+constexpr int kTiles = (4 + 2 * kRing) * kHalf;
+constexpr int kSmem = kTiles + (int)ri_align16(sizeof(Control));
+static_assert(kSmem <= 227 * 1024, "shared memory");
+static_assert((kMaxRequests + 1 + kMaxEntries + 1) * 4 <= 2 * kRing * kHalf, "the tables of the plan lie in the ring");
+
+struct Args : Pages {
+  const int32_t* starts;     // rows of the requests [batch + 1]; SHARED: requests of the groups [groups + 1]
+  const int32_t* shared;     // SHARED: [groups] slots in common
+  const uint16_t* q;
+  const void* keys;
+  const void* values;
+  int64_t q_stride;          // elements
+  uint16_t* out;
+  float* lse;                // or null
+  float* part_o;             // rows of 128, a segment's in the order [channels / 4][rows][4]
+  float2* part_ml;           // (reference in the log2 domain, sum)
+  int* meta;                 // prompt: [CTAs][kMeta]; SHARED: CTAs (first, last) of the items [groups, then own][hk * batch]
+  int64_t part_own;          // SHARED: rows of partial results in front of those of the requests' own slots
+  int n_seq, groups, n_rows; // sequences: requests, or groups and then requests; rows of q
+  int gs, tile_tokens, max_ctas, part_rows;      // tokens of a tile; rows of a CTA's part of the partial results
+  int window, sink;          // window 0: none
+  float scale2;
+  uint32_t idesc_qk, idesc_pv;
+};
+
+// ---- what there is to do: sequences of rows over a request's slots, cut into pairs of tiles ----------------------------
+struct Seq {
+  int n, q_row, table_row;               // tokens (or requests), the first one's row of q, whose page table
+  int low, rows;                         // slots [low, rows) count; low > 0: a request's own slots behind a group's
+};
+struct Item {
+  int n_tok, front, skip, low, high, sink, steps;
+};
+__device__ __forceinline__ int clamped(int x, int most) { return min(max(x, 0), most); }
+// The group that request b is in, or -1.
+__device__ __forceinline__ int group_of(const Args& a, int b) {
+  int lo = 0, hi = a.groups;             // starts[lo] <= b < starts[hi], if it is in one
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    (a.starts[mid] <= b ? lo : hi) = mid;
+  }
+  return a.starts[lo] <= b && b < a.starts[lo + 1] ? lo : -1;
+}
+// What requests of group g have in common: as far as the first one's slots go.
+__device__ __forceinline__ int in_common(const Args& a, int g) {
+  const int b = clamped(a.starts[g], a.batch);
+  return b < a.batch ? clamped(a.shared[g], rows_of(a, b)) : 0;
+}
+template <bool SHARED>
+__device__ __forceinline__ Seq seq_of(const Args& a, int v) {
+  Seq s = {0, 0, v, 0, 0};
+  if (!SHARED) {
+    s.q_row = clamped(a.starts[v], a.n_rows);
+    s.n = max(0, clamped(a.starts[v + 1], a.n_rows) - s.q_row);
+    s.rows = rows_of(a, v);
+  } else if (v < a.groups) {
+    s.q_row = clamped(a.starts[v], a.batch);
+    s.table_row = min(s.q_row, a.batch - 1);
+    s.rows = in_common(a, v);
+    s.n = s.rows > 0 ? max(0, clamped(a.starts[v + 1], a.batch) - s.q_row) : 0;
+  } else {
+    s.q_row = s.table_row = v - a.groups;
+    const int g = group_of(a, s.q_row);
+    s.rows = rows_of(a, s.q_row);
+    s.low = g >= 0 ? min(in_common(a, g), s.rows) : 0;
+    s.n = s.rows > s.low ? 1 : 0;
+  }
+  return s;
+}
+__device__ __forceinline__ int pairs_of(const Args& a, const Seq& s) { return (s.n + 2 * a.tile_tokens - 1) / (2 * a.tile_tokens); }
+template <bool SHARED>
+__device__ __forceinline__ Item item_of(const Args& a, const Seq& s, int p) {
+  Item it;
+  const int first = p * 2 * a.tile_tokens;
+  it.n_tok = min(s.n - first, 2 * a.tile_tokens);
+  it.low = s.low;
+  it.high = s.rows;
+  it.sink = 0;
+  if (!SHARED) {
+    const int slot = s.rows - s.n + first;                // of the first token
+    it.high = clamped(slot + it.n_tok, s.rows);
+    if (a.window > 0) it.low = clamped(slot - a.window + 1, it.high);
+    it.sink = min(a.sink, it.low);
+  }
+  const int tile = it.low / kTile;
+  it.front = min((it.sink + kTile - 1) / kTile, tile);
+  it.skip = tile - it.front;
+  it.steps = max(1, (it.high + kTile - 1) / kTile - it.skip);      // rows that see nothing still have outputs
+  return it;
+}
+
+// ---- the CTA's range ----------------------------------------------------------------------------------------------------
+// Exclusive sum of x over the CTA's threads; `total` becomes the sum of all.
+__device__ __forceinline__ int block_scan(int x, int* tmp, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int incl = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) tmp[warp] = incl;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += tmp[w];
+    total += tmp[w];
+  }
+  __syncthreads();
+  return before + incl - x;
+}
+// The last i < n with table[i] <= x (table[0] <= x).
+__device__ __forceinline__ int last_at_most(const int* table, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    (table[mid] <= x ? lo : hi) = mid;
+  }
+  return lo;
+}
+// Tables of the pairs in front of every sequence and of the steps in front of every 2^k pairs (of one KV head) are made by all
+// threads together; then one looks up where the CTA's range begins, another where it ends.
+template <bool SHARED>
+__device__ __forceinline__ void plan(const Args& a, int* table, Control& s) {
+  const int tid = threadIdx.x;
+  int* pairs = table;
+  int* steps = table + a.n_seq + 1;
+  int total = 0;
+  {
+    const int each = (a.n_seq + kThreads - 1) / kThreads, v0 = min(tid * each, a.n_seq), v1 = min(v0 + each, a.n_seq);
+    int sum = 0, first = a.n_seq;
+    for (int v = v0; v < v1; ++v) {
+      const int n = pairs_of(a, seq_of<SHARED>(a, v));
+      pairs[v] = sum;
+      if (n > 0) first = min(first, v);
+      sum += n;
+    }
+    if (first < a.n_seq) atomicMin(&s.first, first);
+    const int before = block_scan(sum, s.scan, total);
+    for (int v = v0; v < v1; ++v) pairs[v] += before;
+    if (tid == 0) pairs[a.n_seq] = total;
+  }
+  __syncthreads();
+  const int n_pairs = total;
+  int k = 0;
+  while ((n_pairs - 1) >> k >= kMaxEntries) ++k;
+  const int entries = n_pairs > 0 ? ((n_pairs - 1) >> k) + 1 : 0;
+  {
+    const int each = (entries + kThreads - 1) / kThreads, e0 = min(tid * each, entries), e1 = min(e0 + each, entries);
+    int sum = 0;
+    if (e0 < e1) {
+      int at = e0 << k, v = last_at_most(pairs, a.n_seq, at);
+      Seq seq = seq_of<SHARED>(a, v);
+      for (int e = e0; e < e1; ++e) {
+        steps[e] = sum;
+        for (const int end = min((e + 1) << k, n_pairs); at < end; ++at) {
+          if (at >= pairs[v + 1]) {
+            do ++v;
+            while (at >= pairs[v + 1]);
+            seq = seq_of<SHARED>(a, v);
+          }
+          sum += item_of<SHARED>(a, seq, at - pairs[v]).steps;
+        }
+      }
+    }
+    const int before = block_scan(sum, s.scan, total);
+    for (int e = e0; e < e1; ++e) steps[e] += before;
+  }
+  __syncthreads();
+  if (tid < 2) {
+    const int64_t all = (int64_t)total * a.hk;
+    const int n_ctas = (int)min((int64_t)a.max_ctas, all), c = (int)blockIdx.x + tid;
+    int* place = tid == 0 ? s.begin : s.end;
+    const int64_t x = c < n_ctas ? all * c / n_ctas : all;
+    int head = a.hk, v = 0, p = 0, step = 0;
+    if (x < all) {
+      head = (int)(x / total);
+      const int y = (int)(x - (int64_t)head * total), e = last_at_most(steps, entries, y);
+      int at = e << k, before = steps[e];
+      v = last_at_most(pairs, a.n_seq, at);
+      Seq seq = seq_of<SHARED>(a, v);
+      for (;;) {
+        p = at - pairs[v];
+        const int n = item_of<SHARED>(a, seq, p).steps;
+        step = y - before;
+        if (step < n) {
+          if (!SHARED && step > 0) {
+            if (step <= kSnap) {
+              step = 0;
+              break;
+            }
+            if (n - step > kSnap) break;
+            step = 0;                      // the next item, which may be the next head's first
+            if (++at == n_pairs) {
+              ++head;
+              v = p = 0;
+              if (head < a.hk) v = last_at_most(pairs, a.n_seq, 0);
+              break;
+            }
+            while (at >= pairs[v + 1]) ++v;
+            p = at - pairs[v];
+          }
+          break;
+        }
+        before += n;
+        ++at;
+        if (at >= pairs[v + 1]) {
+          do ++v;
+          while (at >= pairs[v + 1]);
+          seq = seq_of<SHARED>(a, v);
+        }
+      }
+    }
+    place[0] = head;
+    place[1] = head < a.hk ? v : 0;
+    place[2] = head < a.hk ? p : 0;
+    place[3] = head < a.hk ? step : 0;
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // TMA writes over the tables
+  __syncthreads();
+}
+
+__device__ __forceinline__ float ex2(float x) {       // 2^x; results below 2^-126 become 0
+  float d;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
+  return d;
+}
+// A tile is read four times over: 32 columns a mask, bit i of which says whether column i is seen.
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
+
+// What a thread's row sees, of slots [low, high) and [0, sink).
+struct Sight {
+  int low, high, sink;
+  __device__ __forceinline__ bool all_of(int slot0) const { return slot0 >= low && slot0 + kTile <= high; }
+  __device__ __forceinline__ uint32_t mask(int slot0) const {      // of 32 slots
+    return bits_below(high - slot0) & (~bits_below(low - slot0) | bits_below(sink - slot0));
+  }
+};
+
+// The rows of `bad` once more, one after the other, over the slots of this segment that they see and no others, in 32 bits against
+// the same reference: row i of the warp is lane i's.  `half`: 0 or 1, write these 64 channels; -1: all.
+template <int DT>
+__device__ __noinline__ void redo(const Args& a, const Segment& sg, unsigned bad, const Sight& sight, int row, int q_row, float m, float f, int half) {
+  const int lane = threadIdx.x & 31, n_rows = sg.n_tok * a.gs;
+  while (bad) {
+    const int src = __ffs(bad) - 1;
+    bad &= bad - 1;
+    const Sight see = {__shfl_sync(0xffffffffu, sight.low, src), __shfl_sync(0xffffffffu, sight.high, src), __shfl_sync(0xffffffffu, sight.sink, src)};
+    const int r = __shfl_sync(0xffffffffu, row, src), tok = __shfl_sync(0xffffffffu, q_row, src);
+    const float ref = __shfl_sync(0xffffffffu, m, src), factor = __shfl_sync(0xffffffffu, f, src);
+    const int h = sg.head * a.gs + r % a.gs;
+    auto four = [&](const uint16_t* p, float (&x)[4]) {
+      const uint2 u = *reinterpret_cast<const uint2*>(p + lane * 4);
+      x[0] = Elem<DT>::from_bits((uint16_t)(u.x & 0xffffu)); x[1] = Elem<DT>::from_bits((uint16_t)(u.x >> 16));
+      x[2] = Elem<DT>::from_bits((uint16_t)(u.y & 0xffffu)); x[3] = Elem<DT>::from_bits((uint16_t)(u.y >> 16));
+    };
+    float q[4], k[4], v[4], o[4] = {0.f, 0.f, 0.f, 0.f};
+    four(a.q + (int64_t)tok * a.q_stride + h * RI_HEAD_DIM, q);
+    for (int i = sg.step; i < sg.step + sg.n; ++i) {
+      const int slot0 = (i < sg.front ? i : i + sg.skip) * kTile;
+      for (int slot = slot0; slot < min(slot0 + kTile, see.high); ++slot) {
+        if (slot < see.low && slot >= see.sink) continue;
+        const int id = page_of(a, sg.table_row, slot >> a.shift);
+        const int64_t in_page = ((int64_t)(sg.head << a.shift) + (slot & ((1 << a.shift) - 1))) * RI_HEAD_DIM;
+        four(static_cast<const uint16_t*>(a.keys) + id * a.key_stride + in_page, k);
+        four(static_cast<const uint16_t*>(a.values) + id * a.value_stride + in_page, v);
+        float s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
+#pragma unroll
+        for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+        s *= a.scale2;
+        if (s == -INFINITY) continue;
+        const float p = fmaxf(exp2f(s - ref), 1.17549435e-38f);      // an infinite value is one however little it counts
+        const float weight = s == s ? p : s;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += weight * v[e];
+      }
+    }
+    if (half >= 0 && (lane >> 4) != half) continue;
+    if (sg.part < 0) {
+      const uint2 u = make_uint2(Elem<DT>::pack2(o[0] * factor, o[1] * factor), Elem<DT>::pack2(o[2] * factor, o[3] * factor));
+      *reinterpret_cast<uint2*>(a.out + ((int64_t)tok * a.hk * a.gs + h) * RI_HEAD_DIM + lane * 4) = u;
+    } else {
+      reinterpret_cast<float4*>(a.part_o + (int64_t)sg.part * RI_HEAD_DIM)[lane * n_rows + r] = make_float4(o[0], o[1], o[2], o[3]);
+    }
+  }
+}
+
+template <int DT, bool SHARED>
+__global__ void __launch_bounds__(kThreads, 1)
+paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Args a) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  Control& s = *reinterpret_cast<Control*>(smem + kTiles);
+  const uint32_t sQ = smem_u32(smem), sKV = sQ + 4 * kHalf, bars = smem_u32(s.bars);
+  auto bar_q = [&](int g) { return bars + 8u * g; };
+  auto bar_q_empty = [&](int g) { return bars + 8u * (2 + g); };
+  auto bar_s_full = [&](int g) { return bars + 8u * (4 + g); };
+  auto bar_p_part = [&](int g) { return bars + 8u * (6 + g); };
+  auto bar_p_full = [&](int g) { return bars + 8u * (8 + g); };
+  auto bar_o_full = [&](int g) { return bars + 8u * (10 + g); };
+  auto bar_join = [&](int i) { return bars + 8u * (12 + i); };
+  auto bar_full = [&](int i) { return bars + 8u * (16 + i); };
+  auto bar_empty = [&](int i) { return bars + 8u * (16 + kRing + i); };
+  auto bar_seg = [&](int i) { return bars + 8u * (16 + 2 * kRing + i); };
+  auto bar_seg_empty = [&](int i) { return bars + 8u * (16 + 2 * kRing + kSegments + i); };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = (int)blockIdx.x;
+
+  if (threadIdx.x == 0) {
+    // the swizzle of the tiles goes by addresses: shared memory that does not begin on a boundary of 1 KB gives up at once
+    s.abort = (sQ & 1023u) ? 10 : 0;
+    s.first = 0x7fffffff;
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(bar_q(g), 1); mbar_init(bar_q_empty(g), 1); mbar_init(bar_s_full(g), 1);
+      mbar_init(bar_p_part(g), 4); mbar_init(bar_p_full(g), 4); mbar_init(bar_o_full(g), 1); mbar_init(bar_join(g), 8);
+    }
+    for (int i = 0; i < kRing; ++i) { mbar_init(bar_full(i), 1); mbar_init(bar_empty(i), 1); }
+    for (int i = 0; i < kSegments; ++i) { mbar_init(bar_seg(i), 1); mbar_init(bar_seg_empty(i), 10); }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s.tmem)), "r"(kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s.tmem;
+  volatile int* abort_flag = &s.abort;
+  ri_pdl_wait();
+  ri_pdl_trigger();                        // the kernel that joins waits for the end of this one
+  const bool aligned = s.abort == 0;       // of the whole CTA
+  if (aligned) plan<SHARED>(a, reinterpret_cast<int*>(smem + 4 * kHalf), s);
+
+  // every role goes through the segments one by one, whole warps
+  auto take = [&](int i) {
+    return __all_sync(0xffffffffu, mbar_wait(bar_seg(i % kSegments), (i / kSegments) & 1, abort_flag, 10)) && s.segments[i % kSegments].n > 0;
+  };
+  auto release = [&](int i) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar_seg_empty(i % kSegments));
+  };
+
+  if (aligned) {
+  // registers at launch: 384 x 168; after the split 128 x 96 + 256 x 200, which is less
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    if (warp == 0) {
+      // ---------------- TMA producer: Q_0, K0, Q_1, V0, K1, V1, ... of one segment after the other; a box per lane ----------------
+      const int box = min(1 << a.shift, kTile), mask = (1 << a.shift) - 1, slot_of_lane = lane * box;
+      const uint32_t q_bytes = (uint32_t)(a.tile_tokens * a.gs) * 256;
+      int issued = 0, q_issued[2] = {0, 0};
+      bool ok = true;
+      for (int i = 0; ok && take(i); ++i) {
+        const Segment& sg = s.segments[i % kSegments];
+        const Walk w = sg;
+        const int head = sg.head, low = sg.low, high = sg.high, sink = sg.sink;
+        const int32_t* table = a.table + (int64_t)sg.table_row * a.table_stride;
+        auto load_q = [&](int g) {
+          if (!__all_sync(0xffffffffu, mbar_wait(bar_q_empty(g), (q_issued[g] & 1) ^ 1, abort_flag, 12))) return false;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(bar_q(g), q_bytes);
+            for (int kb = 0; kb < 2; ++kb)
+              tma_load_4d(sQ + (g * 2 + kb) * kHalf, &map_q, bar_q(g), 0, head * a.gs, kb, sg.q_row + g * a.tile_tokens);
+          }
+          __syncwarp();
+          ++q_issued[g];
+          return true;
+        };
+        // this lane's box of the j-th step; one that no row sees is looked up nowhere, and comes from behind the pool, as zeros
+        auto slot_at = [&](int j) { return w.tile(j) * kTile + slot_of_lane; };
+        auto seen = [&](int slot) { return slot_of_lane < kTile && slot < high && (slot + box > low || slot < sink); };
+        auto page_at = [&](int j) { return seen(slot_at(j)) ? table[slot_at(j) >> a.shift] : -1; };
+        int next = page_at(0);
+        ok = load_q(0);
+        for (int j = 0; ok && j < w.n; ++j) {
+          const int id = seen(slot_at(j)) ? page_or_first(a, next) : a.n_pages;
+          const int y = (head << a.shift) + (slot_at(j) & mask);
+          if (j + 1 < w.n) next = page_at(j + 1);
+          for (int t = 0; ok && t < 2; ++t) {
+            const int at = issued % kRing;
+            ok = __all_sync(0xffffffffu, mbar_wait(bar_empty(at), ((issued / kRing) & 1) ^ 1, abort_flag, 13));
+            if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(bar_full(at), 2 * kHalf);
+            __syncwarp();
+            if (slot_of_lane < kTile)
+              for (int kb = 0; kb < 2; ++kb)
+                tma_load_4d(sKV + (at * 2 + kb) * kHalf + slot_of_lane * 128, t ? &map_v : &map_k, bar_full(at), 0, y, kb, id);
+            ++issued;
+            if (j == 0 && t == 0 && w.two) ok = load_q(1);
+          }
+        }
+        release(i);
+      }
+      if (*abort_flag) {     // give the copies still in flight a bounded chance to land before the CTA exits
+        for (int g = 0; g < 2; ++g)
+          if (q_issued[g] > 0) mbar_wait(bar_q(g), (q_issued[g] - 1) & 1, abort_flag, 14);
+        for (int t = max(0, issued - kRing); t < issued; ++t) mbar_wait(bar_full(t % kRing), (t / kRing) & 1, abort_flag, 14);
+      }
+    } else if (warp == 1) {
+      // ---------------- MMA issuer (lane 0; the warp clears what lies behind a request's last slot) ----------------
+      // Per step: P_0.V, then S_0 of the group's next tile, then the same for group 1; behind the last step of a segment come the
+      // first scores of the next one.  S_g of the next tile overwrites the columns P_g was read from: both are products of this
+      // thread, which the tensor pipe takes in order.
+      int tile0 = 0;                       // ring index of the segment's first K tile
+      int q_used[2] = {0, 0}, p_used[2] = {0, 0};
+      auto wait = [&](uint32_t bar, int parity, int where) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, where)); };
+      auto wait_tile = [&](int t) { return wait(bar_full(t % kRing), (t / kRing) & 1, 15); };
+      // ring index of the K tile of group g's step j; its V tile is the next one
+      auto ring_k = [&](const Walk& w, int g, int j) { return tile0 + 2 * w.nth(g, j); };
+      auto issue_qk = [&](const Walk& w, int g, int t, bool last) {
+        if (lane == 0) {
+          const uint32_t sk = sKV + (t % kRing) * 2 * kHalf;
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+            const uint64_t da = umma_desc_sw128(sQ + ((w.two ? g : 0) * 2 + kb) * kHalf), db = umma_desc_sw128(sk + kb * kHalf);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) tc_mma_f16(tmem + g * kTile, da + 2 * k, db + 2 * k, a.idesc_qk, (kb | k) != 0);
+          }
+          tc_commit(bar_s_full(g));          // also says that P_g.V of the tile before has completed
+          if (last) tc_commit(bar_q_empty(w.two ? g : 0));
+          if (!w.two) tc_commit(bar_empty(t % kRing));
+        }
+        __syncwarp();
+      };
+      auto issue_pv = [&](int g, int t, int k0, bool first) {
+        if (lane == 0) {
+          const uint64_t db = umma_desc_mn_sw128(sKV + (t % kRing) * 2 * kHalf, kHalf);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc_mma_f16_ts(tmem + (2 + g) * kTile, tmem + g * kTile + 8 * (k0 + k), db + 128 * (k0 + k), a.idesc_pv, !first || (k0 + k) != 0);
+        }
+        __syncwarp();
+      };
+      // what lies behind the request's last slot, up to the end of its page
+      auto clear = [&](int rows, int tile, int t) {
+        const int r0 = rows - tile * kTile;
+        if (r0 >= kTile) return;
+        const int box = min(1 << a.shift, kTile), r1 = (max(r0, 0) + box - 1) / box * box;
+        uint8_t* v = smem + 4 * kHalf + (t % kRing) * 2 * kHalf;
+        for (int i = max(r0, 0) * 8 + lane; i < r1 * 8; i += 32)
+          for (int kb = 0; kb < 2; ++kb) *reinterpret_cast<uint4*>(v + kb * kHalf + i * 16) = make_uint4(0, 0, 0, 0);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+      };
+      // whether group g's step j is the last user of its Q tile (one tile: the walk's last step, in either group)
+      auto last_of_q = [&](const Walk& w, int g, int j) { return w.nth(g, j) + 1 == w.n; };
+      bool ok = true;
+      for (int i = 0; ok && take(i); ++i) {
+        const Walk w = s.segments[i % kSegments];
+        const int rows = s.segments[i % kSegments].rows;
+        release(i);
+        // first scores of both groups
+        for (int g = 0; ok && g < 2; ++g) {
+          if (w.steps(g) == 0) continue;
+          ok = wait_tile(ring_k(w, g, 0));
+          if (ok && (w.two || g == 0)) ok = wait(bar_q(g), q_used[g]++ & 1, 16);
+          if (!ok) break;
+          tc_fence_after();
+          issue_qk(w, g, ring_k(w, g, 0), last_of_q(w, g, 0));
+        }
+        if (ok && w.two && lane == 0) tc_commit(bar_empty(tile0 % kRing));
+        for (int j = 0; ok && j < w.steps(0); ++j) {
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            if (!ok || j >= w.steps(g)) continue;
+            const int tv = ring_k(w, g, j) + 1;
+            ok = wait_tile(tv);
+            if (!ok) break;
+            if (!w.two || g == 0) clear(rows, w.tile(w.nth(g, j)), tv);
+            ok = wait(bar_p_part(g), p_used[g] & 1, 17);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(g, tv, 0, j == 0);
+            ok = wait(bar_p_full(g), p_used[g] & 1, 18);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(g, tv, 4, false);
+            ++p_used[g];
+            if (!w.two && lane == 0) tc_commit(bar_empty(tv % kRing));
+            if (j + 1 < w.steps(g)) {
+              ok = wait_tile(ring_k(w, g, j + 1));
+              if (!ok) break;
+              tc_fence_after();
+              issue_qk(w, g, ring_k(w, g, j + 1), last_of_q(w, g, j + 1));
+            } else if (lane == 0) {
+              tc_commit(bar_o_full(g));
+            }
+          }
+          if (ok && w.two && lane == 0) {
+            tc_commit(bar_empty((tile0 + 2 * j + 1) % kRing));
+            if (j + 1 < w.n) tc_commit(bar_empty((tile0 + 2 * j + 2) % kRing));
+          }
+        }
+        tile0 += 2 * w.n;
+      }
+    } else if (warp == 2) {
+      // ---------------- segments ----------------
+      if (lane == 0) {
+        int h = s.begin[0], v = s.begin[1], p = s.begin[2], step = s.begin[3];
+        const int h1 = s.end[0], v1 = s.end[1], p1 = s.end[2], step1 = s.end[3], first = s.first;
+        int given = 0, tail = 0, head = 0;                      // prompt: rows of a segment that others go on with; 1 and 2: see below
+        Segment sg = {};
+        auto give = [&] {
+          const int at = given % kSegments;
+          if (!mbar_wait(bar_seg_empty(at), ((given / kSegments) & 1) ^ 1, abort_flag, 19)) return false;
+          s.segments[at] = sg;
+          mbar_arrive(bar_seg(at));
+          ++given;
+          return true;
+        };
+        Seq seq = {};
+        int pairs = 0, of = -1;
+        bool ok = true;
+        while (ok && h < a.hk) {
+          const bool last = h == h1 && v == v1 && p == p1;
+          if (last && step == step1) break;
+          if (of != v) {
+            seq = seq_of<SHARED>(a, v);
+            pairs = pairs_of(a, seq);
+            of = v;
+          }
+          const Item it = item_of<SHARED>(a, seq, p);
+          const int end = last ? step1 : it.steps;
+          sg.table_row = seq.table_row;
+          sg.head = h;
+          sg.q_row = seq.q_row + p * 2 * a.tile_tokens;
+          sg.n_tok = it.n_tok;
+          sg.step = step;
+          sg.n = end - step;
+          sg.front = it.front;
+          sg.skip = it.skip;
+          sg.low = it.low;
+          sg.high = it.high;
+          sg.sink = it.sink;
+          sg.rows = seq.rows;
+          sg.slot0 = seq.rows - seq.n + p * 2 * a.tile_tokens;
+          sg.two = it.n_tok > a.tile_tokens;
+          const bool begins = step == 0, ends = end == it.steps;
+          if (SHARED) {
+            const bool own = v >= a.groups;
+            const int64_t at = (int64_t)h * a.batch + sg.q_row, rows = own ? a.part_own + (int64_t)c * a.gs : (int64_t)c * a.part_rows;
+            sg.part = (int)(rows + at * a.gs);
+            int* ctas = a.meta + 2 * (at + (own ? (int64_t)a.hk * a.batch : 0));
+            if (begins) ctas[0] = c;
+            if (ends) ctas[1] = c;
+          } else {
+            sg.part = begins && ends ? -1 : (2 * c + begins) * a.part_rows;
+            if (!begins) head = ends ? 1 : 2;                   // another CTA's item: it ends here, or goes on behind
+            if (begins && !ends) {
+              tail = sg.n_tok;
+              a.meta[c * kMeta + 2] = h;
+              a.meta[c * kMeta + 3] = sg.q_row;
+            }
+          }
+          ok = give();
+          step = 0;
+          if (last) break;
+          if (++p == pairs) {
+            p = 0;
+            do ++v;
+            while (v < a.n_seq && !(v == v1 && h == h1) && pairs_of(a, seq_of<SHARED>(a, v)) == 0);
+            if (v == a.n_seq) {
+              v = first;
+              ++h;
+            }
+          }
+        }
+        if (!SHARED && a.meta != nullptr) {
+          a.meta[c * kMeta] = tail;
+          a.meta[c * kMeta + 1] = head;
+        }
+        sg.n = 0;
+        if (ok) give();
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    // ---------------- softmax and epilogue: thread = query row = TMEM lane; group g owns S_g and O_g ----------------
+    const int grp = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;      // a warp may touch only its quarter of the lanes
+    const uint32_t t_lane = (uint32_t)(quarter * 32) << 16;
+    const uint32_t tmem_s = tmem + grp * kTile + t_lane, tmem_o = tmem + (2 + grp) * kTile + t_lane;
+    const uint64_t scale_2 = pack_f2(a.scale2, a.scale2);
+    // The reference follows the running maximum in steps of more than 2^kLazy, kAbove below it: fp16's short exponent then holds
+    // probabilities down to 2^-(24 + kAbove) of the largest, which are at most 2^(kAbove + kLazy).
+    constexpr float kLazy = 4.f, kAbove = DT == RI_F16 ? 10.f : 0.f;
+    bool ok = true;
+    int done = 0, outs[2] = {0, 0}, joins = 0;             // tiles of this group, outputs of both groups, joins so far
+    auto meet = [&](int i) {                               // of all eight warps
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_join(i));
+      return (bool)__all_sync(0xffffffffu, mbar_wait(bar_join(i), joins & 1, abort_flag, 10));
+    };
+    for (int i = 0; ok && take(i); ++i) {
+      const Segment& sg = s.segments[i % kSegments];         // stays until the end of the segment
+      const Walk w = sg;
+      const int n = w.steps(grp), tile_row0 = w.two ? grp * a.tile_tokens * a.gs : 0;
+      // the row in its item, its token; rows that fill up a tile are like the last one, so that they hold nobody up
+      const int n_rows = sg.n_tok * a.gs, item_row = tile_row0 + row;
+      const bool valid = row < a.tile_tokens * a.gs && item_row < n_rows;
+      const int q_row = sg.q_row + min(item_row, n_rows - 1) / a.gs;
+      Sight sight = {sg.low, sg.high, 0};
+      if (!SHARED) {
+        const int slot = sg.slot0 + q_row - sg.q_row;
+        sight.high = clamped(slot + 1, sg.rows);
+        sight.low = a.window > 0 ? max(0, slot - a.window + 1) : 0;
+        sight.sink = a.sink;
+      } else {
+        sight.high = min(sg.high, rows_of(a, q_row));
+      }
+      float m_ref = -INFINITY, l_run = 0.f;
+      for (int j = 0; ok && j < n; ++j, ++done) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_s_full(grp), done & 1, abort_flag, 11));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t sr[4][32];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) tc_ld32(tmem_s + x * 32, sr[x]);
+        tc_wait_ld();
+#pragma unroll
+        for (int x = 0; x < 4; ++x) tc_ld_landed(sr[x]);
+
+        const int slot0 = w.tile(w.nth(grp, j)) * kTile;
+        if (!sight.all_of(slot0)) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const uint32_t seen = sight.mask(slot0 + x * 32);
+#pragma unroll
+            for (int y = 0; y < 32; ++y)
+              if (!(seen & (1u << y))) sr[x][y] = 0xff800000u;     // -inf
+          }
+        }
+        float mx[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          mx[x] = fmaxf(__uint_as_float(sr[x][0]), __uint_as_float(sr[x][1]));
+#pragma unroll
+          for (int y = 2; y < 32; y += 2) mx[x] = max3(mx[x], __uint_as_float(sr[x][y]), __uint_as_float(sr[x][y + 1]));
+        }
+        const float m_tile = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * a.scale2 - kAbove;
+        const bool move = m_tile > m_ref + kLazy;              // also true for the first finite tile (m_ref = -inf)
+        if (__any_sync(0xffffffffu, move)) {
+          // the warp's accumulator rows are multiplied anyway, so every row of it catches up with its maximum
+          const float m_new = fmaxf(m_ref, m_tile);
+          const float factor = m_ref == -INFINITY ? 0.f : exp2f(m_ref - m_new);      // 1 when the maximum stays
+          l_run *= factor;
+          m_ref = m_new;
+          if (j > 0) {                                         // rare: bring this warp's rows of O to the new reference
+#pragma unroll 1
+            for (int x = 0; x < 4; ++x) {
+              uint32_t orow[32];
+              tc_ld32(tmem_o + x * 32, orow);
+              tc_wait_ld();
+              tc_ld_landed(orow);
+#pragma unroll
+              for (int y = 0; y < 32; ++y) orow[y] = __float_as_uint(__uint_as_float(orow[y]) * factor);
+              tc_st32(tmem_o + x * 32, orow);
+            }
+          }
+        }
+        // probabilities p = 2^(s * scale - m), packed as the 16-bit operand of the second product: word y of the row = slots 2y, 2y+1
+        const float ref = m_ref == -INFINITY ? 0.f : m_ref;
+        const uint64_t neg_m = pack_f2(-ref, -ref);
+        uint64_t sum2[2] = {0ull, 0ull};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          uint32_t pw[16];
+#pragma unroll
+          for (int y = 0; y < 16; ++y) {
+            const uint64_t e = fma_f2(pack_f2(__uint_as_float(sr[x][2 * y]), __uint_as_float(sr[x][2 * y + 1])), scale_2, neg_m);
+            float e0, e1;
+            unpack_f2(e, e0, e1);
+            const float p0 = ex2(e0), p1 = ex2(e1);
+            sum2[y & 1] = add_f2(sum2[y & 1], pack_f2(p0, p1));
+            pw[y] = Elem<DT>::pack2(p0, p1);
+          }
+          tc_st16(tmem_s + x * 16, pw);
+          if (x == 1) {          // the product over the first 64 slots may start
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_p_part(grp));
+          }
+        }
+        float s0, s1;
+        unpack_f2(add_f2(sum2[0], sum2[1]), s0, s1);
+        l_run += s0 + s1;
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_p_full(grp));
+      }
+      // ---- epilogue, one row per thread.  Two tiles: each group its own.  One: the groups exchange (maximum, sum) through shared
+      //      memory, then each joins half of the channels of both accumulators; the second barrier keeps an accumulator until the
+      //      other group has read it ----
+      float m = m_ref, l = l_run, w0 = 1.f, w1 = 0.f;        // of the row; weights of the accumulators read below
+      if (!w.two) {
+        s.stat[grp][row] = make_float2(m_ref, l_run);
+        ok = ok && meet(0);
+        const float2 other = s.stat[grp ^ 1][row];
+        m = fmaxf(m_ref, other.x);
+        const float f_own = m_ref == -INFINITY ? 0.f : exp2f(m_ref - m), f_other = other.x == -INFINITY ? 0.f : exp2f(other.x - m);
+        l = l_run * f_own + other.y * f_other;
+        w0 = grp ? f_other : f_own;
+        w1 = grp ? f_own : f_other;
+      }
+      const float f = sg.part < 0 ? (l == 0.f ? 0.f : 1.f / l) : 1.f;      // NaN stays one
+      w0 *= f;
+      w1 *= f;
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+        if (w.steps(g) > 0) {              // the other group's outputs count even where nobody here waits for them
+          if (!w.two || g == grp) ok = ok && __all_sync(0xffffffffu, mbar_wait(bar_o_full(g), outs[g] & 1, abort_flag, 11));
+          ++outs[g];
+        }
+      if (ok) {
+        tc_fence_after();
+        const bool both = !w.two && w.steps(1) > 0;
+        const int x0 = w.two ? 0 : grp * 2, x1 = w.two ? 4 : x0 + 2;
+        const int h = sg.head * a.gs + item_row % a.gs;
+        bool bad = false;
+#pragma unroll 1
+        for (int x = x0; x < x1; ++x) {
+          uint32_t o0[32], o1[32];
+          tc_ld32(tmem + (2 + (w.two ? grp : 0)) * kTile + t_lane + x * 32, o0);
+          if (both) tc_ld32(tmem + 3 * kTile + t_lane + x * 32, o1);
+          tc_wait_ld();
+          tc_ld_landed(o0);
+          if (both) tc_ld_landed(o1);
+          if (valid) {
+            float o[32];
+#pragma unroll
+            for (int y = 0; y < 32; ++y) {
+              o[y] = __uint_as_float(o0[y]) * w0 + (both ? __uint_as_float(o1[y]) * w1 : 0.f);
+              bad |= o[y] != o[y];
+            }
+            if (sg.part < 0) {
+              uint4* dst = reinterpret_cast<uint4*>(a.out + ((int64_t)q_row * a.hk * a.gs + h) * RI_HEAD_DIM);
+#pragma unroll
+              for (int y = 0; y < 32; y += 8)
+                dst[x * 4 + y / 8] = make_uint4(Elem<DT>::pack2(o[y], o[y + 1]), Elem<DT>::pack2(o[y + 2], o[y + 3]),
+                                                Elem<DT>::pack2(o[y + 4], o[y + 5]), Elem<DT>::pack2(o[y + 6], o[y + 7]));
+            } else {
+              float4* dst = reinterpret_cast<float4*>(a.part_o + (int64_t)sg.part * RI_HEAD_DIM);
+#pragma unroll
+              for (int y = 0; y < 32; y += 4) dst[(x * 8 + y / 4) * n_rows + item_row] = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+            }
+          }
+        }
+        if (valid && (w.two || grp == 0)) {
+          if (sg.part >= 0) a.part_ml[sg.part + item_row] = make_float2(m, l);
+          else if (a.lse != nullptr) a.lse[(int64_t)q_row * a.hk * a.gs + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+        }
+        const unsigned again = __ballot_sync(0xffffffffu, bad && l == l);
+        if (again) {
+          __syncwarp();
+          redo<DT>(a, sg, again, sight, item_row, q_row, m == -INFINITY ? 0.f : m, f, w.two ? -1 : grp);
+        }
+      }
+      if (!w.two) {
+        ok = ok && meet(1);
+        ++joins;
+      }
+      release(i);
+    }
+  }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && s.abort) *a.status = s.abort;
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+  }
+}
+
+// ---- the parts of an item that fell to several CTAs, joined in their order ---------------------------------------------------
+// Factor of a part against the largest reference; one that is far below it still counts enough to hand on an infinite value.
+__device__ __forceinline__ float part_factor(float m, float most) {
+  return m == -INFINITY ? 0.f : fmaxf(exp2f(m - most), 1.17549435e-38f);
+}
+struct Joined {
+  float m = -INFINITY, l = 0.f;
+  __device__ __forceinline__ void add(float2 ml) {
+    const float most = fmaxf(m, ml.x), ref = most == -INFINITY ? 0.f : most;
+    l = l * exp2f(m - ref) + ml.y * exp2f(ml.x - ref);
+    m = most;
+  }
+  __device__ __forceinline__ float lse() const { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f; }
+  __device__ __forceinline__ float scale() const { return l == 0.f ? 0.f : 1.f / l; }
+};
+
+// ri_paged_prompt: a block per CTA whose range ends inside an item that begins in it, and 32 rows of that item; a lane per row, four
+// times four channels a warp.
+constexpr int kJoinRows = 32, kJoinThreads = 256;
+template <int DT>
+__global__ void __launch_bounds__(kJoinThreads) prompt_join_kernel(const __grid_constant__ Args a) {
+  ri_pdl_enter();
+  const int c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y * kJoinRows + lane;
+  const int* meta = a.meta + c * kMeta;
+  const int h = clamped(meta[2], a.hk - 1), q_row = clamped(meta[3], a.n_rows - 1), n_tok = min(meta[0], min(2 * a.tile_tokens, a.n_rows - q_row));
+  const int n_rows = n_tok * a.gs;
+  if (n_tok <= 0 || row >= n_rows) return;
+  int last = c;                                            // the CTA that has the item's end
+  while (last + 1 < a.max_ctas && meta[(last + 1 - c) * kMeta + 1] == 2) ++last;
+  if (last + 1 < a.max_ctas && meta[(last + 1 - c) * kMeta + 1] == 1) ++last;
+  auto part_at = [&](int i) { return (int64_t)(2 * i + (i == c)) * a.part_rows; };
+  Joined all;
+  for (int i = c; i <= last; ++i) all.add(a.part_ml[part_at(i) + row]);
+  float4 o[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) o[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = c; i <= last; ++i) {
+    const float f = part_factor(a.part_ml[part_at(i) + row].x, all.m);
+    const float4* src = reinterpret_cast<const float4*>(a.part_o + part_at(i) * RI_HEAD_DIM) + warp * 4 * n_rows + row;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float4 y = src[x * n_rows];
+      o[x].x += f * y.x; o[x].y += f * y.y; o[x].z += f * y.z; o[x].w += f * y.w;
+    }
+  }
+  const float f = all.scale();
+  const int64_t at = ((int64_t)q_row + row / a.gs) * a.hk * a.gs + h * a.gs + row % a.gs;
+  uint4* dst = reinterpret_cast<uint4*>(a.out + at * RI_HEAD_DIM) + warp * 2;
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+    dst[x] = make_uint4(Elem<DT>::pack2(o[2 * x].x * f, o[2 * x].y * f), Elem<DT>::pack2(o[2 * x].z * f, o[2 * x].w * f),
+                        Elem<DT>::pack2(o[2 * x + 1].x * f, o[2 * x + 1].y * f), Elem<DT>::pack2(o[2 * x + 1].z * f, o[2 * x + 1].w * f));
+  if (warp == 0 && a.lse != nullptr) a.lse[at] = all.lse();
+}
+
+// ri_paged_shared_decode: a block per request and KV head, a thread per query head and four channels, over the parts of the group's
+// item and then of the request's own.
+template <int DT>
+__global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const __grid_constant__ Args a) {
+  ri_pdl_enter();
+  const int b = blockIdx.x, h = blockIdx.y, quad = threadIdx.x / a.gs, r = threadIdx.x - quad * a.gs;
+  const int g = group_of(a, b), rows = rows_of(a, b), common = g >= 0 ? in_common(a, g) : 0;
+  // the two items: rows of theirs, this one's place among them, their parts
+  const int* ctas = nullptr;
+  int first[2] = {0, 0}, last[2] = {-1, -1}, n_rows[2] = {0, a.gs}, row[2] = {0, r};
+  int64_t part[2] = {0, 0};
+  if (common > 0) {
+    const int b0 = clamped(a.starts[g], a.batch), b1 = clamped(a.starts[g + 1], a.batch), pair = 2 * a.tile_tokens;
+    const int q_row = b0 + (b - b0) / pair * pair;
+    n_rows[0] = min(pair, b1 - q_row) * a.gs;
+    row[0] = (b - q_row) * a.gs + r;
+    part[0] = ((int64_t)h * a.batch + q_row) * a.gs;
+    ctas = a.meta + 2 * ((int64_t)h * a.batch + q_row);
+    first[0] = clamped(ctas[0], a.max_ctas - 1);
+    last[0] = clamped(ctas[1], a.max_ctas - 1);
+  }
+  if (rows > common) {
+    const int64_t item = (int64_t)h * a.batch + b;
+    part[1] = a.part_own + item * a.gs;
+    ctas = a.meta + 2 * (item + (int64_t)a.hk * a.batch);
+    first[1] = clamped(ctas[0], a.max_ctas - 1);
+    last[1] = clamped(ctas[1], a.max_ctas - 1);
+  }
+  if (quad >= RI_HEAD_DIM / 4) return;
+  const int each[2] = {a.part_rows, a.gs};
+  Joined all;
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+#pragma unroll 4
+    for (int c = first[x]; c <= last[x]; ++c) all.add(a.part_ml[part[x] + (int64_t)c * each[x] + row[x]]);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+#pragma unroll 4
+    for (int c = first[x]; c <= last[x]; ++c) {
+      const int64_t at = part[x] + (int64_t)c * each[x];
+      const float f = part_factor(a.part_ml[at + row[x]].x, all.m);
+      const float4 y = reinterpret_cast<const float4*>(a.part_o + at * RI_HEAD_DIM)[quad * n_rows[x] + row[x]];
+      o.x += f * y.x; o.y += f * y.y; o.z += f * y.z; o.w += f * y.w;
+    }
+  const float f = all.scale();
+  const int64_t at = ((int64_t)b * a.hk + h) * a.gs + r;
+  *reinterpret_cast<uint2*>(a.out + at * RI_HEAD_DIM + quad * 4) = make_uint2(Elem<DT>::pack2(o.x * f, o.y * f), Elem<DT>::pack2(o.z * f, o.w * f));
+  if (quad == 0 && a.lse != nullptr) a.lse[at] = all.lse();
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------
+// Queries as (channel of a half, head, half, row): a box is one half of the query heads of a KV head, of a tile's tokens.
+int make_query_map(CUtensorMap* map, const void* q, int64_t q_stride, int q_heads, int rows, int gs, int tokens, int dtype) {
+  EncodeTiledFn enc;
+  const int rc = get_encode_fn(&enc);
+  if (rc != RI_OK) return rc;
+  const cuuint64_t dims[4] = {RI_HEAD_DIM / 2, (cuuint64_t)q_heads, 2, (cuuint64_t)rows};
+  const cuuint64_t strides[3] = {256, 128, (cuuint64_t)q_stride * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)gs, 1, (cuuint32_t)tokens}, estr[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, dtype == RI_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(q),
+                         dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  RI_REQUIRE(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code %d", (int)r);
+  return RI_OK;
+}
+// Keys or values as (channel of a half, row of the page's heads, half, page): a box is one half of the channels of at most a page.
+int make_pool_map(CUtensorMap* map, const void* base, const ri_paged& p, int64_t page_stride) {
+  EncodeTiledFn enc;
+  const int rc = get_encode_fn(&enc);
+  if (rc != RI_OK) return rc;
+  const cuuint64_t dims[4] = {RI_HEAD_DIM / 2, (cuuint64_t)p.kv_heads * p.page_size, 2, (cuuint64_t)p.n_pages};
+  const cuuint64_t strides[3] = {256, 128, (cuuint64_t)page_stride * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)(p.page_size < kTile ? p.page_size : kTile), 1, 1}, estr[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, p.dtype == RI_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                         const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  RI_REQUIRE(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code %d", (int)r);
+  return RI_OK;
+}
+
+int64_t most_items_rows(const ri_paged& p, int rows) {      // rows of an item, at most
+  const int pair = 2 * (kTile / p.group_size);
+  return (int64_t)(rows < pair ? rows : pair) * p.group_size;
+}
+// Whether an item may be cut: it has more steps than two snaps.
+bool may_cut(const ri_paged& p, int rows, int window, int sink) {
+  const int64_t all = (slots_of(p) + kTile - 1) / kTile;
+  if (window == 0) return all > 2 * kSnap;
+  const int64_t pair = 2 * (kTile / p.group_size);
+  const int64_t seen = ((int64_t)window + (rows < pair ? rows : pair) + kTile - 3) / kTile + 1 + ((int64_t)sink + kTile - 1) / kTile;
+  return (seen < all ? seen : all) > 2 * kSnap;
+}
+
+int check_call(const char* what, const ri_paged* p, int64_t sequences) {
+  const int rc = check(p, what);
+  if (rc != RI_OK) return rc;
+  RI_REQUIRE(p->group_size >= 1 && p->group_size <= kHeadsMost, "%s: group_size=%d unsupported (1 to %d)", what, p->group_size, kHeadsMost);
+  RI_REQUIRE(sequences >= 1 && sequences <= kMaxRequests, "%s: %lld requests (and groups) unsupported (%d at most)", what, (long long)sequences,
+             kMaxRequests);
+  return RI_OK;
+}
+
+template <int DT, bool SHARED>
+int launch(const Args& a, const CUtensorMap& map_q, const CUtensorMap& map_k, const CUtensorMap& map_v, bool join, cudaStream_t s) {
+  const int rc = ri_allow_smem<paged_attend_kernel<DT, SHARED>>(kSmem);
+  if (rc != RI_OK) return rc;
+  RI_CUDA_OK(ri_launch_pdl_id(11, paged_attend_kernel<DT, SHARED>, dim3(a.max_ctas), dim3(kThreads), (size_t)kSmem, s, map_q, map_k, map_v, a));
+  if (SHARED) {
+    RI_CUDA_OK(ri_launch_pdl_id(11, shared_join_kernel<DT>, dim3(a.batch, a.hk), dim3(kJoinThreads), 0, s, a));
+  } else if (join) {
+    RI_CUDA_OK(ri_launch_pdl_id(11, prompt_join_kernel<DT>, dim3(a.max_ctas, (a.part_rows + kJoinRows - 1) / kJoinRows), dim3(kJoinThreads), 0, s, a));
+  }
+  return RI_OK;
+}
+
+template <bool SHARED>
+int attend(const char* what, const ri_paged* p, const void* d_q, int64_t q_stride, int rows, Args a, void* d_out, float* d_lse, float scale,
+           bool join, void* stream) {
+  int rc;
+  RI_REQUIRE(p->d_values && d_q && d_out && a.starts, "%s: null pointer", what);
+  RI_REQUIRE(q_stride >= (int64_t)p->kv_heads * p->group_size * RI_HEAD_DIM && q_stride % 8 == 0, "%s: queries overlap or lie at odd places", what);
+  RI_REQUIRE(((uintptr_t)d_q | (uintptr_t)d_out) % 16 == 0, "%s: tensors must be 16-byte aligned", what);
+  RI_REQUIRE(scale > 0.f && scale < 1e30f, "%s: scale must be positive and finite", what);
+  static_cast<Pages&>(a) = view(*p);
+  a.q = static_cast<const uint16_t*>(d_q);
+  a.q_stride = q_stride;
+  a.out = static_cast<uint16_t*>(d_out);
+  a.lse = d_lse;
+  a.n_rows = rows;
+  a.gs = p->group_size;
+  a.tile_tokens = kTile / a.gs;
+  a.part_rows = (int)most_items_rows(*p, rows);
+  a.scale2 = RI_LOG2E * scale;
+  a.keys = p->d_keys;
+  a.values = p->d_values;
+  a.idesc_qk = idesc_f16(p->dtype, kTile, kTile);
+  a.idesc_pv = a.idesc_qk | (1u << 16);      // B = V is MN-major (channels contiguous)
+  int sms = 0;
+  if ((rc = ri_sm_count(&sms)) != RI_OK) return rc;
+  a.max_ctas = sms < kMaxCtas ? sms : kMaxCtas;
+  CUtensorMap map_q, map_k, map_v;
+  if ((rc = make_query_map(&map_q, d_q, q_stride, p->kv_heads * a.gs, rows, a.gs, a.tile_tokens, p->dtype)) != RI_OK) return rc;
+  if ((rc = make_pool_map(&map_k, p->d_keys, *p, p->key_page_stride)) != RI_OK) return rc;
+  if ((rc = make_pool_map(&map_v, p->d_values, *p, p->value_page_stride)) != RI_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return p->dtype == RI_BF16 ? launch<RI_BF16, SHARED>(a, map_q, map_k, map_v, join, s) : launch<RI_F16, SHARED>(a, map_q, map_k, map_v, join, s);
+}
+
+// Workspaces: meta, sums, outputs of the parts.
+int64_t prompt_part_rows(const ri_paged& p, int rows) { return 2 * kMaxCtas * most_items_rows(p, rows); }
+constexpr int64_t kPromptMeta = (int64_t)kMaxCtas * kMeta * 4;
+int64_t shared_meta(const ri_paged& p) { return ri_align_up(16 * (int64_t)p.batch * p.kv_heads, 16); }
+int64_t shared_rows(const ri_paged& p) { return (int64_t)kMaxCtas * most_items_rows(p, p.batch) + (int64_t)p.batch * p.kv_heads * p.group_size; }
+int64_t own_rows(const ri_paged& p) { return ((int64_t)kMaxCtas + (int64_t)p.batch * p.kv_heads) * p.group_size; }
+void place(Args& a, void* d_scratch, int64_t meta, int64_t rows) {
+  a.meta = static_cast<int*>(d_scratch);
+  a.part_o = reinterpret_cast<float*>(static_cast<char*>(d_scratch) + meta);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * RI_HEAD_DIM);
+}
+
+}  // namespace
+
+extern "C" int64_t ri_paged_prompt_scratch_bytes(const ri_paged* p, int32_t rows, int32_t window, int32_t sink) {
+  const int rc = check_call("ri_paged_prompt", p, p ? p->batch : 1);
+  if (rc != RI_OK) return rc;
+  if (rows < 1 || window < 0 || sink < 0) return ri_fail(RI_ERR_INVALID, "ri_paged_prompt: rows=%d window=%d sink=%d unsupported", rows, window, sink);
+  return may_cut(*p, rows, window, sink) ? kPromptMeta + prompt_part_rows(*p, rows) * (RI_HEAD_DIM + 2) * 4 : 0;
+}
+
+extern "C" int ri_paged_prompt(const ri_paged* p, const void* d_q, int64_t q_stride, int32_t rows, const int32_t* d_row_start, int32_t window,
+                               int32_t sink, void* d_out, float* d_lse, float scale, void* d_scratch, void* stream) {
+  const int64_t bytes = ri_paged_prompt_scratch_bytes(p, rows, window, sink);
+  if (bytes < 0) return (int)bytes;
+  RI_REQUIRE((bytes == 0 || d_scratch) && (uintptr_t)d_scratch % 16 == 0, "ri_paged_prompt: the scratch must be there and 16-byte aligned");
+  Args a = {};
+  a.starts = d_row_start;
+  a.n_seq = p->batch;
+  a.window = window;
+  a.sink = sink;
+  if (bytes > 0) place(a, d_scratch, kPromptMeta, prompt_part_rows(*p, rows));
+  return attend<false>("ri_paged_prompt", p, d_q, q_stride, rows, a, d_out, d_lse, scale, bytes > 0, stream);
+}
+
+extern "C" int64_t ri_paged_shared_decode_scratch_bytes(const ri_paged* p, int32_t groups) {
+  const int rc = check_call("ri_paged_shared_decode", p, p ? (int64_t)p->batch + (groups > 0 ? groups : 0) : 1);
+  if (rc != RI_OK) return rc;
+  if (groups < 1) return ri_fail(RI_ERR_INVALID, "ri_paged_shared_decode: groups=%d unsupported", groups);
+  return shared_meta(*p) + (shared_rows(*p) + own_rows(*p)) * (RI_HEAD_DIM + 2) * 4;
+}
+
+extern "C" int ri_paged_shared_decode(const ri_paged* p, const void* d_q, int64_t q_stride, const int32_t* d_group_start, int32_t groups,
+                                      const int32_t* d_shared, void* d_out, float* d_lse, float scale, void* d_scratch, void* stream) {
+  const int64_t bytes = ri_paged_shared_decode_scratch_bytes(p, groups);
+  if (bytes < 0) return (int)bytes;
+  RI_REQUIRE(d_shared && d_scratch, "ri_paged_shared_decode: null pointer");
+  RI_REQUIRE((uintptr_t)d_scratch % 16 == 0, "ri_paged_shared_decode: the scratch must be 16-byte aligned");
+  Args a = {};
+  a.starts = d_group_start;
+  a.shared = d_shared;
+  a.groups = groups;
+  a.n_seq = groups + p->batch;
+  a.part_own = shared_rows(*p);
+  place(a, d_scratch, shared_meta(*p), shared_rows(*p) + own_rows(*p));
+  return attend<true>("ri_paged_shared_decode", p, d_q, q_stride, p->batch, a, d_out, d_lse, scale, true, stream);
+}

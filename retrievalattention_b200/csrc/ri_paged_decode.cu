@@ -17,6 +17,8 @@
 // leaves the scores behind (4 bytes a slot and query head, against 512 a slot for K and V), and the second turns them into
 // probabilities; every slot has one thread, so the sums have one order and no atomics.
 // Short requests that leave the chip room give every group a cluster of CTAs, which does all of this in one kernel.
+// With a window the steps between the first slots and the window are left out: they take no part in the split, and nothing of
+// them, their page numbers among it, is read.
 // B200, bf16, 8 heads of 4: 4 x 131072 slots 318 to 345 us by the GPU, 6.2 to 6.8 TB/s (a copy: 6.6); 4 requests of 20K to 32K with
 // weights 91 us, 4.8 TB/s: the SMs are done after 64 to 78 us, half of them by 68 (some two dozen SMs are the last in every case,
 // whatever the page size, the lengths or the groups of a CTA; without the scores all are done 5 us earlier), and the second kernel
@@ -70,6 +72,35 @@ struct PagedArgs : Pages {
 };
 __device__ __forceinline__ int used_ctas(int total, int max_ctas) { return ri_seq::used_ctas<kPagedWarps>(total, max_ctas); }
 
+// Where a request's rows lie among its slots.
+struct AllSlots {
+  __device__ __forceinline__ int slot(int row) const { return row; }
+  __device__ __forceinline__ bool sees(int row, int rows) const { return row < rows; }
+  __device__ __forceinline__ bool sees_step(int row, int rows) const { return row + 16 <= rows; }      // all of it
+};
+__device__ __forceinline__ AllSlots span_of(const PagedArgs&, int) { return {}; }
+
+// A window: only the last `window` slots and the first `sink` are seen.  Between the two whole steps are left out, so that rows
+// count on behind the first slots' last step where the window's first one begins; the slots of those two that are not seen are masked.
+struct WindowArgs : PagedArgs {
+  int window, sink;
+};
+struct WindowSpan {
+  int front, skip, low, sink;            // rows in front of the gap, slots left out, the window's first slot
+  __device__ __forceinline__ int slot(int row) const { return row < front ? row : row + skip; }
+  __device__ __forceinline__ bool sees(int row, int rows) const { return row < rows && (slot(row) >= low || slot(row) < sink); }
+  __device__ __forceinline__ bool sees_step(int row, int rows) const {
+    return row + 16 <= rows && max(slot(row), sink) >= min(slot(row) + 16, low);
+  }
+};
+__device__ __forceinline__ WindowSpan span_of(const WindowArgs& a, int b) {
+  const int n = ri_page::rows_of(static_cast<const Pages&>(a), b), low = max(0, n - a.window), front = (min(a.sink, low) + 15) & ~15;
+  return {front, max(0, (low & ~15) - front), low, a.sink};
+}
+__device__ __forceinline__ int rows_of(const WindowArgs& a, int b) {
+  return ri_page::rows_of(static_cast<const Pages&>(a), b) - span_of(a, b).skip;
+}
+
 // The scores of a step lie in the order of the lanes that made them: place i holds key (i / 2 % 2) * 8 + i / 4 + (i % 2) * 4.
 __device__ __forceinline__ int slot_in_step(int place) { return (place & ~15) + ((place >> 1) & 1) * 8 + ((place >> 2) & 3) + (place & 1) * 4; }
 
@@ -84,11 +115,11 @@ __device__ __forceinline__ uint2 two_parts(float p0, float p1) {
 }
 
 // BOX: rows of a TMA box.  CLUSTER: a group per cluster, which shares out the group's steps, joins the partial results through
-// distributed shared memory and adds the weights: no second kernel.  LONG: see kLongSteps.
-template <int DT, int BOX, bool WEIGHTS, bool CLUSTER, bool LONG>
+// distributed shared memory and adds the weights: no second kernel.  LONG: see kLongSteps.  Args: PagedArgs or WindowArgs.
+template <int DT, int BOX, bool WEIGHTS, bool CLUSTER, bool LONG, class Args>
 __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                      const __grid_constant__ CUtensorMap map_v,
-                                                                     const __grid_constant__ PagedArgs a) {
+                                                                     const __grid_constant__ Args a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ __align__(8) uint64_t s_full[kPagedWarps][kStages];
@@ -204,22 +235,28 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
     Place at_issue = CLUSTER ? c_first : find_place(a, lo), at = at_issue;
     // pages of the next step to issue; the second one only where a page is half a step
     int id0 = 0, id1 = 0;
+    auto span_issue = span_of(a, at_issue.g / a.hk), span = span_issue;
     auto fetch_ids = [&](int s) {
-      while (s >= at_issue.first + steps_of(at_issue.rows)) next_place(a, at_issue);
-      const int b = at_issue.g / a.hk, row = (s - at_issue.first) * 16;
-      id0 = page_of(a, b, row >> a.shift);
-      if (BOX == 8 && row + 8 < at_issue.rows) id1 = page_of(a, b, (row + 8) >> a.shift);
+      if (s >= at_issue.first + steps_of(at_issue.rows)) {
+        do next_place(a, at_issue);
+        while (s >= at_issue.first + steps_of(at_issue.rows));
+        span_issue = span_of(a, at_issue.g / a.hk);
+      }
+      const int b = at_issue.g / a.hk, row = (s - at_issue.first) * 16, slot = span_issue.slot(row);
+      id0 = page_of(a, b, slot >> a.shift);
+      if (BOX == 8 && row + 8 < at_issue.rows) id1 = page_of(a, b, (slot + 8) >> a.shift);
     };
     auto issue = [&](int s, int stage) {
       if (lane == 0) {
         const uint32_t dst = my_ring_u32 + stage * kStageStride, bar = my_full + 8 * stage;
-        const int row = (s - at_issue.first) * 16, in_page = ((at_issue.g % a.hk) << a.shift) + (row & ((1 << a.shift) - 1));
+        const int row = (s - at_issue.first) * 16, slot = span_issue.slot(row);
+        const int in_page = ((at_issue.g % a.hk) << a.shift) + (slot & ((1 << a.shift) - 1));
         const bool second = BOX == 8 && row + 8 < at_issue.rows;
         mbar_arrive_expect_tx(bar, (BOX == 16 || second) ? kStageBytes : kStageBytes / 2);
         tma_load_4d(dst, &map_k, bar, 0, in_page, 0, id0);
         tma_load_4d(dst + kTensor, &map_v, bar, 0, in_page, 0, id0);
         if (second) {
-          const int in_next = ((at_issue.g % a.hk) << a.shift) + ((row + 8) & ((1 << a.shift) - 1));
+          const int in_next = ((at_issue.g % a.hk) << a.shift) + ((slot + 8) & ((1 << a.shift) - 1));
           tma_load_4d(dst + kBox, &map_k, bar, 0, in_next, 0, id1);
           tma_load_4d(dst + kTensor + kBox, &map_v, bar, 0, in_next, 0, id1);
         }
@@ -250,6 +287,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
         clear();
         do next_place(a, at);
         while (s >= at.first + steps_of(at.rows));
+        span = span_of(a, at.g / a.hk);
         load_q();
       }
       const int base = (s - at.first) * 16;
@@ -269,7 +307,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          s2[jj][e] = base + jj * 8 + t + 4 * e < at.rows ? (c1[e] + c2[e]) * a.scale2 : -INFINITY;
+          s2[jj][e] = span.sees(base + jj * 8 + t + 4 * e, at.rows) ? (c1[e] + c2[e]) * a.scale2 : -INFINITY;
       }
       if (WEIGHTS && r < gs)
         reinterpret_cast<float4*>(a.scores)[((score_step + s) * gs + r) * 4 + t] = make_float4(s2[0][0], s2[0][1], s2[1][0], s2[1][1]);
@@ -321,10 +359,11 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
         issue(s_issue++, stage);
         if (s_issue < hi) fetch_ids(s_issue);
       }
-      if (base + 16 > at.rows) {                      // a group's last step: what lies behind its rows may be anything
+      // what lies behind a group's rows, or in front of its window, may be anything
+      if (!span.sees_step(base, at.rows)) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (base + t + 4 * i >= at.rows) v[i][0] = v[i][1] = make_uint4(0, 0, 0, 0);
+          if (!span.sees(base + t + 4 * i, at.rows)) v[i][0] = v[i][1] = make_uint4(0, 0, 0, 0);
       }
       const uint2 b0 = two_parts<DT>(p[0][0], p[0][1]), b1 = two_parts<DT>(p[1][0], p[1][1]);
       pv_step<DT, true>(last, v, b0.x, b1.x, b0.y, b1.y);
@@ -427,8 +466,8 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
 constexpr int kFoldEach = 2, kFoldSlots = kFoldEach * kFinishThreads;
 constexpr int kFinishBlocks = 4;                         // of an SM
 constexpr int kTogether = 4;                             // partial results of a warp on their way
-template <int DT>
-__global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_kernel(const __grid_constant__ PagedArgs a) {
+template <int DT, class Args>
+__global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_kernel(const __grid_constant__ Args a) {
   extern __shared__ int s_slot[];                        // [most partial results of a group]
   __shared__ float s_m[kMaxHeads], s_l[kMaxHeads], s_o[kFinishThreads / 32][RI_HEAD_DIM];
   __shared__ int s_n;
@@ -630,8 +669,8 @@ int clusters_at_once(int ctas, int* out) {
   RI_CUDA_OK(cudaGetDevice(&dev));
   const bool track = dev >= 0 && dev < 64;
   if (track && (*out = known[dev][ctas].load(std::memory_order_relaxed)) > 0) return RI_OK;
-  auto* kernel = paged_decode_kernel<RI_BF16, 16, true, true, false>;      // all of them have the same shared memory and threads
-  if ((rc = ri_allow_smem<paged_decode_kernel<RI_BF16, 16, true, true, false>>(kPagedSmem)) != RI_OK) return rc;
+  auto* kernel = paged_decode_kernel<RI_BF16, 16, true, true, false, PagedArgs>;      // all of them have the same shared memory and threads
+  if ((rc = ri_allow_smem<paged_decode_kernel<RI_BF16, 16, true, true, false, PagedArgs>>(kPagedSmem)) != RI_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kPagedThreads);
@@ -651,8 +690,8 @@ int clusters_at_once(int ctas, int* out) {
 // warp on (8 heads of 4, a call: 777 slots 11.3 us with two kernels, 9.6 with clusters; 4000 slots, four steps a warp, 11.6 and
 // 9.7; 8000 slots 13.9 and 14.9).
 constexpr int kClusterSteps = 4;                       // of a warp, at most
-int cluster_size(const PagedArgs& a, int* ctas) {
-  const int64_t groups = (int64_t)a.batch * a.hk, steps = (((int64_t)a.width << a.shift) + 15) / 16;
+int cluster_size(const PagedArgs& a, int64_t most, int* ctas) {
+  const int64_t groups = (int64_t)a.batch * a.hk, steps = (most + 15) / 16;
   *ctas = 0;
   if (groups > a.max_ctas || steps > kMaxCluster * kPagedWarps * kClusterSteps) return RI_OK;
   for (int n = 1; n <= kMaxCluster; n *= 2) {
@@ -664,38 +703,49 @@ int cluster_size(const PagedArgs& a, int* ctas) {
   if (steps > (int64_t)*ctas * kPagedWarps * kClusterSteps) *ctas = 0;
   return RI_OK;
 }
-template <int DT, int BOX, bool WEIGHTS, bool LONG>
-int launch_split(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t s) {
-  const int rc = ri_allow_smem<paged_decode_kernel<DT, BOX, WEIGHTS, false, LONG>>(kPagedSmem);
+// The most rows that a request may have.
+int64_t most_rows(const PagedArgs& a) { return (int64_t)a.width << a.shift; }
+int64_t most_rows(const WindowArgs& a) {
+  const int64_t all = most_rows(static_cast<const PagedArgs&>(a)), seen = (int64_t)a.window + a.sink + 30;      // two steps begun
+  return seen < all ? seen : all;
+}
+template <int DT, int BOX, bool WEIGHTS, bool LONG, class Args>
+int launch_split(const Args& a, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t s) {
+  const int rc = ri_allow_smem<paged_decode_kernel<DT, BOX, WEIGHTS, false, LONG, Args>>(kPagedSmem);
   if (rc != RI_OK) return rc;
-  RI_CUDA_OK(ri_launch_pdl_id(11, paged_decode_kernel<DT, BOX, WEIGHTS, false, LONG>, dim3(a.max_ctas), dim3(kPagedThreads), (size_t)kPagedSmem, s,
-                              map_k, map_v, a));
+  RI_CUDA_OK(ri_launch_pdl_id(11, paged_decode_kernel<DT, BOX, WEIGHTS, false, LONG, Args>, dim3(a.max_ctas), dim3(kPagedThreads), (size_t)kPagedSmem,
+                              s, map_k, map_v, a));
   return RI_OK;
 }
-template <int DT, int BOX, bool WEIGHTS>
-int launch_steps(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, int ctas, cudaStream_t s) {
+template <int DT, int BOX, bool WEIGHTS, class Args>
+int launch_steps(const Args& a, const CUtensorMap& map_k, const CUtensorMap& map_v, int ctas, cudaStream_t s) {
   int rc;
   if (ctas > 0) {
-    if ((rc = ri_allow_smem<paged_decode_kernel<DT, BOX, WEIGHTS, true, false>>(kPagedSmem)) != RI_OK) return rc;
-    RI_CUDA_OK(ri_launch_pdl_cluster(11, ctas, paged_decode_kernel<DT, BOX, WEIGHTS, true, false>, dim3(a.batch * a.hk * ctas), dim3(kPagedThreads),
+    if ((rc = ri_allow_smem<paged_decode_kernel<DT, BOX, WEIGHTS, true, false, Args>>(kPagedSmem)) != RI_OK) return rc;
+    RI_CUDA_OK(ri_launch_pdl_cluster(11, ctas, paged_decode_kernel<DT, BOX, WEIGHTS, true, false, Args>, dim3(a.batch * a.hk * ctas), dim3(kPagedThreads),
                                      (size_t)kPagedSmem, s, map_k, map_v, a));
     return RI_OK;
   }
-  const int64_t steps = (int64_t)a.batch * a.hk * ((((int64_t)a.width << a.shift) + 15) / 16);
+  const int64_t steps = (int64_t)a.batch * a.hk * ((most_rows(a) + 15) / 16);
   return steps > (int64_t)a.max_ctas * kPagedWarps * kLongSteps ? launch_split<DT, BOX, WEIGHTS, true>(a, map_k, map_v, s)
                                                                 : launch_split<DT, BOX, WEIGHTS, false>(a, map_k, map_v, s);
 }
 template <int DT, int BOX>
 int launch_steps(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, int ctas, cudaStream_t s) {
-  return a.weight ? launch_steps<DT, BOX, true>(a, map_k, map_v, ctas, s) : launch_steps<DT, BOX, false>(a, map_k, map_v, ctas, s);
+  return a.weight ? launch_steps<DT, BOX, true, PagedArgs>(a, map_k, map_v, ctas, s) : launch_steps<DT, BOX, false, PagedArgs>(a, map_k, map_v, ctas, s);
 }
-template <int DT>
-int launch_paged(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, int box, cudaStream_t s) {
+template <int DT, int BOX>
+int launch_steps(const WindowArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, int ctas, cudaStream_t s) {
+  return launch_steps<DT, BOX, false, WindowArgs>(a, map_k, map_v, ctas, s);
+}
+template <int DT, class Args>
+int launch_paged(const Args& a, const CUtensorMap& map_k, const CUtensorMap& map_v, int box, cudaStream_t s) {
+  const int64_t most = most_rows(a);
   int ctas, rc;
-  if ((rc = cluster_size(a, &ctas)) != RI_OK) return rc;
+  if ((rc = cluster_size(a, most, &ctas)) != RI_OK) return rc;
   rc = box == 8 ? launch_steps<DT, 8>(a, map_k, map_v, ctas, s) : launch_steps<DT, 16>(a, map_k, map_v, ctas, s);
   if (rc != RI_OK || ctas > 0) return rc;
-  const int64_t groups = (int64_t)a.batch * a.hk, most = (int64_t)a.width << a.shift;
+  const int64_t groups = (int64_t)a.batch * a.hk;
   // blocks of a group: for its heads, or with weights its tiles of slots, as many as the chip holds at once
   const int64_t tiles = a.weight ? (most + kFoldSlots - 1) / kFoldSlots : 0, room = kFinishBlocks * (int64_t)a.max_ctas / groups;
   int64_t blocks = tiles > a.gs ? tiles : a.gs;
@@ -703,7 +753,7 @@ int launch_paged(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap
   // partial results of a group: its steps, or all that there are and one more
   const int64_t steps = (most + 15) / 16, parts = (int64_t)a.max_ctas * kPagedWarps;
   const size_t smem = (size_t)(steps < parts ? steps : parts) * 4 + 4;
-  RI_CUDA_OK(ri_launch_pdl_id(11, paged_finish_kernel<DT>, dim3((unsigned)blocks, (unsigned)groups), dim3(kFinishThreads), smem, s, a));
+  RI_CUDA_OK(ri_launch_pdl_id(11, paged_finish_kernel<DT, Args>, dim3((unsigned)blocks, (unsigned)groups), dim3(kFinishThreads), smem, s, a));
   return RI_OK;
 }
 
@@ -719,19 +769,20 @@ extern "C" int64_t ri_paged_decode_scratch_bytes(const ri_paged* p) {
   return floats * 4;
 }
 
-extern "C" int ri_paged_decode(const ri_paged* p, const void* d_q, int64_t q_stride, void* d_out, float* d_lse, float scale,
-                               void* d_scratch, void* stream) {
-  using namespace ri_wave;
+namespace ri_wave {
+namespace {
+
+// window 0: none
+int decode(const char* what, const ri_paged* p, const void* d_q, int64_t q_stride, void* d_out, float* d_lse, float scale, int32_t window,
+           int32_t sink, void* d_scratch, void* stream) {
   int rc;
-  if ((rc = ri_page::check(p, "ri_paged_decode")) != RI_OK) return rc;
-  RI_REQUIRE(p->d_values && d_q && d_out && d_scratch, "ri_paged_decode: null pointer");
-  RI_REQUIRE(p->group_size >= 1 && p->group_size <= kMaxHeads, "ri_paged_decode: group_size=%d unsupported (1 to %d)", p->group_size,
-             kMaxHeads);
-  RI_REQUIRE(q_stride >= (int64_t)p->kv_heads * p->group_size * RI_HEAD_DIM && q_stride % 8 == 0,
-             "ri_paged_decode: queries overlap or lie at odd places");
+  if ((rc = ri_page::check(p, what)) != RI_OK) return rc;
+  RI_REQUIRE(p->d_values && d_q && d_out && d_scratch, "%s: null pointer", what);
+  RI_REQUIRE(p->group_size >= 1 && p->group_size <= kMaxHeads, "%s: group_size=%d unsupported (1 to %d)", what, p->group_size, kMaxHeads);
+  RI_REQUIRE(q_stride >= (int64_t)p->kv_heads * p->group_size * RI_HEAD_DIM && q_stride % 8 == 0, "%s: queries overlap or lie at odd places", what);
   RI_REQUIRE(((uintptr_t)d_q | (uintptr_t)d_out | (uintptr_t)d_scratch) % 16 == 0, "q, out and the scratch must be 16-byte aligned");
-  RI_REQUIRE(scale > 0.f && scale < 1e30f, "ri_paged_decode: scale must be positive and finite");
-  PagedArgs a = {};
+  RI_REQUIRE(scale > 0.f && scale < 1e30f, "%s: scale must be positive and finite", what);
+  WindowArgs a = {};
   static_cast<ri_page::Pages&>(a) = ri_page::view(*p);
   a.q = static_cast<const uint4*>(d_q);
   a.q_stride = q_stride / 8;
@@ -744,6 +795,8 @@ extern "C" int ri_paged_decode(const ri_paged* p, const void* d_q, int64_t q_str
   a.lse = d_lse;
   a.out = static_cast<uint16_t*>(d_out);
   a.scale2 = RI_LOG2E * scale;
+  a.window = window;
+  a.sink = sink;
   int sms = 0;
   if ((rc = ri_sm_count(&sms)) != RI_OK) return rc;
   a.max_ctas = sms < kPagedMaxCtas ? sms : kPagedMaxCtas;
@@ -752,5 +805,22 @@ extern "C" int ri_paged_decode(const ri_paged* p, const void* d_q, int64_t q_str
   if ((rc = make_page_map(&map_k, p->d_keys, *p, p->key_page_stride, box)) != RI_OK) return rc;
   if ((rc = make_page_map(&map_v, p->d_values, *p, p->value_page_stride, box)) != RI_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const PagedArgs& all = a;
+  if (window == 0) return p->dtype == RI_BF16 ? launch_paged<RI_BF16>(all, map_k, map_v, box, s) : launch_paged<RI_F16>(all, map_k, map_v, box, s);
   return p->dtype == RI_BF16 ? launch_paged<RI_BF16>(a, map_k, map_v, box, s) : launch_paged<RI_F16>(a, map_k, map_v, box, s);
+}
+
+}  // namespace
+}  // namespace ri_wave
+
+extern "C" int ri_paged_decode(const ri_paged* p, const void* d_q, int64_t q_stride, void* d_out, float* d_lse, float scale,
+                               void* d_scratch, void* stream) {
+  return ri_wave::decode("ri_paged_decode", p, d_q, q_stride, d_out, d_lse, scale, 0, 0, d_scratch, stream);
+}
+
+extern "C" int ri_paged_decode_window(const ri_paged* p, const void* d_q, int64_t q_stride, int32_t window, int32_t sink, void* d_out,
+                                      float* d_lse, float scale, void* d_scratch, void* stream) {
+  RI_REQUIRE(window >= 1 && sink >= 0, "ri_paged_decode_window: window=%d sink=%d unsupported", window, sink);
+  RI_REQUIRE(p == nullptr || p->d_weight == nullptr, "ri_paged_decode_window: weights are added up over all slots, not over a window");
+  return ri_wave::decode("ri_paged_decode_window", p, d_q, q_stride, d_out, d_lse, scale, window, sink, d_scratch, stream);
 }

@@ -55,14 +55,27 @@ def rmsnorm(x, weight, eps, out, residual=None):
     return out
 
 
-def rope_split(qkv, cos_sin, positions, q, k, v):
-    """Rotate the query/key heads of ``qkv`` ``[rows, (Hq+2Hk)*128]`` at ``positions`` and split into ``q, k, v``."""
+def rope_split(qkv, cos_sin, positions, q, k, v, q_norm=None, k_norm=None, eps=1e-6):
+    """Rotate the query/key heads of ``qkv`` ``[rows, (Hq+2Hk)*128]`` at ``positions`` and split into ``q, k, v``.  ``q_norm`` and
+    ``k_norm`` (``[128]``, or ``[heads, 128]``, of qkv's type): RMS norms of every query and key head in front of the rotation."""
     rows, q_heads, kv_heads = q.shape[0], q.shape[-2], k.shape[-2]
     assert qkv.shape == (rows, (q_heads + 2 * kv_heads) * 128) and cos_sin.dtype == torch.float32
     assert cos_sin.shape[1] == 128 and positions.dtype == torch.int64 and positions.numel() == rows
-    _lib.check(_lib.lib.ri_rope_split(qkv.data_ptr(), cos_sin.data_ptr(), positions.data_ptr(), q.data_ptr(),
-                                      k.data_ptr(), v.data_ptr(), rows, q_heads, kv_heads, cos_sin.shape[0],
-                                      _lib.dtype_code(qkv.dtype), _lib.current_stream()), "ri_rope_split")
+    if q_norm is None and k_norm is None:
+        _lib.check(_lib.lib.ri_rope_split(qkv.data_ptr(), cos_sin.data_ptr(), positions.data_ptr(), q.data_ptr(),
+                                          k.data_ptr(), v.data_ptr(), rows, q_heads, kv_heads, cos_sin.shape[0],
+                                          _lib.dtype_code(qkv.dtype), _lib.current_stream()), "ri_rope_split")
+        return
+    for w, heads in ((q_norm, q_heads), (k_norm, kv_heads)):
+        if w is None or w.dtype != qkv.dtype or w.device != qkv.device or not w.is_contiguous() or w.requires_grad or \
+                w.shape not in ((128,), (heads, 128)):
+            raise ValueError("rope_split: expected dense q_norm and k_norm [128] or [heads, 128] of qkv's type on its GPU")
+    if not 0 <= eps < 1e30:
+        raise ValueError("rope_split: eps must be finite and not negative")
+    _lib.check(_lib.lib.ri_rope_split_norm(qkv.data_ptr(), cos_sin.data_ptr(), positions.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(),
+                                           q_heads if q_norm.dim() == 2 else 1, kv_heads if k_norm.dim() == 2 else 1, float(eps),
+                                           q.data_ptr(), k.data_ptr(), v.data_ptr(), rows, q_heads, kv_heads, cos_sin.shape[0],
+                                           _lib.dtype_code(qkv.dtype), _lib.current_stream()), "ri_rope_split_norm")
 
 
 def silu_and_mul(x, out):

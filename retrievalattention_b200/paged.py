@@ -1,8 +1,11 @@
 """Operators over one layer of a paged KV cache.
 
-* ``rope_paged_append``  rotary positions with several axes (text, images, video) on a fused QKV projection; queries out, keys and
-                         values into the cache's pages;
-* ``paged_decode``       attention of one new token over the pages, optionally adding up the weight that every slot gets;
+* ``rope_paged_append``  rotary positions with several axes (text, images, video) on a fused QKV projection, behind norms of the query
+                         and key heads where a model has them; queries out, keys and values into the cache's pages;
+* ``paged_decode``       attention of one new token over the pages, optionally adding up the weight that every slot gets, or over a
+                         window of the last slots and a few first ones;
+* ``paged_prompt``       the same of several new tokens: prompts of uneven lengths, or pieces of prompts behind what is cached;
+* ``paged_shared_decode``  of one new token of requests that have their first slots in common, which are read once for all;
 * ``paged_observe``      the weight that a prompt's last queries give to its slots;
 * ``paged_evict``        the slots of least weight give way, in place.
 
@@ -47,8 +50,9 @@ def _connect():
     spec = importlib.util.spec_from_file_location("_paged_binding", _BINDING)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
-    names = ("ri_last_error", "ri_rope_paged_append", "ri_paged_decode_scratch_bytes", "ri_paged_decode",
-             "ri_paged_observe_scratch_bytes", "ri_paged_observe", "ri_paged_evict_scratch_bytes", "ri_paged_evict")
+    names = ("ri_last_error", "ri_rope_paged_append", "ri_rope_paged_append_norm", "ri_paged_decode_scratch_bytes", "ri_paged_decode",
+             "ri_paged_decode_window", "ri_paged_prompt_scratch_bytes", "ri_paged_prompt", "ri_paged_shared_decode_scratch_bytes",
+             "ri_paged_shared_decode", "ri_paged_observe_scratch_bytes", "ri_paged_observe", "ri_paged_evict_scratch_bytes", "ri_paged_evict")
     addresses = {n: C.cast(getattr(_lib.lib, n), C.c_void_p).value for n in names}
     addresses["status_word"] = _status.address()
     module.connect(addresses, _status.used, _status.report_word)
@@ -87,7 +91,7 @@ def _axes(axis_of) -> bytes:
 
 
 def rope_paged_append(qkv, cos_sin, positions, axis_of, q, key_pages, value_pages, page_table, lengths, row_start=None, *, weight=None,
-                      token=None, seen=None, keys=None, values=None):
+                      token=None, seen=None, keys=None, values=None, q_norm=None, k_norm=None, eps=1e-6):
     """Rotate the query and key heads of ``qkv`` ``[rows, (q_heads + 2 kv_heads) * 128]`` (rows may lie apart), write the queries to
     ``q`` ``[rows, q_heads, 128]`` and keys and values to the cache, behind the ``lengths`` slots in use (which stay as they are: add
     the rows once the last layer has its own).
@@ -97,19 +101,46 @@ def rope_paged_append(qkv, cos_sin, positions, axis_of, q, key_pages, value_page
     ``axis_of``.  Rows ``row_start[b]`` to ``row_start[b + 1] - 1`` (int32 ``[batch + 1]``) are request ``b``'s; without it row ``b``
     is.  Where ``weight`` and ``token`` are given, the new slots start with weight 0 and the token numbers ``seen[b]``,
     ``seen[b] + 1``, ...  ``keys`` and ``values`` ``[rows, kv_heads, 128]`` take the rows a second time, as
-    ``retroinfer_prefill_attn`` reads them."""
+    ``retroinfer_prefill_attn`` reads them.
+
+    ``q_norm`` and ``k_norm`` (of the pages' type, ``[128]`` or with a weight for every head ``[heads, 128]``): every query and key head is
+    divided by the root of its mean square (plus ``eps``) and multiplied by them in front of the rotation, in 32 bits."""
     native = _native or _connect()
     native.append(qkv, cos_sin, positions, _axes(axis_of), q, key_pages, value_pages, page_table, lengths, row_start, weight, token,
-                  seen, keys, values)
+                  seen, keys, values, q_norm, k_norm, eps)
 
 
-def paged_decode(q, key_pages, value_pages, page_table, lengths, *, out=None, lse=None, weight=None, scale=None):
+def paged_decode(q, key_pages, value_pages, page_table, lengths, *, out=None, lse=None, weight=None, scale=None, window=None, sink=0):
     """Attention of one new token: ``q`` ``[batch, 1, q_heads, 128]`` (requests may lie apart; one to eight query heads to a KV
     head) over the slots in use, which the token's own row is one of.  Returns ``out`` like ``q``; ``lse`` fp32 ``[batch, q_heads]``
     takes the log-sum-exp of the scaled scores (``scale``: 1/sqrt(128)).  A request without slots has out 0 and lse -infinity.
-    ``weight``: every slot's weight grows by the probabilities it got, summed over the query heads of its KV head."""
+    ``weight``: every slot's weight grows by the probabilities it got, summed over the query heads of its KV head.
+
+    ``window``: only the last ``window`` slots are seen, and the first ``sink`` (no ``weight`` then, and no eviction before: slots must
+    be in the order of their tokens).  Steps of 16 slots between the two are not read, nor are their page numbers."""
     native = _native or _connect()
-    return native.decode(q, key_pages, value_pages, page_table, lengths, out, lse, weight, _SCALE if scale is None else scale)
+    return native.decode(q, key_pages, value_pages, page_table, lengths, out, lse, weight, _SCALE if scale is None else scale, window, sink)
+
+
+def paged_prompt(q, key_pages, value_pages, page_table, lengths, row_start, *, window=None, sink=0, out=None, lse=None, scale=None):
+    """Attention of several new tokens of every request over the pages, whole prompts or pieces of them: rows ``row_start[b]`` to
+    ``row_start[b + 1] - 1`` (int32 ``[batch + 1]``, ascending) of ``q`` ``[rows, q_heads, 128]`` (rows may lie apart; one to eight query
+    heads to a KV head) are the last of request ``b``'s slots in use, whose keys and values are in the cache (``rope_paged_append``).
+    The token at slot ``s`` sees the slots up to ``s``; with ``window`` only the last ``window`` of them, and the first ``sink``.  Returns ``out``
+    ``[rows, q_heads, 128]``; ``lse`` fp32 ``[rows, q_heads]`` takes the log-sum-exp.  Rows that belong to no request are left alone;
+    a row in front of its request's first slot (more rows than slots) has out 0 and lse -infinity.  Slots must be in the order of their
+    tokens.  Pages that no row sees are not read, nor are their numbers."""
+    native = _native or _connect()
+    return native.prompt(q, key_pages, value_pages, page_table, lengths, row_start, window, sink, out, lse, _SCALE if scale is None else scale)
+
+
+def paged_shared_decode(q, key_pages, value_pages, page_table, lengths, group_start, shared, *, out=None, lse=None, scale=None):
+    """``paged_decode`` for requests that begin alike: requests ``group_start[g]`` to ``group_start[g + 1] - 1`` (int32 ``[groups + 1]``,
+    ascending) have their first ``shared[g]`` slots (int32 ``[groups]``) in common, which are read once for all of them, through the page
+    table of the first; each request's own slots are those behind.  Requests in no group have nothing in common with others."""
+    native = _native or _connect()
+    return native.shared_decode(q, key_pages, value_pages, page_table, lengths, group_start, shared, out, lse,
+                                _SCALE if scale is None else scale)
 
 
 def paged_observe(q, key_pages, page_table, lengths, weight, *, scale=None):
