@@ -7,8 +7,8 @@
 //
 // The rows of a tile of 128 are tokens (or requests) times the query heads of one KV head, so K and V serve a whole group of heads and a
 // tile spans few tokens: with four heads 32, which is what keeps the masked part of a window small.  An item is up to two neighbouring
-// tiles and a KV head; it walks the tiles of 128 slots that its rows may see, its first slots' and its window's, and no others:
-// of a tile that is brought in, boxes that no row sees are not read but filled with zeros.
+// tiles and a KV head; it walks the boxes (of a page, at most 128 slots) that its rows may see, its first slots' and then its window's,
+// 128 slots a step.  Boxes that no row sees are not read but filled with zeros.
 //   S_g = Q_g.K^T     M 128 x N 128 x K 128, both operands by TMA with the 128-byte swizzle, pages through the page table;
 //   softmax           a thread per query row (= TMEM lane), online, against a lazy reference maximum; P goes back over S as 16-bit pairs;
 //   O_g += P_g.V      A from TMEM, B the V tile as it lies (MN-major), the accumulator in TMEM for the whole walk.
@@ -17,11 +17,13 @@
 // Work: the steps of all items, head by head, are cut into one contiguous range per CTA, of equal length; every CTA works out where its own
 // begins.  An item that falls to several CTAs leaves partial results behind, which a second kernel joins in the order of the sequence.
 // TMEM: S_0 | S_1 | O_0 | O_1.  Warps: TMA producer, MMA issuer, the one that hands out segments (the part of an item that falls to the
-// CTA), one idle, eight softmax warps.  Every wait is bounded; one that runs out is recorded in the status word.
+// CTA), one that clears what lies behind a request's last slot, eight softmax warps.  Every wait is bounded; one that runs out is recorded in the status word.
 // A tile's slots that a row does not see have a probability of 0, and what they hold is finite where it was written as such; where it
 // was not, 0 * infinity leaves a NaN, and the row is done again over what it sees (`redo`).  Slots behind a request's last one may
 // hold anything: they are zeros in shared memory before the product.
 #include <cuda.h>
+
+#include <type_traits>
 
 #include "ri_paged.cuh"
 #include "ri_tc.cuh"
@@ -36,6 +38,7 @@ constexpr int kHalf = kTile * 128;         // bytes of a 128-row x 64-channel ha
 constexpr int kRing = 5;                   // tiles of K and V in shared memory: K0, V0, K1, V1, ...
 constexpr int kThreads = 384;
 constexpr int kSegments = 4;               // segments on their way from the warp that hands them out
+constexpr int kTails = 4;                 // V tiles in the ring that a request's slots end in: it holds three V tiles
 constexpr uint32_t kTmemCols = 512;
 constexpr int kMaxCtas = 160;
 constexpr int kMaxRequests = 16384;        // of a call, or groups and requests together
@@ -43,30 +46,30 @@ constexpr int kMaxEntries = 8192;          // of the table of steps
 // An item's end this many steps from the end of a CTA's range becomes the end of the range: a part of an item costs as much again
 // for its partial result and the second kernel.  Items of at most twice as many are never cut.
 constexpr int kSnap = 4;
+constexpr int kItemCost = 2;               // what an item costs beside its steps (7000 clocks; a step 3400)
 constexpr int kHeadsMost = 8;              // query heads of a KV head
 constexpr int kMeta = 8;                   // ints that a CTA leaves for the kernel that joins
 
-struct Walk {
+// An item's steps go over places: the boxes that hold its first slots, then those from its window's first one on.
+__device__ __forceinline__ int slot_of(int place, int front, int skip) { return place < front ? place : place + skip; }
+struct Segment {
   int step, n;                             // the first of the item's steps here, and how many; 0: no more segments
-  int front, skip;                         // step i is tile i, i < front, else tile i + skip
   int two;                                 // two tiles of rows
-  __device__ __forceinline__ int tile(int j) const { return step + j < front ? step + j : step + j + skip; }      // of the j-th step here
-  __device__ __forceinline__ int steps(int g) const { return two ? n : (n + 1 - g) >> 1; }      // of group g; its j-th one:
-  __device__ __forceinline__ int nth(int g, int j) const { return two ? j : 2 * j + g; }
-};
-struct Segment : Walk {
+  int front, skip;                         // places in front of the gap; slots left out
   int table_row, head;
   int q_row, n_tok;                        // the item's first token (or request), and how many
   int low, high, sink;                     // slots that some row of the item sees: [low, high) and [0, sink)
-  int rows;                                // slots of the request: there is nothing behind
+  int end;                                 // the place behind the request's last slot
   int slot0;                               // ri_paged_prompt: the first token's slot
   int part;                                // rows of partial results in front of this segment's, -1: the item is whole
   int pad;
+  __device__ __forceinline__ int steps(int g) const { return two ? n : (n + 1 - g) >> 1; }      // of group g, and its j-th one
+  __device__ __forceinline__ int nth(int g, int j) const { return step + (two ? j : 2 * j + g); }
 };
 
 // Shared memory.  It has no room to spare, so the barriers and the rest stand behind the ring, in what 227 KB leave.
 struct Control {
-  uint64_t bars[16 + 2 * kRing + 2 * kSegments];
+  uint64_t bars[14 + kTails + 2 * kRing + 2 * kSegments];
   Segment segments[kSegments];
   float2 stat[2][kTile];                   // items of one tile: a row's (maximum, sum) in either group
   int scan[kThreads / 32 + 1];
@@ -107,6 +110,7 @@ struct Seq {
 };
 struct Item {
   int n_tok, front, skip, low, high, sink, steps;
+  __device__ __forceinline__ int cost() const { return steps + kItemCost; }
 };
 __device__ __forceinline__ int clamped(int x, int most) { return min(max(x, 0), most); }
 // The group that request b is in, or -1.
@@ -159,10 +163,10 @@ __device__ __forceinline__ Item item_of(const Args& a, const Seq& s, int p) {
     if (a.window > 0) it.low = clamped(slot - a.window + 1, it.high);
     it.sink = min(a.sink, it.low);
   }
-  const int tile = it.low / kTile;
-  it.front = min((it.sink + kTile - 1) / kTile, tile);
-  it.skip = tile - it.front;
-  it.steps = max(1, (it.high + kTile - 1) / kTile - it.skip);      // rows that see nothing still have outputs
+  const int box = min(1 << a.shift, kTile);
+  it.front = (it.sink + box - 1) & -box;
+  it.skip = max(0, (it.low & -box) - it.front);
+  it.steps = max(1, (it.high - it.skip + kTile - 1) / kTile);      // rows that see nothing still have outputs
   return it;
 }
 
@@ -238,7 +242,7 @@ __device__ __forceinline__ void plan(const Args& a, int* table, Control& s) {
             while (at >= pairs[v + 1]);
             seq = seq_of<SHARED>(a, v);
           }
-          sum += item_of<SHARED>(a, seq, at - pairs[v]).steps;
+          sum += item_of<SHARED>(a, seq, at - pairs[v]).cost();
         }
       }
     }
@@ -260,9 +264,10 @@ __device__ __forceinline__ void plan(const Args& a, int* table, Control& s) {
       Seq seq = seq_of<SHARED>(a, v);
       for (;;) {
         p = at - pairs[v];
-        const int n = item_of<SHARED>(a, seq, p).steps;
-        step = y - before;
-        if (step < n) {
+        const Item it = item_of<SHARED>(a, seq, p);
+        const int n = it.steps;
+        if (y - before < it.cost()) {
+          step = max(0, y - before - kItemCost);
           if (!SHARED && step > 0) {
             if (step <= kSnap) {
               step = 0;
@@ -281,7 +286,7 @@ __device__ __forceinline__ void plan(const Args& a, int* table, Control& s) {
           }
           break;
         }
-        before += n;
+        before += it.cost();
         ++at;
         if (at >= pairs[v + 1]) {
           do ++v;
@@ -299,6 +304,49 @@ __device__ __forceinline__ void plan(const Args& a, int* table, Control& s) {
   __syncthreads();
 }
 
+// 32 bytes, a whole sector of L2, in one instruction where the tensor lies so that it can be.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&u)[8], bool wide) {
+  if (!wide) {
+    static_cast<uint4*>(p)[0] = make_uint4(u[0], u[1], u[2], u[3]);
+    static_cast<uint4*>(p)[1] = make_uint4(u[4], u[5], u[6], u[7]);
+    return;
+  }
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]),
+               "r"(u[5]), "r"(u[6]), "r"(u[7])
+               : "memory");
+}
+// Products and their completion by the one lane for which `one` is set, for whole warps.
+__device__ __forceinline__ void mma_by(uint32_t one, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts_by(uint32_t one, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void commit_by(uint32_t one, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(one)
+      : "memory");
+}
+// Whether a request's slots end inside a box of this tile: what the box brings in behind them may be anything.
+__device__ __forceinline__ bool ends_in_box(int end, int tile, int shift) {
+  const int r = end - tile * kTile;
+  return r > 0 && r < kTile && (r & (min(1 << shift, kTile) - 1)) != 0;
+}
+
 __device__ __forceinline__ float ex2(float x) {       // 2^x; results below 2^-126 become 0
   float d;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
@@ -307,19 +355,19 @@ __device__ __forceinline__ float ex2(float x) {       // 2^x; results below 2^-1
 // A tile is read four times over: 32 columns a mask, bit i of which says whether column i is seen.
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
 
-// What a thread's row sees, of slots [low, high) and [0, sink).
+// What a thread's row sees: places [low, high) and [0, sink).
 struct Sight {
   int low, high, sink;
-  __device__ __forceinline__ bool all_of(int slot0) const { return slot0 >= low && slot0 + kTile <= high; }
-  __device__ __forceinline__ uint32_t mask(int slot0) const {      // of 32 slots
-    return bits_below(high - slot0) & (~bits_below(low - slot0) | bits_below(sink - slot0));
+  __device__ __forceinline__ bool all_of(int place) const { return place >= low && place + kTile <= high; }
+  __device__ __forceinline__ uint32_t mask(int place) const {      // of 32 places
+    return bits_below(high - place) & (~bits_below(low - place) | bits_below(sink - place));
   }
 };
 
 // The rows of `bad` once more, one after the other, over the slots of this segment that they see and no others, in 32 bits against
 // the same reference: row i of the warp is lane i's.  `half`: 0 or 1, write these 64 channels; -1: all.
 template <int DT>
-__device__ __noinline__ void redo(const Args& a, const Segment& sg, unsigned bad, const Sight& sight, int row, int q_row, float m, float f, int half) {
+__device__ __noinline__ void redo(const Args& a, const Segment& sg, unsigned bad, Sight sight, int row, int q_row, float m, float f, int half) {
   const int lane = threadIdx.x & 31, n_rows = sg.n_tok * a.gs;
   while (bad) {
     const int src = __ffs(bad) - 1;
@@ -335,11 +383,9 @@ __device__ __noinline__ void redo(const Args& a, const Segment& sg, unsigned bad
     };
     float q[4], k[4], v[4], o[4] = {0.f, 0.f, 0.f, 0.f};
     four(a.q + (int64_t)tok * a.q_stride + h * RI_HEAD_DIM, q);
-    for (int i = sg.step; i < sg.step + sg.n; ++i) {
-      const int slot0 = (i < sg.front ? i : i + sg.skip) * kTile;
-      for (int slot = slot0; slot < min(slot0 + kTile, see.high); ++slot) {
-        if (slot < see.low && slot >= see.sink) continue;
-        const int id = page_of(a, sg.table_row, slot >> a.shift);
+    for (int at = sg.step * kTile; at < min((sg.step + sg.n) * kTile, see.high); ++at) {
+      if (at >= see.low || at < see.sink) {
+        const int slot = slot_of(at, sg.front, sg.skip), id = page_of(a, sg.table_row, slot >> a.shift);
         const int64_t in_page = ((int64_t)(sg.head << a.shift) + (slot & ((1 << a.shift) - 1))) * RI_HEAD_DIM;
         four(static_cast<const uint16_t*>(a.keys) + id * a.key_stride + in_page, k);
         four(static_cast<const uint16_t*>(a.values) + id * a.value_stride + in_page, v);
@@ -378,10 +424,11 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   auto bar_p_full = [&](int g) { return bars + 8u * (8 + g); };
   auto bar_o_full = [&](int g) { return bars + 8u * (10 + g); };
   auto bar_join = [&](int i) { return bars + 8u * (12 + i); };
-  auto bar_full = [&](int i) { return bars + 8u * (16 + i); };
-  auto bar_empty = [&](int i) { return bars + 8u * (16 + kRing + i); };
-  auto bar_seg = [&](int i) { return bars + 8u * (16 + 2 * kRing + i); };
-  auto bar_seg_empty = [&](int i) { return bars + 8u * (16 + 2 * kRing + kSegments + i); };
+  auto bar_tail = [&](int i) { return bars + 8u * (14 + i % kTails); };
+  auto bar_full = [&](int i) { return bars + 8u * (14 + kTails + i); };
+  auto bar_empty = [&](int i) { return bars + 8u * (14 + kTails + kRing + i); };
+  auto bar_seg = [&](int i) { return bars + 8u * (14 + kTails + 2 * kRing + i); };
+  auto bar_seg_empty = [&](int i) { return bars + 8u * (14 + kTails + 2 * kRing + kSegments + i); };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = (int)blockIdx.x;
 
   if (threadIdx.x == 0) {
@@ -393,7 +440,8 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       mbar_init(bar_p_part(g), 4); mbar_init(bar_p_full(g), 4); mbar_init(bar_o_full(g), 1); mbar_init(bar_join(g), 8);
     }
     for (int i = 0; i < kRing; ++i) { mbar_init(bar_full(i), 1); mbar_init(bar_empty(i), 1); }
-    for (int i = 0; i < kSegments; ++i) { mbar_init(bar_seg(i), 1); mbar_init(bar_seg_empty(i), 10); }
+    for (int i = 0; i < kSegments; ++i) { mbar_init(bar_seg(i), 1); mbar_init(bar_seg_empty(i), 11); }
+    for (int i = 0; i < kTails; ++i) mbar_init(bar_tail(i), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -425,14 +473,14 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     if (warp == 0) {
       // ---------------- TMA producer: Q_0, K0, Q_1, V0, K1, V1, ... of one segment after the other; a box per lane ----------------
-      const int box = min(1 << a.shift, kTile), mask = (1 << a.shift) - 1, slot_of_lane = lane * box;
+      const int box = min(1 << a.shift, kTile), mask = (1 << a.shift) - 1, place_of_lane = lane * box;
       const uint32_t q_bytes = (uint32_t)(a.tile_tokens * a.gs) * 256;
-      int issued = 0, q_issued[2] = {0, 0};
+      int issued = 0, q_issued[2] = {0, 0}, tails = 0;
       bool ok = true;
       for (int i = 0; ok && take(i); ++i) {
         const Segment& sg = s.segments[i % kSegments];
-        const Walk w = sg;
-        const int head = sg.head, low = sg.low, high = sg.high, sink = sg.sink;
+        const int first = sg.step, n = sg.n, two = sg.two, front = sg.front, skip = sg.skip;
+        const int head = sg.head, low = sg.low, high = sg.high, sink = sg.sink, end = sg.end;
         const int32_t* table = a.table + (int64_t)sg.table_row * a.table_stride;
         auto load_q = [&](int g) {
           if (!__all_sync(0xffffffffu, mbar_wait(bar_q_empty(g), (q_issued[g] & 1) ^ 1, abort_flag, 12))) return false;
@@ -446,26 +494,28 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           return true;
         };
         // this lane's box of the j-th step; one that no row sees is looked up nowhere, and comes from behind the pool, as zeros
-        auto slot_at = [&](int j) { return w.tile(j) * kTile + slot_of_lane; };
-        auto seen = [&](int slot) { return slot_of_lane < kTile && slot < high && (slot + box > low || slot < sink); };
+        auto slot_at = [&](int j) { return slot_of((first + j) * kTile + place_of_lane, front, skip); };
+        auto seen = [&](int slot) { return place_of_lane < kTile && slot < high && (slot + box > low || slot < sink); };
         auto page_at = [&](int j) { return seen(slot_at(j)) ? table[slot_at(j) >> a.shift] : -1; };
         int next = page_at(0);
         ok = load_q(0);
-        for (int j = 0; ok && j < w.n; ++j) {
+        for (int j = 0; ok && j < n; ++j) {
           const int id = seen(slot_at(j)) ? page_or_first(a, next) : a.n_pages;
           const int y = (head << a.shift) + (slot_at(j) & mask);
-          if (j + 1 < w.n) next = page_at(j + 1);
+          if (j + 1 < n) next = page_at(j + 1);
           for (int t = 0; ok && t < 2; ++t) {
             const int at = issued % kRing;
             ok = __all_sync(0xffffffffu, mbar_wait(bar_empty(at), ((issued / kRing) & 1) ^ 1, abort_flag, 13));
             if (!ok) break;
-            if (lane == 0) mbar_arrive_expect_tx(bar_full(at), 2 * kHalf);
+            // a V tile that the request's slots end in is full when what lies behind them has been cleared
+            const uint32_t bar = t == 1 && ends_in_box(end, first + j, a.shift) ? bar_tail(tails++) : bar_full(at);
+            if (lane == 0) mbar_arrive_expect_tx(bar, 2 * kHalf);
             __syncwarp();
-            if (slot_of_lane < kTile)
+            if (place_of_lane < kTile)
               for (int kb = 0; kb < 2; ++kb)
-                tma_load_4d(sKV + (at * 2 + kb) * kHalf + slot_of_lane * 128, t ? &map_v : &map_k, bar_full(at), 0, y, kb, id);
+                tma_load_4d(sKV + (at * 2 + kb) * kHalf + place_of_lane * 128, t ? &map_v : &map_k, bar, 0, y, kb, id);
             ++issued;
-            if (j == 0 && t == 0 && w.two) ok = load_q(1);
+            if (j == 0 && t == 0 && two) ok = load_q(1);
           }
         }
         release(i);
@@ -473,104 +523,166 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       if (*abort_flag) {     // give the copies still in flight a bounded chance to land before the CTA exits
         for (int g = 0; g < 2; ++g)
           if (q_issued[g] > 0) mbar_wait(bar_q(g), (q_issued[g] - 1) & 1, abort_flag, 14);
+        for (int t = max(0, tails - kTails); t < tails; ++t) mbar_wait(bar_tail(t), (t / kTails) & 1, abort_flag, 14);
         for (int t = max(0, issued - kRing); t < issued; ++t) mbar_wait(bar_full(t % kRing), (t / kRing) & 1, abort_flag, 14);
       }
     } else if (warp == 1) {
-      // ---------------- MMA issuer (lane 0; the warp clears what lies behind a request's last slot) ----------------
+      // ---------------- MMA issuer ----------------
       // Per step: P_0.V, then S_0 of the group's next tile, then the same for group 1; behind the last step of a segment come the
       // first scores of the next one.  S_g of the next tile overwrites the columns P_g was read from: both are products of this
       // thread, which the tensor pipe takes in order.
-      int tile0 = 0;                       // ring index of the segment's first K tile
-      int q_used[2] = {0, 0}, p_used[2] = {0, 0};
-      auto wait = [&](uint32_t bar, int parity, int where) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, where)); };
-      auto wait_tile = [&](int t) { return wait(bar_full(t % kRing), (t / kRing) & 1, 15); };
-      // ring index of the K tile of group g's step j; its V tile is the next one
-      auto ring_k = [&](const Walk& w, int g, int j) { return tile0 + 2 * w.nth(g, j); };
-      auto issue_qk = [&](const Walk& w, int g, int t, bool last) {
-        if (lane == 0) {
-          const uint32_t sk = sKV + (t % kRing) * 2 * kHalf;
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb) {
-            const uint64_t da = umma_desc_sw128(sQ + ((w.two ? g : 0) * 2 + kb) * kHalf), db = umma_desc_sw128(sk + kb * kHalf);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) tc_mma_f16(tmem + g * kTile, da + 2 * k, db + 2 * k, a.idesc_qk, (kb | k) != 0);
+      // The whole warp goes along without a branch that its lanes could take differently, and one lane's predicate stands before each
+      // product: their operands' places are then in uniform registers, where the instruction takes them from.  The groups are loops,
+      // not copies of the code: all roles together have to fit the instruction cache (8192 tokens, window 128: 67 -> 63 us).
+      const uint32_t one = lane == 0;
+      const uint32_t tmem_u = __reduce_max_sync(0xffffffffu, tmem);
+      auto wait = [&](uint32_t bar, uint32_t parity, int where) {
+        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+        const unsigned long long t0 = global_ns();
+        for (uint32_t spin = 0;; ++spin) {
+          if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+          if ((spin & 255u) == 255u) {
+            if (__any_sync(0xffffffffu, *abort_flag != 0)) return false;
+            if (__any_sync(0xffffffffu, global_ns() - t0 > kWaitLimitNs)) { *abort_flag = where; return false; }
           }
-          tc_commit(bar_s_full(g));          // also says that P_g.V of the tile before has completed
-          if (last) tc_commit(bar_q_empty(w.two ? g : 0));
-          if (!w.two) tc_commit(bar_empty(t % kRing));
+          if (spin > (1u << 28)) { *abort_flag = where + 100; return false; }      // second bound, independent of the timer
         }
-        __syncwarp();
       };
-      auto issue_pv = [&](int g, int t, int k0, bool first) {
-        if (lane == 0) {
-          const uint64_t db = umma_desc_mn_sw128(sKV + (t % kRing) * 2 * kHalf, kHalf);
+      int at = 0, phase = 0;               // the segment's next tile in the ring; the ring's turn
+      uint32_t q_used = 0, p_used = 0;     // parities, a bit for each group
+      // place and parity of the tile that lies `ahead` of the next one
+      auto slot = [&](int ahead) { const int x = at + ahead; return x >= kRing ? x - kRing : x; };
+      auto turn = [&](int ahead) { return (uint32_t)(at + ahead >= kRing ? phase ^ 1 : phase); };
+      auto wait_tile = [&](int ahead) { return wait(bar_full(slot(ahead)), turn(ahead), 15); };
+      auto issue_pv = [&](int g, int tile, int k0, bool first) {
+        const uint64_t db = umma_desc_mn_sw128(sKV + tile * 2 * kHalf, kHalf);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tc_mma_f16_ts(tmem + (2 + g) * kTile, tmem + g * kTile + 8 * (k0 + k), db + 128 * (k0 + k), a.idesc_pv, !first || (k0 + k) != 0);
+        for (int k = 0; k < 4; ++k)
+          mma_ts_by(one, tmem_u + (2 + g) * kTile, tmem_u + g * kTile + 8 * (k0 + k), db + 128 * (k0 + k), a.idesc_pv, !first || (k0 + k) != 0);
+      };
+      auto issue_qk = [&](int g, int q, int tile) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          const uint64_t da = umma_desc_sw128(sQ + (q * 2 + kb) * kHalf), db = umma_desc_sw128(sKV + (tile * 2 + kb) * kHalf);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mma_by(one, tmem_u + g * kTile, da + 2 * k, db + 2 * k, a.idesc_qk, (kb | k) != 0);
         }
-        __syncwarp();
+        commit_by(one, bar_s_full(g));       // also says that P_g.V of the tile before has completed
       };
-      // what lies behind the request's last slot, up to the end of its page
-      auto clear = [&](int rows, int tile, int t) {
-        const int r0 = rows - tile * kTile;
-        if (r0 >= kTile) return;
-        const int box = min(1 << a.shift, kTile), r1 = (max(r0, 0) + box - 1) / box * box;
-        uint8_t* v = smem + 4 * kHalf + (t % kRing) * 2 * kHalf;
-        for (int i = max(r0, 0) * 8 + lane; i < r1 * 8; i += 32)
-          for (int kb = 0; kb < 2; ++kb) *reinterpret_cast<uint4*>(v + kb * kHalf + i * 16) = make_uint4(0, 0, 0, 0);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
+      auto advance = [&] {                   // by a step: K and V
+        at += 2;
+        if (at >= kRing) { at -= kRing; phase ^= 1; }
       };
-      // whether group g's step j is the last user of its Q tile (one tile: the walk's last step, in either group)
-      auto last_of_q = [&](const Walk& w, int g, int j) { return w.nth(g, j) + 1 == w.n; };
-      bool ok = true;
-      for (int i = 0; ok && take(i); ++i) {
-        const Walk w = s.segments[i % kSegments];
-        const int rows = s.segments[i % kSegments].rows;
-        release(i);
-        // first scores of both groups
-        for (int g = 0; ok && g < 2; ++g) {
-          if (w.steps(g) == 0) continue;
-          ok = wait_tile(ring_k(w, g, 0));
-          if (ok && (w.two || g == 0)) ok = wait(bar_q(g), q_used[g]++ & 1, 16);
-          if (!ok) break;
+      // P_g.V of a step whose V tile is there: its first half as soon as there are probabilities for it
+      auto product = [&](int g, int tile, bool first) {
+        if (!wait(bar_p_part(g), (p_used >> g) & 1, 17)) return false;
+        tc_fence_after();
+        issue_pv(g, tile, 0, first);
+        if (!wait(bar_p_full(g), (p_used >> g) & 1, 18)) return false;
+        tc_fence_after();
+        issue_pv(g, tile, 4, false);
+        p_used ^= 1u << g;
+        return true;
+      };
+      auto query = [&](int g) {
+        const bool there = wait(bar_q(g), (q_used >> g) & 1, 16);
+        q_used ^= 1u << g;
+        return there;
+      };
+      // two tiles: both groups use every tile of K and V
+      auto two_tiles = [&](int n) {
+        if (!wait_tile(0)) return false;
+#pragma unroll 1
+        for (int g = 0; g < 2; ++g) {
+          if (!query(g)) return false;
           tc_fence_after();
-          issue_qk(w, g, ring_k(w, g, 0), last_of_q(w, g, 0));
+          issue_qk(g, g, slot(0));
+          if (n == 1) commit_by(one, bar_q_empty(g));
         }
-        if (ok && w.two && lane == 0) tc_commit(bar_empty(tile0 % kRing));
-        for (int j = 0; ok && j < w.steps(0); ++j) {
-#pragma unroll
+        commit_by(one, bar_empty(slot(0)));
+        for (int j = 0; j < n; ++j) {
+#pragma unroll 1
           for (int g = 0; g < 2; ++g) {
-            if (!ok || j >= w.steps(g)) continue;
-            const int tv = ring_k(w, g, j) + 1;
-            ok = wait_tile(tv);
-            if (!ok) break;
-            if (!w.two || g == 0) clear(rows, w.tile(w.nth(g, j)), tv);
-            ok = wait(bar_p_part(g), p_used[g] & 1, 17);
-            if (!ok) break;
-            tc_fence_after();
-            issue_pv(g, tv, 0, j == 0);
-            ok = wait(bar_p_full(g), p_used[g] & 1, 18);
-            if (!ok) break;
-            tc_fence_after();
-            issue_pv(g, tv, 4, false);
-            ++p_used[g];
-            if (!w.two && lane == 0) tc_commit(bar_empty(tv % kRing));
-            if (j + 1 < w.steps(g)) {
-              ok = wait_tile(ring_k(w, g, j + 1));
-              if (!ok) break;
+            if ((g == 0 && !wait_tile(1)) || !product(g, slot(1), j == 0)) return false;
+            if (j + 1 < n) {
+              if (g == 0 && !wait_tile(2)) return false;
               tc_fence_after();
-              issue_qk(w, g, ring_k(w, g, j + 1), last_of_q(w, g, j + 1));
-            } else if (lane == 0) {
-              tc_commit(bar_o_full(g));
+              issue_qk(g, g, slot(2));
+              if (j + 2 == n) commit_by(one, bar_q_empty(g));
+            } else {
+              commit_by(one, bar_o_full(g));
             }
           }
-          if (ok && w.two && lane == 0) {
-            tc_commit(bar_empty((tile0 + 2 * j + 1) % kRing));
-            if (j + 1 < w.n) tc_commit(bar_empty((tile0 + 2 * j + 2) % kRing));
+          commit_by(one, bar_empty(slot(1)));
+          if (j + 1 < n) commit_by(one, bar_empty(slot(2)));
+          advance();
+        }
+        return true;
+      };
+      // one tile: group 0 takes the even steps and group 1 the odd ones, so that step i is computed behind the scores of step i + 1
+      auto one_tile = [&](int n) {
+        if (!wait_tile(0) || !query(0)) return false;
+        tc_fence_after();
+        issue_qk(0, 0, slot(0));
+        if (n == 1) commit_by(one, bar_q_empty(0));
+        commit_by(one, bar_empty(slot(0)));
+        if (n > 1) {
+          if (!wait_tile(2)) return false;
+          tc_fence_after();
+          issue_qk(1, 0, slot(2));
+          if (n == 2) commit_by(one, bar_q_empty(0));
+          commit_by(one, bar_empty(slot(2)));
+        }
+        for (int i = 0; i < n; i += 2) {
+#pragma unroll 1
+          for (int g = 0; g < 2; ++g) {
+            if (i + g >= n) continue;
+            if (!wait_tile(1) || !product(g, slot(1), i == 0)) return false;
+            commit_by(one, bar_empty(slot(1)));
+            advance();
+            if (i + g + 2 < n) {             // the group's next step, one behind the other group's
+              if (!wait_tile(2)) return false;
+              tc_fence_after();
+              issue_qk(g, 0, slot(2));
+              if (i + g + 3 == n) commit_by(one, bar_q_empty(0));
+              commit_by(one, bar_empty(slot(2)));
+            } else {
+              commit_by(one, bar_o_full(g));
+            }
           }
         }
-        tile0 += 2 * w.n;
+        return true;
+      };
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        if (!wait(bar_seg(i % kSegments), (i / kSegments) & 1, 10)) break;
+        const int n = (int)__reduce_max_sync(0xffffffffu, (unsigned)s.segments[i % kSegments].n);
+        const bool two = __any_sync(0xffffffffu, s.segments[i % kSegments].two);
+        if (n == 0) break;
+        release(i);
+        ok = two ? two_tiles(n) : one_tile(n);
+      }
+    } else if (warp == 3) {
+      // ---------------- V tiles that a request's slots end in: zeros behind them, up to the end of their box ----------------
+      int tile0 = 0, tails = 0;
+      bool ok = true;
+      for (int i = 0; ok && take(i); ++i) {
+        const int first = s.segments[i % kSegments].step, n = s.segments[i % kSegments].n, end = s.segments[i % kSegments].end;
+        release(i);
+        for (int j = 0; j < n; ++j) {
+          if (!ends_in_box(end, first + j, a.shift)) continue;
+          const int at = (tile0 + 2 * j + 1) % kRing, box = min(1 << a.shift, kTile), r0 = end - (first + j) * kTile, r1 = (r0 + box - 1) & -box;
+          ok = __all_sync(0xffffffffu, mbar_wait(bar_tail(tails), (tails / kTails) & 1, abort_flag, 15));
+          if (!ok) break;
+          uint8_t* v = smem + 4 * kHalf + at * 2 * kHalf;
+          for (int x = r0 * 8 + lane; x < r1 * 8; x += 32)
+            for (int kb = 0; kb < 2; ++kb) *reinterpret_cast<uint4*>(v + kb * kHalf + x * 16) = make_uint4(0, 0, 0, 0);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_full(at));
+          ++tails;
+        }
+        tile0 += 2 * n;
       }
     } else if (warp == 2) {
       // ---------------- segments ----------------
@@ -611,7 +723,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           sg.low = it.low;
           sg.high = it.high;
           sg.sink = it.sink;
-          sg.rows = seq.rows;
+          sg.end = seq.rows - it.skip;
           sg.slot0 = seq.rows - seq.n + p * 2 * a.tile_tokens;
           sg.two = it.n_tok > a.tile_tokens;
           const bool begins = step == 0, ends = end == it.steps;
@@ -663,34 +775,57 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     // probabilities down to 2^-(24 + kAbove) of the largest, which are at most 2^(kAbove + kLazy).
     constexpr float kLazy = 4.f, kAbove = DT == RI_F16 ? 10.f : 0.f;
     bool ok = true;
-    int done = 0, outs[2] = {0, 0}, joins = 0;             // tiles of this group, outputs of both groups, joins so far
+    // parities of what is waited for next: bit 0 scores, 1 and 2 outputs of the two groups, 3 joins.  A row of scores takes 128
+    // registers, so little else is kept over the steps: what the segment says is read from shared memory where it is needed.
+    uint32_t phases = 0;
     auto meet = [&](int i) {                               // of all eight warps
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_join(i));
-      return (bool)__all_sync(0xffffffffu, mbar_wait(bar_join(i), joins & 1, abort_flag, 10));
+      return (bool)__all_sync(0xffffffffu, mbar_wait(bar_join(i), (phases >> 3) & 1, abort_flag, 10));
     };
     for (int i = 0; ok && take(i); ++i) {
       const Segment& sg = s.segments[i % kSegments];         // stays until the end of the segment
-      const Walk w = sg;
-      const int n = w.steps(grp), tile_row0 = w.two ? grp * a.tile_tokens * a.gs : 0;
       // the row in its item, its token; rows that fill up a tile are like the last one, so that they hold nobody up
-      const int n_rows = sg.n_tok * a.gs, item_row = tile_row0 + row;
-      const bool valid = row < a.tile_tokens * a.gs && item_row < n_rows;
-      const int q_row = sg.q_row + min(item_row, n_rows - 1) / a.gs;
-      Sight sight = {sg.low, sg.high, 0};
-      if (!SHARED) {
-        const int slot = sg.slot0 + q_row - sg.q_row;
-        sight.high = clamped(slot + 1, sg.rows);
-        sight.low = a.window > 0 ? max(0, slot - a.window + 1) : 0;
-        sight.sink = a.sink;
-      } else {
-        sight.high = min(sg.high, rows_of(a, q_row));
-      }
+      auto row_in_item = [&] { return (sg.two ? grp * a.tile_tokens * a.gs : 0) + row; };
+      auto token = [&] { return sg.q_row + min(row_in_item(), sg.n_tok * a.gs - 1) / a.gs; };
+      auto sight_of_row = [&] {
+        const int q_row = token();
+        Sight x = {sg.low - sg.skip, 0, 0};
+        if (!SHARED) {
+          const int slot = sg.slot0 + q_row - sg.q_row;
+          x.high = min(max(slot + 1, 0), sg.end + sg.skip) - sg.skip;
+          x.low = a.window > 0 ? max(0, slot - a.window + 1) - sg.skip : 0;
+          x.sink = a.sink;
+        } else {
+          x.high = min(sg.high, rows_of(a, q_row)) - sg.skip;
+        }
+        return x;
+      };
+      const Sight sight = sight_of_row();
       float m_ref = -INFINITY, l_run = 0.f;
-      for (int j = 0; ok && j < n; ++j, ++done) {
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_s_full(grp), done & 1, abort_flag, 11));
+      for (int j = 0; ok && j < sg.steps(grp); ++j, phases ^= 1) {
+        const int place = sg.nth(grp, j) * kTile;
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_s_full(grp), phases & 1, abort_flag, 11));
         if (!ok) break;
         tc_fence_after();
+        // Columns that are not seen become -infinity where they lie, 32 at a time: a tile's few tokens begin and end seeing close together,
+        // so most of four times 32 columns are seen by all rows of a warp, and a loop is a quarter of the instructions.
+        if (__any_sync(0xffffffffu, !sight.all_of(place))) {
+#pragma unroll 1
+          for (int x = 0; x < 4; ++x) {
+            const uint32_t seen = sight.mask(place + x * 32);
+            if (!__any_sync(0xffffffffu, seen != 0xffffffffu)) continue;
+            uint32_t part[32];
+            tc_ld32(tmem_s + x * 32, part);
+            tc_wait_ld();
+            tc_ld_landed(part);
+#pragma unroll
+            for (int y = 0; y < 32; ++y)
+              if (!(seen & (1u << y))) part[y] = 0xff800000u;      // -inf
+            tc_st32(tmem_s + x * 32, part);
+          }
+          tc_wait_st();
+        }
         uint32_t sr[4][32];
 #pragma unroll
         for (int x = 0; x < 4; ++x) tc_ld32(tmem_s + x * 32, sr[x]);
@@ -698,16 +833,6 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
         for (int x = 0; x < 4; ++x) tc_ld_landed(sr[x]);
 
-        const int slot0 = w.tile(w.nth(grp, j)) * kTile;
-        if (!sight.all_of(slot0)) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const uint32_t seen = sight.mask(slot0 + x * 32);
-#pragma unroll
-            for (int y = 0; y < 32; ++y)
-              if (!(seen & (1u << y))) sr[x][y] = 0xff800000u;     // -inf
-          }
-        }
         float mx[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
@@ -772,7 +897,8 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       //      memory, then each joins half of the channels of both accumulators; the second barrier keeps an accumulator until the
       //      other group has read it ----
       float m = m_ref, l = l_run, w0 = 1.f, w1 = 0.f;        // of the row; weights of the accumulators read below
-      if (!w.two) {
+      const bool two = sg.two;
+      if (!two) {
         s.stat[grp][row] = make_float2(m_ref, l_run);
         ok = ok && meet(0);
         const float2 other = s.stat[grp ^ 1][row];
@@ -787,57 +913,67 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       w1 *= f;
 #pragma unroll
       for (int g = 0; g < 2; ++g)
-        if (w.steps(g) > 0) {              // the other group's outputs count even where nobody here waits for them
-          if (!w.two || g == grp) ok = ok && __all_sync(0xffffffffu, mbar_wait(bar_o_full(g), outs[g] & 1, abort_flag, 11));
-          ++outs[g];
+        if (sg.steps(g) > 0) {             // the other group's outputs count even where nobody here waits for them
+          if (!two || g == grp) ok = ok && __all_sync(0xffffffffu, mbar_wait(bar_o_full(g), (phases >> (1 + g)) & 1, abort_flag, 11));
+          phases ^= 2u << g;
         }
       if (ok) {
         tc_fence_after();
-        const bool both = !w.two && w.steps(1) > 0;
-        const int x0 = w.two ? 0 : grp * 2, x1 = w.two ? 4 : x0 + 2;
+        const bool both = !two && sg.steps(1) > 0;
+        const int n_rows = sg.n_tok * a.gs, item_row = row_in_item(), q_row = token();
+        const bool valid = row < a.tile_tokens * a.gs && item_row < n_rows;
+        const int x0 = two ? 0 : grp * 2, x1 = two ? 4 : x0 + 2;
         const int h = sg.head * a.gs + item_row % a.gs;
+        const bool wide = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
         bool bad = false;
 #pragma unroll 1
-        for (int x = x0; x < x1; ++x) {
-          uint32_t o0[32], o1[32];
-          tc_ld32(tmem + (2 + (w.two ? grp : 0)) * kTile + t_lane + x * 32, o0);
-          if (both) tc_ld32(tmem + 3 * kTile + t_lane + x * 32, o1);
+        for (int x = x0; x < x1; ++x) {                        // 32 channels at a time: it runs once an item, so its code is kept short
+          uint32_t part[32];
+          float o[32];
+          tc_ld32(tmem + (2 + (two ? grp : 0)) * kTile + t_lane + x * 32, part);
           tc_wait_ld();
-          tc_ld_landed(o0);
-          if (both) tc_ld_landed(o1);
+          tc_ld_landed(part);
+#pragma unroll
+          for (int y = 0; y < 32; ++y) o[y] = __uint_as_float(part[y]) * w0;
+          if (both) {
+            tc_ld32(tmem + 3 * kTile + t_lane + x * 32, part);
+            tc_wait_ld();
+            tc_ld_landed(part);
+#pragma unroll
+            for (int y = 0; y < 32; ++y) o[y] += __uint_as_float(part[y]) * w1;
+          }
           if (valid) {
-            float o[32];
 #pragma unroll
-            for (int y = 0; y < 32; ++y) {
-              o[y] = __uint_as_float(o0[y]) * w0 + (both ? __uint_as_float(o1[y]) * w1 : 0.f);
-              bad |= o[y] != o[y];
-            }
+            for (int y = 0; y < 32; ++y) bad |= o[y] != o[y];
             if (sg.part < 0) {
-              uint4* dst = reinterpret_cast<uint4*>(a.out + ((int64_t)q_row * a.hk * a.gs + h) * RI_HEAD_DIM);
+              uint16_t* dst = a.out + ((int64_t)q_row * a.hk * a.gs + h) * RI_HEAD_DIM + x * 32;
 #pragma unroll
-              for (int y = 0; y < 32; y += 8)
-                dst[x * 4 + y / 8] = make_uint4(Elem<DT>::pack2(o[y], o[y + 1]), Elem<DT>::pack2(o[y + 2], o[y + 3]),
-                                                Elem<DT>::pack2(o[y + 4], o[y + 5]), Elem<DT>::pack2(o[y + 6], o[y + 7]));
+              for (int y = 0; y < 32; y += 16) {
+                uint32_t u[8];
+#pragma unroll
+                for (int v = 0; v < 8; ++v) u[v] = Elem<DT>::pack2(o[y + 2 * v], o[y + 2 * v + 1]);
+                store32(dst + y, u, wide);
+              }
             } else {
-              float4* dst = reinterpret_cast<float4*>(a.part_o + (int64_t)sg.part * RI_HEAD_DIM);
+              float4* dst = reinterpret_cast<float4*>(a.part_o + (int64_t)sg.part * RI_HEAD_DIM) + x * 8 * n_rows + item_row;
 #pragma unroll
-              for (int y = 0; y < 32; y += 4) dst[(x * 8 + y / 4) * n_rows + item_row] = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+              for (int y = 0; y < 32; y += 4) dst[y / 4 * n_rows] = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
             }
           }
         }
-        if (valid && (w.two || grp == 0)) {
+        if (valid && (two || grp == 0)) {
           if (sg.part >= 0) a.part_ml[sg.part + item_row] = make_float2(m, l);
           else if (a.lse != nullptr) a.lse[(int64_t)q_row * a.hk * a.gs + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
         }
-        const unsigned again = __ballot_sync(0xffffffffu, bad && l == l);
+        const unsigned again = __ballot_sync(0xffffffffu, valid && bad && l == l);
         if (again) {
           __syncwarp();
-          redo<DT>(a, sg, again, sight, item_row, q_row, m == -INFINITY ? 0.f : m, f, w.two ? -1 : grp);
+          redo<DT>(a, sg, again, sight_of_row(), item_row, q_row, m == -INFINITY ? 0.f : m, f, two ? -1 : grp);
         }
       }
-      if (!w.two) {
+      if (!two) {
         ok = ok && meet(1);
-        ++joins;
+        phases ^= 8;
       }
       release(i);
     }
@@ -997,8 +1133,8 @@ int64_t most_items_rows(const ri_paged& p, int rows) {      // rows of an item, 
 bool may_cut(const ri_paged& p, int rows, int window, int sink) {
   const int64_t all = (slots_of(p) + kTile - 1) / kTile;
   if (window == 0) return all > 2 * kSnap;
-  const int64_t pair = 2 * (kTile / p.group_size);
-  const int64_t seen = ((int64_t)window + (rows < pair ? rows : pair) + kTile - 3) / kTile + 1 + ((int64_t)sink + kTile - 1) / kTile;
+  const int64_t pair = 2 * (kTile / p.group_size), box = p.page_size < kTile ? p.page_size : kTile;
+  const int64_t seen = ((int64_t)window + sink + (rows < pair ? rows : pair) + 2 * box + kTile - 1) / kTile;      // first slots and window in boxes begun
   return (seen < all ? seen : all) > 2 * kSnap;
 }
 
