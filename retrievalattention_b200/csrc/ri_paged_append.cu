@@ -3,7 +3,10 @@
 //     x'_i = x_i c - x_{i+64} s,    x'_{i+64} = x_{i+64} c + x_i s          (query and key heads; values as they are)
 // One axis is the ordinary rotary embedding; text, images and video take (time, height, width).
 // With norms a query or key head is first  x_i <- x_i w_i / sqrt(mean x^2 + eps),  in 32 bits up to the one rounding behind the rotation;
-// the half-warp that has a head has its sum of squares in four shuffles.
+// the half-warp that has a head has its sum of squares in four shuffles.  The root is taken behind the rotation, and weights that are
+// the same for all heads go into the row's cosines and sines, which a service warp multiplies: the rotation is what it was, and the
+// rotating warps, which would be what counts otherwise, have a third more to do, not twice as much.  32768 rows of 32 + 8 heads: 156 us
+// (149 without norms; with the weights loaded and multiplied head by head 210, as pairs 198).  Weights for each head are read so: 198 us.
 // (reference: model_hub/llama.py:232-235 the split, :312-320 the rotation; cache_hub/flash_attn_cache.py:133-151 the append)
 //
 // Bound by the projection, read once and written once.  A row of it lies in one piece and comes in by one bulk copy, three rows
@@ -77,50 +80,53 @@ __device__ __forceinline__ uint4 rotate(const uint4& mine, const uint4& other, c
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// The same behind an RMS norm: `inv` is one over the head's root mean square, w and v the weights of the two pieces.
+// Eight channels as pairs in 32 bits.
 template <int DT>
-__device__ __forceinline__ uint4 rotate_normed(const uint4& mine, const uint4& other, const uint4& w_mine, const uint4& w_other, float inv,
-                                               const float* cs, float sign) {
-  const uint32_t a[4] = {mine.x, mine.y, mine.z, mine.w}, b[4] = {other.x, other.y, other.z, other.w};
-  const uint32_t w[4] = {w_mine.x, w_mine.y, w_mine.z, w_mine.w}, v[4] = {w_other.x, w_other.y, w_other.z, w_other.w};
+__device__ __forceinline__ void unpack_pairs(const uint4& x, uint64_t (&p)[4]) {
+  const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p[i] = pack_f2(Elem<DT>::from_bits((uint16_t)(u[i] & 0xffffu)), Elem<DT>::from_bits((uint16_t)(u[i] >> 16)));
+}
+// The rotation behind an RMS norm: (x A + y B) / rms, pairs at a time.  Sixteen lanes, those of `half_warp`, have a head's pieces.
+template <int DT>
+__device__ __forceinline__ uint4 rotate_normed(const uint64_t (&x)[4], const uint64_t (&y)[4], const uint64_t (&a)[4], const uint64_t (&b)[4],
+                                               float inv) {
+  const uint64_t by = pack_f2(inv, inv);
   uint32_t o[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float r[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      auto part = [&](const uint32_t (&p)[4]) { return Elem<DT>::from_bits((uint16_t)(p[i] >> (16 * e))); };
-      const float x = part(a) * inv * part(w), y = part(b) * inv * part(v);
-      r[e] = x * cs[2 * i + e] + sign * y * cs[8 + 2 * i + e];
-    }
-    o[i] = Elem<DT>::pack2(r[0], r[1]);
+    float lo, hi;
+    unpack_f2(mul_f2(fma_f2(x[i], a[i], mul_f2(y[i], b[i])), by), lo, hi);
+    o[i] = Elem<DT>::pack2(lo, hi);
   }
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
-// Sum of the squares of a head, whose sixteen pieces lie in the lanes of a half-warp.
-template <int DT>
-__device__ __forceinline__ float head_squares(const uint4& mine, unsigned half_warp) {
-  const uint32_t a[4] = {mine.x, mine.y, mine.z, mine.w};
-  float sum = 0.f;
+__device__ __forceinline__ float head_squares(const uint64_t (&x)[4], unsigned half_warp) {
+  uint64_t two = mul_f2(x[0], x[0]);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float x = Elem<DT>::from_bits((uint16_t)(a[i] & 0xffffu)), y = Elem<DT>::from_bits((uint16_t)(a[i] >> 16));
-    sum += x * x + y * y;
-  }
+  for (int i = 1; i < 4; ++i) two = fma_f2(x[i], x[i], two);
+  float sum, odd;
+  unpack_f2(two, sum, odd);
+  sum += odd;
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(half_warp, sum, o);
   return sum;
 }
 
 // What a row needs beside its pieces, fetched by a service warp.
+enum Norm { kNone, kOneWeight, kHeadWeights };      // norms: none, with a weight for all heads, with one for each
+template <int NORM>
 struct alignas(16) RowPlan {
-  float cs[128];             // cosines, sines; read 16 bytes at a time
+  // cosines, sines; kOneWeight: for query and key heads what every channel is multiplied by, and the one it is rotated with, weights
+  // included.  Read 16 bytes at a time
+  float cs[NORM == kOneWeight ? 512 : 128];
   int id, row, token;        // page (-1: none), row in it, token number
 };
 
 // The plans of rows row0 .. row0 + n - 1 (n <= ROWS), whose loads are on their way together: lane r looks for row r's place.
-template <int ROWS>
-__device__ __forceinline__ void plan_rows(const AppendArgs& a, int row0, int n, int lane, RowPlan* plans) {
+// w: kOneWeight, the weights of query and key heads for channels lane + 32 i and, behind them, 64 on.
+template <int ROWS, int NORM>
+__device__ __forceinline__ void plan_rows(const AppendArgs& a, int row0, int n, int lane, const float (&w)[2][4], RowPlan<NORM>* plans) {
   const Pages& p = a.pages;
   int64_t pos[ROWS][2];
 #pragma unroll
@@ -172,15 +178,25 @@ __device__ __forceinline__ void plan_rows(const AppendArgs& a, int row0, int n, 
   for (int r = 0; r < ROWS; ++r)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (r < n) plans[r].cs[lane + 32 * i] = cs[r][i];
+      if (r < n) {
+        if (NORM != kOneWeight) {
+          plans[r].cs[lane + 32 * i] = cs[r][i];
+        } else {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {                  // channel lane + 32 i; it is rotated with the one 64 from it
+            plans[r].cs[256 * k + lane + 32 * i] = w[k][i] * cs[r][i & 1];
+            plans[r].cs[256 * k + 128 + lane + 32 * i] = (i < 2 ? -1.f : 1.f) * w[k][i ^ 2] * cs[r][2 + (i & 1)];
+          }
+        }
+      }
 }
 
 // Work goes by units: an equal part of a row's heads where there are more than kUnitHeads, else a row or a few.
-// ROWS: rows of a unit, at most.  NORM: query and key heads are normalised before they are rotated.
-template <int DT, int ROWS, bool NORM>
+// ROWS: rows of a unit, at most.  NORM: whether and with what weights query and key heads are normalised before they are rotated.
+template <int DT, int ROWS, int NORM>
 __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) rope_append_kernel(const __grid_constant__ AppendArgs a) {
   extern __shared__ __align__(128) uint8_t s_rows[];       // [kStages][unit_heads * 256]
-  __shared__ RowPlan s_plan[kStages][ROWS];
+  __shared__ RowPlan<NORM> s_plan[kStages][ROWS];
   __shared__ __align__(8) uint64_t s_full[kStages], s_empty[kStages];
   __shared__ int s_abort;
   const Pages& p = a.pages;
@@ -205,6 +221,14 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) rope_append_kerne
   if (warp >= kWorkWarps) {
     // ---------------- service warps: every second unit each ----------------
     int i = warp - kWorkWarps;
+    float w[2][4] = {};
+    if (NORM == kOneWeight) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        w[0][x] = Elem<DT>::from_bits(reinterpret_cast<const uint16_t*>(a.q_norm)[lane + 32 * x]);
+        w[1][x] = Elem<DT>::from_bits(reinterpret_cast<const uint16_t*>(a.k_norm)[lane + 32 * x]);
+      }
+    }
     for (; ok && i < mine; i += kServiceWarps) {
       const int s = i % kStages, u = u_lo + i, row = ROWS == 1 ? u / a.units_per_row : u * unit_rows;
       const int head0 = ROWS == 1 ? (u - row * a.units_per_row) * a.unit_heads : 0, n_rows = ROWS == 1 ? 1 : min(unit_rows, a.rows - row);
@@ -215,7 +239,7 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) rope_append_kerne
       __syncwarp();
       if (lane < n_rows)
         bulk_load(smem_u32(s_rows) + s * unit_bytes + lane * bytes, a.qkv + (row + lane) * a.qkv_stride + head0 * 16, bytes, full);
-      plan_rows<ROWS>(a, row, n_rows, lane, s_plan[s]);
+      plan_rows<ROWS, NORM>(a, row, n_rows, lane, w, s_plan[s]);
       __syncwarp();
       if (lane == 0) mbar_arrive(full);
     }
@@ -235,40 +259,17 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) rope_append_kerne
       const uint4* src = reinterpret_cast<const uint4*>(s_rows + s * unit_bytes);
       if (head0 == 0) {
         for (int k = tid; k < n_rows * p.hk; k += kWorkThreads) {
-          const RowPlan& plan = s_plan[s][ROWS == 1 ? 0 : k / p.hk];
+          const RowPlan<NORM>& plan = s_plan[s][ROWS == 1 ? 0 : k / p.hk];
           if (plan.id < 0) continue;
           const int64_t at = record_at(p, plan.id, ROWS == 1 ? k : k % p.hk, plan.row);
           if (p.weight != nullptr) p.weight[at] = 0.f;
           if (p.token != nullptr) p.token[at] = plan.token;
         }
       }
-      float cs[16];                                    // this piece's eight cosines, then its eight sines
       int r = -1, id = -1, at = 0;                     // of row r of the unit
-      for (int j = half; j < n_rows * n; j += kWorkThreads / 16) {
-        if (r < 0 || (ROWS > 1 && j >= (r + 1) * n)) {
-          r = ROWS == 1 ? 0 : j / n;
-          const RowPlan& plan = s_plan[s][r];
-          id = plan.id;
-          at = plan.row;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float4 f = reinterpret_cast<const float4*>(plan.cs)[(k >> 1) * 16 + (c & 7) * 2 + (k & 1)];
-            cs[4 * k] = f.x; cs[4 * k + 1] = f.y; cs[4 * k + 2] = f.z; cs[4 * k + 3] = f.w;
-          }
-        }
-        const int row = row0 + r, head = head0 + j - r * n, h = head - a.hq, hv = h - p.hk;
-        const uint4 x = src[j * 16 + c];
-        uint4 res = x;
-        if (hv < 0) {
-          const uint4 other = src[j * 16 + (c ^ 8)];
-          if (NORM) {
-            const uint4* w = h < 0 ? a.q_norm + head * a.q_norm_stride : a.k_norm + h * a.k_norm_stride;
-            const float inv = rsqrtf(head_squares<DT>(x, half_warp) * (1.f / RI_HEAD_DIM) + a.eps);
-            res = rotate_normed<DT>(x, other, ri_ldg16(w + c), ri_ldg16(w + (c ^ 8)), inv, cs, sign);
-          } else {
-            res = rotate<DT>(x, other, cs, sign);
-          }
-        }
+      // where head `head` of that row goes
+      auto put = [&](int row, int head, const uint4& res) {
+        const int h = head - a.hq, hv = h - p.hk;
         if (h < 0) {
           a.q[((int64_t)row * a.hq + head) * 16 + c] = res;
         } else {
@@ -280,6 +281,72 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) rope_append_kerne
             else a.keys[id * (p.key_stride / 8) + in_page] = res;
           }
         }
+      };
+      if constexpr (NORM == kNone) {
+        float cs[16];                                  // this piece's eight cosines, then its eight sines
+        for (int j = half; j < n_rows * n; j += kWorkThreads / 16) {
+          if (r < 0 || (ROWS > 1 && j >= (r + 1) * n)) {
+            r = ROWS == 1 ? 0 : j / n;
+            const RowPlan<NORM>& plan = s_plan[s][r];
+            id = plan.id;
+            at = plan.row;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float4 f = reinterpret_cast<const float4*>(plan.cs)[(k >> 1) * 16 + (c & 7) * 2 + (k & 1)];
+              cs[4 * k] = f.x; cs[4 * k + 1] = f.y; cs[4 * k + 2] = f.z; cs[4 * k + 3] = f.w;
+            }
+          }
+          const int head = head0 + j - r * n;
+          const uint4 x = src[j * 16 + c];
+          put(row0 + r, head, head >= a.hq + p.hk ? x : rotate<DT>(x, src[j * 16 + (c ^ 8)], cs, sign));
+        }
+      } else {
+        uint64_t fa[4], fb[4];                         // factors of this piece's channels, and of those it is rotated with
+        bool of_keys = false;                          // kOneWeight: whose they are
+        for (int j = half; j < n_rows * n; j += kWorkThreads / 16) {
+          const bool next = r < 0 || (ROWS > 1 && j >= (r + 1) * n);
+          if (next) {
+            r = ROWS == 1 ? 0 : j / n;
+            id = s_plan[s][r].id;
+            at = s_plan[s][r].row;
+          }
+          const int head = head0 + j - r * n;
+          const bool key = head >= a.hq;
+          const uint4 mine16 = src[j * 16 + c];
+          if (head >= a.hq + p.hk) {
+            put(row0 + r, head, mine16);
+            continue;
+          }
+          if (next || (NORM == kOneWeight && key != of_keys)) {
+            of_keys = key;
+            const float* from = s_plan[s][r].cs + (NORM == kOneWeight ? (key ? 256 : 0) + 8 * c : 8 * (c & 7));
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float4 f = reinterpret_cast<const float4*>(from)[k], g = reinterpret_cast<const float4*>(from + (NORM == kOneWeight ? 128 : 64))[k];
+              const float turn = NORM == kOneWeight ? 1.f : sign;
+              fa[2 * k] = pack_f2(f.x, f.y);
+              fa[2 * k + 1] = pack_f2(f.z, f.w);
+              fb[2 * k] = pack_f2(turn * g.x, turn * g.y);
+              fb[2 * k + 1] = pack_f2(turn * g.z, turn * g.w);
+            }
+          }
+          uint64_t x[4], y[4];
+          unpack_pairs<DT>(mine16, x);
+          unpack_pairs<DT>(src[j * 16 + (c ^ 8)], y);
+          const float inv = rsqrtf(head_squares(x, half_warp) * (1.f / RI_HEAD_DIM) + a.eps);
+          if (NORM == kHeadWeights) {
+            const uint4* w = key ? a.k_norm + (head - a.hq) * a.k_norm_stride : a.q_norm + head * a.q_norm_stride;
+            uint64_t wx[4], wy[4];
+            unpack_pairs<DT>(ri_ldg16(w + c), wx);
+            unpack_pairs<DT>(ri_ldg16(w + (c ^ 8)), wy);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              x[k] = mul_f2(x[k], wx[k]);
+              y[k] = mul_f2(y[k], wy[k]);
+            }
+          }
+          put(row0 + r, head, rotate_normed<DT>(x, y, fa, fb, inv));
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&s_empty[s]));
@@ -288,7 +355,7 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) rope_append_kerne
   if (!ok && lane == 0) *p.status = s_abort;
 }
 
-template <int DT, int ROWS, bool NORM>
+template <int DT, int ROWS, int NORM>
 int launch_kernel(const AppendArgs& a, dim3 grid, size_t smem, cudaStream_t s) {
   const int rc = ri_allow_smem<rope_append_kernel<DT, ROWS, NORM>>(kStages * kUnitHeads * 256);
   if (rc != RI_OK) return rc;
@@ -297,7 +364,9 @@ int launch_kernel(const AppendArgs& a, dim3 grid, size_t smem, cudaStream_t s) {
 }
 template <int DT, int ROWS>
 int launch(const AppendArgs& a, dim3 grid, size_t smem, cudaStream_t s) {
-  return a.q_norm != nullptr ? launch_kernel<DT, ROWS, true>(a, grid, smem, s) : launch_kernel<DT, ROWS, false>(a, grid, smem, s);
+  if (a.q_norm == nullptr) return launch_kernel<DT, ROWS, kNone>(a, grid, smem, s);
+  return a.q_norm_stride == 0 && a.k_norm_stride == 0 ? launch_kernel<DT, ROWS, kOneWeight>(a, grid, smem, s)
+                                                      : launch_kernel<DT, ROWS, kHeadWeights>(a, grid, smem, s);
 }
 
 struct Norms {
