@@ -401,9 +401,10 @@ int64_t ri_paged_prompt_scratch_bytes(const ri_paged* p, int32_t rows, int32_t w
 int ri_paged_prompt(const ri_paged* p, const void* d_q, int64_t q_stride, int32_t rows, const int32_t* d_row_start, int32_t window,
                     int32_t sink, void* d_out, float* d_lse, float scale, void* d_scratch, void* stream);
 /* ri_paged_decode where requests have their first slots in common, which are read once for all of them: requests d_group_start[g] ..
- * d_group_start[g + 1] - 1 (ascending; int32 [groups + 1]) have the first d_shared[g] slots in common, which are read through the
- * first one's row of the page table; requests in no group have none.  A request shorter than that sees what it has.  batch + groups at
- * most 16384.  d_weight is not used. */
+ * d_group_start[g + 1] - 1 (ascending; int32 [groups + 1], groups at most batch and 16384) have the first d_shared[g] slots in common:
+ * their rows of the page table begin alike, as far as those slots and the first one's length go.  Requests in no group have none; a
+ * request shorter than that sees what it has.  Where all slots that the table has room for are few, requests are attended one by one.
+ * d_weight must be NULL.  d_scratch: that many bytes of 16-byte aligned device memory, any contents, for this call alone. */
 int64_t ri_paged_shared_decode_scratch_bytes(const ri_paged* p, int32_t groups);
 int ri_paged_shared_decode(const ri_paged* p, const void* d_q, int64_t q_stride, const int32_t* d_group_start, int32_t groups,
                            const int32_t* d_shared, void* d_out, float* d_lse, float scale, void* d_scratch, void* stream);

@@ -2,7 +2,7 @@
 //   out_r = sum_j p_rj v_j,  p_rj = e^{s_rj - lse_r},  s_rj = scale q_r.k_j,  lse_r = log sum_j e^{s_rj},  over the slots j that row r sees:
 // ri_paged_prompt         several new tokens of every request: the token at slot s sees j <= s with j > s - window or j < sink;
 // ri_paged_shared_decode  one new token of every request, where groups of requests have their first slots in common: a group's rows over
-//                         those slots are worked on together, each request's over the slots of its own, and both are joined by log-sum-exp.
+//                         those slots are worked on together here; each request's own slots and the join are ri_paged_decode.cu's.
 // A row that sees nothing, or only scores of -infinity, has out 0 and lse -infinity; a NaN or +infinity among its scores makes both NaN.
 //
 // The rows of a tile of 128 are tokens (or requests) times the query heads of one KV head, so K and V serve a whole group of heads and a
@@ -25,13 +25,15 @@
 
 #include <type_traits>
 
-#include "ri_paged.cuh"
+#include "ri_paged_shared.cuh"
 #include "ri_tc.cuh"
 
 namespace {
 
 using namespace ri_tc;
 using namespace ri_page;
+using ri_shared::clamped;
+using ri_shared::group_of;
 
 constexpr int kTile = 128;                 // query rows of a tile, slots of a step
 constexpr int kHalf = kTile * 128;         // bytes of a 128-row x 64-channel half-tile
@@ -41,7 +43,7 @@ constexpr int kSegments = 4;               // segments on their way from the war
 constexpr int kTails = 4;                 // V tiles in the ring that a request's slots end in: it holds three V tiles
 constexpr uint32_t kTmemCols = 512;
 constexpr int kMaxCtas = 160;
-constexpr int kMaxRequests = 16384;        // of a call, or groups and requests together
+constexpr int kMaxRequests = 16384;        // of a call, or groups
 constexpr int kMaxEntries = 8192;          // of the table of steps
 // An item's end this many steps from the end of a CTA's range becomes the end of the range: a part of an item costs as much again
 // for its partial result and the second kernel.  Items of at most twice as many are never cut.
@@ -92,11 +94,11 @@ struct Args : Pages {
   int64_t q_stride;          // elements
   uint16_t* out;
   float* lse;                // or null
-  float* part_o;             // rows of 128, a segment's in the order [channels / 4][rows][4]
+  float* part_o;             // rows of 128, a segment's in the order [channels / 8][rows][8]
   float2* part_ml;           // (reference in the log2 domain, sum)
-  int* meta;                 // prompt: [CTAs][kMeta]; SHARED: CTAs (first, last) of the items [groups, then own][hk * batch]
-  int64_t part_own;          // SHARED: rows of partial results in front of those of the requests' own slots
-  int n_seq, groups, n_rows; // sequences: requests, or groups and then requests; rows of q
+  int* meta;                 // prompt: [CTAs][kMeta]; SHARED: CTAs (first, last) of the items
+  int32_t* from;             // SHARED: what every request has in common with its group
+  int n_seq, n_rows;         // sequences: requests, or groups; rows of q
   int gs, tile_tokens, max_ctas, part_rows;      // tokens of a tile; rows of a CTA's part of the partial results
   int window, sink;          // window 0: none
   float scale2;
@@ -106,22 +108,12 @@ struct Args : Pages {
 // ---- what there is to do: sequences of rows over a request's slots, cut into pairs of tiles ----------------------------
 struct Seq {
   int n, q_row, table_row;               // tokens (or requests), the first one's row of q, whose page table
-  int low, rows;                         // slots [low, rows) count; low > 0: a request's own slots behind a group's
+  int rows;                              // slots that count
 };
 struct Item {
   int n_tok, front, skip, low, high, sink, steps;
   __device__ __forceinline__ int cost() const { return steps + kItemCost; }
 };
-__device__ __forceinline__ int clamped(int x, int most) { return min(max(x, 0), most); }
-// The group that request b is in, or -1.
-__device__ __forceinline__ int group_of(const Args& a, int b) {
-  int lo = 0, hi = a.groups;             // starts[lo] <= b < starts[hi], if it is in one
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    (a.starts[mid] <= b ? lo : hi) = mid;
-  }
-  return a.starts[lo] <= b && b < a.starts[lo + 1] ? lo : -1;
-}
 // What requests of group g have in common: as far as the first one's slots go.
 __device__ __forceinline__ int in_common(const Args& a, int g) {
   const int b = clamped(a.starts[g], a.batch);
@@ -129,22 +121,16 @@ __device__ __forceinline__ int in_common(const Args& a, int g) {
 }
 template <bool SHARED>
 __device__ __forceinline__ Seq seq_of(const Args& a, int v) {
-  Seq s = {0, 0, v, 0, 0};
+  Seq s = {0, 0, v, 0};
   if (!SHARED) {
     s.q_row = clamped(a.starts[v], a.n_rows);
     s.n = max(0, clamped(a.starts[v + 1], a.n_rows) - s.q_row);
     s.rows = rows_of(a, v);
-  } else if (v < a.groups) {
+  } else {
     s.q_row = clamped(a.starts[v], a.batch);
     s.table_row = min(s.q_row, a.batch - 1);
     s.rows = in_common(a, v);
     s.n = s.rows > 0 ? max(0, clamped(a.starts[v + 1], a.batch) - s.q_row) : 0;
-  } else {
-    s.q_row = s.table_row = v - a.groups;
-    const int g = group_of(a, s.q_row);
-    s.rows = rows_of(a, s.q_row);
-    s.low = g >= 0 ? min(in_common(a, g), s.rows) : 0;
-    s.n = s.rows > s.low ? 1 : 0;
   }
   return s;
 }
@@ -154,7 +140,7 @@ __device__ __forceinline__ Item item_of(const Args& a, const Seq& s, int p) {
   Item it;
   const int first = p * 2 * a.tile_tokens;
   it.n_tok = min(s.n - first, 2 * a.tile_tokens);
-  it.low = s.low;
+  it.low = 0;
   it.high = s.rows;
   it.sink = 0;
   if (!SHARED) {
@@ -405,7 +391,8 @@ __device__ __noinline__ void redo(const Args& a, const Segment& sg, unsigned bad
       const uint2 u = make_uint2(Elem<DT>::pack2(o[0] * factor, o[1] * factor), Elem<DT>::pack2(o[2] * factor, o[3] * factor));
       *reinterpret_cast<uint2*>(a.out + ((int64_t)tok * a.hk * a.gs + h) * RI_HEAD_DIM + lane * 4) = u;
     } else {
-      reinterpret_cast<float4*>(a.part_o + (int64_t)sg.part * RI_HEAD_DIM)[lane * n_rows + r] = make_float4(o[0], o[1], o[2], o[3]);
+      reinterpret_cast<float4*>(a.part_o + (int64_t)sg.part * RI_HEAD_DIM)[((lane >> 1) * n_rows + r) * 2 + (lane & 1)] =
+          make_float4(o[0], o[1], o[2], o[3]);
     }
   }
 }
@@ -456,6 +443,11 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   ri_pdl_wait();
   ri_pdl_trigger();                        // the kernel that joins waits for the end of this one
   const bool aligned = s.abort == 0;       // of the whole CTA
+  if (SHARED)
+    for (int b = c * kThreads + (int)threadIdx.x; b < a.batch; b += (int)gridDim.x * kThreads) {
+      const int g = group_of(a.starts, a.n_seq, b);
+      a.from[b] = g >= 0 ? min(in_common(a, g), rows_of(a, b)) : 0;
+    }
   if (aligned) plan<SHARED>(a, reinterpret_cast<int*>(smem + 4 * kHalf), s);
 
   // every role goes through the segments one by one, whole warps
@@ -728,12 +720,10 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           sg.two = it.n_tok > a.tile_tokens;
           const bool begins = step == 0, ends = end == it.steps;
           if (SHARED) {
-            const bool own = v >= a.groups;
-            const int64_t at = (int64_t)h * a.batch + sg.q_row, rows = own ? a.part_own + (int64_t)c * a.gs : (int64_t)c * a.part_rows;
-            sg.part = (int)(rows + at * a.gs);
-            int* ctas = a.meta + 2 * (at + (own ? (int64_t)a.hk * a.batch : 0));
-            if (begins) ctas[0] = c;
-            if (ends) ctas[1] = c;
+            const int at = h * a.batch + sg.q_row;
+            sg.part = c * a.part_rows + at * a.gs;
+            if (begins) a.meta[2 * at] = c;
+            if (ends) a.meta[2 * at + 1] = c;
           } else {
             sg.part = begins && ends ? -1 : (2 * c + begins) * a.part_rows;
             if (!begins) head = ends ? 1 : 2;                   // another CTA's item: it ends here, or goes on behind
@@ -955,9 +945,9 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 store32(dst + y, u, wide);
               }
             } else {
-              float4* dst = reinterpret_cast<float4*>(a.part_o + (int64_t)sg.part * RI_HEAD_DIM) + x * 8 * n_rows + item_row;
+              float4* dst = reinterpret_cast<float4*>(a.part_o + (int64_t)sg.part * RI_HEAD_DIM) + (x * 4 * n_rows + item_row) * 2;
 #pragma unroll
-              for (int y = 0; y < 32; y += 4) dst[y / 4 * n_rows] = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+              for (int y = 0; y < 32; y += 4) dst[y / 8 * 2 * n_rows + (y / 4 & 1)] = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
             }
           }
         }
@@ -1027,10 +1017,10 @@ __global__ void __launch_bounds__(kJoinThreads) prompt_join_kernel(const __grid_
   for (int x = 0; x < 4; ++x) o[x] = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i = c; i <= last; ++i) {
     const float f = part_factor(a.part_ml[part_at(i) + row].x, all.m);
-    const float4* src = reinterpret_cast<const float4*>(a.part_o + part_at(i) * RI_HEAD_DIM) + warp * 4 * n_rows + row;
+    const float4* src = reinterpret_cast<const float4*>(a.part_o + part_at(i) * RI_HEAD_DIM) + (warp * 2 * n_rows + row) * 2;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      const float4 y = src[x * n_rows];
+      const float4 y = src[(x >> 1) * 2 * n_rows + (x & 1)];
       o[x].x += f * y.x; o[x].y += f * y.y; o[x].z += f * y.z; o[x].w += f * y.w;
     }
   }
@@ -1042,57 +1032,6 @@ __global__ void __launch_bounds__(kJoinThreads) prompt_join_kernel(const __grid_
     dst[x] = make_uint4(Elem<DT>::pack2(o[2 * x].x * f, o[2 * x].y * f), Elem<DT>::pack2(o[2 * x].z * f, o[2 * x].w * f),
                         Elem<DT>::pack2(o[2 * x + 1].x * f, o[2 * x + 1].y * f), Elem<DT>::pack2(o[2 * x + 1].z * f, o[2 * x + 1].w * f));
   if (warp == 0 && a.lse != nullptr) a.lse[at] = all.lse();
-}
-
-// ri_paged_shared_decode: a block per request and KV head, a thread per query head and four channels, over the parts of the group's
-// item and then of the request's own.
-template <int DT>
-__global__ void __launch_bounds__(kJoinThreads) shared_join_kernel(const __grid_constant__ Args a) {
-  ri_pdl_enter();
-  const int b = blockIdx.x, h = blockIdx.y, quad = threadIdx.x / a.gs, r = threadIdx.x - quad * a.gs;
-  const int g = group_of(a, b), rows = rows_of(a, b), common = g >= 0 ? in_common(a, g) : 0;
-  // the two items: rows of theirs, this one's place among them, their parts
-  const int* ctas = nullptr;
-  int first[2] = {0, 0}, last[2] = {-1, -1}, n_rows[2] = {0, a.gs}, row[2] = {0, r};
-  int64_t part[2] = {0, 0};
-  if (common > 0) {
-    const int b0 = clamped(a.starts[g], a.batch), b1 = clamped(a.starts[g + 1], a.batch), pair = 2 * a.tile_tokens;
-    const int q_row = b0 + (b - b0) / pair * pair;
-    n_rows[0] = min(pair, b1 - q_row) * a.gs;
-    row[0] = (b - q_row) * a.gs + r;
-    part[0] = ((int64_t)h * a.batch + q_row) * a.gs;
-    ctas = a.meta + 2 * ((int64_t)h * a.batch + q_row);
-    first[0] = clamped(ctas[0], a.max_ctas - 1);
-    last[0] = clamped(ctas[1], a.max_ctas - 1);
-  }
-  if (rows > common) {
-    const int64_t item = (int64_t)h * a.batch + b;
-    part[1] = a.part_own + item * a.gs;
-    ctas = a.meta + 2 * (item + (int64_t)a.hk * a.batch);
-    first[1] = clamped(ctas[0], a.max_ctas - 1);
-    last[1] = clamped(ctas[1], a.max_ctas - 1);
-  }
-  if (quad >= RI_HEAD_DIM / 4) return;
-  const int each[2] = {a.part_rows, a.gs};
-  Joined all;
-#pragma unroll
-  for (int x = 0; x < 2; ++x)
-#pragma unroll 4
-    for (int c = first[x]; c <= last[x]; ++c) all.add(a.part_ml[part[x] + (int64_t)c * each[x] + row[x]]);
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-  for (int x = 0; x < 2; ++x)
-#pragma unroll 4
-    for (int c = first[x]; c <= last[x]; ++c) {
-      const int64_t at = part[x] + (int64_t)c * each[x];
-      const float f = part_factor(a.part_ml[at + row[x]].x, all.m);
-      const float4 y = reinterpret_cast<const float4*>(a.part_o + at * RI_HEAD_DIM)[quad * n_rows[x] + row[x]];
-      o.x += f * y.x; o.y += f * y.y; o.z += f * y.z; o.w += f * y.w;
-    }
-  const float f = all.scale();
-  const int64_t at = ((int64_t)b * a.hk + h) * a.gs + r;
-  *reinterpret_cast<uint2*>(a.out + at * RI_HEAD_DIM + quad * 4) = make_uint2(Elem<DT>::pack2(o.x * f, o.y * f), Elem<DT>::pack2(o.z * f, o.w * f));
-  if (quad == 0 && a.lse != nullptr) a.lse[at] = all.lse();
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------
@@ -1142,7 +1081,7 @@ int check_call(const char* what, const ri_paged* p, int64_t sequences) {
   const int rc = check(p, what);
   if (rc != RI_OK) return rc;
   RI_REQUIRE(p->group_size >= 1 && p->group_size <= kHeadsMost, "%s: group_size=%d unsupported (1 to %d)", what, p->group_size, kHeadsMost);
-  RI_REQUIRE(sequences >= 1 && sequences <= kMaxRequests, "%s: %lld requests (and groups) unsupported (%d at most)", what, (long long)sequences,
+  RI_REQUIRE(sequences >= 1 && sequences <= kMaxRequests, "%s: %lld requests or groups unsupported (%d at most)", what, (long long)sequences,
              kMaxRequests);
   return RI_OK;
 }
@@ -1152,9 +1091,7 @@ int launch(const Args& a, const CUtensorMap& map_q, const CUtensorMap& map_k, co
   const int rc = ri_allow_smem<paged_attend_kernel<DT, SHARED>>(kSmem);
   if (rc != RI_OK) return rc;
   RI_CUDA_OK(ri_launch_pdl_id(11, paged_attend_kernel<DT, SHARED>, dim3(a.max_ctas), dim3(kThreads), (size_t)kSmem, s, map_q, map_k, map_v, a));
-  if (SHARED) {
-    RI_CUDA_OK(ri_launch_pdl_id(11, shared_join_kernel<DT>, dim3(a.batch, a.hk), dim3(kJoinThreads), 0, s, a));
-  } else if (join) {
+  if (join) {
     RI_CUDA_OK(ri_launch_pdl_id(11, prompt_join_kernel<DT>, dim3(a.max_ctas, (a.part_rows + kJoinRows - 1) / kJoinRows), dim3(kJoinThreads), 0, s, a));
   }
   return RI_OK;
@@ -1162,9 +1099,9 @@ int launch(const Args& a, const CUtensorMap& map_q, const CUtensorMap& map_k, co
 
 template <bool SHARED>
 int attend(const char* what, const ri_paged* p, const void* d_q, int64_t q_stride, int rows, Args a, void* d_out, float* d_lse, float scale,
-           bool join, void* stream) {
+           bool join, cudaStream_t s) {
   int rc;
-  RI_REQUIRE(p->d_values && d_q && d_out && a.starts, "%s: null pointer", what);
+  RI_REQUIRE(p->d_values && d_q && (SHARED || d_out) && a.starts, "%s: null pointer", what);
   RI_REQUIRE(q_stride >= (int64_t)p->kv_heads * p->group_size * RI_HEAD_DIM && q_stride % 8 == 0, "%s: queries overlap or lie at odd places", what);
   RI_REQUIRE(((uintptr_t)d_q | (uintptr_t)d_out) % 16 == 0, "%s: tensors must be 16-byte aligned", what);
   RI_REQUIRE(scale > 0.f && scale < 1e30f, "%s: scale must be positive and finite", what);
@@ -1189,16 +1126,14 @@ int attend(const char* what, const ri_paged* p, const void* d_q, int64_t q_strid
   if ((rc = make_query_map(&map_q, d_q, q_stride, p->kv_heads * a.gs, rows, a.gs, a.tile_tokens, p->dtype)) != RI_OK) return rc;
   if ((rc = make_pool_map(&map_k, p->d_keys, *p, p->key_page_stride)) != RI_OK) return rc;
   if ((rc = make_pool_map(&map_v, p->d_values, *p, p->value_page_stride)) != RI_OK) return rc;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   return p->dtype == RI_BF16 ? launch<RI_BF16, SHARED>(a, map_q, map_k, map_v, join, s) : launch<RI_F16, SHARED>(a, map_q, map_k, map_v, join, s);
 }
 
 // Workspaces: meta, sums, outputs of the parts.
 int64_t prompt_part_rows(const ri_paged& p, int rows) { return 2 * kMaxCtas * most_items_rows(p, rows); }
 constexpr int64_t kPromptMeta = (int64_t)kMaxCtas * kMeta * 4;
-int64_t shared_meta(const ri_paged& p) { return ri_align_up(16 * (int64_t)p.batch * p.kv_heads, 16); }
+int64_t shared_meta(const ri_paged& p) { return ri_align_up(8 * (int64_t)p.batch * p.kv_heads + 4 * (int64_t)p.batch, 16); }
 int64_t shared_rows(const ri_paged& p) { return (int64_t)kMaxCtas * most_items_rows(p, p.batch) + (int64_t)p.batch * p.kv_heads * p.group_size; }
-int64_t own_rows(const ri_paged& p) { return ((int64_t)kMaxCtas + (int64_t)p.batch * p.kv_heads) * p.group_size; }
 void place(Args& a, void* d_scratch, int64_t meta, int64_t rows) {
   a.meta = static_cast<int*>(d_scratch);
   a.part_o = reinterpret_cast<float*>(static_cast<char*>(d_scratch) + meta);
@@ -1225,28 +1160,25 @@ extern "C" int ri_paged_prompt(const ri_paged* p, const void* d_q, int64_t q_str
   a.window = window;
   a.sink = sink;
   if (bytes > 0) place(a, d_scratch, kPromptMeta, prompt_part_rows(*p, rows));
-  return attend<false>("ri_paged_prompt", p, d_q, q_stride, rows, a, d_out, d_lse, scale, bytes > 0, stream);
+  return attend<false>("ri_paged_prompt", p, d_q, q_stride, rows, a, d_out, d_lse, scale, bytes > 0, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int64_t ri_paged_shared_decode_scratch_bytes(const ri_paged* p, int32_t groups) {
-  const int rc = check_call("ri_paged_shared_decode", p, p ? (int64_t)p->batch + (groups > 0 ? groups : 0) : 1);
+int64_t ri_shared::scratch_bytes(const ri_paged& p) { return shared_meta(p) + shared_rows(p) * (RI_HEAD_DIM + 2) * 4; }
+
+int ri_shared::launch(const char* what, const ri_paged* p, const void* d_q, int64_t q_stride, const int32_t* d_group_start, int32_t groups,
+                      const int32_t* d_shared, float scale, void* d_scratch, Parts* parts, cudaStream_t s) {
+  const int rc = check_call(what, p, groups);
   if (rc != RI_OK) return rc;
-  if (groups < 1) return ri_fail(RI_ERR_INVALID, "ri_paged_shared_decode: groups=%d unsupported", groups);
-  return shared_meta(*p) + (shared_rows(*p) + own_rows(*p)) * (RI_HEAD_DIM + 2) * 4;
-}
-
-extern "C" int ri_paged_shared_decode(const ri_paged* p, const void* d_q, int64_t q_stride, const int32_t* d_group_start, int32_t groups,
-                                      const int32_t* d_shared, void* d_out, float* d_lse, float scale, void* d_scratch, void* stream) {
-  const int64_t bytes = ri_paged_shared_decode_scratch_bytes(p, groups);
-  if (bytes < 0) return (int)bytes;
-  RI_REQUIRE(d_shared && d_scratch, "ri_paged_shared_decode: null pointer");
-  RI_REQUIRE((uintptr_t)d_scratch % 16 == 0, "ri_paged_shared_decode: the scratch must be 16-byte aligned");
   Args a = {};
   a.starts = d_group_start;
   a.shared = d_shared;
-  a.groups = groups;
-  a.n_seq = groups + p->batch;
-  a.part_own = shared_rows(*p);
-  place(a, d_scratch, shared_meta(*p), shared_rows(*p) + own_rows(*p));
-  return attend<true>("ri_paged_shared_decode", p, d_q, q_stride, p->batch, a, d_out, d_lse, scale, true, stream);
+  a.n_seq = groups;
+  place(a, d_scratch, shared_meta(*p), shared_rows(*p));
+  a.from = a.meta + 2 * (int64_t)p->batch * p->kv_heads;
+  int sms = 0;
+  const int rc2 = ri_sm_count(&sms);
+  if (rc2 != RI_OK) return rc2;
+  *parts = {d_group_start, a.from, a.meta, a.part_o, a.part_ml, groups, 2 * (kTile / p->group_size), (int)most_items_rows(*p, p->batch),
+            sms < kMaxCtas ? sms : kMaxCtas};
+  return attend<true>(what, p, d_q, q_stride, p->batch, a, nullptr, nullptr, scale, false, s);
 }

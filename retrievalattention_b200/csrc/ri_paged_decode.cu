@@ -26,7 +26,9 @@
 // many partial results: 340 -> 362 and 98 -> 108 us.
 #include <cooperative_groups.h>
 
-#include "ri_paged.cuh"
+#include <type_traits>
+
+#include "ri_paged_shared.cuh"
 #include "ri_step_sequence.cuh"
 #include "ri_tc.cuh"
 #include "ri_wave_attend.cuh"
@@ -99,6 +101,19 @@ __device__ __forceinline__ WindowSpan span_of(const WindowArgs& a, int b) {
 }
 __device__ __forceinline__ int rows_of(const WindowArgs& a, int b) {
   return ri_page::rows_of(static_cast<const Pages&>(a), b) - span_of(a, b).skip;
+}
+
+// The slots of its own that a request has behind those it has in common with others, whose partial results are there already.
+struct SharedArgs : PagedArgs {
+  ri_shared::Parts common;
+};
+__device__ __forceinline__ WindowSpan span_of(const SharedArgs& a, int b) {
+  const int low = a.common.from[b];
+  return {0, low & ~15, low, 0};
+}
+__device__ __forceinline__ int rows_of(const SharedArgs& a, int b) {
+  const int n = ri_page::rows_of(static_cast<const Pages&>(a), b), low = a.common.from[b];
+  return n > low ? n - (low & ~15) : 0;
 }
 
 // The scores of a step lie in the order of the lanes that made them: place i holds key (i / 2 % 2) * 8 + i / 4 + (i % 2) * 4.
@@ -538,7 +553,37 @@ __global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_ke
   if (folds) find_pages(blockIdx.x);
   if (tid == 0) s_n = count;
   ri_pdl_wait();
-  if (n == 0) {
+  // SharedArgs: parts of the item over what the request has in common with others, behind the group's own
+  constexpr bool kShared = std::is_same_v<Args, SharedArgs>;
+  int extra = 0, item_rows = 0, item_row = 0;
+  int64_t item_part = 0;
+  if constexpr (kShared) {
+    if (a.common.from[b] > 0) {
+      const int of = ri_shared::group_of(a.common.starts, a.common.groups, b);
+      const int b0 = ri_shared::clamped(a.common.starts[of], a.batch), b1 = ri_shared::clamped(a.common.starts[of + 1], a.batch);
+      const int first = b0 + (b - b0) / a.common.pair * a.common.pair, item = h_kv * a.batch + first;
+      const int c0 = ri_shared::clamped(a.common.ctas[2 * item], a.common.max_ctas - 1);
+      extra = ri_shared::clamped(a.common.ctas[2 * item + 1], a.common.max_ctas - 1) - c0 + 1;
+      item_rows = min(a.common.pair, b1 - first) * gs;
+      item_row = (b - first) * gs;
+      item_part = (int64_t)c0 * a.common.part_rows + (int64_t)item * gs;
+    }
+  }
+  auto ml_of = [&](int i, int head) {
+    if constexpr (kShared) {
+      if (i >= s_n) return a.common.ml[item_part + (int64_t)(i - s_n) * a.common.part_rows + item_row + head];
+    }
+    return a.part_ml[(int64_t)s_slot[i] * gs + head];
+  };
+  auto four_of = [&](int i, int head) {
+    if constexpr (kShared) {
+      if (i >= s_n)
+        return reinterpret_cast<const float4*>(a.common.o + (item_part + (int64_t)(i - s_n) * a.common.part_rows) * RI_HEAD_DIM)
+            [((lane >> 1) * item_rows + item_row + head) * 2 + (lane & 1)];
+    }
+    return reinterpret_cast<const float4*>(a.part_o + ((int64_t)s_slot[i] * gs + head) * RI_HEAD_DIM)[lane];
+  };
+  if (n == 0 && extra <= 0) {
     for (int h = blockIdx.x; h < gs; h += gridDim.x) {
       if (tid < RI_HEAD_DIM) a.out[((int64_t)g * gs + h) * RI_HEAD_DIM + tid] = 0;
       if (tid == 0 && a.lse != nullptr) a.lse[g * gs + h] = -INFINITY;
@@ -547,7 +592,7 @@ __global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_ke
   }
   if (folds) fetch(blockIdx.x);
   __syncthreads();
-  count = s_n;
+  count = s_n + max(extra, 0);
   if (warp < gs) {
     float M = -INFINITY, L = 0.f;
     for (int i0 = 0; i0 < count; i0 += 32 * kTogether) {
@@ -555,7 +600,7 @@ __global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_ke
 #pragma unroll
       for (int u = 0; u < kTogether; ++u) {
         const int i = i0 + u * 32 + lane;
-        ml[u] = i < count ? a.part_ml[(int64_t)s_slot[i] * gs + warp] : make_float2(-INFINITY, 0.f);
+        ml[u] = i < count ? ml_of(i, warp) : make_float2(-INFINITY, 0.f);
       }
       float most = M;
 #pragma unroll
@@ -590,9 +635,8 @@ __global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_ke
         const int i = i0 + u * (kFinishThreads / 32);
         m[u] = -INFINITY;
         if (i < count) {
-          const int64_t at = (int64_t)s_slot[i] * gs + head;
-          m[u] = a.part_ml[at].x;
-          x[u] = reinterpret_cast<const float4*>(a.part_o + at * RI_HEAD_DIM)[lane];
+          m[u] = ml_of(i, head).x;
+          x[u] = four_of(i, head);
         }
       }
       float most = M;
@@ -720,7 +764,7 @@ int launch_split(const Args& a, const CUtensorMap& map_k, const CUtensorMap& map
 template <int DT, int BOX, bool WEIGHTS, class Args>
 int launch_steps(const Args& a, const CUtensorMap& map_k, const CUtensorMap& map_v, int ctas, cudaStream_t s) {
   int rc;
-  if (ctas > 0) {
+  if constexpr (!std::is_same_v<Args, SharedArgs>) if (ctas > 0) {
     if ((rc = ri_allow_smem<paged_decode_kernel<DT, BOX, WEIGHTS, true, false, Args>>(kPagedSmem)) != RI_OK) return rc;
     RI_CUDA_OK(ri_launch_pdl_cluster(11, ctas, paged_decode_kernel<DT, BOX, WEIGHTS, true, false, Args>, dim3(a.batch * a.hk * ctas), dim3(kPagedThreads),
                                      (size_t)kPagedSmem, s, map_k, map_v, a));
@@ -735,14 +779,18 @@ int launch_steps(const PagedArgs& a, const CUtensorMap& map_k, const CUtensorMap
   return a.weight ? launch_steps<DT, BOX, true, PagedArgs>(a, map_k, map_v, ctas, s) : launch_steps<DT, BOX, false, PagedArgs>(a, map_k, map_v, ctas, s);
 }
 template <int DT, int BOX>
+int launch_steps(const SharedArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, int ctas, cudaStream_t s) {
+  return launch_steps<DT, BOX, false, SharedArgs>(a, map_k, map_v, 0, s);
+}
+template <int DT, int BOX>
 int launch_steps(const WindowArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, int ctas, cudaStream_t s) {
   return launch_steps<DT, BOX, false, WindowArgs>(a, map_k, map_v, ctas, s);
 }
 template <int DT, class Args>
 int launch_paged(const Args& a, const CUtensorMap& map_k, const CUtensorMap& map_v, int box, cudaStream_t s) {
   const int64_t most = most_rows(a);
-  int ctas, rc;
-  if ((rc = cluster_size(a, most, &ctas)) != RI_OK) return rc;
+  int ctas = 0, rc;
+  if (!std::is_same_v<Args, SharedArgs> && (rc = cluster_size(a, most, &ctas)) != RI_OK) return rc;
   rc = box == 8 ? launch_steps<DT, 8>(a, map_k, map_v, ctas, s) : launch_steps<DT, 16>(a, map_k, map_v, ctas, s);
   if (rc != RI_OK || ctas > 0) return rc;
   const int64_t groups = (int64_t)a.batch * a.hk;
@@ -772,9 +820,9 @@ extern "C" int64_t ri_paged_decode_scratch_bytes(const ri_paged* p) {
 namespace ri_wave {
 namespace {
 
-// window 0: none
-int decode(const char* what, const ri_paged* p, const void* d_q, int64_t q_stride, void* d_out, float* d_lse, float scale, int32_t window,
-           int32_t sink, void* d_scratch, void* stream) {
+// Checks of a call, and what all of its kernels go by.
+int prepare(const char* what, const ri_paged* p, const void* d_q, int64_t q_stride, void* d_out, float* d_lse, float scale, void* d_scratch,
+            PagedArgs& a) {
   int rc;
   if ((rc = ri_page::check(p, what)) != RI_OK) return rc;
   RI_REQUIRE(p->d_values && d_q && d_out && d_scratch, "%s: null pointer", what);
@@ -782,7 +830,6 @@ int decode(const char* what, const ri_paged* p, const void* d_q, int64_t q_strid
   RI_REQUIRE(q_stride >= (int64_t)p->kv_heads * p->group_size * RI_HEAD_DIM && q_stride % 8 == 0, "%s: queries overlap or lie at odd places", what);
   RI_REQUIRE(((uintptr_t)d_q | (uintptr_t)d_out | (uintptr_t)d_scratch) % 16 == 0, "q, out and the scratch must be 16-byte aligned");
   RI_REQUIRE(scale > 0.f && scale < 1e30f, "%s: scale must be positive and finite", what);
-  WindowArgs a = {};
   static_cast<ri_page::Pages&>(a) = ri_page::view(*p);
   a.q = static_cast<const uint4*>(d_q);
   a.q_stride = q_stride / 8;
@@ -795,32 +842,69 @@ int decode(const char* what, const ri_paged* p, const void* d_q, int64_t q_strid
   a.lse = d_lse;
   a.out = static_cast<uint16_t*>(d_out);
   a.scale2 = RI_LOG2E * scale;
-  a.window = window;
-  a.sink = sink;
   int sms = 0;
   if ((rc = ri_sm_count(&sms)) != RI_OK) return rc;
   a.max_ctas = sms < kPagedMaxCtas ? sms : kPagedMaxCtas;
-  const int box = p->page_size < 16 ? 8 : 16;
-  CUtensorMap map_k, map_v;
-  if ((rc = make_page_map(&map_k, p->d_keys, *p, p->key_page_stride, box)) != RI_OK) return rc;
-  if ((rc = make_page_map(&map_v, p->d_values, *p, p->value_page_stride, box)) != RI_OK) return rc;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const PagedArgs& all = a;
-  if (window == 0) return p->dtype == RI_BF16 ? launch_paged<RI_BF16>(all, map_k, map_v, box, s) : launch_paged<RI_F16>(all, map_k, map_v, box, s);
-  return p->dtype == RI_BF16 ? launch_paged<RI_BF16>(a, map_k, map_v, box, s) : launch_paged<RI_F16>(a, map_k, map_v, box, s);
+  return RI_OK;
 }
+template <class Args>
+int launch(const ri_paged& p, const Args& a, void* stream) {
+  int rc;
+  const int box = p.page_size < 16 ? 8 : 16;
+  CUtensorMap map_k, map_v;
+  if ((rc = make_page_map(&map_k, p.d_keys, p, p.key_page_stride, box)) != RI_OK) return rc;
+  if ((rc = make_page_map(&map_v, p.d_values, p, p.value_page_stride, box)) != RI_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return p.dtype == RI_BF16 ? launch_paged<RI_BF16>(a, map_k, map_v, box, s) : launch_paged<RI_F16>(a, map_k, map_v, box, s);
+}
+
+// Requests that begin alike are attended together where all slots there may be are more than this many bytes of K and V.  It takes a
+// kernel more, and requests that are attended one by one find much of what others have read in L2.
+constexpr int64_t kAlikeBytes = 48 << 20;
+bool apart(const ri_paged& p) { return (int64_t)p.batch * p.kv_heads * ri_page::slots_of(p) * 4 * RI_HEAD_DIM <= kAlikeBytes; }
+int64_t own_bytes(const ri_paged& p) { return ri_align_up(paged_slots(p) * p.group_size * (RI_HEAD_DIM + 2) * 4, 16); }
 
 }  // namespace
 }  // namespace ri_wave
 
 extern "C" int ri_paged_decode(const ri_paged* p, const void* d_q, int64_t q_stride, void* d_out, float* d_lse, float scale,
                                void* d_scratch, void* stream) {
-  return ri_wave::decode("ri_paged_decode", p, d_q, q_stride, d_out, d_lse, scale, 0, 0, d_scratch, stream);
+  ri_wave::PagedArgs a = {};
+  const int rc = ri_wave::prepare("ri_paged_decode", p, d_q, q_stride, d_out, d_lse, scale, d_scratch, a);
+  return rc != RI_OK ? rc : ri_wave::launch(*p, a, stream);
 }
 
 extern "C" int ri_paged_decode_window(const ri_paged* p, const void* d_q, int64_t q_stride, int32_t window, int32_t sink, void* d_out,
                                       float* d_lse, float scale, void* d_scratch, void* stream) {
   RI_REQUIRE(window >= 1 && sink >= 0, "ri_paged_decode_window: window=%d sink=%d unsupported", window, sink);
   RI_REQUIRE(p == nullptr || p->d_weight == nullptr, "ri_paged_decode_window: weights are added up over all slots, not over a window");
-  return ri_wave::decode("ri_paged_decode_window", p, d_q, q_stride, d_out, d_lse, scale, window, sink, d_scratch, stream);
+  ri_wave::WindowArgs a = {};
+  const int rc = ri_wave::prepare("ri_paged_decode_window", p, d_q, q_stride, d_out, d_lse, scale, d_scratch, a);
+  a.window = window;
+  a.sink = sink;
+  return rc != RI_OK ? rc : ri_wave::launch(*p, a, stream);
+}
+
+extern "C" int64_t ri_paged_shared_decode_scratch_bytes(const ri_paged* p, int32_t groups) {
+  const int rc = ri_page::check(p, "ri_paged_shared_decode");
+  if (rc != RI_OK) return rc;
+  if (p->group_size < 1 || p->group_size > ri_wave::kMaxHeads)
+    return ri_fail(RI_ERR_INVALID, "ri_paged_shared_decode: group_size=%d unsupported", p->group_size);
+  if (groups < 1 || groups > p->batch) return ri_fail(RI_ERR_INVALID, "ri_paged_shared_decode: groups=%d unsupported", groups);
+  return ri_wave::own_bytes(*p) + (ri_wave::apart(*p) ? 0 : ri_shared::scratch_bytes(*p));
+}
+
+extern "C" int ri_paged_shared_decode(const ri_paged* p, const void* d_q, int64_t q_stride, const int32_t* d_group_start, int32_t groups,
+                                      const int32_t* d_shared, void* d_out, float* d_lse, float scale, void* d_scratch, void* stream) {
+  const int64_t bytes = ri_paged_shared_decode_scratch_bytes(p, groups);
+  if (bytes < 0) return (int)bytes;
+  RI_REQUIRE(d_shared && d_group_start, "ri_paged_shared_decode: null pointer");
+  RI_REQUIRE(p->d_weight == nullptr, "ri_paged_shared_decode: weights are not added up where slots are in common");
+  ri_wave::SharedArgs a = {};
+  int rc = ri_wave::prepare("ri_paged_shared_decode", p, d_q, q_stride, d_out, d_lse, scale, d_scratch, a);
+  if (rc != RI_OK) return rc;
+  if (ri_wave::apart(*p)) return ri_wave::launch(*p, static_cast<const ri_wave::PagedArgs&>(a), stream);
+  rc = ri_shared::launch("ri_paged_shared_decode", p, d_q, q_stride, d_group_start, groups, d_shared, scale,
+                         static_cast<char*>(d_scratch) + ri_wave::own_bytes(*p), &a.common, static_cast<cudaStream_t>(stream));
+  return rc != RI_OK ? rc : ri_wave::launch(*p, a, stream);
 }

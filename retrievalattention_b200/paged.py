@@ -136,8 +136,9 @@ def paged_prompt(q, key_pages, value_pages, page_table, lengths, row_start, *, w
 
 def paged_shared_decode(q, key_pages, value_pages, page_table, lengths, group_start, shared, *, out=None, lse=None, scale=None):
     """``paged_decode`` for requests that begin alike: requests ``group_start[g]`` to ``group_start[g + 1] - 1`` (int32 ``[groups + 1]``,
-    ascending) have their first ``shared[g]`` slots (int32 ``[groups]``) in common, which are read once for all of them, through the page
-    table of the first; each request's own slots are those behind.  Requests in no group have nothing in common with others."""
+    ascending) have their first ``shared[g]`` slots (int32 ``[groups]``) in common, that is their rows of the page table begin with the same
+    pages, which are read once for all of them; each request's own slots are those behind.  Requests in no group have nothing in common
+    with others.  Where the page table has room for few slots requests are attended one by one, as ``paged_decode`` does."""
     native = _native or _connect()
     return native.shared_decode(q, key_pages, value_pages, page_table, lengths, group_start, shared, out, lse,
                                 _SCALE if scale is None else scale)

@@ -21,7 +21,19 @@ def begin_alike(layer, groups):
                 x[b][:, :m] = x[first][:, :m]
 
 
+def roomy(table):
+    """The same table with room for more than a million slots a request: with few, requests are attended one by one."""
+    wide = torch.full((table.shape[0], 150000), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    return wide
+
+
 def run(layer, starts, shared, group, seed=0, lse=True, stride=0):
+    run_with(layer, layer.table, starts, shared, group, seed, lse, stride)
+    return run_with(layer, roomy(layer.table), starts, shared, group, seed, lse, stride)
+
+
+def run_with(layer, table, starts, shared, group, seed, lse, stride):
     from retrievalattention_b200 import paged
     from retrievalattention_b200.attn_hub.retroinfer_attn import check_prefill_errors
 
@@ -30,7 +42,7 @@ def run(layer, starts, shared, group, seed=0, lse=True, stride=0):
     q = torch.randn((batch, hq * DIM + stride), generator=gen).to(layer.dtype).cuda()[:, :hq * DIM].view(batch, 1, hq, DIM) if not stride else \
         torch.randn((batch, hq * DIM + stride), generator=gen).to(layer.dtype).cuda()[:, :hq * DIM].unflatten(1, (1, hq, DIM))
     sums = torch.full((batch, hq), 7.0, device="cuda") if lse else None
-    out = paged.paged_shared_decode(q, layer.keys, layer.values, layer.table, layer.lengths, torch.tensor(starts, dtype=torch.int32, device="cuda"),
+    out = paged.paged_shared_decode(q, layer.keys, layer.values, table, layer.lengths, torch.tensor(starts, dtype=torch.int32, device="cuda"),
                                     torch.tensor(shared, dtype=torch.int32, device="cuda"), lse=sums)
     check_prefill_errors()
     for b, n in enumerate(layer.lengths_list):
@@ -104,7 +116,7 @@ def test_infinite_and_nan_slots():
     from retrievalattention_b200 import paged
 
     q = torch.randn(3, 1, 4, DIM, device="cuda").to(torch.bfloat16)
-    out = paged.paged_shared_decode(q, layer.keys, layer.values, layer.table, layer.lengths, torch.tensor([0, 3], dtype=torch.int32, device="cuda"),
+    out = paged.paged_shared_decode(q, layer.keys, layer.values, roomy(layer.table), layer.lengths, torch.tensor([0, 3], dtype=torch.int32, device="cuda"),
                                     torch.tensor([256], dtype=torch.int32, device="cuda"))[:, 0]
     bad = ~torch.isfinite(out)
     want = torch.zeros_like(bad)
@@ -121,7 +133,8 @@ def test_a_captured_call_follows_lengths():
     q = torch.randn(3, 1, 8, DIM, device="cuda").to(torch.bfloat16)
     starts, shared = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 3], [768]))
     out, lse, lengths = torch.empty_like(q), torch.empty(3, 8, device="cuda"), layer.lengths.clone()
-    call = lambda: paged.paged_shared_decode(q, layer.keys, layer.values, layer.table, lengths, starts, shared, out=out, lse=lse)  # noqa: E731
+    table = roomy(layer.table)
+    call = lambda: paged.paged_shared_decode(q, layer.keys, layer.values, table, lengths, starts, shared, out=out, lse=lse)  # noqa: E731
     call()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
