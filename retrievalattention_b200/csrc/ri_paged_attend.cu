@@ -33,7 +33,6 @@ namespace {
 using namespace ri_tc;
 using namespace ri_page;
 using ri_shared::clamped;
-using ri_shared::group_of;
 
 constexpr int kTile = 128;                 // query rows of a tile, slots of a step
 constexpr int kHalf = kTile * 128;         // bytes of a 128-row x 64-channel half-tile
@@ -49,6 +48,9 @@ constexpr int kMaxEntries = 8192;          // of the table of steps
 // for its partial result and the second kernel.  Items of at most twice as many are never cut.
 constexpr int kSnap = 4;
 constexpr int kItemCost = 2;               // what an item costs beside its steps (7000 clocks; a step 3400)
+// Of a CTA, over what groups have in common: more parts of an item than that are slower to join than they are to make (one KV head of 8,
+// 32768 slots: 148 parts 52 us, 65 parts 35; 2 x 6016 slots of 4 heads 51 and 48).
+constexpr int kLeastCost = 4;
 constexpr int kHeadsMost = 8;              // query heads of a KV head
 constexpr int kMeta = 8;                   // ints that a CTA leaves for the kernel that joins
 
@@ -97,7 +99,6 @@ struct Args : Pages {
   float* part_o;             // rows of 128, a segment's in the order [channels / 8][rows][8]
   float2* part_ml;           // (reference in the log2 domain, sum)
   int* meta;                 // prompt: [CTAs][kMeta]; SHARED: CTAs (first, last) of the items
-  int32_t* from;             // SHARED: what every request has in common with its group
   int n_seq, n_rows;         // sequences: requests, or groups; rows of q
   int gs, tile_tokens, max_ctas, part_rows;      // tokens of a tile; rows of a CTA's part of the partial results
   int window, sink;          // window 0: none
@@ -114,11 +115,6 @@ struct Item {
   int n_tok, front, skip, low, high, sink, steps;
   __device__ __forceinline__ int cost() const { return steps + kItemCost; }
 };
-// What requests of group g have in common: as far as the first one's slots go.
-__device__ __forceinline__ int in_common(const Args& a, int g) {
-  const int b = clamped(a.starts[g], a.batch);
-  return b < a.batch ? clamped(a.shared[g], rows_of(a, b)) : 0;
-}
 template <bool SHARED>
 __device__ __forceinline__ Seq seq_of(const Args& a, int v) {
   Seq s = {0, 0, v, 0};
@@ -129,7 +125,7 @@ __device__ __forceinline__ Seq seq_of(const Args& a, int v) {
   } else {
     s.q_row = clamped(a.starts[v], a.batch);
     s.table_row = min(s.q_row, a.batch - 1);
-    s.rows = in_common(a, v);
+    s.rows = ri_shared::in_common(a, a.starts, a.shared, v);
     s.n = s.rows > 0 ? max(0, clamped(a.starts[v + 1], a.batch) - s.q_row) : 0;
   }
   return s;
@@ -189,7 +185,6 @@ __device__ __forceinline__ int last_at_most(const int* table, int n, int x) {
 }
 // Tables of the pairs in front of every sequence and of the steps in front of every 2^k pairs (of one KV head) are made by all
 // threads together; then one looks up where the CTA's range begins, another where it ends.
-template <bool SHARED>
 __device__ __forceinline__ void plan(const Args& a, int* table, Control& s) {
   const int tid = threadIdx.x;
   int* pairs = table;
@@ -199,7 +194,7 @@ __device__ __forceinline__ void plan(const Args& a, int* table, Control& s) {
     const int each = (a.n_seq + kThreads - 1) / kThreads, v0 = min(tid * each, a.n_seq), v1 = min(v0 + each, a.n_seq);
     int sum = 0, first = a.n_seq;
     for (int v = v0; v < v1; ++v) {
-      const int n = pairs_of(a, seq_of<SHARED>(a, v));
+      const int n = pairs_of(a, seq_of<false>(a, v));
       pairs[v] = sum;
       if (n > 0) first = min(first, v);
       sum += n;
@@ -219,16 +214,16 @@ __device__ __forceinline__ void plan(const Args& a, int* table, Control& s) {
     int sum = 0;
     if (e0 < e1) {
       int at = e0 << k, v = last_at_most(pairs, a.n_seq, at);
-      Seq seq = seq_of<SHARED>(a, v);
+      Seq seq = seq_of<false>(a, v);
       for (int e = e0; e < e1; ++e) {
         steps[e] = sum;
         for (const int end = min((e + 1) << k, n_pairs); at < end; ++at) {
           if (at >= pairs[v + 1]) {
             do ++v;
             while (at >= pairs[v + 1]);
-            seq = seq_of<SHARED>(a, v);
+            seq = seq_of<false>(a, v);
           }
-          sum += item_of<SHARED>(a, seq, at - pairs[v]).cost();
+          sum += item_of<false>(a, seq, at - pairs[v]).cost();
         }
       }
     }
@@ -247,14 +242,14 @@ __device__ __forceinline__ void plan(const Args& a, int* table, Control& s) {
       const int y = (int)(x - (int64_t)head * total), e = last_at_most(steps, entries, y);
       int at = e << k, before = steps[e];
       v = last_at_most(pairs, a.n_seq, at);
-      Seq seq = seq_of<SHARED>(a, v);
+      Seq seq = seq_of<false>(a, v);
       for (;;) {
         p = at - pairs[v];
-        const Item it = item_of<SHARED>(a, seq, p);
+        const Item it = item_of<false>(a, seq, p);
         const int n = it.steps;
         if (y - before < it.cost()) {
           step = max(0, y - before - kItemCost);
-          if (!SHARED && step > 0) {
+          if (step > 0) {
             if (step <= kSnap) {
               step = 0;
               break;
@@ -277,7 +272,7 @@ __device__ __forceinline__ void plan(const Args& a, int* table, Control& s) {
         if (at >= pairs[v + 1]) {
           do ++v;
           while (at >= pairs[v + 1]);
-          seq = seq_of<SHARED>(a, v);
+          seq = seq_of<false>(a, v);
         }
       }
     }
@@ -441,14 +436,9 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   const uint32_t tmem = s.tmem;
   volatile int* abort_flag = &s.abort;
   ri_pdl_wait();
-  ri_pdl_trigger();                        // the kernel that joins waits for the end of this one
+  ri_pdl_trigger();                        // the kernels behind wait for the end of this one where they read what it writes
   const bool aligned = s.abort == 0;       // of the whole CTA
-  if (SHARED)
-    for (int b = c * kThreads + (int)threadIdx.x; b < a.batch; b += (int)gridDim.x * kThreads) {
-      const int g = group_of(a.starts, a.n_seq, b);
-      a.from[b] = g >= 0 ? min(in_common(a, g), rows_of(a, b)) : 0;
-    }
-  if (aligned) plan<SHARED>(a, reinterpret_cast<int*>(smem + 4 * kHalf), s);
+  if (!SHARED && aligned) plan(a, reinterpret_cast<int*>(smem + 4 * kHalf), s);
 
   // every role goes through the segments one by one, whole warps
   auto take = [&](int i) {
@@ -678,19 +668,80 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       }
     } else if (warp == 2) {
       // ---------------- segments ----------------
-      if (lane == 0) {
+      int given = 0;
+      Segment sg = {};
+      auto give = [&] {                      // by one lane
+        const int at = given % kSegments;
+        if (!mbar_wait(bar_seg_empty(at), ((given / kSegments) & 1) ^ 1, abort_flag, 19)) return false;
+        s.segments[at] = sg;
+        mbar_arrive(bar_seg(at));
+        ++given;
+        return true;
+      };
+      // steps `step` to `end` - 1 of an item
+      auto describe = [&](const Seq& seq, const Item& it, int h, int p, int step, int end) {
+        sg.table_row = seq.table_row;
+        sg.head = h;
+        sg.q_row = seq.q_row + p * 2 * a.tile_tokens;
+        sg.n_tok = it.n_tok;
+        sg.step = step;
+        sg.n = end - step;
+        sg.front = it.front;
+        sg.skip = it.skip;
+        sg.low = it.low;
+        sg.high = it.high;
+        sg.sink = it.sink;
+        sg.end = seq.rows - it.skip;
+        sg.slot0 = seq.rows - seq.n + p * 2 * a.tile_tokens;
+        sg.two = it.n_tok > a.tile_tokens;
+      };
+      if (SHARED) {
+        // All items of a group have the same steps, so the range is found without tables, by the warp: what code runs once costs by
+        // the instruction (6016 slots, 24 requests: the kernel 21 us with tables).
+        auto cost_of = [&](int g) {
+          if (g >= a.n_seq) return 0;
+          const Seq seq = seq_of<true>(a, g);
+          return pairs_of(a, seq) * ((seq.rows + kTile - 1) / kTile + kItemCost);
+        };
+        int total = 0;
+        for (int g = lane; g < a.n_seq; g += 32) total += cost_of(g);
+        total = __reduce_add_sync(0xffffffffu, total);
+        const int64_t all = (int64_t)total * a.hk;
+        const int n_ctas = (int)min((int64_t)a.max_ctas, (all + kLeastCost - 1) / kLeastCost);
+        const int64_t lo = c < n_ctas ? all * c / n_ctas : all, hi = c < n_ctas ? all * (c + 1) / n_ctas : all;
+        if (lo < hi && lane == 0) {
+          int h = (int)(lo / total), g = 0;
+          int64_t at = (int64_t)h * total;   // the item's place in the sequence
+          bool ok = true;
+          while (ok && at < hi) {
+            const Seq seq = seq_of<true>(a, g);
+            const int pairs = pairs_of(a, seq), steps = (seq.rows + kTile - 1) / kTile, cost = steps + kItemCost;
+            int p = at < lo ? (int)min((int64_t)pairs, (lo - at) / cost) : 0;
+            at += (int64_t)p * cost;
+            for (; ok && p < pairs && at < hi; ++p, at += cost) {
+              const int step = (int)max((int64_t)0, lo - at - kItemCost), end = (int)min((int64_t)steps, max((int64_t)0, hi - at - kItemCost));
+              if (step >= end) continue;
+              describe(seq, item_of<true>(a, seq, p), h, p, step, end);
+              const int item = h * a.batch + sg.q_row;
+              sg.part = c * a.part_rows + item * a.gs;
+              if (step == 0) a.meta[2 * item] = c;
+              if (end == steps) a.meta[2 * item + 1] = c;
+              ok = give();
+            }
+            if (++g == a.n_seq) {
+              g = 0;
+              ++h;
+            }
+          }
+          sg.n = 0;
+          if (ok) give();
+        } else if (lane == 0) {
+          give();
+        }
+      } else if (lane == 0) {
         int h = s.begin[0], v = s.begin[1], p = s.begin[2], step = s.begin[3];
         const int h1 = s.end[0], v1 = s.end[1], p1 = s.end[2], step1 = s.end[3], first = s.first;
-        int given = 0, tail = 0, head = 0;                      // prompt: rows of a segment that others go on with; 1 and 2: see below
-        Segment sg = {};
-        auto give = [&] {
-          const int at = given % kSegments;
-          if (!mbar_wait(bar_seg_empty(at), ((given / kSegments) & 1) ^ 1, abort_flag, 19)) return false;
-          s.segments[at] = sg;
-          mbar_arrive(bar_seg(at));
-          ++given;
-          return true;
-        };
+        int tail = 0, head = 0;              // rows of a segment that others go on with; whether the first one is another CTA's item
         Seq seq = {};
         int pairs = 0, of = -1;
         bool ok = true;
@@ -698,40 +749,20 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           const bool last = h == h1 && v == v1 && p == p1;
           if (last && step == step1) break;
           if (of != v) {
-            seq = seq_of<SHARED>(a, v);
+            seq = seq_of<false>(a, v);
             pairs = pairs_of(a, seq);
             of = v;
           }
-          const Item it = item_of<SHARED>(a, seq, p);
+          const Item it = item_of<false>(a, seq, p);
           const int end = last ? step1 : it.steps;
-          sg.table_row = seq.table_row;
-          sg.head = h;
-          sg.q_row = seq.q_row + p * 2 * a.tile_tokens;
-          sg.n_tok = it.n_tok;
-          sg.step = step;
-          sg.n = end - step;
-          sg.front = it.front;
-          sg.skip = it.skip;
-          sg.low = it.low;
-          sg.high = it.high;
-          sg.sink = it.sink;
-          sg.end = seq.rows - it.skip;
-          sg.slot0 = seq.rows - seq.n + p * 2 * a.tile_tokens;
-          sg.two = it.n_tok > a.tile_tokens;
           const bool begins = step == 0, ends = end == it.steps;
-          if (SHARED) {
-            const int at = h * a.batch + sg.q_row;
-            sg.part = c * a.part_rows + at * a.gs;
-            if (begins) a.meta[2 * at] = c;
-            if (ends) a.meta[2 * at + 1] = c;
-          } else {
-            sg.part = begins && ends ? -1 : (2 * c + begins) * a.part_rows;
-            if (!begins) head = ends ? 1 : 2;                   // another CTA's item: it ends here, or goes on behind
-            if (begins && !ends) {
-              tail = sg.n_tok;
-              a.meta[c * kMeta + 2] = h;
-              a.meta[c * kMeta + 3] = sg.q_row;
-            }
+          describe(seq, it, h, p, step, end);
+          sg.part = begins && ends ? -1 : (2 * c + begins) * a.part_rows;
+          if (!begins) head = ends ? 1 : 2;  // it ends here, or goes on behind
+          if (begins && !ends) {
+            tail = sg.n_tok;
+            a.meta[c * kMeta + 2] = h;
+            a.meta[c * kMeta + 3] = sg.q_row;
           }
           ok = give();
           step = 0;
@@ -739,14 +770,14 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           if (++p == pairs) {
             p = 0;
             do ++v;
-            while (v < a.n_seq && !(v == v1 && h == h1) && pairs_of(a, seq_of<SHARED>(a, v)) == 0);
+            while (v < a.n_seq && !(v == v1 && h == h1) && pairs_of(a, seq_of<false>(a, v)) == 0);
             if (v == a.n_seq) {
               v = first;
               ++h;
             }
           }
         }
-        if (!SHARED && a.meta != nullptr) {
+        if (a.meta != nullptr) {
           a.meta[c * kMeta] = tail;
           a.meta[c * kMeta + 1] = head;
         }
@@ -1132,7 +1163,7 @@ int attend(const char* what, const ri_paged* p, const void* d_q, int64_t q_strid
 // Workspaces: meta, sums, outputs of the parts.
 int64_t prompt_part_rows(const ri_paged& p, int rows) { return 2 * kMaxCtas * most_items_rows(p, rows); }
 constexpr int64_t kPromptMeta = (int64_t)kMaxCtas * kMeta * 4;
-int64_t shared_meta(const ri_paged& p) { return ri_align_up(8 * (int64_t)p.batch * p.kv_heads + 4 * (int64_t)p.batch, 16); }
+int64_t shared_meta(const ri_paged& p) { return ri_align_up(8 * (int64_t)p.batch * p.kv_heads, 16); }
 int64_t shared_rows(const ri_paged& p) { return (int64_t)kMaxCtas * most_items_rows(p, p.batch) + (int64_t)p.batch * p.kv_heads * p.group_size; }
 void place(Args& a, void* d_scratch, int64_t meta, int64_t rows) {
   a.meta = static_cast<int*>(d_scratch);
@@ -1174,11 +1205,10 @@ int ri_shared::launch(const char* what, const ri_paged* p, const void* d_q, int6
   a.shared = d_shared;
   a.n_seq = groups;
   place(a, d_scratch, shared_meta(*p), shared_rows(*p));
-  a.from = a.meta + 2 * (int64_t)p->batch * p->kv_heads;
   int sms = 0;
   const int rc2 = ri_sm_count(&sms);
   if (rc2 != RI_OK) return rc2;
-  *parts = {d_group_start, a.from, a.meta, a.part_o, a.part_ml, groups, 2 * (kTile / p->group_size), (int)most_items_rows(*p, p->batch),
+  *parts = {d_group_start, d_shared, a.meta, a.part_o, a.part_ml, groups, 2 * (kTile / p->group_size), (int)most_items_rows(*p, p->batch),
             sms < kMaxCtas ? sms : kMaxCtas};
   return attend<true>(what, p, d_q, q_stride, p->batch, a, nullptr, nullptr, scale, false, s);
 }

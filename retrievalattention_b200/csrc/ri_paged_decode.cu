@@ -108,11 +108,11 @@ struct SharedArgs : PagedArgs {
   ri_shared::Parts common;
 };
 __device__ __forceinline__ WindowSpan span_of(const SharedArgs& a, int b) {
-  const int low = a.common.from[b];
+  const int low = ri_shared::common_of(a, a.common, b);
   return {0, low & ~15, low, 0};
 }
 __device__ __forceinline__ int rows_of(const SharedArgs& a, int b) {
-  const int n = ri_page::rows_of(static_cast<const Pages&>(a), b), low = a.common.from[b];
+  const int n = ri_page::rows_of(static_cast<const Pages&>(a), b), low = ri_shared::common_of(a, a.common, b);
   return n > low ? n - (low & ~15) : 0;
 }
 
@@ -154,7 +154,10 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
   volatile int* abort_flag = &s_abort;
   // The next kernel may start when the kernel in front of this one has ended, not before: it finds lengths and page tables as
   // they are without waiting for this one.
-  ri_pdl_wait();
+  // SharedArgs: the kernel in front is the one over what requests have in common, which has waited for those before it, and nothing
+  // of its results is read here: this one streams rows on the SMs that the other is done with, and waits at its end.
+  constexpr bool kBeside = std::is_same_v<Args, SharedArgs>;
+  if (!kBeside) ri_pdl_wait();
   ri_pdl_trigger();
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
@@ -168,6 +171,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
     if (n == 0) {                                        // the whole cluster leaves
       for (int i = tid + rank * kPagedThreads; i < gs * RI_HEAD_DIM; i += ctas * kPagedThreads) a.out[(int64_t)g * gs * RI_HEAD_DIM + i] = 0;
       if (rank == 0 && tid < gs && a.lse != nullptr) a.lse[g * gs + tid] = -INFINITY;
+      ri_pdl_wait();
       return;
     }
     c_first = {g, 0, rows};
@@ -176,7 +180,10 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
     score_step = (int64_t)g * steps_of(a.width << a.shift);
   } else {
     const int total = count_steps(a), n_ctas = used_ctas(total, a.max_ctas);
-    if (c >= n_ctas || total == 0) return;
+    if (c >= n_ctas || total == 0) {
+      ri_pdl_wait();
+      return;
+    }
     c_lo = cta_start(c, total, n_ctas);
     c_hi = cta_start(c + 1, total, n_ctas);
     c_first = find_place(a, c_lo);
@@ -394,6 +401,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
       store_partial(at.g);
     }
   }
+  ri_pdl_wait();
   if (!merged) return;
 
   reduce_sum();
@@ -474,20 +482,13 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_decode_kernel(const __
   cluster.sync();                                        // nobody's shared memory goes while others may read it
 }
 
-// What is left once every partial result is there, a group per blockIdx.y: its blocks join the partial results, a query head at
-// a time, and with weights turn the group's scores into probabilities, kFoldSlots slots at a time, a thread per slot.  Every
-// block works out lse of all heads (warp h of head h), so none waits for another.  Which partial results the group has
-// follows from the lengths, so a warp lists them, in the order of the sequence, before the wait for the kernel that makes them.
-constexpr int kFoldEach = 2, kFoldSlots = kFoldEach * kFinishThreads;
-constexpr int kFinishBlocks = 4;                         // of an SM
-constexpr int kTogether = 4;                             // partial results of a warp on their way
-template <int DT, class Args>
-__global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_kernel(const __grid_constant__ Args a) {
-  extern __shared__ int s_slot[];                        // [most partial results of a group]
-  __shared__ float s_m[kMaxHeads], s_l[kMaxHeads], s_o[kFinishThreads / 32][RI_HEAD_DIM];
-  __shared__ int s_n;
-  ri_pdl_trigger();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.y, gs = a.gs, b = g / a.hk, h_kv = g - b * a.hk;
+// A group's rows, the first of its steps in the sequence, and (warp 0) how many partial results it has, which `slots` takes.
+struct Own {
+  int rows, lo, count;
+};
+template <class Args>
+__device__ __forceinline__ Own list_own(const Args& a, int b, int h_kv, int g, int* slots) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int before = 0, all = 0, rows = 0;                     // steps in front of the request (of one KV head), of all; its rows
   for (int i = lane; i < a.batch; i += 32) {
     const int r = rows_of(a, i), steps = steps_of(r);
@@ -522,10 +523,30 @@ __global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_ke
         }
       }
       const unsigned votes = __ballot_sync(0xffffffffu, mine);
-      if (mine) s_slot[count + __popc(votes & ((1u << lane) - 1))] = c * kPagedWarps + w + g;
+      if (mine) slots[count + __popc(votes & ((1u << lane) - 1))] = c * kPagedWarps + w + g;
       count += __popc(votes);
     }
   }
+  return {rows, lo, count};
+}
+
+// What is left once every partial result is there, a group per blockIdx.y: its blocks join the partial results, a query head at
+// a time, and with weights turn the group's scores into probabilities, kFoldSlots slots at a time, a thread per slot.  Every
+// block works out lse of all heads (warp h of head h), so none waits for another.  Which partial results the group has
+// follows from the lengths, so a warp lists them, in the order of the sequence, before the wait for the kernel that makes them.
+constexpr int kFoldEach = 2, kFoldSlots = kFoldEach * kFinishThreads;
+constexpr int kFinishBlocks = 4;                         // of an SM
+constexpr int kTogether = 4;                             // partial results of a warp on their way
+template <int DT, class Args>
+__global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_kernel(const __grid_constant__ Args a) {
+  extern __shared__ int s_slot[];                        // [most partial results of a group]
+  __shared__ float s_m[kMaxHeads], s_l[kMaxHeads], s_o[kFinishThreads / 32][RI_HEAD_DIM];
+  __shared__ int s_n;
+  ri_pdl_trigger();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.y, gs = a.gs, b = g / a.hk, h_kv = g - b * a.hk;
+  const Own own = list_own(a, b, h_kv, g, s_slot);
+  const int rows = own.rows, n = steps_of(rows), lo = own.lo;
+  int count = own.count;
   // a tile of slots: pages (their tables do not change either), then scores and weights
   int id[kFoldEach] = {};
   float sc[kFoldEach][kMaxHeads], old[kFoldEach];
@@ -553,37 +574,7 @@ __global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_ke
   if (folds) find_pages(blockIdx.x);
   if (tid == 0) s_n = count;
   ri_pdl_wait();
-  // SharedArgs: parts of the item over what the request has in common with others, behind the group's own
-  constexpr bool kShared = std::is_same_v<Args, SharedArgs>;
-  int extra = 0, item_rows = 0, item_row = 0;
-  int64_t item_part = 0;
-  if constexpr (kShared) {
-    if (a.common.from[b] > 0) {
-      const int of = ri_shared::group_of(a.common.starts, a.common.groups, b);
-      const int b0 = ri_shared::clamped(a.common.starts[of], a.batch), b1 = ri_shared::clamped(a.common.starts[of + 1], a.batch);
-      const int first = b0 + (b - b0) / a.common.pair * a.common.pair, item = h_kv * a.batch + first;
-      const int c0 = ri_shared::clamped(a.common.ctas[2 * item], a.common.max_ctas - 1);
-      extra = ri_shared::clamped(a.common.ctas[2 * item + 1], a.common.max_ctas - 1) - c0 + 1;
-      item_rows = min(a.common.pair, b1 - first) * gs;
-      item_row = (b - first) * gs;
-      item_part = (int64_t)c0 * a.common.part_rows + (int64_t)item * gs;
-    }
-  }
-  auto ml_of = [&](int i, int head) {
-    if constexpr (kShared) {
-      if (i >= s_n) return a.common.ml[item_part + (int64_t)(i - s_n) * a.common.part_rows + item_row + head];
-    }
-    return a.part_ml[(int64_t)s_slot[i] * gs + head];
-  };
-  auto four_of = [&](int i, int head) {
-    if constexpr (kShared) {
-      if (i >= s_n)
-        return reinterpret_cast<const float4*>(a.common.o + (item_part + (int64_t)(i - s_n) * a.common.part_rows) * RI_HEAD_DIM)
-            [((lane >> 1) * item_rows + item_row + head) * 2 + (lane & 1)];
-    }
-    return reinterpret_cast<const float4*>(a.part_o + ((int64_t)s_slot[i] * gs + head) * RI_HEAD_DIM)[lane];
-  };
-  if (n == 0 && extra <= 0) {
+  if (n == 0) {
     for (int h = blockIdx.x; h < gs; h += gridDim.x) {
       if (tid < RI_HEAD_DIM) a.out[((int64_t)g * gs + h) * RI_HEAD_DIM + tid] = 0;
       if (tid == 0 && a.lse != nullptr) a.lse[g * gs + h] = -INFINITY;
@@ -592,7 +583,7 @@ __global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_ke
   }
   if (folds) fetch(blockIdx.x);
   __syncthreads();
-  count = s_n + max(extra, 0);
+  count = s_n;
   if (warp < gs) {
     float M = -INFINITY, L = 0.f;
     for (int i0 = 0; i0 < count; i0 += 32 * kTogether) {
@@ -600,7 +591,7 @@ __global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_ke
 #pragma unroll
       for (int u = 0; u < kTogether; ++u) {
         const int i = i0 + u * 32 + lane;
-        ml[u] = i < count ? ml_of(i, warp) : make_float2(-INFINITY, 0.f);
+        ml[u] = i < count ? a.part_ml[(int64_t)s_slot[i] * gs + warp] : make_float2(-INFINITY, 0.f);
       }
       float most = M;
 #pragma unroll
@@ -635,8 +626,9 @@ __global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_ke
         const int i = i0 + u * (kFinishThreads / 32);
         m[u] = -INFINITY;
         if (i < count) {
-          m[u] = ml_of(i, head).x;
-          x[u] = four_of(i, head);
+          const int64_t at = (int64_t)s_slot[i] * gs + head;
+          m[u] = a.part_ml[at].x;
+          x[u] = reinterpret_cast<const float4*>(a.part_o + at * RI_HEAD_DIM)[lane];
         }
       }
       float most = M;
@@ -684,6 +676,78 @@ __global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_ke
       *weight_at(tile, e) = old[e] + sum;
     }
   }
+}
+
+// The same where requests have slots in common: a block per group joins the partial results over those and over the request's own, a
+// thread for each query head and four channels.  (As a part of the kernel above, a block for each query head: 64 requests of 8 heads
+// of 4, 14 us.)
+template <int DT>
+__global__ void __launch_bounds__(kFinishThreads, 3) shared_finish_kernel(const __grid_constant__ SharedArgs a) {
+  extern __shared__ int s_slot[];
+  __shared__ int s_n;
+  ri_pdl_trigger();
+  const int gs = a.gs, g = blockIdx.x, b = g / a.hk, h_kv = g - b * a.hk, quad = threadIdx.x / gs, r = threadIdx.x - quad * gs;
+  const Own own = list_own(a, b, h_kv, g, s_slot);
+  if (threadIdx.x == 0) s_n = own.count;
+  ri_pdl_wait();
+  const ri_shared::Parts& x = a.common;
+  int extra = 0, item_rows = 0, item_row = 0;
+  int64_t part = 0;
+  if (ri_shared::common_of(a, x, b) > 0) {
+    const int of = ri_shared::group_of(x.starts, x.groups, b);
+    const int b0 = ri_shared::clamped(x.starts[of], a.batch), b1 = ri_shared::clamped(x.starts[of + 1], a.batch);
+    const int first = b0 + (b - b0) / x.pair * x.pair, item = h_kv * a.batch + first;
+    const int c0 = ri_shared::clamped(x.ctas[2 * item], x.max_ctas - 1);
+    extra = max(0, ri_shared::clamped(x.ctas[2 * item + 1], x.max_ctas - 1) - c0 + 1);
+    item_rows = min(x.pair, b1 - first) * gs;
+    item_row = (b - first) * gs + r;
+    part = (int64_t)c0 * x.part_rows + (int64_t)item * gs;
+  }
+  __syncthreads();
+  const int count = s_n;
+  if (quad >= RI_HEAD_DIM / 4) return;
+  auto ml_of = [&](int i) {
+    return i < extra ? x.ml[part + (int64_t)i * x.part_rows + item_row] : a.part_ml[(int64_t)s_slot[i - extra] * gs + r];
+  };
+  auto four_of = [&](int i) {
+    return i < extra ? reinterpret_cast<const float4*>(x.o + (part + (int64_t)i * x.part_rows) * RI_HEAD_DIM)[((quad >> 1) * item_rows + item_row) * 2 + (quad & 1)]
+                     : reinterpret_cast<const float4*>(a.part_o + ((int64_t)s_slot[i - extra] * gs + r) * RI_HEAD_DIM)[quad];
+  };
+  constexpr int kWide = 8;                                 // partial results on their way
+  float M = -INFINITY, L = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < extra + count; i0 += kWide) {
+    float2 ml[kWide];
+    float4 v[kWide];
+#pragma unroll
+    for (int u = 0; u < kWide; ++u) {
+      const int i = i0 + u;
+      ml[u] = make_float2(-INFINITY, 0.f);
+      v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < extra + count) {
+        ml[u] = ml_of(i);
+        v[u] = four_of(i);
+      }
+    }
+    float most = M;
+#pragma unroll
+    for (int u = 0; u < kWide; ++u) most = fmaxf(most, ml[u].x);
+    const float ref = most == -INFINITY ? 0.f : most, old = exp2f(M - ref);
+    L *= old;
+    o.x *= old; o.y *= old; o.z *= old; o.w *= old;
+#pragma unroll
+    for (int u = 0; u < kWide; ++u) {
+      // a part far below the largest still counts enough to hand on an infinite value
+      const float f = ml[u].x == -INFINITY ? 0.f : fmaxf(exp2f(ml[u].x - ref), 1.17549435e-38f);
+      L += ml[u].y * f;
+      o.x += v[u].x * f; o.y += v[u].y * f; o.z += v[u].z * f; o.w += v[u].w * f;
+    }
+    M = most;
+  }
+  const float f = L == 0.f ? 0.f : 1.f / L;
+  *reinterpret_cast<uint2*>(a.out + ((int64_t)g * gs + r) * RI_HEAD_DIM + quad * 4) =
+      make_uint2(Elem<DT>::pack2(o.x * f, o.y * f), Elem<DT>::pack2(o.z * f, o.w * f));
+  if (quad == 0 && a.lse != nullptr) a.lse[g * gs + r] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
 }
 
 int64_t paged_slots(const ri_paged& p) { return (int64_t)kPagedMaxCtas * kPagedWarps + (int64_t)p.batch * p.kv_heads; }
@@ -793,15 +857,18 @@ int launch_paged(const Args& a, const CUtensorMap& map_k, const CUtensorMap& map
   if (!std::is_same_v<Args, SharedArgs> && (rc = cluster_size(a, most, &ctas)) != RI_OK) return rc;
   rc = box == 8 ? launch_steps<DT, 8>(a, map_k, map_v, ctas, s) : launch_steps<DT, 16>(a, map_k, map_v, ctas, s);
   if (rc != RI_OK || ctas > 0) return rc;
-  const int64_t groups = (int64_t)a.batch * a.hk;
-  // blocks of a group: for its heads, or with weights its tiles of slots, as many as the chip holds at once
-  const int64_t tiles = a.weight ? (most + kFoldSlots - 1) / kFoldSlots : 0, room = kFinishBlocks * (int64_t)a.max_ctas / groups;
-  int64_t blocks = tiles > a.gs ? tiles : a.gs;
-  if (blocks > room) blocks = room > 1 ? room : 1;
   // partial results of a group: its steps, or all that there are and one more
-  const int64_t steps = (most + 15) / 16, parts = (int64_t)a.max_ctas * kPagedWarps;
+  const int64_t groups = (int64_t)a.batch * a.hk, steps = (most + 15) / 16, parts = (int64_t)a.max_ctas * kPagedWarps;
   const size_t smem = (size_t)(steps < parts ? steps : parts) * 4 + 4;
-  RI_CUDA_OK(ri_launch_pdl_id(11, paged_finish_kernel<DT, Args>, dim3((unsigned)blocks, (unsigned)groups), dim3(kFinishThreads), smem, s, a));
+  if constexpr (std::is_same_v<Args, SharedArgs>) {
+    RI_CUDA_OK(ri_launch_pdl_id(11, shared_finish_kernel<DT>, dim3((unsigned)groups), dim3(kFinishThreads), smem, s, a));
+  } else {
+    // blocks of a group: for its heads, or with weights its tiles of slots, as many as the chip holds at once
+    const int64_t tiles = a.weight ? (most + kFoldSlots - 1) / kFoldSlots : 0, room = kFinishBlocks * (int64_t)a.max_ctas / groups;
+    int64_t blocks = tiles > a.gs ? tiles : a.gs;
+    if (blocks > room) blocks = room > 1 ? room : 1;
+    RI_CUDA_OK(ri_launch_pdl_id(11, paged_finish_kernel<DT, Args>, dim3((unsigned)blocks, (unsigned)groups), dim3(kFinishThreads), smem, s, a));
+  }
   return RI_OK;
 }
 
@@ -859,8 +926,10 @@ int launch(const ri_paged& p, const Args& a, void* stream) {
 }
 
 // Requests that begin alike are attended together where all slots there may be are more than this many bytes of K and V.  It takes a
-// kernel more, and requests that are attended one by one find much of what others have read in L2.
-constexpr int64_t kAlikeBytes = 48 << 20;
+// kernel more, and requests that are attended one by one find much of what others have read in L2: 8 heads of 4, 8 requests of 4096
+// slots in common and up to 500 of their own (151 MB) 28 us together and 26 one by one, 16 requests (302 MB) 32 and 45, 8 requests over
+// 16384 slots (554 MB) 41 and 80, 64 over 32768 (9.1 GB) 124 and 1135.
+constexpr int64_t kAlikeBytes = 160 << 20;
 bool apart(const ri_paged& p) { return (int64_t)p.batch * p.kv_heads * ri_page::slots_of(p) * 4 * RI_HEAD_DIM <= kAlikeBytes; }
 int64_t own_bytes(const ri_paged& p) { return ri_align_up(paged_slots(p) * p.group_size * (RI_HEAD_DIM + 2) * 4, 16); }
 

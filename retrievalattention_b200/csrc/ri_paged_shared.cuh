@@ -11,7 +11,7 @@ namespace ri_shared {
 // behind c * part_rows + i * gs rows of 128 floats, in the order [channels / 8][rows][8].
 struct Parts {
   const int32_t* starts;       // [groups + 1] requests
-  int32_t* from;               // [batch]: slots that request b has in common with its group
+  const int32_t* shared;       // [groups] slots
   int* ctas;
   float* o;
   float2* ml;                  // (reference in the log2 domain, sum)
@@ -27,6 +27,18 @@ __device__ __forceinline__ int group_of(const int32_t* starts, int groups, int b
     (starts[mid] <= b ? lo : hi) = mid;
   }
   return starts[lo] <= b && b < starts[lo + 1] ? lo : -1;
+}
+
+// What requests of group g have in common: as far as the first one's slots go.
+template <class Args>
+__device__ __forceinline__ int in_common(const Args& a, const int32_t* starts, const int32_t* shared, int g) {
+  const int b = clamped(starts[g], a.batch);
+  return b < a.batch ? clamped(shared[g], ri_page::rows_of(a, b)) : 0;
+}
+// Slots that request b has in common with its group.
+__device__ __forceinline__ int common_of(const ri_page::Pages& a, const Parts& x, int b) {
+  const int g = group_of(x.starts, x.groups, b);
+  return g >= 0 ? min(in_common(a, x.starts, x.shared, g), ri_page::rows_of(a, b)) : 0;
 }
 
 int64_t scratch_bytes(const ri_paged& p);
