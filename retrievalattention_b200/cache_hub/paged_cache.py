@@ -14,6 +14,10 @@ and of a prompt: ``begin`` with every request's tokens, ``append`` with ``keys``
 ``observe`` with the last queries and ``evict(slack=0)``.  A prompt that takes a released place beside running requests names itself:
 ``begin([0, 57, 0])``, ``append`` with its rows, ``observe(queries, layer, requests=[1])``; so do decode steps of some requests.
 Lengths and pages are known on the host without asking the GPU, so nothing synchronises.
+
+Layers may look back over a window (``attn_window``, ``attn_sink``): ``attend`` and ``prompt`` go by it.  ``prompt`` is the attention of
+the step's rows over the pages, for prompts that follow on what is cached.  ``share(0, [1, 2])``: empty requests begin with the pages of
+request 0, whose prompt has run, and ``attend`` reads what they have in common once for all of them.
 """
 from __future__ import annotations
 
@@ -26,7 +30,8 @@ from .cache import KV_Cache
 class paged_cache(KV_Cache):
     def __init__(self, layer_num: int, batch_size: int, max_length: int, num_key_value_heads: int, num_heads: int,
                  head_dim: int, dtype: torch.dtype, layer_mapping: dict, num_gpus: int, model_size: int, page_size: int = 16,
-                 num_pages: int | None = None, keep: int | None = None, sink: int = 4, recent: int = 64, slack: int = 64) -> None:
+                 num_pages: int | None = None, keep: int | None = None, sink: int = 4, recent: int = 64, slack: int = 64,
+                 attn_window=None, attn_sink: int = 0) -> None:
         # whatever a later call would refuse, before a prompt has run
         if head_dim != paged.DIM:
             raise ValueError("the paged kernels are built for head_dim 128")
@@ -43,9 +48,15 @@ class paged_cache(KV_Cache):
             raise ValueError("the layers of a paged cache lie on one GPU (several GPUs share a model by its heads)")
         if keep is not None and (min(sink, recent, slack) < 0 or keep < 1 or sink + recent > keep):
             raise ValueError(f"keep={keep} slots for {sink} first and {recent} last tokens, slack={slack}")
+        windows = list(attn_window) if isinstance(attn_window, (list, tuple)) else [attn_window] * layer_num
+        if len(windows) != layer_num or any(w is not None and w < 1 for w in windows) or attn_sink < 0:
+            raise ValueError(f"attn_window={attn_window}, attn_sink={attn_sink}: expected a slot or more (or None) for all layers or each")
+        if keep is not None and any(w is not None for w in windows):
+            raise ValueError("a window goes by the order of the slots, which eviction does not keep: attn_window or keep")
         super().__init__(layer_num, batch_size, max_length, num_key_value_heads, num_heads, head_dim, dtype, layer_mapping,
                          num_gpus, model_size)
         self.device = devices.pop()
+        self.attn_window, self.attn_sink = windows, attn_sink
         self.page_size, self.keep, self.sink, self.recent, self.slack = page_size, keep, sink, recent, slack
         width = -(-max_length // page_size)                     # pages of the longest request
         self.num_pages = batch_size * width if num_pages is None else num_pages
@@ -68,6 +79,9 @@ class paged_cache(KV_Cache):
         self._fed = [0] * batch_size                            # tokens of the step
         self._weighed, self._weighing = set(), set()            # requests whose slots were given weights before this step, in it
         self._chosen = {}                                       # the step's tables and lengths, of all and of some requests
+        self._sharers = {}                                      # page: requests that begin with it, where they are several
+        self._groups = None                                     # group_start and shared of `paged.paged_shared_decode`, on the device
+        self._one_each = torch.arange(batch_size + 1, dtype=torch.int32, device=self.device)      # row_start of a row of every request
 
     def _to_device(self, values) -> torch.Tensor:
         return torch.tensor(values, dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
@@ -115,11 +129,13 @@ class paged_cache(KV_Cache):
             self.row_start = self._to_device(starts)
         self.context += max(each)
 
-    def append(self, layer_idx, qkv, cos_sin, positions, axis_of, q, keys=None, values=None) -> None:
-        """The step's rows of a layer: rotate, split, and write to the pages (``paged.rope_paged_append``)."""
+    def append(self, layer_idx, qkv, cos_sin, positions, axis_of, q, keys=None, values=None, q_norm=None, k_norm=None, eps=1e-6) -> None:
+        """The step's rows of a layer: normalise heads where weights are given, rotate, split, and write to the pages
+        (``paged.rope_paged_append``)."""
         paged.rope_paged_append(qkv, cos_sin, positions, axis_of, q, self.key_pages[layer_idx], self.value_pages[layer_idx],
                                 self.page_table, self.held, self.row_start, weight=self.weight[layer_idx],
-                                token=self.token[layer_idx], seen=self.seen, keys=keys, values=values)
+                                token=self.token[layer_idx], seen=self.seen, keys=keys, values=values, q_norm=q_norm, k_norm=k_norm,
+                                eps=eps)
 
     def _of(self, requests):
         """Page table and lengths, of all requests or of some; the layers of a step share them.  A captured call is replayed in later
@@ -142,13 +158,69 @@ class paged_cache(KV_Cache):
         return self._chosen[key]
 
     def attend(self, query_states, layer_idx, out=None, lse=None, requests=None) -> torch.Tensor:
-        """Attention of one new token of every request, ``[batch, 1, heads, 128]``, over its slots (``paged.paged_decode``); with
-        ``keep`` the slots' weights grow by what they are given.  ``requests``: of these alone, in the order of their queries."""
+        """Attention of one new token of every request, ``[batch, 1, heads, 128]``, over its slots (``paged.paged_decode``), or the
+        layer's window of them; with ``keep`` the slots' weights grow by what they are given.  ``requests``: of these alone, in the order of
+        their queries.  Slots that requests next to each other have in common are read once (``paged.paged_shared_decode``)."""
         table, lengths = self._of(requests)
+        pools, window = (self.key_pages[layer_idx], self.value_pages[layer_idx]), self.attn_window[layer_idx]
+        if window is not None:
+            return paged.paged_decode(query_states, *pools, table, lengths, out=out, lse=lse, window=window, sink=self.attn_sink)
+        if self._groups is not None and requests is None:
+            return paged.paged_shared_decode(query_states, *pools, table, lengths, *self._groups, out=out, lse=lse)
         if self.keep is not None:
             self._weighing.update(range(self.batch_size) if requests is None else map(int, requests))
-        return paged.paged_decode(query_states, self.key_pages[layer_idx], self.value_pages[layer_idx], table, lengths, out=out, lse=lse,
-                                  weight=self.weight[layer_idx])
+        return paged.paged_decode(query_states, *pools, table, lengths, out=out, lse=lse, weight=self.weight[layer_idx])
+
+    def prompt(self, query_states, layer_idx, out=None, lse=None) -> torch.Tensor:
+        """Attention of the step's rows ``[rows, heads, 128]``, as ``append`` had them, over their requests' slots, or the layer's window
+        of them (``paged.paged_prompt``).  Not of a request that was evicted from."""
+        if any(e and n for e, n in zip(self._evicted, self._fed)):
+            raise RuntimeError("slots of a request were evicted: what its rows see is not known any more")
+        table, lengths = self._of(None)
+        starts = self._one_each if self.row_start is None else self.row_start
+        return paged.paged_prompt(query_states, self.key_pages[layer_idx], self.value_pages[layer_idx], table, lengths, starts,
+                                  window=self.attn_window[layer_idx], sink=self.attn_sink, out=out, lse=lse)
+
+    def share(self, of: int, requests, slots: int | None = None) -> int:
+        """Let ``requests``, which are empty, begin with the first ``slots`` slots of request ``of`` (default: all of them), as far as
+        they fill pages: nothing is copied.  Returns how many they are.  Not with ``keep``: requests that share pages cannot be evicted
+        from."""
+        requests, n = [int(b) for b in requests], self.length_of[of] if slots is None else slots
+        if self.keep is not None:
+            raise ValueError("requests that share pages cannot be evicted from: share or keep")
+        if not 0 <= n <= self.length_of[of] or of in requests or len(set(requests)) < len(requests) or \
+                any(not 0 <= b < self.batch_size or self.length_of[b] for b in requests):
+            raise ValueError(f"expected up to {self.length_of[of]} slots and empty requests other than {of}")
+        pages = self._pages[of][:n // self.page_size]
+        n = len(pages) * self.page_size
+        if not pages or not requests:
+            return n
+        for id in pages:
+            self._sharers[id] = self._sharers.get(id, 1) + len(requests)
+        at = self._to_device(requests).long()
+        self.page_table[at, :len(pages)] = self._to_device(pages)
+        for x in (self.lengths, self.seen_after):
+            x.index_fill_(0, at, n)
+        for b in requests:
+            self._give_back(b, 0)
+            self._pages[b], self.length_of[b] = list(pages), n
+        self._chosen = {}
+        self._regroup()
+        return n
+
+    def _regroup(self) -> None:
+        """Runs of requests next to each other that begin with the same pages."""
+        first_pages = [next((i for i, id in enumerate(p) if id not in self._sharers), len(p)) for p in self._pages]
+        alike = lambda a, b: next((i for i, (x, y) in enumerate(zip(a, b)) if x != y), min(len(a), len(b)))  # noqa: E731
+        starts, shared, b = [0], [], 0
+        while b < self.batch_size:
+            mine, n, end = self._pages[b][:first_pages[b]], 0, b + 1
+            while mine and end < self.batch_size and (m := alike(mine, self._pages[end])) and m >= n:
+                n, end = m if n == 0 else n, end + 1
+            starts.append(end)
+            shared.append(n * self.page_size)
+            b = end
+        self._groups = (self._to_device(starts), self._to_device(shared)) if any(shared) else None
 
     def observe(self, query_states, layer_idx, requests=None) -> None:
         """Weights from the last queries ``[batch, window, heads, 128]`` of the step's prompts (``paged.paged_observe``).  ``requests``:
@@ -194,13 +266,22 @@ class paged_cache(KV_Cache):
         """Request ``bdx`` is done: its pages go back, and its place may take another one."""
         self._give_back(bdx, 0)
         self.length_of[bdx], self._evicted[bdx], self._fed[bdx], self._chosen = 0, False, 0, {}
+        if self._groups is not None:
+            self._regroup()
         self._weighed.discard(bdx)
         self._weighing.discard(bdx)
         for x in (self.lengths, self.seen_after):
             x[bdx].zero_()
 
     def _give_back(self, bdx: int, keep_pages: int) -> None:
-        self._free.extend(reversed(self._pages[bdx][keep_pages:]))
+        for id in reversed(self._pages[bdx][keep_pages:]):
+            left = self._sharers.get(id, 1) - 1
+            if left == 0:
+                self._free.append(id)
+            if left > 1:
+                self._sharers[id] = left
+            else:
+                self._sharers.pop(id, None)
         del self._pages[bdx][keep_pages:]
 
     @property

@@ -35,6 +35,7 @@ class ModelShape:
     head_dim: int = 128
     rope_theta: float = 5e5
     rms_eps: float = 1e-5
+    qk_norm: bool = False              # RMS norms of query and key heads in front of the rotation
 
     @property
     def qkv_dim(self) -> int:
@@ -115,6 +116,9 @@ class SyntheticDecoder:
                                     gate_up=w(2 * it, h), down=w(h, it),
                                     norm1=torch.ones(h, dtype=dtype, device=device),
                                     norm2=torch.ones(h, dtype=dtype, device=device)))
+            if shape.qk_norm:
+                for name in ("q_norm", "k_norm"):
+                    self.layers[-1][name] = (1 + torch.randn(shape.head_dim, generator=gen, device=device) * 0.1).to(dtype)
         self.cos_sin = cos_sin_cache(max_positions, shape.head_dim, shape.rope_theta, device)
         # the position of the token being decoded, per request (the reference slices position_ids at
         # kv_cache.context, model_hub/llama.py:330-337); advanced on the device after every step
@@ -136,7 +140,7 @@ class SyntheticDecoder:
         rmsnorm(self.residual if x is None else x, L["norm1"], s.rms_eps, self.normed,
                 residual=None if x is None else self.residual)
         qkv = F.linear(self.normed, L["wqkv"])
-        rope_split(qkv, self.cos_sin, self.positions, self.q, self.k, self.v)
+        rope_split(qkv, self.cos_sin, self.positions, self.q, self.k, self.v, L.get("q_norm"), L.get("k_norm"), s.rms_eps)
         self.cache.decode_update_kv_cache(self.k, self.v, ldx)
         # attn_hub.retroinfer_decode_attn is cache.compute; called directly to hand it the output buffer
         attn = self.cache.compute(self.q, ldx, out=self.attn)
@@ -168,7 +172,8 @@ class SyntheticDecoder:
 class PagedDecoder(SyntheticDecoder):
     """The same model over a ``paged_cache``: prompts of uneven lengths in one pass, then a token of every running request a step.
     A request that is done gives its place back (``release``), and another prompt may take it while the rest run on.  ``axis_of``: the position axis of each rotary frequency (``paged.rope_sections``); ``window``: the last queries of a prompt that
-    its slots' weights come from, where the cache evicts."""
+    its slots' weights come from, where the cache evicts.  Requests may begin with what another one has cached (``share``), and take more
+    tokens later (``extend_forward``); layers of a cache with ``attn_window`` look back over their window."""
 
     def __init__(self, shape: ModelShape, cache, batch: int, max_positions: int, device, dtype=torch.bfloat16, seed: int = 0,
                  std: float = 0.02, layers: int | None = None, axis_of=None, window: int = 32):
@@ -184,7 +189,8 @@ class PagedDecoder(SyntheticDecoder):
         s, L = self.shape, self.layers[ldx]
         normed = torch.empty_like(residual)
         rmsnorm(residual if x is None else x, L["norm1"], s.rms_eps, normed, residual=None if x is None else residual)
-        self.cache.append(ldx, F.linear(normed, L["wqkv"]), self.cos_sin, positions, self.axis_of, q, keys, values)
+        self.cache.append(ldx, F.linear(normed, L["wqkv"]), self.cos_sin, positions, self.axis_of, q, keys, values, L.get("q_norm"),
+                          L.get("k_norm"), s.rms_eps)
         o = F.linear(attend().view(residual.shape[0], -1), L["wo"])
         rmsnorm(o, L["norm2"], s.rms_eps, normed, residual=residual)
         gated = torch.empty((residual.shape[0], s.intermediate), dtype=self.dtype, device=self.device)
@@ -219,21 +225,41 @@ class PagedDecoder(SyntheticDecoder):
         ``positions``: ``[axes, tokens]`` for each, from 0 to ``max_positions - 1`` (default: counted up on every axis; given ones are
         looked at, which waits for them).  Logits ``[prompts, vocab]`` of the last tokens; the cache is brought down to its ``keep``
         slots."""
+        return self._prompts(prompts, positions, requests, False)
+
+    def extend_forward(self, prompts, positions=None, requests=None) -> torch.Tensor:
+        """``prefill_forward`` of tokens that follow on what the requests have cached, the rest of a prompt or more of a conversation
+        (default positions: counted on).  Not with eviction."""
+        if self.cache.keep is not None:
+            raise ValueError("tokens that follow on what is cached need all of it: not with eviction")
+        return self._prompts(prompts, positions, requests, True)
+
+    def share(self, of: int, requests, tokens: int | None = None) -> int:
+        """Let ``requests``, which are empty, begin with the first ``tokens`` tokens of request ``of`` (default: all), as far as they
+        fill pages of the cache; returns how many they are.  Positions are counted on from there: hand others to ``extend_forward``."""
+        n = self.cache.share(of, requests, tokens)
+        for b in requests:
+            self._next_position[b] = n
+            self.positions[:, b].fill_(n)
+        return n
+
+    def _prompts(self, prompts, positions, requests, follow: bool) -> torch.Tensor:
         from .attn_hub import retroinfer_prefill_attn
 
         s, counts = self.shape, [int(p.numel()) for p in prompts]
         places = tuple(range(self.batch)) if requests is None else tuple(int(b) for b in requests)
         if len(places) != len(counts) or not places or list(places) != sorted(set(places) & set(range(self.batch))):
             raise ValueError(f"expected a prompt for each of the requests, which ascend from 0 to {self.batch - 1}")
-        if min(counts) < 1 or any(self.cache.length_of[b] for b in places):
+        if min(counts) < 1 or (not follow and any(self.cache.length_of[b] for b in places)):
             raise ValueError("expected prompts of a token or more, and their places in the cache empty")
         all_of_them = len(places) == self.batch
         at, each = None if all_of_them else self._at(places), [0] * self.batch
         for b, n in zip(places, counts):
             each[b] = n
         if positions is None:
-            ends, least = counts, 0
-            positions = [torch.arange(n, device=self.device).expand(self.axes, n) for n in counts]
+            first = [self._next_position[b] if follow else 0 for b in places]
+            ends, least = [i + n for i, n in zip(first, counts)], 0
+            positions = [torch.arange(i, i + n, device=self.device).expand(self.axes, n) for i, n in zip(first, counts)]
         else:
             if len(positions) != len(counts) or any(p.dim() != 2 or p.shape[0] < self.axes or p.shape[1] != n for p, n in zip(positions, counts)):
                 raise ValueError(f"expected positions [{self.axes}, tokens] for every prompt")
@@ -260,6 +286,8 @@ class PagedDecoder(SyntheticDecoder):
         x = None
         for ldx in range(self.n_layers):
             def attend():
+                if follow or self.cache.attn_window[ldx] is not None:
+                    return self.cache.prompt(q, ldx)
                 return torch.cat([retroinfer_prefill_attn(*(t[None, i:i + n] for t in (q, k, v)), True)[0]
                                   for i, n in zip(starts, counts)])
             x = self._layer(ldx, residual, x, where, q, attend, k, v)

@@ -139,3 +139,47 @@ def test_sections_that_are_no_numbers_of_frequencies():
         for bad in ((-1,), (65, -1), (32.5, 31.5)):
             with pytest.raises(ValueError, match="sections"):
                 make_axes(*bad)
+
+
+def test_windows(make):
+    cache = make(layer_num=2, layer_mapping={"0": "cpu", "1": "cpu"}, attn_window=[None, 30], attn_sink=4)
+    assert cache.attn_window == [None, 30] and make(attn_window=30).attn_window == [30]
+    for bad in (dict(attn_window=0), dict(attn_window=[3, 4]), dict(attn_window=3, attn_sink=-1), dict(attn_window=3, keep=80)):
+        with pytest.raises(ValueError):
+            make(**bad)
+
+
+def test_shared_pages_and_their_groups(make):
+    cache = make(batch_size=5, page_size=16, num_pages=30)
+    cache.begin([50, 0, 0, 20, 0])
+    assert cache.share(0, [1, 2]) == 48                       # whole pages
+    assert cache.length_of == [50, 48, 48, 20, 0] and cache.lengths.tolist() == cache.length_of == cache.seen_after.tolist()
+    assert (cache.page_table[:3, :3] == cache.page_table[0, :3]).all() and cache.free_pages == 30 - 4 - 2
+    starts, shared = cache._groups
+    assert starts.tolist() == [0, 3, 4, 5] and shared.tolist() == [48, 0, 0]
+    cache.begin([1, 1, 1, 1, 0])                              # request 0 goes on in its last page, the others on pages of their own
+    assert cache.free_pages == 30 - 4 - 2 - 2
+    assert len({int(cache.page_table[b, 3]) for b in range(3)}) == 3
+    assert cache.share(1, [4], slots=33) == 32
+    assert cache._groups[0].tolist() == [0, 3, 4, 5]
+    cache.release(0)                                          # what others begin with stays
+    assert cache.free_pages == 30 - 4 - 2 - 2 + 1 and cache._groups[0].tolist() == [0, 1, 3, 4, 5] and cache._groups[1].tolist() == [0, 48, 0, 0]
+    cache.release(2)
+    cache.release(4)
+    assert cache._groups is None
+    cache.release(1)
+    cache.release(3)
+    assert cache.free_pages == 30 and not cache._sharers and sorted(cache._free) == list(range(30))
+
+
+def test_what_cannot_be_shared_is_refused(make):
+    cache = make(batch_size=3)
+    cache.begin([40, 3, 0])
+    for of, requests, slots in ((0, [0], None), (0, [1], None), (0, [2, 2], None), (0, [3], None), (0, [2], 41), (0, [2], -1)):
+        with pytest.raises(ValueError):
+            cache.share(of, requests, slots)
+    assert cache.share(1, [2]) == 0 and cache.length_of == [40, 3, 0]
+    cache = make(keep=80)
+    cache.begin([40, 0])
+    with pytest.raises(ValueError, match="evicted"):
+        cache.share(0, [1])
