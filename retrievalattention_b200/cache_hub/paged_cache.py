@@ -80,7 +80,9 @@ class paged_cache(KV_Cache):
         self._weighed, self._weighing = set(), set()            # requests whose slots were given weights before this step, in it
         self._chosen = {}                                       # the step's tables and lengths, of all and of some requests
         self._sharers = {}                                      # page: requests that begin with it, where they are several
-        self._groups = None                                     # group_start and shared of `paged.paged_shared_decode`, on the device
+        # group_start and shared of `paged.paged_shared_decode`, as many groups as requests, so that captured calls follow them
+        self._group_start, self._group_shared = zeros(batch_size + 1, kind=torch.int32), zeros(batch_size, kind=torch.int32)
+        self._alike = False                                     # some requests have slots in common
         self._one_each = torch.arange(batch_size + 1, dtype=torch.int32, device=self.device)      # row_start of a row of every request
 
     def _to_device(self, values) -> torch.Tensor:
@@ -165,8 +167,8 @@ class paged_cache(KV_Cache):
         pools, window = (self.key_pages[layer_idx], self.value_pages[layer_idx]), self.attn_window[layer_idx]
         if window is not None:
             return paged.paged_decode(query_states, *pools, table, lengths, out=out, lse=lse, window=window, sink=self.attn_sink)
-        if self._groups is not None and requests is None:
-            return paged.paged_shared_decode(query_states, *pools, table, lengths, *self._groups, out=out, lse=lse)
+        if self._alike and requests is None:
+            return paged.paged_shared_decode(query_states, *pools, table, lengths, self._group_start, self._group_shared, out=out, lse=lse)
         if self.keep is not None:
             self._weighing.update(range(self.batch_size) if requests is None else map(int, requests))
         return paged.paged_decode(query_states, *pools, table, lengths, out=out, lse=lse, weight=self.weight[layer_idx])
@@ -220,7 +222,10 @@ class paged_cache(KV_Cache):
             starts.append(end)
             shared.append(n * self.page_size)
             b = end
-        self._groups = (self._to_device(starts), self._to_device(shared)) if any(shared) else None
+        more = self.batch_size - len(shared)
+        self._group_start.copy_(self._to_device(starts + [self.batch_size] * more))
+        self._group_shared.copy_(self._to_device(shared + [0] * more))
+        self._alike = any(shared)
 
     def observe(self, query_states, layer_idx, requests=None) -> None:
         """Weights from the last queries ``[batch, window, heads, 128]`` of the step's prompts (``paged.paged_observe``).  ``requests``:
@@ -266,7 +271,7 @@ class paged_cache(KV_Cache):
         """Request ``bdx`` is done: its pages go back, and its place may take another one."""
         self._give_back(bdx, 0)
         self.length_of[bdx], self._evicted[bdx], self._fed[bdx], self._chosen = 0, False, 0, {}
-        if self._groups is not None:
+        if self._alike:
             self._regroup()
         self._weighed.discard(bdx)
         self._weighing.discard(bdx)

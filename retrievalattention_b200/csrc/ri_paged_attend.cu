@@ -250,7 +250,7 @@ __device__ __forceinline__ void plan(const Args& a, int* table, Control& s) {
         if (y - before < it.cost()) {
           step = max(0, y - before - kItemCost);
           if (step > 0) {
-            if (step <= kSnap) {
+            if (step <= kSnap || a.meta == nullptr) {      // no room for partial results: no item is long enough to be cut
               step = 0;
               break;
             }
@@ -1099,14 +1099,16 @@ int64_t most_items_rows(const ri_paged& p, int rows) {      // rows of an item, 
   const int pair = 2 * (kTile / p.group_size);
   return (int64_t)(rows < pair ? rows : pair) * p.group_size;
 }
-// Whether an item may be cut: it has more steps than two snaps.
-bool may_cut(const ri_paged& p, int rows, int window, int sink) {
+// Steps of an item, at most.
+int64_t most_steps(const ri_paged& p, int rows, int window, int sink) {
   const int64_t all = (slots_of(p) + kTile - 1) / kTile;
-  if (window == 0) return all > 2 * kSnap;
+  if (window == 0) return all;
   const int64_t pair = 2 * (kTile / p.group_size), box = p.page_size < kTile ? p.page_size : kTile;
   const int64_t seen = ((int64_t)window + sink + (rows < pair ? rows : pair) + 2 * box + kTile - 1) / kTile;      // first slots and window in boxes begun
-  return (seen < all ? seen : all) > 2 * kSnap;
+  return seen < all ? seen : all;
 }
+// Whether an item may be cut.
+bool may_cut(const ri_paged& p, int rows, int window, int sink) { return most_steps(p, rows, window, sink) > 2 * kSnap; }
 
 int check_call(const char* what, const ri_paged* p, int64_t sequences) {
   const int rc = check(p, what);
@@ -1133,6 +1135,8 @@ int attend(const char* what, const ri_paged* p, const void* d_q, int64_t q_strid
            bool join, cudaStream_t s) {
   int rc;
   RI_REQUIRE(p->d_values && d_q && (SHARED || d_out) && a.starts, "%s: null pointer", what);
+  const int64_t pairs = (int64_t)rows / (2 * (kTile / p->group_size)) + a.n_seq;
+  RI_REQUIRE(pairs * (most_steps(*p, rows, a.window, a.sink) + kItemCost) < (1ll << 31), "%s: too large", what);      // they are counted in 32 bits
   RI_REQUIRE(q_stride >= (int64_t)p->kv_heads * p->group_size * RI_HEAD_DIM && q_stride % 8 == 0, "%s: queries overlap or lie at odd places", what);
   RI_REQUIRE(((uintptr_t)d_q | (uintptr_t)d_out) % 16 == 0, "%s: tensors must be 16-byte aligned", what);
   RI_REQUIRE(scale > 0.f && scale < 1e30f, "%s: scale must be positive and finite", what);

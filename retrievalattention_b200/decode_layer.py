@@ -257,7 +257,7 @@ class PagedDecoder(SyntheticDecoder):
         for b, n in zip(places, counts):
             each[b] = n
         if positions is None:
-            first = [self._next_position[b] if follow else 0 for b in places]
+            first = [self._next_position[b] if self.cache.length_of[b] else 0 for b in places]
             ends, least = [i + n for i, n in zip(first, counts)], 0
             positions = [torch.arange(i, i + n, device=self.device).expand(self.axes, n) for i, n in zip(first, counts)]
         else:

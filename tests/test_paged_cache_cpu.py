@@ -155,18 +155,18 @@ def test_shared_pages_and_their_groups(make):
     assert cache.share(0, [1, 2]) == 48                       # whole pages
     assert cache.length_of == [50, 48, 48, 20, 0] and cache.lengths.tolist() == cache.length_of == cache.seen_after.tolist()
     assert (cache.page_table[:3, :3] == cache.page_table[0, :3]).all() and cache.free_pages == 30 - 4 - 2
-    starts, shared = cache._groups
-    assert starts.tolist() == [0, 3, 4, 5] and shared.tolist() == [48, 0, 0]
+    groups = lambda: (cache._group_start.tolist(), cache._group_shared.tolist())  # noqa: E731
+    assert cache._alike and groups() == ([0, 3, 4, 5, 5, 5], [48, 0, 0, 0, 0])      # filled up with empty ones
     cache.begin([1, 1, 1, 1, 0])                              # request 0 goes on in its last page, the others on pages of their own
     assert cache.free_pages == 30 - 4 - 2 - 2
     assert len({int(cache.page_table[b, 3]) for b in range(3)}) == 3
     assert cache.share(1, [4], slots=33) == 32
-    assert cache._groups[0].tolist() == [0, 3, 4, 5]
+    assert groups() == ([0, 3, 4, 5, 5, 5], [48, 0, 0, 0, 0])
     cache.release(0)                                          # what others begin with stays
-    assert cache.free_pages == 30 - 4 - 2 - 2 + 1 and cache._groups[0].tolist() == [0, 1, 3, 4, 5] and cache._groups[1].tolist() == [0, 48, 0, 0]
+    assert cache.free_pages == 30 - 4 - 2 - 2 + 1 and groups() == ([0, 1, 3, 4, 5, 5], [0, 48, 0, 0, 0])
     cache.release(2)
     cache.release(4)
-    assert cache._groups is None
+    assert not cache._alike
     cache.release(1)
     cache.release(3)
     assert cache.free_pages == 30 and not cache._sharers and sorted(cache._free) == list(range(30))

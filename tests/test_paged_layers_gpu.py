@@ -70,6 +70,9 @@ def test_prompts_steps_and_more_tokens(window, sink, qk_norm):
     for b, p in zip((0, 2), more):
         ids[b] = ids[b][:-1] + list(p)
     check(model, model.extend_forward(more, requests=[0, 2]), ids, (0, 2))
+    model.release(1)                                          # its place's next tokens are another request's first
+    ids[1] = list(prompt(7))
+    check(model, model.extend_forward([torch.stack(ids[1])], requests=[1]), ids, (1,))
     for _ in range(3):
         check(model, model.decode_forward(), ids, range(3))
     check_prefill_errors()
@@ -92,7 +95,7 @@ def test_requests_that_begin_alike(window):
     for b, p in zip((1, 2), rest):
         ids[b] = list(begin[:64]) + list(p)
     check(model, model.extend_forward(rest, requests=[1, 2]), ids, (1, 2))
-    assert (model.cache._groups is not None) and model.cache._groups[1].tolist()[0] == 64
+    assert model.cache._alike and model.cache._group_shared.tolist()[0] == 64
     for step in range(4):
         check(model, model.decode_forward(), ids, (0, 1, 2))
     model.release(0)                                          # the pages that the others begin with stay
@@ -129,7 +132,15 @@ def test_captured_attention_of_requests_that_begin_alike():
     eager = cache.attend(q, 0, lse=other)
     check_prefill_errors()
     # probabilities and outputs are rounded to 16 bits, half a step of 2^-7 each, on either side
-    assert ((out.float() - eager.float()).abs() <= 2.0 ** -6 * (eager.float().abs() + 0.2)).all() and (lse - other).abs().max() <= 1e-4
+    same = lambda: ((out.float() - eager.float()).abs() <= 2.0 ** -6 * (eager.float().abs() + 0.2)).all() and (lse - other).abs().max() <= 1e-4  # noqa: E731
+    assert same()
+    # requests that come and go: the captured call finds the new groups
+    model.release(1)
+    model.prefill_forward([torch.randint(0, 1000, (70,), generator=gen).cuda()], requests=[1])
+    graph.replay()
+    eager = cache.attend(q, 0, lse=other)
+    assert same()
+    check_prefill_errors()
 
 
 def test_refusals():

@@ -183,6 +183,26 @@ def test_pages_that_no_row_sees_are_left_alone():
     run(layer, (300,), 4, window=500, sink=10)
 
 
+def test_pools_past_two_to_the_31_elements():
+    """Rows that lie behind 2^31 elements of a pool, read by the copies and where a row is done again."""
+    first = (1 << 31) // (2 * 64 * DIM) + 5
+    layer = Layer([1500, 300], 2, 64, torch.bfloat16, seed=3, first_page=first)
+    run(layer, (700, 20), 4)
+    v = layer.v[0].clone()
+    v[:, 1400, 3] = float("nan")                        # rows in front of it are done again
+    layer.fill(0, layer.k[0].float(), v.float(), layer.w[0].float(), layer.t[0])
+    from retrievalattention_b200 import paged
+
+    q = torch.randn(100, 8, DIM, device="cuda").to(torch.bfloat16)
+    starts = torch.tensor([0, 100, 100], dtype=torch.int32, device="cuda")
+    out = paged.paged_prompt(q, layer.keys, layer.values, layer.table, torch.tensor([1450, 0], dtype=torch.int32, device="cuda"), starts)
+    clean = torch.nan_to_num(v, nan=0.0)
+    want = attend_rows(q.cpu().double(), layer.k[0][:, :1450], clean[:, :1450], visible(torch.arange(1350, 1450), 1450, None, 0))
+    assert torch.isnan(out[50:, :, 3]).all()
+    out[50:, :, 3], want[0][50:, :, 3], want[2][50:, :, 3] = 0.0, 0.0, 0.0
+    assert close(out, None, *want)
+
+
 def test_scale_and_wide_tables():
     from retrievalattention_b200 import paged
 
