@@ -263,6 +263,49 @@ def test_results_repeat_and_follow_the_stream():
     assert torch.equal(first, again)
 
 
+def test_two_calls_at_once():
+    """On two streams, prompts and shared prefixes beside each other: each result is what it is alone."""
+    from retrievalattention_b200 import paged
+    from retrievalattention_b200.attn_hub.retroinfer_attn import check_prefill_errors
+
+    layer = Layer([3000, 2900, 2800], 2, 16, torch.bfloat16, seed=6)
+    layer.table[1:, :128] = layer.table[0, :128]
+    wide = torch.full((3, 150000), -1, dtype=torch.int32, device="cuda")
+    wide[:, :layer.table.shape[1]] = layer.table
+    q, one = torch.randn(400, 8, DIM, device="cuda").to(torch.bfloat16), torch.randn(3, 1, 8, DIM, device="cuda").to(torch.bfloat16)
+    starts, groups, common = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 300, 310, 400], [0, 3], [2048]))
+    calls = [lambda: paged.paged_prompt(q, layer.keys, layer.values, layer.table, layer.lengths, starts, window=500, sink=4),
+             lambda: paged.paged_shared_decode(one, layer.keys, layer.values, wide, layer.lengths, groups, common),
+             lambda: paged.paged_prompt(q, layer.keys, layer.values, layer.table, layer.lengths, starts)]
+    alone = [call() for call in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    results = [[] for _ in calls]
+    for _ in range(10):
+        for call, stream, got in zip(calls, streams, results):
+            with torch.cuda.stream(stream):
+                got.append(call())
+    torch.cuda.synchronize()
+    check_prefill_errors()
+    for got, want in zip(results, alone):
+        assert all(torch.equal(x, want) for x in got)
+
+
+def test_outputs_on_any_boundary_of_16_bytes():
+    from retrievalattention_b200 import paged
+
+    layer = Layer([200], 2, 16, torch.bfloat16, seed=6)
+    q = torch.randn(100, 8, DIM, device="cuda").to(torch.bfloat16)
+    starts = torch.tensor([0, 100], dtype=torch.int32, device="cuda")
+    args = layer.keys, layer.values, layer.table, layer.lengths, starts
+    want = paged.paged_prompt(q, *args)
+    for off in (8, 16):
+        flat = torch.zeros(q.numel() + 64, dtype=torch.bfloat16, device="cuda")
+        out = flat[off:off + q.numel()].view(q.shape)
+        paged.paged_prompt(q, *args, out=out)
+        assert torch.equal(out, want) and (flat[:off] == 0).all() and (flat[off + q.numel():] == 0).all()
+
+
 def test_bad_page_numbers_are_reported():
     from retrievalattention_b200 import paged
     from retrievalattention_b200.attn_hub.retroinfer_attn import check_prefill_errors
