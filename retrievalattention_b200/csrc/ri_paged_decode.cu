@@ -680,33 +680,41 @@ __global__ void __launch_bounds__(kFinishThreads, kFinishBlocks) paged_finish_ke
 }
 
 // The same where requests have slots in common: a block per group joins the partial results over those and over the request's own, a
-// thread for each query head and four channels.  (As a part of the kernel above, a block for each query head: 64 requests of 8 heads
-// of 4, 14 us.)
+// thread for each query head and four channels, several of them with every n-th part each.  (As a part of the kernel above, a block for
+// each query head: 64 requests of 8 heads of 4, 14 us.)  What it goes by are the call's inputs, so that it is looked up before the wait.
+constexpr int kSharedThreads = 512;
 template <int DT>
-__global__ void __launch_bounds__(kFinishThreads, 3) shared_finish_kernel(const __grid_constant__ SharedArgs a) {
+__global__ void __launch_bounds__(kSharedThreads, 2) shared_finish_kernel(const __grid_constant__ SharedArgs a) {
   extern __shared__ int s_slot[];
   __shared__ int s_n;
+  __shared__ float4 s_o[kSharedThreads];
+  __shared__ float2 s_ml[kSharedThreads];
   ri_pdl_trigger();
-  const int gs = a.gs, g = blockIdx.x, b = g / a.hk, h_kv = g - b * a.hk, quad = threadIdx.x / gs, r = threadIdx.x - quad * gs;
-  const Own own = list_own(a, b, h_kv, g, s_slot);
-  if (threadIdx.x == 0) s_n = own.count;
-  ri_pdl_wait();
+  const int gs = a.gs, g = blockIdx.x, b = g / a.hk, h_kv = g - b * a.hk;
+  const int each = gs * (RI_HEAD_DIM / 4), teams = kSharedThreads / each, team = threadIdx.x / each, t = threadIdx.x - team * each;
+  const int quad = t / gs, r = t - quad * gs;
   const ri_shared::Parts& x = a.common;
-  int extra = 0, item_rows = 0, item_row = 0;
-  int64_t part = 0;
+  int item = -1, item_rows = 0, item_row = 0;              // the group's item, if there is one
   if (ri_shared::common_of(a, x, b) > 0) {
     const int of = ri_shared::group_of(x.starts, x.groups, b);
     const int b0 = ri_shared::clamped(x.starts[of], a.batch), b1 = ri_shared::clamped(x.starts[of + 1], a.batch);
-    const int first = b0 + (b - b0) / x.pair * x.pair, item = h_kv * a.batch + first;
-    const int c0 = ri_shared::clamped(x.ctas[2 * item], x.max_ctas - 1);
-    extra = max(0, ri_shared::clamped(x.ctas[2 * item + 1], x.max_ctas - 1) - c0 + 1);
+    const int first = b0 + (b - b0) / x.pair * x.pair;
+    item = h_kv * a.batch + first;
     item_rows = min(x.pair, b1 - first) * gs;
     item_row = (b - first) * gs + r;
+  }
+  const Own own = list_own(a, b, h_kv, g, s_slot);
+  if (threadIdx.x == 0) s_n = own.count;
+  ri_pdl_wait();
+  int extra = 0;
+  int64_t part = 0;
+  if (item >= 0) {
+    const int c0 = ri_shared::clamped(x.ctas[2 * item], x.max_ctas - 1);
+    extra = max(0, ri_shared::clamped(x.ctas[2 * item + 1], x.max_ctas - 1) - c0 + 1);
     part = (int64_t)c0 * x.part_rows + (int64_t)item * gs;
   }
   __syncthreads();
-  const int count = s_n;
-  if (quad >= RI_HEAD_DIM / 4) return;
+  const int count = extra + s_n;
   auto ml_of = [&](int i) {
     return i < extra ? x.ml[part + (int64_t)i * x.part_rows + item_row] : a.part_ml[(int64_t)s_slot[i - extra] * gs + r];
   };
@@ -714,37 +722,44 @@ __global__ void __launch_bounds__(kFinishThreads, 3) shared_finish_kernel(const 
     return i < extra ? reinterpret_cast<const float4*>(x.o + (part + (int64_t)i * x.part_rows) * RI_HEAD_DIM)[((quad >> 1) * item_rows + item_row) * 2 + (quad & 1)]
                      : reinterpret_cast<const float4*>(a.part_o + ((int64_t)s_slot[i - extra] * gs + r) * RI_HEAD_DIM)[quad];
   };
-  constexpr int kWide = 8;                                 // partial results on their way
+  constexpr int kWide = 4;                                 // partial results on their way
   float M = -INFINITY, L = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < extra + count; i0 += kWide) {
-    float2 ml[kWide];
-    float4 v[kWide];
-#pragma unroll
-    for (int u = 0; u < kWide; ++u) {
-      const int i = i0 + u;
-      ml[u] = make_float2(-INFINITY, 0.f);
-      v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (i < extra + count) {
-        ml[u] = ml_of(i);
-        v[u] = four_of(i);
-      }
-    }
+  // adds parts against the largest reference so far; one far below it still counts enough to hand on an infinite value
+  auto add = [&](const float2* ml, const float4* v, int n) {
     float most = M;
-#pragma unroll
-    for (int u = 0; u < kWide; ++u) most = fmaxf(most, ml[u].x);
+    for (int u = 0; u < n; ++u) most = fmaxf(most, ml[u].x);
     const float ref = most == -INFINITY ? 0.f : most, old = exp2f(M - ref);
     L *= old;
     o.x *= old; o.y *= old; o.z *= old; o.w *= old;
-#pragma unroll
-    for (int u = 0; u < kWide; ++u) {
-      // a part far below the largest still counts enough to hand on an infinite value
+    for (int u = 0; u < n; ++u) {
       const float f = ml[u].x == -INFINITY ? 0.f : fmaxf(exp2f(ml[u].x - ref), 1.17549435e-38f);
       L += ml[u].y * f;
       o.x += v[u].x * f; o.y += v[u].y * f; o.z += v[u].z * f; o.w += v[u].w * f;
     }
     M = most;
-  }
+  };
+  if (team < teams)
+    for (int i0 = team; i0 < count; i0 += kWide * teams) {
+      float2 ml[kWide];
+      float4 v[kWide];
+#pragma unroll
+      for (int u = 0; u < kWide; ++u) {
+        const int i = i0 + u * teams;
+        ml[u] = make_float2(-INFINITY, 0.f);
+        v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < count) {
+          ml[u] = ml_of(i);
+          v[u] = four_of(i);
+        }
+      }
+      add(ml, v, kWide);
+    }
+  s_ml[threadIdx.x] = make_float2(M, L);
+  s_o[threadIdx.x] = o;
+  __syncthreads();
+  if (team > 0) return;
+  for (int u = 1; u < teams; ++u) add(&s_ml[u * each + t], &s_o[u * each + t], 1);
   const float f = L == 0.f ? 0.f : 1.f / L;
   *reinterpret_cast<uint2*>(a.out + ((int64_t)g * gs + r) * RI_HEAD_DIM + quad * 4) =
       make_uint2(Elem<DT>::pack2(o.x * f, o.y * f), Elem<DT>::pack2(o.z * f, o.w * f));
@@ -862,7 +877,7 @@ int launch_paged(const Args& a, const CUtensorMap& map_k, const CUtensorMap& map
   const int64_t groups = (int64_t)a.batch * a.hk, steps = (most + 15) / 16, parts = (int64_t)a.max_ctas * kPagedWarps;
   const size_t smem = (size_t)(steps < parts ? steps : parts) * 4 + 4;
   if constexpr (std::is_same_v<Args, SharedArgs>) {
-    RI_CUDA_OK(ri_launch_pdl_id(11, shared_finish_kernel<DT>, dim3((unsigned)groups), dim3(kFinishThreads), smem, s, a));
+    RI_CUDA_OK(ri_launch_pdl_id(11, shared_finish_kernel<DT>, dim3((unsigned)groups), dim3(kSharedThreads), smem, s, a));
   } else {
     // blocks of a group: for its heads, or with weights its tiles of slots, as many as the chip holds at once
     const int64_t tiles = a.weight ? (most + kFoldSlots - 1) / kFoldSlots : 0, room = kFinishBlocks * (int64_t)a.max_ctas / groups;
