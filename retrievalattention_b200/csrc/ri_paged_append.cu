@@ -5,8 +5,9 @@
 // With norms a query or key head is first  x_i <- x_i w_i / sqrt(mean x^2 + eps),  in 32 bits up to the one rounding behind the rotation;
 // the half-warp that has a head has its sum of squares in four shuffles.  The root is taken behind the rotation, and weights that are
 // the same for all heads go into the row's cosines and sines, which a service warp multiplies: the rotation is what it was, and the
-// rotating warps, which would be what counts otherwise, have a third more to do, not twice as much.  32768 rows of 32 + 8 heads: 156 us
-// (149 without norms; with the weights loaded and multiplied head by head 210, as pairs 198).  Weights for each head are read so: 198 us.
+// rotating warps, which would be what counts otherwise, have a third more to do, not twice as much.  32768 rows of 32 + 8 heads: 153 us
+// (149 without norms; with the weights loaded and multiplied head by head 210).  Weights for each head are multiplied by the lane that has
+// the piece, and the piece that it is rotated with comes from the lane beside it: 176 us (198 with both pieces weighted by both lanes).
 // (reference: model_hub/llama.py:232-235 the split, :312-320 the rotation; cache_hub/flash_attn_cache.py:133-151 the append)
 //
 // Bound by the projection, read once and written once.  A row of it lies in one piece and comes in by one bulk copy, three rows
@@ -332,18 +333,18 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) rope_append_kerne
           }
           uint64_t x[4], y[4];
           unpack_pairs<DT>(mine16, x);
-          unpack_pairs<DT>(src[j * 16 + (c ^ 8)], y);
           const float inv = rsqrtf(head_squares(x, half_warp) * (1.f / RI_HEAD_DIM) + a.eps);
-          if (NORM == kHeadWeights) {
+          if (NORM == kHeadWeights) {                  // the piece it is rotated with comes, weighted, from the lane that has it
             const uint4* w = key ? a.k_norm + (head - a.hq) * a.k_norm_stride : a.q_norm + head * a.q_norm_stride;
-            uint64_t wx[4], wy[4];
+            uint64_t wx[4];
             unpack_pairs<DT>(ri_ldg16(w + c), wx);
-            unpack_pairs<DT>(ri_ldg16(w + (c ^ 8)), wy);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               x[k] = mul_f2(x[k], wx[k]);
-              y[k] = mul_f2(y[k], wy[k]);
+              y[k] = __shfl_xor_sync(half_warp, (unsigned long long)x[k], 8);
             }
+          } else {
+            unpack_pairs<DT>(src[j * 16 + (c ^ 8)], y);
           }
           put(row0 + r, head, rotate_normed<DT>(x, y, fa, fb, inv));
         }
