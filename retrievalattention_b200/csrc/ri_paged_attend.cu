@@ -831,7 +831,10 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         return x;
       };
       const Sight sight = sight_of_row();
-      float m_ref = -INFINITY, l_run = 0.f;
+      // Rows that fill up a tile hold what was there before, or are another request's: they take no part in what a warp decides together,
+      // so that results repeat to the bit.  No score is above their reference.
+      auto is_row = [&] { return row < a.tile_tokens * a.gs && row_in_item() < sg.n_tok * a.gs; };
+      float m_ref = is_row() ? -INFINITY : INFINITY, l_run = 0.f;
       for (int j = 0; ok && j < sg.steps(grp); ++j, phases ^= 1) {
         const int place = sg.nth(grp, j) * kTile;
         ok = __all_sync(0xffffffffu, mbar_wait(bar_s_full(grp), phases & 1, abort_flag, 11));
@@ -950,7 +953,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         tc_fence_after();
         const bool both = !two && sg.steps(1) > 0;
         const int n_rows = sg.n_tok * a.gs, item_row = row_in_item(), q_row = token();
-        const bool valid = row < a.tile_tokens * a.gs && item_row < n_rows;
+        const bool valid = is_row();
         const int x0 = two ? 0 : grp * 2, x1 = two ? 4 : x0 + 2;
         const int h = sg.head * a.gs + item_row % a.gs;
         const bool wide = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;

@@ -263,6 +263,22 @@ def test_results_repeat_and_follow_the_stream():
     assert torch.equal(first, again)
 
 
+@pytest.mark.parametrize("group", [3, 5, 7])
+def test_results_repeat_whatever_ran_before(group):
+    """Rows that fill up a tile hold what another call left in shared memory: nothing of it reaches the rounding of the others."""
+    from retrievalattention_b200 import paged
+
+    layer = Layer([1727, 1606], 2, 64, torch.bfloat16, seed=6)
+    gen = torch.Generator().manual_seed(group)
+    q = torch.randn(2000, 2 * group, DIM, generator=gen).to(torch.bfloat16).cuda()
+    starts = torch.tensor([0, 1000, 2000], dtype=torch.int32, device="cuda")
+    call = lambda x: paged.paged_prompt(x, layer.keys, layer.values, layer.table, layer.lengths, starts, window=1, sink=1)  # noqa: E731
+    want = call(q)
+    for i in range(8):
+        call(q * (100.0 * i))                           # something else in the rows
+        assert torch.equal(call(q), want)
+
+
 def test_two_calls_at_once():
     """On two streams, prompts and shared prefixes beside each other: each result is what it is alone."""
     from retrievalattention_b200 import paged
