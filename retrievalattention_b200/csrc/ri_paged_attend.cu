@@ -356,50 +356,99 @@ struct Sight {
   }
 };
 
-// The rows of `bad` once more, one after the other, over the slots of this segment that they see and no others, in 32 bits against
-// the same reference: row i of the warp is lane i's.  `half`: 0 or 1, write these 64 channels; -1: all.
+// The rows of `bad`, some of whose outputs came out NaN, one after the other: row i of the warp is lane i's, a lane has four channels.
+// What a row sees decides: a channel is NaN or infinite where a slot that the row sees is, and the walk over V ends as soon as NaN is all
+// that is left to be found.  Channels that nothing of the kind explains were spoilt by slots that the row does not see; it is done
+// again over those that it sees and no others, in 32 bits against the same reference.  32768 tokens, a NaN in the first slot's value: 13 ms,
+// 8.6 s with every row done again.  A slot at a time, as more would take registers that the caller needs.  `half`: 0 or 1, write these 64
+// channels; -1: all.
 template <int DT>
 __device__ __noinline__ void redo(const Args& a, const Segment& sg, unsigned bad, Sight sight, int row, int q_row, float m, float f, int half) {
   const int lane = threadIdx.x & 31, n_rows = sg.n_tok * a.gs;
+  auto four = [&](const uint16_t* p, float (&x)[4]) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p + lane * 4);
+    x[0] = Elem<DT>::from_bits((uint16_t)(u.x & 0xffffu)); x[1] = Elem<DT>::from_bits((uint16_t)(u.x >> 16));
+    x[2] = Elem<DT>::from_bits((uint16_t)(u.y & 0xffffu)); x[3] = Elem<DT>::from_bits((uint16_t)(u.y >> 16));
+  };
   while (bad) {
     const int src = __ffs(bad) - 1;
     bad &= bad - 1;
     const Sight see = {__shfl_sync(0xffffffffu, sight.low, src), __shfl_sync(0xffffffffu, sight.high, src), __shfl_sync(0xffffffffu, sight.sink, src)};
     const int r = __shfl_sync(0xffffffffu, row, src), tok = __shfl_sync(0xffffffffu, q_row, src);
     const float ref = __shfl_sync(0xffffffffu, m, src), factor = __shfl_sync(0xffffffffu, f, src);
-    const int h = sg.head * a.gs + r % a.gs;
-    auto four = [&](const uint16_t* p, float (&x)[4]) {
-      const uint2 u = *reinterpret_cast<const uint2*>(p + lane * 4);
-      x[0] = Elem<DT>::from_bits((uint16_t)(u.x & 0xffffu)); x[1] = Elem<DT>::from_bits((uint16_t)(u.x >> 16));
-      x[2] = Elem<DT>::from_bits((uint16_t)(u.y & 0xffffu)); x[3] = Elem<DT>::from_bits((uint16_t)(u.y >> 16));
+    const int h = sg.head * a.gs + r % a.gs, end = min((sg.step + sg.n) * kTile, see.high);
+    const bool mine = half < 0 || (lane >> 4) == half;     // this lane's channels are this warp's
+    uint2* out = reinterpret_cast<uint2*>(a.out + ((int64_t)tok * a.hk * a.gs + h) * RI_HEAD_DIM) + lane;
+    float4* part = reinterpret_cast<float4*>(a.part_o + (int64_t)max(sg.part, 0) * RI_HEAD_DIM) + ((lane >> 1) * n_rows + r) * 2 + (lane & 1);
+    // place `at` of K or V, of this row's head
+    auto row_at = [&](const void* pool, int64_t stride, int at) {
+      const int slot = slot_of(at, sg.front, sg.skip), id = page_of(a, sg.table_row, slot >> a.shift);
+      return static_cast<const uint16_t*>(pool) + id * stride + ((int64_t)(sg.head << a.shift) + (slot & ((1 << a.shift) - 1))) * RI_HEAD_DIM;
     };
-    float q[4], k[4], v[4], o[4] = {0.f, 0.f, 0.f, 0.f};
+    auto seen = [&](int at) { return at >= see.low || at < see.sink; };
+    float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, was[4] = {0.f, 0.f, 0.f, 0.f};
     four(a.q + (int64_t)tok * a.q_stride + h * RI_HEAD_DIM, q);
-    for (int at = sg.step * kTile; at < min((sg.step + sg.n) * kTile, see.high); ++at) {
-      if (at >= see.low || at < see.sink) {
-        const int slot = slot_of(at, sg.front, sg.skip), id = page_of(a, sg.table_row, slot >> a.shift);
-        const int64_t in_page = ((int64_t)(sg.head << a.shift) + (slot & ((1 << a.shift) - 1))) * RI_HEAD_DIM;
-        four(static_cast<const uint16_t*>(a.keys) + id * a.key_stride + in_page, k);
-        four(static_cast<const uint16_t*>(a.values) + id * a.value_stride + in_page, v);
-        float s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
+    if (mine) {                                            // what the owner of the row has just written
+      if (sg.part < 0) {
+        const uint2 u = *out;
+        was[0] = Elem<DT>::from_bits((uint16_t)(u.x & 0xffffu)); was[1] = Elem<DT>::from_bits((uint16_t)(u.x >> 16));
+        was[2] = Elem<DT>::from_bits((uint16_t)(u.y & 0xffffu)); was[3] = Elem<DT>::from_bits((uint16_t)(u.y >> 16));
+      } else {
+        const float4 u = *part;
+        was[0] = u.x; was[1] = u.y; was[2] = u.z; was[3] = u.w;
+      }
+    }
+    auto score = [&](const float (&k)[4]) {
+      float s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
 #pragma unroll
-        for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-        s *= a.scale2;
-        if (s == -INFINITY) continue;
-        const float p = fmaxf(exp2f(s - ref), 1.17549435e-38f);      // an infinite value is one however little it counts
-        const float weight = s == s ? p : s;
+      for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+      return s * a.scale2;
+    };
+    bool open = true;                                      // some NaN is not explained yet
+    for (int at = sg.step * kTile; open && at < end; ++at) {
+      if (!seen(at)) continue;
+      float v[4];
+      four(row_at(a.values, a.value_stride, at), v);
+      bool odd = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) odd |= !(fabsf(v[e]) < INFINITY);
+      if (!__any_sync(0xffffffffu, odd)) continue;
+      float k[4];
+      four(row_at(a.keys, a.key_stride, at), k);
+      if (score(k) == -INFINITY) continue;
+      bool left = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (!(fabsf(v[e]) < INFINITY)) o[e] += v[e];       // an infinite value is one however little it counts
+        left |= was[e] != was[e] && o[e] == o[e];
+      }
+      open = __any_sync(0xffffffffu, left);
+    }
+    bool spoilt = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      spoilt |= was[e] != was[e] && fabsf(o[e]) < INFINITY;
+      if (was[e] == was[e]) o[e] = was[e];                 // right as it is
+    }
+    if (__any_sync(0xffffffffu, spoilt)) {
+      o[0] = o[1] = o[2] = o[3] = 0.f;
+      for (int at = sg.step * kTile; at < end; ++at) {
+        if (!seen(at)) continue;
+        float k[4], v[4];
+        four(row_at(a.keys, a.key_stride, at), k);
+        const float x = score(k);
+        if (x == -INFINITY) continue;
+        four(row_at(a.values, a.value_stride, at), v);
+        const float p = fmaxf(exp2f(x - ref), 1.17549435e-38f), weight = x == x ? p : x;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] += weight * v[e];
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] *= factor;
     }
-    if (half >= 0 && (lane >> 4) != half) continue;
-    if (sg.part < 0) {
-      const uint2 u = make_uint2(Elem<DT>::pack2(o[0] * factor, o[1] * factor), Elem<DT>::pack2(o[2] * factor, o[3] * factor));
-      *reinterpret_cast<uint2*>(a.out + ((int64_t)tok * a.hk * a.gs + h) * RI_HEAD_DIM + lane * 4) = u;
-    } else {
-      reinterpret_cast<float4*>(a.part_o + (int64_t)sg.part * RI_HEAD_DIM)[((lane >> 1) * n_rows + r) * 2 + (lane & 1)] =
-          make_float4(o[0], o[1], o[2], o[3]);
-    }
+    if (!mine) continue;
+    if (sg.part < 0) *out = make_uint2(Elem<DT>::pack2(o[0], o[1]), Elem<DT>::pack2(o[2], o[3]));
+    else *part = make_float4(o[0], o[1], o[2], o[3]);
   }
 }
 

@@ -146,6 +146,32 @@ def test_infinite_and_nan_values_that_a_row_does_not_see(count, held, window, si
             assert torch.equal(torch.isnan(got[r][:, heads, 9]), nan9[r, None].expand(-1, 4))
 
 
+def test_infinities_of_both_signs_and_a_slot_that_counts_nothing():
+    """+infinity and -infinity in a channel make NaN of it, one of them itself; a slot of score -infinity hands on nothing."""
+    from retrievalattention_b200 import paged
+
+    for held in (0, 4000):
+        n = 100 + held
+        layer = Layer([n], 1, 16, torch.bfloat16, seed=8)
+        k, v = layer.k[0].clone(), layer.v[0].clone()
+        at = held // 2 + 3
+        v[:, at, 0], v[:, at + 1, 0] = INF, -INF
+        v[:, at, 1], v[:, at + 2, 2] = INF, -INF
+        k[:, at + 4], k[:, at + 4, 0] = 0.0, -INF
+        v[:, at + 4, 3], v[:, at + 4, 4] = INF, float("nan")
+        layer.fill(0, k.float(), v.float(), layer.w[0].float(), layer.t[0])
+        q = torch.randn((100, 4, DIM), generator=torch.Generator().manual_seed(1)).abs().to(torch.bfloat16).cuda()
+        out = paged.paged_prompt(q, layer.keys, layer.values, layer.table, layer.lengths, torch.tensor([0, 100], dtype=torch.int32, device="cuda"))
+        own = torch.arange(held, n)
+        late = own >= at + 4
+        assert torch.isnan(out[late][..., 0]).all() and (out[late][..., 1] == INF).all() and (out[late][..., 2] == -INF).all()
+        finite = torch.isfinite(k).all(-1)[0] & torch.isfinite(v).all(-1)[0] | (torch.arange(n) == at) | (torch.arange(n) == at + 1) | (torch.arange(n) == at + 2)
+        seen = visible(own, n, None, 0) & finite
+        kc = torch.where(torch.isfinite(k), k, torch.zeros_like(k))
+        want = attend_rows(q.cpu().double(), kc, v, seen)
+        assert close(out[..., 3:], None, *(x[..., 3:] if x.dim() == 3 else x for x in want))
+
+
 def test_scores_of_minus_infinity():
     """Keys that no finite query goes with: such slots count nothing, a row of nothing else is zeros."""
     layer = Layer([140], 1, 16, torch.bfloat16, seed=8)
