@@ -10,7 +10,11 @@
 // tiles and a KV head; it walks the boxes (of a page, at most 128 slots) that its rows may see, its first slots' and then its window's,
 // 128 slots a step.  Boxes that no row sees are not read but filled with zeros.
 //   S_g = Q_g.K^T     M 128 x N 128 x K 128, both operands by TMA with the 128-byte swizzle, pages through the page table;
-//   softmax           a thread per query row (= TMEM lane), online, against a lazy reference maximum; P goes back over S as 16-bit pairs;
+//   softmax           a thread per query row (= TMEM lane), online, against a lazy reference maximum; P goes back over S as 16-bit pairs.
+//                     Prompts: one part, rounded (8 bits of bf16, 11 of fp16), as in ri_prefill_attn.cu: a second one makes half of a step's
+//                     products twice as many.  Against 64 bits the outputs are 2.2e-3 off where the rounding of the result alone gives 1.65e-3
+//                     (fp16 2.6e-4 and 2.0e-4).  What requests have in common: two parts, as ri_paged_decode.cu has for requests that are
+//                     attended one by one, so that what a request gets does not hang on which of the two the call takes;
 //   O_g += P_g.V      A from TMEM, B the V tile as it lies (MN-major), the accumulator in TMEM for the whole walk.
 // Items of two tiles: a group of four softmax warps for each, which share every tile of K and V.  Items of one tile: the groups take
 // its even and its odd steps, and join what they have at the end.
@@ -49,6 +53,7 @@ constexpr int kThreads = 384;
 constexpr int kSegments = 4;               // segments on their way from the warp that hands them out
 constexpr int kTails = 4;                 // V tiles in the ring that a request's slots end in: it holds three V tiles
 constexpr uint32_t kTmemCols = 512;
+constexpr int kLowPart = kTile / 2;        // SHARED: columns of S_g that the probabilities' second parts begin at
 constexpr int kMaxCtas = 160;
 constexpr int kMaxRequests = 16384;        // of a call, or groups
 constexpr int kMaxEntries = 8192;          // of the table of steps
@@ -599,8 +604,11 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       auto issue_pv = [&](int g, int tile, int k0, bool first) {
         const uint64_t db = umma_desc_mn_sw128(sKV + tile * 2 * kHalf, kHalf);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < 4; ++k) {
           mma_ts_by(one, tmem_u + (2 + g) * kTile, tmem_u + g * kTile + 8 * (k0 + k), db + 128 * (k0 + k), a.idesc_pv, !first || (k0 + k) != 0);
+          if (SHARED)
+            mma_ts_by(one, tmem_u + (2 + g) * kTile, tmem_u + g * kTile + kLowPart + 8 * (k0 + k), db + 128 * (k0 + k), a.idesc_pv, 1u);
+        }
       };
       auto issue_qk = [&](int g, int q, int tile) {
 #pragma unroll
@@ -951,7 +959,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          uint32_t pw[16];
+          uint32_t pw[16], low[16];
 #pragma unroll
           for (int y = 0; y < 16; ++y) {
             const uint64_t e = fma_f2(pack_f2(__uint_as_float(sr[x][2 * y]), __uint_as_float(sr[x][2 * y + 1])), scale_2, neg_m);
@@ -960,8 +968,10 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             const float p0 = ex2(e0), p1 = ex2(e1);
             sum2[y & 1] = add_f2(sum2[y & 1], pack_f2(p0, p1));
             pw[y] = Elem<DT>::pack2(p0, p1);
+            if (SHARED) low[y] = Elem<DT>::pack2(p0 - Elem<DT>::from_bits((uint16_t)(pw[y] & 0xffffu)), p1 - Elem<DT>::from_bits((uint16_t)(pw[y] >> 16)));
           }
           tc_st16(tmem_s + x * 16, pw);
+          if (SHARED) tc_st16(tmem_s + kLowPart + x * 16, low);
           if (x == 1) {          // the product over the first 64 slots may start
             tc_wait_st();
             tc_fence_before();
