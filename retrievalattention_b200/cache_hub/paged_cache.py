@@ -71,7 +71,9 @@ class paged_cache(KV_Cache):
         # slots in use and tokens so far in front of the step's rows, and with them
         self.held, self.lengths = (zeros(batch_size, kind=torch.int32) for _ in range(2))
         self.seen, self.seen_after = (zeros(batch_size, kind=torch.int32) for _ in range(2))
-        self.row_start = None                                   # of the step's rows; None: one row of every request
+        # of the step's rows, in one place, so that captured calls follow it; row_start None: one row of every request
+        self._one_each = torch.arange(batch_size + 1, dtype=torch.int32, device=self.device)
+        self._row_start, self.row_start = self._one_each.clone(), None
         self.length_of = [0] * batch_size                       # `lengths` on the host
         self._free = list(range(self.num_pages - 1, -1, -1))
         self._pages = [[] for _ in range(batch_size)]
@@ -83,7 +85,6 @@ class paged_cache(KV_Cache):
         # group_start and shared of `paged.paged_shared_decode`, as many groups as requests, so that captured calls follow them
         self._group_start, self._group_shared = zeros(batch_size + 1, kind=torch.int32), zeros(batch_size, kind=torch.int32)
         self._alike = False                                     # some requests have slots in common
-        self._one_each = torch.arange(batch_size + 1, dtype=torch.int32, device=self.device)      # row_start of a row of every request
 
     def _to_device(self, values) -> torch.Tensor:
         return torch.tensor(values, dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
@@ -123,26 +124,32 @@ class paged_cache(KV_Cache):
             self.lengths.add_(more)
             self.seen_after.add_(more)
         if same and counts == 1:
+            if self.row_start is not None:
+                self._row_start.copy_(self._one_each)
             self.row_start = None
         else:
             starts = [0]
             for n in each:
                 starts.append(starts[-1] + n)
-            self.row_start = self._to_device(starts)
+            self._row_start.copy_(self._to_device(starts))
+            self.row_start = self._row_start
         self.context += max(each)
 
     def append(self, layer_idx, qkv, cos_sin, positions, axis_of, q, keys=None, values=None, q_norm=None, k_norm=None, eps=1e-6) -> None:
         """The step's rows of a layer: normalise heads where weights are given, rotate, split, and write to the pages
-        (``paged.rope_paged_append``)."""
+        (``paged.rope_paged_append``).  A captured call goes by the rows that later steps' ``begin`` shares out."""
         paged.rope_paged_append(qkv, cos_sin, positions, axis_of, q, self.key_pages[layer_idx], self.value_pages[layer_idx],
-                                self.page_table, self.held, self.row_start, weight=self.weight[layer_idx],
+                                self.page_table, self.held, self._row_start if self._captures() else self.row_start, weight=self.weight[layer_idx],
                                 token=self.token[layer_idx], seen=self.seen, keys=keys, values=values, q_norm=q_norm, k_norm=k_norm,
                                 eps=eps)
+
+    def _captures(self) -> bool:
+        return self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()
 
     def _of(self, requests):
         """Page table and lengths, of all requests or of some; the layers of a step share them.  A captured call is replayed in later
         steps, whose requests may be longer: it takes the whole table."""
-        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        if self._captures():
             if requests is not None:
                 raise RuntimeError("calls over some of the requests cannot be captured: which ones is known on the host")
             return self.page_table, self.lengths
@@ -179,8 +186,7 @@ class paged_cache(KV_Cache):
         if any(e and n for e, n in zip(self._evicted, self._fed)):
             raise RuntimeError("slots of a request were evicted: what its rows see is not known any more")
         table, lengths = self._of(None)
-        starts = self._one_each if self.row_start is None else self.row_start
-        return paged.paged_prompt(query_states, self.key_pages[layer_idx], self.value_pages[layer_idx], table, lengths, starts,
+        return paged.paged_prompt(query_states, self.key_pages[layer_idx], self.value_pages[layer_idx], table, lengths, self._row_start,
                                   window=self.attn_window[layer_idx], sink=self.attn_sink, out=out, lse=lse)
 
     def share(self, of: int, requests, slots: int | None = None) -> int:
