@@ -23,7 +23,7 @@
 // TMEM: S_0 | S_1 | O_0 | O_1.  Warps: TMA producer, MMA issuer, the one that hands out segments (the part of an item that falls to the
 // CTA), one that clears what lies behind a request's last slot, eight softmax warps.  Every wait is bounded; one that runs out is recorded in the status word.
 // A tile's slots that a row does not see have a probability of 0, and what they hold is finite where it was written as such; where it
-// was not, 0 * infinity leaves a NaN, and the row is done again over what it sees (`redo`).  Slots behind a request's last one may
+// was not, 0 * infinity leaves a NaN, and the segment is done once more (kAgain).  Slots behind a request's last one may
 // hold anything: they are zeros in shared memory before the product.
 // B200, bf16, 8 heads of 4, one prompt: 8192 tokens 505 us over all slots (the dense prompt kernel: 455), 261 over a window of 2048, 61
 // over one of 128; 32768 tokens over 2048 1.23 to 1.36 ms (2.1 PFLOP over what is seen, 650 us at the cuBLAS rate).  What bounds it: a
@@ -67,6 +67,13 @@ constexpr int kItemCost = 2;
 // Of a CTA, over what groups have in common: more parts of an item than that are slower to join than they are to make (one KV head of 8,
 // 32768 slots: 148 parts 52 us, 65 parts 35; 2 x 6016 slots of 4 heads 51 and 48).
 constexpr int kLeastCost = 4;
+// Where a row's outputs come out NaN while its sum is a number, a slot that it does not see, or gives a probability that vanishes, holds a
+// NaN or an infinity.  The segments that this happened to are done once more, behind the CTA's last one, over tiles of V in which all that
+// is not finite has been made 0; the softmax warps look up what it was, where a row's score says that the slot counts.  So what lies in
+// the cache makes no call more than some ten times as long, and no wait of the pipeline long.  8192 tokens of 8 heads of 4 over all slots:
+// 0.54 ms; with a NaN in the value of slot 4000 1.6, of slot 8100 1.1, in all values 1.8, an infinity in one channel of every slot 5.6.
+// Window 1024 with four first slots, infinities behind those in their page: 0.19 and 0.50.
+constexpr int kAgain = 1024;               // bits; segment i has the i-th modulo that: a second time is right for any
 constexpr int kHeadsMost = 8;              // query heads of a KV head
 constexpr int kMeta = 8;                   // ints that a CTA leaves for the kernel that joins
 
@@ -82,7 +89,7 @@ struct Segment {
   int end;                                 // the place behind the request's last slot
   int slot0;                               // ri_paged_prompt: the first token's slot
   int part;                                // rows of partial results in front of this segment's, -1: the item is whole
-  int pad;
+  int clean;                               // 0, or 1 + what of K and V was loaded before, in tiles modulo 2 kRing: see kAgain
   __device__ __forceinline__ int steps(int g) const { return two ? n : (n + 1 - g) >> 1; }      // of group g, and its j-th one
   __device__ __forceinline__ int nth(int g, int j) const { return step + (two ? j : 2 * j + g); }
 };
@@ -95,6 +102,9 @@ struct Control {
   int scan[kThreads / 32 + 1];
   int begin[4], end[4];                    // where the CTA's range begins and ends: head, sequence, pair of tiles, step
   int first;                               // the first sequence with rows
+  uint32_t again[kAgain / 32];             // segments that are done once more
+  int any_again;
+  uint32_t odd[kRing][kTile / 32];         // done once more: rows of the tile of V that held something else than numbers
   uint32_t tmem;
   int abort;
 };
@@ -361,100 +371,227 @@ struct Sight {
   }
 };
 
-// The rows of `bad`, some of whose outputs came out NaN, one after the other: row i of the warp is lane i's, a lane has four channels.
-// What a row sees decides: a channel is NaN or infinite where a slot that the row sees is, and the walk over V ends as soon as NaN is all
-// that is left to be found.  Channels that nothing of the kind explains were spoilt by slots that the row does not see; it is done
-// again over those that it sees and no others, in 32 bits against the same reference.  32768 tokens, a NaN in the first slot's value: 13 ms,
-// 8.6 s with every row done again.  A slot at a time, as more would take registers that the caller needs.  `half`: 0 or 1, write these 64
-// channels; -1: all.
+// ---- segments that are done once more ------------------------------------------------------------------------------------
 template <int DT>
-__device__ __noinline__ void redo(const Args& a, const Segment& sg, unsigned bad, Sight sight, int row, int q_row, float m, float f, int half) {
-  const int lane = threadIdx.x & 31, n_rows = sg.n_tok * a.gs;
-  auto four = [&](const uint16_t* p, float (&x)[4]) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p + lane * 4);
-    x[0] = Elem<DT>::from_bits((uint16_t)(u.x & 0xffffu)); x[1] = Elem<DT>::from_bits((uint16_t)(u.x >> 16));
-    x[2] = Elem<DT>::from_bits((uint16_t)(u.y & 0xffffu)); x[3] = Elem<DT>::from_bits((uint16_t)(u.y >> 16));
+struct Exponent {
+  static constexpr uint32_t kAll = DT == RI_BF16 ? 0x7f80u : 0x7c00u;      // of a NaN or an infinity
+};
+// Eight values; what is not finite becomes 0.  Whether there was any.
+template <int DT>
+__device__ __forceinline__ bool make_finite(uint4& x) {
+  constexpr uint32_t kBoth = Exponent<DT>::kAll * 0x10001u;
+  auto odd = [](uint32_t& u) {
+    const uint32_t m = __vcmpeq2(u & kBoth, kBoth);
+    u &= ~m;
+    return m;
   };
-  while (bad) {
-    const int src = __ffs(bad) - 1;
-    bad &= bad - 1;
-    const Sight see = {__shfl_sync(0xffffffffu, sight.low, src), __shfl_sync(0xffffffffu, sight.high, src), __shfl_sync(0xffffffffu, sight.sink, src)};
-    const int r = __shfl_sync(0xffffffffu, row, src), tok = __shfl_sync(0xffffffffu, q_row, src);
-    const float ref = __shfl_sync(0xffffffffu, m, src), factor = __shfl_sync(0xffffffffu, f, src);
-    const int h = sg.head * a.gs + r % a.gs, end = min((sg.step + sg.n) * kTile, see.high);
-    const bool mine = half < 0 || (lane >> 4) == half;     // this lane's channels are this warp's
-    uint2* out = reinterpret_cast<uint2*>(a.out + ((int64_t)tok * a.hk * a.gs + h) * RI_HEAD_DIM) + lane;
-    float4* part = reinterpret_cast<float4*>(a.part_o + (int64_t)max(sg.part, 0) * RI_HEAD_DIM) + ((lane >> 1) * n_rows + r) * 2 + (lane & 1);
-    // place `at` of K or V, of this row's head
-    auto row_at = [&](const void* pool, int64_t stride, int at) {
-      const int slot = slot_of(at, sg.front, sg.skip), id = page_of(a, sg.table_row, slot >> a.shift);
-      return static_cast<const uint16_t*>(pool) + id * stride + ((int64_t)(sg.head << a.shift) + (slot & ((1 << a.shift) - 1))) * RI_HEAD_DIM;
-    };
-    auto seen = [&](int at) { return at >= see.low || at < see.sink; };
-    float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, was[4] = {0.f, 0.f, 0.f, 0.f};
-    four(a.q + (int64_t)tok * a.q_stride + h * RI_HEAD_DIM, q);
-    if (mine) {                                            // what the owner of the row has just written
-      if (sg.part < 0) {
-        const uint2 u = *out;
-        was[0] = Elem<DT>::from_bits((uint16_t)(u.x & 0xffffu)); was[1] = Elem<DT>::from_bits((uint16_t)(u.x >> 16));
-        was[2] = Elem<DT>::from_bits((uint16_t)(u.y & 0xffffu)); was[3] = Elem<DT>::from_bits((uint16_t)(u.y >> 16));
-      } else {
-        const float4 u = *part;
-        was[0] = u.x; was[1] = u.y; was[2] = u.z; was[3] = u.w;
-      }
-    }
-    auto score = [&](const float (&k)[4]) {
-      float s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
+  return (odd(x.x) | odd(x.y) | odd(x.z) | odd(x.w)) != 0;
+}
+// Which channels a row gets +infinity (words 0 to 3), -infinity (4 to 7) or, with both, NaN from; channel 4 i + e is bit i of word e.
+// Of the step's slots `odd` (a bit for each of 128), those whose score is more than -infinity count, however little; eight of them at a
+// time, for their values' way here.  A row all of whose channels are NaN learns nothing more.
+template <int DT>
+__device__ __noinline__ void note_odd(const Args& a, const Segment& sg, const uint32_t* odd, uint32_t tmem_s, int place, uint32_t* got) {
+  constexpr int kTogether = 8;
+  const int lane = threadIdx.x & 31;
+  const uint16_t* head = static_cast<const uint16_t*>(a.values) + ((int64_t)sg.head << a.shift) * RI_HEAD_DIM + 4 * lane;
+  uint32_t sum[8];
 #pragma unroll
-      for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-      return s * a.scale2;
-    };
-    bool open = true;                                      // some NaN is not explained yet
-    for (int at = sg.step * kTile; open && at < end; ++at) {
-      if (!seen(at)) continue;
-      float v[4];
-      four(row_at(a.values, a.value_stride, at), v);
-      bool odd = false;
+  for (int i = 0; i < 8; ++i) sum[i] = got[i];
+#pragma unroll 1
+  for (int x = 0; x < kTile / 32; ++x) {
+    const uint32_t here = odd[x];
+    if (!__any_sync(0xffffffffu, here != 0)) continue;
+    uint32_t part[32], counts = 0;
+    tc_ld32(tmem_s + x * 32, part);
+    tc_wait_ld();
+    tc_ld_landed(part);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) odd |= !(fabsf(v[e]) < INFINITY);
-      if (!__any_sync(0xffffffffu, odd)) continue;
-      float k[4];
-      four(row_at(a.keys, a.key_stride, at), k);
-      if (score(k) == -INFINITY) continue;
-      bool left = false;
+    for (int y = 0; y < 32; ++y)
+      if (__uint_as_float(part[y]) * a.scale2 != -INFINITY) counts |= 1u << y;
+    const uint32_t all = sum[0] & sum[1] & sum[2] & sum[3] & sum[4] & sum[5] & sum[6] & sum[7];
+    counts = all == 0xffffffffu ? 0u : counts & here;
+    uint32_t left = __reduce_or_sync(0xffffffffu, counts);
+    const int slot = slot_of(place + x * 32 + lane, sg.front, sg.skip), row = slot & ((1 << a.shift) - 1);      // of this lane's place
+    const int id = left & (1u << lane) ? page_of(a, sg.table_row, slot >> a.shift) : 0;
+    while (left != 0) {
+      uint32_t bit[kTogether];
+      uint2 u[kTogether];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (!(fabsf(v[e]) < INFINITY)) o[e] += v[e];       // an infinite value is one however little it counts
-        left |= was[e] != was[e] && o[e] == o[e];
-      }
-      open = __any_sync(0xffffffffu, left);
-    }
-    bool spoilt = false;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      spoilt |= was[e] != was[e] && fabsf(o[e]) < INFINITY;
-      if (was[e] == was[e]) o[e] = was[e];                 // right as it is
-    }
-    if (__any_sync(0xffffffffu, spoilt)) {
-      o[0] = o[1] = o[2] = o[3] = 0.f;
-      for (int at = sg.step * kTile; at < end; ++at) {
-        if (!seen(at)) continue;
-        float k[4], v[4];
-        four(row_at(a.keys, a.key_stride, at), k);
-        const float x = score(k);
-        if (x == -INFINITY) continue;
-        four(row_at(a.values, a.value_stride, at), v);
-        const float p = fmaxf(exp2f(x - ref), 1.17549435e-38f), weight = x == x ? p : x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] += weight * v[e];
+      for (int k = 0; k < kTogether; ++k) {
+        bit[k] = left & (0u - left);
+        left ^= bit[k];
+        const int of = __ffs(bit[k] != 0 ? bit[k] : bit[0]) - 1;
+        u[k] = *reinterpret_cast<const uint2*>(head + __shfl_sync(0xffffffffu, id, of) * a.value_stride + __shfl_sync(0xffffffffu, row, of) * RI_HEAD_DIM);
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] *= factor;
+      for (int k = 0; k < kTogether; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t v = ((e < 2 ? u[k].x : u[k].y) >> (16 * (e & 1))) & 0xffffu, size = v & 0x7fffu;
+          const bool nan = size > Exponent<DT>::kAll, inf = size == Exponent<DT>::kAll;
+          const uint32_t plus = __ballot_sync(0xffffffffu, nan || (inf && v == size)), minus = __ballot_sync(0xffffffffu, nan || (inf && v != size));
+          if (counts & bit[k]) {
+            sum[e] |= plus;
+            sum[4 + e] |= minus;
+          }
+        }
     }
-    if (!mine) continue;
-    if (sg.part < 0) *out = make_uint2(Elem<DT>::pack2(o[0], o[1]), Elem<DT>::pack2(o[2], o[3]));
-    else *part = make_float4(o[0], o[1], o[2], o[3]);
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) got[i] = sum[i];
+}
+// Puts them into the row's accumulator, whose products are done.
+__device__ __noinline__ void put_odd(uint32_t tmem_o, const uint32_t* got) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) any |= got[i];
+  if (!__any_sync(0xffffffffu, any != 0)) return;
+#pragma unroll 1
+  for (int x = 0; x < 4; ++x) {
+    uint32_t o[32];
+    tc_ld32(tmem_o + x * 32, o);
+    tc_wait_ld();
+    tc_ld_landed(o);
+#pragma unroll
+    for (int y = 0; y < 32; ++y) {
+      const uint32_t bit = 1u << (8 * x + y / 4);
+      const bool plus = got[y & 3] & bit, minus = got[4 + (y & 3)] & bit;
+      if (plus || minus) o[y] = plus && minus ? 0x7fffffffu : (plus ? 0x7f800000u : 0xff800000u);
+    }
+    tc_st32(tmem_o + x * 32, o);
+  }
+  tc_wait_st();
+}
+
+// ---- softmax of a segment's steps, by the warp that has the rows ---------------------------------------------------------
+// l_run and m_ref become a row's sum and the reference that it and the outputs go by; `phase`: of the scores' barrier.  False: it gave up.
+// The reference follows the running maximum in steps of more than 2^kLazy, kAbove below it: fp16's short exponent then holds
+// probabilities down to 2^-(24 + kAbove) of the largest, which are at most 2^(kAbove + kLazy).
+template <int DT, bool SHARED, bool CLEAN>
+__device__ __forceinline__ bool softmax_steps(const Args& a, Control& s, const Segment& sg, const Sight& sight, uint32_t tmem_s, uint32_t tmem_o,
+                                              int grp, uint32_t phase, float& m_ref, float& l_run, uint32_t* got) {
+  constexpr float kLazy = 4.f, kAbove = DT == RI_F16 ? 10.f : 0.f;
+  const int lane = threadIdx.x & 31;
+  const uint32_t bars = smem_u32(s.bars);
+  volatile int* abort_flag = &s.abort;
+  const uint64_t scale_2 = pack_f2(a.scale2, a.scale2);
+  for (int j = 0; j < sg.steps(grp); ++j) {
+    const int place = sg.nth(grp, j) * kTile;
+    if (!__all_sync(0xffffffffu, mbar_wait(bars + 8u * (4 + grp), (phase ^ j) & 1, abort_flag, 11))) return false;
+    tc_fence_after();
+    // Columns that are not seen become -infinity where they lie, 32 at a time: a tile's few tokens begin and end seeing close together,
+    // so most of four times 32 columns are seen by all rows of a warp, and a loop is a quarter of the instructions.
+    if (__any_sync(0xffffffffu, !sight.all_of(place))) {
+#pragma unroll 1
+      for (int x = 0; x < 4; ++x) {
+        const uint32_t seen = sight.mask(place + x * 32);
+        if (!__any_sync(0xffffffffu, seen != 0xffffffffu)) continue;
+        uint32_t part[32];
+        tc_ld32(tmem_s + x * 32, part);
+        tc_wait_ld();
+        tc_ld_landed(part);
+#pragma unroll
+        for (int y = 0; y < 32; ++y)
+          if (!(seen & (1u << y))) part[y] = 0xff800000u;      // -inf
+        tc_st32(tmem_s + x * 32, part);
+      }
+      tc_wait_st();
+    }
+    if constexpr (CLEAN) {                               // what the step's tile of V held is known once it is clean
+      const int tile = sg.clean + 2 * (sg.nth(grp, j) - sg.step), at = tile % kRing;
+      if (!__all_sync(0xffffffffu, mbar_wait(bars + 8u * (14 + kTails + at), (tile / kRing) & 1, abort_flag, 11))) return false;
+      note_odd<DT>(a, sg, s.odd[at], tmem_s, place, got);
+    }
+    uint32_t sr[4][32];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) tc_ld32(tmem_s + x * 32, sr[x]);
+    tc_wait_ld();
+#pragma unroll
+    for (int x = 0; x < 4; ++x) tc_ld_landed(sr[x]);
+
+    float mx[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      mx[x] = fmaxf(__uint_as_float(sr[x][0]), __uint_as_float(sr[x][1]));
+#pragma unroll
+      for (int y = 2; y < 32; y += 2) mx[x] = max3(mx[x], __uint_as_float(sr[x][y]), __uint_as_float(sr[x][y + 1]));
+    }
+    const float m_tile = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * a.scale2 - kAbove;
+    const bool move = m_tile > m_ref + kLazy;              // also true for the first finite tile (m_ref = -inf)
+    if (__any_sync(0xffffffffu, move)) {
+      // the warp's accumulator rows are multiplied anyway, so every row of it catches up with its maximum
+      const float m_new = fmaxf(m_ref, m_tile);
+      const float factor = m_ref == -INFINITY ? 0.f : exp2f(m_ref - m_new);      // 1 when the maximum stays
+      l_run *= factor;
+      m_ref = m_new;
+      if (j > 0) {                                         // rare: bring this warp's rows of O to the new reference
+#pragma unroll 1
+        for (int x = 0; x < 4; ++x) {
+          uint32_t orow[32];
+          tc_ld32(tmem_o + x * 32, orow);
+          tc_wait_ld();
+          tc_ld_landed(orow);
+#pragma unroll
+          for (int y = 0; y < 32; ++y) orow[y] = __float_as_uint(__uint_as_float(orow[y]) * factor);
+          tc_st32(tmem_o + x * 32, orow);
+        }
+      }
+    }
+    // probabilities p = 2^(s * scale - m), packed as the 16-bit operand of the second product: word y of the row = slots 2y, 2y+1
+    const float ref = m_ref == -INFINITY ? 0.f : m_ref;
+    const uint64_t neg_m = pack_f2(-ref, -ref);
+    uint64_t sum2[2] = {0ull, 0ull};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      uint32_t pw[16], low[16];
+#pragma unroll
+      for (int y = 0; y < 16; ++y) {
+        const uint64_t e = fma_f2(pack_f2(__uint_as_float(sr[x][2 * y]), __uint_as_float(sr[x][2 * y + 1])), scale_2, neg_m);
+        float e0, e1;
+        unpack_f2(e, e0, e1);
+        const float p0 = ex2(e0), p1 = ex2(e1);
+        sum2[y & 1] = add_f2(sum2[y & 1], pack_f2(p0, p1));
+        pw[y] = Elem<DT>::pack2(p0, p1);
+        if (SHARED) low[y] = Elem<DT>::pack2(p0 - Elem<DT>::from_bits((uint16_t)(pw[y] & 0xffffu)), p1 - Elem<DT>::from_bits((uint16_t)(pw[y] >> 16)));
+      }
+      tc_st16(tmem_s + x * 16, pw);
+      if (SHARED) tc_st16(tmem_s + kLowPart + x * 16, low);
+      if (x == 1) {          // the product over the first 64 slots may start
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars + 8u * (6 + grp));
+      }
+    }
+    float s0, s1;
+    unpack_f2(add_f2(sum2[0], sum2[1]), s0, s1);
+    l_run += s0 + s1;
+    tc_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bars + 8u * (8 + grp));
+  }
+  return true;
+}
+// The same over clean tiles, and what those held goes into the accumulators.  Called where nothing of the ordinary steps is in registers.
+struct Sums {
+  float m, l;
+  bool ok;
+};
+template <int DT, bool SHARED>
+__device__ __noinline__ Sums clean_steps(const Args& a, Control& s, const Segment& sg, Sight sight, uint32_t tmem_s, uint32_t tmem_o, int grp,
+                                         uint32_t phases, float m_ref) {
+  Sums sums = {m_ref, 0.f, true};
+  uint32_t got[8] = {};
+  sums.ok = softmax_steps<DT, SHARED, true>(a, s, sg, sight, tmem_s, tmem_o, grp, phases & 1, sums.m, sums.l, got);
+  if (sums.ok && sg.steps(grp) > 0) {
+    sums.ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(s.bars) + 8u * (10 + grp), (phases >> (1 + grp)) & 1, &s.abort, 11));
+    tc_fence_after();
+    if (sums.ok) put_odd(tmem_o, got);
+    tc_fence_before();
+  }
+  return sums;
 }
 
 template <int DT, bool SHARED>
@@ -482,6 +619,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     // the swizzle of the tiles goes by addresses: shared memory that does not begin on a boundary of 1 KB gives up at once
     s.abort = (sQ & 1023u) ? 10 : 0;
     s.first = 0x7fffffff;
+    s.any_again = 0;
     for (int g = 0; g < 2; ++g) {
       mbar_init(bar_q(g), 1); mbar_init(bar_q_empty(g), 1); mbar_init(bar_s_full(g), 1);
       mbar_init(bar_p_part(g), 4); mbar_init(bar_p_full(g), 4); mbar_init(bar_o_full(g), 1); mbar_init(bar_join(g), 8);
@@ -491,6 +629,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     for (int i = 0; i < kTails; ++i) mbar_init(bar_tail(i), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (threadIdx.x < kAgain / 32) s.again[threadIdx.x] = 0;
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s.tmem)), "r"(kTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
@@ -514,7 +653,15 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     if (lane == 0) mbar_arrive(bar_seg_empty(i % kSegments));
   };
 
+  // Behind the last segment, once, all of them: whether there are some to be done once more.  They follow as the first ones did.
+  auto all_done = [&](int i) {
+    release(i);
+    asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+    return __any_sync(0xffffffffu, *static_cast<volatile int*>(&s.any_again) != 0 && *abort_flag == 0);
+  };
+
   if (aligned) {
+  int pass = 0;
   // registers at launch: 384 x 168; after the split 128 x 96 + 256 x 200, which is less
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
@@ -524,9 +671,13 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       const uint32_t q_bytes = (uint32_t)(a.tile_tokens * a.gs) * 256;
       int issued = 0, q_issued[2] = {0, 0}, tails = 0;
       bool ok = true;
-      for (int i = 0; ok && take(i); ++i) {
+      for (int i = 0; ok; ++i) {
+        if (!take(i)) {
+          if (pass++ == 1 || !all_done(i)) break;
+          continue;
+        }
         const Segment& sg = s.segments[i % kSegments];
-        const int first = sg.step, n = sg.n, two = sg.two, front = sg.front, skip = sg.skip;
+        const int first = sg.step, n = sg.n, two = sg.two, front = sg.front, skip = sg.skip, clean = sg.clean;
         const int head = sg.head, low = sg.low, high = sg.high, sink = sg.sink, end = sg.end;
         const int32_t* table = a.table + (int64_t)sg.table_row * a.table_stride;
         auto load_q = [&](int g) {
@@ -554,8 +705,8 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             const int at = issued % kRing;
             ok = __all_sync(0xffffffffu, mbar_wait(bar_empty(at), ((issued / kRing) & 1) ^ 1, abort_flag, 13));
             if (!ok) break;
-            // a V tile that the request's slots end in is full when what lies behind them has been cleared
-            const uint32_t bar = t == 1 && ends_in_box(end, first + j, a.shift) ? bar_tail(tails++) : bar_full(at);
+            // a V tile that the request's slots end in is full when what lies behind them has been cleared; a clean one like it
+            const uint32_t bar = t == 1 && (clean != 0 || ends_in_box(end, first + j, a.shift)) ? bar_tail(tails++) : bar_full(at);
             if (lane == 0) mbar_arrive_expect_tx(bar, 2 * kHalf);
             __syncwarp();
             if (place_of_lane < kTile)
@@ -567,6 +718,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
         release(i);
       }
+      if (pass == 0) all_done(0);
       if (*abort_flag) {     // give the copies still in flight a bounded chance to land before the CTA exits
         for (int g = 0; g < 2; ++g)
           if (q_issued[g] > 0) mbar_wait(bar_q(g), (q_issued[g] - 1) & 1, abort_flag, 14);
@@ -708,25 +860,56 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         if (!wait(bar_seg(i % kSegments), (i / kSegments) & 1, 10)) break;
         const int n = (int)__reduce_max_sync(0xffffffffu, (unsigned)s.segments[i % kSegments].n);
         const bool two = __any_sync(0xffffffffu, s.segments[i % kSegments].two);
-        if (n == 0) break;
+        if (n == 0) {
+          if (pass++ == 1 || !all_done(i)) break;
+          continue;
+        }
         release(i);
         ok = two ? two_tiles(n) : one_tile(n);
       }
+      if (pass == 0) all_done(0);
     } else if (warp == 3) {
-      // ---------------- V tiles that a request's slots end in: zeros behind them, up to the end of their box ----------------
+      // ---------------- V tiles that a request's slots end in: zeros behind them, up to the end of their box; clean tiles ----------------
       int tile0 = 0, tails = 0;
       bool ok = true;
-      for (int i = 0; ok && take(i); ++i) {
+      for (int i = 0; ok; ++i) {
+        if (!take(i)) {
+          if (pass++ == 1 || !all_done(i)) break;
+          continue;
+        }
         const int first = s.segments[i % kSegments].step, n = s.segments[i % kSegments].n, end = s.segments[i % kSegments].end;
+        const bool clean = s.segments[i % kSegments].clean != 0;
         release(i);
         for (int j = 0; j < n; ++j) {
-          if (!ends_in_box(end, first + j, a.shift)) continue;
+          if (!clean && !ends_in_box(end, first + j, a.shift)) continue;
           const int at = (tile0 + 2 * j + 1) % kRing, box = min(1 << a.shift, kTile), r0 = end - (first + j) * kTile, r1 = (r0 + box - 1) & -box;
           ok = __all_sync(0xffffffffu, mbar_wait(bar_tail(tails), (tails / kTails) & 1, abort_flag, 15));
           if (!ok) break;
           uint8_t* v = smem + 4 * kHalf + at * 2 * kHalf;
-          for (int x = r0 * 8 + lane; x < r1 * 8; x += 32)
-            for (int kb = 0; kb < 2; ++kb) *reinterpret_cast<uint4*>(v + kb * kHalf + x * 16) = make_uint4(0, 0, 0, 0);
+          if (clean) {                       // what lies behind the last slot may stay where it is finite: probabilities of 0
+#pragma unroll 1
+            for (int w = 0; w < kTile / 32; ++w) {
+              uint32_t rows = 0;
+#pragma unroll 1
+              for (int kb = 0; kb < 2; ++kb) {
+                uint4* piece = reinterpret_cast<uint4*>(v + kb * kHalf + w * 32 * 128) + lane;      // eight lanes a row
+#pragma unroll
+                for (int y = 0; y < 8; ++y) {
+                  uint4 x = piece[32 * y];
+                  const bool odd = make_finite<DT>(x);
+                  if (odd) piece[32 * y] = x;
+                  const uint32_t votes = __ballot_sync(0xffffffffu, odd);
+#pragma unroll
+                  for (int r = 0; r < 4; ++r)
+                    if ((votes >> (8 * r)) & 0xffu) rows |= 1u << (4 * y + r);
+                }
+              }
+              if (lane == 0) s.odd[at][w] = rows;
+            }
+          } else {
+            for (int x = r0 * 8 + lane; x < r1 * 8; x += 32)
+              for (int kb = 0; kb < 2; ++kb) *reinterpret_cast<uint4*>(v + kb * kHalf + x * 16) = make_uint4(0, 0, 0, 0);
+          }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_full(at));
@@ -734,17 +917,28 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
         tile0 += 2 * n;
       }
+      if (pass == 0) all_done(0);
     } else if (warp == 2) {
       // ---------------- segments ----------------
-      int given = 0;
+      int given = 0, index = 0, tiles = 0;   // the segment's number; tiles of K and V in front of it, modulo 2 kRing
       Segment sg = {};
       auto give = [&] {                      // by one lane
+        if (pass == 1 && sg.n > 0) {
+          const int k = index++ % kAgain;
+          if (!((s.again[k / 32] >> (k % 32)) & 1u)) return true;
+        }
+        sg.clean = pass == 0 ? 0 : 1 + tiles;
+        tiles = (tiles + 2 * sg.n) % (2 * kRing);
         const int at = given % kSegments;
         if (!mbar_wait(bar_seg_empty(at), ((given / kSegments) & 1) ^ 1, abort_flag, 19)) return false;
         s.segments[at] = sg;
         mbar_arrive(bar_seg(at));
         ++given;
         return true;
+      };
+      auto again = [&] {                     // as all_done, but this warp has nothing to release
+        asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+        return __any_sync(0xffffffffu, *static_cast<volatile int*>(&s.any_again) != 0 && *abort_flag == 0);
       };
       // steps `step` to `end` - 1 of an item
       auto describe = [&](const Seq& seq, const Item& it, int h, int p, int step, int end) {
@@ -763,95 +957,99 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         sg.slot0 = seq.rows - seq.n + p * 2 * a.tile_tokens;
         sg.two = it.n_tok > a.tile_tokens;
       };
-      if (SHARED) {
-        // All items of a group have the same steps, so the range is found without tables, by the warp: what code runs once costs by
-        // the instruction (6016 slots, 24 requests: the kernel 21 us with tables).
-        auto cost_of = [&](int g) {
-          if (g >= a.n_seq) return 0;
-          const Seq seq = seq_of<true>(a, g);
-          return pairs_of(a, seq) * ((seq.rows + kTile - 1) / kTile + kItemCost);
-        };
-        int total = 0;
-        for (int g = lane; g < a.n_seq; g += 32) total += cost_of(g);
-        total = __reduce_add_sync(0xffffffffu, total);
-        const int64_t all = (int64_t)total * a.hk;
-        const int n_ctas = (int)min((int64_t)a.max_ctas, (all + kLeastCost - 1) / kLeastCost);
-        const int64_t lo = c < n_ctas ? all * c / n_ctas : all, hi = c < n_ctas ? all * (c + 1) / n_ctas : all;
-        if (lo < hi && lane == 0) {
-          int h = (int)(lo / total), g = 0;
-          int64_t at = (int64_t)h * total;   // the item's place in the sequence
-          bool ok = true;
-          while (ok && at < hi) {
+#pragma unroll 1
+      do {
+        if (SHARED) {
+          // All items of a group have the same steps, so the range is found without tables, by the warp: what code runs once costs by
+          // the instruction (6016 slots, 24 requests: the kernel 21 us with tables).
+          auto cost_of = [&](int g) {
+            if (g >= a.n_seq) return 0;
             const Seq seq = seq_of<true>(a, g);
-            const int pairs = pairs_of(a, seq), steps = (seq.rows + kTile - 1) / kTile, cost = steps + kItemCost;
-            int p = at < lo ? (int)min((int64_t)pairs, (lo - at) / cost) : 0;
-            at += (int64_t)p * cost;
-            for (; ok && p < pairs && at < hi; ++p, at += cost) {
-              const int step = (int)max((int64_t)0, lo - at - kItemCost), end = (int)min((int64_t)steps, max((int64_t)0, hi - at - kItemCost));
-              if (step >= end) continue;
-              describe(seq, item_of<true>(a, seq, p), h, p, step, end);
-              const int item = h * a.batch + sg.q_row;
-              sg.part = c * a.part_rows + item * a.gs;
-              if (step == 0) a.meta[2 * item] = c;
-              if (end == steps) a.meta[2 * item + 1] = c;
-              ok = give();
+            return pairs_of(a, seq) * ((seq.rows + kTile - 1) / kTile + kItemCost);
+          };
+          int total = 0;
+          for (int g = lane; g < a.n_seq; g += 32) total += cost_of(g);
+          total = __reduce_add_sync(0xffffffffu, total);
+          const int64_t all = (int64_t)total * a.hk;
+          const int n_ctas = (int)min((int64_t)a.max_ctas, (all + kLeastCost - 1) / kLeastCost);
+          const int64_t lo = c < n_ctas ? all * c / n_ctas : all, hi = c < n_ctas ? all * (c + 1) / n_ctas : all;
+          if (lo < hi && lane == 0) {
+            int h = (int)(lo / total), g = 0;
+            int64_t at = (int64_t)h * total;   // the item's place in the sequence
+            bool ok = true;
+            while (ok && at < hi) {
+              const Seq seq = seq_of<true>(a, g);
+              const int pairs = pairs_of(a, seq), steps = (seq.rows + kTile - 1) / kTile, cost = steps + kItemCost;
+              int p = at < lo ? (int)min((int64_t)pairs, (lo - at) / cost) : 0;
+              at += (int64_t)p * cost;
+              for (; ok && p < pairs && at < hi; ++p, at += cost) {
+                const int step = (int)max((int64_t)0, lo - at - kItemCost), end = (int)min((int64_t)steps, max((int64_t)0, hi - at - kItemCost));
+                if (step >= end) continue;
+                describe(seq, item_of<true>(a, seq, p), h, p, step, end);
+                const int item = h * a.batch + sg.q_row;
+                sg.part = c * a.part_rows + item * a.gs;
+                if (step == 0) a.meta[2 * item] = c;
+                if (end == steps) a.meta[2 * item + 1] = c;
+                ok = give();
+              }
+              if (++g == a.n_seq) {
+                g = 0;
+                ++h;
+              }
             }
-            if (++g == a.n_seq) {
-              g = 0;
-              ++h;
+            sg.n = 0;
+            if (ok) give();
+          } else if (lane == 0) {
+            give();
+          }
+        } else if (lane == 0) {
+          int h = s.begin[0], v = s.begin[1], p = s.begin[2], step = s.begin[3];
+          const int h1 = s.end[0], v1 = s.end[1], p1 = s.end[2], step1 = s.end[3], first = s.first;
+          int tail = 0, head = 0;              // rows of a segment that others go on with; whether the first one is another CTA's item
+          Seq seq = {};
+          int pairs = 0, of = -1;
+          bool ok = true;
+          while (ok && h < a.hk) {
+            const bool last = h == h1 && v == v1 && p == p1;
+            if (last && step == step1) break;
+            if (of != v) {
+              seq = seq_of<false>(a, v);
+              pairs = pairs_of(a, seq);
+              of = v;
             }
+            const Item it = item_of<false>(a, seq, p);
+            const int end = last ? step1 : it.steps;
+            const bool begins = step == 0, ends = end == it.steps;
+            describe(seq, it, h, p, step, end);
+            sg.part = begins && ends ? -1 : (2 * c + begins) * a.part_rows;
+            if (!begins) head = ends ? 1 : 2;  // it ends here, or goes on behind
+            if (begins && !ends) {
+              tail = sg.n_tok;
+              a.meta[c * kMeta + 2] = h;
+              a.meta[c * kMeta + 3] = sg.q_row;
+            }
+            ok = give();
+            step = 0;
+            if (last) break;
+            if (++p == pairs) {
+              p = 0;
+              do ++v;
+              while (v < a.n_seq && !(v == v1 && h == h1) && pairs_of(a, seq_of<false>(a, v)) == 0);
+              if (v == a.n_seq) {
+                v = first;
+                ++h;
+              }
+            }
+          }
+          if (a.meta != nullptr) {
+            a.meta[c * kMeta] = tail;
+            a.meta[c * kMeta + 1] = head;
           }
           sg.n = 0;
           if (ok) give();
-        } else if (lane == 0) {
-          give();
         }
-      } else if (lane == 0) {
-        int h = s.begin[0], v = s.begin[1], p = s.begin[2], step = s.begin[3];
-        const int h1 = s.end[0], v1 = s.end[1], p1 = s.end[2], step1 = s.end[3], first = s.first;
-        int tail = 0, head = 0;              // rows of a segment that others go on with; whether the first one is another CTA's item
-        Seq seq = {};
-        int pairs = 0, of = -1;
-        bool ok = true;
-        while (ok && h < a.hk) {
-          const bool last = h == h1 && v == v1 && p == p1;
-          if (last && step == step1) break;
-          if (of != v) {
-            seq = seq_of<false>(a, v);
-            pairs = pairs_of(a, seq);
-            of = v;
-          }
-          const Item it = item_of<false>(a, seq, p);
-          const int end = last ? step1 : it.steps;
-          const bool begins = step == 0, ends = end == it.steps;
-          describe(seq, it, h, p, step, end);
-          sg.part = begins && ends ? -1 : (2 * c + begins) * a.part_rows;
-          if (!begins) head = ends ? 1 : 2;  // it ends here, or goes on behind
-          if (begins && !ends) {
-            tail = sg.n_tok;
-            a.meta[c * kMeta + 2] = h;
-            a.meta[c * kMeta + 3] = sg.q_row;
-          }
-          ok = give();
-          step = 0;
-          if (last) break;
-          if (++p == pairs) {
-            p = 0;
-            do ++v;
-            while (v < a.n_seq && !(v == v1 && h == h1) && pairs_of(a, seq_of<false>(a, v)) == 0);
-            if (v == a.n_seq) {
-              v = first;
-              ++h;
-            }
-          }
-        }
-        if (a.meta != nullptr) {
-          a.meta[c * kMeta] = tail;
-          a.meta[c * kMeta + 1] = head;
-        }
-        sg.n = 0;
-        if (ok) give();
-      }
+        __syncwarp();
+      } while (pass++ == 0 && again());
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
@@ -859,10 +1057,6 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const int grp = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;      // a warp may touch only its quarter of the lanes
     const uint32_t t_lane = (uint32_t)(quarter * 32) << 16;
     const uint32_t tmem_s = tmem + grp * kTile + t_lane, tmem_o = tmem + (2 + grp) * kTile + t_lane;
-    const uint64_t scale_2 = pack_f2(a.scale2, a.scale2);
-    // The reference follows the running maximum in steps of more than 2^kLazy, kAbove below it: fp16's short exponent then holds
-    // probabilities down to 2^-(24 + kAbove) of the largest, which are at most 2^(kAbove + kLazy).
-    constexpr float kLazy = 4.f, kAbove = DT == RI_F16 ? 10.f : 0.f;
     bool ok = true;
     // parities of what is waited for next: bit 0 scores, 1 and 2 outputs of the two groups, 3 joins.  A row of scores takes 128
     // registers, so little else is kept over the steps: what the segment says is read from shared memory where it is needed.
@@ -872,7 +1066,11 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       if (lane == 0) mbar_arrive(bar_join(i));
       return (bool)__all_sync(0xffffffffu, mbar_wait(bar_join(i), (phases >> 3) & 1, abort_flag, 10));
     };
-    for (int i = 0; ok && take(i); ++i) {
+    for (int i = 0; ok; ++i) {
+      if (!take(i)) {
+        if (pass++ == 1 || !all_done(i)) break;
+        continue;
+      }
       const Segment& sg = s.segments[i % kSegments];         // stays until the end of the segment
       // the row in its item, its token; rows that fill up a tile are like the last one, so that they hold nobody up
       auto row_in_item = [&] { return (sg.two ? grp * a.tile_tokens * a.gs : 0) + row; };
@@ -895,98 +1093,15 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       // so that results repeat to the bit.  No score is above their reference.
       auto is_row = [&] { return row < a.tile_tokens * a.gs && row_in_item() < sg.n_tok * a.gs; };
       float m_ref = is_row() ? -INFINITY : INFINITY, l_run = 0.f;
-      for (int j = 0; ok && j < sg.steps(grp); ++j, phases ^= 1) {
-        const int place = sg.nth(grp, j) * kTile;
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_s_full(grp), phases & 1, abort_flag, 11));
-        if (!ok) break;
-        tc_fence_after();
-        // Columns that are not seen become -infinity where they lie, 32 at a time: a tile's few tokens begin and end seeing close together,
-        // so most of four times 32 columns are seen by all rows of a warp, and a loop is a quarter of the instructions.
-        if (__any_sync(0xffffffffu, !sight.all_of(place))) {
-#pragma unroll 1
-          for (int x = 0; x < 4; ++x) {
-            const uint32_t seen = sight.mask(place + x * 32);
-            if (!__any_sync(0xffffffffu, seen != 0xffffffffu)) continue;
-            uint32_t part[32];
-            tc_ld32(tmem_s + x * 32, part);
-            tc_wait_ld();
-            tc_ld_landed(part);
-#pragma unroll
-            for (int y = 0; y < 32; ++y)
-              if (!(seen & (1u << y))) part[y] = 0xff800000u;      // -inf
-            tc_st32(tmem_s + x * 32, part);
-          }
-          tc_wait_st();
-        }
-        uint32_t sr[4][32];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) tc_ld32(tmem_s + x * 32, sr[x]);
-        tc_wait_ld();
-#pragma unroll
-        for (int x = 0; x < 4; ++x) tc_ld_landed(sr[x]);
-
-        float mx[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          mx[x] = fmaxf(__uint_as_float(sr[x][0]), __uint_as_float(sr[x][1]));
-#pragma unroll
-          for (int y = 2; y < 32; y += 2) mx[x] = max3(mx[x], __uint_as_float(sr[x][y]), __uint_as_float(sr[x][y + 1]));
-        }
-        const float m_tile = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * a.scale2 - kAbove;
-        const bool move = m_tile > m_ref + kLazy;              // also true for the first finite tile (m_ref = -inf)
-        if (__any_sync(0xffffffffu, move)) {
-          // the warp's accumulator rows are multiplied anyway, so every row of it catches up with its maximum
-          const float m_new = fmaxf(m_ref, m_tile);
-          const float factor = m_ref == -INFINITY ? 0.f : exp2f(m_ref - m_new);      // 1 when the maximum stays
-          l_run *= factor;
-          m_ref = m_new;
-          if (j > 0) {                                         // rare: bring this warp's rows of O to the new reference
-#pragma unroll 1
-            for (int x = 0; x < 4; ++x) {
-              uint32_t orow[32];
-              tc_ld32(tmem_o + x * 32, orow);
-              tc_wait_ld();
-              tc_ld_landed(orow);
-#pragma unroll
-              for (int y = 0; y < 32; ++y) orow[y] = __float_as_uint(__uint_as_float(orow[y]) * factor);
-              tc_st32(tmem_o + x * 32, orow);
-            }
-          }
-        }
-        // probabilities p = 2^(s * scale - m), packed as the 16-bit operand of the second product: word y of the row = slots 2y, 2y+1
-        const float ref = m_ref == -INFINITY ? 0.f : m_ref;
-        const uint64_t neg_m = pack_f2(-ref, -ref);
-        uint64_t sum2[2] = {0ull, 0ull};
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          uint32_t pw[16], low[16];
-#pragma unroll
-          for (int y = 0; y < 16; ++y) {
-            const uint64_t e = fma_f2(pack_f2(__uint_as_float(sr[x][2 * y]), __uint_as_float(sr[x][2 * y + 1])), scale_2, neg_m);
-            float e0, e1;
-            unpack_f2(e, e0, e1);
-            const float p0 = ex2(e0), p1 = ex2(e1);
-            sum2[y & 1] = add_f2(sum2[y & 1], pack_f2(p0, p1));
-            pw[y] = Elem<DT>::pack2(p0, p1);
-            if (SHARED) low[y] = Elem<DT>::pack2(p0 - Elem<DT>::from_bits((uint16_t)(pw[y] & 0xffffu)), p1 - Elem<DT>::from_bits((uint16_t)(pw[y] >> 16)));
-          }
-          tc_st16(tmem_s + x * 16, pw);
-          if (SHARED) tc_st16(tmem_s + kLowPart + x * 16, low);
-          if (x == 1) {          // the product over the first 64 slots may start
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar_p_part(grp));
-          }
-        }
-        float s0, s1;
-        unpack_f2(add_f2(sum2[0], sum2[1]), s0, s1);
-        l_run += s0 + s1;
-        tc_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_p_full(grp));
+      if (sg.clean == 0) {
+        ok = softmax_steps<DT, SHARED, false>(a, s, sg, sight, tmem_s, tmem_o, grp, phases & 1, m_ref, l_run, nullptr);
+      } else {
+        const Sums sums = clean_steps<DT, SHARED>(a, s, sg, sight, tmem_s, tmem_o, grp, phases, m_ref);
+        m_ref = sums.m;
+        l_run = sums.l;
+        ok = sums.ok;
       }
+      phases ^= sg.steps(grp) & 1;
       // ---- epilogue, one row per thread.  Two tiles: each group its own.  One: the groups exchange (maximum, sum) through shared
       //      memory, then each joins half of the channels of both accumulators; the second barrier keeps an accumulator until the
       //      other group has read it ----
@@ -1005,6 +1120,11 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       const float f = sg.part < 0 ? (l == 0.f ? 0.f : 1.f / l) : 1.f;      // NaN stays one
       w0 *= f;
       w1 *= f;
+      if (sg.clean != 0) {                                   // an infinite value is one however little its group counts
+        constexpr float kLeast = 1.17549435e-38f;
+        w0 = w0 < kLeast && l != 0.f ? kLeast : w0;
+        w1 = w1 < kLeast && l != 0.f ? kLeast : w1;
+      }
 #pragma unroll
       for (int g = 0; g < 2; ++g)
         if (sg.steps(g) > 0) {             // the other group's outputs count even where nobody here waits for them
@@ -1059,10 +1179,9 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           if (sg.part >= 0) a.part_ml[sg.part + item_row] = make_float2(m, l);
           else if (a.lse != nullptr) a.lse[(int64_t)q_row * a.hk * a.gs + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
         }
-        const unsigned again = __ballot_sync(0xffffffffu, valid && bad && l == l);
-        if (again) {
-          __syncwarp();
-          redo<DT>(a, sg, again, sight_of_row(), item_row, q_row, m == -INFINITY ? 0.f : m, f, two ? -1 : grp);
+        if (__any_sync(0xffffffffu, valid && bad && l == l) && pass == 0 && lane == 0) {
+          atomicOr(&s.again[i % kAgain / 32], 1u << (i % 32));
+          s.any_again = 1;
         }
       }
       if (!two) {
@@ -1071,6 +1190,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       }
       release(i);
     }
+    if (pass == 0) all_done(0);
   }
   }
 
