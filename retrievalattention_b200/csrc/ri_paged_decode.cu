@@ -725,15 +725,16 @@ __global__ void __launch_bounds__(kSharedThreads, 2) shared_finish_kernel(const 
   constexpr int kWide = 4;                                 // partial results on their way
   float M = -INFINITY, L = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  // adds parts against the largest reference so far; one far below it still counts enough to hand on an infinite value
+  // adds parts against the largest reference so far; one far below it, or what was there, still counts enough to hand on an infinite value
+  auto factor = [](float m, float ref) { return m == -INFINITY ? 0.f : fmaxf(exp2f(m - ref), 1.17549435e-38f); };
   auto add = [&](const float2* ml, const float4* v, int n) {
     float most = M;
     for (int u = 0; u < n; ++u) most = fmaxf(most, ml[u].x);
-    const float ref = most == -INFINITY ? 0.f : most, old = exp2f(M - ref);
+    const float ref = most == -INFINITY ? 0.f : most, old = factor(M, ref);
     L *= old;
     o.x *= old; o.y *= old; o.z *= old; o.w *= old;
     for (int u = 0; u < n; ++u) {
-      const float f = ml[u].x == -INFINITY ? 0.f : fmaxf(exp2f(ml[u].x - ref), 1.17549435e-38f);
+      const float f = factor(ml[u].x, ref);
       L += ml[u].y * f;
       o.x += v[u].x * f; o.y += v[u].y * f; o.z += v[u].z * f; o.w += v[u].w * f;
     }

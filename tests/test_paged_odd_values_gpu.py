@@ -163,3 +163,31 @@ def test_they_take_no_more_than_a_few_times_as_long(places):
     check_prefill_errors()
     print(f"{plain:.3f} -> {odd:.3f} ms")
     assert odd <= 12 * plain, (plain, odd)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("prefix", [256, 12800])
+@pytest.mark.parametrize("own_above", [True, False])
+def test_an_infinite_value_far_below_the_other_part(own_above, prefix, dtype):
+    """Scores in common and a request's own lie 120 apart (2^-173, nothing in 32 bits); an infinite value of the lower ones is handed on
+    whichever part comes first."""
+    from retrievalattention_b200 import paged
+
+    layer = Layer([prefix + 100, prefix + 9, prefix + 40], 1, 16, dtype, seed=6)
+    begin_alike(layer, ((0, 3, prefix // 16),))
+    for b, n in enumerate(layer.lengths_list):
+        k, v = layer.k[b] * 0.05, layer.v[b].clone()
+        k[:, :, 0] = 0.0
+        k[:, prefix:, 0] = (120.0 if own_above else -120.0) * DIM ** 0.5 / 16
+        if own_above:
+            v[:, prefix // 3, 5], v[:, prefix - 1, 6] = INF, -INF
+        else:
+            v[:, prefix + 3, 5], v[:, n - 1, 6] = INF, -INF
+        layer.fill(b, k.float(), v.float(), layer.w[b].float(), layer.t[b])
+    q = torch.randn((3, 1, 4, DIM), generator=torch.Generator().manual_seed(2)) * 0.1
+    q[..., 0] = 16
+    out = paged.paged_shared_decode(q.to(dtype).cuda(), layer.keys, layer.values, roomy(layer.table), layer.lengths,
+                                    torch.tensor([0, 3], dtype=torch.int32, device="cuda"), torch.tensor([prefix], dtype=torch.int32, device="cuda"))
+    out = out.float().cpu()
+    assert (out[..., 5] == INF).all() and (out[..., 6] == -INF).all(), out[:, 0, :, 5:7]
+    assert torch.isfinite(out[..., [c for c in range(DIM) if c not in (5, 6)]]).all()
