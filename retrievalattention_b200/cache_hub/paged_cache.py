@@ -216,18 +216,30 @@ class paged_cache(KV_Cache):
         self._regroup()
         return n
 
-    def _regroup(self) -> None:
-        """Runs of requests next to each other that begin with the same pages."""
-        first_pages = [next((i for i, id in enumerate(p) if id not in self._sharers), len(p)) for p in self._pages]
+    def _in_common(self, which):
+        """Runs of requests next to each other in ``which`` that begin with the same pages, so that the fewest slots are read: the first of
+        every run (and the end), the slots that it has in common."""
         alike = lambda a, b: next((i for i, (x, y) in enumerate(zip(a, b)) if x != y), min(len(a), len(b)))  # noqa: E731
-        starts, shared, b = [0], [], 0
-        while b < self.batch_size:
-            mine, n, end = self._pages[b][:first_pages[b]], 0, b + 1
-            while mine and end < self.batch_size and (m := alike(mine, self._pages[end])) and m >= n:
-                n, end = m if n == 0 else n, end + 1
-            starts.append(end)
+        pages = [self._pages[b] for b in which]
+        common = [alike(a, b) for a, b in zip(pages, pages[1:])]
+        best = [(0, 0, 0)]                                      # of the first j requests: pages saved, where the last run begins, its pages
+        for j in range(1, len(pages) + 1):
+            top, least = (best[j - 1][0], j - 1, 0), None
+            for i in range(j - 2, max(-1, j - 513), -1):        # a run of more than 512 may as well be two
+                least = common[i] if least is None else min(least, common[i])
+                if least == 0:
+                    break
+                top = max(top, (best[i][0] + (j - 1 - i) * least, i, least))
+            best.append(top)
+        starts, shared, j = [len(pages)], [], len(pages)
+        while j > 0:
+            _, j, n = best[j]
+            starts.append(j)
             shared.append(n * self.page_size)
-            b = end
+        return starts[::-1], shared[::-1]
+
+    def _regroup(self) -> None:
+        starts, shared = self._in_common(range(self.batch_size))
         more = self.batch_size - len(shared)
         self._group_start.copy_(self._to_device(starts + [self.batch_size] * more))
         self._group_shared.copy_(self._to_device(shared + [0] * more))
