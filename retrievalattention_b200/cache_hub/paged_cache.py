@@ -84,7 +84,7 @@ class paged_cache(KV_Cache):
         self._sharers = {}                                      # page: requests that begin with it, where they are several
         # group_start and shared of `paged.paged_shared_decode`, as many groups as requests, so that captured calls follow them
         self._group_start, self._group_shared = zeros(batch_size + 1, kind=torch.int32), zeros(batch_size, kind=torch.int32)
-        self._alike = False                                     # some requests have slots in common
+        self._alike, self._grouped = False, {}                  # some next to each other have slots in common; groups of some of the requests
 
     def _to_device(self, values) -> torch.Tensor:
         return torch.tensor(values, dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
@@ -169,13 +169,14 @@ class paged_cache(KV_Cache):
     def attend(self, query_states, layer_idx, out=None, lse=None, requests=None) -> torch.Tensor:
         """Attention of one new token of every request, ``[batch, 1, heads, 128]``, over its slots (``paged.paged_decode``), or the
         layer's window of them; with ``keep`` the slots' weights grow by what they are given.  ``requests``: of these alone, in the order of
-        their queries.  Slots that requests next to each other have in common are read once (``paged.paged_shared_decode``)."""
+        their queries.  Slots that requests next to each other, in that order, have in common are read once (``paged.paged_shared_decode``)."""
         table, lengths = self._of(requests)
         pools, window = (self.key_pages[layer_idx], self.value_pages[layer_idx]), self.attn_window[layer_idx]
         if window is not None:
             return paged.paged_decode(query_states, *pools, table, lengths, out=out, lse=lse, window=window, sink=self.attn_sink)
-        if self._alike and requests is None:
-            return paged.paged_shared_decode(query_states, *pools, table, lengths, self._group_start, self._group_shared, out=out, lse=lse)
+        groups = self._groups_of(requests)
+        if groups is not None:
+            return paged.paged_shared_decode(query_states, *pools, table, lengths, *groups, out=out, lse=lse)
         if self.keep is not None:
             self._weighing.update(range(self.batch_size) if requests is None else map(int, requests))
         return paged.paged_decode(query_states, *pools, table, lengths, out=out, lse=lse, weight=self.weight[layer_idx])
@@ -238,7 +239,22 @@ class paged_cache(KV_Cache):
             shared.append(n * self.page_size)
         return starts[::-1], shared[::-1]
 
+    def _groups_of(self, requests):
+        """Of all requests, or of some in their order; None where they have nothing in common."""
+        if requests is None:
+            return (self._group_start, self._group_shared) if self._alike else None
+        if not self._sharers:
+            return None
+        key = tuple(int(b) for b in requests)
+        if key not in self._grouped:
+            starts, shared = self._in_common(key)
+            if len(self._grouped) > 15:                         # kept over the steps, not for every choice that there ever was
+                self._grouped = {}
+            self._grouped[key] = (self._to_device(starts), self._to_device(shared)) if any(shared) else None
+        return self._grouped[key]
+
     def _regroup(self) -> None:
+        self._grouped = {}
         starts, shared = self._in_common(range(self.batch_size))
         more = self.batch_size - len(shared)
         self._group_start.copy_(self._to_device(starts + [self.batch_size] * more))
@@ -289,7 +305,7 @@ class paged_cache(KV_Cache):
         """Request ``bdx`` is done: its pages go back, and its place may take another one."""
         self._give_back(bdx, 0)
         self.length_of[bdx], self._evicted[bdx], self._fed[bdx], self._chosen = 0, False, 0, {}
-        if self._alike:
+        if self._alike or self._grouped:
             self._regroup()
         self._weighed.discard(bdx)
         self._weighing.discard(bdx)

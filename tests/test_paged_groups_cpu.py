@@ -46,3 +46,39 @@ def test_the_fewest_slots_are_read(make):  # noqa: F811
         assert sum((j - i - 1) * n for i, j, n in zip(starts, starts[1:], shared)) == most * cache.page_size
         for i, j, n in zip(starts, starts[1:], shared):
             assert all(cache._pages[x][:n // cache.page_size] == cache._pages[i][:n // cache.page_size] for x in range(i, j))
+
+
+def called(cache, monkeypatch):
+    """What `attend` calls, with the groups it hands over."""
+    from retrievalattention_b200 import paged
+
+    calls = []
+    monkeypatch.setattr(paged, "paged_decode", lambda q, *args, **rest: calls.append(None))
+    monkeypatch.setattr(paged, "paged_shared_decode", lambda q, k, v, table, lengths, starts, shared, **rest: calls.append((starts.tolist(), shared.tolist())))
+    return calls
+
+
+def test_some_of_the_requests_are_grouped_too(make, monkeypatch):  # noqa: F811
+    """One of those that begin alike is done: the others still read once what they have in common."""
+    cache = make(batch_size=5, max_length=40000, page_size=16, num_pages=2600, num_key_value_heads=8, num_heads=32)
+    calls = called(cache, monkeypatch)
+    cache.begin([32768, 0, 0, 0, 40])
+    assert cache.share(0, [1, 2, 3]) == 32768
+    cache.release(2)
+    for step in range(2):
+        cache.begin([1, 1, 0, 1, 1])
+        cache.attend(None, 0, requests=[0, 1, 3, 4])
+        assert calls.pop() == ([0, 3, 4], [32768, 0])
+        cache.attend(None, 0, requests=(4, 3, 1))               # in the order of their queries
+        assert calls.pop() == ([0, 1, 3], [0, 32768])
+        cache.attend(None, 0, requests=[4])
+        cache.attend(None, 0, requests=[3, 4])
+        assert calls == [None, None] and not calls.clear()
+    cache.release(0)                                            # groups of before are not gone by
+    cache.begin([1, 1, 0, 1, 1])
+    cache.attend(None, 0, requests=[0, 1, 3, 4])
+    assert calls.pop() == ([0, 1, 3, 4], [0, 32768, 0])
+    cache.release(1)
+    cache.begin([0, 0, 0, 1, 1])
+    cache.attend(None, 0, requests=[3, 4])
+    assert calls.pop() is None
