@@ -17,7 +17,7 @@ Lengths and pages are known on the host without asking the GPU, so nothing synch
 
 Layers may look back over a window (``attn_window``, ``attn_sink``): ``attend`` and ``prompt`` go by it.  ``prompt`` is the attention of
 the step's rows over the pages, for prompts that follow on what is cached.  ``share(0, [1, 2])``: empty requests begin with the pages of
-request 0, whose prompt has run, and ``attend`` reads what they have in common once for all of them.
+request 0, whose prompt has run, and ``attend`` reads what they have in common once for all of them, where that is enough to be faster.
 """
 from __future__ import annotations
 
@@ -84,7 +84,8 @@ class paged_cache(KV_Cache):
         self._sharers = {}                                      # page: requests that begin with it, where they are several
         # group_start and shared of `paged.paged_shared_decode`, as many groups as requests, so that captured calls follow them
         self._group_start, self._group_shared = zeros(batch_size + 1, kind=torch.int32), zeros(batch_size, kind=torch.int32)
-        self._alike, self._grouped = False, {}                  # some next to each other have slots in common; groups of some of the requests
+        self._alike, self._together = False, False              # some next to each other have slots in common, and enough of them
+        self._grouped = {}                                      # groups of some of the requests
 
     def _to_device(self, values) -> torch.Tensor:
         return torch.tensor(values, dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
@@ -169,7 +170,8 @@ class paged_cache(KV_Cache):
     def attend(self, query_states, layer_idx, out=None, lse=None, requests=None) -> torch.Tensor:
         """Attention of one new token of every request, ``[batch, 1, heads, 128]``, over its slots (``paged.paged_decode``), or the
         layer's window of them; with ``keep`` the slots' weights grow by what they are given.  ``requests``: of these alone, in the order of
-        their queries.  Slots that requests next to each other, in that order, have in common are read once (``paged.paged_shared_decode``)."""
+        their queries.  Slots that requests next to each other, in that order, have in common are read once (``paged.paged_shared_decode``),
+        where they are many enough."""
         table, lengths = self._of(requests)
         pools, window = (self.key_pages[layer_idx], self.value_pages[layer_idx]), self.attn_window[layer_idx]
         if window is not None:
@@ -239,10 +241,21 @@ class paged_cache(KV_Cache):
             shared.append(n * self.page_size)
         return starts[::-1], shared[::-1]
 
+    # What is read once for several requests has to be this many MB of keys and values less, and as many more for each request, or they
+    # are attended one by one: it takes two kernels more, and what others have just read is often found in L2.  8 heads of 4, one by one and
+    # together: 2 requests of 65536 slots in common (268 MB) 85 and 87 us, 8 of 8192 (235 MB) 50 and 48, of 16384 (470 MB) 85 and 60, 64 of
+    # 2048 (529 MB) 97 and 81, of 1024 in front of 4096 of their own (264 MB) 206 and 247, 256 of 512 (535 MB) 149 and 210, of 2048 351 and 214.
+    _PAYS_MB, _PAYS_MB_EACH = 256, 4
+
+    def _pays(self, starts, shared) -> bool:
+        saved = sum((j - i - 1) * n for i, j, n in zip(starts, starts[1:], shared))
+        return saved > 0 and saved * self.kv_head * 4 * paged.DIM >= (self._PAYS_MB + self._PAYS_MB_EACH * starts[-1]) << 20
+
     def _groups_of(self, requests):
-        """Of all requests, or of some in their order; None where they have nothing in common."""
+        """Of all requests, or of some in their order; None where one by one is faster.  Captured calls take what is alike now for a sign
+        of what later steps have in common."""
         if requests is None:
-            return (self._group_start, self._group_shared) if self._alike else None
+            return (self._group_start, self._group_shared) if self._alike and (self._together or self._captures()) else None
         if not self._sharers:
             return None
         key = tuple(int(b) for b in requests)
@@ -250,7 +263,7 @@ class paged_cache(KV_Cache):
             starts, shared = self._in_common(key)
             if len(self._grouped) > 15:                         # kept over the steps, not for every choice that there ever was
                 self._grouped = {}
-            self._grouped[key] = (self._to_device(starts), self._to_device(shared)) if any(shared) else None
+            self._grouped[key] = (self._to_device(starts), self._to_device(shared)) if self._pays(starts, shared) else None
         return self._grouped[key]
 
     def _regroup(self) -> None:
@@ -259,7 +272,7 @@ class paged_cache(KV_Cache):
         more = self.batch_size - len(shared)
         self._group_start.copy_(self._to_device(starts + [self.batch_size] * more))
         self._group_shared.copy_(self._to_device(shared + [0] * more))
-        self._alike = any(shared)
+        self._alike, self._together = any(shared), self._pays(starts, shared)
 
     def observe(self, query_states, layer_idx, requests=None) -> None:
         """Weights from the last queries ``[batch, window, heads, 128]`` of the step's prompts (``paged.paged_observe``).  ``requests``:

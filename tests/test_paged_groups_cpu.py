@@ -62,6 +62,8 @@ def test_some_of_the_requests_are_grouped_too(make, monkeypatch):  # noqa: F811
     """One of those that begin alike is done: the others still read once what they have in common."""
     cache = make(batch_size=5, max_length=40000, page_size=16, num_pages=2600, num_key_value_heads=8, num_heads=32)
     calls = called(cache, monkeypatch)
+    for name in ("_PAYS_MB", "_PAYS_MB_EACH"):                  # whatever it saves
+        monkeypatch.setattr(cache, name, 0, raising=False)
     cache.begin([32768, 0, 0, 0, 40])
     assert cache.share(0, [1, 2, 3]) == 32768
     cache.release(2)
@@ -81,4 +83,29 @@ def test_some_of_the_requests_are_grouped_too(make, monkeypatch):  # noqa: F811
     cache.release(1)
     cache.begin([0, 0, 0, 1, 1])
     cache.attend(None, 0, requests=[3, 4])
+    assert calls.pop() is None
+
+
+def test_little_in_common_is_not_worth_a_kernel(make, monkeypatch):  # noqa: F811
+    """A page in common in front of long requests: one by one, all of them or some; a captured call goes by the groups all the same, which
+    may have more in common when it is replayed."""
+    args = dict(batch_size=3, max_length=70000, page_size=16, num_pages=9000, num_key_value_heads=8, num_heads=32)
+    cache = make(**args)
+    calls = called(cache, monkeypatch)
+    cache.begin([30, 0, 30000])
+    cache.share(0, [1])
+    cache.begin([30000, 30000, 1])
+    cache.attend(None, 0)
+    cache.attend(None, 0, requests=[0, 1])
+    assert calls == [None, None] and cache._alike
+    monkeypatch.setattr(cache, "_captures", lambda: True)
+    cache.attend(None, 0)
+    assert calls.pop() == ([0, 2, 3, 3], [16, 0, 0])
+    monkeypatch.setattr(cache, "_captures", lambda: False)
+    cache = make(**args)                                        # 265 MB (of 2^20) of keys and values in common
+    cache.begin([68010, 0, 1])
+    cache.share(0, [1], 68000)
+    cache.attend(None, 0, requests=[0, 1])                      # 256 and 4 for each of two requests
+    assert calls.pop() == ([0, 2], [68000])
+    cache.attend(None, 0)                                       # of three
     assert calls.pop() is None
