@@ -32,8 +32,8 @@ typedef enum ri_status {
 enum { RI_BF16 = 0, RI_F16 = 1 };
 enum { RI_HEAD_DIM = 128 };
 /* in a status word: a row did not fit its dense cache; a page table entry names no page; a row did not fit its request's page
- * table; other values name the wait that gave up */
-enum { RI_STATUS_CACHE_FULL = 60, RI_STATUS_PAGE_ID = 61, RI_STATUS_PAGES_FULL = 62 };
+ * table; rows of a prompt's requests do not ascend; other values name the wait that gave up */
+enum { RI_STATUS_CACHE_FULL = 60, RI_STATUS_PAGE_ID = 61, RI_STATUS_PAGES_FULL = 62, RI_STATUS_ROW_START = 63 };
 
 const char* ri_last_error(void);
 int ri_version(void);
@@ -392,7 +392,7 @@ int ri_paged_decode_window(const ri_paged* p, const void* d_q, int64_t q_stride,
                            float scale, void* d_scratch, void* stream);
 /* Attention of the last tokens in use, several of every request: d_q `rows` rows of kv_heads * group_size heads of 128, q_stride elements
  * apart; rows d_row_start[b] .. d_row_start[b + 1] - 1 (ascending, within `rows`) are those of request b's last tokens, whose keys and values
- * are in the cache.  The token at slot s sees the slots j <= s with j > s - window (window 0: all of them) or j < sink.  d_out [rows,
+ * are in the cache; where d_row_start descends nothing is written (RI_STATUS_ROW_START in *d_status).  The token at slot s sees the slots j <= s with j > s - window (window 0: all of them) or j < sink.  d_out [rows,
  * q_heads, 128] and d_lse [rows, q_heads] (or NULL) as for ri_paged_decode; rows that belong to no request are left as they were, and
  * a row in front of its request's first slot sees nothing.  group_size 1 to 8, batch at most 16384.  Slots must be in the order of their
  * tokens.  Pages that no row sees are not read, nor are their numbers.  d_scratch: that many bytes of 16-byte aligned device memory

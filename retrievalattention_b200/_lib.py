@@ -15,7 +15,7 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("RI_B200_LIB") or os.path.join(_PKG, "lib", "libri_b200.so")
 
 RI_BF16, RI_F16 = 0, 1
-RI_STATUS_CACHE_FULL, RI_STATUS_PAGE_ID, RI_STATUS_PAGES_FULL = 60, 61, 62
+RI_STATUS_CACHE_FULL, RI_STATUS_PAGE_ID, RI_STATUS_PAGES_FULL, RI_STATUS_ROW_START = 60, 61, 62, 63
 
 
 class WaveLayer(C.Structure):

@@ -102,6 +102,7 @@ struct Control {
   int scan[kThreads / 32 + 1];
   int begin[4], end[4];                    // where the CTA's range begins and ends: head, sequence, pair of tiles, step
   int first;                               // the first sequence with rows
+  int descends;                            // some sequence's rows begin in front of those of the one before it
   uint32_t again[kAgain / 32];             // segments that are done once more
   int any_again;
   uint32_t odd[kRing][kTile / 32];         // done once more: rows of the tile of V that held something else than numbers
@@ -220,6 +221,7 @@ __device__ __forceinline__ void plan(const Args& a, int* table, Control& s) {
     const int each = (a.n_seq + kThreads - 1) / kThreads, v0 = min(tid * each, a.n_seq), v1 = min(v0 + each, a.n_seq);
     int sum = 0, first = a.n_seq;
     for (int v = v0; v < v1; ++v) {
+      if (a.starts[v + 1] < a.starts[v]) s.descends = 1;
       const int n = pairs_of(a, seq_of<false>(a, v));
       pairs[v] = sum;
       if (n > 0) first = min(first, v);
@@ -231,7 +233,9 @@ __device__ __forceinline__ void plan(const Args& a, int* table, Control& s) {
     if (tid == 0) pairs[a.n_seq] = total;
   }
   __syncthreads();
-  const int n_pairs = total;
+  // Rows that several requests claim could be more than there are, and more than what is counted here has bits for: nothing is done.
+  if (s.descends != 0 && tid == 0) *a.status = RI_STATUS_ROW_START;
+  const int n_pairs = s.descends != 0 ? 0 : total;
   int k = 0;
   while ((n_pairs - 1) >> k >= kMaxEntries) ++k;
   const int entries = n_pairs > 0 ? ((n_pairs - 1) >> k) + 1 : 0;
@@ -619,6 +623,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     // the swizzle of the tiles goes by addresses: shared memory that does not begin on a boundary of 1 KB gives up at once
     s.abort = (sQ & 1023u) ? 10 : 0;
     s.first = 0x7fffffff;
+    s.descends = 0;
     s.any_again = 0;
     for (int g = 0; g < 2; ++g) {
       mbar_init(bar_q(g), 1); mbar_init(bar_q_empty(g), 1); mbar_init(bar_s_full(g), 1);

@@ -22,8 +22,9 @@ The layer is a handful of tensors that the caller owns (``cache_hub.paged_cache`
                                 a wide one than the longest request needs (``page_table[:, :pages]``)
 
 Every call is asynchronous on the current stream, allocates its workspace from torch's caching allocator and can be captured in a
-CUDA graph.  Lengths and page tables are read on the device: an entry that names no page, or a row that its request's table has no
-slot for, is reported by the next call or by ``attn_hub.check_prefill_errors``.  There are no gradients.
+CUDA graph.  Lengths and page tables are read on the device: an entry that names no page, a row that its request's table has no
+slot for, or a prompt's ``row_start`` that descends, is reported by the next call or by ``attn_hub.check_prefill_errors``.  There are
+no gradients.
 """
 from __future__ import annotations
 
@@ -124,8 +125,9 @@ def paged_decode(q, key_pages, value_pages, page_table, lengths, *, out=None, ls
 
 def paged_prompt(q, key_pages, value_pages, page_table, lengths, row_start, *, window=None, sink=0, out=None, lse=None, scale=None):
     """Attention of several new tokens of every request over the pages, whole prompts or pieces of them: rows ``row_start[b]`` to
-    ``row_start[b + 1] - 1`` (int32 ``[batch + 1]``, ascending) of ``q`` ``[rows, q_heads, 128]`` (rows may lie apart; one to eight query
-    heads to a KV head) are the last of request ``b``'s slots in use, whose keys and values are in the cache (``rope_paged_append``).
+    ``row_start[b + 1] - 1`` (int32 ``[batch + 1]``, ascending: otherwise nothing is written) of ``q`` ``[rows, q_heads, 128]`` (rows may lie
+    apart; one to eight query heads to a KV head) are the last of request ``b``'s slots in use, whose keys and values are in the cache
+    (``rope_paged_append``).
     The token at slot ``s`` sees the slots up to ``s``; with ``window`` only the last ``window`` of them, and the first ``sink``.  Returns ``out``
     ``[rows, q_heads, 128]``; ``lse`` fp32 ``[rows, q_heads]`` takes the log-sum-exp.  Rows that belong to no request are left alone;
     a row in front of its request's first slot (more rows than slots) has out 0 and lse -infinity.  Slots must be in the order of their

@@ -1,7 +1,7 @@
 """The process's status word, on the host.
 
 Prefill, decode (dense, paged, wave) kernels record in it that a device-side wait gave up, the appends that a row did not fit, and
-the kernels over paged caches that a page table names no page (0: none of it): one word in page-locked host memory for all devices and streams, replays of CUDA graphs among them.  The
+the kernels over paged caches that a page table names no page or that rows of several requests overlap (0: none of it): one word in page-locked host memory for all devices and streams, replays of CUDA graphs among them.  The
 kernels only write it, so a failure stays inside its call; it stays set until it is reported, by ``check`` or by the first call
 that finds it set.
 """
@@ -57,6 +57,8 @@ def check() -> None:
             raise RuntimeError("a page table entry names no page of the pool")
         if code == _lib.RI_STATUS_PAGES_FULL:
             raise RuntimeError("a token's rows did not fit the pages of its request")
+        if code == _lib.RI_STATUS_ROW_START:
+            raise RuntimeError("row_start descends: nothing was attended")
         raise RuntimeError(f"{_kernel(code)} gave up on a device-side wait (code {code})")
 
 
