@@ -196,6 +196,8 @@ class paged_cache(KV_Cache):
         """Let ``requests``, which are empty, begin with the first ``slots`` slots of request ``of`` (default: all of them), as far as
         they fill pages: nothing is copied.  Returns how many they are.  Not with ``keep``: requests that share pages cannot be evicted
         from."""
+        if not 0 <= of < self.batch_size:
+            raise ValueError(f"request {of} of {self.batch_size}")
         requests, n = [int(b) for b in requests], self.length_of[of] if slots is None else slots
         if self.keep is not None:
             raise ValueError("requests that share pages cannot be evicted from: share or keep")

@@ -237,6 +237,7 @@ class PagedDecoder(SyntheticDecoder):
     def share(self, of: int, requests, tokens: int | None = None) -> int:
         """Let ``requests``, which are empty, begin with the first ``tokens`` tokens of request ``of`` (default: all), as far as they
         fill pages of the cache; returns how many they are.  Positions are counted on from there: hand others to ``extend_forward``."""
+        requests = [int(b) for b in requests]
         n = self.cache.share(of, requests, tokens)
         for b in requests:
             self._next_position[b] = n
