@@ -49,14 +49,14 @@ class paged_cache(KV_Cache):
         if keep is not None and (min(sink, recent, slack) < 0 or keep < 1 or sink + recent > keep):
             raise ValueError(f"keep={keep} slots for {sink} first and {recent} last tokens, slack={slack}")
         windows = list(attn_window) if isinstance(attn_window, (list, tuple)) else [attn_window] * layer_num
-        if len(windows) != layer_num or any(w is not None and w < 1 for w in windows) or attn_sink < 0:
+        if len(windows) != layer_num or any(w is not None and (w != int(w) or w < 1) for w in windows) or attn_sink != int(attn_sink) or attn_sink < 0:
             raise ValueError(f"attn_window={attn_window}, attn_sink={attn_sink}: expected a slot or more (or None) for all layers or each")
         if keep is not None and any(w is not None for w in windows):
             raise ValueError("a window goes by the order of the slots, which eviction does not keep: attn_window or keep")
         super().__init__(layer_num, batch_size, max_length, num_key_value_heads, num_heads, head_dim, dtype, layer_mapping,
                          num_gpus, model_size)
         self.device = devices.pop()
-        self.attn_window, self.attn_sink = windows, attn_sink
+        self.attn_window, self.attn_sink = [None if w is None else int(w) for w in windows], int(attn_sink)
         self.page_size, self.keep, self.sink, self.recent, self.slack = page_size, keep, sink, recent, slack
         width = -(-max_length // page_size)                     # pages of the longest request
         self.num_pages = batch_size * width if num_pages is None else num_pages

@@ -24,3 +24,16 @@ def test_requests_that_are_none(make, of):  # noqa: F811
     with pytest.raises(ValueError, match="of 3"):
         cache.share(of, [0])
     assert cache.length_of == [0, 0, 40] and not cache._sharers
+
+
+def test_windows_that_are_no_numbers_of_slots(make):  # noqa: F811
+    import math
+
+    for bad in (dict(attn_window=2.5), dict(attn_window=[2.5]), dict(attn_window=30, attn_sink=0.5)):
+        with pytest.raises(ValueError, match="attn_window"):
+            make(**bad)
+    for bad in (math.inf, math.nan):                            # no window is None
+        with pytest.raises((ValueError, OverflowError)):
+            make(attn_window=bad)
+    cache = make(attn_window=30.0, attn_sink=4.0)
+    assert cache.attn_window == [30] and all(type(x) is int for x in cache.attn_window + [cache.attn_sink])
