@@ -90,6 +90,8 @@ __global__ void __launch_bounds__(kNormThreads) rmsnorm_kernel(const uint4* __re
 // half (neox pairing: element j with element j + 64).  cos_sin: fp32 [positions, 128], cosines in
 // the first 64 columns, sines in the last 64, as the reference builds it (model_hub/llama.py:81-84, :109).
 // NORM: query and key heads are first x_i <- x_i w_i / sqrt(mean x^2 + eps); `q_norm` and `k_norm` step by 0 or 16 pieces a head.
+// It is a decode step's kernel, a block of 16 threads for each head of a row: 32 + 8 heads 1.6 us for a row, 1.7 for 4, 3.6 for 64, 51 for 1024,
+// with norms or without, one weight or one for each head.  Prompts have ri_rope_paged_append (32768 rows 155 us; here 1.6 ms).
 struct HeadNorms {
   const uint4* q;
   const uint4* k;

@@ -5,9 +5,9 @@
 // With norms a query or key head is first  x_i <- x_i w_i / sqrt(mean x^2 + eps),  in 32 bits up to the one rounding behind the rotation;
 // the half-warp that has a head has its sum of squares in four shuffles.  The root is taken behind the rotation, and weights that are
 // the same for all heads go into the row's cosines and sines, which a service warp multiplies: the rotation is what it was, and the
-// rotating warps, which would be what counts otherwise, have a third more to do, not twice as much.  32768 rows of 32 + 8 heads: 153 us
-// (149 without norms; with the weights loaded and multiplied head by head 210).  Weights for each head are multiplied by the lane that has
-// the piece, and the piece that it is rotated with comes from the lane beside it: 176 us (198 with both pieces weighted by both lanes).
+// rotating warps, which would be what counts otherwise, have a third more to do, not twice as much.  32768 rows of 32 + 8 heads: 155 to 167 us
+// (146 to 149 without norms; with the weights loaded and multiplied head by head 210).  Weights for each head are multiplied by the lane that has
+// the piece, and the piece that it is rotated with comes from the lane beside it: 176 to 180 us (198 with both pieces weighted by both lanes).
 // (reference: model_hub/llama.py:232-235 the split, :312-320 the rotation; cache_hub/flash_attn_cache.py:133-151 the append)
 //
 // Bound by the projection, read once and written once.  A row of it lies in one piece and comes in by one bulk copy, three rows

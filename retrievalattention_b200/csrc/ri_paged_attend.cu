@@ -14,7 +14,8 @@
 //                     Prompts: one part, rounded (8 bits of bf16, 11 of fp16), as in ri_prefill_attn.cu: a second one makes half of a step's
 //                     products twice as many.  Against 64 bits the outputs are 2.2e-3 off where the rounding of the result alone gives 1.65e-3
 //                     (fp16 2.6e-4 and 2.0e-4).  What requests have in common: two parts, as ri_paged_decode.cu has for requests that are
-//                     attended one by one, so that what a request gets does not hang on which of the two the call takes;
+//                     attended one by one, so that what a request gets does not hang on which of the two the call takes (64 requests over
+//                     32768 slots, the call: 124 us with one part, 138 with two);
 //   O_g += P_g.V      A from TMEM, B the V tile as it lies (MN-major), the accumulator in TMEM for the whole walk.
 // Items of two tiles: a group of four softmax warps for each, which share every tile of K and V.  Items of one tile: the groups take
 // its even and its odd steps, and join what they have at the end.
@@ -25,8 +26,9 @@
 // A tile's slots that a row does not see have a probability of 0, and what they hold is finite where it was written as such; where it
 // was not, 0 * infinity leaves a NaN, and the segment is done once more (kAgain).  Slots behind a request's last one may
 // hold anything: they are zeros in shared memory before the product.
-// B200, bf16, 8 heads of 4, one prompt: 8192 tokens 505 us over all slots (the dense prompt kernel: 455), 261 over a window of 2048, 61
-// over one of 128; 32768 tokens over 2048 1.23 to 1.36 ms (2.1 PFLOP over what is seen, 650 us at the cuBLAS rate).  What bounds it: a
+// B200, bf16, 8 heads of 4, one prompt, a call among others: 8192 tokens 512 to 532 us over all slots (the dense prompt kernel: 464), 297 to
+// 305 over a window of 2048, 70 over one of 128; 32768 tokens over 2048 1.20 ms, 1.43 under the power cap (2.1 PFLOP over what is seen,
+// 650 us at the cuBLAS rate).  What bounds it: a
 // step of two tiles keeps the tensor pipe's queue full for 3200 clocks (16 products of M 128 N 128 K 16 a tile, at 100 clocks each where
 // shared memory's bandwidth would allow 64; the pipe counts as active for half of them); an item costs 7000 more, for the first scores, the
 // outputs and masked columns; a launch 12 us until its first probabilities, most of it code that runs for the first time.  Measured and

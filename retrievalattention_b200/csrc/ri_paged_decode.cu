@@ -18,7 +18,7 @@
 // probabilities; every slot has one thread, so the sums have one order and no atomics.
 // Short requests that leave the chip room give every group a cluster of CTAs, which does all of this in one kernel.
 // With a window the steps between the first slots and the window are left out: they take no part in the split, and nothing of
-// them, their page numbers among it, is read.  32 requests, window 8192, 8 heads of 4: 178 us, 6.0 TB/s.
+// them, their page numbers among it, is read.  32 requests, window 8192, 8 heads of 4: 170 to 190 us, 5.7 to 6.3 TB/s.
 // Requests that begin alike: this kernel has each one's own slots, beside the one of ri_paged_attend.cu over what they have in common.
 // B200, bf16, 8 heads of 4: 4 x 131072 slots 318 to 345 us by the GPU, 6.2 to 6.8 TB/s (a copy: 6.6); 4 requests of 20K to 32K with
 // weights 91 us, 4.8 TB/s: the SMs are done after 64 to 78 us, half of them by 68 (some two dozen SMs are the last in every case,
@@ -943,9 +943,9 @@ int launch(const ri_paged& p, const Args& a, void* stream) {
 }
 
 // Requests that begin alike are attended together where all slots there may be are more than this many bytes of K and V.  It takes a
-// kernel more, and requests that are attended one by one find much of what others have read in L2: 8 heads of 4, 8 requests of 4096
-// slots in common and up to 500 of their own (151 MB) 28 us together and 26 one by one, 16 requests (302 MB) 32 and 45, 8 requests over
-// 16384 slots (554 MB) 41 and 80, 64 over 32768 (9.1 GB) 124 and 1135.
+// kernel more, and requests that are attended one by one find much of what others have read in L2: 8 heads of 4, L2 flushed, 8 requests of
+// 4096 slots in common and 500 of their own (151 MB) 42 us together and 34 one by one, 16 requests (302 MB) 48 and 52, 8 requests over
+// 16384 slots (554 MB) 60 and 85; 64 over 32768 (9.1 GB), not flushed, 138 and 1140.
 constexpr int64_t kAlikeBytes = 160 << 20;
 bool apart(const ri_paged& p) { return (int64_t)p.batch * p.kv_heads * ri_page::slots_of(p) * 4 * RI_HEAD_DIM <= kAlikeBytes; }
 int64_t own_bytes(const ri_paged& p) { return ri_align_up(paged_slots(p) * p.group_size * (RI_HEAD_DIM + 2) * 4, 16); }
