@@ -224,7 +224,13 @@ class paged_cache(KV_Cache):
     def _in_common(self, which):
         """Runs of requests next to each other in ``which`` that begin with the same pages, so that the fewest slots are read: the first of
         every run (and the end), the slots that it has in common."""
-        alike = lambda a, b: next((i for i, (x, y) in enumerate(zip(a, b)) if x != y), min(len(a), len(b)))  # noqa: E731
+        def alike(a, b):                                        # by halves: lists of thousands of pages, between two steps
+            low, high = 0, min(len(a), len(b))
+            while low < high:
+                mid = (low + high + 1) // 2
+                low, high = (mid, high) if a[low:mid] == b[low:mid] else (low, mid - 1)
+            return low
+
         pages = [self._pages[b] for b in which]
         common = [alike(a, b) for a, b in zip(pages, pages[1:])]
         best = [(0, 0, 0)]                                      # of the first j requests: pages saved, where the last run begins, its pages
