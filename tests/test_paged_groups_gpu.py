@@ -58,3 +58,48 @@ def test_requests_that_run_on(monkeypatch):
         check(cache, q, out, lse, running)
     assert len(shared_calls) == 5
     assert [x[1].max().item() for x in shared_calls] == [n] * 5
+
+
+def test_a_model_whose_requests_begin_alike(monkeypatch):
+    """Prompts, a nested prefix, steps, and requests that are done, over the kernels that read once what is in common (whole page tables, and
+    whatever that saves), against the model in 32 bits."""
+    from test_paged_layers_gpu import check as check_model, small
+
+    from retrievalattention_b200 import paged
+    from retrievalattention_b200.attn_hub.retroinfer_attn import check_prefill_errors
+
+    model = small((None, 24), batch=5, max_length=120000)
+    cache = model.cache
+    rows = lambda requests: slice(None) if requests is None else torch.tensor(requests, device="cuda")  # noqa: E731
+    monkeypatch.setattr(cache, "_of", lambda requests: (cache.page_table[rows(requests)], cache.lengths[rows(requests)]))
+    for name in ("_PAYS_MB", "_PAYS_MB_EACH"):
+        monkeypatch.setattr(cache, name, 0)
+    calls, shared_decode = [], paged.paged_shared_decode
+    monkeypatch.setattr(paged, "paged_shared_decode", lambda *args, **rest: calls.append(args[6].tolist()) or shared_decode(*args, **rest))
+    gen = torch.Generator().manual_seed(2)
+    prompt = lambda n: torch.randint(0, 1000, (n,), generator=gen).cuda()  # noqa: E731
+    begin, document = prompt(35), prompt(150)
+    for b in range(1, 5):
+        model.release(b)
+    ids = [list(begin), None, None, None, None]
+    check_model(model, model.prefill_forward([begin], requests=[0]), ids, (0,))
+    assert model.share(0, [1]) == 32
+    ids[1] = list(begin[:32]) + list(document)
+    check_model(model, model.extend_forward([document], requests=[1]), ids, (1,))
+    assert model.share(1, [2, 3], 182) == 176
+    rest = [torch.cat([document[144:], prompt(n)]) for n in (3, 20)]
+    for b, p in zip((2, 3), rest):
+        ids[b] = list(begin[:32]) + list(document[:144]) + list(p)
+    check_model(model, model.extend_forward(rest, requests=[2, 3]), ids, (2, 3))
+    other = prompt(40)
+    ids[4] = list(other)
+    check_model(model, model.prefill_forward([other], requests=[4]), ids, (4,))
+    for done in (None, 2, 0):
+        if done is not None:
+            model.release(done)
+        running = [b for b in range(5) if b not in model._released]
+        for _ in range(3):
+            check_model(model, model.decode_forward(), ids, running)
+    check_prefill_errors()
+    # of layers without a window: groups of all, of 0, 1, 3, 4 and of 1, 3, 4
+    assert calls == [[0, 176, 0, 0, 0]] * 3 + [[0, 176, 0]] * 3 + [[176, 0]] * 3
